@@ -8,6 +8,22 @@ tcgen05 kernels (``libda_b200.so``, C ABI in ``include/da_b200.h``).
 """
 
 from .config import DoubleAttentionConfig, experiment_config, experiment_names
+from .eight_bit import (
+    Checkpoint8,
+    Int8Rows,
+    add_layernorm_int8,
+    add_rmsnorm_int8,
+    checkpoint8,
+    feedforward_checkpoint8,
+    gelu_checkpoint8,
+    gelu_checkpoint8_backward,
+    int8_linear,
+    layernorm_int8,
+    linear_checkpoint8,
+    quantize_int8,
+    rmsnorm_int8,
+    weight_grad_checkpoint8,
+)
 from .graphs import GraphedModuleStep
 from .modules import (
     DoubleAttentionAux,
@@ -20,17 +36,31 @@ from .modules import (
 from .ops import assemble_score_maps, dictionary_route, routed_attention
 
 __all__ = [
+    "Checkpoint8",
     "DoubleAttentionAux",
     "DoubleAttentionBlock",
     "DoubleAttentionConfig",
     "DoubleAttentionLM",
     "DoubleAttentionStack",
     "GraphedModuleStep",
+    "Int8Rows",
     "SharedDictionaryAttention",
     "SharedDictionaryBank",
+    "add_layernorm_int8",
+    "add_rmsnorm_int8",
     "assemble_score_maps",
+    "checkpoint8",
     "dictionary_route",
     "experiment_config",
     "experiment_names",
+    "feedforward_checkpoint8",
+    "gelu_checkpoint8",
+    "gelu_checkpoint8_backward",
+    "int8_linear",
+    "layernorm_int8",
+    "linear_checkpoint8",
+    "quantize_int8",
+    "rmsnorm_int8",
     "routed_attention",
+    "weight_grad_checkpoint8",
 ]

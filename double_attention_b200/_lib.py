@@ -88,6 +88,15 @@ SIGNATURES: dict[str, list] = {
     "da_add_layernorm_fwd": [_p, _p, _i32, _p, _p, _i64, _i64, _f32, _p, _p, _i32, _p, _p, _p],
     "da_add_layernorm_bwd": [_p, _i32, _p, _p, _p, _p, _p, _i64, _i64, _p, _p, _i32, _p, _i32, _p, _p, _p],
     "da_layernorm_bwd_blocks": [_i64],
+    "da_norm_int8": [_p, _i32, _i64, _p, _i32, _i64, _p, _i32, _p, _i32, _i32, _i64, _i64, _f32, _p, _i64, _p, _i64,
+                     _p, _p],
+    "da_dequant_int8": [_p, _i64, _p, _i64, _i64, _p, _i32, _i64, _p],
+    "da_gemm_i8": [_p, _i64, _p, _p, _i64, _p, _p, _i32, _i32, _p, _i64, _i32, _i64, _i64, _i64, _p, _p],
+    "da_checkpoint8": [_p, _i32, _i64, _i64, _i64, _i32, _p, _i64, _p, _p, _p],
+    "da_checkpoint8_restore": [_p, _p, _i64, _i64, _p, _i32, _i64, _p],
+    "da_checkpoint8_gelu_bwd": [_p, _i32, _i64, _p, _p, _i64, _i64, _p, _i64, _p, _i64, _p],
+    "da_checkpoint8_wgrad_workspace_elems": [_i64, _i64, _i64],  # returns int64 (set below)
+    "da_checkpoint8_wgrad": [_p, _i32, _i64, _p, _p, _i64, _i64, _i64, _p, _i32, _i64, _p, _i64, _p, _p],
 }
 
 _lock = threading.Lock()
@@ -132,6 +141,7 @@ def lib() -> ctypes.CDLL:
             handle.da_attn_fwd_workspace_size.restype = ctypes.c_int64
             handle.da_gemm_splitk_workspace_elems.restype = ctypes.c_int64
             handle.da_col_sum_workspace_elems.restype = ctypes.c_int64
+            handle.da_checkpoint8_wgrad_workspace_elems.restype = ctypes.c_int64
             handle.da_kernel_launches.argtypes = []
             handle.da_kernel_launches.restype = ctypes.c_uint64
             _lib = handle

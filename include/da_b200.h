@@ -480,6 +480,63 @@ DA_API int da_add_layernorm_bwd(const void* dy, int dy_dtype, const float* d_res
                                 float* dx, void* d_branch, int branch_dtype, float* partial, int partial_blocks,
                                 float* dgamma, float* dbeta, void* stream);
 
+/* ---- eight-bit operators ----------------------------------------------
+ * No reference counterpart: an int8 serving path for the layers around the
+ * routed attention (norms modules.py:294-356, Linear layers :143-157, :212, :272,
+ * :339-346) and 8-bit activation checkpoints for their training. */
+
+/* int8 rows with a scale each: row r of [rows, D] stands for q[r, :] * scale[r].
+ *   kind 0 (quantise)   y = x
+ *   kind 1 (RMS norm)   y = r w / sqrt(mean(r^2) + eps)
+ *   kind 2 (LayerNorm)  y = (r - mean) / sqrt(var + eps) * w + b
+ * with r = x + branch rounded to x's dtype (branch null: r = x; else r is also
+ * written to x_out in x's dtype), scale = max|y| / 127, q = rint(y / scale).  weight
+ * [D] may be null (kinds 1 and 2), bias [D] too (kind 2, with weight).  A row whose
+ * largest |y| (kind 1: |r w|) is at most 1e-36 becomes q = 0, scale = 0; a row
+ * holding NaN or infinity gets a NaN or infinite scale.  x, branch, weight and bias
+ * in any of DA_F16 / DA_BF16 / DA_F32, row strides ldx, ldb, ldo, ldq in elements, any
+ * alignment (16-byte aligned rows with D a multiple of 8 take vector accesses). */
+DA_API int da_norm_int8(const void* x, int x_dtype, int64_t ldx, const void* branch, int branch_dtype, int64_t ldb,
+                        const void* weight, int weight_dtype, const void* bias, int bias_dtype, int kind,
+                        int64_t rows, int64_t D, float eps, void* x_out, int64_t ldo, int8_t* q, int64_t ldq,
+                        float* scale, void* stream);
+/* out [rows, D] = q * scale in out_dtype. */
+DA_API int da_dequant_int8(const int8_t* q, int64_t ldq, const float* scale, int64_t rows, int64_t D, void* out,
+                           int out_dtype, int64_t ldo, void* stream);
+/* C[m, n] = f((sum_k A[m, k] B[n, k]) a_scale[m] b_scale[n] + bias[n]): A [M, K] and
+ * B [N, K] int8 row-major, 16-byte aligned with row strides multiples of 16; the sum
+ * exact in int32 (K at most 131071); f identity (gelu = 0) or GELU; bias [N] in
+ * bias_dtype or null; C row-major in c_dtype, any alignment. */
+DA_API int da_gemm_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, int64_t ldb,
+                      const float* b_scale, const void* bias, int bias_dtype, int gelu, void* C, int64_t ldc,
+                      int c_dtype, int64_t M, int64_t N, int64_t K, int* status, void* stream);
+
+/* 8-bit checkpoint of x [rows, D] (fp16 / bf16): q [rows, ceil(D / 32) * 32] int8
+ * (16-byte aligned, dense, columns past D zero) and e [rows, ceil(D / 32)] int8 with
+ * x ~ q * 2^e, e shared by 32 columns: the smallest that covers the block's largest
+ * |x| with 127, within [-24, 9] for fp16 and [-126, 121] for bf16; e = -128 marks a
+ * block that held a NaN or an infinity and decodes to NaN.  With gelu set, h = GELU(x)
+ * in x's dtype too (else h may be null). */
+DA_API int da_checkpoint8(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t D, int gelu, void* h,
+                          int64_t ldh, int8_t* q, int8_t* e, void* stream);
+/* out [rows, D] = q * 2^e in dtype (exact in the dtype that was checkpointed, and in fp32). */
+DA_API int da_checkpoint8_restore(const int8_t* q, const int8_t* e, int64_t rows, int64_t D, void* out, int dtype,
+                                  int64_t ldo, void* stream);
+/* GELU backward from the checkpoint of its input z: dz = dh * GELU'(z), and h = GELU(z)
+ * when h is not null; dh, dz and h in dtype (fp16 / bf16). */
+DA_API int da_checkpoint8_gelu_bwd(const void* dh, int dtype, int64_t lddh, const int8_t* q, const int8_t* e,
+                                   int64_t rows, int64_t D, void* dz, int64_t lddz, void* h, int64_t ldh,
+                                   void* stream);
+/* Weight gradient from the checkpoint of the layer's input: out[n, k] = sum over the
+ * rows of dy[t, n] * q[t, k] 2^e[t, k / 32], accumulated in fp32 and stored in fp32 or
+ * dy's dtype; dy [rows, N] 16-byte aligned with ldy a multiple of 8.  The rows' partial
+ * sums go to `workspace` (fp32, da_checkpoint8_wgrad_workspace_elems elements, else
+ * DA_ERR_WORKSPACE) and are added in a fixed order: bit-reproducible. */
+DA_API int64_t da_checkpoint8_wgrad_workspace_elems(int64_t rows, int64_t N, int64_t K);
+DA_API int da_checkpoint8_wgrad(const void* dy, int dtype, int64_t ldy, const int8_t* q, const int8_t* e,
+                                int64_t rows, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,
+                                float* workspace, int64_t workspace_elems, int* status, void* stream);
+
 /* ---- building-block check -------------------------------------------
  * No reference counterpart: D[128, n] = A[128, k] * B^T computed by one
  * tcgen05 tile (cta_group 1 or 2) for testing the descriptor layouts.
