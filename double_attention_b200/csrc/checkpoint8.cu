@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p, bool
     if ((c & 3) == 0) p.e[(row * p.per_row.d + c) >> 2] = (int8_t)(finite ? e : kNotFinite);
     if (p.gelu) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = gelu8(v[j]);
+      for (int j = 0; j < 8; j += 2) gelu2(v[j], v[j + 1]);
       store_row8(p.h, p.dtype, row * p.ldh, col, p.D, vec_h, v);
     }
   }
@@ -133,10 +133,11 @@ __global__ void __launch_bounds__(256) checkpoint8_gelu_bwd_kernel(const CkptArg
     load_row8(p.x, p.dtype, row * p.ldx, col, p.D, vec_x, d);
     restore8(p, row * p.per_row.d + c, z);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const NormalCdf n = normal_cdf(z[j]);
-      d[j] *= fmaf(z[j] * n.density, 0.39894228040143268f, n.cdf);
-      z[j] *= n.cdf;
+    for (int j = 0; j < 8; j += 2) {
+      float s0, s1;
+      gelu_grad2(z[j], z[j + 1], s0, s1);
+      d[j] *= s0;
+      d[j + 1] *= s1;
     }
     store_row8(p.dz, p.dtype, row * p.lddz, col, p.D, vec_dz, d);
     if (p.h) store_row8(p.h, p.dtype, row * p.ldh, col, p.D, vec_h, z);

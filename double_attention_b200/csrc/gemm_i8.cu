@@ -3,8 +3,6 @@
 // A [M, K] are int8 activations with a scale per token, B [N, K] int8 weights with a scale per output
 // channel.  The sum is exact in int32 (|A|, |B| <= 128 and K <= 131071), so any split of K and any order give
 // the same bits; it is converted to fp32, scaled and rounded once to C's dtype.
-//
-// 64 x 64 tiles, dp4a on operands staged in shared memory, 4 x 4 outputs per thread.
 #include "common.cuh"
 #include "host_util.h"
 #include "vec8.cuh"
@@ -23,45 +21,270 @@ struct Params {
   void* c;
   int64_t lda, ldb, ldc;
   int M, N, K, bias_dtype, c_dtype, gelu;
+  int tma_c;  // C's rows take TMA stores (16-byte aligned base and stride)
+  int* status;
 };
 
-__global__ void __launch_bounds__(256) gemm_kernel(const Params p) {
-  __shared__ int sa[16][65], sb[16][65];  // [K group of 4][row]
+// One output before its rounding to C's dtype: every kernel here computes exactly this.
+DA_DEV float finish(int acc, float sa, float sb, float bias) { return __fmaf_rn(__fmul_rn((float)acc, sa), sb, bias); }
+
+DA_DEV float col_bias(const Params& p, int n) { return p.bias ? load1(p.bias, p.bias_dtype, n) : 0.f; }
+
+// ----------------------------------------------------------------------------------------------- large products
+// Persistent CTA pairs: a pair computes 256 x 256 tiles (each CTA 128 rows of A and, of every K stage, half of
+// B's rows) with cta_group::2 kind::i8 instructions of 256 x 256 x 32; two int32 accumulators of 256 TMEM columns
+// each, so that the epilogue of one tile runs under the products of the next.
+// A stage holds 128 bytes of K (5 stages of 32 KB; 3 stages of 64 KB measured the same).
+struct Pair {
+  static constexpr int kTile = 256;  // rows and columns of a pair's tile
+  static constexpr int kOperand = 128 * 128;
+  static constexpr int kStageBytes = 2 * kOperand;
+  static constexpr int kStages = 5;
+  static constexpr int kBuffers = 2;  // 4 KB output boxes per epilogue warp
+  static constexpr int kEpilogueWarps = 8;
+  static constexpr int kOff = kStages * kStageBytes;
+  static constexpr int kSmem = kOff + kEpilogueWarps * kBuffers * 4096;
+  static constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // warps 0, 2 TMA; 1 MMA; 3 idle; then the epilogue
+  static constexpr int kGroupM = 8;  // row tiles that run through the columns together (A and B stay in L2)
+};
+
+template <int kOut, bool kGelu>
+__global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __grid_constant__ CUtensorMap ta,
+                                                                              const __grid_constant__ CUtensorMap tb,
+                                                                              const __grid_constant__ CUtensorMap tc,
+                                                                              const Params p) {
+  using C = Pair;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[C::kStages], empty[C::kStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = (int)(cluster_ctarank() & 1u);
+  const int m_tiles = (p.M + C::kTile - 1) / C::kTile, n_tiles = (p.N + C::kTile - 1) / C::kTile;
+  const int tiles = m_tiles * n_tiles, pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+  const int my_tiles = pair < tiles ? (tiles - 1 - pair) / pairs + 1 : 0;
+  const int nk = (p.K + 127) / 128;
+  Abort ab{&abort_flag, p.status};
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * C::kEpilogueWarps);  // every epilogue warp of both CTAs
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc<2>(&tmem_base, 2 * C::kTile);
+    tmem_relinquish<2>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
   grid_dependency_wait();
   grid_launch_dependents();
-  const int64_t m0 = (int64_t)blockIdx.x * 64;
-  const int n0 = blockIdx.y * 64;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < p.K; k0 += 64) {
-    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-      const int r = i / 16, g = i % 16, k = k0 + g * 4;
-      int va = 0, vb = 0;
-      for (int e = 0; e < 4; ++e) {
-        if (k + e < p.K && m0 + r < p.M) va |= (int)(uint8_t)p.a[(m0 + r) * p.lda + k + e] << (8 * e);
-        if (k + e < p.K && n0 + r < p.N) vb |= (int)(uint8_t)p.b[(int64_t)(n0 + r) * p.ldb + k + e] << (8 * e);
+  const uint32_t tmem = tmem_base;
+  auto tile_mn = [&](int i, int& m0, int& n0) {
+    const int t = pair + i * pairs;
+    const int group = t / (C::kGroupM * n_tiles), in = t - group * C::kGroupM * n_tiles;
+    const int height = min(C::kGroupM, m_tiles - group * C::kGroupM);
+    m0 = (group * C::kGroupM + in % height) * C::kTile;
+    n0 = in / height * C::kTile;
+  };
+
+  if ((warp == 0 || warp == 2) && lane == 0) {
+    // ---------------------------------------------------------------- TMA producers (alternate stages)
+    const int pi = warp == 0 ? 0 : 1;
+    prefetch_tmap(&ta);
+    prefetch_tmap(&tb);
+    bool ok = true;
+    int it = 0, last = -1;
+    for (int i = 0; ok && i < my_tiles; ++i) {
+      int m0, n0;
+      tile_mn(i, m0, n0);
+      for (int kb = 0; kb < nk; ++kb, ++it) {
+        if ((it & 1) != pi) continue;
+        const int s = it % C::kStages;
+        if (!mbar_wait(&empty[s], ((it / C::kStages) & 1u) ^ 1u, ab, 71)) { ok = false; break; }
+        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * C::kStageBytes);
+        const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+        uint8_t* sa = smem + s * C::kStageBytes;
+        tma_load_2d_pair(&ta, bar, sa, kb * 128, m0 + rank * 128);
+        tma_load_2d_pair(&tb, bar, sa + C::kOperand, kb * 128, n0 + rank * 128);
+        last = it;
       }
-      sa[g][r] = va;
-      sb[g][r] = vb;
     }
-    __syncthreads();
-    for (int g = 0; g < 16; ++g)
+    // After a wait that gave up, this producer's loads in flight.  (Otherwise every load has been consumed before
+    // the epilogue's last tile; and a stage's phase may have moved on by two, which a wait would not notice.)
+    if (rank == 0 && !ok)
+      for (int j = (last - C::kStages + 1 > 0 ? last - C::kStages + 1 : 0); j <= last; ++j)
+        if ((j & 1) == pi) mbar_wait_drain(&full[j % C::kStages], (j / C::kStages) & 1u);
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ---------------------------------------------------------------- MMA issuer (leader)
+    const uint32_t idesc = idesc_i8(C::kTile, C::kTile);
+    bool ok = true;
+    int it = 0;
+    for (int i = 0; ok && i < my_tiles; ++i) {
+      const int buf = i & 1;
+      if (i >= 2 && !mbar_wait(&acc_empty[buf], ((i >> 1) - 1) & 1u, ab, 72)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + buf * C::kTile;
+      for (int kb = 0; kb < nk; ++kb, ++it) {
+        const int s = it % C::kStages;
+        if (!mbar_wait(&full[s], (it / C::kStages) & 1u, ab, 73)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t sa = smem_u32(smem + s * C::kStageBytes);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int k = 0; k < 4; ++k)
+          mma_i8_ss<2>(d, sdesc_sw128(sa + k * 32, 16, 1024), sdesc_sw128(sa + C::kOperand + k * 32, 16, 1024), idesc,
+                       (kb > 0 || k > 0) ? 1u : 0u);
+        mma_commit_pair(smem_u32(&empty[s]));
+      }
+      if (ok) mma_commit_pair(smem_u32(&acc_full[buf]));
+    }
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------------- epilogue: a warp takes 32 rows x 128 columns
+    const int quad = warp & 3, half = (warp - 4) / 4;
+    uint8_t* box = smem + C::kOff + (warp - 4) * C::kBuffers * 4096;
+    const bool vec_cols = reinterpret_cast<uintptr_t>(p.sb) % 16 == 0 &&
+                          (!p.bias || (p.bias_dtype == DA_F32 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0));
+    constexpr int per_box = kOut == DA_F32 ? 32 : 64;  // columns in 128 bytes
+    int boxes = 0;
+    bool ok = true;
+    for (int i = 0; i < my_tiles; ++i) {
+      const int buf = i & 1;
+      int m0, n0;
+      tile_mn(i, m0, n0);
+      const int row0 = m0 + rank * 128 + quad * 32, row = row0 + lane;
+      const float sa = row < p.M ? p.sa[row] : 0.f;
+      if (ok) ok = mbar_wait(&acc_full[buf], (i >> 1) & 1u, ab, 74);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      if (ok) {
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+          const int col = n0 + half * 128 + c;
+          float v[32];
+          tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + buf * C::kTile + half * 128 + c, v);
+          tmem_wait_ld();
+          if (c == 96) {  // the last columns of this accumulator are in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[buf]), 0));
+          }
+          if (col >= p.N || row0 >= p.M) continue;
+          if (vec_cols && col + 32 <= p.N) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sa[g][ty + 16 * i], sb[g][tx + 16 * j], acc[i][j]);
-    __syncthreads();
+            for (int e = 0; e < 32; e += 4) {
+              const float4 s = __ldg(reinterpret_cast<const float4*>(p.sb + col + e));
+              float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (p.bias) b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + col + e));
+              v[e] = finish(__float_as_int(v[e]), sa, s.x, b.x);
+              v[e + 1] = finish(__float_as_int(v[e + 1]), sa, s.y, b.y);
+              v[e + 2] = finish(__float_as_int(v[e + 2]), sa, s.z, b.z);
+              v[e + 3] = finish(__float_as_int(v[e + 3]), sa, s.w, b.w);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              v[e] = col + e < p.N ? finish(__float_as_int(v[e]), sa, p.sb[col + e], col_bias(p, col + e)) : 0.f;
+          }
+          if constexpr (kGelu) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) gelu2(v[e], v[e + 1]);
+          }
+          const bool first = c % per_box == 0;
+          if (first) {  // a free output box
+            if (lane == 0) tma_store_wait_read<C::kBuffers - 1>();
+            __syncwarp();
+          }
+          const uint32_t dst = smem_u32(box + boxes % C::kBuffers * 4096);
+          if constexpr (kOut == DA_F32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              st_shared_v4(dst + sw128_offset(lane, e), __float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]),
+                           __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3]));
+          } else {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              w[e] = kOut == DA_BF16 ? pack_bf16x2(v[2 * e], v[2 * e + 1]) : pack_f16x2(v[2 * e], v[2 * e + 1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              st_shared_v4(dst + sw128_offset(lane, (first ? 0 : 4) + e), w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+          }
+          if ((c + 32) % per_box != 0 && col + 32 < p.N) continue;  // the box's second half follows
+          const int col0 = first ? col : col - 32;
+          if (p.tma_c) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tc, box + boxes % C::kBuffers * 4096, col0, row0);
+              tma_store_commit();
+            }
+          } else {  // rows of C that no TMA store takes: lanes along the columns
+            __syncwarp();
+            const int cols = min(per_box, p.N - col0), rows = min(32, p.M - row0);
+            const uint8_t* b = box + boxes % C::kBuffers * 4096;
+            for (int r = 0; r < rows; ++r)
+              for (int e = lane; e < cols; e += 32) {
+                const int64_t at = (int64_t)(row0 + r) * p.ldc + col0 + e;
+                if constexpr (kOut == DA_F32)
+                  static_cast<float*>(p.c)[at] = *reinterpret_cast<const float*>(b + sw128_offset(r, e / 4) + e % 4 * 4);
+                else
+                  static_cast<uint16_t*>(p.c)[at] = *reinterpret_cast<const uint16_t*>(b + sw128_offset(r, e / 8) + e % 8 * 2);
+              }
+            __syncwarp();
+          }
+          ++boxes;
+        }
+      }
+    }
+    if (lane == 0) tma_store_wait_all();
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty + 16 * i;
-      const int n = n0 + tx + 16 * j;
-      if (m >= p.M || n >= p.N) continue;
-      float y = (float)acc[i][j] * p.sa[m] * p.sb[n];
-      if (p.bias) y += load1(p.bias, p.bias_dtype, n);
-      if (p.gelu) y = gelu8(y);
-      store1(p.c, p.c_dtype, m * p.ldc + n, y);
-    }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 1) tmem_dealloc<2>(tmem, 2 * C::kTile);
+}
+
+template <int kOut, bool kGelu>
+int launch_pair(const Params& p, cudaStream_t st) {
+  using C = Pair;
+  constexpr int elem = kOut == DA_F32 ? 4 : 2;
+  CUtensorMap ta, tb, tc;
+  if (int rc = make_tmap_2d(&ta, p.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.M, p.lda, 128, 128)) return rc;
+  if (int rc = make_tmap_2d(&tb, p.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.N, p.ldb, 128, 128)) return rc;
+  tc = ta;
+  if (p.tma_c) {
+    const CUtensorMapDataType dt = kOut == DA_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : kOut == DA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if (int rc = make_tmap_2d(&tc, p.c, dt, elem, p.N, p.M, (uint64_t)p.ldc * elem, 128 / elem, 32)) return rc;
+  }
+  auto kern = gemm_pair_kernel<kOut, kGelu>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem + 1024) != cudaSuccess)
+    return record_cuda_error();
+  const int64_t tiles = (int64_t)((p.M + C::kTile - 1) / C::kTile) * ((p.N + C::kTile - 1) / C::kTile);
+  const int pairs = tiles < sm_count() / 2 ? (int)tiles : sm_count() / 2;
+  return launch_kernel(kern, dim3(2 * pairs), dim3(C::kThreads), C::kSmem + 1024, st, true, ta, tb, tc, p);
+}
+
+int dispatch_pair(const Params& p, cudaStream_t st) {
+  switch (p.c_dtype * 2 + (p.gelu ? 1 : 0)) {
+    case DA_F16 * 2: return launch_pair<DA_F16, false>(p, st);
+    case DA_F16 * 2 + 1: return launch_pair<DA_F16, true>(p, st);
+    case DA_BF16 * 2: return launch_pair<DA_BF16, false>(p, st);
+    case DA_BF16 * 2 + 1: return launch_pair<DA_BF16, true>(p, st);
+    case DA_F32 * 2: return launch_pair<DA_F32, false>(p, st);
+    default: return launch_pair<DA_F32, true>(p, st);
+  }
 }
 
 }  // namespace i8
@@ -72,14 +295,19 @@ extern "C" int da_gemm_i8(const int8_t* A, int64_t lda, const float* a_scale, co
                           int c_dtype, int64_t M, int64_t N, int64_t K, int* status, void* stream) {
   using namespace da;
   if (!A || !B || !a_scale || !b_scale || !C || !status) return DA_ERR_NULL;
-  if (M <= 0 || N <= 0 || K <= 0 || K > i8::kMaxK || M > 0x7fffffffLL || N > 0x3fffffLL || lda < K || ldb < K || ldc < N)
+  // (the tile count stays an int)
+  if (M <= 0 || N <= 0 || K <= 0 || K > i8::kMaxK || M > 0x3fffffffLL || N > 0x3fffffffLL || lda < K || ldb < K ||
+      ldc < N || ((M + 255) / 256) * ((N + 255) / 256) > 0x3fffffffLL)
     return DA_ERR_SHAPE;
   if (c_dtype < DA_F16 || c_dtype > DA_F32 || (bias && (bias_dtype < DA_F16 || bias_dtype > DA_F32)))
     return DA_ERR_DTYPE;
   if (lda % 16 || ldb % 16 || reinterpret_cast<uintptr_t>(A) % 16 || reinterpret_cast<uintptr_t>(B) % 16)
     return DA_ERR_ALIGN;
   if (int rc = bind_device(A)) return rc;
-  const i8::Params p{A, B, a_scale, b_scale, bias, C, lda, ldb, ldc, (int)M, (int)N, (int)K, bias_dtype, c_dtype, gelu};
-  const dim3 grid((unsigned)((M + 63) / 64), (unsigned)((N + 63) / 64));
-  return launch_kernel(i8::gemm_kernel, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), false, p);
+  const int elem = c_dtype == DA_F32 ? 4 : 2;
+  const int tma_c = reinterpret_cast<uintptr_t>(C) % 16 == 0 && ldc * elem % 16 == 0;
+  const i8::Params p{A,      B,      a_scale, b_scale,    bias,    C,    lda,   ldb,   ldc,
+                     (int)M, (int)N, (int)K,  bias_dtype, c_dtype, gelu, tma_c, status};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return i8::dispatch_pair(p, st);
 }

@@ -95,24 +95,75 @@ DA_DEV void unpack_s8x8(uint2 w, float* v) {
     v[e] = __uint_as_float(__byte_perm(u[e >> 2], 0x4b000000u, 0x7540 | (e & 3))) - 8388736.f;
 }
 
-// GELU in its exact form, z times the normal distribution function, and its derivative.  The distribution
-// function comes from Hastings' approximation of erfc (Abramowitz and Stegun 7.1.26, absolute error at
-// most 1.5e-7): with x = |z| / sqrt(2) and t = 1 / (1 + 0.3275911 x), erfc(x) = t (a1 + ... + a5 t^4) exp(-x^2),
-// whose exponential is the density that the derivative needs too.
-struct NormalCdf {
-  float cdf, density;  // Phi(z), and exp(-z^2 / 2) without its factor 1 / sqrt(2 pi)
+// Two fp32 values in one register pair; multiplications and additions of pairs take one issue slot.
+struct F2 {
+  unsigned long long v;
 };
-DA_DEV NormalCdf normal_cdf(float z) {
-  const float x = fabsf(z) * 0.70710678118654752f;
-  const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-  float poly = fmaf(1.061405429f, t, -1.453152027f);
-  poly = fmaf(poly, t, 1.421413741f);
-  poly = fmaf(poly, t, -0.284496736f);
-  poly = fmaf(poly, t, 0.254829592f);
-  const float density = ex2(z * z * -0.72134752044448170f);  // exp(-z^2 / 2)
-  const float tail = 0.5f * poly * t * density;              // Phi(-|z|)
-  return {z >= 0.f ? 1.f - tail : tail, density};
+DA_DEV F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
 }
-DA_DEV float gelu8(float z) { return z * normal_cdf(z).cdf; }
+DA_DEV void split(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+DA_DEV F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+DA_DEV F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+DA_DEV F2 dup(float a) { return f2(a, a); }
+
+// The lower tail of the normal distribution, Phi(-|z|), and its density without the factor 1 / sqrt(2 pi), for
+// two values: Hastings' approximation of erfc (Abramowitz and Stegun 7.1.26, absolute error at most 1.5e-7).
+// With x = |z| / sqrt(2) and t = 1 / (1 + 0.3275911 x), erfc(x) = t (a1 + ... + a5 t^4) exp(-x^2), and Phi(-|z|) is
+// half of it; the exponential is the density that GELU's derivative needs too.  The two reciprocals come from
+// one, of their product (|z| is cut at 1e4, where the density is 0): the special-function unit, 16 lanes a clock
+// against 128 for additions, is what bounds an epilogue with GELU.
+constexpr float kCut = 1e4f;
+DA_DEV void normal_tail2(float z0, float z1, F2& tail, F2& density) {
+  const F2 z = f2(z0, z1);
+  const F2 arg = mul2(mul2(z, dup(-0.72134752044448170f)), z);  // -z^2 / 2 in base 2
+  const F2 a = fma2(f2(fminf(fabsf(z0), kCut), fminf(fabsf(z1), kCut)), dup(0.23164188f), dup(1.f));
+  float a0, a1, g0, g1;
+  split(a, a0, a1);
+  split(arg, g0, g1);
+  const F2 t = mul2(dup(__fdividef(1.f, a0 * a1)), f2(a1, a0));
+  density = f2(ex2(g0), ex2(g1));
+  F2 poly = fma2(t, dup(0.5f * 1.061405429f), dup(0.5f * -1.453152027f));
+  poly = fma2(poly, t, dup(0.5f * 1.421413741f));
+  poly = fma2(poly, t, dup(0.5f * -0.284496736f));
+  poly = fma2(poly, t, dup(0.5f * 0.254829592f));
+  tail = mul2(mul2(poly, t), density);
+}
+
+// GELU in its exact form: z Phi(z) = max(z, 0) - |z| Phi(-|z|); an infinity keeps its limit, inf or 0.
+DA_DEV float gelu_of(float z, float tail) {
+  return fmaf(-fminf(fabsf(z), kCut), tail, fmaxf(z, 0.f));  // (NaN: max is 0, but the tail is NaN)
+}
+DA_DEV void gelu2(float& z0, float& z1) {
+  F2 tail, density;
+  normal_tail2(z0, z1, tail, density);
+  float t0, t1;
+  split(tail, t0, t1);
+  z0 = gelu_of(z0, t0);
+  z1 = gelu_of(z1, t1);
+}
+
+// GELU'(z) = Phi(z) + z density / sqrt(2 pi), and z becomes GELU(z).
+DA_DEV void gelu_grad2(float& z0, float& z1, float& s0, float& s1) {
+  F2 tail, density;
+  normal_tail2(z0, z1, tail, density);
+  float t0, t1, d0, d1;
+  split(tail, t0, t1);
+  split(mul2(mul2(density, dup(0.39894228040143268f)), f2(z0, z1)), d0, d1);
+  s0 = d0 + (z0 > 0.f ? 1.f - t0 : t0);
+  s1 = d1 + (z1 > 0.f ? 1.f - t1 : t1);
+  z0 = gelu_of(z0, t0);
+  z1 = gelu_of(z1, t1);
+}
 
 }  // namespace da
