@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
           if (c == 96) {  // the last columns of this accumulator are in registers
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[buf]), 0));
+            if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&acc_empty[buf]), 0));
           }
           if (col >= p.N || row0 >= p.M) continue;
           if (vec_cols && col + 32 <= p.N) {
