@@ -40,10 +40,9 @@ struct Pair {
   static constexpr int kOperand = 128 * 128;
   static constexpr int kStageBytes = 2 * kOperand;
   static constexpr int kStages = 5;
-  static constexpr int kBuffers = 2;  // 4 KB output boxes per epilogue warp
-  static constexpr int kEpilogueWarps = 8;
+  static constexpr int kEpilogueWarps = 16;
   static constexpr int kOff = kStages * kStageBytes;
-  static constexpr int kSmem = kOff + kEpilogueWarps * kBuffers * 4096;
+  static constexpr int kSmem = kOff + kEpilogueWarps * 4096  /* an output box per epilogue warp */;
   static constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // warps 0, 2 TMA; 1 MMA; 3 idle; then the epilogue
   static constexpr int kGroupM = 8;  // row tiles that run through the columns together (A and B stay in L2)
 };
@@ -149,13 +148,12 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
       if (ok) mma_commit_pair(smem_u32(&acc_full[buf]));
     }
   } else if (warp >= 4) {
-    // ---------------------------------------------------------------- epilogue: a warp takes 32 rows x 128 columns
-    const int quad = warp & 3, half = (warp - 4) / 4;
-    uint8_t* box = smem + C::kOff + (warp - 4) * C::kBuffers * 4096;
+    // ---------------------------------------------------------------- epilogue: a warp takes 32 rows x 64 columns
+    const int quad = warp & 3, part = (warp - 4) / 4;
+    uint8_t* box = smem + C::kOff + (warp - 4) * 4096;
     const bool vec_cols = reinterpret_cast<uintptr_t>(p.sb) % 16 == 0 &&
                           (!p.bias || (p.bias_dtype == DA_F32 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0));
     constexpr int per_box = kOut == DA_F32 ? 32 : 64;  // columns in 128 bytes
-    int boxes = 0;
     bool ok = true;
     for (int i = 0; i < my_tiles; ++i) {
       const int buf = i & 1;
@@ -168,12 +166,12 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
       tc_fence_after();
       if (ok) {
 #pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          const int col = n0 + half * 128 + c;
+        for (int c = 0; c < 64; c += 32) {
+          const int col = n0 + part * 64 + c;
           float v[32];
-          tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + buf * C::kTile + half * 128 + c, v);
+          tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + buf * C::kTile + part * 64 + c, v);
           tmem_wait_ld();
-          if (c == 96) {  // the last columns of this accumulator are in registers
+          if (c == 32) {  // the last columns of this accumulator are in registers
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&acc_empty[buf]), 0));
@@ -201,10 +199,10 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
           }
           const bool first = c % per_box == 0;
           if (first) {  // a free output box
-            if (lane == 0) tma_store_wait_read<C::kBuffers - 1>();
+            if (lane == 0) tma_store_wait_read<0>();
             __syncwarp();
           }
-          const uint32_t dst = smem_u32(box + boxes % C::kBuffers * 4096);
+          const uint32_t dst = smem_u32(box);
           if constexpr (kOut == DA_F32) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -225,13 +223,13 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
-              tma_store_2d(&tc, box + boxes % C::kBuffers * 4096, col0, row0);
+              tma_store_2d(&tc, box, col0, row0);
               tma_store_commit();
             }
           } else {  // rows of C that no TMA store takes: lanes along the columns
             __syncwarp();
             const int cols = min(per_box, p.N - col0), rows = min(32, p.M - row0);
-            const uint8_t* b = box + boxes % C::kBuffers * 4096;
+            const uint8_t* b = box;
             for (int r = 0; r < rows; ++r)
               for (int e = lane; e < cols; e += 32) {
                 const int64_t at = (int64_t)(row0 + r) * p.ldc + col0 + e;
@@ -242,7 +240,6 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
               }
             __syncwarp();
           }
-          ++boxes;
         }
       }
     }
@@ -287,6 +284,222 @@ int dispatch_pair(const Params& p, cudaStream_t st) {
   }
 }
 
+// ----------------------------------------------------------------------------------------------- few tokens
+// Up to a few hundred tokens the weights' bytes and the length of one CTA's chain of K stages set the time, not the
+// products.  Here the output channels are the instruction's 128 rows and the tokens its columns (kTn of them, so
+// one token costs a 128 x 16 instruction, not 128 x 256), and the K stages of a tile are split over a cluster of
+// up to 8 CTAs: each leaves its int32 sums in shared memory, and after a cluster barrier every CTA adds all of the
+// cluster's sums for its share of the tokens through distributed shared memory (exact, so in any order) and
+// stores them.
+template <int kTn>
+struct Few {
+  static constexpr int kStageBytes = (128 + kTn) * 128;
+  static constexpr int kStages = kTn == 128 ? 6 : 8;
+  static constexpr int kSumBytes = kTn * 128 * 4;  // aliases the stages, which every product has read by then
+  static constexpr int kSmem = kStages * kStageBytes;
+  static constexpr int kCols = kTn < 32 ? 32 : kTn;  // TMEM columns
+  static constexpr int kThreads = 192;               // warp 0 TMA, 1 MMA, 2-5 epilogue
+  static_assert(kSumBytes <= kSmem);
+};
+
+template <int kTn, int kSplits>
+__global__ void __launch_bounds__(Few<kTn>::kThreads, 1) gemm_few_kernel(const __grid_constant__ CUtensorMap ta,
+                                                                         const __grid_constant__ CUtensorMap tb,
+                                                                         const Params p) {
+  using C = Few<kTn>;
+  constexpr int splits = kSplits;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[C::kStages], empty[C::kStages], done;
+  __shared__ float scale[kTn];
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
+  const int n_tiles = (p.N + 127) / 128;
+  const int n0 = tile % n_tiles * 128, m0 = tile / n_tiles * kTn;
+  const int nk_all = (p.K + 127) / 128, per = (nk_all + splits - 1) / splits;
+  const int kb0 = rank * per, nk = max(0, min(per, nk_all - kb0));
+  Abort ab{&abort_flag, p.status};
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(&tmem_base, C::kCols);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const uint32_t tmem = tmem_base;
+  int ch_n = p.N;  // an epilogue thread's first channel, the scales and biases of its two
+  float s0 = 0.f, s1 = 0.f, b0 = 0.f, b1 = 0.f;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      int kb = 0;
+      for (; kb < nk; ++kb) {
+        const int s = kb % C::kStages;
+        if (!mbar_wait(&empty[s], ((kb / C::kStages) & 1u) ^ 1u, ab, 75)) { ok = false; break; }
+        mbar_arrive_expect_tx(&full[s], C::kStageBytes);
+        tma_load_2d(&tb, &full[s], smem + s * C::kStageBytes, (kb0 + kb) * 128, n0);
+        tma_load_2d(&ta, &full[s], smem + s * C::kStageBytes + 128 * 128, (kb0 + kb) * 128, m0);
+      }
+      for (int j = max(0, kb - C::kStages); !ok && j < kb; ++j)
+        mbar_wait_drain(&full[j % C::kStages], (j / C::kStages) & 1u);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int kb = 0; kb < nk; ++kb) {
+        const int s = kb % C::kStages;
+        ok = mbar_wait(&full[s], (kb / C::kStages) & 1u, ab, 76);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t sw = smem_u32(smem + s * C::kStageBytes), sx = sw + 128 * 128;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_i8_ss<1>(tmem, sdesc_sw128(sw + k * 32, 16, 1024), sdesc_sw128(sx + k * 32, 16, 1024), idesc_i8(128, kTn),
+                       (kb > 0 || k > 0) ? 1u : 0u);
+        mma_commit<1>(smem_u32(&empty[s]));
+      }
+      mma_commit<1>(smem_u32(&done));
+      if (!ok) mbar_wait_drain(&done, 0);
+    }
+  } else {
+    const int quad = warp & 3, t = threadIdx.x - 64;
+    // what the stores need, fetched under the products
+    for (int i = t; i < kTn; i += 128) scale[i] = m0 + i < p.M ? p.sa[m0 + i] : 0.f;
+    ch_n = n0 + t % 64 * 2;
+    if (ch_n < p.N) {
+      s0 = p.sb[ch_n];
+      b0 = col_bias(p, ch_n);
+    }
+    if (ch_n + 1 < p.N) {
+      s1 = p.sb[ch_n + 1];
+      b1 = col_bias(p, ch_n + 1);
+    }
+    bool ok = mbar_wait(&done, 0, ab, 77);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    // sums [token][channel]
+    int* sums = reinterpret_cast<int*>(smem);
+#pragma unroll 1
+    for (int c = 0; c < kTn; c += 16) {
+      float v[16];
+      tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + c, v);
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sums[(c + e) * 128 + quad * 32 + lane] = ok && nk > 0 ? __float_as_int(v[e]) : 0;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (splits > 1) cluster_sync();
+  if (warp >= 2 && ch_n < p.N) {
+    // a thread takes two neighbouring channels of every second token of this CTA's share, kAtOnce tokens together
+    constexpr int kAtOnce = kSplits == 8 ? 2 : 4;
+    const int t = threadIdx.x - 64;
+    const int tokens = min(kTn, p.M - m0), share = (tokens + splits - 1) / splits;
+    const int last = min(tokens, (rank + 1) * share);
+    const int elem = p.c_dtype == DA_F32 ? 4 : 2;
+    const bool two = ch_n + 1 < p.N;
+    const bool pair = two && p.ldc % 2 == 0 && reinterpret_cast<uintptr_t>(p.c) % (2 * elem) == 0;
+    uint32_t peer[kSplits];
+#pragma unroll
+    for (int r = 0; r < kSplits; ++r) {
+      const uint32_t own = smem_u32(smem) + t % 64 * 8;
+      peer[r] = kSplits > 1 ? mapa_shared(own, (uint32_t)(rank + r) % kSplits) : own;
+    }
+    for (int tok0 = rank * share + t / 64; tok0 < last; tok0 += 2 * kAtOnce) {
+      int a0[kAtOnce] = {}, a1[kAtOnce] = {};
+#pragma unroll
+      for (int r = 0; r < kSplits; ++r)
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int tok = min(tok0 + 2 * u, kTn - 1);
+          int x, y;
+          asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(peer[r] + tok * 512));
+          a0[u] += x;
+          a1[u] += y;
+        }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int tok = tok0 + 2 * u;
+        if (tok >= last) break;
+        const float sa = scale[tok];
+        float y0 = finish(a0[u], sa, s0, b0), y1 = two ? finish(a1[u], sa, s1, b1) : 0.f;
+        if (p.gelu) gelu2(y0, y1);
+        const int64_t at = (int64_t)(m0 + tok) * p.ldc + ch_n;
+        if (pair) {
+          if (p.c_dtype == DA_F32) *reinterpret_cast<float2*>(static_cast<float*>(p.c) + at) = make_float2(y0, y1);
+          else *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.c) + at) =
+                   p.c_dtype == DA_BF16 ? pack_bf16x2(y0, y1) : pack_f16x2(y0, y1);
+        } else {
+          store1(p.c, p.c_dtype, at, y0);
+          if (two) store1(p.c, p.c_dtype, at + 1, y1);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (splits > 1) cluster_sync();  // peers may still read this CTA's sums
+  if (warp == 1) tmem_dealloc<1>(tmem, C::kCols);
+}
+
+template <int kTn, int kSplits>
+int launch_few(const Params& p, cudaStream_t st) {
+  using C = Few<kTn>;
+  CUtensorMap ta, tb;
+  if (int rc = make_tmap_2d(&ta, p.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.M, p.lda, 128, kTn)) return rc;
+  if (int rc = make_tmap_2d(&tb, p.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.N, p.ldb, 128, 128)) return rc;
+  auto kern = gemm_few_kernel<kTn, kSplits>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem + 1024) != cudaSuccess)
+    return record_cuda_error();
+  const int64_t tiles = (int64_t)((p.N + 127) / 128) * ((p.M + kTn - 1) / kTn);
+  return launch_cluster(kern, dim3((unsigned)(tiles * kSplits)), dim3(C::kThreads), C::kSmem + 1024, st, kSplits, ta, tb,
+                        p);
+}
+template <int kTn>
+int dispatch_few(const Params& p, int splits, cudaStream_t st) {
+  switch (splits) {
+    case 1: return launch_few<kTn, 1>(p, st);
+    case 2: return launch_few<kTn, 2>(p, st);
+    case 4: return launch_few<kTn, 4>(p, st);
+    default: return launch_few<kTn, 8>(p, st);
+  }
+}
+
+// The few-token kernel where every tile gets two CTAs or more, or there are at most 256 tokens and its tiles fit on
+// the SMs at once.  Measured (us, few against pair): 1 x 4096 x 4096 5.8 / 14.0, 128 x 4096 x 4096 9.6 / 14.7,
+// 256 x 4096 x 4096 12.7 / 14.9, 512 x 4096 x 4096 17.4 / 15.9, 1024 x 512 x 1536 12.8 / 10.0.
+int dispatch(const Params& p, cudaStream_t st) {
+  const int tn = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
+  const int64_t tiles = (int64_t)((p.N + 127) / 128) * ((p.M + tn - 1) / tn);
+  const int sms = sm_count();
+  if (2 * tiles > sms && (p.M > 256 || tiles > sms)) return dispatch_pair(p, st);
+  // as many K ranges as fill the SMs, none shorter than 2 stages
+  const int nk = (p.K + 127) / 128;
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= sms && nk >= splits * 2 * 2) splits *= 2;
+  switch (tn) {
+    case 16: return dispatch_few<16>(p, splits, st);
+    case 32: return dispatch_few<32>(p, splits, st);
+    case 64: return dispatch_few<64>(p, splits, st);
+    default: return dispatch_few<128>(p, splits, st);
+  }
+}
+
 }  // namespace i8
 }  // namespace da
 
@@ -309,5 +522,5 @@ extern "C" int da_gemm_i8(const int8_t* A, int64_t lda, const float* a_scale, co
   const i8::Params p{A,      B,      a_scale, b_scale,    bias,    C,    lda,   ldb,   ldc,
                      (int)M, (int)N, (int)K,  bias_dtype, c_dtype, gelu, tma_c, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return i8::dispatch_pair(p, st);
+  return i8::dispatch(p, st);
 }
