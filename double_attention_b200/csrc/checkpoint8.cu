@@ -11,8 +11,10 @@
 //   GELU backward from the kept z:  dz = dh gelu'(z),  h = gelu(z) once more, for the next layer's weight gradient.
 //
 // Layout: q [rows, ceil(D / 32) * 32] int8, columns past D zero; e [rows, ceil(D / 32)] int8.
-// Bound: HBM (5 bytes an element forward, 7 backward); a thread takes 8 columns, so the 4 threads of a block
-// find its maximum with two shuffles and no row-wide reduction is needed, whatever the width.
+// Bound: HBM, whose writes run at 3.9 TB/s alone (a copy: 6.5 TB/s read and written).  A thread takes 8 columns,
+// so the 4 threads of a block find its maximum with two shuffles and no row-wide reduction is needed, whatever the
+// width.  Dense tensors whose width is a multiple of 32 run as one long row (kFlat); any other width, stride or
+// alignment finds its row by a multiplication and checks its columns.
 #include "common.cuh"
 #include "host_util.h"
 #include "vec8.cuh"
@@ -21,7 +23,7 @@ namespace da {
 namespace {
 
 constexpr int kNotFinite = -128;
-constexpr int kItems = 4;  // groups of 8 columns per thread
+constexpr int kItems = 4;  // groups of 8 columns per thread, all loaded before the first is used
 
 struct CkptArgs {
   const void* x;  // z or dh
@@ -30,143 +32,242 @@ struct CkptArgs {
   int8_t* q;
   int8_t* e;
   int64_t ldx, ldh, lddz, row0;
-  int64_t items;  // groups of 8 columns in this launch (< 2^31)
+  int64_t items;  // groups of 8 columns in this launch (below 2^31 unless flat)
   Div31 per_row;  // groups of 8 columns in a row of q (a multiple of 4)
-  int D, dtype, gelu, e_min, e_max;
+  int D, gelu, e_min, e_max;
+  int vec_x, vec_h, vec_dz;  // 16-byte rows
 };
 
-DA_DEV void load_row8(const void* p, int dtype, int64_t base, int col, int D, bool vec, float* v) {
-  if (vec && col + 8 <= D) {
-    load8(p, dtype, base + col, v);
-  } else {
+// Eight 16-bit values of a row, those past D as 0.
+template <typename T>
+DA_DEV uint4 load_row8(const void* p, int64_t base, int col, int D, bool vec) {
+  const T* src = static_cast<const T*>(p) + base + col;
+  if (vec && col + 8 <= D) return *reinterpret_cast<const uint4*>(src);
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < D ? load1(p, dtype, base + col + i) : 0.f;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = col + 2 * i < D ? reinterpret_cast<const uint16_t*>(src)[2 * i] : 0;
+    const uint32_t hi = col + 2 * i + 1 < D ? reinterpret_cast<const uint16_t*>(src)[2 * i + 1] : 0;
+    w[i] = lo | hi << 16;
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
-DA_DEV void store_row8(void* p, int dtype, int64_t base, int col, int D, bool vec, const float* v) {
+template <typename T>
+DA_DEV void store_row8(void* p, int64_t base, int col, int D, bool vec, const F2* v) {
+  T* dst = static_cast<T*>(p) + base + col;
+  const uint32_t w[4] = {narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]), narrow<T>(v[3])};
   if (vec && col + 8 <= D) {
-    store8(p, dtype, base + col, v);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (col + i < D) store1(p, dtype, base + col + i, v[i]);
+      if (col + i < D) reinterpret_cast<uint16_t*>(dst)[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
   }
 }
 
 // 2^e, e in [-126, 127].
 DA_DEV float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-__global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p, bool vec_x, bool vec_h) {
+struct Place {  // of a group of 8 columns
+  int64_t row, group;
+  int col;
+};
+template <bool kFlat>
+DA_DEV Place place_of(const CkptArgs& p, int64_t i) {
+  if constexpr (kFlat) return {0, i, 0};
+  const uint32_t r = p.per_row.div((uint32_t)i), c = (uint32_t)i - r * p.per_row.d;
+  return {p.row0 + r, (p.row0 + r) * p.per_row.d + c, (int)c * 8};
+}
+template <typename T, bool kFlat>
+DA_DEV uint4 load_place(const CkptArgs& p, const Place& at) {
+  if constexpr (kFlat) return __ldcs(reinterpret_cast<const uint4*>(p.x) + at.group);
+  return load_row8<T>(p.x, at.row * p.ldx, at.col, p.D, p.vec_x);
+}
+template <typename T, bool kFlat>
+DA_DEV void store_place(const CkptArgs& p, void* out, int64_t ld, int vec, const Place& at, const F2* v) {
+  if constexpr (kFlat)
+    reinterpret_cast<uint4*>(out)[at.group] = make_uint4(narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]), narrow<T>(v[3]));
+  else
+    store_row8<T>(out, at.row * ld, at.col, p.D, vec, v);
+}
+
+template <typename T, bool kFlat>
+__global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
+  const int64_t first = (int64_t)blockIdx.x * (256 * kItems) + threadIdx.x;
+  uint4 raw[kItems];
+  Place at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    const int64_t i = ((int64_t)blockIdx.x * kItems + k) * 256 + threadIdx.x;
-    // the 4 threads of a block of columns stay or leave together (items is a multiple of 4)
-    const unsigned mask = __ballot_sync(0xffffffffu, i < p.items);
-    if (i >= p.items) continue;
-    const uint32_t r = p.per_row.div((uint32_t)i), c = (uint32_t)i - r * p.per_row.d;
-    const int64_t row = p.row0 + r;
-    const int col = (int)c * 8;
-    float v[8];
-    load_row8(p.x, p.dtype, row * p.ldx, col, p.D, vec_x, v);
-    uint32_t a = 0;
+    raw[k] = make_uint4(0, 0, 0, 0);
+    at[k] = place_of<kFlat>(p, first + k * 256);
+    if (first + k * 256 < p.items) raw[k] = load_place<T, kFlat>(p, at[k]);
+  }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a = max(a, __float_as_uint(v[j]) & 0x7fffffffu);
-    a = max(a, __shfl_xor_sync(mask, a, 1));
-    a = max(a, __shfl_xor_sync(mask, a, 2));
-    // a = m 2^E with 1 <= m < 2: 127 * 2^(E - 6) covers it if m <= 1.984375 (mantissa bits 0x7e0000)
-    int e = (int)(a >> 23) - 127 - 6 + ((a & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+  for (int k = 0; k < kItems; ++k) {
+    // the 16-bit patterns without their signs order as integers, NaN above infinity above every number
+    uint32_t m = __vmaxu2(__vmaxu2(raw[k].x & 0x7fff7fffu, raw[k].y & 0x7fff7fffu),
+                          __vmaxu2(raw[k].z & 0x7fff7fffu, raw[k].w & 0x7fff7fffu));
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    m = max(m & 0xffffu, m >> 16);
+    uint32_t a;  // as fp32
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) a = m << 16;
+    else a = __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+    // a = f 2^E with 1 <= f < 2: 127 * 2^(E - 6) covers it if f <= 1.984375 (mantissa bits 0x7e0000)
+    const int fit = (int)(a >> 23) - 127 - 6 + ((a & 0x7fffffu) > 0x7e0000u ? 1 : 0);
     const bool finite = a < 0x7f800000u;
-    e = max(p.e_min, min(p.e_max, e));
-    const float inv = pow2i(-e);
-    int o[8];
+    const int e = max(p.e_min, min(p.e_max, fit));
+    const F2 inv = dup(pow2i(-e));
+    F2 v[4] = {widen<T>(raw[k].x), widen<T>(raw[k].y), widen<T>(raw[k].z), widen<T>(raw[k].w)};
+    uint2 q;
+    if (fit <= p.e_max) {
+      const F2 at_unit = dup(kRoundAt);
+      q.x = low_bytes(fma2(v[0], inv, at_unit), fma2(v[1], inv, at_unit));
+      q.y = low_bytes(fma2(v[2], inv, at_unit), fma2(v[3], inv, at_unit));
+    } else {  // saturating, or not finite
+      int o[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = finite ? max(-127, min(127, __float2int_rn(v[j] * inv))) : 0;
-    *reinterpret_cast<uint2*>(p.q + (row * p.per_row.d + c) * 8) = pack_s8x8(o);
-    if ((c & 3) == 0) p.e[(row * p.per_row.d + c) >> 2] = (int8_t)(finite ? e : kNotFinite);
-    if (p.gelu) {
+      for (int j = 0; j < 4; ++j) {
+        float lo, hi;
+        split(mul2(v[j], inv), lo, hi);
+        o[2 * j] = finite ? max(-127, min(127, __float2int_rn(lo))) : 0;
+        o[2 * j + 1] = finite ? max(-127, min(127, __float2int_rn(hi))) : 0;
+      }
+      q = pack_s8x8(o);
+    }
+    if (first + k * 256 < p.items) {
+      *reinterpret_cast<uint2*>(p.q + at[k].group * 8) = q;
+      if ((at[k].group & 3) == 0) p.e[at[k].group >> 2] = (int8_t)(finite ? e : kNotFinite);
+      if (p.gelu) {
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) gelu2(v[j], v[j + 1]);
-      store_row8(p.h, p.dtype, row * p.ldh, col, p.D, vec_h, v);
+        for (int j = 0; j < 4; ++j) v[j] = gelu2(v[j]);
+        store_place<T, kFlat>(p, p.h, p.ldh, p.vec_h, at[k], v);
+      }
     }
   }
 }
 
 // A kept group's 8 values.
-DA_DEV void restore8(const CkptArgs& p, int64_t group, float* v) {
-  unpack_s8x8(*reinterpret_cast<const uint2*>(p.q + group * 8), v);
-  const int e = p.e[group >> 2];
-  const float unit = e == kNotFinite ? __uint_as_float(0x7fffffffu) : pow2i(e);
+DA_DEV void restore8(uint2 q, int e, F2* v) {
+  const F2 unit = dup(e == kNotFinite ? __uint_as_float(0x7fffffffu) : pow2i(e));
+  signed_bytes(q.x, v[0], v[1]);
+  signed_bytes(q.y, v[2], v[3]);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] *= unit;
+  for (int j = 0; j < 4; ++j) v[j] = mul2(v[j], unit);
 }
 
-__global__ void __launch_bounds__(256) checkpoint8_restore_kernel(const CkptArgs p, bool vec_h) {
+template <typename T, bool kFlat>
+__global__ void __launch_bounds__(256) checkpoint8_restore_kernel(const CkptArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
+  const int64_t first = (int64_t)blockIdx.x * (256 * kItems) + threadIdx.x;
+  uint2 q[kItems];
+  int e[kItems];
+  Place at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    const int64_t i = ((int64_t)blockIdx.x * kItems + k) * 256 + threadIdx.x;
-    if (i >= p.items) continue;
-    const uint32_t r = p.per_row.div((uint32_t)i), c = (uint32_t)i - r * p.per_row.d;
-    const int64_t row = p.row0 + r;
-    float v[8];
-    restore8(p, row * p.per_row.d + c, v);
-    store_row8(p.h, p.dtype, row * p.ldh, (int)c * 8, p.D, vec_h, v);
-  }
-}
-
-__global__ void __launch_bounds__(256) checkpoint8_gelu_bwd_kernel(const CkptArgs p, bool vec_x, bool vec_h,
-                                                                   bool vec_dz) {
-  grid_dependency_wait();
-  grid_launch_dependents();
-#pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int64_t i = ((int64_t)blockIdx.x * kItems + k) * 256 + threadIdx.x;
-    if (i >= p.items) continue;
-    const uint32_t r = p.per_row.div((uint32_t)i), c = (uint32_t)i - r * p.per_row.d;
-    const int64_t row = p.row0 + r;
-    const int col = (int)c * 8;
-    if (col >= p.D) continue;
-    float z[8], d[8];
-    load_row8(p.x, p.dtype, row * p.ldx, col, p.D, vec_x, d);
-    restore8(p, row * p.per_row.d + c, z);
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      float s0, s1;
-      gelu_grad2(z[j], z[j + 1], s0, s1);
-      d[j] *= s0;
-      d[j + 1] *= s1;
+    at[k] = place_of<kFlat>(p, first + k * 256);
+    if (first + k * 256 < p.items) {
+      q[k] = *reinterpret_cast<const uint2*>(p.q + at[k].group * 8);
+      e[k] = p.e[at[k].group >> 2];
     }
-    store_row8(p.dz, p.dtype, row * p.lddz, col, p.D, vec_dz, d);
-    if (p.h) store_row8(p.h, p.dtype, row * p.ldh, col, p.D, vec_h, z);
+  }
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    if (first + k * 256 >= p.items) continue;
+    F2 v[4];
+    restore8(q[k], e[k], v);
+    if constexpr (std::is_same<T, float>::value) {
+      float* dst = static_cast<float*>(p.h) + at[k].row * p.ldh + (kFlat ? at[k].group * 8 : at[k].col);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float lo, hi;
+        split(v[j], lo, hi);
+        if (kFlat || at[k].col + 2 * j < p.D) dst[2 * j] = lo;
+        if (kFlat || at[k].col + 2 * j + 1 < p.D) dst[2 * j + 1] = hi;
+      }
+    } else {
+      store_place<T, kFlat>(p, p.h, p.ldh, p.vec_h, at[k], v);
+    }
   }
 }
 
-// Runs `launch(args, grid)` over slabs of rows whose item count stays below 2^31.
-template <typename F>
-int over_rows(CkptArgs p, int64_t rows, F&& launch) {
+template <typename T, bool kFlat>
+__global__ void __launch_bounds__(256) checkpoint8_gelu_bwd_kernel(const CkptArgs p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int64_t first = (int64_t)blockIdx.x * (256 * kItems) + threadIdx.x;
+  uint4 raw[kItems];
+  uint2 q[kItems];
+  int e[kItems];
+  Place at[kItems];
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    at[k] = place_of<kFlat>(p, first + k * 256);
+    if (first + k * 256 < p.items) {
+      raw[k] = load_place<T, kFlat>(p, at[k]);
+      q[k] = *reinterpret_cast<const uint2*>(p.q + at[k].group * 8);
+      e[k] = p.e[at[k].group >> 2];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    if (first + k * 256 >= p.items || (!kFlat && at[k].col >= p.D)) continue;
+    F2 z[4], d[4] = {widen<T>(raw[k].x), widen<T>(raw[k].y), widen<T>(raw[k].z), widen<T>(raw[k].w)};
+    restore8(q[k], e[k], z);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d[j] = mul2(d[j], gelu_grad2(z[j]));
+    store_place<T, kFlat>(p, p.dz, p.lddz, p.vec_dz, at[k], d);
+    if (p.h) store_place<T, kFlat>(p, p.h, p.ldh, p.vec_h, at[k], z);
+  }
+}
+
+// Runs the kernel over all groups: at once where the tensors are one long row, else over slabs of rows whose items
+// stay below 2^31.
+template <typename T, template <typename, bool> class Kernel>
+int run(CkptArgs p, int64_t rows, bool flat, cudaStream_t st) {
+  const int64_t per_block = 256 * kItems;
+  if (flat && rows * p.per_row.d / per_block < 0x7fffffffLL) {
+    p.items = rows * p.per_row.d;
+    return launch_kernel(Kernel<T, true>::get(), dim3((unsigned)((p.items + per_block - 1) / per_block)), dim3(256), 0, st,
+                         false, p);
+  }
   const int64_t slab = Div31::kMax / p.per_row.d;
   for (int64_t r0 = 0; r0 < rows; r0 += slab) {
     p.row0 = r0;
     p.items = (rows - r0 < slab ? rows - r0 : slab) * (int64_t)p.per_row.d;
-    const dim3 grid((unsigned)((p.items + 256 * kItems - 1) / (256 * kItems)));
-    if (int rc = launch(p, grid)) return rc;
+    if (int rc = launch_kernel(Kernel<T, false>::get(), dim3((unsigned)((p.items + per_block - 1) / per_block)), dim3(256),
+                               0, st, false, p))
+      return rc;
   }
   return DA_OK;
 }
+template <typename T, bool kFlat>
+struct Forward {
+  static auto get() { return checkpoint8_kernel<T, kFlat>; }
+};
+template <typename T, bool kFlat>
+struct Restore {
+  static auto get() { return checkpoint8_restore_kernel<T, kFlat>; }
+};
+template <typename T, bool kFlat>
+struct GeluBackward {
+  static auto get() { return checkpoint8_gelu_bwd_kernel<T, kFlat>; }
+};
 
-CkptArgs make_args(int64_t D, int dtype) {
-  CkptArgs p{nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, 0, 0, 0, Div31((uint32_t)((D + 31) / 32 * 4)),
-             (int)D, dtype, 0, -126, 121};
+CkptArgs make_args(int64_t D, int dtype, const int8_t* q, const int8_t* e) {
+  CkptArgs p{nullptr, nullptr, nullptr, const_cast<int8_t*>(q), const_cast<int8_t*>(e), 0, 0, 0, 0, 0,
+             Div31((uint32_t)((D + 31) / 32 * 4)), (int)D, 0, -126, 121, 0, 0, 0};
   if (dtype == DA_F16) {
     p.e_min = -24;
     p.e_max = 9;
   }
   return p;
 }
-
+// Rows that follow one another without a gap and fill their blocks, on 16 bytes.
+bool dense(const void* p, int64_t ld, int64_t D) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld == D && D % 32 == 0; }
 bool bad_shape(int64_t rows, int64_t D) { return rows <= 0 || D <= 0 || D > 0x7fffff00LL; }
 bool half_dtype(int d) { return d == DA_F16 || d == DA_BF16; }
 
@@ -181,18 +282,17 @@ extern "C" int da_checkpoint8(const void* x, int dtype, int64_t ldx, int64_t row
   if (!half_dtype(dtype)) return DA_ERR_DTYPE;
   if (reinterpret_cast<uintptr_t>(q) % 16) return DA_ERR_ALIGN;
   if (int rc = bind_device(x)) return rc;
-  CkptArgs p = make_args(D, dtype);
+  CkptArgs p = make_args(D, dtype, q, e);
   p.x = x;
   p.ldx = ldx;
   p.h = h;
   p.ldh = ldh;
-  p.q = q;
-  p.e = e;
   p.gelu = gelu;
-  const bool vx = vec8_ok(x, dtype, ldx), vh = vec8_ok(h, dtype, ldh);
-  return over_rows(p, rows, [&](const CkptArgs& a, dim3 grid) {
-    return launch_kernel(checkpoint8_kernel, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), false, a, vx, vh);
-  });
+  p.vec_x = vec8_ok(x, dtype, ldx);
+  p.vec_h = vec8_ok(h, dtype, ldh);
+  const bool flat = dense(x, ldx, D) && (!gelu || dense(h, ldh, D));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == DA_BF16 ? run<__nv_bfloat16, Forward>(p, rows, flat, st) : run<__half, Forward>(p, rows, flat, st);
 }
 
 extern "C" int da_checkpoint8_restore(const int8_t* q, const int8_t* e, int64_t rows, int64_t D, void* out, int dtype,
@@ -203,16 +303,14 @@ extern "C" int da_checkpoint8_restore(const int8_t* q, const int8_t* e, int64_t 
   if (!half_dtype(dtype) && dtype != DA_F32) return DA_ERR_DTYPE;
   if (reinterpret_cast<uintptr_t>(q) % 16) return DA_ERR_ALIGN;
   if (int rc = bind_device(q)) return rc;
-  CkptArgs p = make_args(D, dtype);
-  p.q = const_cast<int8_t*>(q);
-  p.e = const_cast<int8_t*>(e);
+  CkptArgs p = make_args(D, dtype, q, e);
   p.h = out;
   p.ldh = ldo;
-  const bool vo = vec8_ok(out, dtype, ldo);
-  return over_rows(p, rows, [&](const CkptArgs& a, dim3 grid) {
-    return launch_kernel(checkpoint8_restore_kernel, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), false, a,
-                         vo);
-  });
+  p.vec_h = vec8_ok(out, dtype, ldo);
+  const bool flat = dense(out, ldo, D);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == DA_F32) return run<float, Restore>(p, rows, flat, st);
+  return dtype == DA_BF16 ? run<__nv_bfloat16, Restore>(p, rows, flat, st) : run<__half, Restore>(p, rows, flat, st);
 }
 
 extern "C" int da_checkpoint8_gelu_bwd(const void* dh, int dtype, int64_t lddh, const int8_t* q, const int8_t* e,
@@ -224,18 +322,18 @@ extern "C" int da_checkpoint8_gelu_bwd(const void* dh, int dtype, int64_t lddh, 
   if (!half_dtype(dtype)) return DA_ERR_DTYPE;
   if (reinterpret_cast<uintptr_t>(q) % 16) return DA_ERR_ALIGN;
   if (int rc = bind_device(dh)) return rc;
-  CkptArgs p = make_args(D, dtype);
+  CkptArgs p = make_args(D, dtype, q, e);
   p.x = dh;
   p.ldx = lddh;
-  p.q = const_cast<int8_t*>(q);
-  p.e = const_cast<int8_t*>(e);
   p.dz = dz;
   p.lddz = lddz;
   p.h = h;
   p.ldh = ldh;
-  const bool vx = vec8_ok(dh, dtype, lddh), vh = vec8_ok(h, dtype, ldh), vz = vec8_ok(dz, dtype, lddz);
-  return over_rows(p, rows, [&](const CkptArgs& a, dim3 grid) {
-    return launch_kernel(checkpoint8_gelu_bwd_kernel, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), false, a,
-                         vx, vh, vz);
-  });
+  p.vec_x = vec8_ok(dh, dtype, lddh);
+  p.vec_dz = vec8_ok(dz, dtype, lddz);
+  p.vec_h = vec8_ok(h, dtype, ldh);
+  const bool flat = dense(dh, lddh, D) && dense(dz, lddz, D) && (!h || dense(h, ldh, D));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == DA_BF16 ? run<__nv_bfloat16, GeluBackward>(p, rows, flat, st)
+                          : run<__half, GeluBackward>(p, rows, flat, st);
 }

@@ -28,6 +28,11 @@ struct Params {
 // One output before its rounding to C's dtype: every kernel here computes exactly this.
 DA_DEV float finish(int acc, float sa, float sb, float bias) { return __fmaf_rn(__fmul_rn((float)acc, sa), sb, bias); }
 
+// The same for two neighbouring columns, whose accumulators come as bits.
+DA_DEV F2 finish2(float acc0, float acc1, float sa, F2 sb, F2 bias) {
+  return fma2(mul2(f2((float)__float_as_int(acc0), (float)__float_as_int(acc1)), dup(sa)), sb, bias);
+}
+
 DA_DEV float col_bias(const Params& p, int n) { return p.bias ? load1(p.bias, p.bias_dtype, n) : 0.f; }
 
 // ----------------------------------------------------------------------------------------------- large products
@@ -177,25 +182,26 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
             if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&acc_empty[buf]), 0));
           }
           if (col >= p.N || row0 >= p.M) continue;
+          F2 y[16];
           if (vec_cols && col + 32 <= p.N) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const float4 s = __ldg(reinterpret_cast<const float4*>(p.sb + col + e));
+            for (int e = 0; e < 8; ++e) {
+              const float4 s = __ldg(reinterpret_cast<const float4*>(p.sb + col) + e);
               float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (p.bias) b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + col + e));
-              v[e] = finish(__float_as_int(v[e]), sa, s.x, b.x);
-              v[e + 1] = finish(__float_as_int(v[e + 1]), sa, s.y, b.y);
-              v[e + 2] = finish(__float_as_int(v[e + 2]), sa, s.z, b.z);
-              v[e + 3] = finish(__float_as_int(v[e + 3]), sa, s.w, b.w);
+              if (p.bias) b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + col) + e);
+              y[2 * e] = finish2(v[4 * e], v[4 * e + 1], sa, f2(s.x, s.y), f2(b.x, b.y));
+              y[2 * e + 1] = finish2(v[4 * e + 2], v[4 * e + 3], sa, f2(s.z, s.w), f2(b.z, b.w));
             }
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               v[e] = col + e < p.N ? finish(__float_as_int(v[e]), sa, p.sb[col + e], col_bias(p, col + e)) : 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = f2(v[2 * e], v[2 * e + 1]);
           }
           if constexpr (kGelu) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) gelu2(v[e], v[e + 1]);
+            for (int e = 0; e < 16; ++e) y[e] = gelu2(y[e]);
           }
           const bool first = c % per_box == 0;
           if (first) {  // a free output box
@@ -205,17 +211,19 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
           const uint32_t dst = smem_u32(box);
           if constexpr (kOut == DA_F32) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              st_shared_v4(dst + sw128_offset(lane, e), __float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]),
-                           __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3]));
+            for (int e = 0; e < 8; ++e) {
+              float a0, a1, a2, a3;
+              split(y[2 * e], a0, a1);
+              split(y[2 * e + 1], a2, a3);
+              st_shared_v4(dst + sw128_offset(lane, e), __float_as_uint(a0), __float_as_uint(a1), __float_as_uint(a2),
+                           __float_as_uint(a3));
+            }
           } else {
-            uint32_t w[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              w[e] = kOut == DA_BF16 ? pack_bf16x2(v[2 * e], v[2 * e + 1]) : pack_f16x2(v[2 * e], v[2 * e + 1]);
+            using T = typename std::conditional<kOut == DA_BF16, __nv_bfloat16, __half>::type;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              st_shared_v4(dst + sw128_offset(lane, (first ? 0 : 4) + e), w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+              st_shared_v4(dst + sw128_offset(lane, (first ? 0 : 4) + e), narrow<T>(y[4 * e]), narrow<T>(y[4 * e + 1]),
+                           narrow<T>(y[4 * e + 2]), narrow<T>(y[4 * e + 3]));
           }
           if ((c + 32) % per_box != 0 && col + 32 < p.N) continue;  // the box's second half follows
           const int col0 = first ? col : col - 32;
@@ -439,7 +447,7 @@ __global__ void __launch_bounds__(Few<kTn>::kThreads, 1) gemm_few_kernel(const _
         if (tok >= last) break;
         const float sa = scale[tok];
         float y0 = finish(a0[u], sa, s0, b0), y1 = two ? finish(a1[u], sa, s1, b1) : 0.f;
-        if (p.gelu) gelu2(y0, y1);
+        if (p.gelu) split(gelu2(f2(y0, y1)), y0, y1);
         const int64_t at = (int64_t)(m0 + tok) * p.ldc + ch_n;
         if (pair) {
           if (p.c_dtype == DA_F32) *reinterpret_cast<float2*>(static_cast<float*>(p.c) + at) = make_float2(y0, y1);

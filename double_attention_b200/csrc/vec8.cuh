@@ -95,7 +95,7 @@ DA_DEV void unpack_s8x8(uint2 w, float* v) {
     v[e] = __uint_as_float(__byte_perm(u[e >> 2], 0x4b000000u, 0x7540 | (e & 3))) - 8388736.f;
 }
 
-// Two fp32 values in one register pair; multiplications and additions of pairs take one issue slot.
+// Two fp32 values in one register pair; additions and multiplications of pairs take one issue slot.
 struct F2 {
   unsigned long long v;
 };
@@ -104,7 +104,13 @@ DA_DEV F2 f2(float a, float b) {
   asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
   return r;
 }
+DA_DEV F2 dup(float a) { return f2(a, a); }
 DA_DEV void split(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+DA_DEV F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
 DA_DEV F2 mul2(F2 a, F2 b) {
   F2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
@@ -115,23 +121,54 @@ DA_DEV F2 fma2(F2 a, F2 b, F2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
 }
-DA_DEV F2 dup(float a) { return f2(a, a); }
+// A pair of 16-bit values in fp32, and two fp32 values rounded to a pair.
+template <typename T>
+DA_DEV F2 widen(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  const float2 f = unpack2<T>(w);
+  return f2(f.x, f.y);
+}
+template <typename T>
+DA_DEV uint32_t narrow(F2 x) {
+  float a, b;
+  split(x, a, b);
+  return pack2<T>(a, b);
+}
 
-// The lower tail of the normal distribution, Phi(-|z|), and its density without the factor 1 / sqrt(2 pi), for
-// two values: Hastings' approximation of erfc (Abramowitz and Stegun 7.1.26, absolute error at most 1.5e-7).
-// With x = |z| / sqrt(2) and t = 1 / (1 + 0.3275911 x), erfc(x) = t (a1 + ... + a5 t^4) exp(-x^2), and Phi(-|z|) is
-// half of it; the exponential is the density that GELU's derivative needs too.  The two reciprocals come from
-// one, of their product (|z| is cut at 1e4, where the density is 0): the special-function unit, 16 lanes a clock
-// against 128 for additions, is what bounds an epilogue with GELU.
-constexpr float kCut = 1e4f;
-DA_DEV void normal_tail2(float z0, float z1, F2& tail, F2& density) {
-  const F2 z = f2(z0, z1);
-  const F2 arg = mul2(mul2(z, dup(-0.72134752044448170f)), z);  // -z^2 / 2 in base 2
-  const F2 a = fma2(f2(fminf(fabsf(z0), kCut), fminf(fabsf(z1), kCut)), dup(0.23164188f), dup(1.f));
-  float a0, a1, g0, g1;
-  split(a, a0, a1);
-  split(arg, g0, g1);
-  const F2 t = mul2(dup(__fdividef(1.f, a0 * a1)), f2(a1, a0));
+// Integers by addition: for |v| < 2^22, v + kRoundAt rounds v to the nearest integer (ties to even), which the
+// low byte of the sum's bits holds in two's complement when it lies in [-128, 127].
+constexpr float kRoundAt = 12582912.f;  // 1.5 * 2^23
+// The low bytes of four such sums.
+DA_DEV uint32_t low_bytes(F2 lo, F2 hi) {
+  float a, b, c, d;
+  split(lo, a, b);
+  split(hi, c, d);
+  return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
+                     __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
+}
+// Four bytes as signed integers in fp32: a byte xor 0x80 in the low mantissa bits of 2^23 is 2^23 + 128 + value.
+DA_DEV void signed_bytes(uint32_t w, F2& lo, F2& hi) {
+  w ^= 0x80808080u;
+  auto one = [&](uint32_t sel) { return __uint_as_float(__byte_perm(w, 0x4b000000u, sel)); };
+  lo = add2(f2(one(0x7540), one(0x7541)), dup(-8388736.f));
+  hi = add2(f2(one(0x7542), one(0x7543)), dup(-8388736.f));
+}
+
+// The lower tail of the normal distribution, Phi(-|z|), for two values, their densities without the factor
+// 1 / sqrt(2 pi), and -|z|: Hastings' approximation of erfc (Abramowitz and Stegun 7.1.26, absolute error at most
+// 1.5e-7).  With x = |z| / sqrt(2) and t = 1 / (1 + 0.3275911 x), erfc(x) = t (a1 + ... + a5 t^4) exp(-x^2), and
+// Phi(-|z|) is half of it; the exponential is the density that GELU's derivative needs too.
+// The two reciprocals come from one, of their product (|z| is cut at 1e4, where the density is 0): the
+// special-function unit, 16 lanes a clock against 128 for additions, and the issue slots are what a kernel with
+// GELU runs out of.
+DA_DEV void normal_tail2(F2 z, F2& tail, F2& density, F2& minus_abs) {
+  float z0, z1, a0, a1, g0, g1, r;
+  split(z, z0, z1);
+  minus_abs = f2(fmaxf(-fabsf(z0), -1e4f), fmaxf(-fabsf(z1), -1e4f));
+  split(fma2(minus_abs, dup(-0.23164188f), dup(1.f)), a0, a1);
+  split(mul2(mul2(z, dup(-0.72134752044448170f)), z), g0, g1);  // -z^2 / 2 in base 2
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a0 * a1));
+  const F2 t = f2(r * a1, r * a0);
   density = f2(ex2(g0), ex2(g1));
   F2 poly = fma2(t, dup(0.5f * 1.061405429f), dup(0.5f * -1.453152027f));
   poly = fma2(poly, t, dup(0.5f * 1.421413741f));
@@ -139,31 +176,28 @@ DA_DEV void normal_tail2(float z0, float z1, F2& tail, F2& density) {
   poly = fma2(poly, t, dup(0.5f * 0.254829592f));
   tail = mul2(mul2(poly, t), density);
 }
-
-// GELU in its exact form: z Phi(z) = max(z, 0) - |z| Phi(-|z|); an infinity keeps its limit, inf or 0.
-DA_DEV float gelu_of(float z, float tail) {
-  return fmaf(-fminf(fabsf(z), kCut), tail, fmaxf(z, 0.f));  // (NaN: max is 0, but the tail is NaN)
+// max(z, 0) - |z| Phi(-|z|) = z Phi(z): GELU in its exact form.  An infinity keeps its limit, inf or 0.
+DA_DEV F2 gelu_of(F2 z, F2 tail, F2 minus_abs) {
+  float z0, z1;
+  split(z, z0, z1);
+  return fma2(minus_abs, tail, f2(fmaxf(z0, 0.f), fmaxf(z1, 0.f)));  // (NaN: max is 0, but the tail is NaN)
 }
-DA_DEV void gelu2(float& z0, float& z1) {
-  F2 tail, density;
-  normal_tail2(z0, z1, tail, density);
-  float t0, t1;
-  split(tail, t0, t1);
-  z0 = gelu_of(z0, t0);
-  z1 = gelu_of(z1, t1);
+DA_DEV F2 gelu2(F2 z) {
+  F2 tail, density, minus_abs;
+  normal_tail2(z, tail, density, minus_abs);
+  return gelu_of(z, tail, minus_abs);
 }
-
-// GELU'(z) = Phi(z) + z density / sqrt(2 pi), and z becomes GELU(z).
-DA_DEV void gelu_grad2(float& z0, float& z1, float& s0, float& s1) {
-  F2 tail, density;
-  normal_tail2(z0, z1, tail, density);
-  float t0, t1, d0, d1;
-  split(tail, t0, t1);
-  split(mul2(mul2(density, dup(0.39894228040143268f)), f2(z0, z1)), d0, d1);
-  s0 = d0 + (z0 > 0.f ? 1.f - t0 : t0);
-  s1 = d1 + (z1 > 0.f ? 1.f - t1 : t1);
-  z0 = gelu_of(z0, t0);
-  z1 = gelu_of(z1, t1);
+// GELU'(z) = Phi(z) + z density / sqrt(2 pi), Phi(z) = 1/2 + sign(z) (1/2 - Phi(-|z|)); z becomes GELU(z).
+DA_DEV F2 gelu_grad2(F2& z) {
+  F2 tail, density, minus_abs;
+  normal_tail2(z, tail, density, minus_abs);
+  float z0, z1, h0, h1;
+  split(z, z0, z1);
+  split(fma2(tail, dup(-1.f), dup(0.5f)), h0, h1);
+  const F2 odd = f2(copysignf(h0, z0), copysignf(h1, z1));
+  const F2 slope = add2(fma2(mul2(density, dup(0.39894228040143268f)), z, odd), dup(0.5f));
+  z = gelu_of(z, tail, minus_abs);
+  return slope;
 }
 
 }  // namespace da
