@@ -23,6 +23,7 @@ struct Params {
   int M, N, K, bias_dtype, c_dtype, gelu;
   int tma_c;  // C's rows take TMA stores (16-byte aligned base and stride)
   int* status;
+  Div31 per_group;  // the pair kernel: tiles in a group of 8 rows of tiles
 };
 
 // One output before its rounding to C's dtype: every kernel here computes exactly this.
@@ -95,11 +96,12 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
   grid_launch_dependents();
   const uint32_t tmem = tmem_base;
   auto tile_mn = [&](int i, int& m0, int& n0) {
-    const int t = pair + i * pairs;
-    const int group = t / (C::kGroupM * n_tiles), in = t - group * C::kGroupM * n_tiles;
-    const int height = min(C::kGroupM, m_tiles - group * C::kGroupM);
-    m0 = (group * C::kGroupM + in % height) * C::kTile;
-    n0 = in / height * C::kTile;
+    const uint32_t t = pair + i * pairs;
+    const uint32_t group = p.per_group.div(t), in = t - group * p.per_group.d;
+    const uint32_t height = min(C::kGroupM, m_tiles - (int)group * C::kGroupM);
+    const uint32_t n = height == C::kGroupM ? in / C::kGroupM : in / height;
+    m0 = (int)(group * C::kGroupM + in - n * height) * C::kTile;
+    n0 = (int)n * C::kTile;
   };
 
   if ((warp == 0 || warp == 2) && lane == 0) {
@@ -158,6 +160,7 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
     uint8_t* box = smem + C::kOff + (warp - 4) * 4096;
     const bool vec_cols = reinterpret_cast<uintptr_t>(p.sb) % 16 == 0 &&
                           (!p.bias || (p.bias_dtype == DA_F32 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0));
+    constexpr int kStep = 16;  // columns at a time: what GELU and its constants need stays in 96 registers
     constexpr int per_box = kOut == DA_F32 ? 32 : 64;  // columns in 128 bytes
     bool ok = true;
     for (int i = 0; i < my_tiles; ++i) {
@@ -171,21 +174,21 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
       tc_fence_after();
       if (ok) {
 #pragma unroll 1
-        for (int c = 0; c < 64; c += 32) {
+        for (int c = 0; c < 64; c += kStep) {
           const int col = n0 + part * 64 + c;
-          float v[32];
-          tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + buf * C::kTile + part * 64 + c, v);
+          float v[kStep];
+          tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + buf * C::kTile + part * 64 + c, v);
           tmem_wait_ld();
-          if (c == 32) {  // the last columns of this accumulator are in registers
+          if (c + kStep == 64) {  // the last columns of this accumulator are in registers
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&acc_empty[buf]), 0));
           }
           if (col >= p.N || row0 >= p.M) continue;
-          F2 y[16];
-          if (vec_cols && col + 32 <= p.N) {
+          F2 y[kStep / 2];
+          if (vec_cols && col + kStep <= p.N) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < kStep / 4; ++e) {
               const float4 s = __ldg(reinterpret_cast<const float4*>(p.sb + col) + e);
               float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
               if (p.bias) b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + col) + e);
@@ -194,39 +197,39 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
+            for (int e = 0; e < kStep; ++e)
               v[e] = col + e < p.N ? finish(__float_as_int(v[e]), sa, p.sb[col + e], col_bias(p, col + e)) : 0.f;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = f2(v[2 * e], v[2 * e + 1]);
+            for (int e = 0; e < kStep / 2; ++e) y[e] = f2(v[2 * e], v[2 * e + 1]);
           }
           if constexpr (kGelu) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = gelu2(y[e]);
+            for (int e = 0; e < kStep / 2; ++e) y[e] = gelu2(y[e]);
           }
-          const bool first = c % per_box == 0;
-          if (first) {  // a free output box
+          const int in_box = c % per_box;
+          if (in_box == 0) {  // a free output box
             if (lane == 0) tma_store_wait_read<0>();
             __syncwarp();
           }
           const uint32_t dst = smem_u32(box);
           if constexpr (kOut == DA_F32) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < kStep / 4; ++e) {
               float a0, a1, a2, a3;
               split(y[2 * e], a0, a1);
               split(y[2 * e + 1], a2, a3);
-              st_shared_v4(dst + sw128_offset(lane, e), __float_as_uint(a0), __float_as_uint(a1), __float_as_uint(a2),
-                           __float_as_uint(a3));
+              st_shared_v4(dst + sw128_offset(lane, in_box / 4 + e), __float_as_uint(a0), __float_as_uint(a1),
+                           __float_as_uint(a2), __float_as_uint(a3));
             }
           } else {
             using T = typename std::conditional<kOut == DA_BF16, __nv_bfloat16, __half>::type;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              st_shared_v4(dst + sw128_offset(lane, (first ? 0 : 4) + e), narrow<T>(y[4 * e]), narrow<T>(y[4 * e + 1]),
+            for (int e = 0; e < kStep / 8; ++e)
+              st_shared_v4(dst + sw128_offset(lane, in_box / 8 + e), narrow<T>(y[4 * e]), narrow<T>(y[4 * e + 1]),
                            narrow<T>(y[4 * e + 2]), narrow<T>(y[4 * e + 3]));
           }
-          if ((c + 32) % per_box != 0 && col + 32 < p.N) continue;  // the box's second half follows
-          const int col0 = first ? col : col - 32;
+          if (in_box + kStep != per_box && col + kStep < p.N) continue;  // more of the box follows
+          const int col0 = col - in_box;
           if (p.tma_c) {
             fence_proxy_async();
             __syncwarp();
@@ -528,7 +531,8 @@ extern "C" int da_gemm_i8(const int8_t* A, int64_t lda, const float* a_scale, co
   const int elem = c_dtype == DA_F32 ? 4 : 2;
   const int tma_c = reinterpret_cast<uintptr_t>(C) % 16 == 0 && ldc * elem % 16 == 0;
   const i8::Params p{A,      B,      a_scale, b_scale,    bias,    C,    lda,   ldb,   ldc,
-                     (int)M, (int)N, (int)K,  bias_dtype, c_dtype, gelu, tma_c, status};
+                     (int)M, (int)N, (int)K,  bias_dtype, c_dtype, gelu, tma_c, status,
+                     Div31((uint32_t)((N + 255) / 256 * 8))};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return i8::dispatch(p, st);
 }
