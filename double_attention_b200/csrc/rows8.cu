@@ -9,11 +9,10 @@
 // does not depend on the order in which the squares are added; maxima do not either.
 //
 // A row whose largest |v| is at most 1e-36 (127 / a would overflow) becomes q = 0 with scale 0.  A row that
-// holds a NaN or an infinity gets a scale of NaN or infinity, so that it never decodes to plausible
-// numbers: |v| is compared as an unsigned integer, which orders NaN above infinity above every number.
+// holds a NaN or an infinity gets a scale of NaN, so that it never decodes to plausible numbers.
 //
-// Bound: HBM.  One pass; a row stays in registers between its reductions (one warp per row up to 1024
-// columns, one block per row up to 32768; wider rows are read again, mostly from L2).
+// Bound: HBM.  One pass; a row stays in registers between its reductions (a warp up to 1024 columns, a block of up to
+// 512 threads up to 16384; wider rows are read again, mostly from L2).
 #include "common.cuh"
 #include "host_util.h"
 #include "vec8.cuh"
@@ -35,6 +34,7 @@ struct NormArgs {
   int64_t ldx, ldb, ldo, ldq, rows;
   int x_dtype, branch_dtype, weight_dtype, bias_dtype, kind, D;
   float eps;
+  int aligned;  // weight and bias start on 16 bytes
 };
 
 // Sum and largest bit pattern over the kT threads of a row (kT a multiple of 32; a block-wide row uses
@@ -68,10 +68,20 @@ DA_DEV uint32_t row_max(uint32_t v, float* red) {
 
 DA_DEV uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// The largest magnitude of three; a NaN wins.
+DA_DEV float max_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // The row's factor on v and its scale from the largest |v| and rstd (1 for the quantiser and the LayerNorm).
 DA_DEV void row_scale(uint32_t amax_bits, float rstd, float& inv, float& scale) {
   const float amax = __uint_as_float(amax_bits);
-  if (amax <= kTiny && rstd == rstd) {  // (false for NaN)
+  if (amax_bits >= 0x7f800000u) {
+    inv = 0.f;
+    scale = __uint_as_float(0x7fffffffu);
+  } else if (amax <= kTiny && rstd == rstd) {  // (false for a NaN)
     inv = 0.f;
     scale = 0.f;
   } else {
@@ -84,146 +94,269 @@ DA_DEV int quant(float v, float inv) {  // NaN converts to 0
   return max(-127, min(127, __float2int_rn(v * inv)));
 }
 
-// kT threads per row, 8 * kNV elements per thread; kVec: 8 consecutive columns per access (16-byte aligned
-// rows, D a multiple of 8), else single elements kT columns apart.
-template <int kT, int kNV, bool kVec>
-__global__ void __launch_bounds__(kT > 256 ? kT : 256) norm_int8_kernel(const NormArgs p) {
-  constexpr int kBlock = kT > 256 ? kT : 256;
+// Eight values as four pairs.
+template <typename T>
+struct Eight {  // as loaded
+  uint4 w;
+  DA_DEV void load(const void* p, int64_t off) { w = *reinterpret_cast<const uint4*>(static_cast<const T*>(p) + off); }
+  DA_DEV void pairs(F2* v) const {
+    v[0] = widen<T>(w.x);
+    v[1] = widen<T>(w.y);
+    v[2] = widen<T>(w.z);
+    v[3] = widen<T>(w.w);
+  }
+  DA_DEV void from(const F2* v) { w = make_uint4(narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]), narrow<T>(v[3])); }
+  DA_DEV void store(void* p, int64_t off) const { *reinterpret_cast<uint4*>(static_cast<T*>(p) + off) = w; }
+};
+template <>
+struct Eight<float> {
+  float4 a, b;
+  DA_DEV void load(const void* p, int64_t off) {
+    a = reinterpret_cast<const float4*>(static_cast<const float*>(p) + off)[0];
+    b = reinterpret_cast<const float4*>(static_cast<const float*>(p) + off)[1];
+  }
+  DA_DEV void pairs(F2* v) const {
+    v[0] = f2(a.x, a.y);
+    v[1] = f2(a.z, a.w);
+    v[2] = f2(b.x, b.y);
+    v[3] = f2(b.z, b.w);
+  }
+  DA_DEV void from(const F2* v) {
+    split(v[0], a.x, a.y);
+    split(v[1], a.z, a.w);
+    split(v[2], b.x, b.y);
+    split(v[3], b.z, b.w);
+  }
+  DA_DEV void store(void* p, int64_t off) const {
+    reinterpret_cast<float4*>(static_cast<float*>(p) + off)[0] = a;
+    reinterpret_cast<float4*>(static_cast<float*>(p) + off)[1] = b;
+  }
+};
+template <typename T>
+constexpr int code_of() {
+  return std::is_same<T, float>::value ? DA_F32 : std::is_same<T, __nv_bfloat16>::value ? DA_BF16 : DA_F16;
+}
+struct None {};
+
+// Eight weights (or biases) from column `col` on, columns outside [0, D) as 0.  `aligned`: p is on 16 bytes; then
+// fp32 comes in as the two or three aligned groups of 4 that hold the columns (eight single loads a thread, each
+// warp-wide over 8 lines, set the time of shifted rows: 30001 x 1501 in 61 us, so in 45).
+template <bool kShift>
+DA_DEV void load_columns(const void* p, int dtype, bool aligned, int col, int D, F2* v) {
+  const int skip = col & 3;  // the same for the whole row
+  if (!kShift && dtype == DA_F32) {
+    Eight<float> e;
+    e.load(p, col);
+    e.pairs(v);
+  } else if (kShift && dtype == DA_F32 && aligned && col >= skip && col - skip + 12 <= D) {
+    const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p) + col - skip);
+    const float4 a = __ldg(src), b = __ldg(src + 1), c = __ldg(src + 2);
+    const float f[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
+    auto from = [&](int k) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = f2(f[k + 2 * i], f[k + 2 * i + 1]);
+    };
+    if (skip == 0) from(0);
+    else if (skip == 1) from(1);
+    else if (skip == 2) from(2);
+    else from(3);
+  } else {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = col + i >= 0 && col + i < D ? load1(p, dtype, col + i) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
+  }
+}
+
+// kT threads per row, 8 * kNV elements per thread, 16 bytes an access.  kShift: dense tensors of any width D.  Their
+// row r starts r D mod 8 elements after a multiple of 8, so a thread takes the groups of 8 that are aligned in
+// memory; the row's first and last groups mask what belongs to its neighbours, and q, whose rows do start on 16
+// bytes, goes through shared memory to be moved by the row's offset.
+template <typename TX, typename TB, int kKind, int kT, int kNV, bool kShift>
+__global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const NormArgs p) {
+  constexpr int kBlock = kT == 32 ? 256 : kT;  // 8 rows, a warp each, or one
+  constexpr bool kBranch = !std::is_same<TB, None>::value;
+  constexpr int kSlots = kNV * kT + 1;  // groups of a row's window, and one more that a shifted read touches
   __shared__ float red[kBlock / 32];
+  __shared__ uint2 moved[kShift ? kBlock / kT * kSlots : 1];
   grid_dependency_wait();
   grid_launch_dependents();
   const int t = threadIdx.x % kT;
   const int64_t row = (int64_t)blockIdx.x * (kBlock / kT) + threadIdx.x / kT;
   if (row >= p.rows) return;  // a whole warp (kT = 32) or never (one row per block)
-  float v[kNV][8];
+  const int off = kShift ? (int)(row * p.D % 8) : 0;  // the row's start within its first group
+  const int64_t bx = kShift ? row * p.D - off : row * p.ldx, bb = kShift ? bx : row * p.ldb, bo = kShift ? bx : row * p.ldo;
+  const int end = off + p.D;  // the row is [off, end) of the window
+  Eight<TX> x[kNV];
+  Eight<typename std::conditional<kBranch, TB, float>::type> br[kBranch ? kNV : 1];
 #pragma unroll
   for (int c = 0; c < kNV; ++c) {
-    if constexpr (kVec) {
-      const int col = (c * kT + t) * 8;
-      if (col < p.D) {
-        load8(p.x, p.x_dtype, row * p.ldx + col, v[c]);
+    const int at = (c * kT + t) * 8;
+    if (at < end) {
+      // (only the tensor's very last group can reach past its end)
+      if (!kShift || bx + at + 8 <= p.rows * p.D) {
+        x[c].load(p.x, bx + at);
+        if constexpr (kBranch) br[c].load(p.branch, bb + at);
       } else {
+        float f[8];
+        F2 v[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
-      }
-    } else {
+        for (int i = 0; i < 8; ++i) f[i] = at + i < end ? load1(p.x, code_of<TX>(), bx + at + i) : 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int col = (c * 8 + e) * kT + t;
-        v[c][e] = col < p.D ? load1(p.x, p.x_dtype, row * p.ldx + col) : 0.f;
+        for (int i = 0; i < 4; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
+        x[c].from(v);
+        if constexpr (kBranch) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = at + i < end ? load1(p.branch, code_of<TB>(), bb + at + i) : 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
+          br[c].from(v);
+        }
       }
     }
   }
-  if (p.branch) {
+  F2 v[kNV][4];
+  const F2 zero = dup(0.f);
+  auto inside = [&](int at, F2* w) {  // zeroes what lies outside the row
+    if (at >= off && at + 8 <= end) return;
 #pragma unroll
-    for (int c = 0; c < kNV; ++c) {
-      if constexpr (kVec) {
-        const int col = (c * kT + t) * 8;
-        if (col < p.D) {
-          float b[8];
-          load8(p.branch, p.branch_dtype, row * p.ldb + col, b);
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      split(w[i], a, b);
+      const int k = at + 2 * i;
+      w[i] = f2(k >= off && k < end ? a : 0.f, k + 1 >= off && k + 1 < end ? b : 0.f);
+    }
+  };
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[c][e] = round_to(v[c][e] + b[e], p.x_dtype);
-          store8(p.x_out, p.x_dtype, row * p.ldo + col, v[c]);
-        }
-      } else {
+  for (int c = 0; c < kNV; ++c) {
+    const int at = (c * kT + t) * 8;
+    if (at < end) {
+      x[c].pairs(v[c]);
+      if constexpr (kBranch) {
+        F2 b[4];
+        br[c].pairs(b);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int col = (c * 8 + e) * kT + t;
-          if (col < p.D) {
-            v[c][e] = round_to(v[c][e] + load1(p.branch, p.branch_dtype, row * p.ldb + col), p.x_dtype);
-            store1(p.x_out, p.x_dtype, row * p.ldo + col, v[c][e]);
+        for (int i = 0; i < 4; ++i) v[c][i] = add2(v[c][i], b[i]);
+        x[c].from(v[c]);
+        if (!kShift || (at >= off && at + 8 <= end)) {
+          x[c].store(p.x_out, bo + at);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float f[2];
+            split(v[c][i / 2], f[0], f[1]);
+            if (at + i >= off && at + i < end) store1(p.x_out, code_of<TX>(), bo + at + i, f[i % 2]);
           }
         }
+        x[c].pairs(v[c]);  // as rounded to the residual's dtype
       }
+      if constexpr (kShift) inside(at, v[c]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[c][i] = zero;
     }
   }
   float rstd = 1.f;
-  if (p.kind != kQuantize) {
-    float s = 0.f, mean = 0.f;
-    if (p.kind == kLayer) {
+  if constexpr (kKind != kQuantize) {
+    auto total = [&](F2 s) {
+      float a, b;
+      split(s, a, b);
+      return row_sum<kT>(a + b, red) / (float)p.D;
+    };
+    F2 mean = zero, s = zero;
+    if constexpr (kKind == kLayer) {
 #pragma unroll
       for (int c = 0; c < kNV; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += v[c][e];
-      mean = row_sum<kT>(s, red) / (float)p.D;
-      s = 0.f;
+        for (int i = 0; i < 4; ++i) s = add2(s, v[c][i]);
+      mean = dup(-total(s));
+      s = zero;
     }
 #pragma unroll
-    for (int c = 0; c < kNV; ++c)
+    for (int c = 0; c < kNV; ++c) {
+      if constexpr (kKind == kLayer) {
+        const int at = (c * kT + t) * 8;
+        if (at < end) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int col = kVec ? (c * kT + t) * 8 + e : (c * 8 + e) * kT + t;
-        const float d = col < p.D ? v[c][e] - mean : 0.f;
-        s = fmaf(d, d, s);
+          for (int i = 0; i < 4; ++i) v[c][i] = add2(v[c][i], mean);
+          if constexpr (kShift) inside(at, v[c]);
+        }
       }
-    rstd = 1.f / sqrtf(row_sum<kT>(s, red) / (float)p.D + p.eps);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = fma2(v[c][i], v[c][i], s);
+    }
+    rstd = 1.f / sqrtf(total(s) + p.eps);
 #pragma unroll
     for (int c = 0; c < kNV; ++c) {
-      float w[8], b[8];
-      if constexpr (kVec) {
-        const int col = (c * kT + t) * 8;
-        if (col < p.D) {
-          if (p.weight) load8(p.weight, p.weight_dtype, col, w);
-          if (p.bias) load8(p.bias, p.bias_dtype, col, b);
+      const int at = (c * kT + t) * 8;
+      if (at >= end) continue;
+      F2 w[4];
+      if (p.weight) load_columns<kShift>(p.weight, p.weight_dtype, p.aligned, at - off, p.D, w);
+      if constexpr (kKind == kRms) {
+        if (p.weight) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[c][i] = mul2(v[c][i], w[i]);
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int col = (c * 8 + e) * kT + t;
-          if (col < p.D) {
-            if (p.weight) w[e] = load1(p.weight, p.weight_dtype, col);
-            if (p.bias) b[e] = load1(p.bias, p.bias_dtype, col);
-          }
-        }
-      }
+        for (int i = 0; i < 4; ++i) v[c][i] = mul2(v[c][i], dup(rstd));
+        if (p.weight) {
+          F2 b[4] = {zero, zero, zero, zero};
+          if (p.bias) load_columns<kShift>(p.bias, p.bias_dtype, p.aligned, at - off, p.D, b);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int col = kVec ? (c * kT + t) * 8 + e : (c * 8 + e) * kT + t;
-        if (col < p.D) {
-          if (p.kind == kRms) {
-            if (p.weight) v[c][e] *= w[e];
-          } else {
-            v[c][e] = (v[c][e] - mean) * rstd;
-            if (p.weight) v[c][e] = fmaf(v[c][e], w[e], p.bias ? b[e] : 0.f);
-          }
+          for (int i = 0; i < 4; ++i) v[c][i] = fma2(v[c][i], w[i], b[i]);
         }
       }
     }
   }
-  uint32_t a = 0;
+  float a = 0.f;
 #pragma unroll
   for (int c = 0; c < kNV; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a = max(a, abs_bits(v[c][e]));  // columns past D hold 0
-  a = row_max<kT>(a, red);
+    for (int i = 0; i < 4; ++i) {
+      float lo, hi;
+      split(v[c][i], lo, hi);
+      a = max_abs(a, lo, hi);
+    }
   float inv, scale;
-  row_scale(a, p.kind == kRms ? rstd : 1.f, inv, scale);
+  row_scale(row_max<kT>(__float_as_uint(a) & 0x7fffffffu, red), kKind == kRms ? rstd : 1.f, inv, scale);
+  // |v inv| exceeds 127 by a rounding at most
+  auto bytes = [&](F2 lo, F2 hi) {
+    return low_bytes(add2(mul2(lo, dup(inv)), dup(kRoundAt)), add2(mul2(hi, dup(inv)), dup(kRoundAt)));
+  };
+  uint2* slots = moved + (kShift ? threadIdx.x / kT * kSlots : 0);
 #pragma unroll
   for (int c = 0; c < kNV; ++c) {
-    if constexpr (kVec) {
-      const int col = (c * kT + t) * 8;
-      if (col < p.D) {
-        int o[8];
+    const int at = (c * kT + t) * 8;
+    if (at >= end) continue;
+    const uint2 o = make_uint2(bytes(v[c][0], v[c][1]), bytes(v[c][2], v[c][3]));
+    if constexpr (kShift) slots[c * kT + t] = o;
+    else *reinterpret_cast<uint2*>(p.q + row * p.ldq + at) = o;
+  }
+  if constexpr (kShift) {
+    if constexpr (kT == 32) __syncwarp();
+    else __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = quant(v[c][e], inv);
-        *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) = pack_s8x8(o);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int col = (c * 8 + e) * kT + t;
-        if (col < p.D) p.q[row * p.ldq + col] = (int8_t)quant(v[c][e], inv);
-      }
+    for (int c = 0; c < kNV; ++c) {
+      const int col = (c * kT + t) * 8;  // bytes col .. + 8 of the row are off further on in the window
+      if (col >= p.D) continue;
+      const uint2 lo = slots[c * kT + t], hi = slots[c * kT + t + 1];
+      const uint32_t w[4] = {lo.x, lo.y, hi.x, hi.y};
+      const bool second = off >= 4;
+      const uint32_t w0 = second ? w[1] : w[0], w1 = second ? w[2] : w[1], w2 = second ? w[3] : w[2];
+      // (past the row's end these are bytes of no meaning, in the padding of q's row)
+      *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) =
+          make_uint2(__funnelshift_r(w0, w1, off % 4 * 8), __funnelshift_r(w1, w2, off % 4 * 8));
     }
   }
   if (t == 0) p.scale[row] = scale;
 }
 
-// Rows wider than the register variants hold: one block per row, the row read again for every reduction
-// (each thread reads back only what it wrote itself).
-__global__ void __launch_bounds__(1024) norm_int8_wide_kernel(const NormArgs p) {
-  constexpr int kT = 1024;
+// Any strides, alignments and mixtures of dtypes: one block per row, an element a load (each thread reads back only
+// what it wrote itself); rows wider than the register variants hold come here too.
+template <int kT>
+__global__ void __launch_bounds__(kT) norm_int8_any_kernel(const NormArgs p) {
   __shared__ float red[kT / 32];
   grid_dependency_wait();
   grid_launch_dependents();
@@ -272,42 +405,126 @@ __global__ void __launch_bounds__(1024) norm_int8_wide_kernel(const NormArgs p) 
   if (threadIdx.x == 0) p.scale[row] = scale;
 }
 
-// out = q * scale, one rounding to the output dtype; a thread takes 8 columns of one row.
-template <bool kVec>
+// out = q * scale, one rounding to the output dtype.  A thread takes 8 outputs: of a row that starts on 16 bytes, or
+// (kShift) 8 aligned ones of a dense tensor of any width, whose bytes of q are then two loads and a shift; else
+// (kVec false) one by one.
+template <typename T, bool kVec, bool kShift>
 __global__ void __launch_bounds__(256) dequant_int8_kernel(const int8_t* q, int64_t ldq, const float* scale,
                                                            int64_t row0, int64_t items, Div31 per_row, int D,
-                                                           void* out, int out_dtype, int64_t ldo) {
+                                                           void* out, int64_t ldo) {
+  constexpr int kItems = 4;  // a thread's, all loaded before the first is used
   grid_dependency_wait();
   grid_launch_dependents();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= items) return;
-  const uint32_t r = per_row.div((uint32_t)i);
-  const int64_t row = row0 + r;
-  const int col = (int)((uint32_t)i - r * per_row.d) * 8;
-  const float s = scale[row];
-  if constexpr (kVec) {
-    float v[8];
-    unpack_s8x8(*reinterpret_cast<const uint2*>(q + row * ldq + col), v);
+  uint2 w[kItems];
+  float s[kItems];
+  int64_t row[kItems];
+  int col[kItems];  // of the first output; negative in a shifted row's first group
+  auto live = [&](int k) { return col[k] < D; };
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= s;
-    store8(out, out_dtype, row * ldo + col, v);
-  } else {
-    for (int e = 0; e < 8 && col + e < D; ++e)
-      store1(out, out_dtype, row * ldo + col + e, (float)q[row * ldq + col + e] * s);
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = ((int64_t)blockIdx.x * kItems + k) * 256 + threadIdx.x;
+    const uint32_t r = per_row.div((uint32_t)i);
+    row[k] = row0 + r;
+    const int at = (int)((uint32_t)i - r * per_row.d) * 8;
+    const int off = kShift ? (int)(row[k] * D % 8) : 0;
+    col[k] = i < items ? at - off : D;
+    if (!live(k)) continue;
+    s[k] = scale[row[k]];
+    const int8_t* src = q + row[k] * ldq + at;
+    if constexpr (!kVec) {
+      uint32_t b[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b[e] = at + e < D ? (uint8_t)src[e] : 0;
+      w[k] = make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24, b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
+    } else if constexpr (!kShift) {
+      w[k] = *reinterpret_cast<const uint2*>(src);
+    } else {  // bytes at - off .. + 8: of the aligned eight before, and of those from `at` on
+      const uint2 zero = make_uint2(0, 0);
+      const uint2 lo = off && at > 0 ? *reinterpret_cast<const uint2*>(src - 8) : zero;
+      const uint2 hi = at < D ? *reinterpret_cast<const uint2*>(src) : zero;
+      const uint32_t v[4] = {lo.x, lo.y, hi.x, hi.y};
+      const int skip = 8 - off;  // 1 to 8 bytes of the sixteen
+      const uint32_t w0 = skip >= 4 ? v[1] : v[0], w1 = skip >= 4 ? v[2] : v[1], w2 = skip >= 4 ? v[3] : v[2];
+      w[k] = skip == 8 ? hi : make_uint2(__funnelshift_r(w0, w1, skip % 4 * 8), __funnelshift_r(w1, w2, skip % 4 * 8));
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    if (!live(k)) continue;
+    F2 v[4];
+    signed_bytes(w[k].x, v[0], v[1]);
+    signed_bytes(w[k].y, v[2], v[3]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = mul2(v[e], dup(s[k]));
+    const int64_t base = row[k] * ldo + col[k];
+    if (kVec && col[k] >= 0 && col[k] + 8 <= D) {
+      Eight<T> o;
+      o.from(v);
+      o.store(out, base);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float f[2];
+        split(v[e / 2], f[0], f[1]);
+        if (col[k] + e >= 0 && col[k] + e < D) store1(out, code_of<T>(), base + e, f[e % 2]);
+      }
+    }
   }
 }
 
-template <int kT, bool kVec>
-int launch_norm(const NormArgs& p, cudaStream_t st) {
-  constexpr int kBlock = kT > 256 ? kT : 256;
-  const int64_t blocks = (p.rows + kBlock / kT - 1) / (kBlock / kT);
+template <typename T>
+int launch_dequant(const int8_t* q, int64_t ldq, const float* scale, int64_t rows, int64_t D, void* out, int64_t ldo,
+                   cudaStream_t st) {
+  const bool q8 = ldq % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0;
+  const bool rows16 = q8 && D % 8 == 0 && vec8_ok(out, code_of<T>(), ldo);
+  const bool shift = !rows16 && q8 && ldo == D && vec8_ok(out, code_of<T>(), 8) && ldq >= (D + 7) / 8 * 8;
+  const Div31 per_row((uint32_t)((D + (shift ? 7 : 0) + 7) / 8));
+  const int64_t slab = Div31::kMax / per_row.d;  // rows whose items stay below 2^31
+  auto kern = rows16 ? dequant_int8_kernel<T, true, false>
+                     : shift ? dequant_int8_kernel<T, true, true> : dequant_int8_kernel<T, false, false>;
+  for (int64_t r0 = 0; r0 < rows; r0 += slab) {
+    const int64_t n = (rows - r0 < slab ? rows - r0 : slab) * per_row.d;
+    if (int rc = launch_kernel(kern, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, st, false, q, ldq, scale, r0, n, per_row,
+                               (int)D, out, ldo))
+      return rc;
+  }
+  return DA_OK;
+}
+
+template <typename TX, typename TB, int kKind, bool kShift, int kT, int kNV>
+int launch_t(const NormArgs& p, cudaStream_t st) {
+  const int64_t blocks = kT == 32 ? (p.rows + 7) / 8 : p.rows;
   if (blocks > 0x7fffffffLL) return DA_ERR_SHAPE;
-  const dim3 grid((unsigned)blocks), block(kBlock);
-  const int nv = (p.D + kT * 8 - 1) / (kT * 8);
-  if (kT == 1024 || nv > 3) return launch_kernel(norm_int8_kernel<kT, 4, kVec>, grid, block, 0, st, false, p);
-  if (nv == 3) return launch_kernel(norm_int8_kernel<kT, 3, kVec>, grid, block, 0, st, false, p);
-  if (nv == 2) return launch_kernel(norm_int8_kernel<kT, 2, kVec>, grid, block, 0, st, false, p);
-  return launch_kernel(norm_int8_kernel<kT, 1, kVec>, grid, block, 0, st, false, p);
+  return launch_kernel(norm_int8_kernel<TX, TB, kKind, kT, kNV, kShift>, dim3((unsigned)blocks),
+                       dim3(kT == 32 ? 256 : kT), 0, st, false, p);
+}
+// As few threads a row as hold it with 32 values each: more loads in flight a thread and fewer warps at a barrier
+// (a block of 256 for every row above 1024 columns: 30001 x 1501 in 82 us, against 61 us so).
+template <typename TX, typename TB, int kKind, bool kShift>
+int launch_shift(const NormArgs& p, cudaStream_t st) {
+  const int window = p.D + (kShift ? 7 : 0);
+  if (window <= 256) return launch_t<TX, TB, kKind, kShift, 32, 1>(p, st);
+  if (window <= 512) return launch_t<TX, TB, kKind, kShift, 32, 2>(p, st);
+  if (window <= 1024) return launch_t<TX, TB, kKind, kShift, 32, 4>(p, st);
+  if (window <= 2048) return launch_t<TX, TB, kKind, kShift, 64, 4>(p, st);
+  if (window <= 4096) return launch_t<TX, TB, kKind, kShift, 128, 4>(p, st);
+  if (window <= 8192) return launch_t<TX, TB, kKind, kShift, 256, 4>(p, st);
+  return launch_t<TX, TB, kKind, kShift, 512, 4>(p, st);
+}
+template <typename TX, typename TB>
+int launch_types(const NormArgs& p, bool shift, cudaStream_t st) {
+  if constexpr (std::is_same<TB, None>::value)
+    if (p.kind == kQuantize)
+      return shift ? launch_shift<TX, TB, kQuantize, true>(p, st) : launch_shift<TX, TB, kQuantize, false>(p, st);
+  if (p.kind == kRms) return shift ? launch_shift<TX, TB, kRms, true>(p, st) : launch_shift<TX, TB, kRms, false>(p, st);
+  return shift ? launch_shift<TX, TB, kLayer, true>(p, st) : launch_shift<TX, TB, kLayer, false>(p, st);
+}
+int launch_any(const NormArgs& p, cudaStream_t st) {
+  if (p.rows > 0x7fffffffLL) return DA_ERR_SHAPE;
+  const dim3 grid((unsigned)p.rows);
+  if (p.D <= 512) return launch_kernel(norm_int8_any_kernel<64>, grid, dim3(64), 0, st, false, p);
+  if (p.D <= 8192) return launch_kernel(norm_int8_any_kernel<256>, grid, dim3(256), 0, st, false, p);
+  return launch_kernel(norm_int8_any_kernel<1024>, grid, dim3(1024), 0, st, false, p);
 }
 
 bool float_dtype(int d) { return d == DA_F16 || d == DA_BF16 || d == DA_F32; }
@@ -332,16 +549,27 @@ extern "C" int da_norm_int8(const void* x, int x_dtype, int64_t ldx, const void*
   if (int rc = bind_device(x)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const NormArgs p{x,    branch, weight,  bias,         x_out,        q,          scale, ldx,    ldb, ldo,
-                   ldq,  rows,   x_dtype, branch_dtype, weight_dtype, bias_dtype, kind,  (int)D, eps};
-  const bool vec = D % 8 == 0 && vec8_ok(x, x_dtype, ldx) && (!branch || vec8_ok(branch, branch_dtype, ldb)) &&
-                   (!branch || vec8_ok(x_out, x_dtype, ldo)) && (!weight || vec8_ok(weight, weight_dtype, 8)) &&
-                   (!bias || vec8_ok(bias, bias_dtype, 8)) && ldq % 8 == 0 &&
-                   reinterpret_cast<uintptr_t>(q) % 8 == 0;
-  if (D <= 1024) return vec ? launch_norm<32, true>(p, st) : launch_norm<32, false>(p, st);
-  if (D <= 8192) return vec ? launch_norm<256, true>(p, st) : launch_norm<256, false>(p, st);
-  if (D <= 32768) return vec ? launch_norm<1024, true>(p, st) : launch_norm<1024, false>(p, st);
-  if (rows > 0x7fffffffLL) return DA_ERR_SHAPE;
-  return launch_kernel(norm_int8_wide_kernel, dim3((unsigned)rows), dim3(1024), 0, st, false, p);
+                   ldq,  rows,   x_dtype, branch_dtype, weight_dtype, bias_dtype, kind,  (int)D, eps,
+                   (reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(bias)) % 16 == 0};
+  // 16-byte groups of 8 elements: rows that all start on one, or dense tensors of any width
+  const bool based = vec8_ok(x, x_dtype, 8) && (!branch || (vec8_ok(branch, branch_dtype, 8) && vec8_ok(x_out, x_dtype, 8))) &&
+                     ldq % 8 == 0 && ldq >= (D + 7) / 8 * 8 && reinterpret_cast<uintptr_t>(q) % 8 == 0;
+  const bool rows16 = D % 8 == 0 && vec8_ok(x, x_dtype, ldx) &&
+                      (!branch || (vec8_ok(branch, branch_dtype, ldb) && vec8_ok(x_out, x_dtype, ldo))) &&
+                      (!weight || vec8_ok(weight, weight_dtype, 8)) && (!bias || vec8_ok(bias, bias_dtype, 8));
+  const bool dense = ldx == D && (!branch || (ldb == D && ldo == D));
+  const bool shift = !rows16;
+  if (!based || !(rows16 || dense) || D + (shift ? 7 : 0) > 16384) return launch_any(p, st);
+  if (x_dtype == DA_F32) {
+    if (!branch) return launch_types<float, None>(p, shift, st);
+    if (branch_dtype == DA_F32) return launch_types<float, float>(p, shift, st);
+    if (branch_dtype == DA_BF16) return launch_types<float, __nv_bfloat16>(p, shift, st);
+    return launch_types<float, __half>(p, shift, st);
+  }
+  if (branch && branch_dtype != x_dtype) return launch_any(p, st);
+  if (x_dtype == DA_BF16)
+    return branch ? launch_types<__nv_bfloat16, __nv_bfloat16>(p, shift, st) : launch_types<__nv_bfloat16, None>(p, shift, st);
+  return branch ? launch_types<__half, __half>(p, shift, st) : launch_types<__half, None>(p, shift, st);
 }
 
 extern "C" int da_dequant_int8(const int8_t* q, int64_t ldq, const float* scale, int64_t rows, int64_t D, void* out,
@@ -352,17 +580,7 @@ extern "C" int da_dequant_int8(const int8_t* q, int64_t ldq, const float* scale,
   if (!float_dtype(out_dtype)) return DA_ERR_DTYPE;
   if (int rc = bind_device(q)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool vec = D % 8 == 0 && ldq % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 && vec8_ok(out, out_dtype, ldo);
-  const Div31 per_row((uint32_t)((D + 7) / 8));
-  const int64_t slab = Div31::kMax / per_row.d;  // rows whose items stay below 2^31
-  for (int64_t r0 = 0; r0 < rows; r0 += slab) {
-    const int64_t n = (rows - r0 < slab ? rows - r0 : slab) * per_row.d;
-    const dim3 grid((unsigned)((n + 255) / 256));
-    const int rc = vec ? launch_kernel(dequant_int8_kernel<true>, grid, dim3(256), 0, st, false, q, ldq, scale, r0, n,
-                                       per_row, (int)D, out, out_dtype, ldo)
-                       : launch_kernel(dequant_int8_kernel<false>, grid, dim3(256), 0, st, false, q, ldq, scale, r0, n,
-                                       per_row, (int)D, out, out_dtype, ldo);
-    if (rc) return rc;
-  }
-  return DA_OK;
+  if (out_dtype == DA_F32) return launch_dequant<float>(q, ldq, scale, rows, D, out, ldo, st);
+  if (out_dtype == DA_BF16) return launch_dequant<__nv_bfloat16>(q, ldq, scale, rows, D, out, ldo, st);
+  return launch_dequant<__half>(q, ldq, scale, rows, D, out, ldo, st);
 }

@@ -28,37 +28,6 @@ inline bool vec8_ok(const void* p, int dtype, int64_t ld) {  // 16-byte accesses
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (dtype == DA_F32 ? 4 : 2) % 16 == 0;
 }
 
-DA_DEV void load8(const void* p, int dtype, int64_t off, float* v) {
-  if (dtype == DA_F32) {
-    const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + off);
-    const float4 a = s[0], b = s[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + off);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = dtype == DA_BF16 ? unpack2<__nv_bfloat16>(u[e]) : unpack2<__half>(u[e]);
-      v[2 * e] = f.x;
-      v[2 * e + 1] = f.y;
-    }
-  }
-}
-
-DA_DEV void store8(void* p, int dtype, int64_t off, const float* v) {
-  if (dtype == DA_F32) {
-    float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + off);
-    d[0] = make_float4(v[0], v[1], v[2], v[3]);
-    d[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    uint32_t u[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      u[e] = dtype == DA_BF16 ? pack2<__nv_bfloat16>(v[2 * e], v[2 * e + 1]) : pack2<__half>(v[2 * e], v[2 * e + 1]);
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + off) = make_uint4(u[0], u[1], u[2], u[3]);
-  }
-}
-
 DA_DEV float load1(const void* p, int dtype, int64_t off) {
   if (dtype == DA_F32) return static_cast<const float*>(p)[off];
   if (dtype == DA_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[off]);
@@ -85,14 +54,6 @@ DA_DEV uint2 pack_s8x8(const int* o) {
     return __byte_perm(lo, hi, 0x5410);
   };
   return make_uint2(four(o), four(o + 4));
-}
-
-// Eight bytes as signed integers in fp32: a byte xor 0x80 in the low mantissa bits of 2^23 is 2^23 + 128 + value.
-DA_DEV void unpack_s8x8(uint2 w, float* v) {
-  const uint32_t u[2] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u};
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    v[e] = __uint_as_float(__byte_perm(u[e >> 2], 0x4b000000u, 0x7540 | (e & 3))) - 8388736.f;
 }
 
 // Two fp32 values in one register pair; additions and multiplications of pairs take one issue slot.

@@ -493,9 +493,11 @@ DA_API int da_add_layernorm_bwd(const void* dy, int dy_dtype, const float* d_res
  * written to x_out in x's dtype), scale = max|y| / 127, q = rint(y / scale).  weight
  * [D] may be null (kinds 1 and 2), bias [D] too (kind 2, with weight).  A row whose
  * largest |y| (kind 1: |r w|) is at most 1e-36 becomes q = 0, scale = 0; a row
- * holding NaN or infinity gets a NaN or infinite scale.  x, branch, weight and bias
+ * holding a NaN or an infinity gets a NaN for its scale (and any q).  x, branch, weight and bias
  * in any of DA_F16 / DA_BF16 / DA_F32, row strides ldx, ldb, ldo, ldq in elements, any
- * alignment (16-byte aligned rows with D a multiple of 8 take vector accesses). */
+ * alignment (rows that start on 16 bytes with D a multiple of 8, and dense tensors of any
+ * D with ldq at least D rounded up to 8, take vector accesses; bytes of a q row past D are
+ * then written too). */
 DA_API int da_norm_int8(const void* x, int x_dtype, int64_t ldx, const void* branch, int branch_dtype, int64_t ldb,
                         const void* weight, int weight_dtype, const void* bias, int bias_dtype, int kind,
                         int64_t rows, int64_t D, float eps, void* x_out, int64_t ldo, int8_t* q, int64_t ldq,
