@@ -25,6 +25,7 @@ from .eight_bit import (
     weight_grad_checkpoint8,
 )
 from .graphs import GraphedModuleStep
+from .int8_model import Int8DoubleAttentionLM, Int8Linear
 from .modules import (
     DoubleAttentionAux,
     DoubleAttentionBlock,
@@ -43,6 +44,8 @@ __all__ = [
     "DoubleAttentionLM",
     "DoubleAttentionStack",
     "GraphedModuleStep",
+    "Int8DoubleAttentionLM",
+    "Int8Linear",
     "Int8Rows",
     "SharedDictionaryAttention",
     "SharedDictionaryBank",

@@ -276,9 +276,8 @@ int launch_pair(const Params& p, cudaStream_t st) {
                                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if (int rc = make_tmap_2d(&tc, p.c, dt, elem, p.N, p.M, (uint64_t)p.ldc * elem, 128 / elem, 32)) return rc;
   }
-  auto kern = gemm_pair_kernel<kOut, kGelu>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem + 1024) != cudaSuccess)
-    return record_cuda_error();
+  constexpr auto kern = gemm_pair_kernel<kOut, kGelu>;
+  if (int rc = allow_smem<kern>(C::kSmem + 1024)) return rc;
   const int64_t tiles = (int64_t)((p.M + C::kTile - 1) / C::kTile) * ((p.N + C::kTile - 1) / C::kTile);
   const int pairs = tiles < sm_count() / 2 ? (int)tiles : sm_count() / 2;
   return launch_kernel(kern, dim3(2 * pairs), dim3(C::kThreads), C::kSmem + 1024, st, true, ta, tb, tc, p);
@@ -474,9 +473,8 @@ int launch_few(const Params& p, cudaStream_t st) {
   CUtensorMap ta, tb;
   if (int rc = make_tmap_2d(&ta, p.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.M, p.lda, 128, kTn)) return rc;
   if (int rc = make_tmap_2d(&tb, p.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.N, p.ldb, 128, 128)) return rc;
-  auto kern = gemm_few_kernel<kTn, kSplits>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem + 1024) != cudaSuccess)
-    return record_cuda_error();
+  constexpr auto kern = gemm_few_kernel<kTn, kSplits>;
+  if (int rc = allow_smem<kern>(C::kSmem + 1024)) return rc;
   const int64_t tiles = (int64_t)((p.N + 127) / 128) * ((p.M + kTn - 1) / kTn);
   return launch_cluster(kern, dim3((unsigned)(tiles * kSplits)), dim3(C::kThreads), C::kSmem + 1024, st, kSplits, ta, tb,
                         p);

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/da_b200.h"
 
 namespace da {
@@ -100,6 +102,21 @@ int launch_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, c
   cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...) != cudaSuccess) return record_cuda_error();
   note_launch();
+  return DA_OK;
+}
+
+// Raises the dynamic shared memory limit of a kernel, once per device (the call takes longer than a launch's other
+// host work).
+template <auto kKernel>
+int allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return record_cuda_error();
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return DA_OK;
+  if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return record_cuda_error();
+  done.fetch_or(bit, std::memory_order_relaxed);
   return DA_OK;
 }
 

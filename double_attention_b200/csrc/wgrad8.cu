@@ -374,9 +374,8 @@ Plan plan_for(int64_t rows, int64_t N, int64_t K) {
 
 template <typename T, typename TO>
 int launch(const CUtensorMap& ty, const CUtensorMap& tq, const Params& p, cudaStream_t st) {
-  auto kern = wgrad_kernel<T, TO>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem + 1024) != cudaSuccess)
-    return record_cuda_error();
+  constexpr auto kern = wgrad_kernel<T, TO>;
+  if (int rc = allow_smem<kern>(kSmem + 1024)) return rc;
   const int64_t items = (int64_t)((p.N + kTile - 1) / kTile) * ((p.K + kTile - 1) / kTile) * p.splits;
   const int pairs = items < sm_count() / 2 ? (int)items : sm_count() / 2;
   return launch_kernel(kern, dim3(2 * pairs), dim3(kThreads), kSmem + 1024, st, true, ty, tq, p);

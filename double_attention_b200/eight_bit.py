@@ -17,6 +17,7 @@ Every numeric step runs in the kernels of ``libda_b200.so``; unsupported inputs 
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import NamedTuple
 
@@ -24,11 +25,10 @@ import torch
 from torch import Tensor
 
 from . import _lib, ops
-from ._lib import call, dtype_code, ptr, stream_ptr
+from ._lib import call, ptr
 
 BLOCK = 32          # columns of a checkpoint that share one exponent
 MAX_INNER = 131071  # K of an int8 product: 128 * 128 * K stays below 2^31
-_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _HALF = (torch.float16, torch.bfloat16)
 
 # The block's feed-forward branch keeps its activations in 8 bits when set (see feedforward_checkpoint8):
@@ -38,60 +38,87 @@ FEEDFORWARD_CHECKPOINT8 = False
 
 
 # ----------------------------------------------------------------------------- helpers
-def _launch(device: torch.device, name: str, *args) -> None:
-    """One library call on ``device``'s current stream, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, stream_ptr(device))
+# A call on a few rows is over on the device in 2 to 4 us, so the checks here read each attribute once and make no
+# views where the memory already lies as the kernel wants it.
+_CODES = {torch.float16: _lib.DA_F16, torch.bfloat16: _lib.DA_BF16, torch.float32: _lib.DA_F32}
+
+
+def _launch(device: int, name: str, *args) -> None:
+    """One library call on the current stream of CUDA device ``device``, whichever device is current."""
+    if device == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            call(name, *args, stream_ptr(device))
+            call(name, *args, torch._C._cuda_getCurrentRawStream(device))
 
 
-def _check_cuda(name: str, first: Tensor, *others: Tensor | None) -> torch.device:
-    if not first.is_cuda:
+def _new(shape, dtype: torch.dtype, device: torch.device) -> Tensor:
+    """A new dense tensor (torch.empty_strided takes 1.5 us on the host, torch.empty 2 to 4.5)."""
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
+    if len(shape) == 1:
+        return torch.empty_strided(shape, (1,), dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _device_of(name: str, first: Tensor, *others: Tensor | None) -> int:
+    device = first.get_device()
+    if device < 0:
         raise ValueError(f"{name} requires CUDA tensors")
-    device = first.device
     for t in others:
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} requires its tensors on one device, got {device} and {t.device}")
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"{name} requires its tensors on one device, got {first.device} and {t.device}")
     return device
 
 
-def _check_float(name: str, what: str, t: Tensor, allowed=_FLOATS) -> None:
-    if t.dtype not in allowed:
-        names = ", ".join(str(d).removeprefix("torch.") for d in allowed)
-        raise ValueError(f"{name} takes {what} in {names}, got {t.dtype}")
+def _float_code(name: str, what: str, t: Tensor) -> int:
+    code = _CODES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} takes {what} in float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _half_code(name: str, what: str, t: Tensor) -> int:
+    if t.dtype not in _HALF:
+        raise ValueError(f"{name} takes {what} in bfloat16 or float16, got {t.dtype}")
+    return _CODES[t.dtype]
 
 
 def _inference_only(name: str, *tensors: Tensor | None) -> None:
-    if ops._grad_wanted(*tensors):
-        raise RuntimeError(f"{name} has no backward: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no backward: call it under torch.no_grad() or on detached tensors")
 
 
-def _rows(t: Tensor) -> Tensor:
-    """``t`` [..., D] as [rows, D] with unit column stride; a view where its strides allow one."""
+def _rows(t: Tensor) -> tuple[Tensor, int, int]:
+    """``(t, rows, row stride)`` of ``t`` [..., D] with unit column stride: as it lies, or a copy that has it."""
+    d = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // d, d
     if t.ndim != 2:
-        t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+        t = t.reshape(-1, d)
+    if t.stride(1) != 1 and d > 1:
+        t = t.contiguous()
+    return t, t.shape[0], t.stride(0)
 
 
 def _round_up(n: int, to: int) -> int:
     return -(-n // to) * to
 
 
-def _aligned_rows(t: Tensor, elements: int) -> Tensor:
-    """[rows, D] with rows starting on 16 bytes (``elements`` of them): as is, or copied to padded rows."""
-    rows, d = t.shape
-    stride = t.stride(0)
-    if t.data_ptr() % 16 == 0 and (rows == 1 or (stride >= d and stride % elements == 0)):
-        return t
-    out = torch.empty(rows, _round_up(d, elements), dtype=t.dtype, device=t.device)[:, :d]
-    return out.copy_(t)
-
-
-def _stride16(t: Tensor, elements: int) -> int:
-    """The row stride handed to a kernel that wants 16-byte rows (a single row has none of its own)."""
-    return t.stride(0) if t.shape[0] > 1 else _round_up(t.shape[1], elements)
+def _rows16(t: Tensor, elements: int) -> tuple[Tensor, int, int]:
+    """As :func:`_rows`, every row on 16 bytes (``elements`` of them): as it lies, or copied to padded rows."""
+    t, rows, stride = _rows(t)
+    d = t.shape[-1]
+    if t.data_ptr() % 16 == 0:
+        if stride % elements == 0 and stride >= d:
+            return t, rows, stride
+        if rows == 1:  # has no stride of its own
+            return t, rows, _round_up(d, elements)
+    out = _new((rows, _round_up(d, elements)), t.dtype, t.device)
+    out[:, :d] = t.reshape(rows, d)
+    return out, rows, out.shape[1]
 
 
 # ----------------------------------------------------------------------------- int8 rows
@@ -108,29 +135,29 @@ class Int8Rows(NamedTuple):
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> Tensor:
         """The values the rows stand for, each rounded once to ``dtype``."""
-        q, scale = _check_rows("Int8Rows.dequantize", self)
-        if dtype not in _FLOATS:
-            raise ValueError(f"Int8Rows.dequantize writes float32, bfloat16 or float16, got {dtype}")
-        out = torch.empty(self.values.shape, dtype=dtype, device=q.device)
+        name = "Int8Rows.dequantize"
+        device = _check_rows(name, self)
+        if dtype not in _CODES:
+            raise ValueError(f"{name} writes float32, bfloat16 or float16, got {dtype}")
+        out = _new(self.values.shape, dtype, self.values.device)
         if out.numel():
-            rows, d = q.shape
-            _launch(q.device, "da_dequant_int8", q.data_ptr(), q.stride(0), scale.data_ptr(), rows, d,
-                    out.data_ptr(), dtype_code(dtype), d)
+            q, rows, stride = _rows(self.values)
+            d = q.shape[-1]
+            _launch(device, "da_dequant_int8", q.data_ptr(), stride, self.scale.contiguous().data_ptr(), rows, d,
+                    out.data_ptr(), _CODES[dtype], d)
         return out
 
 
-def _check_rows(name: str, x: Int8Rows) -> tuple[Tensor, Tensor]:
-    """``(values [rows, K], scale [rows])`` of int8 rows, checked."""
+def _check_rows(name: str, x: Int8Rows) -> int:
+    """The device of int8 rows, checked."""
     values, scale = x
-    if values.dtype != torch.int8 or values.ndim < 1:
-        raise ValueError(f"{name} takes int8 rows [..., K], got {values.dtype} {tuple(values.shape)}")
-    if scale.dtype != torch.float32 or scale.shape != values.shape[:-1]:
-        raise ValueError(f"{name} takes one fp32 scale per row {tuple(values.shape[:-1])}, "
+    shape = values.shape
+    if values.dtype != torch.int8 or not shape or not shape[-1]:
+        raise ValueError(f"{name} takes int8 rows [..., K] with K at least 1, got {values.dtype} {tuple(shape)}")
+    if scale.dtype != torch.float32 or scale.shape != shape[:-1]:
+        raise ValueError(f"{name} takes one fp32 scale per row {tuple(shape[:-1])}, "
                          f"got {scale.dtype} {tuple(scale.shape)}")
-    _check_cuda(name, values, scale)
-    if scale.ndim != 1:
-        scale = scale.reshape(-1)
-    return _rows(values), scale if scale.is_contiguous() else scale.contiguous()
+    return _device_of(name, values, scale)
 
 
 _QUANTIZE, _RMS, _LAYER = 0, 1, 2
@@ -138,54 +165,48 @@ _QUANTIZE, _RMS, _LAYER = 0, 1, 2
 
 def _norm_int8(name: str, x: Tensor, branch: Tensor | None, weight: Tensor | None, bias: Tensor | None, kind: int,
                eps: float) -> tuple[Tensor | None, Int8Rows]:
-    device = _check_cuda(name, x, branch, weight, bias)
-    if x.ndim < 1 or x.shape[-1] < 1:
-        raise ValueError(f"{name} takes rows [..., D] with D at least 1, got {tuple(x.shape)}")
-    d = x.shape[-1]
-    _check_float(name, "x", x)
+    device = _device_of(name, x, branch, weight, bias)
+    shape = x.shape
+    if not shape or not shape[-1]:
+        raise ValueError(f"{name} takes rows [..., D] with D at least 1, got {tuple(shape)}")
+    d = shape[-1]
+    x_code = _float_code(name, "x", x)
+    b_code = w_code = bias_code = 0
     if branch is not None:
-        if branch.shape != x.shape:
-            raise ValueError(f"branch shape {tuple(branch.shape)} does not match the residual {tuple(x.shape)}")
-        _check_float(name, "the branch", branch)
-    for what, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _check_float(name, what, t)
-            if t.shape != (d,):
-                raise ValueError(f"{name} takes a {what} of shape [{d}], got {tuple(t.shape)}")
+        if branch.shape != shape:
+            raise ValueError(f"branch shape {tuple(branch.shape)} does not match the residual {tuple(shape)}")
+        b_code = _float_code(name, "the branch", branch)
+    if weight is not None:
+        w_code = _float_code(name, "weight", weight)
+        weight = weight.contiguous()
+        if bias is not None:
+            bias_code = _float_code(name, "bias", bias)
+            bias = bias.contiguous()
     _inference_only(name, x, branch, weight, bias)
-    lead = x.shape[:-1]
-    x2 = _rows(x)
-    rows = x2.shape[0]
-    x_out = b2 = None
-    if branch is not None:
-        b2 = _rows(branch)
-        x_out = torch.empty(x.shape, dtype=x.dtype, device=device)
     pitch = _round_up(d, 16)
-    q = torch.empty(rows, pitch, dtype=torch.int8, device=device)
-    scale = torch.empty(lead, dtype=torch.float32, device=device)
+    lead = shape[:-1]
+    q = _new((*lead, pitch), torch.int8, x.device)
+    scale = _new(lead, torch.float32, x.device)
+    x2, rows, ldx = _rows(x)
+    x_out, b2, ldb = None, None, 0
+    if branch is not None:
+        x_out = _new(shape, x.dtype, x.device)
+        b2, _, ldb = _rows(branch)
     if rows:
-        w = None if weight is None else weight.contiguous()
-        b = None if bias is None else bias.contiguous()
-        _launch(device, "da_norm_int8", x2.data_ptr(), dtype_code(x.dtype), x2.stride(0), ptr(b2),
-                0 if b2 is None else dtype_code(b2.dtype), 0 if b2 is None else b2.stride(0), ptr(w),
-                0 if w is None else dtype_code(w.dtype), ptr(b), 0 if b is None else dtype_code(b.dtype), kind, rows, d,
-                eps, ptr(x_out), d, q.data_ptr(), pitch, scale.data_ptr())
-    if pitch != d:
-        q = q[:, :d]
-    if len(lead) != 1:
-        q = q.unflatten(0, lead) if lead else q[0]
-    return x_out, Int8Rows(q, scale)
+        _launch(device, "da_norm_int8", x2.data_ptr(), x_code, ldx, ptr(b2), b_code, ldb, ptr(weight), w_code, ptr(bias),
+                bias_code, kind, rows, d, eps, ptr(x_out), d, q.data_ptr(), pitch, scale.data_ptr())
+    return x_out, Int8Rows(q if pitch == d else q[..., :d], scale)
 
 
 def _rms_args(norm, x: Tensor) -> tuple[Tensor | None, float]:
-    if not isinstance(norm, torch.nn.RMSNorm) or tuple(norm.normalized_shape) != (x.shape[-1],):
-        raise ValueError(f"expected an nn.RMSNorm over the last dimension of x ({x.shape[-1]}), got {norm}")
+    if not isinstance(norm, torch.nn.RMSNorm) or norm.normalized_shape != x.shape[-1:]:
+        raise ValueError(f"expected an nn.RMSNorm over the last dimension of x {tuple(x.shape)}, got {norm}")
     return norm.weight, torch.finfo(x.dtype).eps if norm.eps is None else norm.eps
 
 
 def _layer_args(norm, x: Tensor) -> tuple[Tensor | None, Tensor | None, float]:
-    if not isinstance(norm, torch.nn.LayerNorm) or tuple(norm.normalized_shape) != (x.shape[-1],):
-        raise ValueError(f"expected an nn.LayerNorm over the last dimension of x ({x.shape[-1]}), got {norm}")
+    if not isinstance(norm, torch.nn.LayerNorm) or norm.normalized_shape != x.shape[-1:]:
+        raise ValueError(f"expected an nn.LayerNorm over the last dimension of x {tuple(x.shape)}, got {norm}")
     return norm.weight, norm.bias, norm.eps
 
 
@@ -231,33 +252,33 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Tensor | None = None, *, ge
     The sum over K (at most 131071) is exact; it is scaled, biased and activated in fp32 and rounded once to
     ``dtype`` (bf16, fp16 or fp32).  x [..., K], weight [N, K], bias [N] in any float dtype."""
     name = "int8_linear"
-    xq, xs = _check_rows(name, x)
-    wq, ws = _check_rows(name, weight)
-    if weight.values.ndim != 2:
-        raise ValueError(f"{name} takes a weight [N, K], got {tuple(weight.values.shape)}")
-    n, k = wq.shape
-    device = _check_cuda(name, xq, wq, bias)
-    if xq.shape[1] != k or not 0 < k <= MAX_INNER or n < 1:
-        raise ValueError(f"{name}: x {tuple(x.values.shape)} and weight {tuple(weight.values.shape)} must share "
+    device = _check_rows(name, x)
+    w_shape = weight.values.shape
+    if _check_rows(name, weight) != device or len(w_shape) != 2:
+        raise ValueError(f"{name} takes a weight [N, K] on x's device, got {tuple(w_shape)} on {weight.values.device}")
+    n, k = w_shape
+    if x.values.shape[-1] != k or k > MAX_INNER or n < 1:
+        raise ValueError(f"{name}: x {tuple(x.values.shape)} and weight {tuple(w_shape)} must share "
                          f"an inner size of 1 to {MAX_INNER}")
-    if dtype not in _FLOATS:
+    code = _CODES.get(dtype)
+    if code is None:
         raise ValueError(f"{name} writes float32, bfloat16 or float16, got {dtype}")
-    bias_code = 0
+    bias_ptr, bias_code = None, 0
     if bias is not None:
-        _check_float(name, "a bias", bias)
-        if bias.shape != (n,):
-            raise ValueError(f"{name} takes a bias of shape [{n}], got {tuple(bias.shape)}")
+        bias_code = _float_code(name, "a bias", bias)
+        if bias.shape != (n,) or bias.get_device() != device:
+            raise ValueError(f"{name} takes a bias of shape [{n}] on x's device, got {tuple(bias.shape)} on {bias.device}")
         _inference_only(name, bias)
         bias = bias.contiguous()
-        bias_code = dtype_code(bias.dtype)
-    lead = x.values.shape[:-1]
-    out = torch.empty(*lead, n, dtype=dtype, device=device)
-    rows = xq.shape[0]
+        bias_ptr = bias.data_ptr()
+    out = _new((*x.values.shape[:-1], n), dtype, x.values.device)
+    xq, rows, ldx = _rows16(x.values, 16)
     if rows:
-        xq, wq = _aligned_rows(xq, 16), _aligned_rows(wq, 16)
-        _launch(device, "da_gemm_i8", xq.data_ptr(), _stride16(xq, 16), xs.data_ptr(), wq.data_ptr(), _stride16(wq, 16),
-                ws.data_ptr(), ptr(bias), bias_code, int(gelu), out.data_ptr(), n, dtype_code(dtype), rows, n, k,
-                ops.workspace(device).status.data_ptr())
+        wq, _, ldw = _rows16(weight.values, 16)
+        xs, ws = x.scale.contiguous(), weight.scale.contiguous()
+        _launch(device, "da_gemm_i8", xq.data_ptr(), ldx, xs.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), bias_ptr,
+                bias_code, int(gelu), out.data_ptr(), n, code, rows, n, k,
+                ops.workspace(out.device).status.data_ptr())
     return out
 
 
@@ -282,44 +303,45 @@ class Checkpoint8:
     def restore(self) -> Tensor:
         """The values the checkpoint stands for, in the activation's shape and dtype."""
         device = _check_checkpoint("Checkpoint8.restore", self)
-        out = torch.empty(self.shape, dtype=self.dtype, device=device)
+        out = _new(self.shape, self.dtype, self.values.device)
         if out.numel():
             d = self.shape[-1]
             _launch(device, "da_checkpoint8_restore", self.values.data_ptr(), self.exponent.data_ptr(), self.rows, d,
-                    out.data_ptr(), dtype_code(self.dtype), d)
+                    out.data_ptr(), _CODES[self.dtype], d)
         return out
 
 
-def _check_checkpoint(name: str, c: Checkpoint8) -> torch.device:
-    d = c.shape[-1]
+def _check_checkpoint(name: str, c: Checkpoint8) -> int:
+    """The device of a checkpoint, checked."""
+    values, exponent, shape = c.values, c.exponent, c.shape
+    d = shape[-1]
     blocks = -(-d // BLOCK)
-    rows = 1
-    for s in c.shape[:-1]:
-        rows *= s
-    if (c.dtype not in _HALF or d < 1 or c.values.dtype != torch.int8 or c.exponent.dtype != torch.int8
-            or c.values.shape != (rows, blocks * BLOCK) or c.exponent.shape != (rows, blocks)
-            or not c.values.is_contiguous() or not c.exponent.is_contiguous() or c.values.data_ptr() % 16):
+    rows = math.prod(shape[:-1])
+    if (c.dtype not in _HALF or d < 1 or values.dtype != torch.int8 or exponent.dtype != torch.int8
+            or values.shape != (rows, blocks * BLOCK) or exponent.shape != (rows, blocks)
+            or not values.is_contiguous() or not exponent.is_contiguous() or values.data_ptr() % 16):
         raise ValueError(f"{name} takes a checkpoint of a 16-bit activation: dense int8 values "
-                         f"[{rows}, {blocks * BLOCK}] and exponents [{rows}, {blocks}], got {c.dtype} "
-                         f"{tuple(c.values.shape)}, {tuple(c.exponent.shape)}")
-    return _check_cuda(name, c.values, c.exponent)
+                         f"[{rows}, {blocks * BLOCK}] on 16 bytes and exponents [{rows}, {blocks}], got {c.dtype} "
+                         f"{tuple(values.shape)}, {tuple(exponent.shape)}")
+    return _device_of(name, values, exponent)
 
 
 def _checkpoint8(name: str, x: Tensor, gelu: bool) -> tuple[Tensor | None, Checkpoint8]:
-    device = _check_cuda(name, x)
-    _check_float(name, "an activation", x, _HALF)
-    if x.ndim < 1 or x.shape[-1] < 1:
-        raise ValueError(f"{name} takes rows [..., D] with D at least 1, got {tuple(x.shape)}")
-    x2 = _rows(x)
-    rows, d = x2.shape
+    device = _device_of(name, x)
+    code = _half_code(name, "an activation", x)
+    shape = x.shape
+    if not shape or not shape[-1]:
+        raise ValueError(f"{name} takes rows [..., D] with D at least 1, got {tuple(shape)}")
+    x2, rows, ldx = _rows(x)
+    d = shape[-1]
     blocks = -(-d // BLOCK)
-    values = torch.empty(rows, blocks * BLOCK, dtype=torch.int8, device=device)
-    exponent = torch.empty(rows, blocks, dtype=torch.int8, device=device)
-    h = torch.empty(x.shape, dtype=x.dtype, device=device) if gelu else None
+    values = _new((rows, blocks * BLOCK), torch.int8, x.device)
+    exponent = _new((rows, blocks), torch.int8, x.device)
+    h = _new(shape, x.dtype, x.device) if gelu else None
     if rows:
-        _launch(device, "da_checkpoint8", x2.data_ptr(), dtype_code(x.dtype), x2.stride(0), rows, d, int(gelu), ptr(h), d,
-                values.data_ptr(), exponent.data_ptr())
-    return h, Checkpoint8(values, exponent, tuple(x.shape), x.dtype)
+        _launch(device, "da_checkpoint8", x2.data_ptr(), code, ldx, rows, d, int(gelu), ptr(h), d, values.data_ptr(),
+                exponent.data_ptr())
+    return h, Checkpoint8(values, exponent, tuple(shape), x.dtype)
 
 
 def checkpoint8(x: Tensor) -> Checkpoint8:
@@ -339,16 +361,16 @@ def gelu_checkpoint8_backward(dh: Tensor, kept: Checkpoint8) -> tuple[Tensor, Te
     the next layer's weight gradient."""
     name = "gelu_checkpoint8_backward"
     device = _check_checkpoint(name, kept)
-    _check_cuda(name, kept.values, dh)
-    if tuple(dh.shape) != kept.shape or dh.dtype != kept.dtype:
-        raise ValueError(f"{name}: dh {dh.dtype} {tuple(dh.shape)} does not match the checkpoint {kept.dtype} {kept.shape}")
+    if dh.shape != kept.shape or dh.dtype != kept.dtype or dh.get_device() != device:
+        raise ValueError(f"{name}: dh {dh.dtype} {tuple(dh.shape)} on {dh.device} does not match the checkpoint "
+                         f"{kept.dtype} {kept.shape} on {kept.values.device}")
     _inference_only(name, dh)
-    dz = torch.empty(kept.shape, dtype=dh.dtype, device=device)
-    h = torch.empty(kept.shape, dtype=dh.dtype, device=device)
-    if dz.numel():
-        d2 = _rows(dh)
-        rows, d = d2.shape
-        _launch(device, "da_checkpoint8_gelu_bwd", d2.data_ptr(), dtype_code(dh.dtype), d2.stride(0), kept.values.data_ptr(),
+    dz = _new(kept.shape, dh.dtype, dh.device)
+    h = _new(kept.shape, dh.dtype, dh.device)
+    d2, rows, ldd = _rows(dh)
+    if rows:
+        d = kept.shape[-1]
+        _launch(device, "da_checkpoint8_gelu_bwd", d2.data_ptr(), _CODES[dh.dtype], ldd, kept.values.data_ptr(),
                 kept.exponent.data_ptr(), rows, d, dz.data_ptr(), d, h.data_ptr(), d)
     return dz, h
 
@@ -359,25 +381,24 @@ def weight_grad_checkpoint8(dy: Tensor, kept: Checkpoint8, dtype: torch.dtype | 
     fp32)."""
     name = "weight_grad_checkpoint8"
     device = _check_checkpoint(name, kept)
-    _check_cuda(name, kept.values, dy)
-    if tuple(dy.shape[:-1]) != kept.shape[:-1] or dy.dtype != kept.dtype or dy.shape[-1] < 1:
-        raise ValueError(f"{name}: dy {dy.dtype} {tuple(dy.shape)} does not match the checkpoint {kept.dtype} {kept.shape}")
+    shape = dy.shape
+    if not shape or shape[:-1] != kept.shape[:-1] or not shape[-1] or dy.dtype != kept.dtype or dy.get_device() != device:
+        raise ValueError(f"{name}: dy {dy.dtype} {tuple(shape)} on {dy.device} does not match the checkpoint "
+                         f"{kept.dtype} {kept.shape} on {kept.values.device}")
     dtype = dtype or dy.dtype
-    if dtype not in (torch.float32, dy.dtype):
+    if dtype != torch.float32 and dtype != dy.dtype:
         raise ValueError(f"{name} stores fp32 or dy's {dy.dtype}, got {dtype}")
     _inference_only(name, dy)
-    n, k = dy.shape[-1], kept.shape[-1]
-    out = torch.empty(n, k, dtype=dtype, device=device)
-    d2 = _rows(dy)
-    rows = d2.shape[0]
+    n, k = shape[-1], kept.shape[-1]
+    out = _new((n, k), dtype, dy.device)
+    d2, rows, ldd = _rows16(dy, 8)
     if not rows:
         return out.zero_()
-    d2 = _aligned_rows(d2, 8)
-    elems = int(_lib.lib().da_checkpoint8_wgrad_workspace_elems(rows, n, k))
-    work = torch.empty(max(elems, 4), dtype=torch.float32, device=device)
-    _launch(device, "da_checkpoint8_wgrad", d2.data_ptr(), dtype_code(dy.dtype), _stride16(d2, 8), kept.values.data_ptr(),
-            kept.exponent.data_ptr(), rows, n, k, out.data_ptr(), dtype_code(dtype), k, work.data_ptr(), work.numel(),
-            ops.workspace(device).status.data_ptr())
+    elems = _lib.lib().da_checkpoint8_wgrad_workspace_elems(rows, n, k)
+    work = _new((elems,), torch.float32, dy.device) if elems else None
+    _launch(device, "da_checkpoint8_wgrad", d2.data_ptr(), _CODES[dy.dtype], ldd, kept.values.data_ptr(),
+            kept.exponent.data_ptr(), rows, n, k, out.data_ptr(), _CODES[dtype], k, ptr(work), elems,
+            ops.workspace(out.device).status.data_ptr())
     return out
 
 

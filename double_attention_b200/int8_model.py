@@ -1,0 +1,128 @@
+"""A trained ``DoubleAttentionLM`` served in int8.
+
+:class:`Int8DoubleAttentionLM` quantises every Linear of the model once (a scale per output channel) and runs
+its forward on the eight-bit operators: each norm adds the pending branch and leaves int8 rows, the projections
+and the feed-forward layers multiply int8 rows, the route and the outer attention between them stay on their
+16-bit kernels.  Per layer that is four int8 products (Q and K together, V, output, two of the feed-forward)
+between two fused norms.  Inference only; the model it is built from is left as it is.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor, nn
+
+from . import ops
+from .eight_bit import Int8Rows, add_layernorm_int8, int8_linear, layernorm_int8, quantize_int8
+from .modules import DoubleAttentionBlock, DoubleAttentionLM
+
+_HALF = (torch.float16, torch.bfloat16)
+_ATTENTION_ROWS = 128  # rows (batch times length) below which the attention kernels have no tile
+
+
+class Int8Linear(nn.Module):
+    """A Linear whose weight is held in int8 with a scale per output channel and whose bias in fp32.
+
+    ``forward`` takes int8 rows, or activations that it quantises per token first; with ``gelu`` the output
+    goes through GELU in the product's epilogue."""
+
+    def __init__(self, weight: Tensor, bias: Tensor | None, dtype: torch.dtype) -> None:
+        super().__init__()
+        rows = quantize_int8(weight.detach())
+        self.register_buffer("weight", rows.values)
+        self.register_buffer("scale", rows.scale)
+        self.register_buffer("bias", None if bias is None else bias.detach().float().clone())
+        self.dtype = dtype
+
+    def forward(self, x: Tensor | Int8Rows, *, gelu: bool = False) -> Tensor:
+        rows = x if isinstance(x, Int8Rows) else quantize_int8(x)
+        return int8_linear(rows, Int8Rows(self.weight, self.scale), self.bias, gelu=gelu, dtype=self.dtype)
+
+
+class _Int8Block(nn.Module):
+    def __init__(self, block: DoubleAttentionBlock, dtype: torch.dtype) -> None:
+        super().__init__()
+        attention, cfg = block.attention, block.attention.config
+        if cfg.q_dictionary_feedforward:
+            raise NotImplementedError("int8 serving does not cover the Q-dictionary feed-forward")
+        first, act, second, _ = block.feedforward
+        if act.approximate != "none":
+            raise NotImplementedError("int8 serving covers the exact form of GELU")
+        self.config = cfg
+        self.attention_norm, self.feedforward_norm = block.attention_norm, block.feedforward_norm
+        self.query_key = Int8Linear(torch.cat((attention.query.weight, attention.key.weight)), None, dtype)
+        self.value = Int8Linear(attention.value.weight, attention.value.bias, torch.bfloat16)  # as the attention reads it
+        self.output = None
+        if isinstance(attention.output, nn.Linear):
+            self.output = Int8Linear(attention.output.weight, None, dtype)
+        self.first = Int8Linear(first.weight, first.bias, dtype)
+        self.second = Int8Linear(second.weight, second.bias, dtype)
+        beta, scales = ops.temperatures(attention.log_beta, attention.log_score_scales)
+        self.register_buffer("beta", beta.clone())
+        self.register_buffer("scales", scales.clone())
+        logits = attention.map_mix_logits
+        self.register_buffer("map_weights", None if logits is None else torch.softmax(logits.float(), dim=0))
+
+    def attend(self, rows: Int8Rows, views: ops.DictionaryViews) -> Tensor:
+        cfg = self.config
+        batch, tokens = rows.scale.shape
+        projected, value = self.query_key(rows), self.value(rows)
+        length = tokens
+        if cfg.causal and batch * tokens < _ATTENTION_ROWS:
+            # positions after the last one, which no query sees, fill the attention's smallest tile
+            length = -(-_ATTENTION_ROWS // batch)
+            projected = nn.functional.pad(projected, (0, 0, 0, length - tokens))
+            value = nn.functional.pad(value, (0, 0, 0, length - tokens))
+        routed = ops.route_projected(projected.view(batch * length, -1), views, self.beta, cfg, batch, length)
+        if cfg.map_combine == "weighted_sum":
+            combined = ops.routed_attention_mixed(routed, value, self.scales, self.map_weights, cfg)
+        else:
+            combined = ops.routed_attention_maps(routed, value, self.scales, cfg).permute(0, 2, 1, 3).flatten(2)
+        combined = combined[:, :tokens]
+        return combined if self.output is None else self.output(combined)
+
+    def forward(self, x: Tensor, pending: Tensor | None, views: ops.DictionaryViews) -> tuple[Tensor, Tensor]:
+        """``x + pending`` through the block; returns the residual and the feed-forward branch still to be added."""
+        if pending is None:
+            rows = layernorm_int8(x, self.attention_norm)
+        else:
+            x, rows = add_layernorm_int8(x, pending, self.attention_norm)
+        x, rows = add_layernorm_int8(x, self.attend(rows, views), self.feedforward_norm)
+        return x, self.second(self.first(rows, gelu=True))
+
+
+class Int8DoubleAttentionLM(nn.Module):
+    """``DoubleAttentionLM`` in int8: ``Int8DoubleAttentionLM(lm)(token_ids)`` gives the logits [B, T, V].
+
+    ``lm`` must be on an sm_100 GPU; its embeddings, norms and dictionaries are shared, not copied.  ``dtype`` is
+    the 16-bit type of the activations between the int8 products and of the logits."""
+
+    def __init__(self, lm: DoubleAttentionLM, dtype: torch.dtype = torch.bfloat16) -> None:
+        super().__init__()
+        if dtype not in _HALF:
+            raise ValueError(f"int8 serving computes in bfloat16 or float16 between its products, got {dtype}")
+        weight = lm.token_embedding.weight
+        ops.resolve_backend("auto", weight, dtype)
+        with torch.no_grad():
+            self.max_sequence_length = lm.max_sequence_length
+            self.token_embedding, self.position_embedding = lm.token_embedding, lm.position_embedding
+            self.final_norm = lm.final_norm
+            stack = lm.stack
+            self.blocks = nn.ModuleList(_Int8Block(b, dtype) for b in stack.blocks)
+            self.lm_head = Int8Linear(lm.lm_head.weight, None, dtype)
+            self._views = [ops.dictionary_views(b.raw_key, b.raw_value, stack.config.eps, dtype) for b in stack.banks]
+            self._bank_of = [min(i // stack.dictionary_group_size, len(stack.banks) - 1) for i in range(len(stack.blocks))]
+
+    @torch.no_grad()
+    def forward(self, token_ids: Tensor) -> Tensor:
+        if token_ids.ndim != 2:
+            raise ValueError("token_ids must have shape [B, T]")
+        length = token_ids.shape[1]
+        if length > self.max_sequence_length:
+            raise ValueError(f"sequence length {length} exceeds configured maximum {self.max_sequence_length}")
+        positions = torch.arange(length, device=token_ids.device)
+        x = (self.token_embedding(token_ids) + self.position_embedding(positions)[None]).float()
+        pending = None
+        for block, bank in zip(self.blocks, self._bank_of):
+            x, pending = block(x, pending, self._views[bank])
+        return self.lm_head(add_layernorm_int8(x, pending, self.final_norm)[1])

@@ -20,7 +20,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
-from . import ops
+from . import eight_bit, ops
 from .config import DoubleAttentionConfig
 
 # The reference exposes this switch to compare fused and separate Q/K
@@ -270,6 +270,9 @@ class DoubleAttentionBlock(nn.Module):
                             normalized_dictionary: tuple[Tensor, Tensor] | None) -> Tensor:
         if not self.attention.config.q_dictionary_feedforward:
             first, act, second, drop = self.feedforward
+            if (eight_bit.FEEDFORWARD_CHECKPOINT8 and torch.is_grad_enabled() and act.approximate == "none"
+                    and eight_bit.checkpoint8_supported(normalized_x, first, second)):
+                return drop(eight_bit.feedforward_checkpoint8(normalized_x, first, second))
             if (ops.BLOCK_LINEAR_ON_TCGEN05 and act.approximate == "none"
                     and ops.feedforward_supported(normalized_x, first, second)):
                 return drop(ops.feedforward(normalized_x, first, second))  # GELU fused into the GEMMs
