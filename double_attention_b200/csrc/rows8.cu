@@ -91,7 +91,7 @@ DA_DEV void row_scale(uint32_t amax_bits, float rstd, float& inv, float& scale) 
 }
 
 DA_DEV int quant(float v, float inv) {  // NaN converts to 0
-  return max(-127, min(127, __float2int_rn(v * inv)));
+  return max(-127, min(127, __float2int_rn(__fmul_rn(v, inv))));
 }
 
 // Eight values as four pairs.
@@ -321,10 +321,14 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
     }
   float inv, scale;
   row_scale(row_max<kT>(__float_as_uint(a) & 0x7fffffffu, red), kKind == kRms ? rstd : 1.f, inv, scale);
-  // |v inv| exceeds 127 by a rounding at most
-  auto bytes = [&](F2 lo, F2 hi) {
-    return low_bytes(add2(mul2(lo, dup(inv)), dup(kRoundAt)), add2(mul2(hi, dup(inv)), dup(kRoundAt)));
+  // |v inv| exceeds 127 by a rounding at most.  The product is rounded before the sum (a fused pair would round once,
+  // and an element in 1e5 would differ from the other variants' rint(v inv)).
+  auto whole = [&](F2 x) {
+    float lo, hi;
+    split(x, lo, hi);
+    return f2(__fadd_rn(__fmul_rn(lo, inv), kRoundAt), __fadd_rn(__fmul_rn(hi, inv), kRoundAt));
   };
+  auto bytes = [&](F2 lo, F2 hi) { return low_bytes(whole(lo), whole(hi)); };
   uint2* slots = moved + (kShift ? threadIdx.x / kT * kSlots : 0);
 #pragma unroll
   for (int c = 0; c < kNV; ++c) {

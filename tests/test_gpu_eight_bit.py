@@ -122,6 +122,18 @@ def test_int8_rows_do_not_depend_on_layout(d: int) -> None:
     assert torch.equal(same.values, one_row := same.values[:1].expand(5, d)) and one_row.shape == (5, d)
 
 
+@pytest.mark.parametrize("d", [512, 1501, 8190])
+def test_int8_rows_round_as_separate_operations_do(d: int) -> None:
+    """q = rint(v * (127 / max|v|)) with each operation rounded to fp32, in every variant and bit for bit."""
+    x = _randn(4000, d, seed=d)
+    norm = _norm("rms", d)
+    for rows, v in ((da.quantize_int8(x), x), (da.rmsnorm_int8(x, norm), x * norm.weight),
+                    (da.quantize_int8(F.pad(x, (1, 0))[:, 1:]), x)):
+        amax = v.abs().amax(1, keepdim=True)
+        q = torch.round(v * (torch.full_like(amax, 127.0) / amax))
+        assert torch.equal(rows.values.float(), q)
+
+
 def test_int8_rows_of_zeros_tiny_and_non_finite_rows() -> None:
     d = 520
     x = _randn(9, d, seed=5)
