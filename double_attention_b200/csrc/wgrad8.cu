@@ -35,7 +35,7 @@ constexpr int kThreads = 128 + kGroups * 128;  // warps 0, 3 dY; 1 MMA; 2 q; 4-1
 
 struct Params {
   const int8_t* e;
-  void* out;        // dW, or the partial sums [split, N, ldo]
+  void* out;        // dW, or the partial sums where the rows are split
   int64_t ldo;
   int rows, split_rows, N, K, splits, blocks;
   int vec;  // rows of `out` take 16-byte stores
@@ -83,9 +83,16 @@ DA_DEV uint32_t unit_pair(int e) {
   return __byte_perm(u, 0, 0x1010);
 }
 
-template <typename T, typename TO>
+// Partial sums lie as the threads hold them, a row each: [split][tile][CTA of the pair][4 columns][128 rows], so that a
+// warp stores 512 bytes at once (row-major, 16 bytes a row, the stores of a split took 4 us).
+DA_DEV float4* partial_at(void* base, int tiles, int split, int tile, int rank, int col4, int row) {
+  return static_cast<float4*>(base) + ((((int64_t)split * tiles + tile) * 2 + rank) * (kTile / 4) + col4) * 128 + row;
+}
+
+// kExpanded: X comes expanded from memory (tx is its map, not q's) and no warp converts.
+template <typename T, typename TO, bool kExpanded>
 __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constant__ CUtensorMap ty,
-                                                            const __grid_constant__ CUtensorMap tq, const Params p) {
+                                                            const __grid_constant__ CUtensorMap tx, const Params p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t y_full[kStages], x_full[kStages], empty[kStages], raw_full[kRawStages], raw_empty[kRawStages];
@@ -142,6 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
     // ---------------------------------------------------------------- dY producers (alternate stages)
     const int pi = warp == 0 ? 0 : 1;
     prefetch_tmap(&ty);
+    if (kExpanded) prefetch_tmap(&tx);
     bool ok = true;
     int it = 0, last = -1;
     for (int i = 0; ok && i < my_items; ++i) {
@@ -151,12 +159,17 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
         if ((it & 1) != pi) continue;
         const int s = it % kStages;
         if (!mbar_wait(&empty[s], ((it / kStages) & 1u) ^ 1u, ab, 81)) { ok = false; break; }
-        if (rank == 0) mbar_arrive_expect_tx(&y_full[s], 2 * kHalfTile);
+        if (rank == 0) mbar_arrive_expect_tx(&y_full[s], (kExpanded ? 4 : 2) * kHalfTile);
         const uint32_t bar = mapa_shared(smem_u32(&y_full[s]), 0);
         uint8_t* dst = smem + s * kHalfTile;
         const int x = n0 + rank * 128, y = t0 + t * kRows;
         tma_load_2d_pair(&ty, bar, dst, x, y);
         tma_load_2d_pair(&ty, bar, dst + kRows * 128, x + 64, y);
+        if constexpr (kExpanded) {
+          dst += kOffX;
+          tma_load_2d_pair(&tx, bar, dst, k0 + rank * 128, y);
+          tma_load_2d_pair(&tx, bar, dst + kRows * 128, k0 + rank * 128 + 64, y);
+        }
         last = it;
       }
     }
@@ -164,9 +177,9 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
     if (rank == 0 && !ok)
       for (int j = (last - kStages + 1 > 0 ? last - kStages + 1 : 0); j <= last; ++j)
         if ((j & 1) == pi) mbar_wait_drain(&y_full[j % kStages], (j / kStages) & 1u);
-  } else if (warp == 2 && lane == 0) {
+  } else if (!kExpanded && warp == 2 && lane == 0) {
     // ---------------------------------------------------------------- q producer
-    prefetch_tmap(&tq);
+    prefetch_tmap(&tx);
     bool ok = true;
     int it = 0;
     for (int i = 0; ok && i < my_items; ++i) {
@@ -176,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
         const int s = it % kRawStages;
         if (!mbar_wait(&raw_empty[s], ((it / kRawStages) & 1u) ^ 1u, ab, 82)) { ok = false; break; }
         mbar_arrive_expect_tx(&raw_full[s], kRaw);
-        tma_load_2d(&tq, &raw_full[s], smem + kOffRaw + s * kRaw, k0 + rank * 128, t0 + t * kRows);
+        tma_load_2d(&tx, &raw_full[s], smem + kOffRaw + s * kRaw, k0 + rank * 128, t0 + t * kRows);
       }
     }
     for (int j = (it - kRawStages > 0 ? it - kRawStages : 0); !ok && j < it; ++j)
@@ -193,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
         const int s = it % kStages, buf = chunk & 1;
         const uint32_t parity = (it / kStages) & 1u;
         if (t % kChunk == 0 && chunk >= 2 && !mbar_wait(&acc_empty[buf], ((chunk >> 1) - 1) & 1u, ab, 83)) { ok = false; break; }
-        if (!mbar_wait(&y_full[s], parity, ab, 84) || !mbar_wait(&x_full[s], parity, ab, 85)) { ok = false; break; }
+        if (!mbar_wait(&y_full[s], parity, ab, 84) || (!kExpanded && !mbar_wait(&x_full[s], parity, ab, 85))) { ok = false; break; }
         tc_fence_after();
         const uint32_t sy = smem_u32(smem + s * kHalfTile), sx = smem_u32(smem + kOffX + s * kHalfTile);
 #pragma unroll
@@ -213,9 +226,10 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
     // row (lane of its quadrant of TMEM) x 64 columns.
     const int group = warp / 4 - 1, quad = warp & 3, tid = threadIdx.x % 128;
     const int r = tid / 8, j = tid % 8;
-    // the 32 bytes it writes per row are chunks 2 (j % 4) and + 1 of 64-column block j / 4; block 1 goes through
-    // them in the other order, so that the 8 threads of a row touch all banks at once
-    const int swap = j / 4;
+    // the 32 bytes it writes per row are chunks 2 (j % 4) and + 1 of 64-column block j / 4.  Block 1 goes through them
+    // in the other order, so that the 8 threads of a row write to all banks at once, and so do odd rows, so that two
+    // rows read from all banks at once.
+    const int swap = (j / 4) ^ (r & 1);
     const uint32_t src_off = kOffRaw + r * 128 + j * 16 + 8 * swap;
     const uint32_t dst_off = kOffX + (j / 4) * (kRows * 128) + r * 128;
     const uint32_t c0 = ((2 * (j % 4) + swap) ^ (r & 7)) << 4, c1 = ((2 * (j % 4) + (swap ^ 1)) ^ (r & 7)) << 4;
@@ -263,11 +277,11 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
       };
       const int chunks = (nt + kChunk - 1) / kChunk;
       int t = (group - it % kGroups + kGroups) % kGroups;  // the group's first stage of this item
-      uint32_t e_next = exponents(t), e_after = exponents(t + kGroups);
+      uint32_t e_next = kExpanded ? 0 : exponents(t), e_after = kExpanded ? 0 : exponents(t + kGroups);
       for (int c = 0; ok && c < chunks; ++c) {
         const int t_end = min(nt, (c + 1) * kChunk);
 #pragma unroll 1
-        for (; t < t_end; t += kGroups) {
+        for (; !kExpanded && t < t_end; t += kGroups) {
           const uint32_t e4 = e_next;
           e_next = e_after;
           e_after = exponents(t + 2 * kGroups);
@@ -298,28 +312,35 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
       chunk += chunks;
       if (!ok) break;
       const int row = n0 + rank * 128 + quad * 32 + lane, col = k0 + group * 64;
-      if (row < p.N && col < p.K) {
-        TO* dst = static_cast<TO*>(p.out) + ((int64_t)z * p.N + row) * p.ldo + col;
-        if (p.vec && col + 64 <= p.K) {
-          if constexpr (std::is_same<TO, float>::value) {
+      if (row >= p.N || col >= p.K) continue;
+      if (p.splits > 1) {
+        float4* dst = partial_at(p.out, k_tiles * n_tiles, z, (pair + i * pairs) / p.splits, rank, group * 16,
+                                 quad * 32 + lane);
 #pragma unroll
-            for (int q = 0; q < 64; q += 4)
-              *reinterpret_cast<float4*>(dst + q) = make_float4(sum[q], sum[q + 1], sum[q + 2], sum[q + 3]);
-          } else {
+        for (int q = 0; q < 64; q += 4)
+          if (col + q < p.K) dst[q / 4 * 128] = make_float4(sum[q], sum[q + 1], sum[q + 2], sum[q + 3]);
+        continue;
+      }
+      TO* dst = static_cast<TO*>(p.out) + (int64_t)row * p.ldo + col;
+      if (p.vec && col + 64 <= p.K) {
+        if constexpr (std::is_same<TO, float>::value) {
 #pragma unroll
-            for (int q = 0; q < 64; q += 8)
-              *reinterpret_cast<uint4*>(dst + q) =
-                  make_uint4(pack2<TO>(sum[q], sum[q + 1]), pack2<TO>(sum[q + 2], sum[q + 3]),
-                             pack2<TO>(sum[q + 4], sum[q + 5]), pack2<TO>(sum[q + 6], sum[q + 7]));
-          }
+          for (int q = 0; q < 64; q += 4)
+            *reinterpret_cast<float4*>(dst + q) = make_float4(sum[q], sum[q + 1], sum[q + 2], sum[q + 3]);
         } else {
 #pragma unroll
-          for (int q = 0; q < 64; ++q)
-            if (col + q < p.K) {
-              if constexpr (std::is_same<TO, float>::value) dst[q] = sum[q];
-              else dst[q] = from_f32<TO>(sum[q]);
-            }
+          for (int q = 0; q < 64; q += 8)
+            *reinterpret_cast<uint4*>(dst + q) =
+                make_uint4(pack2<TO>(sum[q], sum[q + 1]), pack2<TO>(sum[q + 2], sum[q + 3]),
+                           pack2<TO>(sum[q + 4], sum[q + 5]), pack2<TO>(sum[q + 6], sum[q + 7]));
         }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 64; ++q)
+          if (col + q < p.K) {
+            if constexpr (std::is_same<TO, float>::value) dst[q] = sum[q];
+            else dst[q] = from_f32<TO>(sum[q]);
+          }
       }
     }
   }
@@ -329,38 +350,60 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
   if (warp == 1) tmem_dealloc<2>(tmem, 2 * kTile);
 }
 
-// dW = the splits' partial sums [split, N, pitch], added in split order, four columns per thread.
+// dW = the splits' partial sums.  A block takes 32 rows x 4 columns; its 8 warps add a range of the splits each, in
+// order, and the first adds the 8 sums in order.
 template <typename TO>
-__global__ void __launch_bounds__(256) reduce_kernel(const float* partial, int splits, int N, int K, int pitch,
-                                                     void* out, int64_t ldo) {
+__global__ void __launch_bounds__(256) reduce_kernel(const float* partial, int splits, int k_tiles, int n_tiles, int N,
+                                                     int K, TO* out, int64_t ldo) {
+  __shared__ float4 part[8][32];
   grid_dependency_wait();
   grid_launch_dependents();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int per_row = pitch / 4;
-  if (i >= (int64_t)N * per_row) return;
-  const int64_t row = i / per_row;
-  const int col = (int)(i % per_row) * 4;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int quad = blockIdx.x % 4, col4 = blockIdx.x / 4 % (kTile / 4), half = blockIdx.x / kTile;  // half = tile * 2 + rank
+  const int tile = half / 2, rank = half % 2;
+  const int row = tile / k_tiles * kTile + rank * 128 + quad * 32 + lane, col = tile % k_tiles * kTile + col4 * 4;
+  if (col >= K || tile / k_tiles * kTile + rank * 128 + quad * 32 >= N) return;  // the whole block
+  const int per = (splits + 7) / 8, z0 = warp * per, z1 = min(splits, z0 + per);
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int z = 0; z < splits; ++z) {
-    const float4 v = *reinterpret_cast<const float4*>(partial + ((int64_t)z * N + row) * pitch + col);
+  if (row < N) {
+    const float4* src = partial_at(const_cast<float*>(partial), k_tiles * n_tiles, 0, tile, rank, col4, quad * 32 + lane);
+    const int64_t step = (int64_t)k_tiles * n_tiles * (kTile * kTile / 4);
+#pragma unroll 5
+    for (int z = z0; z < z1; ++z) {
+      const float4 v = src[z * step];
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+  }
+  part[warp][lane] = s;
+  __syncthreads();
+  if (warp > 0 || row >= N) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) {
+    const float4 v = part[w][lane];
     s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
   }
-  TO* dst = static_cast<TO*>(out) + row * ldo + col;
+  TO* dst = out + row * ldo + col;
   const float v[4] = {s.x, s.y, s.z, s.w};
-  for (int q = 0; q < 4 && col + q < K; ++q) {
-    if constexpr (std::is_same<TO, float>::value) dst[q] = v[q];
-    else dst[q] = from_f32<TO>(v[q]);
+  if (col + 4 <= K && ldo % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+    if constexpr (std::is_same<TO, float>::value) *reinterpret_cast<float4*>(dst) = s;
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<TO>(s.x, s.y), pack2<TO>(s.z, s.w));
+  } else {
+    for (int q = 0; q < 4 && col + q < K; ++q) {
+      if constexpr (std::is_same<TO, float>::value) dst[q] = v[q];
+      else dst[q] = from_f32<TO>(v[q]);
+    }
   }
 }
 
 struct Plan {
   int splits;
   int64_t split_rows;
-  int pitch;  // row pitch of a partial sum
+  bool expanded;
+  int64_t x_elems, elems;  // workspace (fp32 elements): the expanded X, and with the partial sums behind it
 };
 // The rows are split while there are fewer tiles than CTA pairs; a split has at least 256 rows.
 Plan plan_for(int64_t rows, int64_t N, int64_t K) {
-  const int64_t tiles = ((N + kTile - 1) / kTile) * ((K + kTile - 1) / kTile);
+  const int64_t n_tiles = (N + kTile - 1) / kTile, tiles = n_tiles * ((K + kTile - 1) / kTile);
   int64_t s = (sm_count() / 2) / tiles;
   const int64_t most = (rows + 255) / 256;
   if (s > most) s = most;
@@ -368,17 +411,60 @@ Plan plan_for(int64_t rows, int64_t N, int64_t K) {
   Plan p;
   p.split_rows = (rows + s * kRows - 1) / (s * kRows) * kRows;
   p.splits = (int)((rows + p.split_rows - 1) / p.split_rows);
-  p.pitch = (int)((K + 3) / 4 * 4);
+  // Expanding X into memory first costs 3 bytes of traffic a value and saves every row of tiles its conversion.
+  // Measured (us, converting in the kernel against expanding first): 262144 rows, 1536 x 512 429 / 386 and
+  // 512 x 1536 423 / 498; 8192 rows, 4096 x 4096 343 / 243; 16384 rows, 640 x 2000 69 / 64.
+  p.expanded = N > 3 * kTile;
+  p.x_elems = p.expanded ? (rows * ((K + 31) / 32 * 16) + 63) / 64 * 64 : 0;
+  p.elems = p.x_elems + (p.splits > 1 ? p.splits * tiles * kTile * kTile : 0);
   return p;
 }
 
-template <typename T, typename TO>
-int launch(const CUtensorMap& ty, const CUtensorMap& tq, const Params& p, cudaStream_t st) {
-  constexpr auto kern = wgrad_kernel<T, TO>;
+template <typename T, typename TO, bool kExpanded>
+int launch(const CUtensorMap& ty, const CUtensorMap& tx, const Params& p, cudaStream_t st) {
+  constexpr auto kern = wgrad_kernel<T, TO, kExpanded>;
   if (int rc = allow_smem<kern>(kSmem + 1024)) return rc;
   const int64_t items = (int64_t)((p.N + kTile - 1) / kTile) * ((p.K + kTile - 1) / kTile) * p.splits;
   const int pairs = items < sm_count() / 2 ? (int)items : sm_count() / 2;
-  return launch_kernel(kern, dim3(2 * pairs), dim3(kThreads), kSmem + 1024, st, true, ty, tq, p);
+  return launch_kernel(kern, dim3(2 * pairs), dim3(kThreads), kSmem + 1024, st, true, ty, tx, p);
+}
+
+// The product of one 16-bit type, and the sum of the splits.
+template <typename T>
+int run(const void* dy, int64_t ldy, const int8_t* q, const int8_t* e, int64_t rows, int64_t N, int64_t K, void* out,
+        int out_dtype, int64_t ldo, float* workspace, const Plan& plan, int* status, cudaStream_t st) {
+  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const int64_t blocks = (K + 31) / 32;
+  const bool split = plan.splits > 1;
+  float* partial = workspace + plan.x_elems;
+  CUtensorMap ty, tx;
+  if (int rc = make_tmap_2d(&ty, dy, dt, 2, N, rows, (uint64_t)ldy * 2, 64, kRows)) return rc;
+  if (plan.expanded) {
+    if (int rc = da_checkpoint8_restore(q, e, rows, blocks * 32, workspace, bf16 ? DA_BF16 : DA_F16, blocks * 32, st))
+      return rc;
+    if (int rc = make_tmap_2d(&tx, workspace, dt, 2, blocks * 32, rows, blocks * 64, 64, kRows)) return rc;
+  } else {
+    if (int rc = make_tmap_2d(&tx, q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, blocks * 32, rows, blocks * 32, 128, kRows, false))
+      return rc;
+  }
+  const int vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ldo * (out_dtype == DA_F32 ? 4 : 2) % 16 == 0;
+  const Params p{e,      split ? partial : out, ldo,         (int)rows,   (int)plan.split_rows,
+                 (int)N, (int)K,                plan.splits, (int)blocks, vec,
+                 status};
+  int rc;
+  if (split || out_dtype == DA_F32)
+    rc = plan.expanded ? launch<T, float, true>(ty, tx, p, st) : launch<T, float, false>(ty, tx, p, st);
+  else
+    rc = plan.expanded ? launch<T, T, true>(ty, tx, p, st) : launch<T, T, false>(ty, tx, p, st);
+  if (rc || !split) return rc;
+  const int k_tiles = (int)((K + kTile - 1) / kTile), n_tiles = (int)((N + kTile - 1) / kTile);
+  const dim3 grid((unsigned)(k_tiles * n_tiles * 2 * kTile));
+  if (out_dtype == DA_F32)
+    return launch_kernel(reduce_kernel<float>, grid, dim3(256), 0, st, false, (const float*)partial, plan.splits, k_tiles,
+                         n_tiles, (int)N, (int)K, static_cast<float*>(out), ldo);
+  return launch_kernel(reduce_kernel<T>, grid, dim3(256), 0, st, false, (const float*)partial, plan.splits, k_tiles, n_tiles,
+                       (int)N, (int)K, static_cast<T*>(out), ldo);
 }
 
 }  // namespace wg8
@@ -386,8 +472,7 @@ int launch(const CUtensorMap& ty, const CUtensorMap& tq, const Params& p, cudaSt
 
 extern "C" int64_t da_checkpoint8_wgrad_workspace_elems(int64_t rows, int64_t N, int64_t K) {
   if (rows <= 0 || N <= 0 || K <= 0) return -1;
-  const da::wg8::Plan plan = da::wg8::plan_for(rows, N, K);
-  return plan.splits > 1 ? (int64_t)plan.splits * N * plan.pitch : 0;
+  return da::wg8::plan_for(rows, N, K).elems;
 }
 
 extern "C" int da_checkpoint8_wgrad(const void* dy, int dtype, int64_t ldy, const int8_t* q, const int8_t* e,
@@ -400,38 +485,10 @@ extern "C" int da_checkpoint8_wgrad(const void* dy, int dtype, int64_t ldy, cons
   if ((dtype != DA_F16 && dtype != DA_BF16) || (out_dtype != DA_F32 && out_dtype != dtype)) return DA_ERR_DTYPE;
   if (ldy % 8 || reinterpret_cast<uintptr_t>(dy) % 16 || reinterpret_cast<uintptr_t>(q) % 16) return DA_ERR_ALIGN;
   const wg8::Plan plan = wg8::plan_for(rows, N, K);
-  const bool split = plan.splits > 1;
-  if (split && (!workspace || workspace_elems < (int64_t)plan.splits * N * plan.pitch)) return DA_ERR_WORKSPACE;
-  if (split && reinterpret_cast<uintptr_t>(workspace) % 16) return DA_ERR_ALIGN;
+  if (plan.elems && (!workspace || workspace_elems < plan.elems)) return DA_ERR_WORKSPACE;
+  if (plan.elems && reinterpret_cast<uintptr_t>(workspace) % 256) return DA_ERR_ALIGN;
   if (int rc = bind_device(dy)) return rc;
-  const int64_t blocks = (K + 31) / 32;
-  const bool bf16 = dtype == DA_BF16;
-  CUtensorMap ty, tq;
-  if (int rc = make_tmap_2d(&ty, dy, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, N, rows,
-                            (uint64_t)ldy * 2, 64, wg8::kRows))
-    return rc;
-  if (int rc = make_tmap_2d(&tq, q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, blocks * 32, rows, blocks * 32, 128, wg8::kRows, false))
-    return rc;
-  const int64_t pitch = split ? plan.pitch : ldo;
-  const int vec = split || (reinterpret_cast<uintptr_t>(out) % 16 == 0 && ldo * (out_dtype == DA_F32 ? 4 : 2) % 16 == 0);
-  const wg8::Params p{e,      split ? workspace : out, pitch,       (int)rows,   (int)plan.split_rows,
-                      (int)N, (int)K,                  plan.splits, (int)blocks, vec,
-                      status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int rc;
-  if (split || out_dtype == DA_F32)
-    rc = bf16 ? wg8::launch<__nv_bfloat16, float>(ty, tq, p, st) : wg8::launch<__half, float>(ty, tq, p, st);
-  else
-    rc = bf16 ? wg8::launch<__nv_bfloat16, __nv_bfloat16>(ty, tq, p, st) : wg8::launch<__half, __half>(ty, tq, p, st);
-  if (rc || !split) return rc;
-  const dim3 grid((unsigned)((N * (plan.pitch / 4) + 255) / 256));
-  const float* part = workspace;
-  if (out_dtype == DA_F32)
-    return launch_kernel(wg8::reduce_kernel<float>, grid, dim3(256), 0, st, false, part, plan.splits, (int)N, (int)K,
-                         plan.pitch, out, ldo);
-  if (bf16)
-    return launch_kernel(wg8::reduce_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, false, part, plan.splits, (int)N,
-                         (int)K, plan.pitch, out, ldo);
-  return launch_kernel(wg8::reduce_kernel<__half>, grid, dim3(256), 0, st, false, part, plan.splits, (int)N, (int)K,
-                       plan.pitch, out, ldo);
+  return dtype == DA_BF16 ? wg8::run<__nv_bfloat16>(dy, ldy, q, e, rows, N, K, out, out_dtype, ldo, workspace, plan, status, st)
+                          : wg8::run<__half>(dy, ldy, q, e, rows, N, K, out, out_dtype, ldo, workspace, plan, status, st);
 }

@@ -25,7 +25,7 @@ import torch
 from torch import Tensor
 
 from . import _lib, ops
-from ._lib import call, ptr
+from ._lib import ptr
 
 BLOCK = 32          # columns of a checkpoint that share one exponent
 MAX_INNER = 131071  # K of an int8 product: 128 * 128 * K stays below 2^31
@@ -43,13 +43,21 @@ FEEDFORWARD_CHECKPOINT8 = False
 _CODES = {torch.float16: _lib.DA_F16, torch.bfloat16: _lib.DA_BF16, torch.float32: _lib.DA_F32}
 
 
+_entries: dict = {}  # bound entry points by name
+
+
 def _launch(device: int, name: str, *args) -> None:
     """One library call on the current stream of CUDA device ``device``, whichever device is current."""
+    entry = _entries.get(name)
+    if entry is None:
+        entry = _entries[name] = getattr(_lib.lib(), name)
     if device == torch._C._cuda_getDevice():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+        status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+            status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        _lib.check(name, status)
 
 
 def _new(shape, dtype: torch.dtype, device: torch.device) -> Tensor:
@@ -111,8 +119,8 @@ def _rows16(t: Tensor, elements: int) -> tuple[Tensor, int, int]:
     """As :func:`_rows`, every row on 16 bytes (``elements`` of them): as it lies, or copied to padded rows."""
     t, rows, stride = _rows(t)
     d = t.shape[-1]
-    if t.data_ptr() % 16 == 0:
-        if stride % elements == 0 and stride >= d:
+    if not t.data_ptr() % 16:
+        if not stride % elements and stride >= d:
             return t, rows, stride
         if rows == 1:  # has no stride of its own
             return t, rows, _round_up(d, elements)
