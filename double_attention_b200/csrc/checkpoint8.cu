@@ -13,8 +13,9 @@
 // Layout: q [rows, ceil(D / 32) * 32] int8, columns past D zero; e [rows, ceil(D / 32)] int8.
 // Bound: HBM, whose writes run at 3.9 TB/s alone (a copy: 6.5 TB/s read and written).  A thread takes 8 columns,
 // so the 4 threads of a block find its maximum with two shuffles and no row-wide reduction is needed, whatever the
-// width.  Dense tensors whose width is a multiple of 32 run as one long row (kFlat); any other width, stride or
-// alignment finds its row by a multiplication and checks its columns.
+// width.  Dense tensors whose width is a multiple of 32 run as one long row; the others find their row by a
+// multiplication, and where the rows start off 16-byte words the values are moved between registers rather than
+// loaded and stored one by one (kDense: GELU backward of 50000 x 1001 in 172 us, one by one in 263; restoring 49 and 140).
 #include "common.cuh"
 #include "host_util.h"
 #include "vec8.cuh"
@@ -31,12 +32,16 @@ struct CkptArgs {
   void* dz;
   int8_t* q;
   int8_t* e;
-  int64_t ldx, ldh, lddz, row0;
+  int64_t ldx, ldh, lddz, row0, rows;
   int64_t items;  // groups of 8 columns in this launch (below 2^31 unless flat)
   Div31 per_row;  // groups of 8 columns in a row of q (a multiple of 4)
   int D, gelu, e_min, e_max;
   int vec_x, vec_h, vec_dz;  // 16-byte rows
 };
+
+// How a tensor's rows lie: one long row; dense rows of any width, whose groups of 8 columns start anywhere in a 16-byte
+// word; or anything.
+enum : int { kFlat = 0, kDense = 1, kAny = 2 };
 
 // Eight 16-bit values of a row, those past D as 0.
 template <typename T>
@@ -53,15 +58,63 @@ DA_DEV uint4 load_row8(const void* p, int64_t base, int col, int D, bool vec) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <typename T>
-DA_DEV void store_row8(void* p, int64_t base, int col, int D, bool vec, const F2* v) {
+DA_DEV void store_row8(void* p, int64_t base, int col, int D, bool vec, uint4 v) {
   T* dst = static_cast<T*>(p) + base + col;
-  const uint32_t w[4] = {narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]), narrow<T>(v[3])};
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   if (vec && col + 8 <= D) {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(dst) = v;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (col + i < D) reinterpret_cast<uint16_t*>(dst)[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+  }
+}
+
+// The same of a dense tensor: the two aligned 16-byte words that hold the values, moved together.
+DA_DEV uint4 load_dense8(const void* p, int64_t flat, int64_t total, int col, int D) {
+  const uint16_t* src = static_cast<const uint16_t*>(p);
+  const int m = (int)(flat & 7);
+  if (flat - m + 16 > total) return load_row8<uint16_t>(p, flat - col, col, D, false);  // the tensor's last values
+  const uint4 a = *reinterpret_cast<const uint4*>(src + flat - m);
+  const uint4 b = m ? *reinterpret_cast<const uint4*>(src + flat - m + 8) : a;
+  uint4 v = shift16(a, b, m);
+  if (col + 8 > D) {  // the next row's values
+    uint32_t* w = &v.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int left = D - col - 2 * i;
+      w[i] = left >= 2 ? w[i] : left == 1 ? w[i] & 0xffffu : 0;
+    }
+  }
+  return v;
+}
+// Stores 8 values of a row at `flat`: each aligned 16-byte word by the lane whose values end in it, with the values
+// before them from the lane below; what has no such neighbour in this warp and row goes value by value.  Every lane
+// of the warp calls it.
+DA_DEV void store_dense8(void* p, int64_t flat, int col, int D, bool live, uint4 v) {
+  const int lane = threadIdx.x & 31, m = (int)(flat & 7);
+  uint4 below;
+  below.x = __shfl_up_sync(0xffffffffu, v.x, 1);
+  below.y = __shfl_up_sync(0xffffffffu, v.y, 1);
+  below.z = __shfl_up_sync(0xffffffffu, v.z, 1);
+  below.w = __shfl_up_sync(0xffffffffu, v.w, 1);
+  if (!live) return;
+  uint16_t* dst = static_cast<uint16_t*>(p) + flat;
+  const bool before = lane > 0 && col > 0, after = lane < 31 && col + 8 < D;
+  const uint4 w = m ? shift16(below, v, 8 - m) : v;  // columns col - m .. + 8
+  if ((before || m == 0) && col - m + 8 <= D) {
+    *reinterpret_cast<uint4*>(dst - m) = w;
+  } else {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if ((before || i >= m) && col - m + i < D) dst[i - m] = (uint16_t)(u[i / 2] >> (i % 2 * 16));
+  }
+  if (!after) {  // nobody above takes the last m values
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 1; i < 8; ++i)
+      if (i >= 8 - m && col + i < D) dst[i] = (uint16_t)(u[i / 2] >> (i % 2 * 16));
   }
 }
 
@@ -72,26 +125,35 @@ struct Place {  // of a group of 8 columns
   int64_t row, group;
   int col;
 };
-template <bool kFlat>
+template <int kLies>
 DA_DEV Place place_of(const CkptArgs& p, int64_t i) {
-  if constexpr (kFlat) return {0, i, 0};
+  if constexpr (kLies == kFlat) return {0, i, 0};
   const uint32_t r = p.per_row.div((uint32_t)i), c = (uint32_t)i - r * p.per_row.d;
   return {p.row0 + r, (p.row0 + r) * p.per_row.d + c, (int)c * 8};
 }
-template <typename T, bool kFlat>
+template <typename T, int kLies>
 DA_DEV uint4 load_place(const CkptArgs& p, const Place& at) {
-  if constexpr (kFlat) return __ldcs(reinterpret_cast<const uint4*>(p.x) + at.group);
+  if constexpr (kLies == kFlat) return __ldcs(reinterpret_cast<const uint4*>(p.x) + at.group);
+  if constexpr (kLies == kDense) {
+    if (at.col >= p.D) return make_uint4(0, 0, 0, 0);
+    return load_dense8(p.x, at.row * p.D + at.col, p.rows * p.D, at.col, p.D);
+  }
   return load_row8<T>(p.x, at.row * p.ldx, at.col, p.D, p.vec_x);
 }
-template <typename T, bool kFlat>
-DA_DEV void store_place(const CkptArgs& p, void* out, int64_t ld, int vec, const Place& at, const F2* v) {
-  if constexpr (kFlat)
-    reinterpret_cast<uint4*>(out)[at.group] = make_uint4(narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]), narrow<T>(v[3]));
-  else
-    store_row8<T>(out, at.row * ld, at.col, p.D, vec, v);
+// (kDense: called by every lane)
+template <typename T, int kLies>
+DA_DEV void store_place(const CkptArgs& p, void* out, int64_t ld, int vec, const Place& at, bool live, const F2* v) {
+  const uint4 w = make_uint4(narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]), narrow<T>(v[3]));
+  if constexpr (kLies == kFlat) {
+    if (live) reinterpret_cast<uint4*>(out)[at.group] = w;
+  } else if constexpr (kLies == kDense) {
+    store_dense8(out, at.row * p.D + at.col, at.col, p.D, live && at.col < p.D, w);
+  } else {
+    if (live) store_row8<T>(out, at.row * ld, at.col, p.D, vec, w);
+  }
 }
 
-template <typename T, bool kFlat>
+template <typename T, int kLies>
 __global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
@@ -101,8 +163,8 @@ __global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p) {
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     raw[k] = make_uint4(0, 0, 0, 0);
-    at[k] = place_of<kFlat>(p, first + k * 256);
-    if (first + k * 256 < p.items) raw[k] = load_place<T, kFlat>(p, at[k]);
+    at[k] = place_of<kLies>(p, first + k * 256);
+    if (first + k * 256 < p.items) raw[k] = load_place<T, kLies>(p, at[k]);
   }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
@@ -140,11 +202,11 @@ __global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p) {
     if (first + k * 256 < p.items) {
       *reinterpret_cast<uint2*>(p.q + at[k].group * 8) = q;
       if ((at[k].group & 3) == 0) p.e[at[k].group >> 2] = (int8_t)(finite ? e : kNotFinite);
-      if (p.gelu) {
+    }
+    if (p.gelu) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = gelu2(v[j]);
-        store_place<T, kFlat>(p, p.h, p.ldh, p.vec_h, at[k], v);
-      }
+      for (int j = 0; j < 4; ++j) v[j] = gelu2(v[j]);
+      store_place<T, kLies>(p, p.h, p.ldh, p.vec_h, at[k], first + k * 256 < p.items, v);
     }
   }
 }
@@ -158,17 +220,17 @@ DA_DEV void restore8(uint2 q, int e, F2* v) {
   for (int j = 0; j < 4; ++j) v[j] = mul2(v[j], unit);
 }
 
-template <typename T, bool kFlat>
+template <typename T, int kLies>
 __global__ void __launch_bounds__(256) checkpoint8_restore_kernel(const CkptArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int64_t first = (int64_t)blockIdx.x * (256 * kItems) + threadIdx.x;
-  uint2 q[kItems];
-  int e[kItems];
+  uint2 q[kItems] = {};
+  int e[kItems] = {};
   Place at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    at[k] = place_of<kFlat>(p, first + k * 256);
+    at[k] = place_of<kLies>(p, first + k * 256);
     if (first + k * 256 < p.items) {
       q[k] = *reinterpret_cast<const uint2*>(p.q + at[k].group * 8);
       e[k] = p.e[at[k].group >> 2];
@@ -176,89 +238,94 @@ __global__ void __launch_bounds__(256) checkpoint8_restore_kernel(const CkptArgs
   }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    if (first + k * 256 >= p.items) continue;
+    const bool live = first + k * 256 < p.items;
+    if (kLies != kDense && !live) continue;
     F2 v[4];
     restore8(q[k], e[k], v);
     if constexpr (std::is_same<T, float>::value) {
-      float* dst = static_cast<float*>(p.h) + at[k].row * p.ldh + (kFlat ? at[k].group * 8 : at[k].col);
+      if (!live) continue;
+      constexpr bool flat = kLies == kFlat;
+      float* dst = static_cast<float*>(p.h) + at[k].row * p.ldh + (flat ? at[k].group * 8 : at[k].col);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float lo, hi;
         split(v[j], lo, hi);
-        if (kFlat || at[k].col + 2 * j < p.D) dst[2 * j] = lo;
-        if (kFlat || at[k].col + 2 * j + 1 < p.D) dst[2 * j + 1] = hi;
+        if (flat || at[k].col + 2 * j < p.D) dst[2 * j] = lo;
+        if (flat || at[k].col + 2 * j + 1 < p.D) dst[2 * j + 1] = hi;
       }
     } else {
-      store_place<T, kFlat>(p, p.h, p.ldh, p.vec_h, at[k], v);
+      store_place<T, kLies>(p, p.h, p.ldh, p.vec_h, at[k], live, v);
     }
   }
 }
 
-template <typename T, bool kFlat>
+template <typename T, int kLies>
 __global__ void __launch_bounds__(256) checkpoint8_gelu_bwd_kernel(const CkptArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int64_t first = (int64_t)blockIdx.x * (256 * kItems) + threadIdx.x;
-  uint4 raw[kItems];
-  uint2 q[kItems];
-  int e[kItems];
+  uint4 raw[kItems] = {};
+  uint2 q[kItems] = {};
+  int e[kItems] = {};
   Place at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    at[k] = place_of<kFlat>(p, first + k * 256);
+    at[k] = place_of<kLies>(p, first + k * 256);
     if (first + k * 256 < p.items) {
-      raw[k] = load_place<T, kFlat>(p, at[k]);
+      raw[k] = load_place<T, kLies>(p, at[k]);
       q[k] = *reinterpret_cast<const uint2*>(p.q + at[k].group * 8);
       e[k] = p.e[at[k].group >> 2];
     }
   }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    if (first + k * 256 >= p.items || (!kFlat && at[k].col >= p.D)) continue;
+    const bool live = first + k * 256 < p.items;
+    if (kLies != kDense && !live) continue;
     F2 z[4], d[4] = {widen<T>(raw[k].x), widen<T>(raw[k].y), widen<T>(raw[k].z), widen<T>(raw[k].w)};
     restore8(q[k], e[k], z);
 #pragma unroll
     for (int j = 0; j < 4; ++j) d[j] = mul2(d[j], gelu_grad2(z[j]));
-    store_place<T, kFlat>(p, p.dz, p.lddz, p.vec_dz, at[k], d);
-    if (p.h) store_place<T, kFlat>(p, p.h, p.ldh, p.vec_h, at[k], z);
+    store_place<T, kLies>(p, p.dz, p.lddz, p.vec_dz, at[k], live, d);
+    if (p.h) store_place<T, kLies>(p, p.h, p.ldh, p.vec_h, at[k], live, z);
   }
 }
 
 // Runs the kernel over all groups: at once where the tensors are one long row, else over slabs of rows whose items
 // stay below 2^31.
-template <typename T, template <typename, bool> class Kernel>
-int run(CkptArgs p, int64_t rows, bool flat, cudaStream_t st) {
+template <typename T, template <typename, int> class Kernel>
+int run(CkptArgs p, int64_t rows, int lies, cudaStream_t st) {
   const int64_t per_block = 256 * kItems;
-  if (flat && rows * p.per_row.d / per_block < 0x7fffffffLL) {
+  auto grid = [&] { return dim3((unsigned)((p.items + per_block - 1) / per_block)); };
+  p.rows = rows;
+  if (lies == kFlat && rows * p.per_row.d / per_block < 0x7fffffffLL) {
     p.items = rows * p.per_row.d;
-    return launch_kernel(Kernel<T, true>::get(), dim3((unsigned)((p.items + per_block - 1) / per_block)), dim3(256), 0, st,
-                         false, p);
+    return launch_kernel(Kernel<T, kFlat>::get(), grid(), dim3(256), 0, st, false, p);
   }
   const int64_t slab = Div31::kMax / p.per_row.d;
   for (int64_t r0 = 0; r0 < rows; r0 += slab) {
     p.row0 = r0;
     p.items = (rows - r0 < slab ? rows - r0 : slab) * (int64_t)p.per_row.d;
-    if (int rc = launch_kernel(Kernel<T, false>::get(), dim3((unsigned)((p.items + per_block - 1) / per_block)), dim3(256),
-                               0, st, false, p))
-      return rc;
+    const int rc = lies == kDense ? launch_kernel(Kernel<T, kDense>::get(), grid(), dim3(256), 0, st, false, p)
+                                  : launch_kernel(Kernel<T, kAny>::get(), grid(), dim3(256), 0, st, false, p);
+    if (rc) return rc;
   }
   return DA_OK;
 }
-template <typename T, bool kFlat>
+template <typename T, int kLies>
 struct Forward {
-  static auto get() { return checkpoint8_kernel<T, kFlat>; }
+  static auto get() { return checkpoint8_kernel<T, kLies>; }
 };
-template <typename T, bool kFlat>
+template <typename T, int kLies>
 struct Restore {
-  static auto get() { return checkpoint8_restore_kernel<T, kFlat>; }
+  static auto get() { return checkpoint8_restore_kernel<T, kLies>; }
 };
-template <typename T, bool kFlat>
+template <typename T, int kLies>
 struct GeluBackward {
-  static auto get() { return checkpoint8_gelu_bwd_kernel<T, kFlat>; }
+  static auto get() { return checkpoint8_gelu_bwd_kernel<T, kLies>; }
 };
 
 CkptArgs make_args(int64_t D, int dtype, const int8_t* q, const int8_t* e) {
-  CkptArgs p{nullptr, nullptr, nullptr, const_cast<int8_t*>(q), const_cast<int8_t*>(e), 0, 0, 0, 0, 0,
+  CkptArgs p{nullptr, nullptr, nullptr, const_cast<int8_t*>(q), const_cast<int8_t*>(e), 0, 0, 0, 0, 0, 0,
              Div31((uint32_t)((D + 31) / 32 * 4)), (int)D, 0, -126, 121, 0, 0, 0};
   if (dtype == DA_F16) {
     p.e_min = -24;
@@ -266,8 +333,14 @@ CkptArgs make_args(int64_t D, int dtype, const int8_t* q, const int8_t* e) {
   }
   return p;
 }
-// Rows that follow one another without a gap and fill their blocks, on 16 bytes.
-bool dense(const void* p, int64_t ld, int64_t D) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld == D && D % 32 == 0; }
+// How a tensor lies, and the common way of two (absent tensors lie flat).  Rows on 16 bytes whose width is a multiple of
+// 8 need no moving: kAny, with its vector accesses.
+int lies_of(const void* p, int64_t ld, int64_t D) {
+  if (!p) return kFlat;
+  if (reinterpret_cast<uintptr_t>(p) % 16 || ld != D) return kAny;
+  return D % 32 == 0 ? kFlat : D % 8 == 0 ? kAny : kDense;
+}
+int common(int a, int b) { return a > b ? a : b; }
 bool bad_shape(int64_t rows, int64_t D) { return rows <= 0 || D <= 0 || D > 0x7fffff00LL; }
 bool half_dtype(int d) { return d == DA_F16 || d == DA_BF16; }
 
@@ -290,9 +363,9 @@ extern "C" int da_checkpoint8(const void* x, int dtype, int64_t ldx, int64_t row
   p.gelu = gelu;
   p.vec_x = vec8_ok(x, dtype, ldx);
   p.vec_h = vec8_ok(h, dtype, ldh);
-  const bool flat = dense(x, ldx, D) && (!gelu || dense(h, ldh, D));
+  const int lies = common(lies_of(x, ldx, D), gelu ? lies_of(h, ldh, D) : kFlat);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == DA_BF16 ? run<__nv_bfloat16, Forward>(p, rows, flat, st) : run<__half, Forward>(p, rows, flat, st);
+  return dtype == DA_BF16 ? run<__nv_bfloat16, Forward>(p, rows, lies, st) : run<__half, Forward>(p, rows, lies, st);
 }
 
 extern "C" int da_checkpoint8_restore(const int8_t* q, const int8_t* e, int64_t rows, int64_t D, void* out, int dtype,
@@ -307,10 +380,10 @@ extern "C" int da_checkpoint8_restore(const int8_t* q, const int8_t* e, int64_t 
   p.h = out;
   p.ldh = ldo;
   p.vec_h = vec8_ok(out, dtype, ldo);
-  const bool flat = dense(out, ldo, D);
+  const int lies = lies_of(out, ldo, D);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == DA_F32) return run<float, Restore>(p, rows, flat, st);
-  return dtype == DA_BF16 ? run<__nv_bfloat16, Restore>(p, rows, flat, st) : run<__half, Restore>(p, rows, flat, st);
+  if (dtype == DA_F32) return run<float, Restore>(p, rows, lies == kDense ? kAny : lies, st);
+  return dtype == DA_BF16 ? run<__nv_bfloat16, Restore>(p, rows, lies, st) : run<__half, Restore>(p, rows, lies, st);
 }
 
 extern "C" int da_checkpoint8_gelu_bwd(const void* dh, int dtype, int64_t lddh, const int8_t* q, const int8_t* e,
@@ -332,8 +405,8 @@ extern "C" int da_checkpoint8_gelu_bwd(const void* dh, int dtype, int64_t lddh, 
   p.vec_x = vec8_ok(dh, dtype, lddh);
   p.vec_dz = vec8_ok(dz, dtype, lddz);
   p.vec_h = vec8_ok(h, dtype, ldh);
-  const bool flat = dense(dh, lddh, D) && dense(dz, lddz, D) && (!h || dense(h, ldh, D));
+  const int lies = common(lies_of(dh, lddh, D), common(lies_of(dz, lddz, D), lies_of(h, ldh, D)));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == DA_BF16 ? run<__nv_bfloat16, GeluBackward>(p, rows, flat, st)
-                          : run<__half, GeluBackward>(p, rows, flat, st);
+  return dtype == DA_BF16 ? run<__nv_bfloat16, GeluBackward>(p, rows, lies, st)
+                          : run<__half, GeluBackward>(p, rows, lies, st);
 }

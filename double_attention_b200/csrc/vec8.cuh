@@ -96,6 +96,20 @@ DA_DEV uint32_t narrow(F2 x) {
   return pack2<T>(a, b);
 }
 
+// Eight 16-bit values from the m-th on (m in [0, 8]) of the sixteen in a, b.
+DA_DEV uint4 shift16(uint4 a, uint4 b, int m) {
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t u[6], v[5];
+#pragma unroll
+  for (int i = 0; i < 6; ++i) u[i] = m & 4 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) v[i] = m & 2 ? u[i + 1] : u[i];
+  if (m == 8) return b;
+  return m & 1 ? make_uint4(__funnelshift_r(v[0], v[1], 16), __funnelshift_r(v[1], v[2], 16),
+                            __funnelshift_r(v[2], v[3], 16), __funnelshift_r(v[3], v[4], 16))
+               : make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 // Integers by addition: for |v| < 2^22, v + kRoundAt rounds v to the nearest integer (ties to even), which the
 // low byte of the sum's bits holds in two's complement when it lies in [-128, 127].
 constexpr float kRoundAt = 12582912.f;  // 1.5 * 2^23
