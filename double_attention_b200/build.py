@@ -2,7 +2,9 @@
 
 Every ``csrc/*.cu`` file is compiled with nvcc for ``sm_100a`` and linked
 into one shared library exporting the C ABI declared in
-``include/da_b200.h``.  Object files go to ``_build/`` at the repository
+``include/da_b200.h``.  ``csrc/host/host_calls.cpp``, the host side of the
+eight-bit operators' calls, becomes the extension module ``_host_calls.so``
+beside it (the host compiler against this Python and PyTorch).  Object files go to ``_build/`` at the repository
 root; a file is recompiled only when it or a header changed.
 
 Usage: ``python -m double_attention_b200.build [--force] [-j N]``.
@@ -67,6 +69,35 @@ def _compile(nvcc: str, src: Path, obj: Path, verbose_ptxas: bool) -> tuple[Path
     return src, proc.stdout + proc.stderr
 
 
+HOST_SRC = CSRC / "host" / "host_calls.cpp"
+HOST_PATH = PACKAGE_DIR / "_host_calls.so"
+
+
+def build_host_calls(force: bool = False) -> Path:
+    """Compile the ``_host_calls`` extension module when its source, the ABI header or PyTorch changed."""
+    import sysconfig
+
+    import torch
+
+    include, root = sysconfig.get_paths()["include"], Path(torch.__file__).resolve().parent
+    newest = max(p.stat().st_mtime for p in (HOST_SRC, *INCLUDE.glob("*.h"), root / "version.py"))
+    if HOST_PATH.exists() and HOST_PATH.stat().st_mtime > newest and not force:
+        return HOST_PATH
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    system = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include", Path(include)]
+    tmp = HOST_PATH.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+           *(a for p in system for a in ("-isystem", str(p))), str(HOST_SRC), "-o", str(tmp), f"-L{root / 'lib'}",
+           "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", f"-L{PACKAGE_DIR}",
+           f"-l:{LIB_PATH.name}", "-Wl,-rpath,$ORIGIN"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"the host compiler failed for {HOST_SRC.name}:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, HOST_PATH)
+    return HOST_PATH
+
+
 def build(force: bool = False, jobs: int | None = None, verbose_ptxas: bool = False) -> Path:
     """Compile (incrementally) and link the library; returns its path."""
     nvcc = nvcc_path()
@@ -95,6 +126,7 @@ def build(force: bool = False, jobs: int | None = None, verbose_ptxas: bool = Fa
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
         os.replace(tmp, LIB_PATH)
+    build_host_calls(force)
     if verbose_ptxas and logs:
         print("\n".join(logs))
     return LIB_PATH

@@ -38,8 +38,25 @@ FEEDFORWARD_CHECKPOINT8 = False
 
 
 # ----------------------------------------------------------------------------- helpers
-# A call on a few rows is over on the device in 2 to 4 us, so the checks here read each attribute once and make no
-# views where the memory already lies as the kernel wants it.
+# A call on a few rows is over on the device in 2 to 4 us.  Tensors that lie as the kernels want them go through the
+# _host_calls extension, which checks, allocates and launches in 4 to 6 us on the host; it answers None for anything
+# else, and the functions here then copy, find the device or say what is wrong (10 to 15 us).
+_host_module = None
+
+
+def _host():
+    global _host_module
+    if _host_module is None:
+        _lib.lib()
+        try:
+            from . import _host_calls
+        except ImportError as error:
+            raise RuntimeError("_host_calls.so is not built; run `python -m double_attention_b200.build`") from error
+        _host_calls.set_check(_lib.check)
+        _host_module = _host_calls
+    return _host_module
+
+
 _CODES = {torch.float16: _lib.DA_F16, torch.bfloat16: _lib.DA_BF16, torch.float32: _lib.DA_F32}
 
 
@@ -144,15 +161,20 @@ class Int8Rows(NamedTuple):
     def dequantize(self, dtype: torch.dtype = torch.float32) -> Tensor:
         """The values the rows stand for, each rounded once to ``dtype``."""
         name = "Int8Rows.dequantize"
-        device = _check_rows(name, self)
-        if dtype not in _CODES:
+        code = _CODES.get(dtype)
+        if code is None:
             raise ValueError(f"{name} writes float32, bfloat16 or float16, got {dtype}")
+        if self.values.is_cuda:
+            out = _host().dequantize(self.values, self.scale, code)
+            if out is not None:
+                return out
+        device = _check_rows(name, self)
         out = _new(self.values.shape, dtype, self.values.device)
         if out.numel():
             q, rows, stride = _rows(self.values)
             d = q.shape[-1]
             _launch(device, "da_dequant_int8", q.data_ptr(), stride, self.scale.contiguous().data_ptr(), rows, d,
-                    out.data_ptr(), _CODES[dtype], d)
+                    out.data_ptr(), code, d)
         return out
 
 
@@ -173,6 +195,10 @@ _QUANTIZE, _RMS, _LAYER = 0, 1, 2
 
 def _norm_int8(name: str, x: Tensor, branch: Tensor | None, weight: Tensor | None, bias: Tensor | None, kind: int,
                eps: float) -> tuple[Tensor | None, Int8Rows]:
+    if x.is_cuda:
+        made = _host().norm(x, branch, weight, bias, kind, eps)
+        if made is not None:
+            return made[0], Int8Rows(made[1], made[2])
     device = _device_of(name, x, branch, weight, bias)
     shape = x.shape
     if not shape or not shape[-1]:
@@ -260,6 +286,14 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Tensor | None = None, *, ge
     The sum over K (at most 131071) is exact; it is scaled, biased and activated in fp32 and rounded once to
     ``dtype`` (bf16, fp16 or fp32).  x [..., K], weight [N, K], bias [N] in any float dtype."""
     name = "int8_linear"
+    code = _CODES.get(dtype)
+    if code is None:
+        raise ValueError(f"{name} writes float32, bfloat16 or float16, got {dtype}")
+    if x.values.is_cuda:
+        out = _host().linear(x.values, x.scale, weight.values, weight.scale, bias, gelu, code,
+                             ops.workspace(x.values.device).status)
+        if out is not None:
+            return out
     device = _check_rows(name, x)
     w_shape = weight.values.shape
     if _check_rows(name, weight) != device or len(w_shape) != 2:
@@ -268,9 +302,6 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Tensor | None = None, *, ge
     if x.values.shape[-1] != k or k > MAX_INNER or n < 1:
         raise ValueError(f"{name}: x {tuple(x.values.shape)} and weight {tuple(w_shape)} must share "
                          f"an inner size of 1 to {MAX_INNER}")
-    code = _CODES.get(dtype)
-    if code is None:
-        raise ValueError(f"{name} writes float32, bfloat16 or float16, got {dtype}")
     bias_ptr, bias_code = None, 0
     if bias is not None:
         bias_code = _float_code(name, "a bias", bias)
@@ -335,6 +366,10 @@ def _check_checkpoint(name: str, c: Checkpoint8) -> int:
 
 
 def _checkpoint8(name: str, x: Tensor, gelu: bool) -> tuple[Tensor | None, Checkpoint8]:
+    if x.is_cuda:
+        made = _host().checkpoint(x, gelu)
+        if made is not None:
+            return made[0], Checkpoint8(made[1], made[2], tuple(x.shape), x.dtype)
     device = _device_of(name, x)
     code = _half_code(name, "an activation", x)
     shape = x.shape
@@ -368,6 +403,10 @@ def gelu_checkpoint8_backward(dh: Tensor, kept: Checkpoint8) -> tuple[Tensor, Te
     """``(dh * GELU'(z), GELU(z))`` with z as kept: the gradient of GELU's input, and its output once more for
     the next layer's weight gradient."""
     name = "gelu_checkpoint8_backward"
+    if dh.is_cuda and dh.shape == kept.shape and dh.dtype == kept.dtype:
+        made = _host().gelu_backward(dh, kept.values, kept.exponent)
+        if made is not None:
+            return made
     device = _check_checkpoint(name, kept)
     if dh.shape != kept.shape or dh.dtype != kept.dtype or dh.get_device() != device:
         raise ValueError(f"{name}: dh {dh.dtype} {tuple(dh.shape)} on {dh.device} does not match the checkpoint "
@@ -388,12 +427,16 @@ def weight_grad_checkpoint8(dy: Tensor, kept: Checkpoint8, dtype: torch.dtype | 
     accumulated in fp32 in a fixed order (bit-reproducible) and stored in ``dtype`` (dy's, the default, or
     fp32)."""
     name = "weight_grad_checkpoint8"
+    shape, dtype = dy.shape, dtype or dy.dtype
+    if (shape[:-1] == kept.shape[:-1] and dy.dtype == kept.dtype and dtype in (torch.float32, dy.dtype) and dy.is_cuda):
+        made = _host().weight_grad(dy, kept.values, kept.exponent, kept.shape[-1], _CODES[dtype],
+                                   ops.workspace(dy.device).status)
+        if made is not None:
+            return made
     device = _check_checkpoint(name, kept)
-    shape = dy.shape
     if not shape or shape[:-1] != kept.shape[:-1] or not shape[-1] or dy.dtype != kept.dtype or dy.get_device() != device:
         raise ValueError(f"{name}: dy {dy.dtype} {tuple(shape)} on {dy.device} does not match the checkpoint "
                          f"{kept.dtype} {kept.shape} on {kept.values.device}")
-    dtype = dtype or dy.dtype
     if dtype != torch.float32 and dtype != dy.dtype:
         raise ValueError(f"{name} stores fp32 or dy's {dy.dtype}, got {dtype}")
     _inference_only(name, dy)

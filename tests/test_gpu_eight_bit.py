@@ -533,3 +533,84 @@ def test_feedforward_checkpoint8_gradients_and_memory() -> None:
     assert sum(kept) - weights < 0.33 * (sum(full) - weights)
     again = grads(da.feedforward_checkpoint8, [])[1]
     assert all(torch.equal(a, b) for a, b in zip(g8, again)), "two runs differ"
+
+
+# ----------------------------------------------------------------------------- capture, the other device side, long tensors
+def test_eight_bit_calls_replay_from_a_graph() -> None:
+    x, branch = _randn(33, 512, seed=1), _randn(33, 512, seed=2, dtype=BF16)
+    norm, w = _norm("rms", 512), da.quantize_int8(_randn(640, 512, seed=3))
+    dy = _randn(33, 128, seed=4, dtype=BF16)
+
+    def step():
+        x_out, rows = da.add_rmsnorm_int8(x, branch, norm)
+        h, kept = da.gelu_checkpoint8(da.int8_linear(rows, w))
+        dz, _ = da.gelu_checkpoint8_backward(h, kept)
+        return x_out, h, dz, da.weight_grad_checkpoint8(dy, kept)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (7, 8):
+        x.copy_(_randn(33, 512, seed=seed))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+def test_both_host_paths_give_the_same(monkeypatch) -> None:
+    """The extension's calls against the Python ones, which take what it leaves."""
+    class Nothing:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    def results():
+        x, branch = _randn(2, 9, 200, seed=1), _randn(2, 9, 200, seed=2, dtype=F16)
+        x_out, rows = da.add_layernorm_int8(x, branch, _norm("layer", 200))
+        bare = da.rmsnorm_int8(x, _norm("rms", 200, affine=False))
+        y = da.int8_linear(rows, da.quantize_int8(_randn(40, 200, seed=3)), _randn(40, seed=4), gelu=True, dtype=F16)
+        h, kept = da.gelu_checkpoint8(y)
+        dz, again = da.gelu_checkpoint8_backward(h, kept)
+        dw = da.weight_grad_checkpoint8(h, da.checkpoint8(x.half()), F32)
+        return [x_out, *rows, *bare, rows.dequantize(BF16), y, h, kept.values, kept.exponent, dz, again, dw]
+
+    fast = results()
+    monkeypatch.setattr(eight_bit, "_host_module", Nothing())
+    slow = results()
+    assert all(a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(fast, slow))
+
+
+def test_tensors_of_more_than_2_to_the_31_elements() -> None:
+    """Offsets past 32 bits: the last rows of tensors of 2.5e9 elements against the same rows alone."""
+    rows, d = 300_000, 8192
+    x = torch.empty(rows, d, dtype=BF16, device="cuda")
+    tail = _randn(500, d, seed=1, dtype=BF16)
+    x.zero_()[-500:] = tail
+    alone, got = da.quantize_int8(tail), da.quantize_int8(x)
+    assert torch.equal(got.values[-500:], alone.values) and torch.equal(got.scale[-500:], alone.scale)
+    assert torch.equal(got.dequantize(BF16)[-500:], alone.dequantize(BF16))
+    w = da.quantize_int8(_randn(300, d, seed=2))
+    assert torch.equal(da.int8_linear(got, w)[-500:], da.int8_linear(alone, w))
+    del got
+    h, kept = da.gelu_checkpoint8(x)
+    h1, kept1 = da.gelu_checkpoint8(tail)
+    assert torch.equal(h[-500:], h1) and torch.equal(kept.values[-500:], kept1.values)
+    assert torch.equal(kept.restore()[-500:], kept1.restore())
+    dz, _ = da.gelu_checkpoint8_backward(x, kept)
+    assert torch.equal(dz[-500:], da.gelu_checkpoint8_backward(tail, kept1)[0])
+    del h, dz
+    few = _randn(rows, 8, seed=3, dtype=BF16)
+    # x is zero in all other rows; the last 500 rows add in another order, in one split
+    dw, dw1 = da.weight_grad_checkpoint8(few, kept, F32), da.weight_grad_checkpoint8(few[-500:], kept1, F32)
+    size = few[-500:].float().abs().t() @ kept1.restore().float().abs()
+    assert (dw - dw1).abs().le(2.0**-23 * 100 * size).all()
+    back = da.weight_grad_checkpoint8(x, da.checkpoint8(few), F32)  # dy of 2.5e9 elements
+    ones = da.weight_grad_checkpoint8(tail, da.checkpoint8(few[-500:]), F32)
+    size = tail.float().abs().t() @ few[-500:].float().abs()
+    assert (back - ones).abs().le(2.0**-23 * 100 * size).all()
+    out = da.int8_linear(da.Int8Rows(torch.ones(rows, 16, dtype=torch.int8, device="cuda"), torch.ones(rows, device="cuda")),
+                         da.Int8Rows(torch.ones(d, 16, dtype=torch.int8, device="cuda"), torch.ones(d, device="cuda")))
+    assert out[-500:].eq(16).all() and out[:, -1].eq(16).all()
