@@ -11,7 +11,8 @@
 //   GELU backward from the kept z:  dz = dh gelu'(z),  h = gelu(z) once more, for the next layer's weight gradient.
 //
 // Layout: q [rows, ceil(D / 32) * 32] int8, columns past D zero; e [rows, ceil(D / 32)] int8.
-// Bound: HBM, whose writes run at 3.9 TB/s alone (a copy: 6.5 TB/s read and written).  A thread takes 8 columns,
+// Bound: HBM.  Measured at 262144 x 1536: forward with GELU 299 us (5 bytes an element, 6.7 TB/s), without 181, backward
+// 412 us (7 bytes, 6.8 TB/s), restore 179 us (6.7 TB/s).  A thread takes 8 columns,
 // so the 4 threads of a block find its maximum with two shuffles and no row-wide reduction is needed, whatever the
 // width.  Dense tensors whose width is a multiple of 32 run as one long row; the others find their row by a
 // multiplication, and where the rows start off 16-byte words the values are moved between registers rather than

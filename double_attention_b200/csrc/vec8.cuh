@@ -1,5 +1,5 @@
-// Eight consecutive elements of a row at a time, in any of the library's float types or in int8, and the
-// division that turns a flat item index into a row: shared by the kernels of the eight-bit operators.
+// Pieces that the kernels of the eight-bit operators share: the division that turns a flat item index into a row,
+// single values of any float type, packed fp32 pairs, bytes to and from fp32, and GELU.
 #pragma once
 
 #include "../../include/da_b200.h"

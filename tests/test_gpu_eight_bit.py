@@ -212,7 +212,7 @@ def _check_linear(x: da.Int8Rows, w: da.Int8Rows, bias, gelu: bool, dtype) -> No
 
 
 LINEAR_SHAPES = [(1, 1, 1), (1, 512, 1536), (1, 1536, 512), (2, 33, 5), (7, 100, 130), (16, 256, 256), (24, 4096, 512),
-                 (31, 1000, 765), (64, 512, 1000), (65, 130, 128), (100, 48, 300), (129, 2048, 257), (256, 512, 1536),
+                 (31, 1000, 765), (64, 512, 1000), (65, 130, 128), (5, 1100, 200), (40, 2250, 129), (100, 48, 300), (129, 2048, 257), (256, 512, 1536),
                  (300, 96, 1), (511, 1024, 520), (1000, 520, 1032), (2100, 512, 1536), (4097, 64, 768)]
 
 
