@@ -250,14 +250,28 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
             __syncwarp();
             const int cols = min(per_box, p.N - col0), rows = min(32, p.M - row0);
             const uint8_t* b = box;
-            for (int r = 0; r < rows; ++r)
-              for (int e = lane; e < cols; e += 32) {
-                const int64_t at = (int64_t)(row0 + r) * p.ldc + col0 + e;
-                if constexpr (kOut == DA_F32)
-                  static_cast<float*>(p.c)[at] = *reinterpret_cast<const float*>(b + sw128_offset(r, e / 4) + e % 4 * 4);
-                else
-                  static_cast<uint16_t*>(p.c)[at] = *reinterpret_cast<const uint16_t*>(b + sw128_offset(r, e / 8) + e % 8 * 2);
+            using E = typename std::conditional<kOut == DA_F32, float, uint16_t>::type;
+            E* dst = static_cast<E*>(p.c) + (int64_t)row0 * p.ldc + col0;
+            auto value = [&](int r, int e) {
+              return *reinterpret_cast<const E*>(b + sw128_offset(r, e * sizeof(E) / 16) + e * sizeof(E) % 16);
+            };
+            if (rows == 32 && cols == per_box) {  // 8 rows' reads before their writes
+#pragma unroll 1
+              for (int r0 = 0; r0 < 32; r0 += 8) {
+                E v[8][per_box / 32];
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+#pragma unroll
+                  for (int e = 0; e < per_box / 32; ++e) v[r][e] = value(r0 + r, lane + 32 * e);
+#pragma unroll
+                for (int r = 0; r < 8; ++r, dst += p.ldc)
+#pragma unroll
+                  for (int e = 0; e < per_box / 32; ++e) dst[lane + 32 * e] = v[r][e];
               }
+            } else {
+              for (int r = 0; r < rows; ++r, dst += p.ldc)
+                for (int e = lane; e < cols; e += 32) dst[e] = value(r, e);
+            }
             __syncwarp();
           }
         }
