@@ -40,9 +40,9 @@ struct CkptArgs {
   int vec_x, vec_h, vec_dz;  // 16-byte rows
 };
 
-// How a tensor's rows lie: one long row; dense rows of any width, whose groups of 8 columns start anywhere in a 16-byte
-// word; or anything.
-enum : int { kFlat = 0, kDense = 1, kAny = 2 };
+// How a tensor's rows lie: one long row; rows on 16-byte words whose width is a multiple of 8; dense rows of any other
+// width, whose groups of 8 columns start anywhere in a 16-byte word; or anything.
+enum : int { kFlat = 0, kVec = 1, kDense = 2, kAny = 3 };
 
 // Eight 16-bit values of a row, those past D as 0.
 template <typename T>
@@ -71,13 +71,21 @@ DA_DEV void store_row8(void* p, int64_t base, int col, int D, bool vec, uint4 v)
   }
 }
 
-// The same of a dense tensor: the two aligned 16-byte words that hold the values, moved together.
+// The same of a dense tensor: the two aligned 16-byte words that hold the values, moved together.  What only a row's ends
+// or the tensor's need stands in functions of its own, which the others branch around.
+__device__ __noinline__ uint4 load_last8(const uint16_t* src, int left) {  // `left` values, then zeros
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < left) w[i / 2] |= (uint32_t)src[i] << (i % 2 * 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 DA_DEV uint4 load_dense8(const void* p, int64_t flat, int64_t total, int col, int D) {
-  const uint16_t* src = static_cast<const uint16_t*>(p);
+  const uint16_t* src = static_cast<const uint16_t*>(p) + flat;
   const int m = (int)(flat & 7);
-  if (flat - m + 16 > total) return load_row8<uint16_t>(p, flat - col, col, D, false);  // the tensor's last values
-  const uint4 a = *reinterpret_cast<const uint4*>(src + flat - m);
-  const uint4 b = m ? *reinterpret_cast<const uint4*>(src + flat - m + 8) : a;
+  if (flat + 16 > total) return load_last8(src, D - col);
+  const uint4 a = *reinterpret_cast<const uint4*>(src - m);
+  const uint4 b = *reinterpret_cast<const uint4*>(src - m + 8);
   uint4 v = shift16(a, b, m);
   if (col + 8 > D) {  // the next row's values
     uint32_t* w = &v.x;
@@ -89,11 +97,17 @@ DA_DEV uint4 load_dense8(const void* p, int64_t flat, int64_t total, int col, in
   }
   return v;
 }
+__device__ __noinline__ void store_some(uint16_t* dst, uint4 v, int from, int to) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i >= from && i < to) dst[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+}
 // Stores 8 values of a row at `flat`: each aligned 16-byte word by the lane whose values end in it, with the values
-// before them from the lane below; what has no such neighbour in this warp and row goes value by value.  Every lane
-// of the warp calls it.
+// before them from the lane below; only a row's ends go value by value.  Every lane of the warp calls it, and the
+// first 4 hold the last groups of the warp before (see index_of).
 DA_DEV void store_dense8(void* p, int64_t flat, int col, int D, bool live, uint4 v) {
-  const int lane = threadIdx.x & 31, m = (int)(flat & 7);
+  const int m = (int)(flat & 7);
   uint4 below;
   below.x = __shfl_up_sync(0xffffffffu, v.x, 1);
   below.y = __shfl_up_sync(0xffffffffu, v.y, 1);
@@ -101,26 +115,30 @@ DA_DEV void store_dense8(void* p, int64_t flat, int col, int D, bool live, uint4
   below.w = __shfl_up_sync(0xffffffffu, v.w, 1);
   if (!live) return;
   uint16_t* dst = static_cast<uint16_t*>(p) + flat;
-  const bool before = lane > 0 && col > 0, after = lane < 31 && col + 8 < D;
-  const uint4 w = m ? shift16(below, v, 8 - m) : v;  // columns col - m .. + 8
-  if ((before || m == 0) && col - m + 8 <= D) {
-    *reinterpret_cast<uint4*>(dst - m) = w;
-  } else {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if ((before || i >= m) && col - m + i < D) dst[i - m] = (uint16_t)(u[i / 2] >> (i % 2 * 16));
-  }
-  if (!after) {  // nobody above takes the last m values
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 1; i < 8; ++i)
-      if (i >= 8 - m && col + i < D) dst[i] = (uint16_t)(u[i / 2] >> (i % 2 * 16));
-  }
+  const uint4 w = shift16(below, v, 8 - m);  // columns col - m .. + 8
+  if (col >= m && col - m + 8 <= D) *reinterpret_cast<uint4*>(dst - m) = w;
+  else store_some(dst - m, w, col > 0 ? 0 : m, min(8, D - col + m));
+  if (col + 8 >= D) store_some(dst, v, 8 - m, D - col);  // nobody above takes the last m values
 }
 
 // 2^e, e in [-126, 127].
 DA_DEV float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// The k-th group of a thread.  Dense rows: a warp takes 28 new groups, its first 4 lanes again the block before them
+// (without storing), whose values complete the first 16-byte word; so no word waits for another warp.
+constexpr int kNew = 28;
+template <int kLies>
+DA_DEV int64_t index_of(int k) {
+  if constexpr (kLies == kDense)
+    return (((int64_t)blockIdx.x * kItems + k) * 8 + threadIdx.x / 32) * kNew + (int)(threadIdx.x % 32) - (32 - kNew);
+  return ((int64_t)blockIdx.x * kItems + k) * 256 + threadIdx.x;
+}
+template <int kLies>
+DA_DEV bool loads(const CkptArgs& p, int64_t i) { return i < p.items && (kLies != kDense || i >= 0); }
+template <int kLies>
+DA_DEV bool stores(const CkptArgs& p, int64_t i) {
+  return i < p.items && (kLies != kDense || threadIdx.x % 32 >= 32 - kNew);
+}
 
 struct Place {  // of a group of 8 columns
   int64_t row, group;
@@ -135,6 +153,10 @@ DA_DEV Place place_of(const CkptArgs& p, int64_t i) {
 template <typename T, int kLies>
 DA_DEV uint4 load_place(const CkptArgs& p, const Place& at) {
   if constexpr (kLies == kFlat) return __ldcs(reinterpret_cast<const uint4*>(p.x) + at.group);
+  if constexpr (kLies == kVec) {
+    if (at.col >= p.D) return make_uint4(0, 0, 0, 0);
+    return __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + at.row * p.ldx + at.col));
+  }
   if constexpr (kLies == kDense) {
     if (at.col >= p.D) return make_uint4(0, 0, 0, 0);
     return load_dense8(p.x, at.row * p.D + at.col, p.rows * p.D, at.col, p.D);
@@ -147,6 +169,8 @@ DA_DEV void store_place(const CkptArgs& p, void* out, int64_t ld, int vec, const
   const uint4 w = make_uint4(narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]), narrow<T>(v[3]));
   if constexpr (kLies == kFlat) {
     if (live) reinterpret_cast<uint4*>(out)[at.group] = w;
+  } else if constexpr (kLies == kVec) {
+    if (live && at.col < p.D) *reinterpret_cast<uint4*>(static_cast<T*>(out) + at.row * ld + at.col) = w;
   } else if constexpr (kLies == kDense) {
     store_dense8(out, at.row * p.D + at.col, at.col, p.D, live && at.col < p.D, w);
   } else {
@@ -158,14 +182,13 @@ template <typename T, int kLies>
 __global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
-  const int64_t first = (int64_t)blockIdx.x * (256 * kItems) + threadIdx.x;
   uint4 raw[kItems];
   Place at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     raw[k] = make_uint4(0, 0, 0, 0);
-    at[k] = place_of<kLies>(p, first + k * 256);
-    if (first + k * 256 < p.items) raw[k] = load_place<T, kLies>(p, at[k]);
+    at[k] = place_of<kLies>(p, index_of<kLies>(k));
+    if (loads<kLies>(p, index_of<kLies>(k))) raw[k] = load_place<T, kLies>(p, at[k]);
   }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
@@ -200,14 +223,15 @@ __global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p) {
       }
       q = pack_s8x8(o);
     }
-    if (first + k * 256 < p.items) {
+    const bool live = stores<kLies>(p, index_of<kLies>(k));
+    if (live) {
       *reinterpret_cast<uint2*>(p.q + at[k].group * 8) = q;
       if ((at[k].group & 3) == 0) p.e[at[k].group >> 2] = (int8_t)(finite ? e : kNotFinite);
     }
     if (p.gelu) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = gelu2(v[j]);
-      store_place<T, kLies>(p, p.h, p.ldh, p.vec_h, at[k], first + k * 256 < p.items, v);
+      store_place<T, kLies>(p, p.h, p.ldh, p.vec_h, at[k], live, v);
     }
   }
 }
@@ -225,34 +249,37 @@ template <typename T, int kLies>
 __global__ void __launch_bounds__(256) checkpoint8_restore_kernel(const CkptArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
-  const int64_t first = (int64_t)blockIdx.x * (256 * kItems) + threadIdx.x;
   uint2 q[kItems] = {};
   int e[kItems] = {};
   Place at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    at[k] = place_of<kLies>(p, first + k * 256);
-    if (first + k * 256 < p.items) {
+    at[k] = place_of<kLies>(p, index_of<kLies>(k));
+    if (loads<kLies>(p, index_of<kLies>(k))) {
       q[k] = *reinterpret_cast<const uint2*>(p.q + at[k].group * 8);
       e[k] = p.e[at[k].group >> 2];
     }
   }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    const bool live = first + k * 256 < p.items;
+    const bool live = stores<kLies>(p, index_of<kLies>(k));
     if (kLies != kDense && !live) continue;
     F2 v[4];
     restore8(q[k], e[k], v);
     if constexpr (std::is_same<T, float>::value) {
       if (!live) continue;
-      constexpr bool flat = kLies == kFlat;
-      float* dst = static_cast<float*>(p.h) + at[k].row * p.ldh + (flat ? at[k].group * 8 : at[k].col);
+      float* dst = static_cast<float*>(p.h) + (kLies == kFlat ? at[k].group * 8 : at[k].row * p.ldh + at[k].col);
+      float f[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float lo, hi;
-        split(v[j], lo, hi);
-        if (flat || at[k].col + 2 * j < p.D) dst[2 * j] = lo;
-        if (flat || at[k].col + 2 * j + 1 < p.D) dst[2 * j + 1] = hi;
+      for (int j = 0; j < 4; ++j) split(v[j], f[2 * j], f[2 * j + 1]);
+      if constexpr (kLies == kFlat || kLies == kVec) {
+        if (kLies == kVec && at[k].col >= p.D) continue;
+        reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
+        reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (at[k].col + j < p.D) dst[j] = f[j];
       }
     } else {
       store_place<T, kLies>(p, p.h, p.ldh, p.vec_h, at[k], live, v);
@@ -264,15 +291,14 @@ template <typename T, int kLies>
 __global__ void __launch_bounds__(256) checkpoint8_gelu_bwd_kernel(const CkptArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
-  const int64_t first = (int64_t)blockIdx.x * (256 * kItems) + threadIdx.x;
   uint4 raw[kItems] = {};
   uint2 q[kItems] = {};
   int e[kItems] = {};
   Place at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    at[k] = place_of<kLies>(p, first + k * 256);
-    if (first + k * 256 < p.items) {
+    at[k] = place_of<kLies>(p, index_of<kLies>(k));
+    if (loads<kLies>(p, index_of<kLies>(k))) {
       raw[k] = load_place<T, kLies>(p, at[k]);
       q[k] = *reinterpret_cast<const uint2*>(p.q + at[k].group * 8);
       e[k] = p.e[at[k].group >> 2];
@@ -280,7 +306,7 @@ __global__ void __launch_bounds__(256) checkpoint8_gelu_bwd_kernel(const CkptArg
   }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    const bool live = first + k * 256 < p.items;
+    const bool live = stores<kLies>(p, index_of<kLies>(k));
     if (kLies != kDense && !live) continue;
     F2 z[4], d[4] = {widen<T>(raw[k].x), widen<T>(raw[k].y), widen<T>(raw[k].z), widen<T>(raw[k].w)};
     restore8(q[k], e[k], z);
@@ -295,9 +321,11 @@ __global__ void __launch_bounds__(256) checkpoint8_gelu_bwd_kernel(const CkptArg
 // stay below 2^31.
 template <typename T, template <typename, int> class Kernel>
 int run(CkptArgs p, int64_t rows, int lies, cudaStream_t st) {
-  const int64_t per_block = 256 * kItems;
-  auto grid = [&] { return dim3((unsigned)((p.items + per_block - 1) / per_block)); };
   p.rows = rows;
+  // a warp of kDense reads groups that another one stores: not where the result replaces the input
+  if (lies == kDense && p.x && (p.h == p.x || p.dz == p.x)) lies = kAny;
+  const int64_t per_block = (lies == kDense ? 8 * kNew : 256) * kItems;
+  auto grid = [&] { return dim3((unsigned)((p.items + per_block - 1) / per_block)); };
   if (lies == kFlat && rows * p.per_row.d / per_block < 0x7fffffffLL) {
     p.items = rows * p.per_row.d;
     return launch_kernel(Kernel<T, kFlat>::get(), grid(), dim3(256), 0, st, false, p);
@@ -306,8 +334,9 @@ int run(CkptArgs p, int64_t rows, int lies, cudaStream_t st) {
   for (int64_t r0 = 0; r0 < rows; r0 += slab) {
     p.row0 = r0;
     p.items = (rows - r0 < slab ? rows - r0 : slab) * (int64_t)p.per_row.d;
-    const int rc = lies == kDense ? launch_kernel(Kernel<T, kDense>::get(), grid(), dim3(256), 0, st, false, p)
-                                  : launch_kernel(Kernel<T, kAny>::get(), grid(), dim3(256), 0, st, false, p);
+    const int rc = lies == kVec     ? launch_kernel(Kernel<T, kVec>::get(), grid(), dim3(256), 0, st, false, p)
+                   : lies == kDense ? launch_kernel(Kernel<T, kDense>::get(), grid(), dim3(256), 0, st, false, p)
+                                    : launch_kernel(Kernel<T, kAny>::get(), grid(), dim3(256), 0, st, false, p);
     if (rc) return rc;
   }
   return DA_OK;
@@ -334,12 +363,13 @@ CkptArgs make_args(int64_t D, int dtype, const int8_t* q, const int8_t* e) {
   }
   return p;
 }
-// How a tensor lies, and the common way of two (absent tensors lie flat).  Rows on 16 bytes whose width is a multiple of
-// 8 need no moving: kAny, with its vector accesses.
+// How a tensor lies, and the common way of two (absent tensors lie flat; kVec and kDense differ in D, so never meet).
 int lies_of(const void* p, int64_t ld, int64_t D) {
   if (!p) return kFlat;
-  if (reinterpret_cast<uintptr_t>(p) % 16 || ld != D) return kAny;
-  return D % 32 == 0 ? kFlat : D % 8 == 0 ? kAny : kDense;
+  if (reinterpret_cast<uintptr_t>(p) % 16) return kAny;
+  if (ld == D && D % 32 == 0) return kFlat;
+  if (D % 8 == 0) return ld % 8 == 0 ? kVec : kAny;
+  return ld == D ? kDense : kAny;
 }
 int common(int a, int b) { return a > b ? a : b; }
 bool bad_shape(int64_t rows, int64_t D) { return rows <= 0 || D <= 0 || D > 0x7fffff00LL; }

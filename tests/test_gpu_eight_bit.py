@@ -614,3 +614,44 @@ def test_tensors_of_more_than_2_to_the_31_elements() -> None:
     out = da.int8_linear(da.Int8Rows(torch.ones(rows, 16, dtype=torch.int8, device="cuda"), torch.ones(rows, device="cuda")),
                          da.Int8Rows(torch.ones(d, 16, dtype=torch.int8, device="cuda"), torch.ones(d, device="cuda")))
     assert out[-500:].eq(16).all() and out[:, -1].eq(16).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [8, 40, 1000, 1536])
+def test_checkpoint_layouts_give_the_same_bits(d: int, dtype) -> None:
+    """Rows on 16-byte words of a wider tensor, rows off them, and one row for all."""
+    rows = 67
+    z, dh = (2.5 * _randn(rows, d, seed=d)).to(dtype), _randn(rows, d, seed=d + 1, dtype=dtype)
+    h, kept = da.gelu_checkpoint8(z)
+    dz, again = da.gelu_checkpoint8_backward(dh, kept)
+    for left, right in ((8, 16), (8, 1), (3, 5)):
+        wide_z, wide_dh = (F.pad(t, (left, right))[:, left:-right] for t in (z, dh))
+        h1, kept1 = da.gelu_checkpoint8(wide_z)
+        assert torch.equal(h1, h) and torch.equal(kept1.values, kept.values) and torch.equal(kept1.exponent, kept.exponent)
+        dz1, again1 = da.gelu_checkpoint8_backward(wide_dh, kept)
+        assert torch.equal(dz1, dz) and torch.equal(again1, again)
+    h1, kept1 = da.gelu_checkpoint8(z[:1].expand(rows, d))
+    assert torch.equal(h1, h[:1].expand(rows, d)) and torch.equal(kept1.values, kept.values[:1].expand(rows, -1))
+
+
+@pytest.mark.parametrize("d", [1, 31, 33, 1000, 1001, 1024])
+def test_checkpoint_results_in_place_of_their_input(d: int) -> None:
+    """The C entries, with an output at the address of the input; and values restored to fp32."""
+    rows = 700
+    z, dh = (2.5 * _randn(rows, d, seed=d)).to(BF16), _randn(rows, d, seed=d + 1, dtype=BF16)
+    h, kept = da.gelu_checkpoint8(z)
+    dz, again = da.gelu_checkpoint8_backward(dh, kept)
+    q, e = torch.empty_like(kept.values), torch.empty_like(kept.exponent)
+    own, code = z.clone(), eight_bit._CODES[BF16]
+    eight_bit._launch(0, "da_checkpoint8", own.data_ptr(), code, d, rows, d, 1, own.data_ptr(), d, q.data_ptr(), e.data_ptr())
+    assert torch.equal(own, h) and torch.equal(q, kept.values) and torch.equal(e, kept.exponent)
+    kept_args = (q.data_ptr(), e.data_ptr(), rows, d)
+    for dz_in_place in (True, False):
+        own, other = dh.clone(), torch.empty_like(dh)
+        a, b = (own, other) if dz_in_place else (other, own)
+        eight_bit._launch(0, "da_checkpoint8_gelu_bwd", own.data_ptr(), code, d, *kept_args, a.data_ptr(), d, b.data_ptr(), d)
+        assert torch.equal(a, dz) and torch.equal(b, again)
+    for ld in (d, d + 3, (d + 7) // 8 * 8 + 8):
+        wide = torch.full((rows, ld), -7.0, device="cuda")
+        eight_bit._launch(0, "da_checkpoint8_restore", *kept_args, wide.data_ptr(), eight_bit._CODES[F32], ld)
+        assert torch.equal(wide[:, :d], kept.restore().float()) and wide[:, d:].eq(-7).all()
