@@ -15,8 +15,10 @@
 // 412 us (7 bytes, 6.8 TB/s), restore 179 us (6.7 TB/s).  A thread takes 8 columns,
 // so the 4 threads of a block find its maximum with two shuffles and no row-wide reduction is needed, whatever the
 // width.  Dense tensors whose width is a multiple of 32 run as one long row; the others find their row by a
-// multiplication, and where the rows start off 16-byte words the values are moved between registers rather than
-// loaded and stored one by one (kDense: GELU backward of 50000 x 1001 in 172 us, one by one in 263; restoring 49 and 140).
+// multiplication (kVec: 50000 x 1000 in 48 us forward and 72 backward; 1024 wide 40 and 56), and where the rows start off
+// 16-byte words the values are moved between registers rather than loaded and stored one by one (kDense: GELU backward
+// of 50000 x 1001 in 135 us, one by one in 263; restoring 39 and 140; forward 90).  What bounds those is instructions:
+// the shifts and the rows' places.
 #include "common.cuh"
 #include "host_util.h"
 #include "vec8.cuh"
@@ -33,7 +35,8 @@ struct CkptArgs {
   void* dz;
   int8_t* q;
   int8_t* e;
-  int64_t ldx, ldh, lddz, row0, rows;
+  int64_t ldx, ldh, lddz;
+  int64_t left;   // values of a dense tensor from this launch's first one on
   int64_t items;  // groups of 8 columns in this launch (below 2^31 unless flat)
   Div31 per_row;  // groups of 8 columns in a row of q (a multiple of 4)
   int D, gelu, e_min, e_max;
@@ -128,30 +131,35 @@ DA_DEV float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 // (without storing), whose values complete the first 16-byte word; so no word waits for another warp.
 constexpr int kNew = 28;
 template <int kLies>
-DA_DEV int64_t index_of(int k) {
+using Index = std::conditional_t<kLies == kFlat, int64_t, int>;
+template <int kLies>
+DA_DEV Index<kLies> index_of(int k) {
   if constexpr (kLies == kDense)
-    return (((int64_t)blockIdx.x * kItems + k) * 8 + threadIdx.x / 32) * kNew + (int)(threadIdx.x % 32) - (32 - kNew);
-  return ((int64_t)blockIdx.x * kItems + k) * 256 + threadIdx.x;
+    return (int)((blockIdx.x * kItems + k) * 8 + threadIdx.x / 32) * kNew + (int)(threadIdx.x % 32) - (32 - kNew);
+  return ((Index<kLies>)blockIdx.x * kItems + k) * 256 + threadIdx.x;
 }
 template <int kLies>
-DA_DEV bool loads(const CkptArgs& p, int64_t i) { return i < p.items && (kLies != kDense || i >= 0); }
+DA_DEV bool loads(const CkptArgs& p, Index<kLies> i) {
+  return i < (Index<kLies>)p.items && (kLies != kDense || i >= 0);
+}
 template <int kLies>
-DA_DEV bool stores(const CkptArgs& p, int64_t i) {
-  return i < p.items && (kLies != kDense || threadIdx.x % 32 >= 32 - kNew);
+DA_DEV bool stores(const CkptArgs& p, Index<kLies> i) {
+  return i < (Index<kLies>)p.items && (kLies != kDense || threadIdx.x % 32 >= 32 - kNew);
 }
 
+template <int kLies>
 struct Place {  // of a group of 8 columns
-  int64_t row, group;
-  int col;
+  Index<kLies> group;
+  int row, col;
 };
 template <int kLies>
-DA_DEV Place place_of(const CkptArgs& p, int64_t i) {
-  if constexpr (kLies == kFlat) return {0, i, 0};
+DA_DEV Place<kLies> place_of(const CkptArgs& p, Index<kLies> i) {
+  if constexpr (kLies == kFlat) return {i, 0, 0};
   const uint32_t r = p.per_row.div((uint32_t)i), c = (uint32_t)i - r * p.per_row.d;
-  return {p.row0 + r, (p.row0 + r) * p.per_row.d + c, (int)c * 8};
+  return {i, (int)r, (int)c * 8};
 }
 template <typename T, int kLies>
-DA_DEV uint4 load_place(const CkptArgs& p, const Place& at) {
+DA_DEV uint4 load_place(const CkptArgs& p, const Place<kLies>& at) {
   if constexpr (kLies == kFlat) return __ldcs(reinterpret_cast<const uint4*>(p.x) + at.group);
   if constexpr (kLies == kVec) {
     if (at.col >= p.D) return make_uint4(0, 0, 0, 0);
@@ -159,20 +167,20 @@ DA_DEV uint4 load_place(const CkptArgs& p, const Place& at) {
   }
   if constexpr (kLies == kDense) {
     if (at.col >= p.D) return make_uint4(0, 0, 0, 0);
-    return load_dense8(p.x, at.row * p.D + at.col, p.rows * p.D, at.col, p.D);
+    return load_dense8(p.x, (int64_t)at.row * p.D + at.col, p.left, at.col, p.D);
   }
   return load_row8<T>(p.x, at.row * p.ldx, at.col, p.D, p.vec_x);
 }
 // (kDense: called by every lane)
 template <typename T, int kLies>
-DA_DEV void store_place(const CkptArgs& p, void* out, int64_t ld, int vec, const Place& at, bool live, const F2* v) {
+DA_DEV void store_place(const CkptArgs& p, void* out, int64_t ld, int vec, const Place<kLies>& at, bool live, const F2* v) {
   const uint4 w = make_uint4(narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]), narrow<T>(v[3]));
   if constexpr (kLies == kFlat) {
     if (live) reinterpret_cast<uint4*>(out)[at.group] = w;
   } else if constexpr (kLies == kVec) {
     if (live && at.col < p.D) *reinterpret_cast<uint4*>(static_cast<T*>(out) + at.row * ld + at.col) = w;
   } else if constexpr (kLies == kDense) {
-    store_dense8(out, at.row * p.D + at.col, at.col, p.D, live && at.col < p.D, w);
+    store_dense8(out, (int64_t)at.row * p.D + at.col, at.col, p.D, live && at.col < p.D, w);
   } else {
     if (live) store_row8<T>(out, at.row * ld, at.col, p.D, vec, w);
   }
@@ -183,7 +191,7 @@ __global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
   uint4 raw[kItems];
-  Place at[kItems];
+  Place<kLies> at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     raw[k] = make_uint4(0, 0, 0, 0);
@@ -225,7 +233,7 @@ __global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p) {
     }
     const bool live = stores<kLies>(p, index_of<kLies>(k));
     if (live) {
-      *reinterpret_cast<uint2*>(p.q + at[k].group * 8) = q;
+      *reinterpret_cast<uint2*>(p.q + (int64_t)at[k].group * 8) = q;
       if ((at[k].group & 3) == 0) p.e[at[k].group >> 2] = (int8_t)(finite ? e : kNotFinite);
     }
     if (p.gelu) {
@@ -251,12 +259,12 @@ __global__ void __launch_bounds__(256) checkpoint8_restore_kernel(const CkptArgs
   grid_launch_dependents();
   uint2 q[kItems] = {};
   int e[kItems] = {};
-  Place at[kItems];
+  Place<kLies> at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     at[k] = place_of<kLies>(p, index_of<kLies>(k));
     if (loads<kLies>(p, index_of<kLies>(k))) {
-      q[k] = *reinterpret_cast<const uint2*>(p.q + at[k].group * 8);
+      q[k] = *reinterpret_cast<const uint2*>(p.q + (int64_t)at[k].group * 8);
       e[k] = p.e[at[k].group >> 2];
     }
   }
@@ -294,13 +302,13 @@ __global__ void __launch_bounds__(256) checkpoint8_gelu_bwd_kernel(const CkptArg
   uint4 raw[kItems] = {};
   uint2 q[kItems] = {};
   int e[kItems] = {};
-  Place at[kItems];
+  Place<kLies> at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     at[k] = place_of<kLies>(p, index_of<kLies>(k));
     if (loads<kLies>(p, index_of<kLies>(k))) {
       raw[k] = load_place<T, kLies>(p, at[k]);
-      q[k] = *reinterpret_cast<const uint2*>(p.q + at[k].group * 8);
+      q[k] = *reinterpret_cast<const uint2*>(p.q + (int64_t)at[k].group * 8);
       e[k] = p.e[at[k].group >> 2];
     }
   }
@@ -321,7 +329,6 @@ __global__ void __launch_bounds__(256) checkpoint8_gelu_bwd_kernel(const CkptArg
 // stay below 2^31.
 template <typename T, template <typename, int> class Kernel>
 int run(CkptArgs p, int64_t rows, int lies, cudaStream_t st) {
-  p.rows = rows;
   // a warp of kDense reads groups that another one stores: not where the result replaces the input
   if (lies == kDense && p.x && (p.h == p.x || p.dz == p.x)) lies = kAny;
   const int64_t per_block = (lies == kDense ? 8 * kNew : 256) * kItems;
@@ -330,13 +337,21 @@ int run(CkptArgs p, int64_t rows, int lies, cudaStream_t st) {
     p.items = rows * p.per_row.d;
     return launch_kernel(Kernel<T, kFlat>::get(), grid(), dim3(256), 0, st, false, p);
   }
-  const int64_t slab = Div31::kMax / p.per_row.d;
+  auto skip = [](auto* ptr, int64_t n) { return ptr ? ptr + n : ptr; };
+  const int64_t slab = (Div31::kMax - 2 * per_block) / p.per_row.d / 8 * 8;  // (a slab starts as aligned as its tensor)
   for (int64_t r0 = 0; r0 < rows; r0 += slab) {
-    p.row0 = r0;
-    p.items = (rows - r0 < slab ? rows - r0 : slab) * (int64_t)p.per_row.d;
-    const int rc = lies == kVec     ? launch_kernel(Kernel<T, kVec>::get(), grid(), dim3(256), 0, st, false, p)
-                   : lies == kDense ? launch_kernel(Kernel<T, kDense>::get(), grid(), dim3(256), 0, st, false, p)
-                                    : launch_kernel(Kernel<T, kAny>::get(), grid(), dim3(256), 0, st, false, p);
+    const int64_t n = rows - r0 < slab ? rows - r0 : slab;
+    CkptArgs s = p;
+    s.x = skip(static_cast<const T*>(p.x), r0 * p.ldx);
+    s.h = skip(static_cast<T*>(p.h), r0 * p.ldh);
+    s.dz = skip(static_cast<T*>(p.dz), r0 * p.lddz);
+    s.q += r0 * p.per_row.d * 8;
+    s.e += r0 * p.per_row.d / 4;
+    s.left = (rows - r0) * p.D;
+    s.items = p.items = n * p.per_row.d;
+    const int rc = lies == kVec     ? launch_kernel(Kernel<T, kVec>::get(), grid(), dim3(256), 0, st, false, s)
+                   : lies == kDense ? launch_kernel(Kernel<T, kDense>::get(), grid(), dim3(256), 0, st, false, s)
+                                    : launch_kernel(Kernel<T, kAny>::get(), grid(), dim3(256), 0, st, false, s);
     if (rc) return rc;
   }
   return DA_OK;
@@ -355,7 +370,7 @@ struct GeluBackward {
 };
 
 CkptArgs make_args(int64_t D, int dtype, const int8_t* q, const int8_t* e) {
-  CkptArgs p{nullptr, nullptr, nullptr, const_cast<int8_t*>(q), const_cast<int8_t*>(e), 0, 0, 0, 0, 0, 0,
+  CkptArgs p{nullptr, nullptr, nullptr, const_cast<int8_t*>(q), const_cast<int8_t*>(e), 0, 0, 0, 0, 0,
              Div31((uint32_t)((D + 31) / 32 * 4)), (int)D, 0, -126, 121, 0, 0, 0};
   if (dtype == DA_F16) {
     p.e_min = -24;
@@ -372,7 +387,7 @@ int lies_of(const void* p, int64_t ld, int64_t D) {
   return ld == D ? kDense : kAny;
 }
 int common(int a, int b) { return a > b ? a : b; }
-bool bad_shape(int64_t rows, int64_t D) { return rows <= 0 || D <= 0 || D > 0x7fffff00LL; }
+bool bad_shape(int64_t rows, int64_t D) { return rows <= 0 || D <= 0 || D > 0x7fff0000LL; }  // (8 rows of items stay below 2^31)
 bool half_dtype(int d) { return d == DA_F16 || d == DA_BF16; }
 
 }  // namespace

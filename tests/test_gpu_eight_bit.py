@@ -655,3 +655,20 @@ def test_checkpoint_results_in_place_of_their_input(d: int) -> None:
         wide = torch.full((rows, ld), -7.0, device="cuda")
         eight_bit._launch(0, "da_checkpoint8_restore", *kept_args, wide.data_ptr(), eight_bit._CODES[F32], ld)
         assert torch.equal(wide[:, :d], kept.restore().float()) and wide[:, d:].eq(-7).all()
+
+
+@pytest.mark.parametrize("d", [1, 8])
+def test_checkpoint_of_more_rows_than_one_launch_takes(d: int) -> None:
+    """A checkpoint pads rows to 32 columns: past 2^31 groups of 8, with offsets into it past 2^34."""
+    rows = 2**29 + 5000
+    ends = (2.5 * _randn(10_000, d, seed=d)).to(BF16)
+    z = torch.zeros(rows, d, dtype=BF16, device="cuda")
+    z[:10_000], z[-10_000:] = ends, ends
+    h, kept = da.gelu_checkpoint8(z)
+    h1, kept1 = da.gelu_checkpoint8(ends)
+    dz1, _ = da.gelu_checkpoint8_backward(ends, kept1)
+    back, back1 = kept.restore(), kept1.restore()
+    dz, _ = da.gelu_checkpoint8_backward(z, kept)
+    for part in (slice(None, 10_000), slice(-10_000, None)):
+        assert torch.equal(h[part], h1) and torch.equal(back[part], back1) and torch.equal(dz[part], dz1)
+        assert torch.equal(kept.values[part], kept1.values) and torch.equal(kept.exponent[part], kept1.exponent)
