@@ -21,7 +21,7 @@ struct Params {
   void* c;
   int64_t lda, ldb, ldc;
   int M, N, K, bias_dtype, c_dtype, gelu;
-  int alternate;  // the pair kernel's epilogue warps take turns
+  int turns;  // the pair kernel's epilogue warps take turns
   int tma_c;  // C's rows take TMA stores (16-byte aligned base and stride)
   int* status;
   Div31 per_group;  // the pair kernel: tiles in a group of 8 rows of tiles
@@ -41,30 +41,34 @@ DA_DEV float col_bias(const Params& p, int n) { return p.bias ? load1(p.bias, p.
 // Persistent CTA pairs: a pair computes 256 x 256 tiles (each CTA 128 rows of A and, of every K stage, half of
 // B's rows) with cta_group::2 kind::i8 instructions of 256 x 256 x 32; two int32 accumulators of 256 TMEM columns
 // each, so that the epilogue of one tile runs under the products of the next.
-// A stage holds 128 bytes of K (5 stages of 32 KB; 3 stages of 64 KB measured the same).
+// A stage holds 128 bytes of K (5 stages of 32 KB for long K; 3 stages of 64 KB measured the same; 4 leave room for the
+// columns' scales where K is short, and cost 2 % where it is long).
 //
 // Bound: long K by the tensor pipe (79 % active; a dependent instruction takes ~180 cycles, 136 at the nominal rate):
 // 8192 x 4096 x 4096 in 89 us, 3.1 POP/s, 16384 x 8192 x 8192 in 650 us, 3.4 POP/s.  Short K by the output: 32768 x 512 x
-// 1536 in 31 us, its 100 MB near the 3.4 to 3.9 TB/s at which HBM takes writes alone; with GELU 48 us, half of the issue
-// slots gone to the epilogue.
+// 1536 in 30 us, its 100 MB near the 3.4 to 3.9 TB/s at which HBM takes writes alone; with GELU 42.6 us, of which the
+// stores are not the bound (an earlier form at 47.4 us took 45.5 without them): the epilogue's 16 instructions a value
+// fill 59 % of the issue slots, and 4 warps a scheduler, which 96 registers allow, do not cover the waits in their chains.
+template <bool kTurns>  // of the epilogue warps: see the epilogue
 struct Pair {
   static constexpr int kTile = 256;  // rows and columns of a pair's tile
   static constexpr int kOperand = 128 * 128;
   static constexpr int kStageBytes = 2 * kOperand;
-  static constexpr int kStages = 5;
+  static constexpr int kStages = kTurns ? 5 : 4;
   static constexpr int kEpilogueWarps = 16;
-  static constexpr int kOff = kStages * kStageBytes;
-  static constexpr int kSmem = kOff + kEpilogueWarps * 4096  /* an output box per epilogue warp */;
+  static constexpr int kOff = kStages * kStageBytes;         // an output box per epilogue warp
+  static constexpr int kColumns = kOff + kEpilogueWarps * 4096;  // and the scales and biases of its columns
+  static constexpr int kSmem = kColumns + (kTurns ? 0 : kEpilogueWarps * 512);
   static constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // warps 0, 2 TMA; 1 MMA; 3 idle; then the epilogue
   static constexpr int kGroupM = 8;  // row tiles that run through the columns together (A and B stay in L2)
 };
 
-template <int kOut, bool kGelu>
-__global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __grid_constant__ CUtensorMap ta,
+template <int kOut, bool kGelu, bool kTurns>
+__global__ void __launch_bounds__(Pair<kTurns>::kThreads, 1) gemm_pair_kernel(const __grid_constant__ CUtensorMap ta,
                                                                               const __grid_constant__ CUtensorMap tb,
                                                                               const __grid_constant__ CUtensorMap tc,
                                                                               const Params p) {
-  using C = Pair;
+  using C = Pair<kTurns>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[C::kStages], empty[C::kStages], acc_full[2], acc_empty[2];
@@ -86,7 +90,7 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], p.alternate ? C::kEpilogueWarps : 2 * C::kEpilogueWarps);  // its epilogue warps in both CTAs
+      mbar_init(&acc_empty[b], kTurns ? C::kEpilogueWarps : 2 * C::kEpilogueWarps);  // its epilogue warps in both CTAs
     }
     fence_mbar_init();
   }
@@ -162,13 +166,40 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- epilogue.  All 16 warps take every tile, 32 rows
-    // x 64 columns each; or, alternating, 8 warps every second tile (and accumulator), 32 x 128 each, so that one
+    // x 64 columns each; or, in turns, 8 warps every second tile (and accumulator), 32 x 128 each, so that one
     // group's waits lie under the other's arithmetic.
-    const int quad = warp & 3, turn = p.alternate ? (warp - 4) / 8 : 0, turns = p.alternate ? 2 : 1;
-    const int part = p.alternate ? (warp - 4) / 4 & 1 : (warp - 4) / 4, width = 64 * turns;
+    constexpr int turns = kTurns ? 2 : 1, width = 64 * turns;
+    const int quad = warp & 3, turn = kTurns ? (warp - 4) / 8 : 0, part = kTurns ? (warp - 4) / 4 & 1 : (warp - 4) / 4;
     uint8_t* box = smem + C::kOff + (warp - 4) * 4096;
     const bool vec_cols = reinterpret_cast<uintptr_t>(p.sb) % 16 == 0 &&
                           (!p.bias || (p.bias_dtype == DA_F32 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0));
+    // Short K: a tile's scales and biases, fetched a tile ahead (a lane two columns) and read back from shared memory as
+    // (s, s, b, b), and its column steps unrolled.  Loading them where they are used waited at every step: 32768 x 512 x
+    // 1536 with GELU 48.7 us, now 46.9, unrolled 43.0; without 31.5, 29.9 and 29.6.
+    float4* columns = reinterpret_cast<float4*>(smem + C::kColumns) + (warp - 4) * 32;
+    float4 next = make_float4(0.f, 0.f, 0.f, 0.f);
+    float next_sa = 0.f;
+    const bool vec2 = reinterpret_cast<uintptr_t>(p.sb) % 8 == 0 &&
+                          (!p.bias || (p.bias_dtype == DA_F32 && reinterpret_cast<uintptr_t>(p.bias) % 8 == 0));
+    auto fetch = [&](int i) {
+      if (i >= my_tiles) return;
+      int m0, n0;
+      tile_mn(i, m0, n0);
+      const int row = m0 + rank * 128 + quad * 32 + lane;
+      next_sa = row < p.M ? p.sa[row] : 0.f;
+      if (kTurns) return;
+      const int n = n0 + part * width + lane * 2;
+      if (vec2 && n + 2 <= p.N) {
+        const float2 t = __ldg(reinterpret_cast<const float2*>(p.sb + n));
+        const float2 u = p.bias ? __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(p.bias) + n))
+                                : make_float2(0.f, 0.f);
+        next = make_float4(t.x, t.y, u.x, u.y);
+      } else {
+        if (n < p.N) next.x = p.sb[n], next.z = col_bias(p, n);
+        if (n + 1 < p.N) next.y = p.sb[n + 1], next.w = col_bias(p, n + 1);
+      }
+    };
+    fetch(turn);
     constexpr int kStep = 16;  // columns at a time: what GELU and its constants need stays in 96 registers
     constexpr int per_box = kOut == DA_F32 ? 32 : 64;  // columns in 128 bytes
     bool ok = true;
@@ -176,13 +207,19 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
       const int buf = i & 1;
       int m0, n0;
       tile_mn(i, m0, n0);
-      const int row0 = m0 + rank * 128 + quad * 32, row = row0 + lane;
-      const float sa = row < p.M ? p.sa[row] : 0.f;
+      const int row0 = m0 + rank * 128 + quad * 32;
+      const float sa = next_sa;
+      if constexpr (!kTurns) {
+        __syncwarp();
+        columns[lane] = next;
+        __syncwarp();
+      }
+      fetch(i + turns);
       if (ok) ok = mbar_wait(&acc_full[buf], (i >> 1) & 1u, ab, 74);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       if (ok) {
-#pragma unroll 1
+#pragma unroll (kTurns ? 1 : 4)
         for (int c = 0; c < width; c += kStep) {
           const int col = n0 + part * width + c;
           float v[kStep];
@@ -195,7 +232,13 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
           }
           if (col >= p.N || row0 >= p.M) continue;
           F2 y[kStep / 2];
-          if (vec_cols && col + kStep <= p.N) {
+          if constexpr (!kTurns) {
+#pragma unroll
+            for (int e = 0; e < kStep / 2; ++e) {
+              const float4 at = columns[c / 2 + e];
+              y[e] = finish2(v[2 * e], v[2 * e + 1], sa, f2(at.x, at.y), f2(at.z, at.w));
+            }
+          } else if (vec_cols && col + kStep <= p.N) {
 #pragma unroll
             for (int e = 0; e < kStep / 4; ++e) {
               const float4 s = __ldg(reinterpret_cast<const float4*>(p.sb + col) + e);
@@ -285,9 +328,9 @@ __global__ void __launch_bounds__(Pair::kThreads, 1) gemm_pair_kernel(const __gr
   if (warp == 1) tmem_dealloc<2>(tmem, 2 * C::kTile);
 }
 
-template <int kOut, bool kGelu>
+template <int kOut, bool kGelu, bool kTurns>
 int launch_pair(const Params& p, cudaStream_t st) {
-  using C = Pair;
+  using C = Pair<kTurns>;
   constexpr int elem = kOut == DA_F32 ? 4 : 2;
   CUtensorMap ta, tb, tc;
   if (int rc = make_tmap_2d(&ta, p.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K, p.M, p.lda, 128, 128)) return rc;
@@ -299,22 +342,17 @@ int launch_pair(const Params& p, cudaStream_t st) {
                                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if (int rc = make_tmap_2d(&tc, p.c, dt, elem, p.N, p.M, (uint64_t)p.ldc * elem, 128 / elem, 32)) return rc;
   }
-  constexpr auto kern = gemm_pair_kernel<kOut, kGelu>;
+  constexpr auto kern = gemm_pair_kernel<kOut, kGelu, kTurns>;
   if (int rc = allow_smem<kern>(C::kSmem + 1024)) return rc;
   const int64_t tiles = (int64_t)((p.M + C::kTile - 1) / C::kTile) * ((p.N + C::kTile - 1) / C::kTile);
   const int pairs = tiles < sm_count() / 2 ? (int)tiles : sm_count() / 2;
   return launch_kernel(kern, dim3(2 * pairs), dim3(C::kThreads), C::kSmem + 1024, st, true, ta, tb, tc, p);
 }
 
+template <int kOut>
 int dispatch_pair(const Params& p, cudaStream_t st) {
-  switch (p.c_dtype * 2 + (p.gelu ? 1 : 0)) {
-    case DA_F16 * 2: return launch_pair<DA_F16, false>(p, st);
-    case DA_F16 * 2 + 1: return launch_pair<DA_F16, true>(p, st);
-    case DA_BF16 * 2: return launch_pair<DA_BF16, false>(p, st);
-    case DA_BF16 * 2 + 1: return launch_pair<DA_BF16, true>(p, st);
-    case DA_F32 * 2: return launch_pair<DA_F32, false>(p, st);
-    default: return launch_pair<DA_F32, true>(p, st);
-  }
+  if (p.turns) return p.gelu ? launch_pair<kOut, true, true>(p, st) : launch_pair<kOut, false, true>(p, st);
+  return p.gelu ? launch_pair<kOut, true, false>(p, st) : launch_pair<kOut, false, false>(p, st);
 }
 
 // ----------------------------------------------------------------------------------------------- few tokens
@@ -522,7 +560,9 @@ int dispatch(const Params& p, cudaStream_t st) {
   const int tn = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
   const int64_t tiles = (int64_t)((p.N + 127) / 128) * ((p.M + tn - 1) / tn);
   const int sms = sm_count();
-  if (2 * tiles > sms && (p.M > 256 || tiles > sms)) return dispatch_pair(p, st);
+  if (2 * tiles > sms && (p.M > 256 || tiles > sms)) return p.c_dtype == DA_F16    ? dispatch_pair<DA_F16>(p, st)
+                                                                    : p.c_dtype == DA_BF16 ? dispatch_pair<DA_BF16>(p, st)
+                                                                                           : dispatch_pair<DA_F32>(p, st);
   // as many K ranges as fill the SMs, none shorter than 2 stages
   const int nk = (p.K + 127) / 128;
   int splits = 1;
@@ -554,12 +594,13 @@ extern "C" int da_gemm_i8(const int8_t* A, int64_t lda, const float* a_scale, co
   if (int rc = bind_device(A)) return rc;
   const int elem = c_dtype == DA_F32 ? 4 : 2;
   // A long K loop hides the wait of a turn for its next accumulator, a short one does not.  Measured (us, all warps on
-  // every tile against turns): 32768 x 512 x 1536 31.2 / 34.5, with GELU 47.7 / 50.9; 32768 x 1024 x 1536 47.3 / 46.3;
-  // 32768 x 2048 x 1536 80.8 / 76.8; 8192 x 4096 x 4096 91.8 / 89.3.
-  const int alternate = K >= 1536;
+  // every tile against turns): 32768 x 512 x 1536 29.9 / 36.0, with GELU 42.4 / 52.0; 32768 x 768 x 1536 39.2 / 41.1, 45.9
+  // / 56.2; 32768 x 1024 x 1536 49.2 / 46.8, 53.0 / 60.1; 32768 x 1536 x 1536 with GELU 72.5 / 71.7; 8192 x 4096 x 4096 93.8
+  // / 88.8.
+  const int turns = K >= (gelu ? 1536 : 1024);
   const int tma_c = reinterpret_cast<uintptr_t>(C) % 16 == 0 && ldc * elem % 16 == 0;
   const i8::Params p{A,      B,      a_scale, b_scale,    bias,    C,    lda,   ldb,   ldc,
-                     (int)M, (int)N, (int)K,  bias_dtype, c_dtype, gelu, alternate, tma_c, status,
+                     (int)M, (int)N, (int)K,  bias_dtype, c_dtype, gelu, turns, tma_c, status,
                      Div31((uint32_t)((N + 255) / 256 * 8))};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return i8::dispatch(p, st);

@@ -227,6 +227,22 @@ def test_int8_linear_matches_its_definition(rows: int, k: int, n: int) -> None:
     _check_linear(x, w, bias.to(BF16), False, BF16)
 
 
+@pytest.mark.parametrize(("rows", "k", "n"), [(20_011, 80, 1029), (15_000, 1030, 1288), (9_001, 1600, 1501)])
+def test_int8_linear_of_many_tiles(rows: int, k: int, n: int) -> None:
+    """Several output tiles for each pair of SMs, ragged at both edges, with scales and biases at odd addresses."""
+    w = da.quantize_int8(_randn(n, k, seed=1) * k**-0.5)
+    x = da.quantize_int8(_randn(rows, k, seed=2, dtype=BF16))
+    bias = _randn(n + 1, seed=3)
+    w_odd = da.Int8Rows(w.values, torch.cat((w.scale[:1], w.scale))[1:])
+    for gelu in (False, True):
+        _check_linear(x, w, bias[:-1], gelu, BF16)
+        _check_linear(x, w, None, gelu, F16)
+        _check_linear(x, w_odd, bias[1:], gelu, F32)
+        _check_linear(x, w_odd, bias[1:].to(F16), gelu, BF16)
+    alone = da.Int8Rows(x.values[-300:-44].contiguous(), x.scale[-300:-44].contiguous())
+    assert torch.equal(da.int8_linear(x, w, bias[:-1], gelu=True)[-300:-44], da.int8_linear(alone, w, bias[:-1], gelu=True))
+
+
 @pytest.mark.parametrize(("rows", "n"), [(2, 3), (40, 130), (300, 520)])
 def test_int8_linear_sums_exactly_at_the_largest_inner_size(rows: int, n: int) -> None:
     k = eight_bit.MAX_INNER
