@@ -245,17 +245,15 @@ PyObject* weight_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t nn = dy->sizes().back(), rows = dy->numel() / nn;
   if (!kept_ok(q, e, rows, k)) Py_RETURN_NONE;
   Tensor padded;  // rows on 16 bytes
-  int64_t ldy = nn;
-  if (nn % 8 || reinterpret_cast<uintptr_t>(dy->data_ptr()) % 16) {
-    ldy = (nn + 7) / 8 * 8;
-    padded = c.empty({rows, ldy}, dy->scalar_type());
-    at::slice(padded, 1, 0, nn).copy_(dy->view({rows, nn}));
+  if (nn % 8 == 0 && reinterpret_cast<uintptr_t>(dy->data_ptr()) % 16) {
+    padded = c.empty({rows, nn}, dy->scalar_type());
+    padded.copy_(dy->view({rows, nn}));
     dy = &padded;
   }
   Tensor dw = c.empty({nn, k}, type_of(out_code)), work;
   const int64_t elems = da_checkpoint8_wgrad_workspace_elems(rows, nn, k);
   if (elems > 0) work = c.empty({elems}, at::kFloat);
-  const int status = da_checkpoint8_wgrad(dy->data_ptr(), code(dy), ldy, static_cast<const int8_t*>(q->data_ptr()),
+  const int status = da_checkpoint8_wgrad(dy->data_ptr(), code(dy), nn, static_cast<const int8_t*>(q->data_ptr()),
                                           static_cast<const int8_t*>(e->data_ptr()), rows, nn, k, dw.data_ptr(),
                                           (int)out_code, k, elems > 0 ? static_cast<float*>(work.data_ptr()) : nullptr,
                                           elems, static_cast<int*>(word->data_ptr()), c.stream());

@@ -442,9 +442,11 @@ def weight_grad_checkpoint8(dy: Tensor, kept: Checkpoint8, dtype: torch.dtype | 
     _inference_only(name, dy)
     n, k = shape[-1], kept.shape[-1]
     out = _new((n, k), dtype, dy.device)
-    d2, rows, ldd = _rows16(dy, 8)
+    d2, rows, ldd = _rows16(dy, 8) if n % 8 == 0 else _rows(dy)
     if not rows:
         return out.zero_()
+    if ldd < n:  # (one row, or rows that share their values)
+        d2, ldd = d2.contiguous(), n
     elems = _lib.lib().da_checkpoint8_wgrad_workspace_elems(rows, n, k)
     work = _new((elems,), torch.float32, dy.device) if elems else None
     _launch(device, "da_checkpoint8_wgrad", d2.data_ptr(), _CODES[dy.dtype], ldd, kept.values.data_ptr(),

@@ -531,11 +531,12 @@ DA_API int da_checkpoint8_gelu_bwd(const void* dh, int dtype, int64_t lddh, cons
                                    void* stream);
 /* Weight gradient from the checkpoint of the layer's input: out[n, k] = sum over the
  * rows of dy[t, n] * q[t, k] 2^e[t, k / 32], accumulated in fp32 and stored in fp32 or
- * dy's dtype; dy [rows, N] 16-byte aligned with ldy a multiple of 8.  `workspace` (fp32,
- * da_checkpoint8_wgrad_workspace_elems elements, 256-byte aligned; null where the query
- * returns 0; else DA_ERR_WORKSPACE) holds the layer's input in dtype where many output
- * columns read it (N above 768), and the partial sums where the rows are split over CTAs;
- * they are added in a fixed order: bit-reproducible. */
+ * dy's dtype; dy [rows, N] 16-byte aligned with ldy a multiple of 8 where N is one, else
+ * with any rows.  `workspace` (fp32, da_checkpoint8_wgrad_workspace_elems elements,
+ * 256-byte aligned; null where the query returns 0; else DA_ERR_WORKSPACE) holds the
+ * layer's input in dtype where many output columns read it (N above 768), dy on 16-byte
+ * rows where N is no multiple of 8, and the partial sums where the rows are split over
+ * CTAs; they are added in a fixed order: bit-reproducible. */
 DA_API int64_t da_checkpoint8_wgrad_workspace_elems(int64_t rows, int64_t N, int64_t K);
 DA_API int da_checkpoint8_wgrad(const void* dy, int dtype, int64_t ldy, const int8_t* q, const int8_t* e,
                                 int64_t rows, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,

@@ -441,6 +441,25 @@ def test_weight_grad_from_a_checkpoint(rows: int, n: int, k: int, dtype) -> None
     assert torch.equal(da.weight_grad_checkpoint8(moved, kept, F32), da.weight_grad_checkpoint8(dy, kept, F32))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize(("rows", "n", "k"), [(1, 9, 40), (2, 1, 33), (77, 129, 64), (700, 1001, 130), (6000, 777, 520)])
+def test_weight_grad_of_odd_widths_in_any_layout(rows: int, n: int, k: int, dtype) -> None:
+    """dY off 16-byte rows, at any address: the bits of the same dY laid out on them."""
+    dy, kept = _randn(rows, n, seed=2, dtype=dtype), da.checkpoint8(_randn(rows, k, seed=1, dtype=dtype))
+    want = da.weight_grad_checkpoint8(F.pad(dy, (0, -n % 8))[:, :n], kept, F32)
+    xk = kept.restore().double()
+    allowed = 2.0**-23 * (rows / 16 + 64) * (dy.double().abs().t() @ xk.abs()) + 2.0**-150
+    assert (want.double() - dy.double().t() @ xk).abs().le(1.01 * 2.0**-24 * want.double().abs() + allowed).all()
+    flat = torch.full((rows * (n + 5) + 16,), math.nan, dtype=dtype, device="cuda")
+    for off, ld in ((0, n), (1, n), (7, n), (3, n + 5), (0, n + 3)):
+        moved = flat[off:].as_strided((rows, n), (ld, 1))
+        flat.fill_(math.nan)
+        moved.copy_(dy)
+        assert torch.equal(da.weight_grad_checkpoint8(moved, kept, F32), want)
+    one = dy[:1].expand(rows, n)
+    assert torch.equal(da.weight_grad_checkpoint8(one, kept, F32), da.weight_grad_checkpoint8(one.contiguous(), kept, F32))
+
+
 def test_weight_grad_of_no_rows_and_of_bad_blocks() -> None:
     kept = da.checkpoint8(torch.empty(0, 64, dtype=BF16, device="cuda"))
     dw = da.weight_grad_checkpoint8(torch.empty(0, 16, dtype=BF16, device="cuda"), kept)
