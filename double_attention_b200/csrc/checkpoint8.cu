@@ -15,10 +15,9 @@
 // 412 us (7 bytes, 6.8 TB/s), restore 179 us (6.7 TB/s).  A thread takes 8 columns,
 // so the 4 threads of a block find its maximum with two shuffles and no row-wide reduction is needed, whatever the
 // width.  Dense tensors whose width is a multiple of 32 run as one long row; the others find their row by a
-// multiplication (kVec: 50000 x 1000 in 48 us forward and 72 backward; 1024 wide 40 and 56), and where the rows start off
-// 16-byte words the values are moved between registers rather than loaded and stored one by one (kDense: GELU backward
-// of 50000 x 1001 in 135 us, one by one in 263; restoring 39 and 140; forward 90).  What bounds those is instructions:
-// the shifts and the rows' places.
+// multiplication.  Rows on 16-byte words (kVec): 50000 x 1000 in 48 us forward, 58 backward, 25 restored (1024 wide 41, 55
+// and 25).  Dense rows that start anywhere in one go through shared memory (kDense): 50000 x 1001 in 61, 88 and 30 us,
+// bound by instructions and shared memory (a value at a time backward took 263, restoring 140).
 #include "common.cuh"
 #include "host_util.h"
 #include "vec8.cuh"
@@ -74,79 +73,15 @@ DA_DEV void store_row8(void* p, int64_t base, int col, int D, bool vec, uint4 v)
   }
 }
 
-// The same of a dense tensor: the two aligned 16-byte words that hold the values, moved together.  What only a row's ends
-// or the tensor's need stands in functions of its own, which the others branch around.
-__device__ __noinline__ uint4 load_last8(const uint16_t* src, int left) {  // `left` values, then zeros
-  uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < left) w[i / 2] |= (uint32_t)src[i] << (i % 2 * 16);
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-DA_DEV uint4 load_dense8(const void* p, int64_t flat, int64_t total, int col, int D) {
-  const uint16_t* src = static_cast<const uint16_t*>(p) + flat;
-  const int m = (int)(flat & 7);
-  if (flat + 16 > total) return load_last8(src, D - col);
-  const uint4 a = *reinterpret_cast<const uint4*>(src - m);
-  const uint4 b = *reinterpret_cast<const uint4*>(src - m + 8);
-  uint4 v = shift16(a, b, m);
-  if (col + 8 > D) {  // the next row's values
-    uint32_t* w = &v.x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int left = D - col - 2 * i;
-      w[i] = left >= 2 ? w[i] : left == 1 ? w[i] & 0xffffu : 0;
-    }
-  }
-  return v;
-}
-__device__ __noinline__ void store_some(uint16_t* dst, uint4 v, int from, int to) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i >= from && i < to) dst[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
-}
-// Stores 8 values of a row at `flat`: each aligned 16-byte word by the lane whose values end in it, with the values
-// before them from the lane below; only a row's ends go value by value.  Every lane of the warp calls it, and the
-// first 4 hold the last groups of the warp before (see index_of).
-DA_DEV void store_dense8(void* p, int64_t flat, int col, int D, bool live, uint4 v) {
-  const int m = (int)(flat & 7);
-  uint4 below;
-  below.x = __shfl_up_sync(0xffffffffu, v.x, 1);
-  below.y = __shfl_up_sync(0xffffffffu, v.y, 1);
-  below.z = __shfl_up_sync(0xffffffffu, v.z, 1);
-  below.w = __shfl_up_sync(0xffffffffu, v.w, 1);
-  if (!live) return;
-  uint16_t* dst = static_cast<uint16_t*>(p) + flat;
-  const uint4 w = shift16(below, v, 8 - m);  // columns col - m .. + 8
-  if (col >= m && col - m + 8 <= D) *reinterpret_cast<uint4*>(dst - m) = w;
-  else store_some(dst - m, w, col > 0 ? 0 : m, min(8, D - col + m));
-  if (col + 8 >= D) store_some(dst, v, 8 - m, D - col);  // nobody above takes the last m values
-}
-
 // 2^e, e in [-126, 127].
 DA_DEV float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// The k-th group of a thread.  Dense rows: a warp takes 28 new groups, its first 4 lanes again the block before them
-// (without storing), whose values complete the first 16-byte word; so no word waits for another warp.
-constexpr int kNew = 28;
 template <int kLies>
 using Index = std::conditional_t<kLies == kFlat, int64_t, int>;
 template <int kLies>
-DA_DEV Index<kLies> index_of(int k) {
-  if constexpr (kLies == kDense)
-    return (int)((blockIdx.x * kItems + k) * 8 + threadIdx.x / 32) * kNew + (int)(threadIdx.x % 32) - (32 - kNew);
+DA_DEV Index<kLies> index_of(int k) {  // the k-th group of a thread
   return ((Index<kLies>)blockIdx.x * kItems + k) * 256 + threadIdx.x;
 }
-template <int kLies>
-DA_DEV bool loads(const CkptArgs& p, Index<kLies> i) {
-  return i < (Index<kLies>)p.items && (kLies != kDense || i >= 0);
-}
-template <int kLies>
-DA_DEV bool stores(const CkptArgs& p, Index<kLies> i) {
-  return i < (Index<kLies>)p.items && (kLies != kDense || threadIdx.x % 32 >= 32 - kNew);
-}
-
 template <int kLies>
 struct Place {  // of a group of 8 columns
   Index<kLies> group;
@@ -158,6 +93,92 @@ DA_DEV Place<kLies> place_of(const CkptArgs& p, Index<kLies> i) {
   const uint32_t r = p.per_row.div((uint32_t)i), c = (uint32_t)i - r * p.per_row.d;
   return {i, (int)r, (int)c * 8};
 }
+
+// kDense: the values of a block's groups are one run of a dense tensor, which goes through shared memory: in 16-byte words
+// on the tensor's side and, on the threads', whose groups start at any value, in 32-bit words moved by half a word.
+// (Shifted in registers, with the words' other values from neighbouring lanes, storing alone took 15 instructions a
+// value: 50000 x 1001 in 90 us forward and 135 backward, now 61 and 88.)
+struct Run {
+  int64_t base, first, end;  // the values [first, end), base = first rounded down to 16 bytes
+};
+constexpr int kRunWords = 256 * kItems + 1;  // of 16 bytes
+DA_DEV Run run_of(const CkptArgs& p) {
+  auto flat = [&](int i) {
+    const Place<kDense> at = place_of<kDense>(p, i);
+    return (int64_t)at.row * p.D + min(at.col, p.D);
+  };
+  const int i0 = blockIdx.x * (256 * kItems);
+  const int64_t first = flat(i0);
+  return {first & ~int64_t(7), first, flat(min((int)p.items, i0 + 256 * kItems))};
+}
+DA_DEV void load_run(const void* p, const Run& run, int64_t left, uint4* buf) {
+  const uint16_t* src = static_cast<const uint16_t*>(p) + run.base;
+  const int words = (int)((run.end - run.base + 7) / 8), whole = (int)min((int64_t)words, (left - run.base) / 8);
+  uint4 v[kItems];
+#pragma unroll
+  for (int k = 0; k < kItems; ++k)
+    if (k * 256 + (int)threadIdx.x < whole) v[k] = __ldcs(reinterpret_cast<const uint4*>(src) + k * 256 + threadIdx.x);
+#pragma unroll
+  for (int k = 0; k < kItems; ++k)
+    if (k * 256 + (int)threadIdx.x < whole) buf[k * 256 + threadIdx.x] = v[k];
+  // the 1025th word, and the tensor's last values
+  if (threadIdx.x == 0 && whole == kRunWords) buf[kRunWords - 1] = reinterpret_cast<const uint4*>(src)[kRunWords - 1];
+  if (whole < words && threadIdx.x < 8 && run.base + whole * 8 + threadIdx.x < run.end)
+    reinterpret_cast<uint16_t*>(buf)[whole * 8 + threadIdx.x] = src[whole * 8 + threadIdx.x];
+}
+// A group's 8 values, those past D as 0.
+DA_DEV uint4 take_run(const uint4* buf, const Run& run, const Place<kDense>& at, int D) {
+  if (at.col >= D) return make_uint4(0, 0, 0, 0);
+  const int off = (int)((int64_t)at.row * D + at.col - run.base), s = off % 2 * 16;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(buf) + off / 2;
+  uint4 v = make_uint4(__funnelshift_r(w[0], w[1], s), __funnelshift_r(w[1], w[2], s), __funnelshift_r(w[2], w[3], s),
+                       __funnelshift_r(w[3], w[4], s));
+  if (at.col + 8 > D) {  // the next row's values
+    uint32_t* u = &v.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int left = D - at.col - 2 * i;
+      u[i] = left >= 2 ? u[i] : left == 1 ? u[i] & 0xffffu : 0;
+    }
+  }
+  return v;
+}
+DA_DEV void put_run(uint4* buf, const Run& run, const Place<kDense>& at, int D, uint4 v) {
+  if (at.col >= D) return;
+  const int off = (int)((int64_t)at.row * D + at.col - run.base);
+  uint16_t* h = reinterpret_cast<uint16_t*>(buf) + off;
+  uint32_t* w = reinterpret_cast<uint32_t*>(buf) + (off + 1) / 2;
+  if (at.col + 8 > D) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (at.col + i < D) h[i] = (uint16_t)(u[i / 2] >> (i % 2 * 16));
+  } else if (off % 2) {
+    h[0] = (uint16_t)v.x;
+    w[0] = __funnelshift_r(v.x, v.y, 16);
+    w[1] = __funnelshift_r(v.y, v.z, 16);
+    w[2] = __funnelshift_r(v.z, v.w, 16);
+    h[7] = (uint16_t)(v.w >> 16);
+  } else {
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
+  }
+}
+DA_DEV void store_run(void* p, const Run& run, const uint4* buf) {
+  uint16_t* dst = static_cast<uint16_t*>(p) + run.base;
+  const int from = (int)(run.first - run.base), to = (int)(run.end - run.base);
+#pragma unroll
+  for (int k = 0; k <= kItems; ++k) {
+    const int w = k * 256 + threadIdx.x;
+    if (w * 8 >= from && w * 8 + 8 <= to) {
+      reinterpret_cast<uint4*>(dst)[w] = buf[w];
+    } else if (w * 8 < to && w * 8 + 8 > from) {  // a word shared with another block, or past the tensor
+      for (int i = max(from, w * 8); i < min(to, w * 8 + 8); ++i) dst[i] = reinterpret_cast<const uint16_t*>(buf)[i];
+    }
+  }
+}
 template <typename T, int kLies>
 DA_DEV uint4 load_place(const CkptArgs& p, const Place<kLies>& at) {
   if constexpr (kLies == kFlat) return __ldcs(reinterpret_cast<const uint4*>(p.x) + at.group);
@@ -165,39 +186,57 @@ DA_DEV uint4 load_place(const CkptArgs& p, const Place<kLies>& at) {
     if (at.col >= p.D) return make_uint4(0, 0, 0, 0);
     return __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + at.row * p.ldx + at.col));
   }
-  if constexpr (kLies == kDense) {
-    if (at.col >= p.D) return make_uint4(0, 0, 0, 0);
-    return load_dense8(p.x, (int64_t)at.row * p.D + at.col, p.left, at.col, p.D);
-  }
   return load_row8<T>(p.x, at.row * p.ldx, at.col, p.D, p.vec_x);
 }
-// (kDense: called by every lane)
+// (kDense: to the block's shared memory)
 template <typename T, int kLies>
-DA_DEV void store_place(const CkptArgs& p, void* out, int64_t ld, int vec, const Place<kLies>& at, bool live, const F2* v) {
+DA_DEV void store_place(const CkptArgs& p, void* out, int64_t ld, int vec, const Place<kLies>& at, const F2* v, uint4* buf,
+                        const Run& run) {
   const uint4 w = make_uint4(narrow<T>(v[0]), narrow<T>(v[1]), narrow<T>(v[2]), narrow<T>(v[3]));
   if constexpr (kLies == kFlat) {
-    if (live) reinterpret_cast<uint4*>(out)[at.group] = w;
+    reinterpret_cast<uint4*>(out)[at.group] = w;
   } else if constexpr (kLies == kVec) {
-    if (live && at.col < p.D) *reinterpret_cast<uint4*>(static_cast<T*>(out) + at.row * ld + at.col) = w;
+    if (at.col < p.D) *reinterpret_cast<uint4*>(static_cast<T*>(out) + at.row * ld + at.col) = w;
   } else if constexpr (kLies == kDense) {
-    store_dense8(out, (int64_t)at.row * p.D + at.col, at.col, p.D, live && at.col < p.D, w);
+    put_run(buf, run, at, p.D, w);
   } else {
-    if (live) store_row8<T>(out, at.row * ld, at.col, p.D, vec, w);
+    store_row8<T>(out, at.row * ld, at.col, p.D, vec, w);
   }
 }
+// The groups' 8 values each.
+template <typename T, int kLies>
+DA_DEV void load_places(const CkptArgs& p, const Place<kLies> (&at)[kItems], uint4 (&raw)[kItems], uint4* buf,
+                        const Run& run) {
+  if constexpr (kLies == kDense) {
+    load_run(p.x, run, p.left, buf);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kItems; ++k)
+      raw[k] = at[k].group < (int)p.items ? take_run(buf, run, at[k], p.D) : make_uint4(0, 0, 0, 0);
+    __syncthreads();  // (a result may take the place)
+  } else {
+#pragma unroll
+    for (int k = 0; k < kItems; ++k)
+      raw[k] = at[k].group < (Index<kLies>)p.items ? load_place<T, kLies>(p, at[k]) : make_uint4(0, 0, 0, 0);
+  }
+}
+template <int kLies, int kBuffers>
+struct Buffers {
+  uint4 words[kLies == kDense ? kBuffers : 1][kLies == kDense ? kRunWords + 1 : 1];  // (a take reads a word further)
+};
 
 template <typename T, int kLies>
 __global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
+  __shared__ Buffers<kLies, 1> buffers;
+  uint4* buf = buffers.words[0];
+  const Run run = kLies == kDense ? run_of(p) : Run{};
   uint4 raw[kItems];
   Place<kLies> at[kItems];
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    raw[k] = make_uint4(0, 0, 0, 0);
-    at[k] = place_of<kLies>(p, index_of<kLies>(k));
-    if (loads<kLies>(p, index_of<kLies>(k))) raw[k] = load_place<T, kLies>(p, at[k]);
-  }
+  for (int k = 0; k < kItems; ++k) at[k] = place_of<kLies>(p, index_of<kLies>(k));
+  load_places<T, kLies>(p, at, raw, buf, run);
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     // the 16-bit patterns without their signs order as integers, NaN above infinity above every number
@@ -231,7 +270,7 @@ __global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p) {
       }
       q = pack_s8x8(o);
     }
-    const bool live = stores<kLies>(p, index_of<kLies>(k));
+    const bool live = at[k].group < (Index<kLies>)p.items;
     if (live) {
       *reinterpret_cast<uint2*>(p.q + (int64_t)at[k].group * 8) = q;
       if ((at[k].group & 3) == 0) p.e[at[k].group >> 2] = (int8_t)(finite ? e : kNotFinite);
@@ -239,8 +278,12 @@ __global__ void __launch_bounds__(256) checkpoint8_kernel(const CkptArgs p) {
     if (p.gelu) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = gelu2(v[j]);
-      store_place<T, kLies>(p, p.h, p.ldh, p.vec_h, at[k], live, v);
+      if (live) store_place<T, kLies>(p, p.h, p.ldh, p.vec_h, at[k], v, buf, run);
     }
+  }
+  if (kLies == kDense && p.gelu) {
+    __syncthreads();
+    store_run(p.h, run, buf);
   }
 }
 
@@ -257,25 +300,26 @@ template <typename T, int kLies>
 __global__ void __launch_bounds__(256) checkpoint8_restore_kernel(const CkptArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
+  __shared__ Buffers<kLies, 1> buffers;
+  uint4* buf = buffers.words[0];
+  const Run run = kLies == kDense ? run_of(p) : Run{};
   uint2 q[kItems] = {};
   int e[kItems] = {};
   Place<kLies> at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     at[k] = place_of<kLies>(p, index_of<kLies>(k));
-    if (loads<kLies>(p, index_of<kLies>(k))) {
+    if (at[k].group < (Index<kLies>)p.items) {
       q[k] = *reinterpret_cast<const uint2*>(p.q + (int64_t)at[k].group * 8);
       e[k] = p.e[at[k].group >> 2];
     }
   }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    const bool live = stores<kLies>(p, index_of<kLies>(k));
-    if (kLies != kDense && !live) continue;
+    if (at[k].group >= (Index<kLies>)p.items) continue;
     F2 v[4];
     restore8(q[k], e[k], v);
     if constexpr (std::is_same<T, float>::value) {
-      if (!live) continue;
       float* dst = static_cast<float*>(p.h) + (kLies == kFlat ? at[k].group * 8 : at[k].row * p.ldh + at[k].col);
       float f[8];
 #pragma unroll
@@ -290,8 +334,12 @@ __global__ void __launch_bounds__(256) checkpoint8_restore_kernel(const CkptArgs
           if (at[k].col + j < p.D) dst[j] = f[j];
       }
     } else {
-      store_place<T, kLies>(p, p.h, p.ldh, p.vec_h, at[k], live, v);
+      store_place<T, kLies>(p, p.h, p.ldh, p.vec_h, at[k], v, buf, run);
     }
+  }
+  if constexpr (kLies == kDense) {
+    __syncthreads();
+    store_run(p.h, run, buf);
   }
 }
 
@@ -299,29 +347,36 @@ template <typename T, int kLies>
 __global__ void __launch_bounds__(256) checkpoint8_gelu_bwd_kernel(const CkptArgs p) {
   grid_dependency_wait();
   grid_launch_dependents();
-  uint4 raw[kItems] = {};
+  __shared__ Buffers<kLies, 2> buffers;
+  uint4 *buf = buffers.words[0], *buf_h = buffers.words[kLies == kDense];
+  const Run run = kLies == kDense ? run_of(p) : Run{};
+  uint4 raw[kItems];
   uint2 q[kItems] = {};
   int e[kItems] = {};
   Place<kLies> at[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     at[k] = place_of<kLies>(p, index_of<kLies>(k));
-    if (loads<kLies>(p, index_of<kLies>(k))) {
-      raw[k] = load_place<T, kLies>(p, at[k]);
+    if (at[k].group < (Index<kLies>)p.items) {
       q[k] = *reinterpret_cast<const uint2*>(p.q + (int64_t)at[k].group * 8);
       e[k] = p.e[at[k].group >> 2];
     }
   }
+  load_places<T, kLies>(p, at, raw, buf, run);
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    const bool live = stores<kLies>(p, index_of<kLies>(k));
-    if (kLies != kDense && !live) continue;
+    if (at[k].group >= (Index<kLies>)p.items) continue;
     F2 z[4], d[4] = {widen<T>(raw[k].x), widen<T>(raw[k].y), widen<T>(raw[k].z), widen<T>(raw[k].w)};
     restore8(q[k], e[k], z);
 #pragma unroll
     for (int j = 0; j < 4; ++j) d[j] = mul2(d[j], gelu_grad2(z[j]));
-    store_place<T, kLies>(p, p.dz, p.lddz, p.vec_dz, at[k], live, d);
-    if (p.h) store_place<T, kLies>(p, p.h, p.ldh, p.vec_h, at[k], live, z);
+    store_place<T, kLies>(p, p.dz, p.lddz, p.vec_dz, at[k], d, buf, run);
+    if (p.h) store_place<T, kLies>(p, p.h, p.ldh, p.vec_h, at[k], z, buf_h, run);
+  }
+  if constexpr (kLies == kDense) {
+    __syncthreads();
+    store_run(p.dz, run, buf);
+    if (p.h) store_run(p.h, run, buf_h);
   }
 }
 
@@ -329,9 +384,7 @@ __global__ void __launch_bounds__(256) checkpoint8_gelu_bwd_kernel(const CkptArg
 // stay below 2^31.
 template <typename T, template <typename, int> class Kernel>
 int run(CkptArgs p, int64_t rows, int lies, cudaStream_t st) {
-  // a warp of kDense reads groups that another one stores: not where the result replaces the input
-  if (lies == kDense && p.x && (p.h == p.x || p.dz == p.x)) lies = kAny;
-  const int64_t per_block = (lies == kDense ? 8 * kNew : 256) * kItems;
+  const int64_t per_block = 256 * kItems;
   auto grid = [&] { return dim3((unsigned)((p.items + per_block - 1) / per_block)); };
   if (lies == kFlat && rows * p.per_row.d / per_block < 0x7fffffffLL) {
     p.items = rows * p.per_row.d;
