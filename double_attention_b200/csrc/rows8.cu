@@ -68,6 +68,25 @@ DA_DEV uint32_t row_max(uint32_t v, float* red) {
   return v;
 }
 
+// Both at once for a row over several warps, behind one barrier (`red`, two slots a warp, not in use).
+template <int kT>
+DA_DEV void row_sum_max(float& v, uint32_t& m, float* red) {
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0) {
+    red[threadIdx.x >> 5] = v;
+    red[kT / 32 + (threadIdx.x >> 5)] = __uint_as_float(m);
+  }
+  __syncthreads();
+  v = 0.f;
+  m = 0;
+#pragma unroll
+  for (int i = 0; i < kT / 32; ++i) {
+    v += red[i];
+    m = max(m, __float_as_uint(red[kT / 32 + i]));
+  }
+}
+
 DA_DEV uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // The largest magnitude of three; a NaN wins.
@@ -180,7 +199,7 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
   constexpr int kBlock = kT == 32 ? 256 : kT;  // 8 rows, a warp each, or one
   constexpr bool kBranch = !std::is_same<TB, None>::value;
   constexpr int kSlots = kNV * kT + 1;  // groups of a row's window, and one more that a shifted read touches
-  __shared__ float red[kBlock / 32];
+  __shared__ float red[2 * (kBlock / 32)];
   __shared__ uint2 moved[kShift ? kBlock / kT * kSlots : 1];
   grid_dependency_wait();
   grid_launch_dependents();
@@ -259,31 +278,50 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
       for (int i = 0; i < 4; ++i) v[c][i] = zero;
     }
   }
-  float rstd = 1.f;
-  if constexpr (kKind != kQuantize) {
+  float rstd = 1.f, squares = 0.f;
+  if constexpr (kKind == kRms) {
+    // v = r w needs no sum: rows over several warps are reduced once, to sum and largest value (16384 x 8192 from fp16 in
+    // 79 us, with a barrier for each 99).  A warp's own sum waits for none: taken first, with its root under the weights'
+    // loads, 100000 x 512 takes 31 us, else 34.
+    F2 s = zero;
+#pragma unroll
+    for (int c = 0; c < kNV; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = fma2(v[c][i], v[c][i], s);
+    float lo, hi;
+    split(s, lo, hi);
+    squares = lo + hi;
+    if constexpr (kT == 32) rstd = 1.f / sqrtf(row_sum<kT>(squares, red) / (float)p.D + p.eps);
+#pragma unroll
+    for (int c = 0; c < kNV; ++c) {
+      const int at = (c * kT + t) * 8;
+      if (!p.weight || at >= end) continue;
+      F2 w[4];
+      load_columns<kShift>(p.weight, p.weight_dtype, p.aligned, at - off, p.D, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[c][i] = mul2(v[c][i], w[i]);
+    }
+  }
+  if constexpr (kKind == kLayer) {
     auto total = [&](F2 s) {
       float a, b;
       split(s, a, b);
       return row_sum<kT>(a + b, red) / (float)p.D;
     };
-    F2 mean = zero, s = zero;
-    if constexpr (kKind == kLayer) {
+    F2 s = zero;
 #pragma unroll
-      for (int c = 0; c < kNV; ++c)
+    for (int c = 0; c < kNV; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s = add2(s, v[c][i]);
-      mean = dup(-total(s));
-      s = zero;
-    }
+      for (int i = 0; i < 4; ++i) s = add2(s, v[c][i]);
+    const F2 mean = dup(-total(s));
+    s = zero;
 #pragma unroll
     for (int c = 0; c < kNV; ++c) {
-      if constexpr (kKind == kLayer) {
-        const int at = (c * kT + t) * 8;
-        if (at < end) {
+      const int at = (c * kT + t) * 8;
+      if (at < end) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[c][i] = add2(v[c][i], mean);
-          if constexpr (kShift) inside(at, v[c]);
-        }
+        for (int i = 0; i < 4; ++i) v[c][i] = add2(v[c][i], mean);
+        if constexpr (kShift) inside(at, v[c]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) s = fma2(v[c][i], v[c][i], s);
@@ -293,22 +331,14 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
     for (int c = 0; c < kNV; ++c) {
       const int at = (c * kT + t) * 8;
       if (at >= end) continue;
-      F2 w[4];
-      if (p.weight) load_columns<kShift>(p.weight, p.weight_dtype, p.aligned, at - off, p.D, w);
-      if constexpr (kKind == kRms) {
-        if (p.weight) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[c][i] = mul2(v[c][i], w[i]);
-        }
-      } else {
+      for (int i = 0; i < 4; ++i) v[c][i] = mul2(v[c][i], dup(rstd));
+      if (p.weight) {
+        F2 w[4], b[4] = {zero, zero, zero, zero};
+        load_columns<kShift>(p.weight, p.weight_dtype, p.aligned, at - off, p.D, w);
+        if (p.bias) load_columns<kShift>(p.bias, p.bias_dtype, p.aligned, at - off, p.D, b);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[c][i] = mul2(v[c][i], dup(rstd));
-        if (p.weight) {
-          F2 b[4] = {zero, zero, zero, zero};
-          if (p.bias) load_columns<kShift>(p.bias, p.bias_dtype, p.aligned, at - off, p.D, b);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[c][i] = fma2(v[c][i], w[i], b[i]);
-        }
+        for (int i = 0; i < 4; ++i) v[c][i] = fma2(v[c][i], w[i], b[i]);
       }
     }
   }
@@ -322,7 +352,14 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
       a = max_abs(a, lo, hi);
     }
   float inv, scale;
-  row_scale(row_max<kT>(__float_as_uint(a) & 0x7fffffffu, red), kKind == kRms ? rstd : 1.f, inv, scale);
+  uint32_t largest = abs_bits(a);
+  if constexpr (kKind == kRms && kT > 32) {
+    row_sum_max<kT>(squares, largest, red);
+    rstd = 1.f / sqrtf(squares / (float)p.D + p.eps);
+  } else {
+    largest = row_max<kT>(largest, red);
+  }
+  row_scale(largest, kKind == kRms ? rstd : 1.f, inv, scale);
   // |v inv| exceeds 127 by a rounding at most.  The product is rounded before the sum (a fused pair would round once,
   // and an element in 1e5 would differ from the other variants' rint(v inv)).
   auto whole = [&](F2 x) {
