@@ -39,52 +39,69 @@ struct NormArgs {
   int aligned;  // weight and bias start on 16 bytes
 };
 
-// Sum and largest bit pattern over the kT threads of a row (kT a multiple of 32; a block-wide row uses
-// `red`, one slot per warp).
+// Sum and largest bit pattern over the threads of a row: a warp (kT = 32), a block of kT threads, or the block whatever
+// its size (kT = 0; at most 32 warps).  `red`: a slot a warp.  Every thread adds in the same order (a butterfly adds
+// the same pairs in every lane).
+DA_DEV float warp_sum(float v) {
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <int kT>
+DA_DEV float add_warps(const float* red) {
+  if constexpr (kT == 0) {
+    const int lane = threadIdx.x & 31;
+    return warp_sum(lane < (int)blockDim.x / 32 ? red[lane] : 0.f);
+  }
+  float v = 0.f;
+#pragma unroll
+  for (int i = 0; i < kT / 32; ++i) v += red[i];
+  return v;
+}
+template <int kT>
+DA_DEV uint32_t max_warps(const float* red) {
+  if constexpr (kT == 0) {
+    const int lane = threadIdx.x & 31;
+    return __reduce_max_sync(0xffffffffu, lane < (int)blockDim.x / 32 ? __float_as_uint(red[lane]) : 0);
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < kT / 32; ++i) m = max(m, __float_as_uint(red[i]));
+  return m;
+}
 template <int kT>
 DA_DEV float row_sum(float v, float* red) {
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if constexpr (kT > 32) {
+  v = warp_sum(v);
+  if constexpr (kT != 32) {
     __syncthreads();
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = 0.f;
-#pragma unroll
-    for (int i = 0; i < kT / 32; ++i) v += red[i];  // same order in every thread
+    v = add_warps<kT>(red);
   }
   return v;
 }
 template <int kT>
-DA_DEV uint32_t row_max(uint32_t v, float* red) {
-  v = __reduce_max_sync(0xffffffffu, v);
-  if constexpr (kT > 32) {
+DA_DEV uint32_t row_max(uint32_t m, float* red) {
+  m = __reduce_max_sync(0xffffffffu, m);
+  if constexpr (kT != 32) {
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = __uint_as_float(v);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = __uint_as_float(m);
     __syncthreads();
-    v = 0;
-#pragma unroll
-    for (int i = 0; i < kT / 32; ++i) v = max(v, __float_as_uint(red[i]));
+    m = max_warps<kT>(red);
   }
-  return v;
+  return m;
 }
-
-// Both at once for a row over several warps, behind one barrier (`red`, two slots a warp, not in use).
+// Both at once for a row over several warps, behind one barrier (`red`, 64 slots, not in use).
 template <int kT>
 DA_DEV void row_sum_max(float& v, uint32_t& m, float* red) {
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  v = warp_sum(v);
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0) {
     red[threadIdx.x >> 5] = v;
-    red[kT / 32 + (threadIdx.x >> 5)] = __uint_as_float(m);
+    red[32 + (threadIdx.x >> 5)] = __uint_as_float(m);
   }
   __syncthreads();
-  v = 0.f;
-  m = 0;
-#pragma unroll
-  for (int i = 0; i < kT / 32; ++i) {
-    v += red[i];
-    m = max(m, __float_as_uint(red[kT / 32 + i]));
-  }
+  v = add_warps<kT>(red);
+  m = max_warps<kT>(red + 32);
 }
 
 DA_DEV uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -190,21 +207,21 @@ DA_DEV void load_columns(const void* p, int dtype, bool aligned, int col, int D,
   }
 }
 
-// kT threads per row, 8 * kNV elements per thread, 16 bytes an access.  kShift: dense tensors of any width D.  Their
+// A warp (kT = 32) or a block (of kT threads, or any) per row, 8 * kNV elements per thread, 16 bytes an access.  kShift: dense tensors of any width D.  Their
 // row r starts r D mod 8 elements after a multiple of 8, so a thread takes the groups of 8 that are aligned in
 // memory; the row's first and last groups mask what belongs to its neighbours, and q, whose rows do start on 16
 // bytes, goes through shared memory to be moved by the row's offset.
 template <typename TX, typename TB, int kKind, int kT, int kNV, bool kShift>
-__global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const NormArgs p) {
-  constexpr int kBlock = kT == 32 ? 256 : kT;  // 8 rows, a warp each, or one
+__global__ void __launch_bounds__(kT == 32 ? 256 : kT ? kT : 512) norm_int8_kernel(const NormArgs p) {
   constexpr bool kBranch = !std::is_same<TB, None>::value;
-  constexpr int kSlots = kNV * kT + 1;  // groups of a row's window, and one more that a shifted read touches
-  __shared__ float red[2 * (kBlock / 32)];
-  __shared__ uint2 moved[kShift ? kBlock / kT * kSlots : 1];
+  const int threads = kT ? kT : blockDim.x;  // of a row; 8 rows, a warp each, or one
+  const int slots_of_row = kNV * threads + 1;      // groups of a row's window, and one more that a shifted read touches
+  __shared__ float red[kT == 32 ? 1 : 64];
+  extern __shared__ uint2 moved[];  // kShift
   grid_dependency_wait();
   grid_launch_dependents();
-  const int t = threadIdx.x % kT;
-  const int64_t row = (int64_t)blockIdx.x * (kBlock / kT) + threadIdx.x / kT;
+  const int in_block = kT == 32 ? threadIdx.x / 32 : 0, t = kT == 32 ? threadIdx.x % 32 : threadIdx.x;
+  const int64_t row = kT == 32 ? (int64_t)blockIdx.x * 8 + in_block : blockIdx.x;
   if (row >= p.rows) return;  // a whole warp (kT = 32) or never (one row per block)
   const int off = kShift ? (int)(row * p.D % 8) : 0;  // the row's start within its first group
   const int64_t bx = kShift ? row * p.D - off : row * p.ldx, bb = kShift ? bx : row * p.ldb, bo = kShift ? bx : row * p.ldo;
@@ -213,7 +230,7 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
   Eight<typename std::conditional<kBranch, TB, float>::type> br[kBranch ? kNV : 1];
 #pragma unroll
   for (int c = 0; c < kNV; ++c) {
-    const int at = (c * kT + t) * 8;
+    const int at = (c * threads + t) * 8;
     if (at < end) {
       // (only the tensor's very last group can reach past its end)
       if (!kShift || bx + at + 8 <= p.rows * p.D) {
@@ -251,7 +268,7 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
   };
 #pragma unroll
   for (int c = 0; c < kNV; ++c) {
-    const int at = (c * kT + t) * 8;
+    const int at = (c * threads + t) * 8;
     if (at < end) {
       x[c].pairs(v[c]);
       if constexpr (kBranch) {
@@ -294,7 +311,7 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
     if constexpr (kT == 32) rstd = 1.f / sqrtf(row_sum<kT>(squares, red) / (float)p.D + p.eps);
 #pragma unroll
     for (int c = 0; c < kNV; ++c) {
-      const int at = (c * kT + t) * 8;
+      const int at = (c * threads + t) * 8;
       if (!p.weight || at >= end) continue;
       F2 w[4];
       load_columns<kShift>(p.weight, p.weight_dtype, p.aligned, at - off, p.D, w);
@@ -317,7 +334,7 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
     s = zero;
 #pragma unroll
     for (int c = 0; c < kNV; ++c) {
-      const int at = (c * kT + t) * 8;
+      const int at = (c * threads + t) * 8;
       if (at < end) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[c][i] = add2(v[c][i], mean);
@@ -329,7 +346,7 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
     rstd = 1.f / sqrtf(total(s) + p.eps);
 #pragma unroll
     for (int c = 0; c < kNV; ++c) {
-      const int at = (c * kT + t) * 8;
+      const int at = (c * threads + t) * 8;
       if (at >= end) continue;
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[c][i] = mul2(v[c][i], dup(rstd));
@@ -353,7 +370,7 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
     }
   float inv, scale;
   uint32_t largest = abs_bits(a);
-  if constexpr (kKind == kRms && kT > 32) {
+  if constexpr (kKind == kRms && kT != 32) {
     row_sum_max<kT>(squares, largest, red);
     rstd = 1.f / sqrtf(squares / (float)p.D + p.eps);
   } else {
@@ -368,13 +385,13 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
     return f2(__fadd_rn(__fmul_rn(lo, inv), kRoundAt), __fadd_rn(__fmul_rn(hi, inv), kRoundAt));
   };
   auto bytes = [&](F2 lo, F2 hi) { return low_bytes(whole(lo), whole(hi)); };
-  uint2* slots = moved + (kShift ? threadIdx.x / kT * kSlots : 0);
+  uint2* slots = moved + in_block * slots_of_row;
 #pragma unroll
   for (int c = 0; c < kNV; ++c) {
-    const int at = (c * kT + t) * 8;
+    const int at = (c * threads + t) * 8;
     if (at >= end) continue;
     const uint2 o = make_uint2(bytes(v[c][0], v[c][1]), bytes(v[c][2], v[c][3]));
-    if constexpr (kShift) slots[c * kT + t] = o;
+    if constexpr (kShift) slots[c * threads + t] = o;
     else *reinterpret_cast<uint2*>(p.q + row * p.ldq + at) = o;
   }
   if constexpr (kShift) {
@@ -382,9 +399,9 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
     else __syncthreads();
 #pragma unroll
     for (int c = 0; c < kNV; ++c) {
-      const int col = (c * kT + t) * 8;  // bytes col .. + 8 of the row are off further on in the window
+      const int col = (c * threads + t) * 8;  // bytes col .. + 8 of the row are off further on in the window
       if (col >= p.D) continue;
-      const uint2 lo = slots[c * kT + t], hi = slots[c * kT + t + 1];
+      const uint2 lo = slots[c * threads + t], hi = slots[c * threads + t + 1];
       const uint32_t w[4] = {lo.x, lo.y, hi.x, hi.y};
       const bool second = off >= 4;
       const uint32_t w0 = second ? w[1] : w[0], w1 = second ? w[2] : w[1], w2 = second ? w[3] : w[2];
@@ -400,7 +417,7 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT) norm_int8_kernel(const No
 // what it wrote itself); rows wider than the register variants hold come here too.
 template <int kT>
 __global__ void __launch_bounds__(kT) norm_int8_any_kernel(const NormArgs p) {
-  __shared__ float red[kT / 32];
+  __shared__ float red[32];
   grid_dependency_wait();
   grid_launch_dependents();
   const int64_t row = blockIdx.x;
@@ -417,7 +434,7 @@ __global__ void __launch_bounds__(kT) norm_int8_any_kernel(const NormArgs p) {
   }
   float mean = 0.f, rstd = 1.f;
   if (p.kind != kQuantize) {
-    s = row_sum<kT>(s, red) / (float)p.D;
+    s = row_sum<0>(s, red) / (float)p.D;
     if (p.kind == kLayer) {
       mean = s;
       s = 0.f;
@@ -425,7 +442,7 @@ __global__ void __launch_bounds__(kT) norm_int8_any_kernel(const NormArgs p) {
         const float d = load1(src, p.x_dtype, base + col) - mean;
         s = fmaf(d, d, s);
       }
-      s = row_sum<kT>(s, red) / (float)p.D;
+      s = row_sum<0>(s, red) / (float)p.D;
     }
     rstd = 1.f / sqrtf(s + p.eps);
   }
@@ -441,7 +458,7 @@ __global__ void __launch_bounds__(kT) norm_int8_any_kernel(const NormArgs p) {
   };
   uint32_t a = 0;
   for (int col = threadIdx.x; col < p.D; col += kT) a = max(a, abs_bits(value(col)));
-  a = row_max<kT>(a, red);
+  a = row_max<0>(a, red);
   float inv, scale;
   row_scale(a, p.kind == kRms ? rstd : 1.f, inv, scale);
   for (int col = threadIdx.x; col < p.D; col += kT) p.q[row * p.ldq + col] = (int8_t)quant(value(col), inv);
@@ -535,24 +552,29 @@ int launch_dequant(const int8_t* q, int64_t ldq, const float* scale, int64_t row
 }
 
 template <typename TX, typename TB, int kKind, bool kShift, int kT, int kNV>
-int launch_t(const NormArgs& p, cudaStream_t st) {
+int launch_t(const NormArgs& p, int threads, cudaStream_t st) {
   const int64_t blocks = kT == 32 ? (p.rows + 7) / 8 : p.rows;
   if (blocks > 0x7fffffffLL) return DA_ERR_SHAPE;
-  return launch_kernel(norm_int8_kernel<TX, TB, kKind, kT, kNV, kShift>, dim3((unsigned)blocks),
-                       dim3(kT == 32 ? 256 : kT), 0, st, false, p);
+  const int smem = !kShift ? 0 : kT == 32 ? 8 * (kNV * 32 + 1) * 8 : (kNV * threads + 1) * 8;
+  return launch_kernel(norm_int8_kernel<TX, TB, kKind, kT, kNV, kShift>, dim3((unsigned)blocks), dim3(threads), smem, st,
+                       false, p);
 }
 // As few threads a row as hold it with 32 values each: more loads in flight a thread and fewer warps at a barrier
-// (a block of 256 for every row above 1024 columns: 30001 x 1501 in 82 us, against 61 us so).
+// (a block of 256 for every row above 1024 columns: 30001 x 1501 in 82 us, against 61 us so), and none that idle
+// (in powers of two, 16384 x 8191 with an fp32 residual took 403 us, so 255).  A size that the compiler does not know
+// costs 5 to 10 % (16384 x 8192 from fp16 in 80 us, else 88), so the common ones are known.
 template <typename TX, typename TB, int kKind, bool kShift>
 int launch_shift(const NormArgs& p, cudaStream_t st) {
   const int window = p.D + (kShift ? 7 : 0);
-  if (window <= 256) return launch_t<TX, TB, kKind, kShift, 32, 1>(p, st);
-  if (window <= 512) return launch_t<TX, TB, kKind, kShift, 32, 2>(p, st);
-  if (window <= 1024) return launch_t<TX, TB, kKind, kShift, 32, 4>(p, st);
-  if (window <= 2048) return launch_t<TX, TB, kKind, kShift, 64, 4>(p, st);
-  if (window <= 4096) return launch_t<TX, TB, kKind, kShift, 128, 4>(p, st);
-  if (window <= 8192) return launch_t<TX, TB, kKind, kShift, 256, 4>(p, st);
-  return launch_t<TX, TB, kKind, kShift, 512, 4>(p, st);
+  if (window <= 256) return launch_t<TX, TB, kKind, kShift, 32, 1>(p, 256, st);
+  if (window <= 512) return launch_t<TX, TB, kKind, kShift, 32, 2>(p, 256, st);
+  if (window <= 768) return launch_t<TX, TB, kKind, kShift, 32, 3>(p, 256, st);
+  if (window <= 1024) return launch_t<TX, TB, kKind, kShift, 32, 4>(p, 256, st);
+  const int threads = (window + 1023) / 1024 * 32;
+  if (threads == 64) return launch_t<TX, TB, kKind, kShift, 64, 4>(p, threads, st);
+  if (threads == 128) return launch_t<TX, TB, kKind, kShift, 128, 4>(p, threads, st);
+  if (threads == 256) return launch_t<TX, TB, kKind, kShift, 256, 4>(p, threads, st);
+  return launch_t<TX, TB, kKind, kShift, 0, 4>(p, threads, st);
 }
 template <typename TX, typename TB>
 int launch_types(const NormArgs& p, bool shift, cudaStream_t st) {
