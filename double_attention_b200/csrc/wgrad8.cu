@@ -358,22 +358,22 @@ __global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constan
   if (warp == 1) tmem_dealloc<2>(tmem, 2 * kTile);
 }
 
-// dW = the splits' partial sums.  A block takes 32 rows x 4 columns; its 8 warps add a range of the splits each, in
-// order, and the first adds the 8 sums in order.
-template <typename TO>
+// dW = the splits' partial sums.  kWays warps add a range of the splits each for 32 rows x 4 columns, in order, and the first
+// adds their sums in order.
+template <typename TO, int kWays>
 __global__ void __launch_bounds__(256) reduce_kernel(const float* partial, int splits, int k_tiles, int n_tiles, int N,
                                                      int K, TO* out, int64_t ldo) {
   __shared__ float4 part[8][32];
   grid_dependency_wait();
   grid_launch_dependents();
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int quad = blockIdx.x % 4, col4 = blockIdx.x / 4 % (kTile / 4), half = blockIdx.x / kTile;  // half = tile * 2 + rank
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, way = warp % kWays;
+  const int piece = blockIdx.x * (8 / kWays) + warp / kWays;
+  const int quad = piece % 4, col4 = piece / 4 % (kTile / 4), half = piece / kTile;  // half = tile * 2 + rank
   const int tile = half / 2, rank = half % 2;
   const int row = tile / k_tiles * kTile + rank * 128 + quad * 32 + lane, col = tile % k_tiles * kTile + col4 * 4;
-  if (col >= K || tile / k_tiles * kTile + rank * 128 + quad * 32 >= N) return;  // the whole block
-  const int per = (splits + 7) / 8, z0 = warp * per, z1 = min(splits, z0 + per);
+  const int per = (splits + kWays - 1) / kWays, z0 = way * per, z1 = min(splits, z0 + per);
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (row < N) {
+  if (row < N && col < K) {
     const float4* src = partial_at(const_cast<float*>(partial), k_tiles * n_tiles, 0, tile, rank, col4, quad * 32 + lane);
     const int64_t step = (int64_t)k_tiles * n_tiles * (kTile * kTile / 4);
 #pragma unroll 5
@@ -382,12 +382,14 @@ __global__ void __launch_bounds__(256) reduce_kernel(const float* partial, int s
       s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
   }
-  part[warp][lane] = s;
-  __syncthreads();
-  if (warp > 0 || row >= N) return;
+  if constexpr (kWays > 1) {
+    part[warp][lane] = s;
+    __syncthreads();
+  }
+  if (way > 0 || row >= N || col >= K) return;
 #pragma unroll
-  for (int w = 1; w < 8; ++w) {
-    const float4 v = part[w][lane];
+  for (int w = 1; w < kWays; ++w) {
+    const float4 v = part[warp + w][lane];
     s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
   }
   TO* dst = out + row * ldo + col;
@@ -410,7 +412,6 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* src, in
                                                          Div31 per_row, int N, uint16_t* dst) {
   grid_dependency_wait();
   grid_launch_dependents();
-  const int64_t to = (int64_t)per_row.d * 8;
   uint4 v[kCopies];
 #pragma unroll
   for (int k = 0; k < kCopies; ++k) {
@@ -455,7 +456,8 @@ struct Plan {
   bool expanded;
   int64_t x_elems, y_elems, elems;  // workspace (fp32 elements): the expanded X, dY on 16-byte rows, and the partial sums
 };
-// The rows are split while there are fewer tiles than CTA pairs; a split has at least 256 rows.
+// The rows are split while there are fewer tiles than CTA pairs; a split has at least 256 rows (1000 rows, 512 x 512 in
+// 13.5 us; at least 128 12.9, at least 512 15.2; 256 rows 10.3, 12.0 and 10.2).
 Plan plan_for(int64_t rows, int64_t N, int64_t K) {
   const int64_t n_tiles = (N + kTile - 1) / kTile, tiles = n_tiles * ((K + kTile - 1) / kTile);
   int64_t s = (sm_count() / 2) / tiles;
@@ -520,12 +522,16 @@ int run(const void* dy, int64_t ldy, const int8_t* q, const int8_t* e, int64_t r
     rc = plan.expanded ? launch<T, T, true>(ty, tx, p, st) : launch<T, T, false>(ty, tx, p, st);
   if (rc || !split) return rc;
   const int k_tiles = (int)((K + kTile - 1) / kTile), n_tiles = (int)((N + kTile - 1) / kTile);
-  const dim3 grid((unsigned)(k_tiles * n_tiles * 2 * kTile));
-  if (out_dtype == DA_F32)
-    return launch_kernel(reduce_kernel<float>, grid, dim3(256), 0, st, false, (const float*)partial, plan.splits, k_tiles,
-                         n_tiles, (int)N, (int)K, static_cast<float*>(out), ldo);
-  return launch_kernel(reduce_kernel<T>, grid, dim3(256), 0, st, false, (const float*)partial, plan.splits, k_tiles, n_tiles,
-                       (int)N, (int)K, static_cast<T*>(out), ldo);
+  // Measured (us, 2 / 8 warps a piece): 9 splits of 392 x 1000 17.2 / 19.8, 6 of 1536 x 512 15.9 / 19.7, 16 of 512 x 512
+  // 14.8 / 15.0, 37 of 128 x 384 18.8 / 15.3, 74 of 128 x 128 25.7 / 19.4.
+  auto sum = [&](auto* to) {
+    using TO = std::remove_pointer_t<decltype(to)>;
+    const unsigned pieces = (unsigned)(k_tiles * n_tiles * 2 * kTile);
+    const bool few = plan.splits <= 16;
+    return launch_kernel(few ? reduce_kernel<TO, 2> : reduce_kernel<TO, 8>, dim3(few ? pieces / 4 : pieces), dim3(256), 0, st,
+                         false, (const float*)partial, plan.splits, k_tiles, n_tiles, (int)N, (int)K, to, ldo);
+  };
+  return out_dtype == DA_F32 ? sum(static_cast<float*>(out)) : sum(static_cast<T*>(out));
 }
 
 }  // namespace wg8
