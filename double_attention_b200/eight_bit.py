@@ -235,7 +235,8 @@ def _norm_int8(name: str, x: Tensor, branch: Tensor | None, weight: Tensor | Non
 def _rms_args(norm, x: Tensor) -> tuple[Tensor | None, float]:
     if not isinstance(norm, torch.nn.RMSNorm) or norm.normalized_shape != x.shape[-1:]:
         raise ValueError(f"expected an nn.RMSNorm over the last dimension of x {tuple(x.shape)}, got {norm}")
-    return norm.weight, torch.finfo(x.dtype).eps if norm.eps is None else norm.eps
+    # (without an eps of its own nn.RMSNorm takes that of the type it computes in, fp32 for all types here)
+    return norm.weight, torch.finfo(torch.float32).eps if norm.eps is None else norm.eps
 
 
 def _layer_args(norm, x: Tensor) -> tuple[Tensor | None, Tensor | None, float]:
