@@ -3,11 +3,14 @@
 :class:`Int8DoubleAttentionLM` quantises every Linear of the model once (a scale per output channel) and runs
 its forward on the eight-bit operators: each norm adds the pending branch and leaves int8 rows, the projections
 and the feed-forward layers multiply int8 rows, the route and the outer attention between them stay on their
-16-bit kernels.  Per layer that is four int8 products (Q and K together, V, output, two of the feed-forward)
-between two fused norms.  Inference only; the model it is built from is left as it is.
+16-bit kernels.  Per layer that is five int8 products (Q and K together, V, output, two of the feed-forward)
+between two fused norms.  Inference only; the model it is built from is left as it is, and nothing that happens to it
+later reaches the served one.
 """
 
 from __future__ import annotations
+
+import copy
 
 import torch
 from torch import Tensor, nn
@@ -39,6 +42,22 @@ class Int8Linear(nn.Module):
         return int8_linear(rows, Int8Rows(self.weight, self.scale), self.bias, gelu=gelu, dtype=self.dtype)
 
 
+def _frozen(module: nn.Module) -> nn.Module:
+    return copy.deepcopy(module).requires_grad_(False)
+
+
+class _Bank(nn.Module):
+    """A bank's normalised dictionaries as the route reads them."""
+
+    def __init__(self, views: ops.DictionaryViews) -> None:
+        super().__init__()
+        for name in ("key", "key_t", "value", "value_t", "key_max"):
+            self.register_buffer(name, getattr(views, name).clone())
+
+    def views(self) -> ops.DictionaryViews:
+        return ops.DictionaryViews(self.key, self.key_t, self.value, self.value_t, self.key_max, self.key, self.value)
+
+
 class _Int8Block(nn.Module):
     def __init__(self, block: DoubleAttentionBlock, dtype: torch.dtype) -> None:
         super().__init__()
@@ -49,7 +68,7 @@ class _Int8Block(nn.Module):
         if act.approximate != "none":
             raise NotImplementedError("int8 serving covers the exact form of GELU")
         self.config = cfg
-        self.attention_norm, self.feedforward_norm = block.attention_norm, block.feedforward_norm
+        self.attention_norm, self.feedforward_norm = _frozen(block.attention_norm), _frozen(block.feedforward_norm)
         self.query_key = Int8Linear(torch.cat((attention.query.weight, attention.key.weight)), None, dtype)
         self.value = Int8Linear(attention.value.weight, attention.value.bias, torch.bfloat16)  # as the attention reads it
         self.output = None
@@ -94,7 +113,8 @@ class _Int8Block(nn.Module):
 class Int8DoubleAttentionLM(nn.Module):
     """``DoubleAttentionLM`` in int8: ``Int8DoubleAttentionLM(lm)(token_ids)`` gives the logits [B, T, V].
 
-    ``lm`` must be on an sm_100 GPU; its embeddings, norms and dictionaries are shared, not copied.  ``dtype`` is
+    ``lm`` must be on an sm_100 GPU.  What it has learned is copied, all at this moment: a later training step or
+    ``load_state_dict`` of ``lm`` changes nothing here, and all of it is in this module's ``state_dict``.  ``dtype`` is
     the 16-bit type of the activations between the int8 products and of the logits."""
 
     def __init__(self, lm: DoubleAttentionLM, dtype: torch.dtype = torch.bfloat16) -> None:
@@ -105,12 +125,13 @@ class Int8DoubleAttentionLM(nn.Module):
         ops.resolve_backend("auto", weight, dtype)
         with torch.no_grad():
             self.max_sequence_length = lm.max_sequence_length
-            self.token_embedding, self.position_embedding = lm.token_embedding, lm.position_embedding
-            self.final_norm = lm.final_norm
+            self.token_embedding, self.position_embedding = _frozen(lm.token_embedding), _frozen(lm.position_embedding)
+            self.final_norm = _frozen(lm.final_norm)
             stack = lm.stack
             self.blocks = nn.ModuleList(_Int8Block(b, dtype) for b in stack.blocks)
             self.lm_head = Int8Linear(lm.lm_head.weight, None, dtype)
-            self._views = [ops.dictionary_views(b.raw_key, b.raw_value, stack.config.eps, dtype) for b in stack.banks]
+            self.banks = nn.ModuleList(_Bank(ops.dictionary_views(b.raw_key, b.raw_value, stack.config.eps, dtype))
+                                       for b in stack.banks)
             self._bank_of = [min(i // stack.dictionary_group_size, len(stack.banks) - 1) for i in range(len(stack.blocks))]
 
     @torch.no_grad()
@@ -122,7 +143,8 @@ class Int8DoubleAttentionLM(nn.Module):
             raise ValueError(f"sequence length {length} exceeds configured maximum {self.max_sequence_length}")
         positions = torch.arange(length, device=token_ids.device)
         x = (self.token_embedding(token_ids) + self.position_embedding(positions)[None]).float()
+        views = [bank.views() for bank in self.banks]
         pending = None
         for block, bank in zip(self.blocks, self._bank_of):
-            x, pending = block(x, pending, self._views[bank])
+            x, pending = block(x, pending, views[bank])
         return self.lm_head(add_layernorm_int8(x, pending, self.final_norm)[1])
