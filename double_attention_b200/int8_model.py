@@ -23,11 +23,23 @@ _HALF = (torch.float16, torch.bfloat16)
 _ATTENTION_ROWS = 128  # rows (batch times length) below which the attention kernels have no tile
 
 
-class Int8Linear(nn.Module):
+class _FixedTypes(nn.Module):
+    """A module that moves between devices and keeps its tensors' types: ``half()``, ``to(dtype)`` and the like on it
+    or on a module around it leave them, since its products read int8 values with fp32 scales."""
+
+    def _apply(self, fn, recurse: bool = True):
+        def move(t: Tensor) -> Tensor:
+            moved = fn(t)
+            return moved if moved.dtype == t.dtype else t.to(moved.device)
+
+        return super()._apply(move, recurse)
+
+
+class Int8Linear(_FixedTypes):
     """A Linear whose weight is held in int8 with a scale per output channel and whose bias in fp32.
 
     ``forward`` takes int8 rows, or activations that it quantises per token first; with ``gelu`` the output
-    goes through GELU in the product's epilogue."""
+    goes through GELU in the product's epilogue.  ``dtype`` is the output's; ``half()`` and ``to(dtype)`` change no type."""
 
     def __init__(self, weight: Tensor, bias: Tensor | None, dtype: torch.dtype) -> None:
         super().__init__()
@@ -110,12 +122,12 @@ class _Int8Block(nn.Module):
         return x, self.second(self.first(rows, gelu=True))
 
 
-class Int8DoubleAttentionLM(nn.Module):
+class Int8DoubleAttentionLM(_FixedTypes):
     """``DoubleAttentionLM`` in int8: ``Int8DoubleAttentionLM(lm)(token_ids)`` gives the logits [B, T, V].
 
     ``lm`` must be on an sm_100 GPU.  What it has learned is copied, all at this moment: a later training step or
     ``load_state_dict`` of ``lm`` changes nothing here, and all of it is in this module's ``state_dict``.  ``dtype`` is
-    the 16-bit type of the activations between the int8 products and of the logits."""
+    the 16-bit type of the activations between the int8 products and of the logits; no type changes later."""
 
     def __init__(self, lm: DoubleAttentionLM, dtype: torch.dtype = torch.bfloat16) -> None:
         super().__init__()

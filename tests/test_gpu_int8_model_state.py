@@ -60,3 +60,19 @@ def test_served_model_moves_as_a_whole() -> None:
     assert {t.device.type for t in (*served.parameters(), *served.buffers())} == {"cpu"}
     assert torch.cuda.memory_allocated() - before <= logits.numel() * 2 + 1024, "tensors that no move reaches"
     assert torch.equal(served.to("cuda")(ids), logits)
+
+
+@pytest.mark.parametrize("change", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.double(),
+                                    lambda m: m.to("cpu", torch.float16).to("cuda"),
+                                    lambda m: torch.nn.Sequential(m).half()[0]])
+def test_types_stay_as_they_were_made(change) -> None:
+    served, ids = da.Int8DoubleAttentionLM(_lm()), _ids(2, 64)
+    logits, types = served(ids), {name: t.dtype for name, t in served.state_dict().items()}
+    served = change(served)
+    assert {name: t.dtype for name, t in served.state_dict().items()} == types
+    assert torch.equal(served(ids), logits)
+    torch.manual_seed(3)
+    layer = da.Int8Linear(torch.randn(40, 200, device="cuda"), torch.randn(40, device="cuda"), torch.float16)
+    x = torch.randn(5, 200, device="cuda")
+    y = layer(x)
+    assert torch.equal(change(layer)(x), y) and layer.scale.dtype == layer.bias.dtype == torch.float32
