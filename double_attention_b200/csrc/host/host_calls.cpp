@@ -2,13 +2,14 @@
 //
 // A call on one token is over on the device in 2 to 4 us; from Python, checking the tensors, allocating the outputs
 // and converting the arguments takes 8 to 15.  The functions here do the same for tensors that lie as the kernels
-// want them (dense, on the current device, of the right types, nothing requiring a gradient) in 4 to 6 us, launch
-// included, and return None for anything else, which the Python functions then check, copy or refuse.  The
-// kernels and their C entry points are the same either way.
+// want them (dense, on the current device, of the right types, nothing requiring a gradient or carrying a tangent) in
+// 4 to 6 us, launch included, and return None for anything else, which the Python functions then check, copy or
+// refuse.  The kernels and their C entry points are the same either way.
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/slice.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -37,7 +38,7 @@ at::ScalarType type_of(int64_t code) {
 }
 
 // The tensor of an argument; null for None.  Sets `ok` to false for anything else, and where a kernel could not read
-// the tensor in place: off the device, not dense, or part of a gradient.
+// the tensor in place: off the device, not dense, or part of a gradient or of a forward-mode derivative.
 const Tensor* plain(PyObject* o, c10::DeviceIndex device, bool dense, bool* ok) {
   if (o == Py_None) return nullptr;
   if (!THPVariable_Check(o)) {
@@ -46,7 +47,8 @@ const Tensor* plain(PyObject* o, c10::DeviceIndex device, bool dense, bool* ok) 
   }
   const Tensor& t = THPVariable_Unpack(o);
   if (!t.is_cuda() || t.get_device() != device || (dense && !t.is_contiguous()) ||
-      (t.requires_grad() && c10::GradMode::is_enabled()))
+      (t.requires_grad() && c10::GradMode::is_enabled()) ||
+      (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()))
     *ok = false;
   return &t;
 }

@@ -4,7 +4,8 @@ Serving.  A norm leaves its rows in int8 with one scale per token (:func:`add_rm
 :func:`add_layernorm_int8` and their forms without a branch), activations that no norm precedes go
 through :func:`quantize_int8` -- as do the weights, once, with one scale per output channel -- and
 :func:`int8_linear` multiplies the two on the int8 tensor cores, from a single token to long batches.
-These operators have no backward; called on tensors that require a gradient they raise.
+These operators have no backward; called on tensors that require a gradient, or that carry a forward-mode
+tangent, they raise.
 
 Training.  :func:`gelu_checkpoint8` keeps GELU's input in 8 bits (blocks of 32 columns sharing a
 power-of-two scale) in place of the 16-bit tensor, :func:`gelu_checkpoint8_backward` and
@@ -23,6 +24,7 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 from ._lib import ptr
@@ -110,10 +112,15 @@ def _half_code(name: str, what: str, t: Tensor) -> int:
 
 
 def _inference_only(name: str, *tensors: Tensor | None) -> None:
+    """Raises where a result would have to carry a gradient or a forward-mode tangent."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{name} has no backward: call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0 and forward_ad._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative: call it on primal tensors")
 
 
 def _rows(t: Tensor) -> tuple[Tensor, int, int]:
@@ -169,6 +176,7 @@ class Int8Rows(NamedTuple):
             if out is not None:
                 return out
         device = _check_rows(name, self)
+        _inference_only(name, self.scale)
         out = _new(self.values.shape, dtype, self.values.device)
         if out.numel():
             q, rows, stride = _rows(self.values)
@@ -308,9 +316,9 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Tensor | None = None, *, ge
         bias_code = _float_code(name, "a bias", bias)
         if bias.shape != (n,) or bias.get_device() != device:
             raise ValueError(f"{name} takes a bias of shape [{n}] on x's device, got {tuple(bias.shape)} on {bias.device}")
-        _inference_only(name, bias)
         bias = bias.contiguous()
         bias_ptr = bias.data_ptr()
+    _inference_only(name, x.scale, weight.scale, bias)
     out = _new((*x.values.shape[:-1], n), dtype, x.values.device)
     xq, rows, ldx = _rows16(x.values, 16)
     if rows:

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn as nn
 
 import double_attention_b200 as da
@@ -45,3 +46,45 @@ def test_rms_norm_without_an_eps_takes_the_modules_own(dtype) -> None:
             r = (x if rows is not added else x_out).double()
             exact = r / torch.sqrt(r.square().mean(-1, keepdim=True) + 2.0**-23)
             assert (got - exact).abs().le(0.502 * exact.abs().amax(-1, keepdim=True) / 127).all()
+
+
+def _rows_and_weight() -> tuple[da.Int8Rows, da.Int8Rows]:
+    return da.quantize_int8(_randn(4, 32, seed=1)), da.quantize_int8(_randn(64, 32, seed=2))
+
+
+def test_a_scale_that_requires_a_gradient_is_refused() -> None:
+    """The result would have no graph, and the scale would silently get no gradient."""
+    x, w = _rows_and_weight()
+    learned = lambda rows: da.Int8Rows(rows.values, rows.scale.clone().requires_grad_())
+    want, decoded = da.int8_linear(x, w), x.dequantize()
+    for call in (lambda: da.int8_linear(learned(x), w), lambda: da.int8_linear(x, learned(w)),
+                 lambda: learned(x).dequantize(), lambda: learned(x).dequantize(BF16)):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+    with torch.no_grad():
+        assert torch.equal(da.int8_linear(learned(x), learned(w)), want)
+        assert torch.equal(learned(x).dequantize(), decoded)
+
+
+def test_forward_mode_tangents_are_refused() -> None:
+    x32, x16 = _randn(4, 32, seed=1), _randn(4, 32, seed=1, dtype=BF16)
+    rms, layer = nn.RMSNorm(32).cuda().requires_grad_(False), nn.LayerNorm(32).cuda().requires_grad_(False)
+    x, w = _rows_and_weight()
+    kept, bias = da.checkpoint8(x16), _randn(64, seed=3)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: da.quantize_int8(dual(x32)), lambda: da.rmsnorm_int8(dual(x16), rms),
+                     lambda: da.add_layernorm_int8(x32, dual(x32), layer), lambda: da.add_rmsnorm_int8(dual(x32), x32, rms),
+                     lambda: da.int8_linear(da.Int8Rows(x.values, dual(x.scale)), w),
+                     lambda: da.int8_linear(x, da.Int8Rows(w.values, dual(w.scale))),
+                     lambda: da.int8_linear(x, w, dual(bias)), lambda: da.Int8Rows(x.values, dual(x.scale)).dequantize(),
+                     lambda: da.checkpoint8(dual(x16)), lambda: da.gelu_checkpoint8(dual(x16)),
+                     lambda: da.gelu_checkpoint8_backward(dual(x16), kept),
+                     lambda: da.weight_grad_checkpoint8(dual(x16), kept)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call()
+        # primal tensors, and duals where the mode is off, pass
+        assert torch.equal(da.quantize_int8(x32).values, x.values)
+        with forward_ad._set_fwd_grad_enabled(False):
+            assert torch.equal(da.quantize_int8(dual(x32)).values, x.values)
