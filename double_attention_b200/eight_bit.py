@@ -464,6 +464,35 @@ def weight_grad_checkpoint8(dy: Tensor, kept: Checkpoint8, dtype: torch.dtype | 
     return out
 
 
+class _FirstOrder(torch.autograd.Function):
+    """A gradient as it is; differentiated again (it depends on dout, on what was kept and on the weights), it raises."""
+
+    @staticmethod
+    def forward(ctx, grad: Tensor, dout: Tensor, name: str):  # type: ignore[override]
+        ctx.name = name
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):  # type: ignore[override]
+        raise RuntimeError(f"{ctx.name} has no second derivative")
+
+
+def _first_order(name: str):
+    """A Function's backward that runs outside any graph; under create_graph=True its results raise when differentiated."""
+
+    def of(backward):
+        def wrapped(ctx, dout: Tensor):
+            with torch.no_grad():
+                grads = backward(ctx, dout)
+            if not torch.is_grad_enabled():
+                return grads
+            return tuple(None if g is None else _FirstOrder.apply(g.detach().requires_grad_(), dout, name) for g in grads)
+
+        return wrapped
+
+    return of
+
+
 class _LinearCheckpoint8(torch.autograd.Function):
     """y = x W^T (+ b) on the tcgen05 GEMM; x is kept for dW in 8 bits."""
 
@@ -478,6 +507,7 @@ class _LinearCheckpoint8(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_first_order("linear_checkpoint8")
     def backward(ctx, dout: Tensor):  # type: ignore[override]
         w, *kept = ctx.saved_tensors
         shape, dtype, weight_dtype, bias_dtype = ctx.meta
@@ -520,6 +550,7 @@ class _FeedForwardCheckpoint8(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_first_order("feedforward_checkpoint8")
     def backward(ctx, dout: Tensor):  # type: ignore[override]
         w1c, w2c, xv, xe, zv, ze = ctx.saved_tensors
         x_shape, z_shape, dtype = ctx.meta

@@ -88,3 +88,24 @@ def test_forward_mode_tangents_are_refused() -> None:
         assert torch.equal(da.quantize_int8(x32).values, x.values)
         with forward_ad._set_fwd_grad_enabled(False):
             assert torch.equal(da.quantize_int8(dual(x32)).values, x.values)
+
+
+@pytest.mark.parametrize("loss", [lambda y: y.float().sum(), lambda y: y.float().square().sum()])
+@pytest.mark.parametrize("kind", ["linear", "feedforward"])
+def test_gradients_of_checkpointed_layers_raise_when_differentiated(kind: str, loss) -> None:
+    """create_graph=True gives the first derivatives; a penalty on them must not pass as a constant."""
+    torch.manual_seed(1)
+    first, second = nn.Linear(256, 384).cuda().to(BF16), nn.Linear(384, 256).cuda().to(BF16)
+    x = _randn(16, 256, seed=1, dtype=BF16).requires_grad_()
+    params = list(first.parameters()) + (list(second.parameters()) if kind == "feedforward" else [])
+
+    def forward():
+        return loss(da.linear_checkpoint8(x, first) if kind == "linear" else da.feedforward_checkpoint8(x, first, second))
+
+    plain = torch.autograd.grad(forward(), (x, *params))
+    grads = torch.autograd.grad(forward(), (x, *params), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+    for g in grads:
+        assert g.requires_grad and not plain[0].requires_grad
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            g.float().square().sum().backward(retain_graph=True)
