@@ -530,8 +530,8 @@ def _weight_grad_as(dy: Tensor, kept: Checkpoint8, dtype: torch.dtype) -> Tensor
 
 
 class _FeedForwardCheckpoint8(torch.autograd.Function):
-    """second(GELU(first(x))) on the tcgen05 GEMM; x and the pre-activation z are kept in 8 bits, the hidden
-    activation not at all (the backward rebuilds it from z)."""
+    """second(GELU(first(x))) on the tcgen05 GEMM; x (for dW1 alone) and the pre-activation z are kept in 8 bits, the
+    hidden activation not at all (the backward rebuilds it from z)."""
 
     @staticmethod
     def forward(ctx, x2d: Tensor, w1: Tensor, b1: Tensor | None, w2: Tensor, b2: Tensor | None,  # type: ignore[override]
@@ -543,16 +543,16 @@ class _FeedForwardCheckpoint8(torch.autograd.Function):
         h, zk = _checkpoint8("feedforward_checkpoint8", z, True)
         out = torch.empty(m, w2c.shape[0], dtype=dtype, device=x2d.device)
         ops.gemm_ex(h, w2c, False, out, bias=None if b2 is None else b2.to(dtype))
-        xk = _checkpoint8("feedforward_checkpoint8", x2d, False)[1]
-        ctx.save_for_backward(w1c, w2c, xk.values, xk.exponent, zk.values, zk.exponent)
-        ctx.meta = (xk.shape, zk.shape, dtype)
+        xk = _checkpoint8("feedforward_checkpoint8", x2d, False)[1] if ctx.needs_input_grad[1] else None
+        ctx.save_for_backward(w1c, w2c, zk.values, zk.exponent, *(() if xk is None else (xk.values, xk.exponent)))
+        ctx.meta = (tuple(x2d.shape), zk.shape, dtype)
         ctx.param_dtypes = tuple(None if p is None else p.dtype for p in (w1, b1, w2, b2))
         return out
 
     @staticmethod
     @_first_order("feedforward_checkpoint8")
     def backward(ctx, dout: Tensor):  # type: ignore[override]
-        w1c, w2c, xv, xe, zv, ze = ctx.saved_tensors
+        w1c, w2c, zv, ze, *xk = ctx.saved_tensors
         x_shape, z_shape, dtype = ctx.meta
         need, pd = ctx.needs_input_grad, ctx.param_dtypes
         dout = dout.to(dtype).contiguous()
@@ -565,7 +565,7 @@ class _FeedForwardCheckpoint8(torch.autograd.Function):
         if need[4]:
             db2 = ops._bias_grad(dout).to(pd[3])
         if need[1]:
-            dw1 = _weight_grad_as(dz, Checkpoint8(xv, xe, x_shape, dtype), pd[0])  # dW1 = dZ^T . x
+            dw1 = _weight_grad_as(dz, Checkpoint8(*xk, x_shape, dtype), pd[0])  # dW1 = dZ^T . x
         if need[2]:
             db1 = ops._bias_grad(dz).to(pd[1])
         if need[0]:

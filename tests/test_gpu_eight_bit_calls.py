@@ -109,3 +109,22 @@ def test_gradients_of_checkpointed_layers_raise_when_differentiated(kind: str, l
         assert g.requires_grad and not plain[0].requires_grad
         with pytest.raises(RuntimeError, match="no second derivative"):
             g.float().square().sum().backward(retain_graph=True)
+
+
+def test_feedforward_keeps_its_input_for_the_first_weights_gradient_alone() -> None:
+    torch.manual_seed(1)
+    first, second = nn.Linear(256, 384).cuda().to(BF16), nn.Linear(384, 256).cuda().to(BF16)
+    x, dout = _randn(100, 256, seed=1, dtype=BF16).requires_grad_(), _randn(100, 256, seed=2, dtype=BF16)
+
+    def step() -> tuple[int, list]:
+        kept: list = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.numel() * t.element_size()) or t, lambda t: t):
+            y = da.feedforward_checkpoint8(x, first, second)
+        wanted = [x, first.bias, *second.parameters()]
+        return sum(kept), torch.autograd.grad(y, wanted, dout)
+
+    full, grads = step()
+    first.weight.requires_grad_(False)
+    less, same = step()
+    assert full - less == 100 * 256 * 33 // 32
+    assert all(torch.equal(a, b) for a, b in zip(grads, same))
