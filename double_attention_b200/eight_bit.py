@@ -35,7 +35,8 @@ _HALF = (torch.float16, torch.bfloat16)
 
 # The block's feed-forward branch keeps its activations in 8 bits when set (see feedforward_checkpoint8):
 # 4.1 bytes per model-width element and layer instead of 14, for one rounding of the activations that the
-# weight gradients and GELU's derivative read.
+# weight gradients and GELU's derivative read.  A branch whose modules have hooks, or a forward of their own, is
+# called as modules, its activations in 16 bits.
 FEEDFORWARD_CHECKPOINT8 = False
 
 
@@ -578,6 +579,17 @@ def _linear_rows(x: Tensor) -> tuple[Tensor, torch.dtype]:
     dtype = ops._linear_dtype(x)
     x2d = x.reshape(-1, x.shape[-1]).to(dtype)
     return (x2d if x2d.is_contiguous() else x2d.contiguous()), dtype
+
+
+def own_forward(module: torch.nn.Module, kind: type) -> bool:
+    """Whether ``module`` computes something else than ``kind`` does (a subclass, or a forward set on it)."""
+    return type(module).forward is not kind.forward or "forward" in vars(module)
+
+
+def is_plain(module: torch.nn.Module, kind: type) -> bool:
+    """Whether calling ``module`` runs ``kind``'s forward and nothing else: no forward of its own, no hooks."""
+    return not (own_forward(module, kind) or module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                or module._backward_pre_hooks or torch.nn.modules.module._has_any_global_hook())
 
 
 def checkpoint8_supported(x: Tensor, *layers: torch.nn.Linear) -> bool:

@@ -266,12 +266,17 @@ class DoubleAttentionBlock(nn.Module):
         x, normalized_x = ops.add_layernorm(x, branch, self.feedforward_norm)
         return x, self._feedforward_branch(normalized_x, bank, normalized_dictionary)
 
+    def _plain_feedforward(self) -> bool:
+        first, act, second, _ = self.feedforward
+        return (eight_bit.is_plain(self.feedforward, nn.Sequential) and eight_bit.is_plain(first, nn.Linear)
+                and eight_bit.is_plain(act, nn.GELU) and eight_bit.is_plain(second, nn.Linear))
+
     def _feedforward_branch(self, normalized_x: Tensor, bank: SharedDictionaryBank,
                             normalized_dictionary: tuple[Tensor, Tensor] | None) -> Tensor:
         if not self.attention.config.q_dictionary_feedforward:
             first, act, second, drop = self.feedforward
-            if (eight_bit.FEEDFORWARD_CHECKPOINT8 and torch.is_grad_enabled() and act.approximate == "none"
-                    and eight_bit.checkpoint8_supported(normalized_x, first, second)):
+            if (eight_bit.FEEDFORWARD_CHECKPOINT8 and torch.is_grad_enabled() and self._plain_feedforward()
+                    and act.approximate == "none" and eight_bit.checkpoint8_supported(normalized_x, first, second)):
                 return drop(eight_bit.feedforward_checkpoint8(normalized_x, first, second))
             if (ops.BLOCK_LINEAR_ON_TCGEN05 and act.approximate == "none"
                     and ops.feedforward_supported(normalized_x, first, second)):

@@ -1,0 +1,55 @@
+"""Host-side choices of the eight-bit operators that need no GPU."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.nn as nn
+
+from double_attention_b200 import DoubleAttentionBlock, eight_bit, experiment_config
+
+
+class _Adapted(nn.Linear):
+    def forward(self, x):
+        return super().forward(x) + 1
+
+
+@pytest.mark.parametrize("change", ["none", "hook", "pre-hook", "backward hook", "sequence hook", "subclass", "instance",
+                                    "activation", "global hook"])
+def test_a_feed_forward_with_hooks_or_forwards_of_its_own_is_called_as_modules(change: str, monkeypatch) -> None:
+    """With activations kept in 8 bits the branch reads the layers' weights; what its modules do besides has to run."""
+    block = DoubleAttentionBlock(experiment_config("a1"), feedforward_dim=1536)
+    calls: list[str] = []
+    monkeypatch.setattr(eight_bit, "FEEDFORWARD_CHECKPOINT8", True)
+    monkeypatch.setattr(eight_bit, "checkpoint8_supported", lambda x, *layers: True)
+    monkeypatch.setattr(eight_bit, "feedforward_checkpoint8", lambda x, first, second: calls.append("kept") or torch.zeros_like(x))
+    note, handle = lambda *args: calls.append(change), None
+    if change == "hook":
+        block.feedforward[2].register_forward_hook(note)
+    elif change == "pre-hook":
+        block.feedforward[0].register_forward_pre_hook(note)
+    elif change == "backward hook":
+        block.feedforward[0].register_full_backward_hook(note)
+    elif change == "sequence hook":
+        block.feedforward.register_forward_hook(note)
+    elif change == "subclass":
+        block.feedforward[0] = _Adapted(512, 1536)
+    elif change == "instance":
+        block.feedforward[0].forward = lambda x, layer=block.feedforward[0]: nn.functional.linear(x, 2 * layer.weight, layer.bias)
+    elif change == "activation":
+        block.feedforward[1] = nn.ReLU()
+    elif change == "global hook":
+        handle = nn.modules.module.register_module_forward_hook(note)
+    x = torch.randn(2, 3, 512)
+    try:
+        y = block._feedforward_branch(x, None, None)
+        if change == "none":
+            assert calls == ["kept"]
+        else:
+            assert "kept" not in calls
+            assert torch.equal(y, block.feedforward(x))
+            if "hook" in change and "backward" not in change:
+                assert change in calls
+    finally:
+        if handle is not None:
+            handle.remove()
