@@ -16,7 +16,7 @@ import torch
 from torch import Tensor, nn
 
 from . import ops
-from .eight_bit import Int8Rows, add_layernorm_int8, int8_linear, layernorm_int8, quantize_int8
+from .eight_bit import Int8Rows, add_layernorm_int8, int8_linear, layernorm_int8, own_forward, quantize_int8
 from .modules import DoubleAttentionBlock, DoubleAttentionLM
 
 _HALF = (torch.float16, torch.bfloat16)
@@ -54,6 +54,12 @@ class Int8Linear(_FixedTypes):
         return int8_linear(rows, Int8Rows(self.weight, self.scale), self.bias, gelu=gelu, dtype=self.dtype)
 
 
+def _int8(layer: nn.Module, dtype: torch.dtype) -> Int8Linear:
+    if own_forward(layer, nn.Linear):
+        raise NotImplementedError(f"int8 serving covers layers that compute as nn.Linear does, got {layer}")
+    return Int8Linear(layer.weight, layer.bias, dtype)
+
+
 def _frozen(module: nn.Module) -> nn.Module:
     return copy.deepcopy(module).requires_grad_(False)
 
@@ -77,17 +83,14 @@ class _Int8Block(nn.Module):
         if cfg.q_dictionary_feedforward:
             raise NotImplementedError("int8 serving does not cover the Q-dictionary feed-forward")
         first, act, second, _ = block.feedforward
-        if act.approximate != "none":
-            raise NotImplementedError("int8 serving covers the exact form of GELU")
+        if own_forward(act, nn.GELU) or act.approximate != "none":
+            raise NotImplementedError(f"int8 serving covers the exact form of GELU, got {act}")
         self.config = cfg
         self.attention_norm, self.feedforward_norm = _frozen(block.attention_norm), _frozen(block.feedforward_norm)
         self.query_key = Int8Linear(torch.cat((attention.query.weight, attention.key.weight)), None, dtype)
         self.value = Int8Linear(attention.value.weight, attention.value.bias, torch.bfloat16)  # as the attention reads it
-        self.output = None
-        if isinstance(attention.output, nn.Linear):
-            self.output = Int8Linear(attention.output.weight, None, dtype)
-        self.first = Int8Linear(first.weight, first.bias, dtype)
-        self.second = Int8Linear(second.weight, second.bias, dtype)
+        self.output = None if type(attention.output) is nn.Identity else _int8(attention.output, dtype)
+        self.first, self.second = _int8(first, dtype), _int8(second, dtype)
         beta, scales = ops.temperatures(attention.log_beta, attention.log_score_scales)
         self.register_buffer("beta", beta.clone())
         self.register_buffer("scales", scales.clone())
@@ -126,7 +129,8 @@ class Int8DoubleAttentionLM(_FixedTypes):
     """``DoubleAttentionLM`` in int8: ``Int8DoubleAttentionLM(lm)(token_ids)`` gives the logits [B, T, V].
 
     ``lm`` must be on an sm_100 GPU.  What it has learned is copied, all at this moment: a later training step or
-    ``load_state_dict`` of ``lm`` changes nothing here, and all of it is in this module's ``state_dict``.  ``dtype`` is
+    ``load_state_dict`` of ``lm`` changes nothing here, and all of it is in this module's ``state_dict``.  Hooks
+    on ``lm``'s modules do not run here; layers with a forward of their own are refused.  ``dtype`` is
     the 16-bit type of the activations between the int8 products and of the logits; no type changes later."""
 
     def __init__(self, lm: DoubleAttentionLM, dtype: torch.dtype = torch.bfloat16) -> None:
@@ -141,7 +145,7 @@ class Int8DoubleAttentionLM(_FixedTypes):
             self.final_norm = _frozen(lm.final_norm)
             stack = lm.stack
             self.blocks = nn.ModuleList(_Int8Block(b, dtype) for b in stack.blocks)
-            self.lm_head = Int8Linear(lm.lm_head.weight, None, dtype)
+            self.lm_head = _int8(lm.lm_head, dtype)
             self.banks = nn.ModuleList(_Bank(ops.dictionary_views(b.raw_key, b.raw_value, stack.config.eps, dtype))
                                        for b in stack.banks)
             self._bank_of = [min(i // stack.dictionary_group_size, len(stack.banks) - 1) for i in range(len(stack.blocks))]

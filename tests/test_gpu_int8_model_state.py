@@ -76,3 +76,26 @@ def test_types_stay_as_they_were_made(change) -> None:
     x = torch.randn(5, 200, device="cuda")
     y = layer(x)
     assert torch.equal(change(layer)(x), y) and layer.scale.dtype == layer.bias.dtype == torch.float32
+
+
+class _Adapted(torch.nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+@pytest.mark.parametrize("where", ["first", "second", "output", "lm_head"])
+def test_layers_with_a_forward_of_their_own_are_refused(where: str) -> None:
+    """Their weight alone would be served."""
+    lm = _lm()
+    block = lm.stack.blocks[1]
+    old = {"first": block.feedforward[0], "second": block.feedforward[2], "output": block.attention.output,
+           "lm_head": lm.lm_head}[where]
+    for new in (_Adapted(old.in_features, old.out_features, old.bias is not None).cuda(), torch.nn.Sequential(old)):
+        if where == "lm_head":
+            lm.lm_head = new
+        elif where == "output":
+            block.attention.output = new
+        else:
+            block.feedforward[0 if where == "first" else 2] = new
+        with pytest.raises(NotImplementedError, match="nn.Linear"):
+            da.Int8DoubleAttentionLM(lm)
