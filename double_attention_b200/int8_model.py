@@ -157,6 +157,8 @@ class Int8DoubleAttentionLM(_FixedTypes):
         length = token_ids.shape[1]
         if length > self.max_sequence_length:
             raise ValueError(f"sequence length {length} exceeds configured maximum {self.max_sequence_length}")
+        if not token_ids.numel():
+            return self.token_embedding.weight.new_empty(*token_ids.shape, self.lm_head.weight.shape[0], dtype=self.lm_head.dtype)
         positions = torch.arange(length, device=token_ids.device)
         x = (self.token_embedding(token_ids) + self.position_embedding(positions)[None]).float()
         views = [bank.views() for bank in self.banks]

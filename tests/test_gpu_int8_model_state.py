@@ -99,3 +99,10 @@ def test_layers_with_a_forward_of_their_own_are_refused(where: str) -> None:
             block.feedforward[0 if where == "first" else 2] = new
         with pytest.raises(NotImplementedError, match="nn.Linear"):
             da.Int8DoubleAttentionLM(lm)
+
+
+@pytest.mark.parametrize("shape", [(0, 5), (2, 0), (0, 0)])
+def test_no_tokens_give_no_logits(shape: tuple[int, int]) -> None:
+    for dtype in (torch.bfloat16, torch.float16):
+        logits = da.Int8DoubleAttentionLM(_lm(layers=1), dtype)(_ids(*shape))
+        assert logits.shape == (*shape, 512) and logits.dtype == dtype and logits.is_cuda
