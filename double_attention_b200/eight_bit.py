@@ -363,7 +363,7 @@ class Checkpoint8:
 def _check_checkpoint(name: str, c: Checkpoint8) -> int:
     """The device of a checkpoint, checked."""
     values, exponent, shape = c.values, c.exponent, c.shape
-    d = shape[-1]
+    d = shape[-1] if shape else 0
     blocks = -(-d // BLOCK)
     rows = math.prod(shape[:-1])
     if (c.dtype not in _HALF or d < 1 or values.dtype != torch.int8 or exponent.dtype != torch.int8
@@ -438,7 +438,7 @@ def weight_grad_checkpoint8(dy: Tensor, kept: Checkpoint8, dtype: torch.dtype | 
     fp32)."""
     name = "weight_grad_checkpoint8"
     shape, dtype = dy.shape, dtype or dy.dtype
-    if (shape[:-1] == kept.shape[:-1] and dy.dtype == kept.dtype and dtype in (torch.float32, dy.dtype) and dy.is_cuda):
+    if (kept.shape and shape[:-1] == kept.shape[:-1] and dy.dtype == kept.dtype and dtype in (torch.float32, dy.dtype) and dy.is_cuda):
         made = _host().weight_grad(dy, kept.values, kept.exponent, kept.shape[-1], _CODES[dtype],
                                    ops.workspace(dy.device).status)
         if made is not None:

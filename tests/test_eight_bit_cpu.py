@@ -53,3 +53,12 @@ def test_a_feed_forward_with_hooks_or_forwards_of_its_own_is_called_as_modules(c
     finally:
         if handle is not None:
             handle.remove()
+
+
+def test_a_checkpoint_without_dimensions_is_refused() -> None:
+    x = torch.zeros(1, 32, dtype=torch.int8)
+    kept = eight_bit.Checkpoint8(x, x[:, :1], (), torch.bfloat16)
+    for call in (kept.restore, lambda: eight_bit.weight_grad_checkpoint8(torch.zeros(8, dtype=torch.bfloat16), kept),
+                 lambda: eight_bit.gelu_checkpoint8_backward(torch.zeros((), dtype=torch.bfloat16), kept)):
+        with pytest.raises(ValueError, match="takes a checkpoint"):
+            call()

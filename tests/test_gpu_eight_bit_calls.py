@@ -128,3 +128,9 @@ def test_feedforward_keeps_its_input_for_the_first_weights_gradient_alone() -> N
     less, same = step()
     assert full - less == 100 * 256 * 33 // 32
     assert all(torch.equal(a, b) for a, b in zip(grads, same))
+
+
+def test_weight_grad_with_a_checkpoint_without_dimensions_is_refused() -> None:
+    x = torch.zeros(1, 32, dtype=torch.int8, device="cuda")
+    with pytest.raises(ValueError, match="takes a checkpoint"):
+        da.weight_grad_checkpoint8(torch.zeros(8, dtype=BF16, device="cuda"), da.Checkpoint8(x, x[:, :1], (), BF16))
