@@ -4,7 +4,8 @@ Every ``csrc/*.cu`` file is compiled with nvcc for ``sm_100a`` and linked
 into one shared library exporting the C ABI declared in
 ``include/da_b200.h``.  ``csrc/host/host_calls.cpp``, the host side of the
 eight-bit operators' calls, becomes the extension module ``_host_calls.so``
-beside it (the host compiler against this Python and PyTorch).  Object files go to ``_build/`` at the repository
+beside it (the host compiler against this Python and PyTorch); where that cannot be built the library can, and
+the calls do without it.  Object files go to ``_build/`` at the repository
 root; a file is recompiled only when it or a header changed.
 
 Usage: ``python -m double_attention_b200.build [--force] [-j N]``.
@@ -18,6 +19,7 @@ import os
 import shutil
 import subprocess
 import sys
+import warnings
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -126,7 +128,12 @@ def build(force: bool = False, jobs: int | None = None, verbose_ptxas: bool = Fa
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
         os.replace(tmp, LIB_PATH)
-    build_host_calls(force)
+    try:
+        build_host_calls(force)
+    except (RuntimeError, OSError, ImportError) as error:  # no host compiler, no headers of Python or PyTorch
+        HOST_PATH.unlink(missing_ok=True)
+        warnings.warn(f"{HOST_PATH.name} was not built: the eight-bit operators' calls take their Python path, about 8 us "
+                      f"slower each ({error})", RuntimeWarning, stacklevel=2)
     if verbose_ptxas and logs:
         print("\n".join(logs))
     return LIB_PATH

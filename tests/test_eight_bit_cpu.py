@@ -2,11 +2,14 @@
 
 from __future__ import annotations
 
+import sys
+import sysconfig
+
 import pytest
 import torch
 import torch.nn as nn
 
-from double_attention_b200 import DoubleAttentionBlock, eight_bit, experiment_config
+from double_attention_b200 import DoubleAttentionBlock, build, eight_bit, experiment_config
 
 
 class _Adapted(nn.Linear):
@@ -62,3 +65,40 @@ def test_a_checkpoint_without_dimensions_is_refused() -> None:
                  lambda: eight_bit.gelu_checkpoint8_backward(torch.zeros((), dtype=torch.bfloat16), kept)):
         with pytest.raises(ValueError, match="takes a checkpoint"):
             call()
+
+
+def _copy_of_the_package(tmp_path, monkeypatch) -> None:
+    """The build's paths moved to ``tmp_path``, with a library that is up to date (no nvcc run)."""
+    for name in ("libda_b200.so", build.HOST_PATH.name):
+        (tmp_path / name).write_bytes(b"")
+    monkeypatch.setattr(build, "PACKAGE_DIR", tmp_path)
+    monkeypatch.setattr(build, "BUILD_DIR", tmp_path)
+    monkeypatch.setattr(build, "LIB_PATH", tmp_path / "libda_b200.so")
+    monkeypatch.setattr(build, "HOST_PATH", tmp_path / build.HOST_PATH.name)
+    monkeypatch.setattr(build, "_needs_build", lambda *args: False)
+    for source in build.CSRC.glob("*.cu"):
+        (tmp_path / f"{source.stem}.o").write_bytes(b"")
+    (tmp_path / "libda_b200.so").write_bytes(b"library")  # newer than its objects
+
+
+@pytest.mark.parametrize("missing", ["compiler", "headers"])
+def test_the_library_builds_without_the_host_extension(missing: str, tmp_path, monkeypatch) -> None:
+    _copy_of_the_package(tmp_path, monkeypatch)
+    build.HOST_PATH.unlink()
+    if missing == "compiler":
+        monkeypatch.setenv("CXX", str(tmp_path / "no-such-compiler"))
+    else:
+        paths = dict(sysconfig.get_paths(), include=str(tmp_path))
+        monkeypatch.setattr(sysconfig, "get_paths", lambda: paths)
+    with pytest.warns(RuntimeWarning, match="was not built"):
+        assert build.build() == build.LIB_PATH
+    assert build.LIB_PATH.read_bytes() == b"library" and not build.HOST_PATH.exists()
+
+
+def test_calls_do_without_the_host_extension(monkeypatch) -> None:
+    monkeypatch.setattr(eight_bit, "_host_module", None)
+    monkeypatch.setitem(sys.modules, "double_attention_b200._host_calls", None)  # (importing it raises ImportError)
+    monkeypatch.delattr(sys.modules["double_attention_b200"], "_host_calls", raising=False)
+    with pytest.warns(RuntimeWarning, match="cannot be used"):
+        host = eight_bit._host()
+    assert host.linear() is None and host.norm(1, 2) is None and eight_bit._host() is host
