@@ -3,7 +3,7 @@
 Every ``csrc/*.cu`` file is compiled with nvcc for ``sm_100a`` and linked
 into one shared library exporting the C ABI declared in
 ``include/da_b200.h``.  ``csrc/host/host_calls.cpp``, the host side of the
-eight-bit operators' calls, becomes the extension module ``_host_calls.so``
+eight-bit operators' calls, becomes the extension module ``_host_calls``
 beside it (the host compiler against this Python and PyTorch); where that cannot be built the library can, and
 the calls do without it.  Object files go to ``_build/`` at the repository
 root; a file is recompiled only when it or a header changed.
@@ -15,10 +15,12 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures
+import hashlib
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import warnings
 from pathlib import Path
 
@@ -72,31 +74,35 @@ def _compile(nvcc: str, src: Path, obj: Path, verbose_ptxas: bool) -> tuple[Path
 
 
 HOST_SRC = CSRC / "host" / "host_calls.cpp"
-HOST_PATH = PACKAGE_DIR / "_host_calls.so"
+# (the name carries the interpreter's ABI: another one does not find the file, and builds its own)
+HOST_PATH = PACKAGE_DIR / f"_host_calls{sysconfig.get_config_var('EXT_SUFFIX')}"
 
 
 def build_host_calls(force: bool = False) -> Path:
-    """Compile the ``_host_calls`` extension module when its source, the ABI header or PyTorch changed."""
-    import sysconfig
-
+    """Compile the ``_host_calls`` extension module unless it was built from the same source, headers, PyTorch and
+    command."""
     import torch
 
     include, root = sysconfig.get_paths()["include"], Path(torch.__file__).resolve().parent
-    newest = max(p.stat().st_mtime for p in (HOST_SRC, *INCLUDE.glob("*.h"), root / "version.py"))
-    if HOST_PATH.exists() and HOST_PATH.stat().st_mtime > newest and not force:
-        return HOST_PATH
     cuda = Path(nvcc_path()).resolve().parent.parent
     system = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include", Path(include)]
-    tmp = HOST_PATH.with_suffix(".so.tmp")
+    tmp, stamp = HOST_PATH.with_suffix(".tmp"), BUILD_DIR / f"{HOST_PATH.name}.stamp"
     cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DDA_TORCH_VERSION="{torch.__version__}"', f"-I{INCLUDE}",
            *(a for p in system for a in ("-isystem", str(p))), str(HOST_SRC), "-o", str(tmp), f"-L{root / 'lib'}",
            "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", f"-L{PACKAGE_DIR}",
            f"-l:{LIB_PATH.name}", "-Wl,-rpath,$ORIGIN"]
+    made_of = hashlib.sha256("\0".join(cmd).encode())
+    for source in (HOST_SRC, *sorted(INCLUDE.glob("*.h"))):
+        made_of.update(source.read_bytes())
+    if HOST_PATH.exists() and stamp.exists() and stamp.read_text() == made_of.hexdigest() and not force:
+        return HOST_PATH
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"the host compiler failed for {HOST_SRC.name}:\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, HOST_PATH)
+    stamp.write_text(made_of.hexdigest())
     return HOST_PATH
 
 

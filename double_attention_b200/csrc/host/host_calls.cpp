@@ -289,4 +289,11 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host_calls", nullptr, -1, g_met
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host_calls(void) { return PyModule_Create(&g_module); }
+PyMODINIT_FUNC PyInit__host_calls(void) {
+  PyObject* m = PyModule_Create(&g_module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", DA_TORCH_VERSION) < 0) {  // whose C++ interface it was built for
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -61,6 +61,9 @@ def _host():
         _lib.lib()
         try:
             from . import _host_calls
+            built_for = getattr(_host_calls, "torch_version", "of unknown version")
+            if built_for != torch.__version__:
+                raise ImportError(f"built for PyTorch {built_for}, this is {torch.__version__}")
         except ImportError as error:
             warnings.warn(f"the _host_calls extension cannot be used ({error}): eight-bit calls take about 8 us longer on the "
                           "host; `python -m double_attention_b200.build` builds it", RuntimeWarning, stacklevel=3)

@@ -102,3 +102,45 @@ def test_calls_do_without_the_host_extension(monkeypatch) -> None:
     with pytest.warns(RuntimeWarning, match="cannot be used"):
         host = eight_bit._host()
     assert host.linear() is None and host.norm(1, 2) is None and eight_bit._host() is host
+
+
+def test_the_host_extension_is_rebuilt_for_another_interpreter_pytorch_source_or_command(tmp_path, monkeypatch) -> None:
+    _copy_of_the_package(tmp_path, monkeypatch)
+    assert build.HOST_PATH.name.endswith(sysconfig.get_config_var("EXT_SUFFIX"))  # as this interpreter looks for it
+    runs: list[list[str]] = []
+
+    def compiler(cmd, **kwargs):
+        runs.append(cmd)
+        build.Path(cmd[cmd.index("-o") + 1]).write_bytes(b"extension")
+        return type("Done", (), {"returncode": 0})()
+
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    source = tmp_path / "host_calls.cpp"
+    source.write_text("one")
+    monkeypatch.setattr(build, "HOST_SRC", source)
+    build.HOST_PATH.write_bytes(b"of unknown origin")
+
+    def runs_of_a_build() -> int:
+        runs.clear()
+        assert build.build_host_calls() == build.HOST_PATH
+        return len(runs)
+
+    assert runs_of_a_build() == 1 and build.HOST_PATH.read_bytes() == b"extension"
+    assert runs_of_a_build() == 0
+    source.write_text("two")
+    assert runs_of_a_build() == 1 and runs_of_a_build() == 0
+    monkeypatch.setattr(torch, "__version__", "0.0")  # an older one than was there
+    assert runs_of_a_build() == 1 and runs_of_a_build() == 0
+    monkeypatch.setenv("CXX", "another")
+    assert runs_of_a_build() == 1 and runs_of_a_build() == 0
+    build.HOST_PATH.unlink()
+    assert runs_of_a_build() == 1
+
+
+def test_an_extension_built_for_another_pytorch_is_not_called(monkeypatch) -> None:
+    from double_attention_b200 import _host_calls
+
+    monkeypatch.setattr(eight_bit, "_host_module", None)
+    monkeypatch.setattr(_host_calls, "torch_version", "0.0")
+    with pytest.warns(RuntimeWarning, match="built for PyTorch 0.0"):
+        assert eight_bit._host() is not _host_calls
