@@ -22,7 +22,7 @@ struct Params {
   int64_t lda, ldb, ldc;
   int M, N, K, bias_dtype, c_dtype, gelu;
   int turns;  // the pair kernel's epilogue warps take turns
-  int tma_c;  // C's rows take TMA stores (16-byte aligned base and stride)
+  int tma_c;  // C's rows take TMA stores (base, stride and width in whole 16-byte words)
   int* status;
   Div31 per_group;  // the pair kernel: tiles in a group of 8 rows of tiles
 };
@@ -598,7 +598,8 @@ extern "C" int da_gemm_i8(const int8_t* A, int64_t lda, const float* a_scale, co
   // / 56.2; 32768 x 1024 x 1536 49.2 / 46.8, 53.0 / 60.1; 32768 x 1536 x 1536 with GELU 72.5 / 71.7; 8192 x 4096 x 4096 93.8
   // / 88.8.
   const int turns = K >= (gelu ? 1536 : 1024);
-  const int tma_c = reinterpret_cast<uintptr_t>(C) % 16 == 0 && ldc * elem % 16 == 0;
+  // A TMA store writes whole 16-byte words: where a row of C ends inside one, it would write into what lies behind.
+  const int tma_c = reinterpret_cast<uintptr_t>(C) % 16 == 0 && ldc * elem % 16 == 0 && N * elem % 16 == 0;
   const i8::Params p{A,      B,      a_scale, b_scale,    bias,    C,    lda,   ldb,   ldc,
                      (int)M, (int)N, (int)K,  bias_dtype, c_dtype, gelu, turns, tma_c, status,
                      Div31((uint32_t)((N + 255) / 256 * 8))};
