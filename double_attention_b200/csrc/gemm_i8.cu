@@ -363,8 +363,9 @@ int dispatch_pair(const Params& p, cudaStream_t st) {
 // cluster's sums for its share of the tokens through distributed shared memory (exact, so in any order) and
 // stores them.
 //
-// Bound: latency.  1 x 512 x 1536 with GELU in 3.7 us, 1 x 4096 x 4096 in 5.8 us (2.9 TB/s of weights), 24 x 4096 x 4096 in
-// 6.5 us, 16 x 8192 x 8192 in 15 us (4.5 TB/s).
+// Bound: latency.  1 x 512 x 1536 with GELU in 3.7 us.  Over 24 layers' weights in turn, which L2 does not hold:
+// 1 x 4096 x 4096 in 6.9 us (2.4 TB/s of weights), 24 x 4096 x 4096 in 7.7 us, 128 x 4096 x 4096 in 10.4 us, 16 x 8192 x 8192 in
+// 14.7 us (4.6 TB/s).  With weights that stay in L2 5.5, 6.1 and 9.1 us for the first three.
 template <int kTn>
 struct Few {
   static constexpr int kStageBytes = (128 + kTn) * 128;
@@ -554,7 +555,7 @@ int dispatch_few(const Params& p, int splits, cudaStream_t st) {
 }
 
 // The few-token kernel where every tile gets two CTAs or more, or there are at most 256 tokens and its tiles fit on
-// the SMs at once.  Measured (us, few against pair): 1 x 4096 x 4096 5.8 / 14.0, 128 x 4096 x 4096 9.6 / 14.7,
+// the SMs at once.  Measured (us, few against pair, weights in L2): 1 x 4096 x 4096 5.8 / 14.0, 128 x 4096 x 4096 9.6 / 14.7,
 // 256 x 4096 x 4096 12.7 / 14.9, 512 x 4096 x 4096 17.4 / 15.9, 1024 x 512 x 1536 12.8 / 10.0.
 int dispatch(const Params& p, cudaStream_t st) {
   const int tn = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;

@@ -14,7 +14,10 @@
 // Bound: HBM.  One pass; a row stays in registers between its reductions (a warp up to 1024 columns, a block of up to
 // 512 threads up to 16384; wider rows are read again, mostly from L2).  Measured: 262144 x 512 from an fp32 residual and a
 // bf16 branch in 215 us (11 bytes an element, 6.9 TB/s), 8192 x 4096 quantised from bf16 in 16 us (6.3 TB/s), one row of
-// 512 in 2.1 us; odd widths: 100003 x 501 in 94 us (5.8 TB/s).
+// 512 in 2.1 us; odd widths: 100003 x 501 in 94 us (5.8 TB/s).  LayerNorm: the same 214 us at 262144 x 512 and 2.4 us for
+// one row; rows over several warps wait at two barriers for each of its three reductions, where the RMS norm has one
+// barrier: 16384 x 4096 with a branch in 76 us (bf16) and 123 us (fp32 residual) against 72 and 112, and without one, with
+// less to read under the waits, 64 against 39 (bf16), 16384 x 8192 from fp16 129 against 80.
 #include "common.cuh"
 #include "host_util.h"
 #include "vec8.cuh"
@@ -414,7 +417,9 @@ __global__ void __launch_bounds__(kT == 32 ? 256 : kT ? kT : 512) norm_int8_kern
 }
 
 // Any strides, alignments and mixtures of dtypes: one block per row, an element a load (each thread reads back only
-// what it wrote itself); rows wider than the register variants hold come here too.
+// what it wrote itself); rows wider than the register variants hold come here too, and 16-bit residuals with a branch of
+// another type.  Three passes of single elements: 16384 x 4096, bf16 residual and fp16 branch, in 357 us (both bf16: 72),
+// 4096 x 20000 from bf16 in 223 us (16384 columns, in registers: 53).
 template <int kT>
 __global__ void __launch_bounds__(kT) norm_int8_any_kernel(const NormArgs p) {
   __shared__ float red[32];

@@ -36,15 +36,17 @@ _HALF = (torch.float16, torch.bfloat16)
 
 # The block's feed-forward branch keeps its activations in 8 bits when set (see feedforward_checkpoint8):
 # 4.1 bytes per model-width element and layer instead of 14, for one rounding of the activations that the
-# weight gradients and GELU's derivative read.  A branch whose modules have hooks, or a forward of their own, is
-# called as modules, its activations in 16 bits.
+# weight gradients and GELU's derivative read.  A training step of the 6-layer a1 model at 256 x 1024 tokens peaks at
+# 22.6 GiB instead of 30.0 and takes 84 ms instead of 80.6 (its products run on this library's GEMM, which without
+# checkpoints takes 88).  A branch whose modules have hooks, or a forward of their own, is called as modules, its
+# activations in 16 bits.
 FEEDFORWARD_CHECKPOINT8 = False
 
 
 # ----------------------------------------------------------------------------- helpers
 # A call on a few rows is over on the device in 2 to 4 us.  Tensors that lie as the kernels want them go through the
 # _host_calls extension, which checks, allocates and launches in 4 to 6 us on the host; it answers None for anything
-# else, and the functions here then copy, find the device or say what is wrong (10 to 15 us).
+# else, and the functions here then copy, find the device or say what is wrong (8 to 16 us).
 _host_module = None
 
 

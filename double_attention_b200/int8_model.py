@@ -6,6 +6,10 @@ and the feed-forward layers multiply int8 rows, the route and the outer attentio
 16-bit kernels.  Per layer that is five int8 products (Q and K together, V, output, two of the feed-forward)
 between two fused norms.  Inference only; the model it is built from is left as it is, and nothing that happens to it
 later reaches the served one.
+
+Measured, 6 layers of a1, feed-forward 1536, vocabulary 2048 (the 16-bit model under autocast beside it): 16 x 1024
+tokens in 1.44 ms (2.39), replayed from a CUDA graph 1.34 (1.62); 64 x 1024 4.65 (5.89); 1 x 128 0.82 (2.38), from a graph
+0.44 (0.48); a single token 1.0, from a graph 0.32.
 """
 
 from __future__ import annotations

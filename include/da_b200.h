@@ -495,9 +495,12 @@ DA_API int da_add_layernorm_bwd(const void* dy, int dy_dtype, const float* d_res
  * largest |y| (kind 1: |r w|) is at most 1e-36 becomes q = 0, scale = 0; a row
  * holding a NaN or an infinity gets a NaN for its scale (and any q).  x, branch, weight and bias
  * in any of DA_F16 / DA_BF16 / DA_F32, row strides ldx, ldb, ldo, ldq in elements, any
- * alignment (rows that start on 16 bytes with D a multiple of 8, and dense tensors of any
- * D with ldq at least D rounded up to 8, take vector accesses; bytes of a q row past D are
- * then written too). */
+ * alignment.  Vector accesses are taken for rows that start on 16 bytes with D a multiple
+ * of 8, and for dense tensors of any D with ldq at least D rounded up to 8 (bytes of a q
+ * row past D, up to that multiple, are then written too), where D is at most 16384 (16377
+ * where it is no multiple of 8) and the branch is absent, of x's type, or beside an fp32 x.
+ * Anything else runs an element at a time, several times slower: wider rows, other strides
+ * and alignments, and an fp16 or bf16 x with a branch of another type. */
 DA_API int da_norm_int8(const void* x, int x_dtype, int64_t ldx, const void* branch, int branch_dtype, int64_t ldb,
                         const void* weight, int weight_dtype, const void* bias, int bias_dtype, int kind,
                         int64_t rows, int64_t D, float eps, void* x_out, int64_t ldo, int8_t* q, int64_t ldq,

@@ -3,7 +3,7 @@
 Tolerances, fixed from the formulas: an int8 row is within half a step of the exact value (plus the fp32
 error of the row's factors, below 2e-3 steps); an int8 product is exact before its scaling, so only the
 four fp32 roundings behind it and the output's own rounding remain; GELU's distribution function carries
-Hastings' 1.5e-7 / 2 and a few fp32 roundings, below 4e-7; a checkpoint's values are exact.
+its polynomial's 1.4e-7 and a few fp32 roundings, below 4e-7; a checkpoint's values are exact.
 """
 
 from __future__ import annotations
