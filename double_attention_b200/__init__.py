@@ -35,6 +35,7 @@ from .modules import (
     SharedDictionaryBank,
 )
 from .ops import assemble_score_maps, dictionary_route, routed_attention
+from .paged import PagedBatch, append_paged, routed_attention_paged
 
 __all__ = [
     "Checkpoint8",
@@ -47,10 +48,12 @@ __all__ = [
     "Int8DoubleAttentionLM",
     "Int8Linear",
     "Int8Rows",
+    "PagedBatch",
     "SharedDictionaryAttention",
     "SharedDictionaryBank",
     "add_layernorm_int8",
     "add_rmsnorm_int8",
+    "append_paged",
     "assemble_score_maps",
     "checkpoint8",
     "dictionary_route",
@@ -65,5 +68,6 @@ __all__ = [
     "quantize_int8",
     "rmsnorm_int8",
     "routed_attention",
+    "routed_attention_paged",
     "weight_grad_checkpoint8",
 ]

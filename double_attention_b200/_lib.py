@@ -97,6 +97,11 @@ SIGNATURES: dict[str, list] = {
     "da_checkpoint8_gelu_bwd": [_p, _i32, _i64, _p, _p, _i64, _i64, _p, _i64, _p, _i64, _p],
     "da_checkpoint8_wgrad_workspace_elems": [_i64, _i64, _i64],  # returns int64 (set below)
     "da_checkpoint8_wgrad": [_p, _i32, _i64, _p, _p, _i64, _i64, _i64, _p, _i32, _i64, _p, _i64, _p, _p],
+    "da_paged_append": [_p, _i32, _i64, _i64, _p, _i32, _i64, _i64, _p, _p, _i32, _i64, _i32, _i32, _i32, _i32, _p, _i64, _i64,
+                        _p, _p, _i64, _p, _p],
+    "da_paged_attn_workspace_size": [_i64, _i64, _i64, _i32, _i64, _i32, _i32, _i32, _i32],  # returns int64 (set below)
+    "da_paged_attn": [_p, _i64, _i64, _i64, _p, _p, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _p, _i64, _i64, _p, _p, _i64,
+                      _i64, _p, _p, _i32, _i32, _p, _p, _i64, _p, _p],
 }
 
 _lock = threading.Lock()
@@ -142,6 +147,7 @@ def lib() -> ctypes.CDLL:
             handle.da_gemm_splitk_workspace_elems.restype = ctypes.c_int64
             handle.da_col_sum_workspace_elems.restype = ctypes.c_int64
             handle.da_checkpoint8_wgrad_workspace_elems.restype = ctypes.c_int64
+            handle.da_paged_attn_workspace_size.restype = ctypes.c_int64
             handle.da_kernel_launches.argtypes = []
             handle.da_kernel_launches.restype = ctypes.c_uint64
             _lib = handle

@@ -27,6 +27,7 @@ enum : int {
   DA_DEV_TIMEOUT = 1,        // a bounded wait ran out
   DA_DEV_ROW_OVERFLOW = 2,   // more low-mass rows than the repair list holds
   DA_DEV_LOW_MASS = 4,       // a softmax row's largest term fell below 2^-100
+  DA_DEV_BAD_PAGE = 8,       // a page table led outside its cache
 };
 
 constexpr unsigned long long kWaitTimeoutNs = 2000000000ull;  // 2 s per wait
@@ -61,6 +62,18 @@ DA_DEV void cluster_sync() {
 
 DA_DEV void named_bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(threads) : "memory");
+}
+
+// named_bar_sync that tells every thread whether any of them brought `v`.
+DA_DEV bool named_bar_or(int id, int threads, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r) : "r"(id), "r"(threads), "r"((uint32_t)v) : "memory");
+  return r != 0;
 }
 
 // ---------------------------------------------------------------- mbarrier
@@ -209,6 +222,14 @@ DA_DEV void tma_load_2d(const void* tmap, uint64_t* bar, void* dst, int x, int y
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4}], [%2];"
       :: "r"(smem_u32(dst)), "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
+}
+
+// 3-D tiled load (see make_tmap_blocks) into this CTA's shared memory, completion on a barrier of this CTA.
+DA_DEV void tma_load_3d(const void* tmap, uint64_t* bar, void* dst, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];"
+      :: "r"(smem_u32(dst)), "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
 // Warms L2 with one 2-D tile of this GPU's global memory (no shared memory,

@@ -1,0 +1,734 @@
+// Outer routed attention of a few new tokens a sequence over a paged cache (decoding, drafts):
+//
+//   Y_t = sum_s alpha_s softmax_{j <= p_t}(gamma_s <q_{s,t}, k_{s,j}>) V_j,   p_t = lengths[b] + t.
+//
+// Such a call reads each sequence's keys and values once and computes little: bytes bound it.  The (map, token) pairs
+// of up to 16 / maps tokens of a sequence are the 16 rows of one matrix product: row (s, t) holds q's branches of map
+// s and zeros in the other branches' columns, so all maps' scores come from one pass over the H R columns of a key
+// tile, and all rows share the value tile.  Each row keeps its own running maximum, sum and output; the maps are
+// mixed once, at the end, which needs no second pass over the keys for their sums.
+//
+// Work: the (sequence, 16 rows) jobs' tiles of 32 keys form one flat list, which the CTAs share evenly, whatever the
+// sequences' lengths.  A job that lies in one CTA is finished there; the pieces of one that does not leave their
+// unnormalised rows in the workspace, and combine_kernel joins them in order.  Which CTA has which piece follows from
+// the lengths alone, so both kernels work it out from the device's own data and the host needs no lengths.
+//
+// A tile: one thread brings the keys and values of 32 positions by TMA (one box each where a page has 32 positions),
+// several tiles ahead; eight warps split the H R columns of the score product and the D columns of the output.
+#include <math.h>
+
+#include "host_util.h"
+#include "paged.cuh"
+
+namespace da {
+namespace paged {
+
+constexpr int kKeys = 32;      // positions a tile
+constexpr int kWarps = 8;      // computing warps; one more brings the tiles
+constexpr int kMaxStages = 8;
+constexpr int kRedPitch = 36;  // floats a row of partial scores
+constexpr int kPPitch = 40;    // 16-bit weights a row
+
+struct FewParams {
+  Cache c;
+  const void* q;
+  int64_t q_branch, q_row;  // strides in elements
+  const float *scales, *weights;
+  void* y;
+  float* part;  // [2 * CTAs][16][D] rows, then [2 * CTAs][2][16] maxima (log2) and sums
+  int* status;
+  int H, R, D, maps, group, lanes;  // lanes: maps rounded up to a power of two; 16 / lanes tokens a job
+  int few_most;                     // sequences with more new tokens are another kernel's
+  int few_rows;                     // combine_kernel's rows a sequence
+  int stages, stage_bytes, key_bytes, brow;
+  int ctas;
+  int per_map, zero_rest;
+};
+
+// Tiles of one job, and of all jobs, of sequence s.
+DA_DEV int job_tiles(const Cache& c, const Sequence& s) { return (int)((positions(c, s) + kKeys - 1) / kKeys); }
+DA_DEV int64_t sequence_tiles(const FewParams& p, const Sequence& s) {
+  if (s.n == 0 || s.n > p.few_most) return 0;
+  const int tokens = 16 / p.lanes;
+  return (int64_t)((s.n + tokens - 1) / tokens) * job_tiles(p.c, s);
+}
+
+// Sum over `threads` threads' values (all of them call it; every one gets it).  `buf` holds 32 entries.
+template <int threads>
+DA_DEV int64_t block_sum(int64_t v, int64_t* buf) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) buf[threadIdx.x / 32] = v;
+  __syncthreads();
+  int64_t t = 0;
+#pragma unroll
+  for (int i = 0; i < threads / 32; ++i) t += buf[i];
+  return t;
+}
+
+// D += A B for a 16 x 16 (row) and a 16 x 8 (column) matrix.
+template <typename T>
+DA_DEV void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+DA_DEV void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+DA_DEV void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+// The pieces of one CTA, in order.  Every thread of the CTA walks them alike.
+struct Walk {
+  int b;
+  int64_t off, left;  // tile of sequence b's list, tiles still to do
+};
+
+struct Piece {
+  Sequence s;
+  int b, job, t0, t1;  // tiles [t0, t1) of the job's
+  int tiles;           // of the whole job
+};
+
+DA_DEV bool next_piece(const FewParams& p, Walk& w, Piece& x) {
+  while (w.left > 0 && w.b < p.c.B) {
+    x.s = sequence(p.c, w.b);
+    const int64_t all = sequence_tiles(p, x.s);
+    if (w.off < all) {
+      x.b = w.b;
+      x.tiles = job_tiles(p.c, x.s);
+      x.job = (int)(w.off / x.tiles);
+      x.t0 = (int)(w.off - (int64_t)x.job * x.tiles);
+      x.t1 = (int)(x.t0 + w.left < x.tiles ? x.t0 + w.left : x.tiles);
+      w.left -= x.t1 - x.t0;
+      w.off += x.t1 - x.t0;
+      return true;
+    }
+    ++w.b;
+    w.off = 0;
+  }
+  return false;
+}
+
+// Positions that some row of the job sees.
+DA_DEV int64_t job_end(const Cache& c, const Sequence& s, int job, int tokens) {
+  const int last = min(s.n, (job + 1) * tokens);
+  const int64_t e = s.held + last;
+  return e < c.capacity ? e : c.capacity;
+}
+
+// kNT: n-tiles of 8 value columns a warp (D = 64 kNT).
+template <typename T, int kNT>
+__global__ void __launch_bounds__(32 * (kWarps + 1), 2) few_kernel(const __grid_constant__ CUtensorMap tk,
+                                                                  const __grid_constant__ CUtensorMap tv,
+                                                                  const FewParams p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* red = reinterpret_cast<float*>(smem + p.stages * p.stage_bytes);    // [8][16][kRedPitch]
+  uint16_t* weight = reinterpret_cast<uint16_t*>(red + kWarps * 16 * kRedPitch);  // [16][kPPitch]
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages];
+  __shared__ int bad[kMaxStages];  // the tile's pages are not all in the cache
+  __shared__ float rescale[16], row_max[16], row_sum[16];
+  __shared__ int64_t buf[32], start_off;
+  __shared__ int start_b, abort_flag;
+
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kWarps);
+    }
+    fence_mbar_init();
+  }
+  grid_dependency_wait();
+  grid_launch_dependents();
+
+  // ---- this CTA's share of the flat list of tiles
+  constexpr int kThreads = 32 * (kWarps + 1);
+  int64_t mine = 0;
+  for (int b = tid; b < p.c.B; b += kThreads) mine += sequence_tiles(p, sequence(p.c, b));
+  const int64_t total = block_sum<kThreads>(mine, buf);
+  if (p.zero_rest) {
+    const int64_t used = clamp64(p.c.starts[p.c.B], 0, p.c.tokens);
+    const int64_t words = (int64_t)(p.per_map ? p.maps : 1) * p.D / 8;
+    uint4* rest = static_cast<uint4*>(p.y) + used * words;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < (p.c.tokens - used) * words; i += (int64_t)gridDim.x * kThreads)
+      rest[i] = make_uint4(0, 0, 0, 0);
+  }
+  const int64_t share = (total + p.ctas - 1) / p.ctas;
+  const int64_t begin = (int64_t)blockIdx.x * share;
+  if (begin >= total) return;
+  {
+    int64_t before = 0;  // tiles of the sequences before this round's
+    for (int base = 0;; base += kThreads) {
+      const int b = base + tid;
+      const int64_t v = b < p.c.B ? sequence_tiles(p, sequence(p.c, b)) : 0;
+      int64_t inc = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
+      }
+      __syncthreads();
+      if (lane == 31) buf[warp] = inc;
+      __syncthreads();
+      int64_t at = before + inc - v, all = 0;
+#pragma unroll
+      for (int i = 0; i <= kWarps; ++i) {
+        if (i < warp) at += buf[i];
+        all += buf[i];
+      }
+      if (begin >= at && begin < at + v) {
+        start_b = b;
+        start_off = begin - at;
+      }
+      before += all;
+      if (begin < before) break;  // (total > begin: found at the latest with the last sequence)
+    }
+    __syncthreads();
+  }
+  Walk walk{start_b, start_off, share < total - begin ? share : total - begin};
+  Abort ab{&abort_flag, p.status};
+  const int tokens = 16 / p.lanes;
+  Piece x;
+  int it = 0;  // tiles so far: stage it % stages
+
+  if (warp == kWarps) {
+    // ---------------------------------------------------------------- brings the tiles
+    if (lane == 0) {
+      prefetch_tmap(&tk);
+      prefetch_tmap(&tv);
+    }
+    bool ok = true;
+    while (ok && next_piece(p, walk, x)) {
+      const int64_t end = job_end(p.c, x.s, x.job, tokens);
+      const int t1 = min(x.t1, (int)((end + kKeys - 1) / kKeys));
+      const int* row = p.c.table + x.b * p.c.table_stride;
+      const int boxes = kKeys / p.brow;
+      int cached = -1, entry = 0;  // this lane's entry of the 32 pages from `cached` on
+      for (int t = x.t0; ok && t < t1; ++t, ++it) {
+        const int st = it % p.stages;
+        if (lane == 0) ok = mbar_wait(&empty[st], ((it / p.stages) & 1u) ^ 1u, ab, 61);
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        if (!ok) break;
+        // pages of the boxes (a box lies in one page); positions past `end` in no page are not fetched
+        const int64_t pos = (int64_t)t * kKeys;
+        const int first = (int)(pos >> p.c.page_shift);
+        if (cached < 0 || first >= cached + 31) {
+          cached = first;
+          const int64_t i = (int64_t)first + lane;
+          entry = i * p.c.page < p.c.capacity ? row[i] : -1;
+        }
+        int good = 0, wrong = 0, slot[2] = {-1, -1};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int64_t at = pos + u * p.brow;
+          if (u >= boxes || at >= end) continue;
+          const int page = __shfl_sync(0xffffffffu, entry, (int)(at >> p.c.page_shift) - cached);
+          if (page < 0 || page >= p.c.pages) {
+            wrong = 1;
+          } else {
+            slot[u] = (page << p.c.page_shift) + (int)(at & (p.c.page - 1));
+            ++good;
+          }
+        }
+        if (lane == 0) {
+          bad[st] = wrong;
+          if (wrong) atomicOr(p.status, DA_DEV_BAD_PAGE);
+          mbar_arrive_expect_tx(&full[st], good * p.brow * 2 * (p.H * p.R + p.D));
+          uint8_t* base = smem + st * p.stage_bytes;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if (slot[u] < 0) continue;
+            tma_load_3d(&tk, &full[st], base + u * p.brow * 2 * p.H * p.R, 0, slot[u], 0);
+            tma_load_3d(&tv, &full[st], base + p.key_bytes + u * p.brow * 2 * p.D, 0, slot[u], 0);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    // the last tiles' loads land before the CTA's shared memory is given back
+    if (lane == 0)
+      for (int i = it > p.stages ? it - p.stages : 0; i < it; ++i) mbar_wait_drain(&full[i % p.stages], (i / p.stages) & 1u);
+    return;
+  }
+
+  // ------------------------------------------------------------------ computes
+  const int g = lane / 4, pair = (lane % 4) * 2;
+  const int steps = p.H * p.R / 16;  // of the score product
+  const float kLog2e = 1.4426950408889634f;
+  const int shift_lanes = p.lanes == 1 ? 0 : p.lanes == 2 ? 1 : 2;
+  const int token_of = tokens - 1, map_shift = 4 - shift_lanes;  // row r: map r >> map_shift, token r & token_of
+  // (After a wait that gave up every warp still walks all pieces, its waits failing at once: the barriers meet.)
+  bool ok = true, first_piece = true;
+  while (next_piece(p, walk, x)) {
+    const int64_t end = job_end(p.c, x.s, x.job, tokens);
+    const int t1 = min(x.t1, (int)((end + kKeys - 1) / kKeys));
+    const int64_t q0 = x.s.first + (int64_t)x.job * tokens;  // packed row of the job's first token
+    const int live = min(tokens, x.s.n - x.job * tokens);
+    // queries of this warp's column steps
+    uint32_t qf[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int ks = warp + 8 * i;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        qf[i][e] = 0;
+        const int r = g + 8 * (e & 1), s = r >> map_shift, t = r & token_of;
+        if (ks < steps && s < p.maps && t < live) {
+          const int col = ks * 16 + pair + 8 * (e >> 1), h = col / p.R;
+          const int h0 = p.H >= p.maps ? s * p.group : s * p.H / p.maps;
+          if (h >= h0 && h < h0 + p.group)
+            qf[i][e] = *reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + h * p.q_branch + (q0 + t) * p.q_row +
+                                                          (col - h * p.R));
+        }
+      }
+    }
+    // the two rows whose softmax this warp runs
+    float m[2], l[2], scale[2];
+    int64_t sees[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 2 * warp + i, s = r >> map_shift, t = r & token_of;
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+      const bool on = s < p.maps && t < live;
+      scale[i] = on ? p.scales[s] * rsqrtf((float)p.group) * kLog2e : 0.f;
+      sees[i] = on ? min(x.s.held + x.job * tokens + t + 1, end) : 0;
+    }
+    float acc[kNT][4];
+#pragma unroll
+    for (int i = 0; i < kNT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+    bool wrong = !x.s.fits;
+
+    for (int t = x.t0; t < t1; ++t, ++it) {
+      const int st = it % p.stages;
+      ok &= mbar_wait(&full[st], (it / p.stages) & 1u, ab, 62);
+      __syncwarp();
+      const uint32_t kb = smem_u32(smem + st * p.stage_bytes), vb = kb + p.key_bytes;
+      const int64_t pos = (int64_t)t * kKeys;
+      wrong |= bad[st] != 0;
+      // ---- partial scores over this warp's columns
+      float sc[4][4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int ks = warp + 8 * i;
+        if (ks < steps) {
+#pragma unroll
+          for (int n2 = 0; n2 < 2; ++n2) {
+            const int key = n2 * 16 + (lane & 7) + ((lane >> 4) << 3);
+            const int box = p.brow == 32 ? 0 : key >> 4, kr = p.brow == 32 ? key : key & 15;
+            uint32_t b[4];
+            ldmatrix4(b, kb + box * (p.brow * 2 * p.H * p.R) + (ks >> 2) * (p.brow * 128) +
+                             sw128_offset(kr, (ks & 3) * 2 + ((lane >> 3) & 1)));
+            mma16816<T>(sc[2 * n2], qf[i], b[0], b[1]);
+            mma16816<T>(sc[2 * n2 + 1], qf[i], b[2], b[3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        float* at = red + (warp * 16 + g) * kRedPitch + n * 8 + pair;
+        *reinterpret_cast<float2*>(at) = make_float2(sc[n][0], sc[n][1]);
+        *reinterpret_cast<float2*>(at + 8 * kRedPitch) = make_float2(sc[n][2], sc[n][3]);
+      }
+      // values of positions that no row sees hold anything: 0 times them must stay 0
+      if (pos + kKeys > end) {
+        for (int i = tid; i < kKeys * kNT * 8; i += 32 * kWarps) {
+          const int key = i / (kNT * 8), chunk = i % (kNT * 8);
+          if (pos + key >= end) {
+            const int box = p.brow == 32 ? 0 : key >> 4, kr = p.brow == 32 ? key : key & 15;
+            st_shared_v4(vb + box * (p.brow * 2 * p.D) + (chunk >> 3) * (p.brow * 128) + sw128_offset(kr, chunk & 7), 0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async();
+      }
+      // A later token's value that is no number stays out of the earlier tokens' rows, which 0 times it would spoil.
+      bool odd = false;
+      if (live > 1 && pos + kKeys > x.s.held + (int64_t)x.job * tokens + 1) {
+        constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+        for (int i = tid; i < kKeys * kNT * 8; i += 32 * kWarps) {
+          const int key = i / (kNT * 8), chunk = i % (kNT * 8);
+          if (pos + key >= end) continue;
+          const int box = p.brow == 32 ? 0 : key >> 4, kr = p.brow == 32 ? key : key & 15;
+          const uint4 w = ld_shared_v4(vb + box * (p.brow * 2 * p.D) + (chunk >> 3) * (p.brow * 128) + sw128_offset(kr, chunk & 7));
+          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd |= (ws[e] & kExp) == kExp || ((ws[e] >> 16) & kExp) == kExp;
+        }
+      }
+      odd = named_bar_or(1, 32 * kWarps, odd);
+      // ---- softmax of two rows a warp, a key a lane
+      const int used = steps < kWarps ? steps : kWarps;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = 2 * warp + i;
+        float v = 0.f;
+        for (int w = 0; w < used; ++w) v += red[(w * 16 + r) * kRedPitch + lane];
+        v = pos + lane < sees[i] ? v * scale[i] : -INFINITY;
+        float top = v;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float next = fmaxf(m[i], top), at = next == -INFINITY ? 0.f : next;
+        const float c = next == -INFINITY ? 1.f : ex2(m[i] - at), e = ex2(v - at);
+        m[i] = next;
+        l[i] = l[i] * c + e;
+        weight[r * kPPitch + lane] = std::is_same<T, __nv_bfloat16>::value ? (uint16_t)pack_bf16x2(e, 0.f) : (uint16_t)pack_f16x2(e, 0.f);
+        if (lane == 0) rescale[r] = c;
+      }
+      named_bar_sync(1, 32 * kWarps);
+      // ---- output columns of this warp
+      const float c0 = rescale[g], c1 = rescale[g + 8];
+      if (__any_sync(0xffffffffu, c0 != 1.f || c1 != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < kNT; ++i) {
+          acc[i][0] *= c0;
+          acc[i][1] *= c0;
+          acc[i][2] *= c1;
+          acc[i][3] *= c1;
+        }
+      }
+      if (odd) {
+#pragma unroll 1
+        for (int key = 0; key < kKeys; ++key) {
+          const float w0 = unpack2<T>(weight[g * kPPitch + key]).x, w1 = unpack2<T>(weight[(g + 8) * kPPitch + key]).x;
+          const int box = p.brow == 32 ? 0 : key >> 4, kr = p.brow == 32 ? key : key & 15;
+#pragma unroll
+          for (int i = 0; i < kNT; ++i) {
+            const int col = (warp * kNT + i) * 8;
+            uint32_t u;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(u) : "r"(vb + box * (p.brow * 2 * p.D) + (col >> 6) * (p.brow * 128) +
+                                                                    sw128_offset(kr, (col & 63) >> 3) + pair * 2));
+            const float2 v = unpack2<T>(u);
+            acc[i][0] += w0 == 0.f ? 0.f : w0 * v.x;
+            acc[i][1] += w0 == 0.f ? 0.f : w0 * v.y;
+            acc[i][2] += w1 == 0.f ? 0.f : w1 * v.x;
+            acc[i][3] += w1 == 0.f ? 0.f : w1 * v.y;
+          }
+        }
+      } else
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
+        uint32_t a[4];
+        ldmatrix4(a, smem_u32(weight) + ((lane & 15) * kPPitch + k2 * 16 + (lane >> 4) * 8) * 2);
+#pragma unroll
+        for (int n2 = 0; n2 < kNT / 2; ++n2) {
+          const int key = k2 * 16 + (lane & 15), col = (warp * kNT + n2 * 2 + (lane >> 4)) * 8;
+          const int box = p.brow == 32 ? 0 : key >> 4, kr = p.brow == 32 ? key : key & 15;
+          uint32_t b[4];
+          ldmatrix4_trans(b, vb + box * (p.brow * 2 * p.D) + (col >> 6) * (p.brow * 128) + sw128_offset(kr, (col & 63) >> 3));
+          mma16816<T>(acc[2 * n2], a, b[0], b[1]);
+          mma16816<T>(acc[2 * n2 + 1], a, b[2], b[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+
+    // ---- rows' sums; the job's output, or this piece of it
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+      if (wrong || !ok) l[i] = NAN;
+      if (lane == 0) {
+        row_max[2 * warp + i] = m[i];
+        row_sum[2 * warp + i] = l[i];
+      }
+    }
+    if (wrong && tid == 0) atomicOr(p.status, DA_DEV_BAD_PAGE);
+    named_bar_sync(1, 32 * kWarps);
+    if (x.t1 - x.t0 == x.tiles) {
+      const int s0 = g >> map_shift, s1 = (g + 8) >> map_shift, k0 = g & token_of, k1 = (g + 8) & token_of;
+      const float w0 = s0 < p.maps ? (p.weights ? p.weights[s0] : 1.f) / row_sum[g] : 0.f;
+      const float w1 = s1 < p.maps ? (p.weights ? p.weights[s1] : 1.f) / row_sum[g + 8] : 0.f;
+      T* y = static_cast<T*>(p.y);
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) {
+        const int col = (warp * kNT + i) * 8 + pair;
+        float a0 = s0 < p.maps ? acc[i][0] * w0 : 0.f, a1 = s0 < p.maps ? acc[i][1] * w0 : 0.f;
+        float b0 = s1 < p.maps ? acc[i][2] * w1 : 0.f, b1 = s1 < p.maps ? acc[i][3] * w1 : 0.f;
+        if (p.per_map) {
+          if (s0 < p.maps && k0 < live)
+            *reinterpret_cast<uint32_t*>(y + ((q0 + k0) * p.maps + s0) * p.D + col) = pack2<T>(a0, a1);
+          if (s1 < p.maps && k1 < live)
+            *reinterpret_cast<uint32_t*>(y + ((q0 + k1) * p.maps + s1) * p.D + col) = pack2<T>(b0, b1);
+          continue;
+        }
+        if (p.lanes == 1) {
+          if (k1 < live) *reinterpret_cast<uint32_t*>(y + (q0 + k1) * p.D + col) = pack2<T>(b0, b1);
+        } else {  // maps of a token: rows 8 apart, and with four maps rows 4 apart too
+          a0 += b0;
+          a1 += b1;
+          if (p.lanes == 4) {
+            a0 += __shfl_xor_sync(0xffffffffu, a0, 16);
+            a1 += __shfl_xor_sync(0xffffffffu, a1, 16);
+          }
+        }
+        if (s0 == 0 && k0 < live) *reinterpret_cast<uint32_t*>(y + (q0 + k0) * p.D + col) = pack2<T>(a0, a1);
+      }
+    } else {
+      const int slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
+      float* rows = p.part + (size_t)slot * 16 * p.D;
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) {
+        const int col = (warp * kNT + i) * 8 + pair;
+        if ((g & token_of) < live && (g >> map_shift) < p.maps)
+          *reinterpret_cast<float2*>(rows + g * p.D + col) = make_float2(acc[i][0], acc[i][1]);
+        if (((g + 8) & token_of) < live && ((g + 8) >> map_shift) < p.maps)
+          *reinterpret_cast<float2*>(rows + (g + 8) * p.D + col) = make_float2(acc[i][2], acc[i][3]);
+      }
+      float* ml = p.part + (size_t)2 * p.ctas * 16 * p.D + (size_t)slot * 32;
+      if (tid < 16) {
+        ml[tid] = row_max[tid];
+        ml[16 + tid] = row_sum[tid];
+      }
+    }
+    first_piece = false;
+    named_bar_sync(1, 32 * kWarps);  // row_max and row_sum are free again
+  }
+}
+
+// One packed row from its pieces c0, c0 + 1, ...: the first in slot `slot0`, the later ones, which open their CTAs, in
+// slots 2 c.
+template <typename T>
+DA_DEV void join(const FewParams& p, int64_t row, int t, int c0, int pieces, int slot0, float (*wts)[512], float4 (*sums)[17]) {
+  const int tid = threadIdx.x, tokens = 16 / p.lanes;
+  const float* ml = p.part + (size_t)2 * p.ctas * 16 * p.D;
+  // each map's weights of the pieces: 2^(m_c - M) / sum, times alpha
+  const int warp = tid / 32, lane = tid % 32;
+  if (warp < p.maps) {
+    const int r = warp * tokens + t;
+    float top = -INFINITY, sum = 0.f;
+    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, ml[(size_t)(i ? 2 * (c0 + i) : slot0) * 32 + r]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int i = lane; i < pieces; i += 32) {
+      const float* at = ml + (size_t)(i ? 2 * (c0 + i) : slot0) * 32;
+      const float e = at[r] == -INFINITY ? 0.f : ex2(at[r] - top);
+      sum += at[16 + r] * e;  // (a NaN sum, of a piece with a bad page, stays)
+      wts[warp][i] = e;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float f = (p.weights ? p.weights[warp] : 1.f) / sum;
+    for (int i = lane; i < pieces; i += 32) wts[warp][i] *= f;
+  }
+  __syncthreads();
+  const int col = blockIdx.y * 64 + (tid % 16) * 4, part = tid / 16;
+  T* y = static_cast<T*>(p.y);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int m = 0; m < p.maps; ++m) {
+#pragma unroll 4
+    for (int i = part; i < pieces; i += 16) {
+      const float w = wts[m][i];
+      const float4 v = *reinterpret_cast<const float4*>(
+          p.part + ((size_t)(i ? 2 * (c0 + i) : slot0) * 16 + m * tokens + t) * p.D + col);
+      if (w == 0.f) continue;  // (a piece that the row does not see)
+      o.x += w * v.x;
+      o.y += w * v.y;
+      o.z += w * v.z;
+      o.w += w * v.w;
+    }
+    if (!p.per_map && m + 1 < p.maps) continue;
+    sums[part][tid % 16] = o;
+    __syncthreads();
+    if (part == 0) {
+      for (int i = 1; i < 16; ++i) {
+        const float4 v = sums[i][tid];
+        o.x += v.x;
+        o.y += v.y;
+        o.z += v.z;
+        o.w += v.w;
+      }
+      const int64_t at = p.per_map ? (row * p.maps + m) * p.D + col : row * p.D + col;
+      *reinterpret_cast<uint2*>(y + at) = make_uint2(pack2<T>(o.x, o.y), pack2<T>(o.z, o.w));
+    }
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    __syncthreads();
+  }
+}
+
+// Joins the pieces of the jobs that lie in several CTAs: one CTA a packed token and 64 columns.
+template <typename T>
+__global__ void __launch_bounds__(256) combine_kernel(const FewParams p) {
+  __shared__ int64_t buf[32];
+  __shared__ float wts[4][512];
+  __shared__ float4 sums[16][17];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int tid = threadIdx.x, b = blockIdx.x / p.few_rows;
+  const Sequence s = sequence(p.c, b);
+  if ((int)(blockIdx.x % p.few_rows) >= s.n || sequence_tiles(p, s) == 0) return;
+  int64_t all = 0, ahead = 0;
+  for (int i = tid; i < p.c.B; i += 256) {
+    const int64_t v = sequence_tiles(p, sequence(p.c, i));
+    all += v;
+    if (i < b) ahead += v;
+  }
+  const int64_t total = block_sum<256>(all, buf);
+  ahead = block_sum<256>(ahead, buf);
+  const int64_t share = (total + p.ctas - 1) / p.ctas;
+  const int tokens = 16 / p.lanes, tiles = job_tiles(p.c, s);
+  for (int i = blockIdx.x % p.few_rows; i < s.n; i += p.few_rows) {
+    const int64_t f0 = ahead + (int64_t)(i / tokens) * tiles, f1 = f0 + tiles;
+    const int c0 = (int)(f0 / share), c1 = (int)((f1 - 1) / share);
+    if (c0 < c1)  // (else finished where it was computed)
+      join<T>(p, s.first + i, i % tokens, c0, c1 - c0 + 1, 2 * c0 + (f0 > c0 * share ? 1 : 0), wts, sums);
+  }
+}
+
+}  // namespace paged
+}  // namespace da
+
+namespace {
+
+using namespace da;
+
+struct FewPlan {
+  int stages, stage_bytes, key_bytes, smem, ctas, few_rows;
+};
+
+constexpr int kFixedBytes = paged::kWarps * 16 * paged::kRedPitch * 4 + 16 * paged::kPPitch * 2 + 1024;
+
+// Shared memory holds as many tiles as fit, at least two, in one CTA an SM -- or in two or three CTAs an SM where their
+// tiles are small, so that one computes while another waits at a barrier.
+FewPlan few_plan(int64_t tokens, int64_t B, int64_t capacity, int64_t max_new, int wide, int D, int lanes) {
+  FewPlan f;
+  f.key_bytes = paged::kKeys * 2 * wide;
+  f.stage_bytes = f.key_bytes + paged::kKeys * 2 * D;
+  int per_sm = 3;
+  for (;; --per_sm) {
+    f.stages = (228 * 1024 / per_sm - 2304 - kFixedBytes) / f.stage_bytes;  // (an SM has 228 KB, a CTA 1 KB of its own)
+    if (per_sm == 1 || f.stages >= 3) break;
+  }
+  if (f.stages > paged::kMaxStages) f.stages = paged::kMaxStages;
+  f.smem = f.stages * f.stage_bytes + kFixedBytes;
+  const int64_t rows = 16 / lanes, jobs = tokens / rows + B < tokens ? tokens / rows + B : tokens;
+  const int64_t tiles = (capacity + paged::kKeys - 1) / paged::kKeys;
+  const int64_t most = (int64_t)sm_count() * per_sm, need = jobs * (tiles > 0 ? tiles : 1);
+  f.ctas = (int)(need < most ? need : most);
+  if (f.ctas < 1) f.ctas = 1;
+  if (f.ctas > 512) f.ctas = 512;  // pieces that combine_kernel has room for
+  f.few_rows = (int)(max_new < 64 ? max_new : 64);
+  return f;
+}
+
+int64_t few_workspace(const FewPlan& f, int D) {
+  return f.ctas > 1 ? (int64_t)2 * f.ctas * (16 * D + 32) * (int64_t)sizeof(float) : 0;
+}
+
+int lanes_of(int maps) { return maps == 1 ? 1 : maps == 2 ? 2 : 4; }
+
+bool attn_shape(int H, int R, int D, int maps) {
+  if (H < 1 || R < 64 || R % 64 || maps < 1 || maps > 4 || (H % maps && maps % H)) return false;
+  if (H > 512 || R > 512 || (H > maps ? H : maps) * R > 512) return false;
+  return D == 128 || D == 256 || D == 512;
+}
+
+template <typename T, int kNT>
+int launch_few(const paged::FewParams& p, const FewPlan& f, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
+  if (int rc = allow_smem<paged::few_kernel<T, kNT>>(225 * 1024 + 768)) return rc;
+  if (int rc = launch_kernel(paged::few_kernel<T, kNT>, dim3((unsigned)f.ctas), dim3(32 * (paged::kWarps + 1)), f.smem, st,
+                             false, tk, tv, p))
+    return rc;
+  if (f.ctas == 1) return DA_OK;
+  return launch_kernel(paged::combine_kernel<T>, dim3((unsigned)(p.c.B * p.few_rows), (unsigned)(p.D / 64)), dim3(256), 0, st,
+                       false, p);
+}
+
+}  // namespace
+
+extern "C" int64_t da_paged_attn_workspace_size(int64_t tokens, int64_t B, int64_t table_cols, int page, int64_t max_new,
+                                                int H, int R, int D, int maps) {
+  if (!attn_shape(H, R, D, maps) || tokens < 0 || B < 0 || table_cols < 0 || page < 1) return -1;
+  if (tokens == 0 || B == 0) return 0;
+  if (max_new < 1 || max_new > tokens) max_new = tokens;
+  return few_workspace(few_plan(tokens, B, table_cols * page, max_new, H * R, D, lanes_of(maps)), D);
+}
+
+extern "C" int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_row_stride, int64_t tokens,
+                             const void* key_pages, const void* value_pages, int dtype, int64_t pages, int page, int H,
+                             int R, int D, int maps, const int* table, int64_t table_stride, int64_t table_cols,
+                             const int* lengths, const int* starts, int64_t B, int64_t max_new, const float* scales,
+                             const float* weights, int per_map, int zero_rest, void* y, void* workspace,
+                             int64_t workspace_bytes, int* status, void* stream) {
+  if (!q || !key_pages || !value_pages || !table || !lengths || !starts || !scales || !y || !status) return DA_ERR_NULL;
+  if (dtype != DA_BF16 && dtype != DA_F16) return DA_ERR_DTYPE;
+  if (!attn_shape(H, R, D, maps)) return DA_ERR_UNSUPPORTED;
+  if (maps > 1 && !per_map && !weights) return DA_ERR_NULL;
+  paged::FewParams p;
+  if (int rc = paged::make_cache(&p.c, table, table_stride, table_cols, lengths, starts, B, tokens, pages, page)) return rc;
+  for (const void* a : {q, key_pages, value_pages, (const void*)y})
+    if (reinterpret_cast<uintptr_t>(a) % 16) return DA_ERR_ALIGN;
+  if (q_row_stride % 8 || (H > 1 && q_branch_stride % 8)) return DA_ERR_ALIGN;
+  if (tokens == 0) return DA_OK;
+  if (B == 0 || B > 0x7fffffff / 64) return DA_ERR_SHAPE;
+  if (max_new < 1 || max_new > tokens) max_new = tokens;
+  if (int rc = bind_device(key_pages)) return rc;
+  const FewPlan f = few_plan(tokens, B, p.c.capacity, max_new, H * R, D, lanes_of(maps));
+  if (workspace_bytes < few_workspace(f, D) || (few_workspace(f, D) && !workspace)) return DA_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return DA_ERR_ALIGN;
+  p.q = q;
+  p.q_branch = q_branch_stride;
+  p.q_row = q_row_stride;
+  p.scales = scales;
+  p.weights = per_map ? nullptr : weights;
+  p.y = y;
+  p.part = static_cast<float*>(workspace);
+  p.status = status;
+  p.H = H;
+  p.R = R;
+  p.D = D;
+  p.maps = maps;
+  p.group = H >= maps ? H / maps : 1;
+  p.lanes = lanes_of(maps);
+  p.few_most = 0x7fffffff;
+  p.few_rows = f.few_rows;
+  p.stages = f.stages;
+  p.stage_bytes = f.stage_bytes;
+  p.key_bytes = f.key_bytes;
+  p.brow = page < paged::kKeys ? page : paged::kKeys;
+  p.ctas = f.ctas;
+  p.per_map = per_map;
+  p.zero_rest = zero_rest;
+  const CUtensorMapDataType dt = dtype == DA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap tk, tv;
+  for (int i = 0; i < 2; ++i) {  // (column in its block of 64, slot, block)
+    const uint64_t width = i ? D : H * R;
+    const uint64_t dims[3] = {64, (uint64_t)pages * page, width / 64};
+    const uint64_t strides[2] = {width * 2, 128};
+    const uint32_t box[3] = {64, (uint32_t)p.brow, (uint32_t)(width / 64)};
+    if (int rc = make_tmap_blocks(i ? &tv : &tk, i ? value_pages : key_pages, dt, 2, 3, dims, strides, box)) return rc;
+  }
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == DA_BF16)
+    return D == 512   ? launch_few<__nv_bfloat16, 8>(p, f, tk, tv, st)
+           : D == 256 ? launch_few<__nv_bfloat16, 4>(p, f, tk, tv, st)
+                      : launch_few<__nv_bfloat16, 2>(p, f, tk, tv, st);
+  return D == 512   ? launch_few<__half, 8>(p, f, tk, tv, st)
+         : D == 256 ? launch_few<__half, 4>(p, f, tk, tv, st)
+                    : launch_few<__half, 2>(p, f, tk, tv, st);
+}

@@ -1,0 +1,173 @@
+"""A paged cache of routed keys and dense values, and the outer routed attention over it.
+
+A served model keeps what the outer attention reads of earlier tokens: the routed keys of every branch and the dense
+value, per layer.  They lie in pages of a fixed number of positions, so that sequences of any lengths share one pool:
+position j of sequence b is slot ``j % page`` of page ``table[b, j // page]``.  A step brings new tokens of some or all
+sequences, packed one sequence after another (:class:`PagedBatch`); :func:`append_paged` puts their keys and values
+into the pages, :func:`routed_attention_paged` lets each new token attend over its sequence up to itself, from single
+tokens to long chunks.  :class:`RoutedCache` holds the pages of all layers of a model and hands them out.
+
+The sizes that vary from step to step are read by the kernels on the device: no call waits for the GPU, and a captured
+graph follows them.  A page number outside the cache, or a length that the table has no room for, is never followed:
+those positions are not written, the tokens that would need them get NaN, and ``ops.device_status`` reports bit 8.
+
+Inference only: the operators raise on tensors that require a gradient.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple, Sequence
+
+import torch
+from torch import Tensor
+
+from . import _lib, ops
+from ._lib import ptr
+from .eight_bit import _CODES, _HALF, _device_of, _inference_only, _launch
+
+BAD_PAGE = 8  # bit of ops.device_status
+
+
+class PagedBatch(NamedTuple):
+    """The sequences of one step.
+
+    table: int32 [B, pages a sequence], unit column stride; entries that no position needs may hold anything.
+    lengths: int32 [B], tokens that each sequence had before the step.
+    starts: int32 [B + 1], where each sequence's new tokens begin among the packed rows (``starts[0]`` is 0, ``starts[B]``
+        their number; rows behind it belong to no sequence, and sequences may have none).
+    max_new: the largest number of new tokens of one sequence, if known: chooses the kernel, changes no result's meaning.
+    """
+
+    table: Tensor
+    lengths: Tensor
+    starts: Tensor
+    max_new: int | None = None
+
+
+def _check_batch(name: str, batch: PagedBatch) -> int:
+    table, lengths, starts, _max_new = batch
+    for what, t in (("table", table), ("lengths", lengths), ("starts", starts)):
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name} takes its {what} in int32, got {t.dtype}")
+    b = lengths.shape[0] if lengths.ndim == 1 else -1
+    if table.ndim != 2 or table.shape[0] != b or starts.shape != (b + 1,):
+        raise ValueError(f"{name} takes a table [B, pages], lengths [B] and starts [B + 1], got {tuple(table.shape)}, "
+                         f"{tuple(lengths.shape)} and {tuple(starts.shape)}")
+    return b
+
+
+def _table_args(batch: PagedBatch) -> tuple[Tensor, Tensor, Tensor]:
+    table = batch.table
+    if table.shape[1] > 1 and table.stride(1) != 1 or table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+        table = table.contiguous()
+    return table, batch.lengths.contiguous(), batch.starts.contiguous()
+
+
+def _check_pages(name: str, key_pages: Tensor, value_pages: Tensor) -> tuple[int, int, int, int, int]:
+    if key_pages.ndim != 4 or value_pages.ndim != 3 or value_pages.shape[:2] != key_pages.shape[:2]:
+        raise ValueError(f"{name} takes key pages [pages, page, H, R] and value pages [pages, page, D], got "
+                         f"{tuple(key_pages.shape)} and {tuple(value_pages.shape)}")
+    if key_pages.dtype not in _HALF or value_pages.dtype != key_pages.dtype:
+        raise ValueError(f"{name} takes pages of one type, bfloat16 or float16, got {key_pages.dtype} and {value_pages.dtype}")
+    if not key_pages.is_contiguous() or not value_pages.is_contiguous():
+        raise ValueError(f"{name} takes contiguous pages")
+    pages, page, h, r = key_pages.shape
+    if page < 16 or page > 65536 or page & (page - 1):
+        raise ValueError(f"{name} takes pages of 16 to 65536 positions, a power of two, got {page}")
+    if not pages:
+        raise ValueError(f"{name} takes at least one page")
+    return pages, page, h, r, value_pages.shape[2]
+
+
+def append_paged(keys: Tensor, values: Tensor, key_pages: Tensor, value_pages: Tensor, batch: PagedBatch) -> None:
+    """Writes the packed new tokens' keys [H, N, R] and values [N, D] behind what their sequences have, in place.
+
+    Token i of sequence b goes to position ``batch.lengths[b] + i``; the lengths stay as they are.  Keys and values in
+    fp32, bf16 or fp16 with unit column stride or any other (copied first then), rounded once to the pages' type.  Nothing
+    but the new positions is written."""
+    name = "append_paged"
+    b = _check_batch(name, batch)
+    pages, page, h, r, d = _check_pages(name, key_pages, value_pages)
+    if keys.ndim != 3 or keys.shape[0] != h or keys.shape[2] != r or values.shape != (keys.shape[1], d):
+        raise ValueError(f"{name} takes keys [{h}, N, {r}] and values [N, {d}], got {tuple(keys.shape)} and {tuple(values.shape)}")
+    if r % 8 or d % 8:
+        raise NotImplementedError(f"{name} covers routing and value widths divisible by 8, got {r} and {d}")
+    k_code, v_code = _CODES.get(keys.dtype), _CODES.get(values.dtype)
+    if k_code is None or v_code is None:
+        raise ValueError(f"{name} takes keys and values in float32, bfloat16 or float16, got {keys.dtype} and {values.dtype}")
+    device = _device_of(name, key_pages, value_pages, keys, values, *batch[:3])
+    _inference_only(name, keys, values, key_pages, value_pages)
+    n = keys.shape[1]
+    if not n or not b:
+        return
+    keys = keys if keys.stride(2) == 1 else keys.contiguous()
+    values = values if values.stride(1) == 1 else values.contiguous()
+    table, lengths, starts = _table_args(batch)
+    _launch(device, "da_paged_append", keys.data_ptr(), k_code, keys.stride(0), keys.stride(1), values.data_ptr(), v_code,
+            values.stride(0), n, key_pages.data_ptr(), value_pages.data_ptr(), _CODES[key_pages.dtype], pages, page, h, r, d,
+            table.data_ptr(), table.stride(0) if b > 1 else table.shape[1], table.shape[1], lengths.data_ptr(),
+            starts.data_ptr(), b, ops.workspace(key_pages.device).status.data_ptr())
+
+
+def _aligned_query(q: Tensor) -> Tensor:
+    """``q`` [H, N, R] with branches and rows on 16 bytes: as it lies, or a copy."""
+    if (q.stride(2) != 1 or q.data_ptr() % 16 or (q.shape[1] > 1 and q.stride(1) % 8)
+            or (q.shape[0] > 1 and q.stride(0) % 8)):
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+    return q
+
+
+def routed_attention_paged(query: Tensor, key_pages: Tensor, value_pages: Tensor, batch: PagedBatch, scales: Tensor,
+                           map_weights: Tensor | None = None, *, out: Tensor | None = None) -> Tensor:
+    """Outer routed attention of the packed new tokens over the pages, after :func:`append_paged` put them there.
+
+    query [H, N, R] of the pages' type; ``scales`` [S] the maps' temperatures, S of H branches as in
+    :func:`assemble_score_maps`.  Token i of sequence b sees positions 0 to ``batch.lengths[b] + i``.  With
+    ``map_weights`` [S], or one map, returns the maps' mixture [N, D]; without, several maps' outputs [N, S, D].  The
+    keys may be of any length: the softmax takes off each row's own maximum.  Rows behind the last sequence are zero,
+    or left as they are in ``out``.
+
+    Supported: R a multiple of 64, D 128, 256 or 512, up to 4 maps and ``max(H, S) * R`` up to 512."""
+    name = "routed_attention_paged"
+    b = _check_batch(name, batch)
+    pages, page, h, r, d = _check_pages(name, key_pages, value_pages)
+    if query.ndim != 3 or query.shape[0] != h or query.shape[2] != r:
+        raise ValueError(f"{name} takes a query [{h}, N, {r}], got {tuple(query.shape)}")
+    if query.dtype != key_pages.dtype:
+        raise ValueError(f"{name} takes a query of the pages' type {key_pages.dtype}, got {query.dtype}")
+    maps = scales.shape[0] if scales.ndim == 1 else 0
+    if not maps or (h % maps and maps % h):
+        raise ValueError(f"{name} takes one scale a map, their number dividing the {h} branches or divided by it, "
+                         f"got {tuple(scales.shape)}")
+    if map_weights is not None and map_weights.shape != (maps,):
+        raise ValueError(f"{name} takes {maps} map weights, got {tuple(map_weights.shape)}")
+    ops._attention_supported(r, d, maps, max(h // maps, 1))
+    n = query.shape[1]
+    per_map = maps > 1 and map_weights is None
+    shape = (n, maps, d) if per_map else (n, d)
+    if out is not None and (out.shape != shape or out.dtype != query.dtype or not out.is_contiguous()
+                            or out.data_ptr() % 16):
+        raise ValueError(f"{name} writes a contiguous, 16-byte aligned {query.dtype} tensor {shape}, got {out.dtype} {tuple(out.shape)}")
+    device = _device_of(name, key_pages, value_pages, query, scales, map_weights, out, *batch[:3])
+    _inference_only(name, query, key_pages, value_pages, scales, map_weights, out)
+    y = torch.empty(shape, dtype=query.dtype, device=query.device) if out is None else out
+    if not n:
+        return y
+    if not b:
+        return y.zero_() if out is None else y
+    query = _aligned_query(query)
+    scales = scales.float().contiguous()
+    weights = None if per_map or map_weights is None else map_weights.float().contiguous()
+    table, lengths, starts = _table_args(batch)
+    most = n if batch.max_new is None else batch.max_new
+    with torch.cuda.device(device):
+        need = _lib.lib().da_paged_attn_workspace_size(n, b, table.shape[1], page, most, h, r, d, maps)
+    work = torch.empty(need, dtype=torch.uint8, device=query.device) if need > 0 else None
+    _launch(device, "da_paged_attn", query.data_ptr(), query.stride(0), query.stride(1), n, key_pages.data_ptr(),
+            value_pages.data_ptr(), _CODES[query.dtype], pages, page, h, r, d, maps, table.data_ptr(),
+            table.stride(0) if b > 1 else table.shape[1], table.shape[1], lengths.data_ptr(), starts.data_ptr(), b, most,
+            scales.data_ptr(), ptr(weights), int(per_map), int(out is None), y.data_ptr(), ptr(work), max(need, 0),
+            ops.workspace(query.device).status.data_ptr())
+    return y

@@ -545,6 +545,44 @@ DA_API int da_checkpoint8_wgrad(const void* dy, int dtype, int64_t ldy, const in
                                 int64_t rows, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,
                                 float* workspace, int64_t workspace_elems, int* status, void* stream);
 
+/* ---- paged cache of routed keys and dense values ----------------------
+ * No reference counterpart: the reference attends over whole sequences only.  A cache's keys
+ * lie in key_pages [pages, page, H, R] and its values in value_pages [pages, page, D], both in
+ * dtype (DA_F16 / DA_BF16), dense and 16-byte aligned; page a power of two, 16 or more, and
+ * pages * page below 2^31.  Position j of sequence b is slot j % page of page table[b, j / page]
+ * (int32, rows table_stride apart, table_cols entries each).  A step brings starts[b + 1] -
+ * starts[b] new tokens of sequence b (int32 [B + 1], starts[0] = 0) behind the lengths[b] (int32
+ * [B]) that it has, packed in that order among `tokens` rows.  table, lengths and starts are
+ * device data: a page number outside [0, pages) or a position past the table is never followed;
+ * it sets bit 8 of status[0]. */
+
+/* Packed row i's key [H, R] (row stride key_row_stride, branches key_branch_stride apart, in
+ * elements) and value [D] into the pages, each in any of DA_F16 / DA_BF16 / DA_F32, rounded once.
+ * R and D multiples of 8.  Rows past starts[B] and all other positions are left alone. */
+DA_API int da_paged_append(const void* keys, int key_dtype, int64_t key_branch_stride, int64_t key_row_stride,
+                           const void* values, int value_dtype, int64_t value_row_stride, int64_t tokens, void* key_pages,
+                           void* value_pages, int dtype, int64_t pages, int page, int H, int R, int D, const int* table,
+                           int64_t table_stride, int64_t table_cols, const int* lengths, const int* starts, int64_t B,
+                           int* status, void* stream);
+
+/* Outer routed attention (modules.py:265-272, ops.py:65-139) of the packed tokens over the pages, the new
+ * tokens' keys and values among them: token i of sequence b sees positions 0 .. lengths[b] + i.
+ * q [H, tokens, R] in dtype, 16-byte aligned, strides multiples of 8.  Maps of H branches as
+ * da_attn_fwd has them: S = maps <= 4 divides H or is divided by it, R a multiple of 64, max(H, S) R
+ * at most 512, D 128, 256 or 512.  y [tokens, D] = sum_s weights[s] A_s V (weights null: one map), or with
+ * per_map the maps' A_s V in [tokens, S, D].  zero_rest: rows past starts[B] become zero (else they are
+ * left alone).  A row whose positions the table or the cache does not all have becomes NaN.
+ * max_new: the largest starts[b + 1] - starts[b], if known (else 0): a choice of kernels, not a
+ * limit.  workspace: da_paged_attn_workspace_size bytes (same arguments, same current device), 16-byte
+ * aligned. */
+DA_API int64_t da_paged_attn_workspace_size(int64_t tokens, int64_t B, int64_t table_cols, int page, int64_t max_new, int H,
+                                            int R, int D, int maps);
+DA_API int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_row_stride, int64_t tokens, const void* key_pages,
+                         const void* value_pages, int dtype, int64_t pages, int page, int H, int R, int D, int maps,
+                         const int* table, int64_t table_stride, int64_t table_cols, const int* lengths, const int* starts,
+                         int64_t B, int64_t max_new, const float* scales, const float* weights, int per_map, int zero_rest,
+                         void* y, void* workspace, int64_t workspace_bytes, int* status, void* stream);
+
 /* ---- building-block check -------------------------------------------
  * No reference counterpart: D[128, n] = A[128, k] * B^T computed by one
  * tcgen05 tile (cta_group 1 or 2) for testing the descriptor layouts.
