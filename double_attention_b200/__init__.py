@@ -36,6 +36,7 @@ from .modules import (
 )
 from .ops import assemble_score_maps, dictionary_route, routed_attention
 from .paged import PagedBatch, append_paged, routed_attention_paged
+from .scoring import TokenLogProbs, token_log_probs
 
 __all__ = [
     "Checkpoint8",
@@ -51,6 +52,7 @@ __all__ = [
     "PagedBatch",
     "SharedDictionaryAttention",
     "SharedDictionaryBank",
+    "TokenLogProbs",
     "add_layernorm_int8",
     "add_rmsnorm_int8",
     "append_paged",
@@ -69,5 +71,6 @@ __all__ = [
     "rmsnorm_int8",
     "routed_attention",
     "routed_attention_paged",
+    "token_log_probs",
     "weight_grad_checkpoint8",
 ]

@@ -583,6 +583,22 @@ DA_API int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_row_s
                          int64_t B, int64_t max_new, const float* scales, const float* weights, int per_map, int zero_rest,
                          void* y, void* workspace, int64_t workspace_bytes, int* status, void* stream);
 
+/* ---- scores of tokens --------------------------------------------------
+ * No reference counterpart (the reference has the mean cross entropy, modules.py:455-460).
+ * logits [rows, V] in dtype (DA_F16 / DA_BF16 / DA_F32), row stride ld, any alignment.
+ * log_probs[r] = log softmax(logits[r])[tokens[r]] (0 for the token -100, NaN for others outside
+ * [0, V)), entropy[r] = -sum p log p; with top > 0 (at most 32 and V) the top largest entries' log
+ * probabilities and indices [rows, top], in order of (value, lowest index), NaN first.  stats (fp32 [rows,
+ * 2], 8-byte aligned, or null): what the backward pass reads.  Sums in fp32. */
+DA_API int da_token_log_probs(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t V, const int64_t* tokens,
+                              int top, float* log_probs, float* entropy, float* top_log_probs, int64_t* top_tokens,
+                              float* stats, void* stream);
+/* d_logits[r, i] = d_log_probs[r] ([i = token] - p_i) - d_entropy[r] p_i (log p_i + entropy[r]) in dtype, row stride
+ * ldd; either of d_log_probs and d_entropy may be null (zeros). */
+DA_API int da_token_log_probs_bwd(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t V, const int64_t* tokens,
+                                  const float* stats, const float* entropy, const float* d_log_probs,
+                                  const float* d_entropy, void* d_logits, int64_t ldd, void* stream);
+
 /* ---- building-block check -------------------------------------------
  * No reference counterpart: D[128, n] = A[128, k] * B^T computed by one
  * tcgen05 tile (cta_group 1 or 2) for testing the descriptor layouts.
