@@ -99,7 +99,7 @@ SIGNATURES: dict[str, list] = {
     "da_checkpoint8_wgrad": [_p, _i32, _i64, _p, _p, _i64, _i64, _i64, _p, _i32, _i64, _p, _i64, _p, _p],
     "da_paged_append": [_p, _i32, _i64, _i64, _p, _i32, _i64, _i64, _p, _p, _i32, _i64, _i32, _i32, _i32, _i32, _p, _i64, _i64,
                         _p, _p, _i64, _p, _p],
-    "da_paged_attn_workspace_size": [_i64, _i64, _i64, _i32, _i64, _i32, _i32, _i32, _i32],  # returns int64 (set below)
+    "da_paged_attn_workspace_size": [_i64, _i64, _i64, _i32, _i64, _i32, _i32, _i32, _i32, _i32],  # returns int64 (set below)
     "da_paged_attn": [_p, _i64, _i64, _i64, _p, _p, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _p, _i64, _i64, _p, _p, _i64,
                       _i64, _p, _p, _i32, _i32, _p, _p, _i64, _p, _p],
     "da_token_log_probs": [_p, _i32, _i64, _i64, _i64, _p, _i32, _p, _p, _p, _p, _p, _p],

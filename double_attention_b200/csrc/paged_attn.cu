@@ -18,7 +18,7 @@
 #include <math.h>
 
 #include "host_util.h"
-#include "paged.cuh"
+#include "paged_chunk.h"
 
 namespace da {
 namespace paged {
@@ -43,12 +43,14 @@ struct FewParams {
   int stages, stage_bytes, key_bytes, brow;
   int ctas;
   int per_map, zero_rest;
+  Plan chunks;                      // of the other kernel, if it ran
+  int chunked;
 };
 
 // Tiles of one job, and of all jobs, of sequence s.
 DA_DEV int job_tiles(const Cache& c, const Sequence& s) { return (int)((positions(c, s) + kKeys - 1) / kKeys); }
-DA_DEV int64_t sequence_tiles(const FewParams& p, const Sequence& s) {
-  if (s.n == 0 || s.n > p.few_most) return 0;
+DA_DEV int64_t sequence_tiles(const FewParams& p, const Sequence& s, int b) {
+  if (s.n == 0 || (s.n > p.few_most && !(p.chunked && left_odd(p.chunks, b)))) return 0;
   const int tokens = 16 / p.lanes;
   return (int64_t)((s.n + tokens - 1) / tokens) * job_tiles(p.c, s);
 }
@@ -108,7 +110,7 @@ struct Piece {
 DA_DEV bool next_piece(const FewParams& p, Walk& w, Piece& x) {
   while (w.left > 0 && w.b < p.c.B) {
     x.s = sequence(p.c, w.b);
-    const int64_t all = sequence_tiles(p, x.s);
+    const int64_t all = sequence_tiles(p, x.s, w.b);
     if (w.off < all) {
       x.b = w.b;
       x.tiles = job_tiles(p.c, x.s);
@@ -162,7 +164,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2) few_kernel(const __grid_
   // ---- this CTA's share of the flat list of tiles
   constexpr int kThreads = 32 * (kWarps + 1);
   int64_t mine = 0;
-  for (int b = tid; b < p.c.B; b += kThreads) mine += sequence_tiles(p, sequence(p.c, b));
+  for (int b = tid; b < p.c.B; b += kThreads) mine += sequence_tiles(p, sequence(p.c, b), b);
   const int64_t total = block_sum<kThreads>(mine, buf);
   if (p.zero_rest) {
     const int64_t used = clamp64(p.c.starts[p.c.B], 0, p.c.tokens);
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2) few_kernel(const __grid_
     int64_t before = 0;  // tiles of the sequences before this round's
     for (int base = 0;; base += kThreads) {
       const int b = base + tid;
-      const int64_t v = b < p.c.B ? sequence_tiles(p, sequence(p.c, b)) : 0;
+      const int64_t v = b < p.c.B ? sequence_tiles(p, sequence(p.c, b), b) : 0;
       int64_t inc = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -581,10 +583,10 @@ __global__ void __launch_bounds__(256) combine_kernel(const FewParams p) {
   grid_launch_dependents();
   const int tid = threadIdx.x, b = blockIdx.x / p.few_rows;
   const Sequence s = sequence(p.c, b);
-  if ((int)(blockIdx.x % p.few_rows) >= s.n || sequence_tiles(p, s) == 0) return;
+  if ((int)(blockIdx.x % p.few_rows) >= s.n || sequence_tiles(p, s, b) == 0) return;
   int64_t all = 0, ahead = 0;
   for (int i = tid; i < p.c.B; i += 256) {
-    const int64_t v = sequence_tiles(p, sequence(p.c, i));
+    const int64_t v = sequence_tiles(p, sequence(p.c, i), i);
     all += v;
     if (i < b) ahead += v;
   }
@@ -661,12 +663,23 @@ int launch_few(const paged::FewParams& p, const FewPlan& f, const CUtensorMap& t
 
 }  // namespace
 
+namespace {
+
+// Sequences of more new tokens go to the chunk kernel, whose tiles have 128 of them: the tiles here, of 16 (map, token) rows,
+// would read the cache once for every 16 / maps of them.
+int few_most(int lanes) { return 64 / lanes; }
+bool has_chunks(int64_t tokens, int64_t max_new, int lanes) { return tokens >= 64 && max_new > few_most(lanes); }
+
+}  // namespace
+
 extern "C" int64_t da_paged_attn_workspace_size(int64_t tokens, int64_t B, int64_t table_cols, int page, int64_t max_new,
-                                                int H, int R, int D, int maps) {
+                                                int H, int R, int D, int maps, int per_map) {
   if (!attn_shape(H, R, D, maps) || tokens < 0 || B < 0 || table_cols < 0 || page < 1) return -1;
   if (tokens == 0 || B == 0) return 0;
   if (max_new < 1 || max_new > tokens) max_new = tokens;
-  return few_workspace(few_plan(tokens, B, table_cols * page, max_new, H * R, D, lanes_of(maps)), D);
+  const int lanes = lanes_of(maps);
+  const int64_t chunks = has_chunks(tokens, max_new, lanes) ? paged::chunk_workspace(tokens, B, few_most(lanes), D, maps, per_map) : 0;
+  return chunks + few_workspace(few_plan(tokens, B, table_cols * page, max_new, H * R, D, lanes), D);
 }
 
 extern "C" int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_row_stride, int64_t tokens,
@@ -685,11 +698,15 @@ extern "C" int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_r
     if (reinterpret_cast<uintptr_t>(a) % 16) return DA_ERR_ALIGN;
   if (q_row_stride % 8 || (H > 1 && q_branch_stride % 8)) return DA_ERR_ALIGN;
   if (tokens == 0) return DA_OK;
-  if (B == 0 || B > 0x7fffffff / 64) return DA_ERR_SHAPE;
+  if (B == 0 || B > 0x7fffffff / 64 || table_cols < 1) return DA_ERR_SHAPE;
   if (max_new < 1 || max_new > tokens) max_new = tokens;
   if (int rc = bind_device(key_pages)) return rc;
-  const FewPlan f = few_plan(tokens, B, p.c.capacity, max_new, H * R, D, lanes_of(maps));
-  if (workspace_bytes < few_workspace(f, D) || (few_workspace(f, D) && !workspace)) return DA_ERR_WORKSPACE;
+  const int lanes = lanes_of(maps);
+  const bool chunked = has_chunks(tokens, max_new, lanes);
+  const FewPlan f = few_plan(tokens, B, p.c.capacity, max_new, H * R, D, lanes);
+  const int64_t chunk_bytes = chunked ? paged::chunk_workspace(tokens, B, few_most(lanes), D, maps, per_map) : 0;
+  const int64_t need = chunk_bytes + few_workspace(f, D);
+  if (workspace_bytes < need || (need && !workspace)) return DA_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return DA_ERR_ALIGN;
   p.q = q;
   p.q_branch = q_branch_stride;
@@ -697,15 +714,17 @@ extern "C" int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_r
   p.scales = scales;
   p.weights = per_map ? nullptr : weights;
   p.y = y;
-  p.part = static_cast<float*>(workspace);
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + chunk_bytes);
   p.status = status;
   p.H = H;
   p.R = R;
   p.D = D;
   p.maps = maps;
   p.group = H >= maps ? H / maps : 1;
-  p.lanes = lanes_of(maps);
-  p.few_most = 0x7fffffff;
+  p.lanes = lanes;
+  p.few_most = chunked ? few_most(lanes) : 0x7fffffff;
+  p.chunked = chunked;
+  if (chunked) p.chunks = paged::chunk_plan(workspace, tokens, B, p.few_most);
   p.few_rows = f.few_rows;
   p.stages = f.stages;
   p.stage_bytes = f.stage_bytes;
@@ -724,6 +743,11 @@ extern "C" int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_r
     if (int rc = make_tmap_blocks(i ? &tv : &tk, i ? value_pages : key_pages, dt, 2, 3, dims, strides, box)) return rc;
   }
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (chunked) {
+    const paged::ChunkArgs a{p.c, q, q_branch_stride, q_row_stride, key_pages, value_pages, dtype, H, R, D, maps, p.group,
+                             scales, weights, per_map, y, p.few_most, workspace, status};
+    if (int rc = paged::chunk_attention(a, st)) return rc;
+  }
   if (dtype == DA_BF16)
     return D == 512   ? launch_few<__nv_bfloat16, 8>(p, f, tk, tv, st)
            : D == 256 ? launch_few<__nv_bfloat16, 4>(p, f, tk, tv, st)

@@ -1,0 +1,50 @@
+// What the two attention kernels over a paged cache share: which sequences each takes, and the plan of the chunks.
+#pragma once
+
+#include "paged.cuh"
+
+namespace da {
+namespace paged {
+
+// The chunk kernel's plan, made on the device from the step's lengths: `head` is {pieces, tiles, 0, 0}; sequence b's tiles
+// of 128 tokens have pieces seq_piece[b] .. seq_piece[b + 1], tile k the pieces tile_piece[k] .. tile_piece[k + 1];
+// piece i is {sequence, tile of the sequence, first key tile, key tiles} and {first piece of its tile, pieces of its
+// tile, 0, 0}.  odd[2 * piece + rank] says that live rows of that CTA came out NaN.
+struct Plan {
+  int* head;
+  int* seq_piece;
+  int* tile_piece;
+  int4* pieces;
+  int* odd;
+  int tiles_most, pieces_most;
+};
+
+struct ChunkArgs {
+  Cache c;
+  const void* q;
+  int64_t q_branch, q_row;
+  const void *key_pages, *value_pages;
+  int dtype, H, R, D, maps, group;
+  const float *scales, *weights;
+  int per_map;
+  void* y;
+  int few_most;  // sequences with at most that many new tokens are the other kernel's
+  void* workspace;
+  int* status;
+};
+
+// Bytes of the workspace for steps of `tokens` rows and B sequences (a multiple of 16).
+int64_t chunk_workspace(int64_t tokens, int64_t B, int few_most, int D, int maps, bool per_map);
+Plan chunk_plan(void* workspace, int64_t tokens, int64_t B, int few_most);
+int chunk_attention(const ChunkArgs& a, cudaStream_t st);
+
+// Whether the chunk kernel left NaN in live rows of sequence b, the other kernel's to compute again: a masked value that is no
+// number spoils the rows of a matrix product, which weigh it with 0.
+DA_DEV bool left_odd(const Plan& p, int b) {
+  int any = 0;
+  for (int i = 2 * p.seq_piece[b]; i < 2 * p.seq_piece[b + 1]; ++i) any |= p.odd[i];
+  return any != 0;
+}
+
+}  // namespace paged
+}  // namespace da

@@ -9,7 +9,7 @@ tokens to long chunks.  :class:`RoutedCache` holds the pages of all layers of a 
 
 The sizes that vary from step to step are read by the kernels on the device: no call waits for the GPU, and a captured
 graph follows them.  A page number outside the cache, or a length that the table has no room for, is never followed:
-those positions are not written, the tokens that would need them get NaN, and ``ops.device_status`` reports bit 8.
+those positions are not written, the tokens that would need them (and others of their tile of 128 new tokens) get NaN, and ``ops.device_status`` reports bit 8.
 
 Inference only: the operators raise on tensors that require a gradient.
 """
@@ -50,6 +50,8 @@ def _check_batch(name: str, batch: PagedBatch) -> int:
         if t.dtype != torch.int32:
             raise ValueError(f"{name} takes its {what} in int32, got {t.dtype}")
     b = lengths.shape[0] if lengths.ndim == 1 else -1
+    if table.ndim == 2 and not table.shape[1]:
+        raise ValueError(f"{name} takes a table of at least one page a sequence")
     if table.ndim != 2 or table.shape[0] != b or starts.shape != (b + 1,):
         raise ValueError(f"{name} takes a table [B, pages], lengths [B] and starts [B + 1], got {tuple(table.shape)}, "
                          f"{tuple(lengths.shape)} and {tuple(starts.shape)}")
@@ -111,8 +113,9 @@ def append_paged(keys: Tensor, values: Tensor, key_pages: Tensor, value_pages: T
 
 def _aligned_query(q: Tensor) -> Tensor:
     """``q`` [H, N, R] with branches and rows on 16 bytes: as it lies, or a copy."""
-    if (q.stride(2) != 1 or q.data_ptr() % 16 or (q.shape[1] > 1 and q.stride(1) % 8)
-            or (q.shape[0] > 1 and q.stride(0) % 8)):
+    h, n, r = q.shape
+    if q.stride(2) != 1 or q.data_ptr() % 16 or n > 1 and (q.stride(1) % 8 or q.stride(1) < r) \
+            or h > 1 and (q.stride(0) % 8 or q.stride(0) < r):
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
@@ -163,7 +166,7 @@ def routed_attention_paged(query: Tensor, key_pages: Tensor, value_pages: Tensor
     table, lengths, starts = _table_args(batch)
     most = n if batch.max_new is None else batch.max_new
     with torch.cuda.device(device):
-        need = _lib.lib().da_paged_attn_workspace_size(n, b, table.shape[1], page, most, h, r, d, maps)
+        need = _lib.lib().da_paged_attn_workspace_size(n, b, table.shape[1], page, most, h, r, d, maps, int(per_map))
     work = torch.empty(need, dtype=torch.uint8, device=query.device) if need > 0 else None
     _launch(device, "da_paged_attn", query.data_ptr(), query.stride(0), query.stride(1), n, key_pages.data_ptr(),
             value_pages.data_ptr(), _CODES[query.dtype], pages, page, h, r, d, maps, table.data_ptr(),

@@ -576,7 +576,7 @@ DA_API int da_paged_append(const void* keys, int key_dtype, int64_t key_branch_s
  * limit.  workspace: da_paged_attn_workspace_size bytes (same arguments, same current device), 16-byte
  * aligned. */
 DA_API int64_t da_paged_attn_workspace_size(int64_t tokens, int64_t B, int64_t table_cols, int page, int64_t max_new, int H,
-                                            int R, int D, int maps);
+                                            int R, int D, int maps, int per_map);
 DA_API int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_row_stride, int64_t tokens, const void* key_pages,
                          const void* value_pages, int dtype, int64_t pages, int page, int H, int R, int D, int maps,
                          const int* table, int64_t table_stride, int64_t table_cols, const int* lengths, const int* starts,

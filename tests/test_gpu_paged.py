@@ -22,9 +22,9 @@ BF16, FP16 = torch.bfloat16, torch.float16
 
 
 class Case:
-    """A cache whose unused slots hold NaN, sequences of ``held`` tokens and ``new`` more, all random."""
+    """A cache whose unused slots hold ``fill``, sequences of ``held`` tokens and ``new`` more, all random."""
 
-    def __init__(self, h, s, r, d, page, dtype, held, new, *, scale=16.0, norm=1.0, seed=0, behind=0):
+    def __init__(self, h, s, r, d, page, dtype, held, new, *, scale=16.0, norm=1.0, seed=0, behind=0, fill=math.nan):
         g = torch.Generator("cuda").manual_seed(seed)
         rand = lambda *shape: torch.randn(*shape, device="cuda", generator=g)  # noqa: E731
         self.h, self.s, self.r, self.d, self.page, self.held, self.new = h, s, r, d, page, held, new
@@ -42,8 +42,8 @@ class Case:
         unit = lambda t: (norm * t / t.norm(dim=-1, keepdim=True)).to(dtype)  # noqa: E731
         self.q, self.k = unit(rand(h, n, r)), unit(rand(h, n, r))
         self.v = rand(n, d).to(dtype)
-        self.key_pages = torch.full((pages, page, h, r), math.nan, dtype=dtype, device="cuda")
-        self.value_pages = torch.full((pages, page, d), math.nan, dtype=dtype, device="cuda")
+        self.key_pages = torch.full((pages, page, h, r), fill, dtype=dtype, device="cuda")
+        self.value_pages = torch.full((pages, page, d), fill, dtype=dtype, device="cuda")
         self.old = []
         for b, a in enumerate(held):
             k, v = unit(rand(a, h, r)), rand(a, d).to(dtype)
@@ -128,10 +128,15 @@ def test_lengths_around_tiles_and_pages(shape, held, new) -> None:
 @pytest.mark.parametrize(("shape", "held", "new"), [((1, 1, 256, 512, 64), [0], [300]), ((1, 1, 512, 512, 128), [700], [129]),
                                                     ((4, 4, 128, 512, 32), [0, 900, 31], [256, 130, 1]),
                                                     ((1, 2, 256, 256, 16), [65, 0], [127, 128]),
-                                                    ((2, 1, 128, 128, 64), [5000], [200]), ((1, 1, 64, 512, 16), [40], [1000])])
+                                                    ((2, 1, 128, 128, 64), [5000], [200]), ((1, 1, 64, 512, 16), [40], [1000]),
+                                                    ((1, 1, 256, 512, 64), [3, 9000, 0, 700], [2, 65, 257, 1030]),
+                                                    ((4, 4, 128, 512, 64), [2, 6000, 0, 700], [20, 65, 257, 630]),
+                                                    ((3, 3, 128, 256, 128), [513], [300]), ((4, 2, 64, 128, 256), [513], [300]),
+                                                    ((1, 1, 192, 256, 64), [513, 0], [300, 128])])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
-def test_chunks(shape, held, new, dtype) -> None:
-    case = Case(*shape, dtype, held, new, seed=2)
+@pytest.mark.parametrize("fill", [math.nan, 30000.0])
+def test_chunks(shape, held, new, dtype, fill) -> None:
+    case = Case(*shape, dtype, held, new, seed=2, fill=fill)
     case.append()
     case.check(case.attend())
     case.check(case.attend(batch=case.batch._replace(max_new=None)))
@@ -141,7 +146,7 @@ def test_chunks(shape, held, new, dtype) -> None:
 @pytest.mark.parametrize("new", [[1, 3], [200, 2]])
 @pytest.mark.parametrize("shape", [(2, 2, 128, 256, 32), (4, 4, 128, 512, 64), (1, 3, 64, 128, 16)])
 def test_outputs_of_each_map(shape, new) -> None:
-    case = Case(*shape, BF16, [100, 2000], new, seed=3)
+    case = Case(*shape, BF16, [100, 2000], new, seed=3, fill=5.0)
     case.append()
     y = case.attend(weights=None)
     assert y.shape == (sum(new), case.s, case.d)
@@ -152,9 +157,29 @@ def test_outputs_of_each_map(shape, new) -> None:
 @pytest.mark.parametrize("norm", [30.0, 1e-3])
 def test_scores_of_any_size(norm, new) -> None:
     """Sharp rows, whose largest score lies hundreds above the others, and flat ones."""
-    case = Case(2, 2, 128, 256, 32, BF16, [600, 77], new, norm=norm, seed=4, scale=1.0 if norm > 1 else 16.0)
-    case.append()
-    case.check(case.attend())
+    for h, s in ((1, 1), (2, 2)):
+        case = Case(h, s, 128, 256, 32, BF16, [600, 77], new, norm=norm, seed=4, scale=1.0 if norm > 1 else 16.0, fill=5.0)
+        case.append()
+        case.check(case.attend())
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_a_maximum_that_grows_along_the_keys(dtype) -> None:
+    """Every key tile's scores lie far above the tile's before it, so that all earlier weights fade."""
+    for h, s in ((1, 1), (2, 2)):
+        case = Case(h, s, 128, 512, 64, dtype, [2500], [300], seed=15, fill=5.0)
+        k, v = case.old[0]
+        ramp = torch.linspace(0.05, 8.0, 2800, device="cuda")[:, None, None]
+        direction = torch.nn.functional.normalize(torch.ones(128, device="cuda"), dim=0)
+        noise = 0.02 * torch.randn(2800, h, 128, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+        keys = (ramp * direction + noise).to(dtype)
+        case.old[0] = (keys[:2500], v)
+        case.key_pages.view(-1, h, 128)[case.slots(0, range(2500))] = keys[:2500]
+        case.k = keys[2500:].transpose(0, 1)
+        case.q = (0.3 * case.q.float() + direction).to(dtype)
+        case.norm = 8.5**0.5 * 1.4**0.5  # of the product |q| |k|
+        case.append()
+        case.check(case.attend())
 
 
 @pytest.mark.parametrize("new", [[6, 40], [200, 170]])
