@@ -24,10 +24,11 @@ namespace da {
 namespace paged {
 
 constexpr int kKeys = 32;      // positions a tile
-constexpr int kWarps = 8;      // computing warps; one more brings the tiles
+constexpr int kScoreWarps = 4, kValueWarps = 4;  // and one warp that brings the tiles
+constexpr int kThreads = 32 * (kScoreWarps + kValueWarps + 1);
 constexpr int kMaxStages = 8;
-constexpr int kRedPitch = 36;  // floats a row of partial scores
 constexpr int kPPitch = 40;    // 16-bit weights a row
+constexpr float kGrow = 8.f;   // log2 of the growth of a row's maximum that its output bears
 
 struct FewParams {
   Cache c;
@@ -134,27 +135,31 @@ DA_DEV int64_t job_end(const Cache& c, const Sequence& s, int job, int tokens) {
   return e < c.capacity ? e : c.capacity;
 }
 
-// kNT: n-tiles of 8 value columns a warp (D = 64 kNT).
-template <typename T, int kNT>
-__global__ void __launch_bounds__(32 * (kWarps + 1), 2) few_kernel(const __grid_constant__ CUtensorMap tk,
-                                                                  const __grid_constant__ CUtensorMap tv,
-                                                                  const FewParams p) {
+// kSteps: column steps of 16 that the queries' registers hold (H R at most 16 kSteps); kNT: value columns in tiles of 8 a
+// warp (D = 32 kNT); kCtas: CTAs an SM.
+template <typename T, int kSteps, int kNT, int kCtas>
+__global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_constant__ CUtensorMap tk,
+                                                             const __grid_constant__ CUtensorMap tv, const FewParams p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* red = reinterpret_cast<float*>(smem + p.stages * p.stage_bytes);    // [8][16][kRedPitch]
-  uint16_t* weight = reinterpret_cast<uint16_t*>(red + kWarps * 16 * kRedPitch);  // [16][kPPitch]
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages];
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], p_full[2], p_empty[2];
   __shared__ int bad[kMaxStages];  // the tile's pages are not all in the cache
-  __shared__ float rescale[16], row_max[16], row_sum[16];
+  __shared__ __align__(16) uint16_t weight[2][16 * kPPitch];
+  __shared__ __align__(16) float warp_max[2][16][kScoreWarps];
+  __shared__ float rescale[2][16], row_max[16], row_sum[kScoreWarps][16];
   __shared__ int64_t buf[32], start_off;
-  __shared__ int start_b, abort_flag;
+  __shared__ int start_b, abort_flag, piece_bad;
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   if (tid == 0) {
     abort_flag = 0;
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kWarps);
+      mbar_init(&empty[i], kValueWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&p_full[i], kScoreWarps);
+      mbar_init(&p_empty[i], kValueWarps);
     }
     fence_mbar_init();
   }
@@ -162,7 +167,6 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2) few_kernel(const __grid_
   grid_launch_dependents();
 
   // ---- this CTA's share of the flat list of tiles
-  constexpr int kThreads = 32 * (kWarps + 1);
   int64_t mine = 0;
   for (int b = tid; b < p.c.B; b += kThreads) mine += sequence_tiles(p, sequence(p.c, b), b);
   const int64_t total = block_sum<kThreads>(mine, buf);
@@ -192,7 +196,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2) few_kernel(const __grid_
       __syncthreads();
       int64_t at = before + inc - v, all = 0;
 #pragma unroll
-      for (int i = 0; i <= kWarps; ++i) {
+      for (int i = 0; i < kThreads / 32; ++i) {
         if (i < warp) at += buf[i];
         all += buf[i];
       }
@@ -209,27 +213,35 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2) few_kernel(const __grid_
   Abort ab{&abort_flag, p.status};
   const int tokens = 16 / p.lanes;
   Piece x;
-  int it = 0;  // tiles so far: stage it % stages
+  int st = 0;         // stage of the next tile
+  uint32_t phase = 0;  // of its barriers
+  auto next_stage = [&]() {
+    if (++st == p.stages) {
+      st = 0;
+      phase ^= 1;
+    }
+  };
+  const int key_box = p.brow * 2 * p.H * p.R, value_box = p.brow * 2 * p.D, block = p.brow * 128;
 
-  if (warp == kWarps) {
+  if (warp == kScoreWarps + kValueWarps) {
     // ---------------------------------------------------------------- brings the tiles
     if (lane == 0) {
       prefetch_tmap(&tk);
       prefetch_tmap(&tv);
     }
     bool ok = true;
+    int brought = 0;
+    const int boxes = kKeys / p.brow;
     while (ok && next_piece(p, walk, x)) {
       const int64_t end = job_end(p.c, x.s, x.job, tokens);
       const int t1 = min(x.t1, (int)((end + kKeys - 1) / kKeys));
       const int* row = p.c.table + x.b * p.c.table_stride;
-      const int boxes = kKeys / p.brow;
       int cached = -1, entry = 0;  // this lane's entry of the 32 pages from `cached` on
-      for (int t = x.t0; ok && t < t1; ++t, ++it) {
-        const int st = it % p.stages;
-        if (lane == 0) ok = mbar_wait(&empty[st], ((it / p.stages) & 1u) ^ 1u, ab, 61);
+      for (int t = x.t0; t < t1; ++t, ++brought, next_stage()) {
+        if (lane == 0) ok = mbar_wait(&empty[st], phase ^ 1u, ab, 61);
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
         if (!ok) break;
-        // pages of the boxes (a box lies in one page); positions past `end` in no page are not fetched
+        // pages of the boxes (a box lies in one page); boxes past `end` are not fetched
         const int64_t pos = (int64_t)t * kKeys;
         const int first = (int)(pos >> p.c.page_shift);
         if (cached < 0 || first >= cached + 31) {
@@ -252,14 +264,13 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2) few_kernel(const __grid_
         }
         if (lane == 0) {
           bad[st] = wrong;
-          if (wrong) atomicOr(p.status, DA_DEV_BAD_PAGE);
-          mbar_arrive_expect_tx(&full[st], good * p.brow * 2 * (p.H * p.R + p.D));
+          mbar_arrive_expect_tx(&full[st], good * (key_box + value_box));
           uint8_t* base = smem + st * p.stage_bytes;
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             if (slot[u] < 0) continue;
-            tma_load_3d(&tk, &full[st], base + u * p.brow * 2 * p.H * p.R, 0, slot[u], 0);
-            tma_load_3d(&tv, &full[st], base + p.key_bytes + u * p.brow * 2 * p.D, 0, slot[u], 0);
+            tma_load_3d(&tk, &full[st], base + u * key_box, 0, slot[u], 0);
+            tma_load_3d(&tv, &full[st], base + p.key_bytes + u * value_box, 0, slot[u], 0);
           }
         }
         __syncwarp();
@@ -267,142 +278,194 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2) few_kernel(const __grid_
     }
     // the last tiles' loads land before the CTA's shared memory is given back
     if (lane == 0)
-      for (int i = it > p.stages ? it - p.stages : 0; i < it; ++i) mbar_wait_drain(&full[i % p.stages], (i / p.stages) & 1u);
+      for (int i = 0; i < min(brought, p.stages); ++i) {
+        if (st-- == 0) {
+          st = p.stages - 1;
+          phase ^= 1;
+        }
+        mbar_wait_drain(&full[st], phase);
+      }
     return;
   }
 
-  // ------------------------------------------------------------------ computes
   const int g = lane / 4, pair = (lane % 4) * 2;
-  const int steps = p.H * p.R / 16;  // of the score product
-  const float kLog2e = 1.4426950408889634f;
-  const int shift_lanes = p.lanes == 1 ? 0 : p.lanes == 2 ? 1 : 2;
-  const int token_of = tokens - 1, map_shift = 4 - shift_lanes;  // row r: map r >> map_shift, token r & token_of
+  const int map_shift = p.lanes == 1 ? 4 : p.lanes == 2 ? 3 : 2, token_of = tokens - 1;
+  // row r: map r >> map_shift, token r & token_of
+  const int s0 = g >> map_shift, s1 = (g + 8) >> map_shift, k0 = g & token_of, k1 = (g + 8) & token_of;
+  uint32_t tile_phase = 0;  // of p_full and p_empty, buffer `pb`
+  int pb = 0;
   // (After a wait that gave up every warp still walks all pieces, its waits failing at once: the barriers meet.)
-  bool ok = true, first_piece = true;
+
+  if (warp < kScoreWarps) {
+    // ------------------------------------------------------------------ scores and weights of 8 positions a warp
+    const int steps = p.H * p.R / 16;
+    const float kLog2e = 1.4426950408889634f;
+    const float scale0 = s0 < p.maps ? p.scales[s0] * rsqrtf((float)p.group) * kLog2e : 0.f;
+    const float scale1 = s1 < p.maps ? p.scales[s1] * rsqrtf((float)p.group) * kLog2e : 0.f;
+    const int key = warp * 8 + (lane & 7), kr = p.brow == 32 ? key : key & 15;
+    const uint32_t key_off = (p.brow == 32 ? 0 : (key >> 4) * key_box) + kr * 128 + (((lane >> 3) ^ (kr & 7)) << 4);
+    while (next_piece(p, walk, x)) {
+      const int64_t end = job_end(p.c, x.s, x.job, tokens);
+      const int t1 = min(x.t1, (int)((end + kKeys - 1) / kKeys));
+      const int64_t q0 = x.s.first + (int64_t)x.job * tokens;  // packed row of the job's first token
+      const int live = min(tokens, x.s.n - x.job * tokens);
+      const bool on0 = s0 < p.maps && k0 < live, on1 = s1 < p.maps && k1 < live;
+      const int64_t sees0 = on0 ? min(x.s.held + x.job * tokens + k0 + 1, end) : 0;
+      const int64_t sees1 = on1 ? min(x.s.held + x.job * tokens + k1 + 1, end) : 0;
+      uint32_t qf[kSteps][4];
+      {
+        const int h0 = p.H >= p.maps ? s0 * p.group : s0 * p.H / p.maps, h1 = p.H >= p.maps ? s1 * p.group : s1 * p.H / p.maps;
+        const T* q = static_cast<const T*>(p.q);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const int h = i * 16 / p.R;  // (a step lies in one branch)
+          const int64_t at = h * p.q_branch + (i * 16 - h * p.R) + pair;
+          const bool in0 = on0 && i < steps && h >= h0 && h < h0 + p.group, in1 = on1 && i < steps && h >= h1 && h < h1 + p.group;
+          const T *r0 = q + at + (q0 + k0) * p.q_row, *r1 = q + at + (q0 + k1) * p.q_row;
+          qf[i][0] = in0 ? *reinterpret_cast<const uint32_t*>(r0) : 0;
+          qf[i][1] = in1 ? *reinterpret_cast<const uint32_t*>(r1) : 0;
+          qf[i][2] = in0 ? *reinterpret_cast<const uint32_t*>(r0 + 8) : 0;
+          qf[i][3] = in1 ? *reinterpret_cast<const uint32_t*>(r1 + 8) : 0;
+        }
+      }
+      float ref0 = -INFINITY, ref1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // rows g and g + 8: offsets, this thread's sums
+      bool wrong = !x.s.fits, ok = true;
+      for (int t = x.t0; t < t1; ++t, next_stage()) {
+        ok &= mbar_wait(&full[st], phase, ab, 62);
+        __syncwarp();
+        wrong |= bad[st] != 0;
+        const uint32_t kb = smem_u32(smem + st * p.stage_bytes) + key_off;
+        float sc[4][4];  // four sums, so that no product waits for the one before it
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSteps / 2; ++i) {
+          if (2 * i < steps) {
+            uint32_t b[4];
+            ldmatrix4(b, (kb + (i >> 1) * block) ^ ((i & 1) << 6));
+            mma16816<T>(sc[(2 * i) & 3], qf[2 * i], b[0], b[1]);
+            mma16816<T>(sc[(2 * i + 1) & 3], qf[2 * i + 1], b[2], b[3]);
+          }
+        }
+        const int64_t at = (int64_t)t * kKeys + warp * 8 + pair;
+        const float v00 = at < sees0 ? (sc[0][0] + sc[1][0] + (sc[2][0] + sc[3][0])) * scale0 : -INFINITY;
+        const float v01 = at + 1 < sees0 ? (sc[0][1] + sc[1][1] + (sc[2][1] + sc[3][1])) * scale0 : -INFINITY;
+        const float v10 = at < sees1 ? (sc[0][2] + sc[1][2] + (sc[2][2] + sc[3][2])) * scale1 : -INFINITY;
+        const float v11 = at + 1 < sees1 ? (sc[0][3] + sc[1][3] + (sc[2][3] + sc[3][3])) * scale1 : -INFINITY;
+        float top0 = fmaxf(v00, v01), top1 = fmaxf(v10, v11);
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, o));
+          top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
+        }
+        if ((lane & 3) == 0) {
+          warp_max[pb][g][warp] = top0;
+          warp_max[pb][g + 8][warp] = top1;
+        }
+        named_bar_sync(1, 32 * kScoreWarps);
+        const float4 w0 = *reinterpret_cast<const float4*>(warp_max[pb][g]), w1 = *reinterpret_cast<const float4*>(warp_max[pb][g + 8]);
+        top0 = fmaxf(fmaxf(w0.x, w0.y), fmaxf(w0.z, w0.w));
+        top1 = fmaxf(fmaxf(w1.x, w1.y), fmaxf(w1.z, w1.w));
+        float c0 = 1.f, c1 = 1.f;
+        if (top0 > ref0 + kGrow || (ref0 == -INFINITY && top0 > ref0)) {
+          c0 = ref0 == -INFINITY ? 1.f : ex2(ref0 - top0);
+          ref0 = top0;
+        }
+        if (top1 > ref1 + kGrow || (ref1 == -INFINITY && top1 > ref1)) {
+          c1 = ref1 == -INFINITY ? 1.f : ex2(ref1 - top1);
+          ref1 = top1;
+        }
+        const float off0 = ref0 == -INFINITY ? 0.f : ref0, off1 = ref1 == -INFINITY ? 0.f : ref1;
+        const float p00 = ex2(v00 - off0), p01 = ex2(v01 - off0), p10 = ex2(v10 - off1), p11 = ex2(v11 - off1);
+        l0 = fmaf(l0, c0, p00 + p01);
+        l1 = fmaf(l1, c1, p10 + p11);
+        ok &= mbar_wait(&p_empty[pb], tile_phase ^ 1u, ab, 63);
+        __syncwarp();
+        *reinterpret_cast<uint32_t*>(&weight[pb][g * kPPitch + warp * 8 + pair]) = pack2<T>(p00, p01);
+        *reinterpret_cast<uint32_t*>(&weight[pb][(g + 8) * kPPitch + warp * 8 + pair]) = pack2<T>(p10, p11);
+        if (warp == 0 && (lane & 3) == 0) {
+          rescale[pb][g] = c0;
+          rescale[pb][g + 8] = c1;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[pb]);
+        pb ^= 1;
+        tile_phase ^= pb == 0;
+      }
+      // ---- the piece's maxima and sums
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+      }
+      if (!ok) l0 = l1 = NAN;
+      if ((lane & 3) == 0) {
+        row_sum[warp][g] = l0;
+        row_sum[warp][g + 8] = l1;
+        if (warp == 0) {
+          row_max[g] = ref0;
+          row_max[g + 8] = ref1;
+        }
+      }
+      if (tid == 0) {
+        piece_bad = wrong;
+        if (wrong) atomicOr(p.status, DA_DEV_BAD_PAGE);
+      }
+      named_bar_sync(2, 32 * (kScoreWarps + kValueWarps));
+      named_bar_sync(2, 32 * (kScoreWarps + kValueWarps));  // they are read
+    }
+    return;
+  }
+
+  // ------------------------------------------------------------------ outputs of D / 4 columns a warp
+  const int w4 = warp - kScoreWarps, col0 = w4 * (kNT * 8);
+  const int kr = lane & 15;  // position of a half tile (a box of 16, or half of one of 32)
+  const uint32_t value_off = (col0 >> 6) * block + kr * 128 + (((((col0 & 63) >> 3) | (lane >> 4)) ^ (kr & 7)) << 4);
+  const uint32_t half_off = p.brow == 32 ? 16 * 128 : value_box;
+  bool first_piece = true;
   while (next_piece(p, walk, x)) {
     const int64_t end = job_end(p.c, x.s, x.job, tokens);
     const int t1 = min(x.t1, (int)((end + kKeys - 1) / kKeys));
-    const int64_t q0 = x.s.first + (int64_t)x.job * tokens;  // packed row of the job's first token
+    const int64_t q0 = x.s.first + (int64_t)x.job * tokens;
     const int live = min(tokens, x.s.n - x.job * tokens);
-    // queries of this warp's column steps
-    uint32_t qf[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int ks = warp + 8 * i;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        qf[i][e] = 0;
-        const int r = g + 8 * (e & 1), s = r >> map_shift, t = r & token_of;
-        if (ks < steps && s < p.maps && t < live) {
-          const int col = ks * 16 + pair + 8 * (e >> 1), h = col / p.R;
-          const int h0 = p.H >= p.maps ? s * p.group : s * p.H / p.maps;
-          if (h >= h0 && h < h0 + p.group)
-            qf[i][e] = *reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + h * p.q_branch + (q0 + t) * p.q_row +
-                                                          (col - h * p.R));
-        }
-      }
-    }
-    // the two rows whose softmax this warp runs
-    float m[2], l[2], scale[2];
-    int64_t sees[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = 2 * warp + i, s = r >> map_shift, t = r & token_of;
-      m[i] = -INFINITY;
-      l[i] = 0.f;
-      const bool on = s < p.maps && t < live;
-      scale[i] = on ? p.scales[s] * rsqrtf((float)p.group) * kLog2e : 0.f;
-      sees[i] = on ? min(x.s.held + x.job * tokens + t + 1, end) : 0;
-    }
     float acc[kNT][4];
 #pragma unroll
     for (int i = 0; i < kNT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
-    bool wrong = !x.s.fits;
-
-    for (int t = x.t0; t < t1; ++t, ++it) {
-      const int st = it % p.stages;
-      ok &= mbar_wait(&full[st], (it / p.stages) & 1u, ab, 62);
-      __syncwarp();
-      const uint32_t kb = smem_u32(smem + st * p.stage_bytes), vb = kb + p.key_bytes;
+    bool ok = true;
+    for (int t = x.t0; t < t1; ++t, next_stage()) {
+      ok &= mbar_wait(&full[st], phase, ab, 64);
+      const uint32_t vb = smem_u32(smem + st * p.stage_bytes) + p.key_bytes;
       const int64_t pos = (int64_t)t * kKeys;
-      wrong |= bad[st] != 0;
-      // ---- partial scores over this warp's columns
-      float sc[4][4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int ks = warp + 8 * i;
-        if (ks < steps) {
-#pragma unroll
-          for (int n2 = 0; n2 < 2; ++n2) {
-            const int key = n2 * 16 + (lane & 7) + ((lane >> 4) << 3);
-            const int box = p.brow == 32 ? 0 : key >> 4, kr = p.brow == 32 ? key : key & 15;
-            uint32_t b[4];
-            ldmatrix4(b, kb + box * (p.brow * 2 * p.H * p.R) + (ks >> 2) * (p.brow * 128) +
-                             sw128_offset(kr, (ks & 3) * 2 + ((lane >> 3) & 1)));
-            mma16816<T>(sc[2 * n2], qf[i], b[0], b[1]);
-            mma16816<T>(sc[2 * n2 + 1], qf[i], b[2], b[3]);
-          }
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        float* at = red + (warp * 16 + g) * kRedPitch + n * 8 + pair;
-        *reinterpret_cast<float2*>(at) = make_float2(sc[n][0], sc[n][1]);
-        *reinterpret_cast<float2*>(at + 8 * kRedPitch) = make_float2(sc[n][2], sc[n][3]);
-      }
-      // values of positions that no row sees hold anything: 0 times them must stay 0
-      if (pos + kKeys > end) {
-        for (int i = tid; i < kKeys * kNT * 8; i += 32 * kWarps) {
-          const int key = i / (kNT * 8), chunk = i % (kNT * 8);
+      bool odd = false;
+      // Values of positions that no row sees hold anything: 0 times them must stay 0.  A later token's value that is no
+      // number stays out of the earlier tokens' rows, which 0 times it would spoil.
+      const bool ragged = pos + kKeys > end, mixed = live > 1 && pos + kKeys > x.s.held + (int64_t)x.job * tokens + 1;
+      if (ragged || mixed) {
+        __syncwarp();
+        constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+        for (int i = tid - 32 * kScoreWarps; i < kKeys * kNT * 4; i += 32 * kValueWarps) {
+          const int key = i / (kNT * 4), chunk = i % (kNT * 4);
+          const int box = p.brow == 32 ? 0 : key >> 4, in = p.brow == 32 ? key : key & 15;
+          const uint32_t at = vb + box * value_box + (chunk >> 3) * block + sw128_offset(in, chunk & 7);
           if (pos + key >= end) {
-            const int box = p.brow == 32 ? 0 : key >> 4, kr = p.brow == 32 ? key : key & 15;
-            st_shared_v4(vb + box * (p.brow * 2 * p.D) + (chunk >> 3) * (p.brow * 128) + sw128_offset(kr, chunk & 7), 0, 0, 0, 0);
+            st_shared_v4(at, 0, 0, 0, 0);
+          } else if (mixed) {
+            const uint4 w = ld_shared_v4(at);
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= (ws[e] & kExp) == kExp || ((ws[e] >> 16) & kExp) == kExp;
           }
         }
         fence_proxy_async();
+        odd = named_bar_or(3, 32 * kValueWarps, odd);
       }
-      // A later token's value that is no number stays out of the earlier tokens' rows, which 0 times it would spoil.
-      bool odd = false;
-      if (live > 1 && pos + kKeys > x.s.held + (int64_t)x.job * tokens + 1) {
-        constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
-        for (int i = tid; i < kKeys * kNT * 8; i += 32 * kWarps) {
-          const int key = i / (kNT * 8), chunk = i % (kNT * 8);
-          if (pos + key >= end) continue;
-          const int box = p.brow == 32 ? 0 : key >> 4, kr = p.brow == 32 ? key : key & 15;
-          const uint4 w = ld_shared_v4(vb + box * (p.brow * 2 * p.D) + (chunk >> 3) * (p.brow * 128) + sw128_offset(kr, chunk & 7));
-          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) odd |= (ws[e] & kExp) == kExp || ((ws[e] >> 16) & kExp) == kExp;
-        }
-      }
-      odd = named_bar_or(1, 32 * kWarps, odd);
-      // ---- softmax of two rows a warp, a key a lane
-      const int used = steps < kWarps ? steps : kWarps;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = 2 * warp + i;
-        float v = 0.f;
-        for (int w = 0; w < used; ++w) v += red[(w * 16 + r) * kRedPitch + lane];
-        v = pos + lane < sees[i] ? v * scale[i] : -INFINITY;
-        float top = v;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float next = fmaxf(m[i], top), at = next == -INFINITY ? 0.f : next;
-        const float c = next == -INFINITY ? 1.f : ex2(m[i] - at), e = ex2(v - at);
-        m[i] = next;
-        l[i] = l[i] * c + e;
-        weight[r * kPPitch + lane] = std::is_same<T, __nv_bfloat16>::value ? (uint16_t)pack_bf16x2(e, 0.f) : (uint16_t)pack_f16x2(e, 0.f);
-        if (lane == 0) rescale[r] = c;
-      }
-      named_bar_sync(1, 32 * kWarps);
-      // ---- output columns of this warp
-      const float c0 = rescale[g], c1 = rescale[g + 8];
+      ok &= mbar_wait(&p_full[pb], tile_phase, ab, 65);
+      __syncwarp();
+      const float c0 = rescale[pb][g], c1 = rescale[pb][g + 8];
       if (__any_sync(0xffffffffu, c0 != 1.f || c1 != 1.f)) {
 #pragma unroll
         for (int i = 0; i < kNT; ++i) {
@@ -415,14 +478,14 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2) few_kernel(const __grid_
       if (odd) {
 #pragma unroll 1
         for (int key = 0; key < kKeys; ++key) {
-          const float w0 = unpack2<T>(weight[g * kPPitch + key]).x, w1 = unpack2<T>(weight[(g + 8) * kPPitch + key]).x;
-          const int box = p.brow == 32 ? 0 : key >> 4, kr = p.brow == 32 ? key : key & 15;
+          const float w0 = unpack2<T>(weight[pb][g * kPPitch + key]).x, w1 = unpack2<T>(weight[pb][(g + 8) * kPPitch + key]).x;
+          const int box = p.brow == 32 ? 0 : key >> 4, in = p.brow == 32 ? key : key & 15;
 #pragma unroll
           for (int i = 0; i < kNT; ++i) {
-            const int col = (warp * kNT + i) * 8;
+            const int col = col0 + i * 8;
             uint32_t u;
-            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(u) : "r"(vb + box * (p.brow * 2 * p.D) + (col >> 6) * (p.brow * 128) +
-                                                                    sw128_offset(kr, (col & 63) >> 3) + pair * 2));
+            asm volatile("ld.shared.b32 %0, [%1];"
+                         : "=r"(u) : "r"(vb + box * value_box + (col >> 6) * block + sw128_offset(in, (col & 63) >> 3) + pair * 2));
             const float2 v = unpack2<T>(u);
             acc[i][0] += w0 == 0.f ? 0.f : w0 * v.x;
             acc[i][1] += w0 == 0.f ? 0.f : w0 * v.y;
@@ -430,46 +493,46 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2) few_kernel(const __grid_
             acc[i][3] += w1 == 0.f ? 0.f : w1 * v.y;
           }
         }
-      } else
+      } else {
 #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2) {
-        uint32_t a[4];
-        ldmatrix4(a, smem_u32(weight) + ((lane & 15) * kPPitch + k2 * 16 + (lane >> 4) * 8) * 2);
+        for (int k2 = 0; k2 < 2; ++k2) {
+          uint32_t a[4];
+          ldmatrix4(a, smem_u32(weight[pb]) + ((lane & 15) * kPPitch + k2 * 16 + (lane >> 4) * 8) * 2);
+          const uint32_t at = vb + value_off + k2 * half_off;
 #pragma unroll
-        for (int n2 = 0; n2 < kNT / 2; ++n2) {
-          const int key = k2 * 16 + (lane & 15), col = (warp * kNT + n2 * 2 + (lane >> 4)) * 8;
-          const int box = p.brow == 32 ? 0 : key >> 4, kr = p.brow == 32 ? key : key & 15;
-          uint32_t b[4];
-          ldmatrix4_trans(b, vb + box * (p.brow * 2 * p.D) + (col >> 6) * (p.brow * 128) + sw128_offset(kr, (col & 63) >> 3));
-          mma16816<T>(acc[2 * n2], a, b[0], b[1]);
-          mma16816<T>(acc[2 * n2 + 1], a, b[2], b[3]);
+          for (int n2 = 0; n2 < kNT / 2; ++n2) {
+            uint32_t b[4];
+            ldmatrix4_trans(b, (at + (n2 >> 2) * block) ^ ((n2 & 3) << 5));
+            mma16816<T>(acc[2 * n2], a, b[0], b[1]);
+            mma16816<T>(acc[2 * n2 + 1], a, b[2], b[3]);
+          }
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[st]);
+      if (lane == 0) {
+        mbar_arrive(&p_empty[pb]);
+        mbar_arrive(&empty[st]);
+      }
+      pb ^= 1;
+      tile_phase ^= pb == 0;
     }
 
-    // ---- rows' sums; the job's output, or this piece of it
+    // ---- the job's output, or this piece of it
+    named_bar_sync(2, 32 * (kScoreWarps + kValueWarps));
+    float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int o = 16; o; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
-      if (wrong || !ok) l[i] = NAN;
-      if (lane == 0) {
-        row_max[2 * warp + i] = m[i];
-        row_sum[2 * warp + i] = l[i];
-      }
+    for (int i = 0; i < kScoreWarps; ++i) {
+      sum0 += row_sum[i][g];
+      sum1 += row_sum[i][g + 8];
     }
-    if (wrong && tid == 0) atomicOr(p.status, DA_DEV_BAD_PAGE);
-    named_bar_sync(1, 32 * kWarps);
+    if (piece_bad || !ok) sum0 = sum1 = NAN;
     if (x.t1 - x.t0 == x.tiles) {
-      const int s0 = g >> map_shift, s1 = (g + 8) >> map_shift, k0 = g & token_of, k1 = (g + 8) & token_of;
-      const float w0 = s0 < p.maps ? (p.weights ? p.weights[s0] : 1.f) / row_sum[g] : 0.f;
-      const float w1 = s1 < p.maps ? (p.weights ? p.weights[s1] : 1.f) / row_sum[g + 8] : 0.f;
+      const float w0 = s0 < p.maps ? (p.weights ? p.weights[s0] : 1.f) / sum0 : 0.f;
+      const float w1 = s1 < p.maps ? (p.weights ? p.weights[s1] : 1.f) / sum1 : 0.f;
       T* y = static_cast<T*>(p.y);
 #pragma unroll
       for (int i = 0; i < kNT; ++i) {
-        const int col = (warp * kNT + i) * 8 + pair;
+        const int col = col0 + i * 8 + pair;
         float a0 = s0 < p.maps ? acc[i][0] * w0 : 0.f, a1 = s0 < p.maps ? acc[i][1] * w0 : 0.f;
         float b0 = s1 < p.maps ? acc[i][2] * w1 : 0.f, b1 = s1 < p.maps ? acc[i][3] * w1 : 0.f;
         if (p.per_map) {
@@ -494,22 +557,23 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), 2) few_kernel(const __grid_
     } else {
       const int slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
       float* rows = p.part + (size_t)slot * 16 * p.D;
+      const bool on0 = s0 < p.maps && k0 < live, on1 = s1 < p.maps && k1 < live;
 #pragma unroll
       for (int i = 0; i < kNT; ++i) {
-        const int col = (warp * kNT + i) * 8 + pair;
-        if ((g & token_of) < live && (g >> map_shift) < p.maps)
-          *reinterpret_cast<float2*>(rows + g * p.D + col) = make_float2(acc[i][0], acc[i][1]);
-        if (((g + 8) & token_of) < live && ((g + 8) >> map_shift) < p.maps)
-          *reinterpret_cast<float2*>(rows + (g + 8) * p.D + col) = make_float2(acc[i][2], acc[i][3]);
+        const int col = col0 + i * 8 + pair;
+        if (on0) *reinterpret_cast<float2*>(rows + g * p.D + col) = make_float2(acc[i][0], acc[i][1]);
+        if (on1) *reinterpret_cast<float2*>(rows + (g + 8) * p.D + col) = make_float2(acc[i][2], acc[i][3]);
       }
       float* ml = p.part + (size_t)2 * p.ctas * 16 * p.D + (size_t)slot * 32;
-      if (tid < 16) {
-        ml[tid] = row_max[tid];
-        ml[16 + tid] = row_sum[tid];
+      if (w4 == 0 && (lane & 3) == 0) {
+        ml[g] = row_max[g];
+        ml[g + 8] = row_max[g + 8];
+        ml[16 + g] = sum0;
+        ml[24 + g] = sum1;
       }
     }
     first_piece = false;
-    named_bar_sync(1, 32 * kWarps);  // row_max and row_sum are free again
+    named_bar_sync(2, 32 * (kScoreWarps + kValueWarps));  // row_max and row_sum are free again
   }
 }
 
@@ -613,21 +677,18 @@ struct FewPlan {
   int stages, stage_bytes, key_bytes, smem, ctas, few_rows;
 };
 
-constexpr int kFixedBytes = paged::kWarps * 16 * paged::kRedPitch * 4 + 16 * paged::kPPitch * 2 + 1024;
+// Two CTAs an SM where queries and outputs leave registers for them (H R and D up to 256): one computes while the other
+// waits.  Shared memory holds as many tiles as fit.
+int ctas_per_sm(int wide, int D) { return wide <= 256 && D <= 256 ? 2 : 1; }
 
-// Shared memory holds as many tiles as fit, at least two, in one CTA an SM -- or in two or three CTAs an SM where their
-// tiles are small, so that one computes while another waits at a barrier.
 FewPlan few_plan(int64_t tokens, int64_t B, int64_t capacity, int64_t max_new, int wide, int D, int lanes) {
   FewPlan f;
   f.key_bytes = paged::kKeys * 2 * wide;
   f.stage_bytes = f.key_bytes + paged::kKeys * 2 * D;
-  int per_sm = 3;
-  for (;; --per_sm) {
-    f.stages = (228 * 1024 / per_sm - 2304 - kFixedBytes) / f.stage_bytes;  // (an SM has 228 KB, a CTA 1 KB of its own)
-    if (per_sm == 1 || f.stages >= 3) break;
-  }
+  const int per_sm = ctas_per_sm(wide, D);
+  f.stages = (227 * 1024 / per_sm - 1024 - 6 * 1024) / f.stage_bytes;  // (a CTA's own 1 KB, fixed buffers, alignment)
   if (f.stages > paged::kMaxStages) f.stages = paged::kMaxStages;
-  f.smem = f.stages * f.stage_bytes + kFixedBytes;
+  f.smem = f.stages * f.stage_bytes + 1024;
   const int64_t rows = 16 / lanes, jobs = tokens / rows + B < tokens ? tokens / rows + B : tokens;
   const int64_t tiles = (capacity + paged::kKeys - 1) / paged::kKeys;
   const int64_t most = (int64_t)sm_count() * per_sm, need = jobs * (tiles > 0 ? tiles : 1);
@@ -650,15 +711,27 @@ bool attn_shape(int H, int R, int D, int maps) {
   return D == 128 || D == 256 || D == 512;
 }
 
-template <typename T, int kNT>
+template <typename T, int kSteps, int kNT, int kCtas>
 int launch_few(const paged::FewParams& p, const FewPlan& f, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
-  if (int rc = allow_smem<paged::few_kernel<T, kNT>>(225 * 1024 + 768)) return rc;
-  if (int rc = launch_kernel(paged::few_kernel<T, kNT>, dim3((unsigned)f.ctas), dim3(32 * (paged::kWarps + 1)), f.smem, st,
+  if (int rc = allow_smem<paged::few_kernel<T, kSteps, kNT, kCtas>>(221 * 1024)) return rc;
+  if (int rc = launch_kernel(paged::few_kernel<T, kSteps, kNT, kCtas>, dim3((unsigned)f.ctas), dim3(paged::kThreads), f.smem, st,
                              false, tk, tv, p))
     return rc;
   if (f.ctas == 1) return DA_OK;
   return launch_kernel(paged::combine_kernel<T>, dim3((unsigned)(p.c.B * p.few_rows), (unsigned)(p.D / 64)), dim3(256), 0, st,
                        false, p);
+}
+
+template <typename T>
+int launch_few(const paged::FewParams& p, const FewPlan& f, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
+  const int wide = p.H * p.R;
+  if (wide <= 256)
+    return p.D == 512   ? launch_few<T, 16, 16, 1>(p, f, tk, tv, st)
+           : p.D == 256 ? launch_few<T, 16, 8, 2>(p, f, tk, tv, st)
+                        : launch_few<T, 16, 4, 2>(p, f, tk, tv, st);
+  return p.D == 512   ? launch_few<T, 32, 16, 1>(p, f, tk, tv, st)
+         : p.D == 256 ? launch_few<T, 32, 8, 1>(p, f, tk, tv, st)
+                      : launch_few<T, 32, 4, 1>(p, f, tk, tv, st);
 }
 
 }  // namespace
@@ -748,11 +821,5 @@ extern "C" int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_r
                              scales, weights, per_map, y, p.few_most, workspace, status};
     if (int rc = paged::chunk_attention(a, st)) return rc;
   }
-  if (dtype == DA_BF16)
-    return D == 512   ? launch_few<__nv_bfloat16, 8>(p, f, tk, tv, st)
-           : D == 256 ? launch_few<__nv_bfloat16, 4>(p, f, tk, tv, st)
-                      : launch_few<__nv_bfloat16, 2>(p, f, tk, tv, st);
-  return D == 512   ? launch_few<__half, 8>(p, f, tk, tv, st)
-         : D == 256 ? launch_few<__half, 4>(p, f, tk, tv, st)
-                    : launch_few<__half, 2>(p, f, tk, tv, st);
+  return dtype == DA_BF16 ? launch_few<__nv_bfloat16>(p, f, tk, tv, st) : launch_few<__half>(p, f, tk, tv, st);
 }
