@@ -167,24 +167,17 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
   grid_launch_dependents();
 
   // ---- this CTA's share of the flat list of tiles
-  int64_t mine = 0;
-  for (int b = tid; b < p.c.B; b += kThreads) mine += sequence_tiles(p, sequence(p.c, b), b);
-  const int64_t total = block_sum<kThreads>(mine, buf);
-  if (p.zero_rest) {
-    const int64_t used = clamp64(p.c.starts[p.c.B], 0, p.c.tokens);
-    const int64_t words = (int64_t)(p.per_map ? p.maps : 1) * p.D / 8;
-    uint4* rest = static_cast<uint4*>(p.y) + used * words;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < (p.c.tokens - used) * words; i += (int64_t)gridDim.x * kThreads)
-      rest[i] = make_uint4(0, 0, 0, 0);
-  }
-  const int64_t share = (total + p.ctas - 1) / p.ctas;
-  const int64_t begin = (int64_t)blockIdx.x * share;
-  if (begin >= total) return;
-  {
+  const int64_t used = p.zero_rest ? clamp64(p.c.starts[p.c.B], 0, p.c.tokens) : p.c.tokens;
+  int64_t total = 0;
+  for (int b = tid; b < p.c.B; b += kThreads) total += sequence_tiles(p, sequence(p.c, b), b);
+  const bool short_list = p.c.B <= kThreads;  // then `total` is still the thread's own sequence's, scanned below
+  if (!short_list) total = block_sum<kThreads>(total, buf);
+  int64_t share = (total + p.ctas - 1) / p.ctas, begin = (int64_t)blockIdx.x * share;
+  if (short_list || begin < total) {
     int64_t before = 0;  // tiles of the sequences before this round's
     for (int base = 0;; base += kThreads) {
       const int b = base + tid;
-      const int64_t v = b < p.c.B ? sequence_tiles(p, sequence(p.c, b), b) : 0;
+      const int64_t v = short_list ? total : b < p.c.B ? sequence_tiles(p, sequence(p.c, b), b) : 0;
       int64_t inc = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -200,15 +193,27 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
         if (i < warp) at += buf[i];
         all += buf[i];
       }
+      if (short_list) {
+        total = all;
+        share = (total + p.ctas - 1) / p.ctas;
+        begin = (int64_t)blockIdx.x * share;
+      }
       if (begin >= at && begin < at + v) {
         start_b = b;
         start_off = begin - at;
       }
       before += all;
-      if (begin < before) break;  // (total > begin: found at the latest with the last sequence)
+      if (short_list || begin < before) break;  // (total > begin: found at the latest with the last sequence)
     }
     __syncthreads();
   }
+  if (used < p.c.tokens) {
+    const int64_t words = (int64_t)(p.per_map ? p.maps : 1) * p.D / 8;
+    uint4* rest = static_cast<uint4*>(p.y) + used * words;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < (p.c.tokens - used) * words; i += (int64_t)gridDim.x * kThreads)
+      rest[i] = make_uint4(0, 0, 0, 0);
+  }
+  if (begin >= total) return;
   Walk walk{start_b, start_off, share < total - begin ? share : total - begin};
   Abort ab{&abort_flag, p.status};
   const int tokens = 16 / p.lanes;
@@ -643,19 +648,24 @@ __global__ void __launch_bounds__(256) combine_kernel(const FewParams p) {
   __shared__ int64_t buf[32];
   __shared__ float wts[4][512];
   __shared__ float4 sums[16][17];
+  const int tid = threadIdx.x, b = blockIdx.x / p.few_rows;
+  // (The pieces' kernel lets this one start after it has itself waited for the kernels before it, so what those wrote --
+  // the step's lengths and the chunks' plan -- may be read before the wait for the pieces.)
+  const Sequence s = sequence(p.c, b);
+  const bool mine = (int)(blockIdx.x % p.few_rows) < s.n && sequence_tiles(p, s, b) > 0;
+  int64_t total = 0, ahead = 0;
+  if (mine) {
+    for (int i = tid; i < p.c.B; i += 256) {
+      const int64_t v = sequence_tiles(p, sequence(p.c, i), i);
+      total += v;
+      if (i < b) ahead += v;
+    }
+    total = block_sum<256>(total, buf);
+    ahead = block_sum<256>(ahead, buf);
+  }
   grid_dependency_wait();
   grid_launch_dependents();
-  const int tid = threadIdx.x, b = blockIdx.x / p.few_rows;
-  const Sequence s = sequence(p.c, b);
-  if ((int)(blockIdx.x % p.few_rows) >= s.n || sequence_tiles(p, s, b) == 0) return;
-  int64_t all = 0, ahead = 0;
-  for (int i = tid; i < p.c.B; i += 256) {
-    const int64_t v = sequence_tiles(p, sequence(p.c, i), i);
-    all += v;
-    if (i < b) ahead += v;
-  }
-  const int64_t total = block_sum<256>(all, buf);
-  ahead = block_sum<256>(ahead, buf);
+  if (!mine) return;
   const int64_t share = (total + p.ctas - 1) / p.ctas;
   const int tokens = 16 / p.lanes, tiles = job_tiles(p.c, s);
   for (int i = blockIdx.x % p.few_rows; i < s.n; i += p.few_rows) {

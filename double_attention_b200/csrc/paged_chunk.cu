@@ -51,112 +51,132 @@ struct ChunkParams {
   int* status;
 };
 
-DA_DEV int chunk_tiles(const Sequence& s, int few_most) { return s.n > few_most ? (s.n + 127) / 128 : 0; }
-// Positions that some row of tile i sees, and their key tiles.
+// Positions that some row of tile i sees.
 DA_DEV int64_t tile_end(const Cache& c, const Sequence& s, int i) {
   const int64_t e = s.held + min(s.n, (i + 1) * 128);
   return e < c.capacity ? e : c.capacity;
 }
-DA_DEV int key_tiles(const Cache& c, const Sequence& s, int i, int nk) { return (int)((tile_end(c, s, i) + nk - 1) / nk); }
 
 // ------------------------------------------------------------------------------------------------ plan
-constexpr int kPlanThreads = 1024;
-
-DA_DEV int64_t plan_sum(int64_t v, int64_t* buf) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) buf[threadIdx.x / 32] = v;
-  __syncthreads();
-  int64_t t = 0;
-  for (int i = 0; i < kPlanThreads / 32; ++i) t += buf[i];
-  return t;
-}
+constexpr int kPlanThreads = 1024, kLengths = 10;
 
 // One CTA: a warp a sequence, a tile a lane.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const Plan plan, int few_most, int nk, int pairs) {
-  __shared__ int64_t buf[32];
-  __shared__ int carry[2], sums[2][32];
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const Plan plan, int few_most, int nk_shift, int pairs) {
+  __shared__ int2 kept[kPlanThreads];  // the first sequences' new tokens (of chunks), and tokens that they had
+  __shared__ unsigned long long units;
+  __shared__ int counts[kLengths], carry[2], sums[2][32];
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  auto over_tiles = [&](auto f) {
-    for (int b = warp; b < c.B; b += kPlanThreads / 32) {
-      const Sequence s = sequence(c, b);
-      const int tiles = chunk_tiles(s, few_most);
-      for (int i = lane; i < tiles; i += 32) f(key_tiles(c, s, i, nk));
-    }
+  auto load = [&](int b) {
+    const Sequence s = sequence(c, b);
+    return make_int2(s.n > few_most ? s.n : 0, (int)s.held);
   };
-  int64_t units = 0;
-  over_tiles([&](int n) { units += n; });
-  units = plan_sum(units, buf);
+  if (threadIdx.x < c.B) kept[threadIdx.x] = load(threadIdx.x);
+  if (threadIdx.x < kLengths) counts[threadIdx.x] = 0;
+  if (threadIdx.x == 0) {
+    units = 0;
+    carry[0] = carry[1] = 0;
+  }
+  __syncthreads();
+  auto get = [&](int b) { return b < kPlanThreads ? kept[b] : load(b); };
+  auto tiles_of = [](int2 s) { return (s.x + 127) >> 7; };
+  auto keys_of = [&](int2 s, int i) {  // key tiles of query tile i
+    const int64_t e = (int64_t)s.y + min(s.x, (i + 1) * 128);
+    return (int)(((e < c.capacity ? e : c.capacity) + (1 << nk_shift) - 1) >> nk_shift);
+  };
+  unsigned long long mine = 0;
+  for (int b = warp; b < c.B; b += kPlanThreads / 32) {
+    const int2 s = get(b);
+    for (int i = lane; i < tiles_of(s); i += 32) mine += keys_of(s, i);
+  }
+  if (mine) atomicAdd(&units, mine);
+  __syncthreads();
   // The pieces' length: of a few that suit one or two rounds of the CTA pairs, the one that is done first, counting a
   // piece's start and end as two key tiles.
+  const int64_t total = (int64_t)units;
+  auto length = [&](int f) {
+    const int64_t round = (int64_t)pairs * (f < 5 ? 1 : 2), base = (total + round - 1) / round;
+    const int64_t more = f % 5 == 0 ? 0 : (base + (16 >> (f % 5 - 1)) - 1) / (16 >> (f % 5 - 1));  // none, a 16th, 8th, 4th, half
+    const int64_t len = base + more;
+    return (int)(len < 1 ? 1 : len);
+  };
+  int len[kLengths], n[kLengths];
+#pragma unroll
+  for (int f = 0; f < kLengths; ++f) {
+    len[f] = length(f);
+    n[f] = 0;
+  }
+  for (int b = warp; b < c.B; b += kPlanThreads / 32) {
+    const int2 s = get(b);
+    for (int i = lane; i < tiles_of(s); i += 32) {
+      const int t = keys_of(s, i);
+#pragma unroll
+      for (int f = 0; f < kLengths; ++f) n[f] += (unsigned)(t + len[f] - 1) / (unsigned)len[f];
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < kLengths; ++f) {
+    n[f] = __reduce_add_sync(0xffffffffu, n[f]);
+    if (lane == 0 && n[f]) atomicAdd(&counts[f], n[f]);
+  }
+  __syncthreads();
   int best = 1;
   int64_t best_cost = INT64_MAX;
-  for (int m = 1; m <= 2; ++m)
-    for (int f = 0; f < 5; ++f) {
-      const int64_t base = (units + (int64_t)pairs * m - 1) / ((int64_t)pairs * m);
-      int64_t len = base + (f == 0 ? 0 : f == 1 ? (base + 15) / 16 : f == 2 ? (base + 7) / 8 : f == 3 ? (base + 3) / 4 : (base + 1) / 2);
-      if (len < 1) len = 1;
-      int64_t n = 0;
-      over_tiles([&](int t) { n += (t + len - 1) / len; });
-      n = plan_sum(n, buf);
-      const int64_t cost = (n + pairs - 1) / pairs * (len + 2);
-      if (cost < best_cost) {
-        best_cost = cost;
-        best = (int)len;
-      }
+#pragma unroll
+  for (int f = 0; f < kLengths; ++f) {
+    const int64_t cost = (int64_t)((counts[f] + pairs - 1) / pairs) * (len[f] + 2);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = len[f];
     }
-  if (threadIdx.x == 0) carry[0] = carry[1] = 0;
-  __syncthreads();
+  }
   // tiles and pieces in order: 32 sequences a turn, one a warp
   for (int base = 0; base < c.B; base += 32) {
     const int b = base + warp;
-    Sequence s{0, 0, 0, true};
-    if (b < c.B) s = sequence(c, b);
-    const int tiles = b < c.B ? chunk_tiles(s, few_most) : 0;
-    int mine = 0;
-    for (int i = lane; i < tiles; i += 32) mine += (key_tiles(c, s, i, nk) + best - 1) / best;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    const int2 s = b < c.B ? get(b) : make_int2(0, 0);
+    const int tiles = tiles_of(s);
+    int count = 0;
+    for (int i = lane; i < tiles; i += 32) count += (unsigned)(keys_of(s, i) + best - 1) / (unsigned)best;
+    count = __reduce_add_sync(0xffffffffu, count);
     if (lane == 0) {
       sums[0][warp] = tiles;
-      sums[1][warp] = mine;
+      sums[1][warp] = count;
     }
     __syncthreads();
-    int tile0 = carry[0], piece0 = carry[1];
-    for (int i = 0; i < warp; ++i) {
-      tile0 += sums[0][i];
-      piece0 += sums[1][i];
-    }
+    const int t = sums[0][lane], k = sums[1][lane];
+    int tile0 = carry[0] + __reduce_add_sync(0xffffffffu, lane < warp ? t : 0);
+    int piece0 = carry[1] + __reduce_add_sync(0xffffffffu, lane < warp ? k : 0);
     __syncthreads();
     if (threadIdx.x == kPlanThreads - 1) {
-      carry[0] = tile0 + sums[0][warp];
-      carry[1] = piece0 + sums[1][warp];
+      carry[0] = tile0 + tiles;
+      carry[1] = piece0 + count;
     }
     if (b < c.B && lane == 0) plan.seq_piece[b] = piece0;
     for (int i0 = 0; i0 < tiles; i0 += 32) {
-      const int i = i0 + lane, n = i < tiles ? key_tiles(c, s, i, nk) : 0, count = (n + best - 1) / best;
-      int at = count;
+      const int i = i0 + lane, keys = i < tiles ? keys_of(s, i) : 0, own = (unsigned)(keys + best - 1) / (unsigned)best;
+      int at = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, at, o);
         if (lane >= o) at += u;
       }
-      const int all = __shfl_sync(0xffffffffu, at, 31), first = piece0 + at - count;
-      if (i < tiles) {
-        plan.tile_piece[tile0 + i] = first;
-        for (int k = 0; k < count; ++k) {
-          plan.pieces[2 * (first + k)] = make_int4(b, i, k * best, min(best, n - k * best));
-          plan.pieces[2 * (first + k) + 1] = make_int4(first, count, 0, 0);
+      const int all = __shfl_sync(0xffffffffu, at, 31), first = piece0 + at - own;
+      if (i < tiles) plan.tile_piece[tile0 + i] = first;
+      // (a tile's pieces side by side: the warp writes one tile after another, a piece a lane)
+      for (int j = 0; j < min(32, tiles - i0); ++j) {
+        const int from = __shfl_sync(0xffffffffu, first, j), many = __shfl_sync(0xffffffffu, own, j);
+        const int last = __shfl_sync(0xffffffffu, keys, j);
+        for (int m = lane; m < many; m += 32) {
+          plan.pieces[2 * (from + m)] = make_int4(b, i0 + j, m * best, min(best, last - m * best));
+          plan.pieces[2 * (from + m) + 1] = make_int4(from, many, 0, 0);
+          *reinterpret_cast<int2*>(plan.odd + 2 * (from + m)) = make_int2(0, 0);
         }
       }
       piece0 += all;
     }
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < 2 * carry[1]; i += kPlanThreads) plan.odd[i] = 0;
   if (threadIdx.x == 0) {
     plan.seq_piece[c.B] = carry[1];
     plan.tile_piece[carry[0]] = carry[1];
@@ -379,15 +399,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             if (!mbar_wait(&v_full[st], (vc / L.nvs) & 1u, ab, 77)) { ok = false; break; }
             tc_fence_after();
             const uint32_t va = smem_u32(smem + L.off_v + st * L.v_stage);
-            for (int i = 0; i < L.npv; ++i) {
-              // MN-major V: rows are keys (K), 128 B = 64 value columns (N);
-              // LBO = distance between 64-column boxes, SBO = 8 key rows.
-              const uint64_t bd0 = sdesc_sw128(va + i * L.per * (64 * 128), 64 * 128, 1024);
-              const uint64_t ad0 = sdesc_sw128(pa + c * (kRows * 128), 16, 1024);
+            // MN-major V: rows are keys (K), 128 B = 64 value columns (N);
+            // LBO = distance between 64-column boxes, SBO = 8 key rows.
+            const uint64_t ad0 = sdesc_sw128(pa + c * (kRows * 128), 16, 1024);
+            const uint64_t bd0 = sdesc_sw128(va, 64 * 128, 1024), bd1 = sdesc_sw128(va + L.per * (64 * 128), 64 * 128, 1024);
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)  // K step of 16 keys: A +32 B (+2), B +16 rows x 128 B (+128)
-                mma_f16_ss<2>(tmem + (uint32_t)(i * (L.nc / 2)), ad0 + 2 * kk, bd0 + 128 * kk, idesc_o,
-                              (v | c | kk) ? 1u : 0u);
+            for (int kk = 0; kk < 4; ++kk) {  // K step of 16 keys: A +32 B (+2), B +16 rows x 128 B (+128)
+              mma_f16_ss<2>(tmem, ad0 + 2 * kk, bd0 + 128 * kk, idesc_o, (v | c | kk) ? 1u : 0u);
+              if (L.npv == 2)  // the two groups' products in turn: neither waits for its own last one
+                mma_f16_ss<2>(tmem + (uint32_t)(L.nc / 2), ad0 + 2 * kk, bd1 + 128 * kk, idesc_o, (v | c | kk) ? 1u : 0u);
             }
             mma_commit_pair(smem_u32(&v_empty[st]));
           }
@@ -677,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   if (warp == 1) tmem_dealloc<2>(tmem, L.tmem_cols);
 }
 
-// Adds the pieces of the tiles that have several: a CTA takes four rows of a tile, a warp half a row.
+// Adds the pieces of the tiles that have several: a warp takes 128 columns of a row.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const ChunkParams p, const bool weighted) {
   grid_dependency_wait();
@@ -687,41 +707,49 @@ __global__ void __launch_bounds__(256) join_kernel(const ChunkParams p, const bo
   if (pieces < 2) return;
   const int4 here = p.plan.pieces[2 * first];
   const Sequence seq = sequence(p.c, here.x);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int trow = blockIdx.y * 4 + warp / 2, t = here.y * 128 + trow;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, parts = p.D / 128;
+  const int trow = blockIdx.y * (8 / parts) + warp / parts, t = here.y * 128 + trow, col = (warp % parts) * 128 + lane * 4;
   if (t >= seq.n) return;
-  float top = -INFINITY, f = 1.f;
   const float* ml = p.part_ml + (size_t)first * 256 + trow;
+  float top = -INFINITY, sum = 0.f;
   if (weighted) {
-    float sum = 0.f;
-    for (int i = 0; i < pieces; ++i) top = fmaxf(top, ml[(size_t)i * 256]);
-    const float at = top == -INFINITY ? 0.f : top;
-    for (int i = 0; i < pieces; ++i) {
-      const float m = ml[(size_t)i * 256];
-      sum += ml[(size_t)i * 256 + 128] * (m == -INFINITY ? 1.f : ex2(m - at));
-    }
-    f = 1.f / sum;
-    top = at;
+    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, ml[(size_t)i * 256]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top == -INFINITY) top = 0.f;
   }
-  const float* src = p.part + ((size_t)first * 128 + trow) * p.D;
-  T* y = static_cast<T*>(p.y) + (seq.first + t) * p.y_row;
-  for (int col = (warp % 2) * (p.D / 2) + lane * 4; col < (warp % 2 + 1) * (p.D / 2); col += 128) {
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-      const float4 v = *reinterpret_cast<const float4*>(src + (size_t)i * 128 * p.D + col);
-      float w = 1.f;
-      if (weighted) {
-        const float m = ml[(size_t)i * 256];
+  const float* src = p.part + ((size_t)first * 128 + trow) * p.D + col;
+  const size_t step = (size_t)128 * p.D;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = 0; base < pieces; base += 32) {
+    float w = 1.f;
+    if (weighted) {
+      w = 0.f;
+      if (base + lane < pieces) {
+        const float m = ml[(size_t)(base + lane) * 256];
         w = m == -INFINITY ? 0.f : ex2(m - top);
+        sum += ml[(size_t)(base + lane) * 256 + 128] * (m == -INFINITY ? 1.f : w);
       }
-      o.x = fmaf(w, v.x, o.x);
-      o.y = fmaf(w, v.y, o.y);
-      o.z = fmaf(w, v.z, o.z);
-      o.w = fmaf(w, v.w, o.w);
     }
-    *reinterpret_cast<uint2*>(y + col) = make_uint2(pack2<T>(o.x * f, o.y * f), pack2<T>(o.z * f, o.w * f));
+    const int n = min(32, pieces - base);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(src + (size_t)(base + i) * step);
+      const float wi = __shfl_sync(0xffffffffu, w, i);
+      o.x = fmaf(wi, v.x, o.x);
+      o.y = fmaf(wi, v.y, o.y);
+      o.z = fmaf(wi, v.z, o.z);
+      o.w = fmaf(wi, v.w, o.w);
+    }
   }
+  float f = 1.f;
+  if (weighted) {
+#pragma unroll
+    for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+    f = 1.f / sum;
+  }
+  T* y = static_cast<T*>(p.y) + (seq.first + t) * p.y_row + col;
+  *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(o.x * f, o.y * f), pack2<T>(o.z * f, o.w * f));
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -785,8 +813,8 @@ int run(const ChunkArgs& a, cudaStream_t st) {
     const uint32_t box[4] = {64, (uint32_t)p.brow_v, (uint32_t)(whole ? L.per : 1), (uint32_t)(whole ? L.npv : 1)};
     if (int rc = make_tmap_blocks(&tv, a.value_pages, dt, 2, 4, dims, strides, box)) return rc;
   }
-  if (int rc = launch_kernel(plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, false, a.c, p.plan, a.few_most, L.nk,
-                             sm_count() / 2))
+  if (int rc = launch_kernel(plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, false, a.c, p.plan, a.few_most,
+                             L.nk == 256 ? 8 : 7, sm_count() / 2))
     return rc;
   const int smem = L.smem + 1024;
   const dim3 grid((unsigned)(2 * pieces)), block(kThreads);
@@ -809,7 +837,7 @@ int run(const ChunkArgs& a, cudaStream_t st) {
     } else if (int rc = launch_kernel(chunk_kernel<T, false>, grid, block, smem, st, true, tq, tk, tv, p)) {
       return rc;
     }
-    if (int rc = launch_kernel(join_kernel<T>, dim3((unsigned)tiles, 32), dim3(256), 0, st, false, p, !mix)) return rc;
+    if (int rc = launch_kernel(join_kernel<T>, dim3((unsigned)tiles, (unsigned)(16 * a.D / 128)), dim3(256), 0, st, false, p, !mix)) return rc;
   }
   return DA_OK;
 }
