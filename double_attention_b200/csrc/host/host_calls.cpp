@@ -1,6 +1,6 @@
-// The host side of the eight-bit operators' ordinary calls, as a Python extension module.
+// The host side of the ordinary calls of the eight-bit, paged and scoring operators, as a Python extension module.
 //
-// A call on one token is over on the device in 2 to 4 us; from Python, checking the tensors, allocating the outputs
+// A call on one token is over on the device in 2 to 10 us; from Python, checking the tensors, allocating the outputs
 // and converting the arguments takes 8 to 15.  The functions here do the same for tensors that lie as the kernels
 // want them (dense, on the current device, of the right types, nothing requiring a gradient or carrying a tangent) in
 // 4 to 6 us, launch included, and return None for anything else, which the Python functions then check, copy or
@@ -264,6 +264,129 @@ PyObject* weight_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Pages [pages, page, H, R] and [pages, page, D] that the kernels read in place.
+struct Pages {
+  int64_t pages = 0, page = 0, H = 0, R = 0, D = 0;
+  int type = -1;
+  bool ok(const Tensor* k, const Tensor* v) {
+    if (!k || !v || k->dim() != 4 || v->dim() != 3 || !half(*k) || v->scalar_type() != k->scalar_type()) return false;
+    pages = k->size(0);
+    page = k->size(1);
+    H = k->size(2);
+    R = k->size(3);
+    D = v->size(2);
+    type = code(k);
+    return pages > 0 && page >= 16 && page <= 65536 && !(page & (page - 1)) && v->size(0) == pages && v->size(1) == page;
+  }
+};
+
+// A step's table, lengths and starts.
+struct Step {
+  const Tensor *table, *lengths, *starts;
+  int64_t B = 0, cols = 0;
+  bool ok() {
+    if (!table || !lengths || !starts || table->scalar_type() != at::kInt || lengths->scalar_type() != at::kInt ||
+        starts->scalar_type() != at::kInt || table->dim() != 2 || lengths->dim() != 1 || starts->dim() != 1)
+      return false;
+    B = table->size(0);
+    cols = table->size(1);
+    return B > 0 && cols > 0 && lengths->size(0) == B && starts->size(0) == B + 1;
+  }
+  const int* at(const Tensor* t) const { return static_cast<const int*>(t->data_ptr()); }
+};
+
+// append_paged(keys, values, key pages, value pages, table, lengths, starts, status word) -> True
+PyObject* append_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) return PyErr_Format(PyExc_TypeError, "append_paged takes 8 arguments");
+  Call c;
+  const Tensor *keys = c.any(a[0]), *values = c.any(a[1]), *kp = c.dense(a[2]), *vp = c.dense(a[3]);
+  Step s{c.dense(a[4]), c.dense(a[5]), c.dense(a[6])};
+  const Tensor* word = c.dense(a[7]);
+  Pages p;
+  if (!c.ok || !keys || !values || !word || !p.ok(kp, vp) || !s.ok() || p.R % 8 || p.D % 8) Py_RETURN_NONE;
+  if (keys->dim() != 3 || keys->size(0) != p.H || keys->size(2) != p.R || keys->stride(2) != 1 || code(keys) < 0 ||
+      values->dim() != 2 || values->size(0) != keys->size(1) || values->size(1) != p.D || values->stride(1) != 1 ||
+      code(values) < 0 || keys->size(1) < 1)
+    Py_RETURN_NONE;
+  const int status = da_paged_append(keys->data_ptr(), code(keys), keys->stride(0), keys->stride(1), values->data_ptr(),
+                                     code(values), values->stride(0), keys->size(1), kp->data_ptr(), vp->data_ptr(), p.type,
+                                     p.pages, (int)p.page, (int)p.H, (int)p.R, (int)p.D, s.at(s.table), s.cols, s.cols,
+                                     s.at(s.lengths), s.at(s.starts), s.B, static_cast<int*>(word->data_ptr()), c.stream());
+  return done("da_paged_append", status, (Py_INCREF(Py_True), Py_True));
+  END_HANDLE_TH_ERRORS
+}
+
+// attend_paged(query, key pages, value pages, table, lengths, starts, most new tokens, scales, weights, status word) -> y
+PyObject* attend_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10) return PyErr_Format(PyExc_TypeError, "attend_paged takes 10 arguments");
+  Call c;
+  const Tensor *q = c.any(a[0]), *kp = c.dense(a[1]), *vp = c.dense(a[2]);
+  Step s{c.dense(a[3]), c.dense(a[4]), c.dense(a[5])};
+  const int64_t max_new = a[6] == Py_None ? 0 : PyLong_AsLongLong(a[6]);
+  const Tensor *scales = c.dense(a[7]), *weights = c.dense(a[8]), *word = c.dense(a[9]);
+  if (PyErr_Occurred()) return nullptr;
+  Pages p;
+  if (!c.ok || !q || !scales || !word || !p.ok(kp, vp) || !s.ok()) Py_RETURN_NONE;
+  const int64_t maps = scales->dim() == 1 ? scales->size(0) : 0, tokens = q->dim() == 3 ? q->size(1) : 0;
+  if (tokens < 1 || q->size(0) != p.H || q->size(2) != p.R || q->scalar_type() != kp->scalar_type() || q->stride(2) != 1 ||
+      reinterpret_cast<uintptr_t>(q->data_ptr()) % 16 || (tokens > 1 && (q->stride(1) % 8 || q->stride(1) < p.R)) ||
+      (p.H > 1 && (q->stride(0) % 8 || q->stride(0) < p.R)))
+    Py_RETURN_NONE;
+  if (maps < 1 || maps > 4 || (p.H % maps && maps % p.H) || scales->scalar_type() != at::kFloat) Py_RETURN_NONE;
+  if (weights && (weights->scalar_type() != at::kFloat || weights->dim() != 1 || weights->size(0) != maps)) Py_RETURN_NONE;
+  const int per_map = maps > 1 && !weights;
+  const int64_t need = da_paged_attn_workspace_size(tokens, s.B, s.cols, (int)p.page, max_new, (int)p.H, (int)p.R, (int)p.D,
+                                                    (int)maps, per_map);
+  if (need < 0) Py_RETURN_NONE;  // (a shape that is not covered)
+  Tensor y = per_map ? c.empty({tokens, maps, p.D}, q->scalar_type()) : c.empty({tokens, p.D}, q->scalar_type()), work;
+  if (need > 0) work = c.empty({need}, at::kByte);
+  const int status = da_paged_attn(
+      q->data_ptr(), q->stride(0), q->stride(1), tokens, kp->data_ptr(), vp->data_ptr(), p.type, p.pages, (int)p.page, (int)p.H,
+      (int)p.R, (int)p.D, (int)maps, s.at(s.table), s.cols, s.cols, s.at(s.lengths), s.at(s.starts), s.B, max_new,
+      static_cast<const float*>(scales->data_ptr()), per_map ? nullptr : static_cast<const float*>(data(weights)), per_map, 1,
+      y.data_ptr(), need > 0 ? work.data_ptr() : nullptr, need, static_cast<int*>(word->data_ptr()), c.stream());
+  if (status) return done("da_paged_attn", status, nullptr);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// score(logits, tokens, top, keep) -> (log_probs, entropy, top_log_probs, top_tokens, stats)
+PyObject* score(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) return PyErr_Format(PyExc_TypeError, "score takes 4 arguments");
+  Call c;
+  const Tensor *x = c.dense(a[0]), *tokens = c.dense(a[1]);
+  const int64_t top = PyLong_AsLongLong(a[2]);
+  const int keep = PyObject_IsTrue(a[3]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!c.ok || !x || !tokens || code(x) < 0 || x->dim() < 1 || tokens->scalar_type() != at::kLong) Py_RETURN_NONE;
+  const at::IntArrayRef sizes = x->sizes(), lead = sizes.slice(0, sizes.size() - 1);
+  const int64_t v = sizes.back(), rows = v ? x->numel() / v : 0;
+  if (rows < 1 || tokens->sizes() != lead || top < 0 || top > 32 || top > v) Py_RETURN_NONE;
+  Tensor log_probs = c.empty(lead, at::kFloat), entropy = c.empty(lead, at::kFloat), top_lp, top_tokens, stats;
+  if (top) {
+    c10::SmallVector<int64_t, 6> wide(sizes.begin(), sizes.end());
+    wide.back() = top;
+    top_lp = c.empty(wide, at::kFloat);
+    top_tokens = c.empty(wide, at::kLong);
+  }
+  if (keep) stats = c.empty({rows, 2}, at::kFloat);
+  const int status = da_token_log_probs(
+      x->data_ptr(), code(x), v, rows, v, static_cast<const int64_t*>(tokens->data_ptr()), (int)top,
+      static_cast<float*>(log_probs.data_ptr()), static_cast<float*>(entropy.data_ptr()),
+      top ? static_cast<float*>(top_lp.data_ptr()) : nullptr, top ? static_cast<int64_t*>(top_tokens.data_ptr()) : nullptr,
+      keep ? static_cast<float*>(stats.data_ptr()) : nullptr, c.stream());
+  if (status) return done("da_token_log_probs", status, nullptr);
+  PyObject* r = PyTuple_New(5);
+  int i = 0;
+  for (Tensor* t : {&log_probs, &entropy, &top_lp, &top_tokens, &stats})
+    PyTuple_SET_ITEM(r, i++, t->defined() ? THPVariable_Wrap(std::move(*t)) : (Py_INCREF(Py_None), Py_None));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
 // set_check(check): what raises the exception for a status
 PyObject* set_check(PyObject*, PyObject* check) {
   Py_INCREF(check);
@@ -282,6 +405,9 @@ PyMethodDef g_methods[] = {{"norm", fast<norm>(), METH_FASTCALL, nullptr},
                            {"checkpoint", fast<checkpoint>(), METH_FASTCALL, nullptr},
                            {"gelu_backward", fast<gelu_backward>(), METH_FASTCALL, nullptr},
                            {"weight_grad", fast<weight_grad>(), METH_FASTCALL, nullptr},
+                           {"append_paged", fast<append_paged>(), METH_FASTCALL, nullptr},
+                           {"attend_paged", fast<attend_paged>(), METH_FASTCALL, nullptr},
+                           {"score", fast<score>(), METH_FASTCALL, nullptr},
                            {"set_check", set_check, METH_O, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 

@@ -23,7 +23,7 @@ from torch import Tensor
 
 from . import _lib, ops
 from ._lib import ptr
-from .eight_bit import _CODES, _HALF, _device_of, _inference_only, _launch
+from .eight_bit import _CODES, _HALF, _device_of, _host, _inference_only, _launch
 
 BAD_PAGE = 8  # bit of ops.device_status
 
@@ -88,6 +88,9 @@ def append_paged(keys: Tensor, values: Tensor, key_pages: Tensor, value_pages: T
     fp32, bf16 or fp16 with unit column stride or any other (copied first then), rounded once to the pages' type.  Nothing
     but the new positions is written."""
     name = "append_paged"
+    if key_pages.is_cuda and _host().append_paged(keys, values, key_pages, value_pages, batch[0], batch[1], batch[2],
+                                                  ops.workspace(key_pages.device).status):
+        return
     b = _check_batch(name, batch)
     pages, page, h, r, d = _check_pages(name, key_pages, value_pages)
     if keys.ndim != 3 or keys.shape[0] != h or keys.shape[2] != r or values.shape != (keys.shape[1], d):
@@ -134,6 +137,10 @@ def routed_attention_paged(query: Tensor, key_pages: Tensor, value_pages: Tensor
 
     Supported: R a multiple of 64, D 128, 256 or 512, up to 4 maps and ``max(H, S) * R`` up to 512."""
     name = "routed_attention_paged"
+    if out is None and query.is_cuda:
+        y = _host().attend_paged(query, key_pages, value_pages, *batch, scales, map_weights, ops.workspace(query.device).status)
+        if y is not None:
+            return y
     b = _check_batch(name, batch)
     pages, page, h, r, d = _check_pages(name, key_pages, value_pages)
     if query.ndim != 3 or query.shape[0] != h or query.shape[2] != r:

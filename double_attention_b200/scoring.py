@@ -12,7 +12,7 @@ import torch
 from torch import Tensor
 
 from ._lib import ptr
-from .eight_bit import _CODES, _FirstOrder, _device_of, _launch, _new, _rows
+from .eight_bit import _CODES, _FirstOrder, _device_of, _host, _launch, _new, _rows
 
 IGNORE = -100   # a token that is none
 MAX_TOP = 32
@@ -34,6 +34,9 @@ class TokenLogProbs(NamedTuple):
 
 
 def _forward(logits: Tensor, tokens: Tensor, top: int, device: int, keep: bool):
+    done = _host().score(logits, tokens, top, keep)
+    if done is not None:
+        return done
     lead, v = logits.shape[:-1], logits.shape[-1]
     x, rows, ld = _rows(logits)
     made = _new(lead, torch.float32, logits.device), _new(lead, torch.float32, logits.device)
@@ -94,6 +97,10 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, top: int = 0) -> TokenLog
 
     Differentiable in ``logits`` through ``log_probs`` and ``entropy`` (the alternatives carry no gradient)."""
     name = "token_log_probs"
+    if logits.is_cuda:
+        done = _host().score(logits, tokens, top, False)  # (None where a gradient or a tangent is wanted)
+        if done is not None:
+            return TokenLogProbs(*done[:4])
     if logits.dtype not in _CODES:
         raise ValueError(f"{name} takes logits in float32, bfloat16 or float16, got {logits.dtype}")
     if not logits.ndim or not logits.shape[-1] or tokens.shape != logits.shape[:-1]:
