@@ -1,18 +1,19 @@
 // Log probabilities of given tokens, the entropy of their distributions and the top alternatives, and the backward pass.
 //
 // Row x of V logits, with m = max x, t_i = (x_i - m) log2 e, l = sum 2^t_i and w = sum 2^t_i t_i:
-//   log p_i = ln 2 (t_i - log2 l),     H = -sum p log p = ln 2 (log2 l - w / l),
+//   log p_i = x_i - m - ln 2 log2 l,     H = -sum p log p = ln 2 (log2 l - w / l),
 //   dL/dx_i = g ([i = token] - p_i) - h p_i (log p_i + H)   for g = dL/d log p_token, h = dL/dH.
 // m, l and w are kept against a running maximum, so the forward reads the logits once (16 bytes a load); the backward
 // reads them again and writes the gradient.  Both are bound by those bytes.  Differences from the row's maximum are
-// formed first and scaled inside one multiply-add, so that logits far from zero lose nothing; an entry of minus
-// infinity counts 0 in l, w and the gradient.  A row with a NaN, with plus infinity or with nothing but minus infinity is
+// formed first and scaled then, so that logits far from zero lose nothing and a row of nothing but the type's lowest value
+// is an even one; an entry of minus infinity counts 0 in l, w and the gradient.  A row with a NaN, with plus infinity or with nothing but minus infinity is
 // NaN, as a softmax of it is.
 //
 // Top alternatives: in order of (value, lowest index), NaN before numbers.  The first pass leaves every warp's (or, where
 // a warp has a row, every lane's) largest value; the top-th largest of those is at most the top-th largest value of the
 // row, and few values lie above it (about 32 H_32 - 32 H_(32 - top) on independent ones), so a second pass, out of L1 and
-// L2, collects what is not below it into a sorted list, one entry a lane.  Ties and hostile orders only make it longer.
+// L2, collects what is not below it and ranks it.  Where ties or hostile orders leave more than there is room for, every
+// warp keeps a sorted list instead, one entry a lane.
 #include <math.h>
 
 #include "host_util.h"
@@ -31,22 +32,29 @@ struct Params {
   const int64_t* tokens;
   float *log_probs, *entropy, *top_log_probs;
   int64_t* top_tokens;
-  float* stats;  // [rows][2]: m log2 e and log2 l, or null
+  float* stats;  // [rows][2]: m and log2 l, or null
 };
 
-// 16 bytes of a row as floats.
+// 16 bytes of a row: `n` elements.  top() is the largest of them, NaN only where all are; or_nan() NaN where any is.
 template <typename T>
 struct Vec {
   static constexpr int n = 8;
-  static DA_DEV void get(uint4 w, float* x) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack2<T>(u[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
+  using Two = std::conditional_t<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>;
+  static DA_DEV Two two(uint32_t u) { return *reinterpret_cast<Two*>(&u); }
+  static DA_DEV uint32_t bits(Two v) { return *reinterpret_cast<uint32_t*>(&v); }
+  static DA_DEV uint4 none() {
+    constexpr uint32_t w = std::is_same<T, __nv_bfloat16>::value ? 0xff80ff80u : 0xfc00fc00u;
+    return make_uint4(w, w, w, w);
   }
+  static DA_DEV float top(uint4 w) {
+    const float2 f = unpack2<T>(bits(__hmax2(__hmax2(two(w.x), two(w.y)), __hmax2(two(w.z), two(w.w)))));
+    return fmaxf(f.x, f.y);
+  }
+  static DA_DEV float or_nan(uint4 w) {
+    const float2 f = unpack2<T>(bits(__hmax2_nan(__hmax2_nan(two(w.x), two(w.y)), __hmax2_nan(two(w.z), two(w.w)))));
+    return f.x != f.x ? f.x : f.y != f.y ? f.y : fmaxf(f.x, f.y);
+  }
+  static DA_DEV F2 pair(uint4 w, int i) { return widen<T>(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w); }
   static DA_DEV float one(const T* p) { return unpack2<T>(*reinterpret_cast<const uint16_t*>(p)).x; }
   static DA_DEV uint4 put(const float* x) {
     return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
@@ -55,17 +63,27 @@ struct Vec {
 template <>
 struct Vec<float> {
   static constexpr int n = 4;
-  static DA_DEV void get(uint4 w, float* x) {
-    x[0] = __uint_as_float(w.x);
-    x[1] = __uint_as_float(w.y);
-    x[2] = __uint_as_float(w.z);
-    x[3] = __uint_as_float(w.w);
+  static DA_DEV uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  static DA_DEV float top(uint4 w) {
+    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
+  static DA_DEV float or_nan(uint4 w) {
+    const float a = __uint_as_float(w.x), b = __uint_as_float(w.y), c = __uint_as_float(w.z), d = __uint_as_float(w.w);
+    return a != a || b != b || c != c || d != d ? NAN : top(w);
+  }
+  static DA_DEV F2 pair(uint4 w, int i) {
+    return i == 0 ? f2(__uint_as_float(w.x), __uint_as_float(w.y)) : f2(__uint_as_float(w.z), __uint_as_float(w.w));
   }
   static DA_DEV float one(const float* p) { return *p; }
   static DA_DEV uint4 put(const float* x) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
   }
 };
+template <typename V>
+DA_DEV void values(uint4 w, float* x) {
+#pragma unroll
+  for (int i = 0; i < V::n / 2; ++i) split(V::pair(w, i), x[2 * i], x[2 * i + 1]);
+}
 
 // A row as elements before the first 16-byte boundary, vectors from there on, and elements behind the last vector.
 template <typename T>
@@ -90,44 +108,72 @@ struct Row {
   }
 };
 
-// Running sums against a running maximum (all in log2 units).
+// The larger of two, NaN where either is.
+DA_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+constexpr float kFar = -10000.f;  // 2^t is 0 there, and 2^t t too, as for t of minus infinity it would not be
+
+// Running sums against a running maximum m of the logits: t = (x - m) log2 e, the difference first.
 struct Sums {
   float m, l, w;  // maximum, sum of 2^t, sum of 2^t t
   DA_DEV void raise(float to) {
     if (to > m) {
-      const float d = m - to;
       if (m != -INFINITY) {
-        const float c = ex2(d);
+        const float d = fmaxf((m - to) * kLog2e, kFar), c = ex2(d);
         w = c * fmaf(l, d, w);
         l *= c;
       }
       m = to;
     }
   }
-  template <int n>
-  DA_DEV void add(const float* x) {
-    float top = x[0];
+  // k vectors at once.
+  template <typename V, int k>
+  DA_DEV void add(const uint4* raw) {
+    float top = V::top(raw[0]);
 #pragma unroll
-    for (int i = 1; i < n; ++i) top = fmaxf(top, x[i]);
-    raise(top * kLog2e);
-    const float at = m == -INFINITY ? 0.f : m;
+    for (int i = 1; i < k; ++i) top = fmaxf(top, V::top(raw[i]));
+    raise(top);
+    const F2 at = dup(m == -INFINITY ? 0.f : -m), scale = dup(kLog2e);
+    F2 ls = f2(l, 0.f), ws = f2(w, 0.f);
 #pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const float t = fmaf(x[i], kLog2e, -at), e = ex2(t);
-      l += e;
-      w = fmaf(e, fmaxf(t, -1000.f), w);  // (2^t is 0 there: so is the term)
+    for (int i = 0; i < k; ++i) {
+#pragma unroll
+      for (int j = 0; j < V::n / 2; ++j) {
+        float a, b;
+        split(mul2(add2(V::pair(raw[i], j), at), scale), a, b);
+        a = max_nan(a, kFar);
+        b = max_nan(b, kFar);
+        const F2 e = f2(ex2(a), ex2(b));
+        ls = add2(ls, e);
+        ws = fma2(e, f2(a, b), ws);
+      }
     }
+    float a, b;
+    split(ls, a, b);
+    l = a + b;
+    split(ws, a, b);
+    w = a + b;
   }
-  DA_DEV void merge(const Sums& o) {
-    Sums a = o;
-    const float to = fmaxf(m, o.m);
-    a.raise(to);
-    raise(to);
-    l += a.l;
-    w += a.w;
+  DA_DEV void add_one(float x) {
+    raise(x);
+    const float t = max_nan((x - (m == -INFINITY ? 0.f : m)) * kLog2e, kFar), e = ex2(t);
+    l += e;
+    w = fmaf(e, t, w);
   }
-  DA_DEV Sums shuffled(int o) const {
-    return {__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, l, o), __shfl_xor_sync(0xffffffffu, w, o)};
+  // Over the warp.
+  DA_DEV void reduce() {
+    float top = m;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    raise(top);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      l += __shfl_xor_sync(0xffffffffu, l, o);
+      w += __shfl_xor_sync(0xffffffffu, w, o);
+    }
   }
 };
 
@@ -169,101 +215,121 @@ struct List {
   }
 };
 
-// The top-th largest of the lanes' values, in every lane.
+// The top-th largest of the lanes' values (no NaN), in every lane: sorted over the warp, the smallest first.
 DA_DEV float nth_largest(float x, int top) {
   const int lane = threadIdx.x % 32;
-  const uint32_t k = order_of(x);
-  int rank = 0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const uint32_t o = __shfl_sync(0xffffffffu, k, i);
-    rank += o > k || (o == k && i < lane);
-  }
-  const uint32_t who = __ballot_sync(0xffffffffu, rank == top - 1);
-  return __shfl_sync(0xffffffffu, x, __ffs(who) - 1);
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j; j >>= 1) {
+      const float o = __shfl_xor_sync(0xffffffffu, x, j);
+      const bool low = ((lane & j) == 0) == ((lane & k) == 0 || k == 32);
+      x = low ? fminf(x, o) : fmaxf(x, o);
+    }
+  return __shfl_sync(0xffffffffu, x, 32 - top);
 }
 
 // kThreads a row: 32 (eight rows a CTA) or 1024.
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads == 32 ? 256 : 1024) forward_kernel(const Params p) {
   using V = Vec<T>;
-  constexpr int kBatch = 16 / V::n;  // vectors whose largest value is found together
+  constexpr int kBatch = 4;  // loads in flight a thread, their largest value found together
+  constexpr int kFound = kThreads == 32 ? 256 : 1024;  // entries that a row has room for
   __shared__ Sums sums[32];
-  __shared__ uint64_t found[1024];
-  __shared__ int count;
+  __shared__ uint64_t found_all[kThreads == 32 ? 8 : 1][kFound];
+  __shared__ int counts[kThreads == 32 ? 8 : 1];
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int tid = kThreads == 32 ? lane : threadIdx.x;
   const int64_t r = kThreads == 32 ? (int64_t)blockIdx.x * 8 + warp : blockIdx.x;
   if (kThreads == 32 && r >= p.rows) return;
+  uint64_t* found = found_all[kThreads == 32 ? warp : 0];
+  int* count = &counts[kThreads == 32 ? warp : 0];
+  auto meet = [] {
+    if constexpr (kThreads == 32) __syncwarp();
+    else __syncthreads();
+  };
+  if (tid == 0) *count = 0;
   const Row<T> row(p.logits, r * p.ld, p.V);
   Sums s{-INFINITY, 0.f, 0.f};
   {
-    int v = tid;
-    for (; v + (2 * kBatch - 1) * kThreads < row.vecs; v += 2 * kBatch * kThreads) {
-      uint4 raw[2 * kBatch];
-#pragma unroll
-      for (int i = 0; i < 2 * kBatch; ++i) raw[i] = row.load(v + i * kThreads);
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        float x[16];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) V::get(raw[b * kBatch + i], x + i * V::n);
-        s.add<16>(x);
-      }
-    }
-    for (; v < row.vecs; v += kThreads) {
-      float x[V::n];
-      V::get(row.load(v), x);
-      s.add<V::n>(x);
-    }
     const int odd = row.odd(tid);
-    if (odd >= 0) {
-      const float x = V::one(row.p + odd);
-      s.add<1>(&x);
-    }
-  }
-  const float own = s.m;  // this thread's largest value times log2 e
+    float x = -INFINITY;
+    if (odd >= 0) x = V::one(row.p + odd);
+    for (int v = tid; v < row.vecs; v += kBatch * kThreads) {
+      uint4 raw[kBatch];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) s.merge(s.shuffled(o));
-  float group = own;
+      for (int i = 0; i < kBatch; ++i) raw[i] = v + i * kThreads < row.vecs ? row.load(v + i * kThreads) : V::none();
+      s.add<V, kBatch>(raw);
+    }
+    if (odd >= 0) s.add_one(x);
+  }
+  float group = s.m;  // lane i: group i's largest value
+  s.reduce();
   if constexpr (kThreads > 32) {
-    group = s.m;  // the warp's
     if (lane == 0) sums[warp] = s;
-    if (threadIdx.x == 0) count = 0;
     __syncthreads();
     s = sums[lane];
-    group = s.m;  // lane i: warp i's
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s.merge(s.shuffled(o));
+    group = s.m;
+    s.reduce();
   }
   const float at = s.m == -INFINITY ? 0.f : s.m, log_l = log2f(s.l);
   if (tid == 0) {
     const int64_t token = p.tokens[r];
     float lp = token == kIgnore ? 0.f : NAN;
-    if (token >= 0 && token < p.V) lp = (fmaf(V::one(row.p + token), kLog2e, -at) - log_l) * kLn2;
+    if (token >= 0 && token < p.V) lp = V::one(row.p + token) - at - log_l * kLn2;
     p.log_probs[r] = lp;
     p.entropy[r] = (log_l - s.w / s.l) * kLn2;
     if (p.stats) reinterpret_cast<float2*>(p.stats)[r] = make_float2(at, log_l);
   }
   if (p.top == 0) return;
 
-  // The groups' maxima are products with log2 e: the floor is taken a little lower, so that no rounding lifts it.
-  float floor = nth_largest(group, p.top) * kLn2;
-  floor -= fabsf(floor) * 1e-6f + 1e-30f;
+  float floor = nth_largest(group, p.top);
+  meet();
+  auto write = [&](uint64_t e, int rank) {
+    p.top_log_probs[r * p.top + rank] = value_of((uint32_t)(e >> 32)) - at - log_l * kLn2;
+    p.top_tokens[r * p.top + rank] = (uint32_t)~(uint32_t)e;
+  };
+  {
+    auto take = [&](float x, int index) {
+      if (x < floor) return;
+      const int i = atomicAdd(count, 1);
+      if (i < kFound) found[i] = entry_of(x, index);
+    };
+#pragma unroll 2
+    for (int v = tid; v < row.vecs; v += kThreads) {
+      const uint4 raw = row.load(v);
+      if (V::or_nan(raw) < floor) continue;
+      float x[V::n];
+      values<V>(raw, x);
+      const int index = row.index(v);
+#pragma unroll
+      for (int i = 0; i < V::n; ++i) take(x[i], index + i);
+    }
+    const int odd = row.odd(tid);
+    if (odd >= 0) take(V::one(row.p + odd), odd);
+  }
+  meet();
+  const int n = *count;
+  if (n <= kFound) {
+    for (int k = tid; k < n; k += kThreads) {  // no two entries are alike: every one has its rank, in whatever place it lies
+      const uint64_t e = found[k];
+      int rank = 0;
+      for (int i = 0; i < n; ++i) rank += found[i] > e;
+      if (rank < p.top) write(e, rank);
+    }
+    return;
+  }
+  // More than there is room for, as where many are equal: sorted lists of the largest, a warp each, taken in as they come.
   List list{0, 0};
   const int all = (row.vecs + kThreads - 1) / kThreads * kThreads;  // every lane takes every turn
   for (int v = tid; v < all; v += kThreads) {
-    float x[V::n];
-#pragma unroll
-    for (int i = 0; i < V::n; ++i) x[i] = -INFINITY;
     const bool in = v < row.vecs;
-    if (in) V::get(row.load(v), x);
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < V::n; ++i) any |= !(x[i] < floor);
-    if (!__ballot_sync(0xffffffffu, in && any)) continue;
+    const uint4 raw = in ? row.load(v) : V::none();
+    if (!__ballot_sync(0xffffffffu, in && !(V::or_nan(raw) < floor))) continue;
+    float x[V::n];
+    values<V>(raw, x);
 #pragma unroll
     for (int i = 0; i < V::n; ++i) list.offer(x[i], row.index(v) + i, in, floor, p.top);
   }
@@ -271,26 +337,17 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : 1024) forward_kernel(co
     const int odd = row.odd(tid);
     list.offer(odd >= 0 ? V::one(row.p + odd) : 0.f, odd, odd >= 0, floor, p.top);
   }
-  auto write = [&](uint64_t e, int rank) {
-    p.top_log_probs[r * p.top + rank] = (fmaf(value_of((uint32_t)(e >> 32)), kLog2e, -at) - log_l) * kLn2;
-    p.top_tokens[r * p.top + rank] = (uint32_t)~(uint32_t)e;
-  };
   if constexpr (kThreads == 32) {
     if (lane < p.top) write(list.mine, lane);
   } else {
-    const uint32_t have = __ballot_sync(0xffffffffu, lane < p.top && list.mine != 0);
-    int base = 0;
-    if (lane == 0 && have) base = atomicAdd(&count, __popc(have));
-    base = __shfl_sync(0xffffffffu, base, 0);
-    if (have >> lane & 1) found[base + __popc(have & ((1u << lane) - 1))] = list.mine;
     __syncthreads();
-    const int n = count;  // at most 32 of each of 32 warps; no two alike, so every one has its rank, in whatever place
-    if ((int)threadIdx.x < n) {
-      const uint64_t e = found[threadIdx.x];
-      int rank = 0;
-      for (int i = 0; i < n; ++i) rank += found[i] > e;
-      if (rank < p.top) write(e, rank);
-    }
+    found[threadIdx.x] = lane < p.top ? list.mine : 0;
+    __syncthreads();
+    const uint64_t e = found[threadIdx.x];
+    if (!e) return;
+    int rank = 0;
+    for (int i = 0; i < kThreads; ++i) rank += found[i] > e;
+    if (rank < p.top) write(e, rank);
   }
 }
 
@@ -327,29 +384,46 @@ __global__ void __launch_bounds__(256) backward_kernel(const BackwardParams p) {
   else if (token < 0 || token >= p.V) g = p.d_log_probs ? NAN : 0.f;
   const float c = fmaf(h, H, g);
   auto grad = [&](float x, int64_t i) {
-    const float t = fmaf(x, kLog2e, -st.x) - st.y;  // log2 p
-    const float d = -ex2(t) * fmaf(h, fmaxf(t, -1000.f), c);
+    const float t = max_nan((x - st.x) * kLog2e - st.y, kFar);  // log2 p
+    const float d = -ex2(t) * fmaf(h, t, c);
     return i == token ? d + g : d;
   };
-  constexpr int kVecs = kSegment / V::n;
+  constexpr int kVecs = kSegment / V::n, kBatch = 4;
   const int v0 = seg * kVecs, v1 = min(row.vecs, v0 + kVecs);
-#pragma unroll 4
-  for (int v = v0 + lane; v < v1; v += 32) {
-    float x[V::n];
-    V::get(row.load(v), x);
-    const int at = row.index(v);
+  const F2 scale = dup(kLog2e), at_m = dup(-st.x), at_l = dup(-st.y), hs = dup(-h), cs = dup(-c);
+  for (int v = v0 + lane; v < v1; v += 32 * kBatch) {
+    uint4 raw[kBatch];
 #pragma unroll
-    for (int i = 0; i < V::n; ++i) x[i] = grad(x[i], at + i);
-    const uint4 w = V::put(x);
-    if (wide) {
-      *reinterpret_cast<uint4*>(out + at) = w;
-    } else if constexpr (sizeof(T) == 4) {
+    for (int k = 0; k < kBatch; ++k) raw[k] = v + 32 * k < v1 ? row.load(v + 32 * k) : V::none();
 #pragma unroll
-      for (int i = 0; i < V::n; ++i) out[at + i] = x[i];
-    } else {
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    for (int k = 0; k < kBatch; ++k) {
+      if (v + 32 * k >= v1) break;
+      const int at = row.index(v + 32 * k);
+      float x[V::n];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) reinterpret_cast<uint16_t*>(out)[at + i] = (uint16_t)(u[i / 2] >> (16 * (i & 1)));
+      for (int i = 0; i < V::n / 2; ++i) {
+        float a, b;
+        split(fma2(add2(V::pair(raw[k], i), at_m), scale, at_l), a, b);  // log2 p
+        a = max_nan(a, kFar);
+        b = max_nan(b, kFar);
+        split(mul2(f2(ex2(a), ex2(b)), fma2(hs, f2(a, b), cs)), x[2 * i], x[2 * i + 1]);
+      }
+      if (token - at >= 0 && token - at < V::n) {
+#pragma unroll
+        for (int i = 0; i < V::n; ++i)
+          if (at + i == token) x[i] += g;
+      }
+      const uint4 w = V::put(x);
+      if (wide) {
+        *reinterpret_cast<uint4*>(out + at) = w;
+      } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < V::n; ++i) out[at + i] = x[i];
+      } else {
+        const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) reinterpret_cast<uint16_t*>(out)[at + i] = (uint16_t)(q[i / 2] >> (16 * (i & 1)));
+      }
     }
   }
   if (seg == 0) {
