@@ -1,7 +1,7 @@
 // Outer routed attention of long chunks of new tokens over a paged cache.
 //
 // The same product as paged_attn.cu's, for sequences that bring many tokens: 128 query tokens a CTA pair, scores and
-// P V on paired tensor-core instructions into TMEM, laid out as attn_fwd.cu's (attn_layout.cuh).  What differs:
+// P V on paired tensor-core instructions into TMEM, folded as attn_fwd.cu's: a row's 64 first and 64 last keys in two lanes.  What differs:
 //   * keys and values come page by page through the table, boxes of a page's positions (up to the tile's); positions
 //     that the sequence does not have are fetched past the end of the cache, where TMA fills in zeros;
 //   * the softmax offset is each row's own maximum, whatever the keys' lengths.  One map: a running maximum, against
@@ -14,32 +14,69 @@
 // are written and computed again by the other kernel, which tells them apart.
 #include <math.h>
 
-#include "attn_layout.cuh"
+#include "attn_common.h"
 #include "host_util.h"
 #include "paged_chunk.h"
 
 namespace da {
 namespace paged {
 
-using attn::kMaxK;
 using attn::kMaxMaps;
-using attn::kMaxPB;
-using attn::kMaxSB;
-using attn::kMaxV;
-using attn::kRows;
-using attn::Layout;
 
-constexpr int kThreads = 320;  // warp roles as in attn_fwd.cu
-constexpr int kValueWarp = 6, kPvWarp = 7, kKeyWarp2 = 8, kValueWarp2 = 9;
+// Warps: 0 brings keys (and the queries), 1 issues the score products, 2 brings values, 3 issues P V, 4 to 11 turn scores
+// into weights: two warps for each 32 lanes of TMEM, 32 columns a thread.
+constexpr int kThreads = 384, kSoftmaxWarps = 8, kFirstSoftmax = 4;
+constexpr int kRows = 64;   // query rows a CTA
+constexpr int kTile = 128;  // keys a tile: 64 a CTA's box, and 64 score columns a TMEM lane
+constexpr int kMaxK = 8, kMaxV = 4, kScores = 4, kWeights = 2;  // most stages; score and weight buffers
 constexpr int kSmem = 224 * 1024;
 constexpr float kGrow = 8.f;  // log2 of the growth of a row's maximum that its outputs bear
+
+// A CTA's shared memory.  Paired loads take about 0.9 us from a stage's release to its next tile, in which a pair of
+// tensor cores consumes about 2000 cycles' worth: rings of 64 KB and more for keys and values keep them fed.
+struct Shape {
+  int rpb, chunks;   // 64-column blocks a branch, and a map
+  int wide, kslots;  // blocks a key stage, stages
+  int nc, npv, per;  // columns a P V product, products, 64-column blocks of one in a CTA
+  int q_bytes, k_stage, v_stage, p_bytes, nvs;
+  int off_k, off_v, off_p, smem, tmem_cols;
+};
+
+inline Shape make_shape(int maps, int group, int R, int D) {
+  Shape s;
+  s.rpb = R / 64;
+  s.chunks = group * s.rpb;
+  s.wide = s.rpb % 4 == 0 ? 4 : s.rpb % 2 == 0 ? 2 : 1;
+  s.nc = D < 256 ? D : 256;
+  s.npv = D / s.nc;
+  s.per = s.nc / 128;
+  s.q_bytes = kRows * maps * group * R * 2;
+  s.k_stage = s.wide * 64 * 128;
+  s.v_stage = 64 * D;  // 64 keys, half of D columns
+  s.p_bytes = kRows * kTile * 2;
+  const int rings = kSmem - s.q_bytes - kWeights * s.p_bytes;
+  // (several maps: one P V for the keys of all of them, so that keys want the room)
+  s.nvs = maps > 1 ? 2 : (rings - 2 * s.k_stage) / s.v_stage;
+  s.nvs = s.nvs > kMaxV ? kMaxV : s.nvs < 2 ? 2 : s.nvs;
+  s.kslots = (rings - s.nvs * s.v_stage) / s.k_stage;
+  s.kslots = s.kslots > kMaxK ? kMaxK : s.kslots;
+  s.off_k = s.q_bytes;
+  s.off_v = s.off_k + s.kslots * s.k_stage;
+  s.off_p = s.off_v + s.nvs * s.v_stage;
+  const int used = s.off_p + kWeights * s.p_bytes;
+  s.smem = used < 120 * 1024 ? 120 * 1024 : used;  // one CTA an SM: TMEM
+  s.tmem_cols = D / 2 + kScores * 64 > 256 ? 512 : 256;
+  if (D / 2 + kScores * 64 > 512) s.tmem_cols = 0;
+  return s;
+}
 
 struct ChunkParams {
   Cache c;
   Plan plan;
+  Shape shape;
   int H, R, D, maps, group, dtype;
   int branch0[kMaxMaps];
-  int brow_k, brow_v;  // positions a box of keys, of values
+  int brow;            // positions a box
   int phase;           // several maps: 1 sums, 2 outputs; one map: 0
   const float *scales, *weights;
   void* y;
@@ -51,17 +88,11 @@ struct ChunkParams {
   int* status;
 };
 
-// Positions that some row of tile i sees.
-DA_DEV int64_t tile_end(const Cache& c, const Sequence& s, int i) {
-  const int64_t e = s.held + min(s.n, (i + 1) * 128);
-  return e < c.capacity ? e : c.capacity;
-}
-
 // ------------------------------------------------------------------------------------------------ plan
-constexpr int kPlanThreads = 1024, kLengths = 10;
+constexpr int kPlanThreads = 1024, kLengths = 10, kEnds = 4;
 
 // One CTA: a warp a sequence, a tile a lane.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const Plan plan, int few_most, int nk_shift, int pairs) {
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const Plan plan, int few_most, int pairs) {
   __shared__ int2 kept[kPlanThreads];  // the first sequences' new tokens (of chunks), and tokens that they had
   __shared__ unsigned long long units;
   __shared__ int counts[kLengths], carry[2], sums[2][32];
@@ -72,6 +103,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
     const Sequence s = sequence(c, b);
     return make_int2(s.n > few_most ? s.n : 0, (int)s.held);
   };
+  constexpr int nk_shift = 7;  // of kTile
   if (threadIdx.x < c.B) kept[threadIdx.x] = load(threadIdx.x);
   if (threadIdx.x < kLengths) counts[threadIdx.x] = 0;
   if (threadIdx.x == 0) {
@@ -93,7 +125,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
   if (mine) atomicAdd(&units, mine);
   __syncthreads();
   // The pieces' length: of a few that suit one or two rounds of the CTA pairs, the one that is done first, counting a
-  // piece's start and end as two key tiles.
+  // piece's start and end as kEnds key tiles.
   const int64_t total = (int64_t)units;
   auto length = [&](int f) {
     const int64_t round = (int64_t)pairs * (f < 5 ? 1 : 2), base = (total + round - 1) / round;
@@ -125,7 +157,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
   int64_t best_cost = INT64_MAX;
 #pragma unroll
   for (int f = 0; f < kLengths; ++f) {
-    const int64_t cost = (int64_t)((counts[f] + pairs - 1) / pairs) * (len[f] + 2);
+    const int64_t cost = (int64_t)((counts[f] + pairs - 1) / pairs) * (len[f] + kEnds);
     if (cost < best_cost) {
       best_cost = cost;
       best = len[f];
@@ -153,6 +185,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
       carry[1] = piece0 + count;
     }
     if (b < c.B && lane == 0) plan.seq_piece[b] = piece0;
+    const Sequence whole = sequence(c, b < c.B ? b : 0);
     for (int i0 = 0; i0 < tiles; i0 += 32) {
       const int i = i0 + lane, keys = i < tiles ? keys_of(s, i) : 0, own = (unsigned)(keys + best - 1) / (unsigned)best;
       int at = own;
@@ -168,8 +201,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
         const int from = __shfl_sync(0xffffffffu, first, j), many = __shfl_sync(0xffffffffu, own, j);
         const int last = __shfl_sync(0xffffffffu, keys, j);
         for (int m = lane; m < many; m += 32) {
-          plan.pieces[2 * (from + m)] = make_int4(b, i0 + j, m * best, min(best, last - m * best));
-          plan.pieces[2 * (from + m) + 1] = make_int4(from, many, 0, 0);
+          plan.pieces[3 * (from + m)] = make_int4(b, i0 + j, m * best, min(best, last - m * best));
+          plan.pieces[3 * (from + m) + 1] = make_int4(from, many, whole.n, whole.fits);
+          plan.pieces[3 * (from + m) + 2] = make_int4((int)whole.first, (int)whole.held, 0, 0);
           *reinterpret_cast<int2*>(plan.odd + 2 * (from + m)) = make_int2(0, 0);
         }
       }
@@ -185,51 +219,40 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
 }
 
 // ------------------------------------------------------------------------------------------------ attention
+DA_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// A stage or buffer of a ring, and the parity of its barrier.
+struct Turn {
+  int i;
+  uint32_t phase;
+  DA_DEV void next(int n) {
+    if (++i == n) {
+      i = 0;
+      phase ^= 1;
+    }
+  }
+};
+
 template <typename T, bool kMix>
 __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ CUtensorMap tq,
                                                             const __grid_constant__ CUtensorMap tk,
-                                                            const __grid_constant__ CUtensorMap tv, const ChunkParams p) {
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+                                                            const __grid_constant__ CUtensorMap tv,
+                                                            const __grid_constant__ ChunkParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];  // (with the static part, all of an SM's 227 KB: none for padding)
   __shared__ uint64_t q_full, o_full;
   __shared__ uint64_t k_full[kMaxK], k_empty[kMaxK], v_full[kMaxV], v_empty[kMaxV];
-  __shared__ uint64_t s_full[kMaxSB], p_full[kMaxSB], p_empty[kMaxPB], pv_full[kMaxPB];
+  __shared__ uint64_t s_full[kScores], s_empty[kScores], p_full[kWeights], p_empty[kWeights];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag, bad_flag;
-  __shared__ float top[2][128];  // the two halves of a row tell each other their maxima
+  __shared__ float top[2][2][128];  // threads that share a row tell each other their maxima
 
-  grid_dependency_wait();  // the plan and the appended tokens are visible from here on
-  grid_launch_dependents();
-  const int piece = blockIdx.x / 2;
-  if (piece >= p.plan.head[0]) return;
-  const Layout L = attn::make_layout(p.maps, p.group, p.R, p.D, kMix, true, kSmem);
+  const Shape& L = p.shape;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_ctarank() & 1u;
-  const int4 here = p.plan.pieces[2 * piece], tile = p.plan.pieces[2 * piece + 1];
-  const Sequence seq = sequence(p.c, here.x);
-  const int64_t end = tile_end(p.c, seq, here.y);
-  const int t0 = here.y * 128;  // first token of the tile in its sequence
-  const int nk = L.nk, nj = here.w;
-  const int maps = kMix ? p.maps : 1;
-  // (the pieces that run side by side start at different tiles of their ranges: any order gives the same rows)
-  const int rot = piece % nj;
-  auto ktile = [&](int j) { return here.z + (j + rot) % nj; };
-  const bool outputs = !kMix || p.phase == 2;
-  const int U = nj * maps;               // score units: (key tile, map)
-  const int nv = outputs ? nj : 0;       // P.V key tiles
-  Abort ab{&abort_flag, p.status};
-  const int* table = p.c.table + here.x * p.c.table_stride;
-  const int outside = p.c.pages << p.c.page_shift;  // a slot past the cache: zeros
-  auto slot_of = [&](int64_t pos) -> int {
-    if (pos >= end) return outside;
-    const int page = table[pos >> p.c.page_shift];
-    if (page < 0 || page >= p.c.pages) {
-      *reinterpret_cast<volatile int*>(&bad_flag) = 1;
-      return outside;
-    }
-    return (page << p.c.page_shift) + (int)(pos & (p.c.page - 1));
-  };
-
   if (threadIdx.x == 0) {
     abort_flag = bad_flag = 0;
     mbar_init(&q_full, 1);
@@ -242,13 +265,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
     }
-    for (int i = 0; i < kMaxSB; ++i) {
+    for (int i = 0; i < kScores; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 2);
+      mbar_init(&s_empty[i], 2 * kSoftmaxWarps);  // each warp of both CTAs
     }
-    for (int i = 0; i < kMaxPB; ++i) {
+    for (int i = 0; i < kWeights; ++i) {
+      mbar_init(&p_full[i], 2 * kSoftmaxWarps);
       mbar_init(&p_empty[i], 1);
-      mbar_init(&pv_full[i], 2);  // a probability tile is complete in both CTAs
     }
     fence_mbar_init();
   }
@@ -256,271 +279,325 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     tmem_alloc<2>(&tmem_base, L.tmem_cols);
     tmem_relinquish<2>();
   }
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tq);
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
 
-  if (warp == 0 || warp == kKeyWarp2) {
-    // ---------------------------------------------------------------- key producers (both CTAs): warp 0
-    // takes the even key stages (and loads q), warp 8 the odd ones
-    if (lane == 0) {
-      const int pi = warp == 0 ? 0 : 1;
-      prefetch_tmap(&tk);
-      if (pi == 0) {
-        prefetch_tmap(&tq);
-        if (rank == 0) mbar_arrive_expect_tx(&q_full, 2 * L.q_bytes);
-        const uint32_t qf = mapa_shared(smem_u32(&q_full), 0);
-        const int row = (int)(seq.first + t0 + 64 * (int)rank);  // (rows past the last token are zeros)
-        for (int s = 0; s < maps; ++s)
-          for (int gi = 0; gi < p.group; ++gi)
-            for (int kb = 0; kb < L.rpb; ++kb)
-              tma_load_4d_pair(&tq, qf, smem + L.off_q + ((s * p.group + gi) * L.rpb + kb) * (kRows * 128), 0, row,
-                               p.branch0[s] + gi, kb);
-      }
-      int kx = 0;  // key stages of both producers
-      const int stage_bytes = L.kbb * L.k_stage, half = nk / 2;
-      const int wide = p.brow_k == half ? L.kbb : 1;  // column blocks a box
-      for (int u = 0; u < U; ++u) {
-        const int j = u / maps, s = u % maps;
-        bool ok = true;
-        for (int c = 0; c < L.kchunks; c += L.kbb, ++kx) {
-          if (kx % 2 != pi) continue;
-          const int st = kx % L.kslots;
-          if (!mbar_wait(&k_empty[st], ((kx / L.kslots) & 1u) ^ 1u, ab, 71)) { ok = false; break; }
-          if (rank == 0) mbar_arrive_expect_tx(&k_full[st], 2 * stage_bytes);
-          const uint32_t kf = mapa_shared(smem_u32(&k_full[st]), 0);
-          const int gi = c / L.rpb, kb = c % L.rpb;  // kbb divides rpb: a stage never spans two branches
-          const int block = (p.branch0[s] + gi) * L.rpb + kb;
-          const int64_t pos = (int64_t)ktile(j) * nk + (int)rank * half;
-          for (int r0 = 0; r0 < half; r0 += p.brow_k) {
-            const int slot = slot_of(pos + r0);
-            for (int e = 0; e < L.kbb; e += wide)
-              tma_load_3d_pair(&tk, kf, smem + L.off_k + st * stage_bytes + e * L.k_stage + r0 * 128, 0, slot, block + e);
+  grid_dependency_wait();  // the plan and the appended tokens are visible from here on
+  grid_launch_dependents();
+  const int piece = blockIdx.x / 2;  // (the plan has room for every CTA pair's piece)
+  const int4 here = p.plan.pieces[3 * piece], tile = p.plan.pieces[3 * piece + 1], seq = p.plan.pieces[3 * piece + 2];
+  const bool on = piece < p.plan.head[0];
+  const int t0 = here.y * 128;  // first token of the tile in its sequence
+  const int n = tile.z, held = seq.y;
+  const int64_t reach = (int64_t)held + min(n, t0 + 128);
+  const int64_t end = reach < p.c.capacity ? reach : p.c.capacity;  // positions that some row sees
+  const int nj = here.w, maps = kMix ? p.maps : 1;
+  const bool outputs = !kMix || p.phase == 2;
+  Abort ab{&abort_flag, p.status};
+  const int* table = p.c.table + here.x * p.c.table_stride;
+  const int outside = p.c.pages << p.c.page_shift;  // a slot past the cache: zeros
+  auto slot_of = [&](int64_t pos) -> int {
+    if (pos >= end) return outside;
+    const int page = table[pos >> p.c.page_shift];
+    if (page < 0 || page >= p.c.pages) {
+      *reinterpret_cast<volatile int*>(&bad_flag) = 1;
+      return outside;
+    }
+    return (page << p.c.page_shift) + (int)(pos & (p.c.page - 1));
+  };
+  // (the pieces that run side by side start at different tiles of their ranges: any order gives the same rows)
+  int first = on ? piece % nj : 0;
+  auto tile_after = [&](int j) { return j + 1 == nj ? 0 : j + 1; };
+
+  if (!on) {
+  } else if (warp == 0) {
+    // ---------------------------------------------------------------- keys (both CTAs)
+    if (elect_one()) {
+      if (rank == 0) mbar_arrive_expect_tx(&q_full, 2 * L.q_bytes);
+      const uint32_t qf = mapa_shared(smem_u32(&q_full), 0), kf = mapa_shared(smem_u32(&k_full[0]), 0);
+      const int row = seq.x + t0 + 64 * (int)rank;  // (rows past the last token are zeros)
+      uint8_t* dst = smem;
+      for (int s = 0; s < maps; ++s)
+        for (int gi = 0; gi < p.group; ++gi)
+          for (int kb = 0; kb < L.rpb; ++kb, dst += kRows * 128)
+            tma_load_4d_pair(&tq, qf, dst, 0, row, p.branch0[s] + gi, kb);
+      Turn st{0, 0};
+      const bool whole = p.brow == 64;
+      bool ok = true;
+      int used = 0;
+      for (int j = 0, kt = first; ok && j < nj; ++j, kt = tile_after(kt)) {
+        const int64_t pos = (int64_t)(here.z + kt) * kTile + (int)rank * 64;
+        const int slot = slot_of(pos);
+        for (int s = 0; ok && s < maps; ++s)
+          for (int c = 0; c < L.chunks; c += L.wide, st.next(L.kslots), ++used) {
+            if (!(ok = mbar_wait(&k_empty[st.i], st.phase ^ 1u, ab, 71))) break;
+            if (rank == 0) mbar_arrive_expect_tx(&k_full[st.i], 2 * L.k_stage);
+            uint8_t* to = smem + L.off_k + st.i * L.k_stage;
+            const int block = p.branch0[s] * L.rpb + c;  // (a map's branches lie side by side)
+            if (whole) {
+              tma_load_3d_pair(&tk, kf + st.i * 8, to, 0, slot, block);
+            } else {
+              for (int r0 = 0; r0 < 64; r0 += p.brow) {
+                const int at = r0 ? slot_of(pos + r0) : slot;
+                for (int e = 0; e < L.wide; ++e)
+                  tma_load_3d_pair(&tk, kf + st.i * 8, to + (e * 64 + r0) * 128, 0, at, block + e);
+              }
+            }
           }
-        }
-        if (!ok) break;
       }
-      if (rank == 0) {  // drain: none of this producer's loads may be in flight at teardown
-        if (pi == 0) mbar_wait_drain(&q_full, 0);
-        for (int c = (kx > L.kslots ? kx - L.kslots : 0); c < kx; ++c)
-          if (c % 2 == pi) mbar_wait_drain(&k_full[c % L.kslots], (c / L.kslots) & 1u);
+      if (rank == 0) {  // none of the loads may be in flight at teardown
+        mbar_wait_drain(&q_full, 0);
+        for (int i = 0; i < min(used, L.kslots); ++i) {
+          if (st.i-- == 0) {
+            st.i = L.kslots - 1;
+            st.phase ^= 1;
+          }
+          mbar_wait_drain(&k_full[st.i], st.phase);
+        }
       }
     }
-  } else if (warp == kValueWarp || warp == kValueWarp2) {
-    // ---------------------------------------------------------------- value producers: warp 6 even
-    // stages, warp 9 odd ones
-    int vc = 0;
-    const int pi = warp == kValueWarp ? 0 : 1;
-    if (lane == 0) {
-      prefetch_tmap(&tv);
-      for (int v = 0; v < nv; ++v) {
-        bool ok = true;
-        for (int c = 0; c < nk / 64; ++c, ++vc) {
-          if (vc % 2 != pi) continue;
-          const int st = vc % L.nvs;
-          if (!mbar_wait(&v_empty[st], ((vc / L.nvs) & 1u) ^ 1u, ab, 72)) { ok = false; break; }
-          if (rank == 0) mbar_arrive_expect_tx(&v_full[st], 2 * L.v_stage);
-          const uint32_t vf = mapa_shared(smem_u32(&v_full[st]), 0);
-          const int64_t pos = (int64_t)ktile(v) * nk + c * 64;
-          uint8_t* dst = smem + L.off_v + st * L.v_stage;
-          for (int r0 = 0; r0 < 64; r0 += p.brow_v) {
-            const int slot = slot_of(pos + r0);
-            if (p.brow_v == 64) {  // one box: this CTA's per column blocks of each of the npv value groups
-              tma_load_4d_pair(&tv, vf, dst, 0, slot, (int)rank * L.per, 0);
-            } else {
+  } else if (warp == 2) {
+    // ---------------------------------------------------------------- values (both CTAs)
+    Turn st{0, 0};
+    int used = 0;
+    const bool mine = elect_one();
+    if (mine && outputs) {
+      const uint32_t vf = mapa_shared(smem_u32(&v_full[0]), 0);
+      bool ok = true;
+      for (int j = 0, kt = first; ok && j < nj; ++j, kt = tile_after(kt))
+        for (int c = 0; c < 2; ++c, st.next(L.nvs), ++used) {
+          const int64_t pos = (int64_t)(here.z + kt) * kTile + c * 64;
+          const int slot = slot_of(pos);
+          if (!(ok = mbar_wait(&v_empty[st.i], st.phase ^ 1u, ab, 72))) break;
+          if (rank == 0) mbar_arrive_expect_tx(&v_full[st.i], 2 * L.v_stage);
+          uint8_t* to = smem + L.off_v + st.i * L.v_stage;
+          if (p.brow == 64) {  // one box: this CTA's column blocks of each of the value groups
+            tma_load_4d_pair(&tv, vf + st.i * 8, to, 0, slot, (int)rank * L.per, 0);
+          } else {
+            for (int r0 = 0; r0 < 64; r0 += p.brow) {
+              const int at = r0 ? slot_of(pos + r0) : slot;
               for (int i = 0; i < L.npv; ++i)
                 for (int e = 0; e < L.per; ++e)
-                  tma_load_4d_pair(&tv, vf, dst + ((i * L.per + e) * 64 + r0) * 128, 0, slot, (int)rank * L.per + e, i);
+                  tma_load_4d_pair(&tv, vf + st.i * 8, to + ((i * L.per + e) * 64 + r0) * 128, 0, at, (int)rank * L.per + e, i);
             }
           }
         }
-        if (!ok) break;
-      }
     }
     __syncwarp();
-    if (outputs) named_bar_sync(2, 192);  // bad_flag is final
-    if (lane == 0 && rank == 0)
-      for (int c = (vc > L.nvs ? vc - L.nvs : 0); c < vc; ++c)
-        if (c % 2 == pi) mbar_wait_drain(&v_full[c % L.nvs], (c / L.nvs) & 1u);
-  } else if (warp == 1 || warp == kPvWarp) {
-    // ---------------------------------------------------------------- MMA issuers (leader): scores on warp 1,
-    // P.V on warp 7
-    if (rank == 0 && lane == 0) {
-      constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-      const uint32_t idesc_s = idesc_f16(128, nk, bf16, false, false);
-      const uint32_t idesc_o = idesc_f16(128, L.nc, bf16, false, true);  // B = V, MN-major
-      const uint32_t qa = smem_u32(smem + L.off_q);
+    if (outputs) named_bar_sync(2, 32 * (kSoftmaxWarps + 1));  // bad_flag is final
+    if (mine && rank == 0)
+      for (int i = 0; i < min(used, L.nvs); ++i) {
+        if (st.i-- == 0) {
+          st.i = L.nvs - 1;
+          st.phase ^= 1;
+        }
+        mbar_wait_drain(&v_full[st.i], st.phase);
+      }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- scores (the pair's leader)
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = idesc_f16(128, kTile, std::is_same<T, __nv_bfloat16>::value, false, false);
+      const uint64_t qd = sdesc_sw128(smem_u32(smem), 16, 1024), kd = sdesc_sw128(smem_u32(smem + L.off_k), 16, 1024);
       bool ok = mbar_wait(&q_full, 0, ab, 73);
       tc_fence_after();
-      if (warp == 1) {
-        // S units in order; a score buffer is reused once the softmax has consumed its previous unit.
-        int kx = 0, st = 0;  // key stages consumed, current slot
-        for (int u = 0; ok && u < U; ++u) {
-          const int sb = u % L.nsb, s = u % maps;
-          if (u >= L.nsb && !mbar_wait(&p_full[sb], ((u - L.nsb) / L.nsb) & 1u, ab, 74)) { ok = false; break; }
-          const uint32_t d = tmem + L.tmem_s + (uint32_t)(sb * L.s_cols);
-          for (int c = 0; ok && c < L.kchunks; ++c) {
-            const int cib = c % L.kbb;  // chunk inside the current stage
-            if (cib == 0) {
-              st = kx % L.kslots;
-              if (!mbar_wait(&k_full[st], (kx / L.kslots) & 1u, ab, 75)) { ok = false; break; }
-              tc_fence_after();
-            }
-            const uint64_t ad0 = sdesc_sw128(qa + (s * L.kchunks + c) * (kRows * 128), 16, 1024);
-            const uint64_t bd0 =
-                sdesc_sw128(smem_u32(smem + L.off_k + (st * L.kbb + cib) * L.k_stage), 16, 1024);
-#pragma unroll
-            for (int kin = 0; kin < 4; ++kin)  // +32 B per K step of 16 = +2 in the encoded address
-              mma_f16_ss<2>(d, ad0 + 2 * kin, bd0 + 2 * kin, idesc_s, (c | kin) ? 1u : 0u);
-            if (cib == L.kbb - 1) {
-              mma_commit_pair(smem_u32(&k_empty[st]));
-              ++kx;
-            }
-          }
-          if (!ok) break;
-          mma_commit_pair(smem_u32(&s_full[sb]));
-        }
-        if (!outputs) {
-          mma_commit_pair(smem_u32(&o_full));
-          mbar_wait_drain(&o_full, 0);  // every score product has completed
-        }
-      } else if (outputs) {
-        // P.V per key tile, as soon as its probability tile and value rows are in shared memory.
-        int vc = 0;
-        for (int v = 0; ok && v < nv; ++v) {
-          const int pb = v % L.npb;
-          if (!mbar_wait(&pv_full[pb], (v / L.npb) & 1u, ab, 76)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t pa = smem_u32(smem + L.off_p + pb * L.p_bytes);
-          for (int c = 0; ok && c < nk / 64; ++c, ++vc) {
-            const int st = vc % L.nvs;
-            if (!mbar_wait(&v_full[st], (vc / L.nvs) & 1u, ab, 77)) { ok = false; break; }
+      Turn st{0, 0}, sb{0, 0};
+      for (int j = 0; ok && j < nj; ++j) {
+        uint64_t a = qd;
+        for (int s = 0; s < maps; ++s, sb.next(kScores)) {
+          if (!(ok = mbar_wait(&s_empty[sb.i], sb.phase ^ 1u, ab, 74))) break;
+          const uint32_t d = tmem + (uint32_t)(p.D / 2 + sb.i * 64);
+          for (int c = 0; c < L.chunks; c += L.wide, st.next(L.kslots)) {
+            if (!(ok = mbar_wait(&k_full[st.i], st.phase, ab, 75))) break;
             tc_fence_after();
-            const uint32_t va = smem_u32(smem + L.off_v + st * L.v_stage);
-            // MN-major V: rows are keys (K), 128 B = 64 value columns (N);
-            // LBO = distance between 64-column boxes, SBO = 8 key rows.
-            const uint64_t ad0 = sdesc_sw128(pa + c * (kRows * 128), 16, 1024);
-            const uint64_t bd0 = sdesc_sw128(va, 64 * 128, 1024), bd1 = sdesc_sw128(va + L.per * (64 * 128), 64 * 128, 1024);
+            uint64_t b = kd + (uint64_t)(st.i * (L.k_stage >> 4));
+            for (int e = 0; e < L.wide; ++e, a += kRows * 128 / 16, b += kRows * 128 / 16)
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {  // K step of 16 keys: A +32 B (+2), B +16 rows x 128 B (+128)
-              mma_f16_ss<2>(tmem, ad0 + 2 * kk, bd0 + 128 * kk, idesc_o, (v | c | kk) ? 1u : 0u);
-              if (L.npv == 2)  // the two groups' products in turn: neither waits for its own last one
-                mma_f16_ss<2>(tmem + (uint32_t)(L.nc / 2), ad0 + 2 * kk, bd1 + 128 * kk, idesc_o, (v | c | kk) ? 1u : 0u);
-            }
-            mma_commit_pair(smem_u32(&v_empty[st]));
+              for (int k = 0; k < 4; ++k)  // +32 B per K step of 16 = +2 in the encoded address
+                mma_f16_ss<2>(d, a + 2 * k, b + 2 * k, idesc, (c | e | k) ? 1u : 0u);
+            mma_commit_pair(smem_u32(&k_empty[st.i]));
           }
           if (!ok) break;
-          mma_commit_pair(smem_u32(&p_empty[pb]));
+          mma_commit_pair(smem_u32(&s_full[sb.i]));
         }
+      }
+      if (!outputs) {
         mma_commit_pair(smem_u32(&o_full));
-        mbar_wait_drain(&o_full, 0);  // every P.V product (and so every score product) has completed
+        mbar_wait_drain(&o_full, 0);  // every score product has completed
       }
     }
-  } else {
-    // ---------------------------------------------------------------- softmax + epilogue (warps 2 to 5)
-    const int quad = warp & 3;
+  } else if (warp == 3) {
+    // ---------------------------------------------------------------- P V (the pair's leader)
+    if (rank == 0 && outputs && elect_one()) {
+      const uint32_t idesc = idesc_f16(128, L.nc, std::is_same<T, __nv_bfloat16>::value, false, true);  // B = V, MN-major
+      const uint64_t pd = sdesc_sw128(smem_u32(smem + L.off_p), 16, 1024);
+      // MN-major V: rows are keys (K), 128 B = 64 value columns (N); LBO = distance between 64-column boxes, SBO = 8 key rows
+      const uint64_t vd = sdesc_sw128(smem_u32(smem + L.off_v), 64 * 128, 1024);
+      const uint64_t group = (uint64_t)(L.per * (64 * 128) >> 4);
+      Turn st{0, 0}, pb{0, 0};
+      bool ok = true;
+      uint32_t more = 0;
+      for (int j = 0; ok && j < nj; ++j, pb.next(kWeights)) {
+        if (!(ok = mbar_wait(&p_full[pb.i], pb.phase, ab, 76))) break;
+        tc_fence_after();
+        uint64_t a = pd + (uint64_t)(pb.i * (L.p_bytes >> 4));
+        for (int c = 0; c < 2; ++c, a += kRows * 128 / 16, st.next(L.nvs)) {
+          if (!(ok = mbar_wait(&v_full[st.i], st.phase, ab, 77))) break;
+          tc_fence_after();
+          const uint64_t b = vd + (uint64_t)(st.i * (L.v_stage >> 4));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // K step of 16 keys: A +32 B (+2), B +16 rows x 128 B (+128)
+            mma_f16_ss<2>(tmem, a + 2 * k, b + 128 * k, idesc, more);
+            if (L.npv == 2) mma_f16_ss<2>(tmem + (uint32_t)(L.nc / 2), a + 2 * k, b + group + 128 * k, idesc, more);
+            more = 1;
+          }
+          mma_commit_pair(smem_u32(&v_empty[st.i]));
+        }
+        if (!ok) break;
+        mma_commit_pair(smem_u32(&p_empty[pb.i]));
+      }
+      mma_commit_pair(smem_u32(&o_full));
+      mbar_wait_drain(&o_full, 0);  // every P V product (and so every score product) has completed
+    }
+  } else if (warp >= kFirstSoftmax) {
+    // ---------------------------------------------------------------- weights, epilogue
+    const int quad = warp & 3, part = (warp - kFirstSoftmax) >> 2;  // lanes of TMEM, and which 32 of their 64 columns
     const int l = quad * 32 + lane;
-    const int r = l & 63, half = l >> 6;
+    const int r = l & 63, half = l >> 6;  // row of the CTA; which 64 keys of a tile
     const int trow = 64 * (int)rank + r;  // row of the tile
     const int t = t0 + trow;              // token of the sequence
-    const bool live = t < seq.n;
-    const int64_t sees = min(seq.held + t + 1, end);
-    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    const uint32_t pf_leader = mapa_shared(smem_u32(&p_full[0]), 0);
-    const uint32_t pv_leader = mapa_shared(smem_u32(&pv_full[0]), 0);
-    const bool arriver = (warp == 2 && lane == 0);
+    const int64_t sees = min((int64_t)held + t + 1, end);
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const uint32_t scores = tmem + lanes + (uint32_t)(p.D / 2 + part * 32);
+    const uint32_t s_leader = mapa_shared(smem_u32(&s_empty[0]), 0), p_leader = mapa_shared(smem_u32(&p_full[0]), 0);
     const float kLog2e = 1.4426950408889634f;
-    const int hc = nk / 2;  // key columns per thread per tile
-    float scale2[kMaxMaps];
-#pragma unroll
-    for (int s = 0; s < kMaxMaps; ++s) scale2[s] = s < maps ? p.scales[s] * rsqrtf((float)p.group) * kLog2e : 0.f;
+    const float gsc = rsqrtf((float)p.group) * kLog2e;
     bool ok = true;
+    Turn sb{0, 0}, pb{0, 0};
 
-    // Number of visible keys among the 32 columns starting at position k0.
-    auto key_limit = [&](int64_t k0) -> int { return (int)clamp64(sees - k0, 0, 32); };
-    // pb >= 0: this unit completed probability tile buffer pb
-    auto finish_unit = [&](int u, int pb) {
-      if (pb >= 0) fence_proxy_async();
-      tc_fence_before();
-      named_bar_sync(1, 128);
-      if (arriver) {
-        mbar_arrive_cluster_relaxed(pf_leader + (u % L.nsb) * 8);  // score buffer read
-        if (pb >= 0) mbar_arrive_remote(pv_leader + pb * 8);         // probability tile written
+    // This thread's 32 scores of the next unit, the buffer given back.
+    auto take = [&](float (&v)[32]) {
+      if (ok) ok = mbar_wait(&s_full[sb.i], sb.phase, ab, 78);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        tc_fence_after();
+        tmem_ld32(scores + (uint32_t)(sb.i * 64), v);
+        tmem_wait_ld();
+        tc_fence_before();
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster_relaxed(s_leader + sb.i * 8);
+      sb.next(kScores);
     };
-    // One thread's 32 weights of a tile, columns half * hc + ch * 32 and on.
-    auto store_weights = [&](uint32_t pa, int ch, const float* e) {
-      const int kc = half * hc + ch * 32;
-      const uint32_t box = pa + (kc >> 6) * (kRows * 128);
-      const int cb = (kc & 63) >> 3;
+    // Visible keys among this thread's 32 of tile kt.
+    auto visible = [&](int kt) -> int {
+      return (int)clamp64(sees - ((int64_t)(here.z + kt) * kTile + half * 64 + part * 32), 0, 32);
+    };
+    // The tile's weights: this thread's 32 columns, then the buffer handed over.
+    auto give = [&](const float (&e)[32]) {
+      if (ok) ok = mbar_wait(&p_empty[pb.i], pb.phase ^ 1u, ab, 79);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        const uint32_t box = smem_u32(smem + L.off_p + pb.i * L.p_bytes) + half * (kRows * 128);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        st_shared_v4(box + sw128_offset(r, cb + i), pack2<T>(e[8 * i], e[8 * i + 1]), pack2<T>(e[8 * i + 2], e[8 * i + 3]),
-                     pack2<T>(e[8 * i + 4], e[8 * i + 5]), pack2<T>(e[8 * i + 6], e[8 * i + 7]));
+        for (int i = 0; i < 4; ++i)
+          st_shared_v4(box + sw128_offset(r, part * 4 + i), pack2<T>(e[8 * i], e[8 * i + 1]), pack2<T>(e[8 * i + 2], e[8 * i + 3]),
+                       pack2<T>(e[8 * i + 4], e[8 * i + 5]), pack2<T>(e[8 * i + 6], e[8 * i + 7]));
+        fence_proxy_async();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(p_leader + pb.i * 8);
+      pb.next(kWeights);
+    };
+    auto hide = [](float (&v)[32], int lim) {
+      if (!__all_sync(0xffffffffu, lim == 32))
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = i < lim ? v[i] : -INFINITY;
+    };
+    auto largest = [](const float (&v)[32]) {
+      float a = v[0], b = v[1], c = v[2], d = v[3];
+#pragma unroll
+      for (int i = 4; i < 32; i += 4) {
+        a = fmaxf(a, v[i]);
+        b = fmaxf(b, v[i + 1]);
+        c = fmaxf(c, v[i + 2]);
+        d = fmaxf(d, v[i + 3]);
+      }
+      return fmaxf(fmaxf(a, b), fmaxf(c, d));
     };
 
-    float factor = 1.f;              // of the outputs in TMEM
-    float ref = -INFINITY, sum = 0.f;  // one map: offset of the weights, this half's sum
+    float factor = 1.f;                // of the outputs in TMEM
+    float ref = -INFINITY, sum = 0.f;  // one map: offset of the weights (log2), this thread's sum
     if constexpr (kMix) {
+      float scale[kMaxMaps];
+#pragma unroll
+      for (int s = 0; s < kMaxMaps; ++s) scale[s] = s < maps ? p.scales[s] * gsc : 0.f;
       if (p.phase == 1) {
-        // ---- each map's maximum and sum of its weights against it
+        // ---- each map's maximum (of the scaled scores) and sum of its weights against it
         float mx[kMaxMaps], sm[kMaxMaps];
 #pragma unroll
         for (int s = 0; s < kMaxMaps; ++s) {
           mx[s] = -INFINITY;
           sm[s] = 0.f;
         }
-        for (int u = 0; u < U; ++u) {
-          const int j = u / maps, s = u % maps, sb = u % L.nsb;
-          if (ok) ok = mbar_wait(&s_full[sb], (u / L.nsb) & 1u, ab, 78);
-          ok = __all_sync(0xffffffffu, ok);
-          if (ok) {
-            tc_fence_after();
-            float m = mx[s], a = sm[s];
-            const float sc = scale2[s];
-            for (int ch = 0; ch < hc / 32; ++ch) {
-              float v[32];
-              tmem_ld32(tmem + lane_base + L.tmem_s + (uint32_t)(sb * L.s_cols + ch * 32), v);
-              tmem_wait_ld();
-              const int lim = key_limit((int64_t)ktile(j) * nk + half * hc + ch * 32);
-              float big = -INFINITY;
+        for (int j = 0, kt = first; j < nj; ++j, kt = tile_after(kt)) {
+          const int lim = visible(kt);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                v[i] = i < lim ? v[i] * sc : -INFINITY;
-                big = fmaxf(big, v[i]);
-              }
-              const float next = fmaxf(m, big), at = next == -INFINITY ? 0.f : next;
-              a *= m == -INFINITY ? 1.f : ex2(m - at);  // (a is 0 then, or NaN)
-              m = next;
+          for (int s = 0; s < kMaxMaps; ++s) {
+            if (s >= maps) break;
+            float v[32];
+            take(v);
+            if (!ok) continue;
 #pragma unroll
-              for (int i = 0; i < 32; ++i) a += ex2(v[i] - at);
+            for (int i = 0; i < 32; ++i) v[i] *= scale[s];
+            hide(v, lim);
+            const float next = fmaxf(mx[s], largest(v)), at = next == -INFINITY ? 0.f : next;
+            float a = 0.f, b = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              a += ex2(v[i] - at);
+              b += ex2(v[i + 1] - at);
             }
-            mx[s] = m;
-            sm[s] = a;
+            sm[s] = fmaf(sm[s], mx[s] == -INFINITY ? 1.f : ex2(mx[s] - at), a + b);  // (the sum is 0 then, or NaN)
+            mx[s] = next;
           }
-          finish_unit(u, -1);
         }
-        for (int s = 0; s < maps; ++s) {
-          top[0][l] = mx[s];
-          top[1][l] = sm[s];
-          named_bar_sync(1, 128);
-          const float m1 = top[0][l ^ 64], a1 = top[1][l ^ 64], m = fmaxf(mx[s], m1), at = m == -INFINITY ? 0.f : m;
-          const float a = sm[s] * (mx[s] == -INFINITY ? 1.f : ex2(mx[s] - at)) + a1 * (m1 == -INFINITY ? 1.f : ex2(m1 - at));
-          if (half == 0) {
+#pragma unroll
+        for (int s = 0; s < kMaxMaps; ++s) {
+          if (s >= maps) break;
+          // the four threads of a row: two halves of the keys, two parts of them
+          float m = mx[s], a = ok ? sm[s] : NAN;
+#pragma unroll
+          for (int step = 0; step < 2; ++step) {
+            top[0][part][l] = m;
+            top[1][part][l] = a;
+            named_bar_sync(1, 32 * kSoftmaxWarps);
+            const float m1 = step ? top[0][part][l ^ 64] : top[0][part ^ 1][l], a1 = step ? top[1][part][l ^ 64] : top[1][part ^ 1][l];
+            const float to = fmaxf(m, m1), at = to == -INFINITY ? 0.f : to;
+            const float own = a * (m == -INFINITY ? 1.f : ex2(m - at)), other = a1 * (m1 == -INFINITY ? 1.f : ex2(m1 - at));
+            a = own + other;
+            m = to;
+            named_bar_sync(1, 32 * kSoftmaxWarps);
+          }
+          if (half == 0 && part == 0) {
             float* dst = p.stats + ((size_t)piece * 2 * maps + s) * 128 + trow;
             dst[0] = m;
-            dst[(size_t)maps * 128] = ok ? a : NAN;
+            dst[(size_t)maps * 128] = a;
           }
-          named_bar_sync(1, 128);
         }
       } else {
         // ---- the pieces' sums of this row; offsets so that the mixture's largest weight is near 1
-        float off2[kMaxMaps], al[kMaxMaps], shift = -INFINITY;
+        float off[kMaxMaps], al[kMaxMaps], shift = -INFINITY;
 #pragma unroll
         for (int s = 0; s < kMaxMaps; ++s) {
-          off2[s] = al[s] = 0.f;
+          off[s] = al[s] = 0.f;
           if (s < maps) {
             const float* src = p.stats + ((size_t)tile.x * 2 * maps + s) * 128 + trow;
             const size_t next = (size_t)2 * maps * 128;
@@ -532,162 +609,158 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
               a += ai * (mi == -INFINITY ? 1.f : ex2(mi - at));
             }
             al[s] = p.weights ? p.weights[s] : 1.f;
-            off2[s] = m + log2f(a);
+            off[s] = m + log2f(a);
             shift = fmaxf(shift, log2f(fabsf(al[s])) - log2f(a));
           }
         }
         shift = fminf(fmaxf(shift, -100.f), 100.f);
         factor = ex2(shift);
-        float pm[64];
-        for (int v = 0; v < nv; ++v) {
-          const int pb = v % L.npb;
-          const uint32_t pa = smem_u32(smem + L.off_p + pb * L.p_bytes);
-          for (int s = 0; s < maps; ++s) {
-            const int u = v * maps + s, sb = u % L.nsb;
-            if (ok) ok = mbar_wait(&s_full[sb], (u / L.nsb) & 1u, ab, 78);
-            if (ok && s == 0 && v >= L.npb) ok = mbar_wait(&p_empty[pb], ((v - L.npb) / L.npb) & 1u, ab, 79);
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) {
-              tc_fence_after();
-              const float sc = scale2[s], off = off2[s] + shift, w = al[s];
-              for (int ch = 0; ch < hc / 32; ++ch) {
-                float sv[32];
-                tmem_ld32(tmem + lane_base + L.tmem_s + (uint32_t)(sb * L.s_cols + ch * 32), sv);
-                tmem_wait_ld();
-                const int lim = key_limit((int64_t)ktile(v) * nk + half * hc + ch * 32);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                  const float e = i < lim ? w * ex2(sv[i] * sc - off) : 0.f;
-                  pm[ch * 32 + i] = s == 0 ? e : pm[ch * 32 + i] + e;
-                }
-              }
-              if (s == maps - 1)
-                for (int ch = 0; ch < hc / 32; ++ch) store_weights(pa, ch, pm + ch * 32);
+        for (int s = 0; s < kMaxMaps; ++s) off[s] += shift;
+        for (int j = 0, kt = first; j < nj; ++j, kt = tile_after(kt)) {
+          const int lim = visible(kt);
+          float pm[32];
+#pragma unroll
+          for (int s = 0; s < kMaxMaps; ++s) {
+            if (s >= maps) break;
+            float v[32];
+            take(v);
+            if (!ok) continue;
+            hide(v, lim);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float e = ex2(fmaf(v[i], scale[s], -off[s]));
+              pm[i] = s == 0 ? al[0] * e : fmaf(al[s], e, pm[i]);
             }
-            finish_unit(u, s == maps - 1 ? pb : -1);
           }
+          give(pm);
         }
       }
     } else {
       // ---- one map: weights against a maximum that follows the row
-      for (int v = 0; v < nv; ++v) {
-        const int pb = v % L.npb, sb = v % L.nsb;
-        const uint32_t pa = smem_u32(smem + L.off_p + pb * L.p_bytes);
-        const uint32_t scores = tmem + lane_base + L.tmem_s + (uint32_t)(sb * L.s_cols);
-        const int64_t k0 = (int64_t)ktile(v) * nk + half * hc;
-        if (ok) ok = mbar_wait(&s_full[sb], (v / L.nsb) & 1u, ab, 78);
-        if (ok && v >= L.npb) ok = mbar_wait(&p_empty[pb], ((v - L.npb) / L.npb) & 1u, ab, 79);
-        ok = __all_sync(0xffffffffu, ok);
+      const float scale = p.scales[0] * gsc;
+      for (int j = 0, kt = first; j < nj; ++j, kt = tile_after(kt)) {
+        float v[32];
+        take(v);
         float big = -INFINITY;
         if (ok) {
-          tc_fence_after();
-          for (int ch = 0; ch < hc / 32; ++ch) {
-            float s[32];
-            tmem_ld32(scores + ch * 32, s);
-            tmem_wait_ld();
-            const int lim = key_limit(k0 + ch * 32);
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < lim) big = fmaxf(big, s[i] * scale2[0]);
-          }
+          for (int i = 0; i < 32; ++i) v[i] *= scale;
+          hide(v, visible(kt));
+          big = largest(v);
         }
-        top[v & 1][l] = big;
-        named_bar_sync(1, 128);
-        big = fmaxf(big, top[v & 1][l ^ 64]);
+        float (&mine)[2][128] = top[j & 1];
+        mine[part][l] = big;
+        named_bar_sync(1, 32 * kSoftmaxWarps);
+        big = fmaxf(fmaxf(mine[0][l], mine[1][l]), fmaxf(mine[0][l ^ 64], mine[1][l ^ 64]));
         const bool grown = big > ref + kGrow || (ref == -INFINITY && big > ref);
         if (__any_sync(0xffffffffu, grown)) {
           const float next = grown ? big : ref;
           const float c = !grown || ref == -INFINITY ? 1.f : ex2(ref - next);
           ref = next;
           sum *= c;
-          if (v > 0 && ok) {  // the outputs so far, once the products into them are done
-            ok = mbar_wait(&p_empty[(v - 1) % L.npb], ((v - 1) / L.npb) & 1u, ab, 80);
+          if (j > 0 && ok && __any_sync(0xffffffffu, c != 1.f)) {  // the outputs so far, once the products into them are done
+            const int before = pb.i == 0 ? kWeights - 1 : pb.i - 1;
+            ok = mbar_wait(&p_empty[before], pb.i == 0 ? pb.phase ^ 1u : pb.phase, ab, 80);
             ok = __all_sync(0xffffffffu, ok);
-            if (ok && __any_sync(0xffffffffu, c != 1.f)) {
+            if (ok) {
               tc_fence_after();
-              for (int col = 0; col < p.D / 2; col += 32) {
+              for (int col = part * (p.D / 4); col < (part + 1) * (p.D / 4); col += 32) {
                 float o[32];
-                tmem_ld32(tmem + lane_base + (uint32_t)col, o);
+                tmem_ld32(tmem + lanes + (uint32_t)col, o);
                 tmem_wait_ld();
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] *= c;
-                tmem_st32(tmem + lane_base + (uint32_t)col, o);
+                tmem_st32(tmem + lanes + (uint32_t)col, o);
               }
               tmem_wait_st();
+              tc_fence_before();
             }
           }
         }
-        if (ok) {
-          const float at = ref == -INFINITY ? 0.f : ref;
-          for (int ch = 0; ch < hc / 32; ++ch) {
-            float s[32];
-            tmem_ld32(scores + ch * 32, s);
-            tmem_wait_ld();
-            const int lim = key_limit(k0 + ch * 32);
-            float part = 0.f;
+        const float at = ref == -INFINITY ? 0.f : ref;
+        float a = 0.f, b = 0.f;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              s[i] = i < lim ? ex2(s[i] * scale2[0] - at) : 0.f;
-              part += s[i];
-            }
-            sum += part;
-            store_weights(pa, ch, s);
-          }
+        for (int i = 0; i < 32; i += 2) {
+          v[i] = ex2(v[i] - at);
+          v[i + 1] = ex2(v[i + 1] - at);
+          a += v[i];
+          b += v[i + 1];
         }
-        finish_unit(v, pb);
+        sum += a + b;
+        give(v);
       }
     }
 
     // ---- epilogue
     if (outputs) {
-      named_bar_sync(2, 192);
-      const bool wrong = !seq.fits || *reinterpret_cast<volatile int*>(&bad_flag);
-      if (wrong && arriver) atomicOr(p.status, DA_DEV_BAD_PAGE);
+      named_bar_sync(2, 32 * (kSoftmaxWarps + 1));
+      const bool wrong = !tile.w || *reinterpret_cast<volatile int*>(&bad_flag);
+      if (wrong && warp == kFirstSoftmax && lane == 0) atomicOr(p.status, DA_DEV_BAD_PAGE);
       if (!kMix) {
-        top[0][l] = sum;
-        named_bar_sync(1, 128);
-        sum += top[0][l ^ 64];
+        top[0][part][l] = sum;
+        named_bar_sync(1, 32 * kSoftmaxWarps);
+        sum = (top[0][0][r] + top[0][1][r]) + (top[0][0][r + 64] + top[0][1][r + 64]);
       }
       if (ok) ok = mbar_wait(&o_full, 0, ab, 81);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      const bool whole = tile.y == 1;
-      if (!kMix && whole) factor = 1.f / sum;
+      const bool single = tile.y == 1;
+      if (!kMix && single) factor = 1.f / sum;
       if (wrong || !ok) factor = NAN;
+      if (!kMix && !single && part == 0 && half == 0 && t < n) {
+        p.part_ml[(size_t)piece * 256 + trow] = ref;
+        p.part_ml[(size_t)piece * 256 + 128 + trow] = wrong || !ok ? NAN : sum;
+      }
       float odd = 0.f;  // becomes NaN with any output that is no number
-      const int64_t row = seq.first + t;
       if (ok) {
-        for (int i = 0; i < L.npv; ++i) {
-          const int col0 = i * L.nc + half * (L.nc / 2);
-          for (int c = 0; c < L.nc / 2; c += 32) {
-            float o[32];
-            tmem_ld32(tmem + lane_base + (uint32_t)(i * (L.nc / 2) + c), o);
-            tmem_wait_ld();
+        // 32 rows by 32 columns at a time go through shared memory (the keys' ring, done with), so that a row's columns
+        // are stored side by side.
+        const uint32_t stage = smem_u32(smem + L.off_k) + (uint32_t)(warp - kFirstSoftmax) * 4096;
+        const int base = trow - lane;       // tile row of lane 0 (a warp's lanes are consecutive rows)
+        for (int tc = part * (p.D / 4); tc < (part + 1) * (p.D / 4); tc += 32) {
+          const int col = tc / (L.nc / 2) * L.nc + half * (L.nc / 2) + tc % (L.nc / 2);
+          float o[32];
+          tmem_ld32(tmem + lanes + (uint32_t)tc, o);
+          tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              odd = fmaf(o[e], 0.f, odd);
-              o[e] *= factor;
+          for (int e = 0; e < 32; ++e) {
+            odd = fmaf(o[e], 0.f, odd);
+            o[e] *= factor;
+          }
+          __syncwarp();
+          if (!single) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              st_shared_v4(stage + sw128_offset(lane, e), __float_as_uint(o[4 * e]), __float_as_uint(o[4 * e + 1]),
+                           __float_as_uint(o[4 * e + 2]), __float_as_uint(o[4 * e + 3]));
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int row = e * 4 + lane / 8;
+              const uint4 w = ld_shared_v4(stage + sw128_offset(row, lane & 7));
+              if (t0 + base + row < n)
+                *reinterpret_cast<uint4*>(p.part + ((size_t)piece * 128 + base + row) * p.D + col + (lane & 7) * 4) = w;
             }
-            if (live && !whole) {
-              float4* dst = reinterpret_cast<float4*>(p.part + ((size_t)piece * 128 + trow) * p.D + col0 + c);
+          } else {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            } else if (live) {
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.y) + row * p.y_row + col0 + c);
+            for (int e = 0; e < 4; ++e)
+              st_shared_v4(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4), pack2<T>(o[8 * e], o[8 * e + 1]),
+                           pack2<T>(o[8 * e + 2], o[8 * e + 3]), pack2<T>(o[8 * e + 4], o[8 * e + 5]),
+                           pack2<T>(o[8 * e + 6], o[8 * e + 7]));
+            __syncwarp();
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                dst[e] = make_uint4(pack2<T>(o[8 * e], o[8 * e + 1]), pack2<T>(o[8 * e + 2], o[8 * e + 3]),
-                                    pack2<T>(o[8 * e + 4], o[8 * e + 5]), pack2<T>(o[8 * e + 6], o[8 * e + 7]));
+            for (int e = 0; e < 4; ++e) {
+              const int row = e * 8 + lane / 4;
+              const uint4 w = ld_shared_v4(stage + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
+              if (t0 + base + row < n)
+                *reinterpret_cast<uint4*>(static_cast<T*>(p.y) + ((int64_t)seq.x + t0 + base + row) * p.y_row + col + (lane & 3) * 8) = w;
             }
           }
         }
       }
-      if (!kMix && live && !whole && half == 0) {
-        p.part_ml[(size_t)piece * 256 + trow] = ref;
-        p.part_ml[(size_t)piece * 256 + 128 + trow] = wrong || !ok ? NAN : sum;
-      }
-      const bool spoiled = named_bar_or(1, 128, live && !wrong && ok && odd != 0.f);
-      if (arriver) p.plan.odd[2 * piece + (int)rank] |= spoiled;
+      const bool spoiled = named_bar_or(1, 32 * kSoftmaxWarps, t < n && !wrong && ok && odd != 0.f);
+      if (warp == kFirstSoftmax && lane == 0) p.plan.odd[2 * piece + (int)rank] |= spoiled;
     }
   }
 
@@ -705,11 +778,10 @@ __global__ void __launch_bounds__(256) join_kernel(const ChunkParams p, const bo
   if ((int)blockIdx.x >= p.plan.head[1]) return;
   const int first = p.plan.tile_piece[blockIdx.x], pieces = p.plan.tile_piece[blockIdx.x + 1] - first;
   if (pieces < 2) return;
-  const int4 here = p.plan.pieces[2 * first];
-  const Sequence seq = sequence(p.c, here.x);
+  const int4 here = p.plan.pieces[3 * first], tile = p.plan.pieces[3 * first + 1], seq = p.plan.pieces[3 * first + 2];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, parts = p.D / 128;
   const int trow = blockIdx.y * (8 / parts) + warp / parts, t = here.y * 128 + trow, col = (warp % parts) * 128 + lane * 4;
-  if (t >= seq.n) return;
+  if (t >= tile.z) return;
   const float* ml = p.part_ml + (size_t)first * 256 + trow;
   float top = -INFINITY, sum = 0.f;
   if (weighted) {
@@ -748,7 +820,7 @@ __global__ void __launch_bounds__(256) join_kernel(const ChunkParams p, const bo
     for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
     f = 1.f / sum;
   }
-  T* y = static_cast<T*>(p.y) + (seq.first + t) * p.y_row + col;
+  T* y = static_cast<T*>(p.y) + ((int64_t)seq.x + t) * p.y_row + col;
   *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(o.x * f, o.y * f), pack2<T>(o.z * f, o.w * f));
 }
 
@@ -765,7 +837,7 @@ void most(int64_t tokens, int64_t B, int few_most, int64_t* tiles, int64_t* piec
 }
 
 int64_t plan_bytes(int64_t B, int64_t tiles, int64_t pieces) {
-  return 16 + round16((B + 1) * 4) + round16((tiles + 1) * 4) + pieces * 32 + round16(pieces * 8);
+  return 16 + round16((B + 1) * 4) + round16((tiles + 1) * 4) + pieces * 48 + round16(pieces * 8);
 }
 
 template <typename T>
@@ -788,10 +860,11 @@ int run(const ChunkArgs& a, cudaStream_t st) {
   p.status = a.status;
   const bool mix = a.maps > 1 && !a.per_map;
   p.maps = mix ? a.maps : 1;
-  const Layout L = attn::make_layout(p.maps, a.group, a.R, a.D, mix, true, kSmem);
-  if (L.nks < 2 || L.nsb < 2) return DA_ERR_UNSUPPORTED;
-  p.brow_k = a.c.page < L.nk / 2 ? a.c.page : L.nk / 2;
-  p.brow_v = a.c.page < 64 ? a.c.page : 64;
+  p.shape = make_shape(p.maps, a.group, a.R, a.D);
+  const Shape& L = p.shape;
+  if (L.kslots < 2 || !L.tmem_cols) return DA_ERR_UNSUPPORTED;
+  p.brow = a.c.page < 64 ? a.c.page : 64;
+  const bool whole = p.brow == 64;
   const CUtensorMapDataType dt = a.dtype == DA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap tq, tk, tv;
   {  // queries: (column in its block of 64, row, branch, block)
@@ -803,22 +876,20 @@ int run(const ChunkArgs& a, cudaStream_t st) {
   {  // keys: (column in its block, slot, block)
     const uint64_t dims[3] = {64, (uint64_t)a.c.pages * a.c.page, (uint64_t)a.H * a.R / 64};
     const uint64_t strides[2] = {(uint64_t)a.H * a.R * 2, 128};
-    const uint32_t box[3] = {64, (uint32_t)p.brow_k, (uint32_t)(p.brow_k == L.nk / 2 ? L.kbb : 1)};
+    const uint32_t box[3] = {64, (uint32_t)p.brow, (uint32_t)(whole ? L.wide : 1)};
     if (int rc = make_tmap_blocks(&tk, a.key_pages, dt, 2, 3, dims, strides, box)) return rc;
   }
   {  // values: (column in its block, slot, block inside an nc-wide group, group)
     const uint64_t dims[4] = {64, (uint64_t)a.c.pages * a.c.page, (uint64_t)L.nc / 64, (uint64_t)a.D / L.nc};
     const uint64_t strides[3] = {(uint64_t)a.D * 2, 128, (uint64_t)L.nc * 2};
-    const bool whole = p.brow_v == 64;
-    const uint32_t box[4] = {64, (uint32_t)p.brow_v, (uint32_t)(whole ? L.per : 1), (uint32_t)(whole ? L.npv : 1)};
+    const uint32_t box[4] = {64, (uint32_t)p.brow, (uint32_t)(whole ? L.per : 1), (uint32_t)(whole ? L.npv : 1)};
     if (int rc = make_tmap_blocks(&tv, a.value_pages, dt, 2, 4, dims, strides, box)) return rc;
   }
   if (int rc = launch_kernel(plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, false, a.c, p.plan, a.few_most,
-                             L.nk == 256 ? 8 : 7, sm_count() / 2))
+                             sm_count() / 2))
     return rc;
-  const int smem = L.smem + 1024;
   const dim3 grid((unsigned)(2 * pieces)), block(kThreads);
-  if (int rc = mix ? allow_smem<chunk_kernel<T, true>>(kSmem + 1024) : allow_smem<chunk_kernel<T, false>>(kSmem + 1024)) return rc;
+  if (int rc = mix ? allow_smem<chunk_kernel<T, true>>(kSmem) : allow_smem<chunk_kernel<T, false>>(kSmem)) return rc;
   for (int s = 0; s < (a.per_map ? a.maps : 1); ++s) {
     for (int m = 0; m < kMaxMaps; ++m) {
       const int map = a.per_map ? s : m;
@@ -831,10 +902,10 @@ int run(const ChunkArgs& a, cudaStream_t st) {
     p.phase = 0;
     if (mix) {
       p.phase = 1;
-      if (int rc = launch_kernel(chunk_kernel<T, true>, grid, block, smem, st, true, tq, tk, tv, p)) return rc;
+      if (int rc = launch_kernel(chunk_kernel<T, true>, grid, block, L.smem, st, true, tq, tk, tv, p)) return rc;
       p.phase = 2;
-      if (int rc = launch_kernel(chunk_kernel<T, true>, grid, block, smem, st, true, tq, tk, tv, p)) return rc;
-    } else if (int rc = launch_kernel(chunk_kernel<T, false>, grid, block, smem, st, true, tq, tk, tv, p)) {
+      if (int rc = launch_kernel(chunk_kernel<T, true>, grid, block, L.smem, st, true, tq, tk, tv, p)) return rc;
+    } else if (int rc = launch_kernel(chunk_kernel<T, false>, grid, block, L.smem, st, true, tq, tk, tv, p)) {
       return rc;
     }
     if (int rc = launch_kernel(join_kernel<T>, dim3((unsigned)tiles, (unsigned)(16 * a.D / 128)), dim3(256), 0, st, false, p, !mix)) return rc;
@@ -863,7 +934,7 @@ Plan chunk_plan(void* workspace, int64_t tokens, int64_t B, int few_most) {
   p.tile_piece = reinterpret_cast<int*>(at);
   at += round16((tiles + 1) * 4);
   p.pieces = reinterpret_cast<int4*>(at);
-  at += pieces * 32;
+  at += pieces * 48;
   p.odd = reinterpret_cast<int*>(at);
   p.tiles_most = (int)tiles;
   p.pieces_most = (int)pieces;

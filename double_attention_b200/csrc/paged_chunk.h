@@ -8,8 +8,8 @@ namespace paged {
 
 // The chunk kernel's plan, made on the device from the step's lengths: `head` is {pieces, tiles, 0, 0}; sequence b's tiles
 // of 128 tokens have pieces seq_piece[b] .. seq_piece[b + 1], tile k the pieces tile_piece[k] .. tile_piece[k + 1];
-// piece i is {sequence, tile of the sequence, first key tile, key tiles} and {first piece of its tile, pieces of its
-// tile, 0, 0}.  odd[2 * piece + rank] says that live rows of that CTA came out NaN.
+// piece i is {sequence, tile of the sequence, first key tile, key tiles}, {first piece of its tile, pieces of its
+// tile, the sequence's new tokens, whether the table holds it} and {its first packed row, tokens that it had, 0, 0}.  odd[2 * piece + rank] says that live rows of that CTA came out NaN.
 struct Plan {
   int* head;
   int* seq_piece;
