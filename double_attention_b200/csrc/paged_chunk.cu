@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         fence_proxy_async();
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(p_leader + pb.i * 8);
+      if (lane == 0) mbar_arrive_remote(p_leader + pb.i * 8);
       pb.next(kWeights);
     };
     auto hide = [](float (&v)[32], int lim) {
