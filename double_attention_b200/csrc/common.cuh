@@ -64,6 +64,11 @@ DA_DEV void named_bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(threads) : "memory");
 }
 
+// Comes to a named barrier without waiting for it.
+DA_DEV void named_bar_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" :: "r"(id), "r"(threads) : "memory");
+}
+
 // named_bar_sync that tells every thread whether any of them brought `v`.
 DA_DEV bool named_bar_or(int id, int threads, bool v) {
   uint32_t r;

@@ -23,9 +23,10 @@ namespace paged {
 
 using attn::kMaxMaps;
 
-// Warps: 0 brings keys (and the queries), 1 issues the score products, 2 brings values, 3 issues P V, 4 to 11 turn scores
-// into weights: two warps for each 32 lanes of TMEM, 32 columns a thread.
-constexpr int kThreads = 384, kSoftmaxWarps = 8, kFirstSoftmax = 4;
+// Warps: 0 brings keys (and the queries), 1 issues the score products, 2 brings values, 3 issues P V; 4 to 11 and 12 to 19
+// turn scores into weights, the two groups taking tiles in turn, so that one computes while the other waits; in a group, two
+// warps share 32 lanes of TMEM, 32 columns a thread.
+constexpr int kThreads = 640, kSoftmaxWarps = 16, kGroupWarps = 8, kFirstSoftmax = 4;
 constexpr int kRows = 64;   // query rows a CTA
 constexpr int kTile = 128;  // keys a tile: 64 a CTA's box, and 64 score columns a TMEM lane
 constexpr int kMaxK = 8, kMaxV = 4, kScores = 4, kWeights = 2;  // most stages; score and weight buffers
@@ -248,7 +249,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   __shared__ uint64_t s_full[kScores], s_empty[kScores], p_full[kWeights], p_empty[kWeights];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag, bad_flag;
-  __shared__ float top[2][2][128];  // threads that share a row tell each other their maxima
+  __shared__ float top[2][2][128];  // what the four threads of a row in a group tell each other
+  __shared__ float row_ref[kRows];             // one map: each row's offset, handed from tile to tile
 
   const Shape& L = p.shape;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -267,10 +269,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     }
     for (int i = 0; i < kScores; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], 2 * kSoftmaxWarps);  // each warp of both CTAs
+      mbar_init(&s_empty[i], 2 * kGroupWarps);  // each warp of a group, of both CTAs
     }
     for (int i = 0; i < kWeights; ++i) {
-      mbar_init(&p_full[i], 2 * kSoftmaxWarps);
+      mbar_init(&p_full[i], 2 * kGroupWarps);
       mbar_init(&p_empty[i], 1);
     }
     fence_mbar_init();
@@ -468,7 +470,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     }
   } else if (warp >= kFirstSoftmax) {
     // ---------------------------------------------------------------- weights, epilogue
-    const int quad = warp & 3, part = (warp - kFirstSoftmax) >> 2;  // lanes of TMEM, and which 32 of their 64 columns
+    const int quad = warp & 3, group = (warp - kFirstSoftmax) / kGroupWarps;  // lanes of TMEM; whose turn
+    const int part = ((warp - kFirstSoftmax) >> 2) & 1;                      // which 32 of a lane's 64 columns
     const int l = quad * 32 + lane;
     const int r = l & 63, half = l >> 6;  // row of the CTA; which 64 keys of a tile
     const int trow = 64 * (int)rank + r;  // row of the tile
@@ -476,13 +479,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     const int64_t sees = min((int64_t)held + t + 1, end);
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t scores = tmem + lanes + (uint32_t)(p.D / 2 + part * 32);
+    float* scratch = reinterpret_cast<float*>(smem + L.off_k);  // [2][4][128]: the keys' ring, when they are done with
     const uint32_t s_leader = mapa_shared(smem_u32(&s_empty[0]), 0), p_leader = mapa_shared(smem_u32(&p_full[0]), 0);
     const float kLog2e = 1.4426950408889634f;
     const float gsc = rsqrtf((float)p.group) * kLog2e;
     bool ok = true;
-    Turn sb{0, 0}, pb{0, 0};
+    Turn sb{0, 0};
 
-    // This thread's 32 scores of the next unit, the buffer given back.
+    // The next unit's scores, 32 a thread; the buffer is given back.
     auto take = [&](float (&v)[32]) {
       if (ok) ok = mbar_wait(&s_full[sb.i], sb.phase, ab, 78);
       ok = __all_sync(0xffffffffu, ok);
@@ -494,18 +498,19 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       }
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster_relaxed(s_leader + sb.i * 8);
-      sb.next(kScores);
     };
-    // Visible keys among this thread's 32 of tile kt.
+    // Visible keys among the thread's 32 of tile kt.
     auto visible = [&](int kt) -> int {
       return (int)clamp64(sees - ((int64_t)(here.z + kt) * kTile + half * 64 + part * 32), 0, 32);
     };
-    // The tile's weights: this thread's 32 columns, then the buffer handed over.
+    // A tile's weights into buffer `group`, as the tiles take turns; p_phase is of its barrier.
+    uint32_t p_phase = 1;
+    const uint32_t box = smem_u32(smem + L.off_p + group * L.p_bytes) + half * (kRows * 128);
     auto give = [&](const float (&e)[32]) {
-      if (ok) ok = mbar_wait(&p_empty[pb.i], pb.phase ^ 1u, ab, 79);
+      if (ok) ok = mbar_wait(&p_empty[group], p_phase, ab, 79);
       ok = __all_sync(0xffffffffu, ok);
+      p_phase ^= 1;
       if (ok) {
-        const uint32_t box = smem_u32(smem + L.off_p + pb.i * L.p_bytes) + half * (kRows * 128);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           st_shared_v4(box + sw128_offset(r, part * 4 + i), pack2<T>(e[8 * i], e[8 * i + 1]), pack2<T>(e[8 * i + 2], e[8 * i + 3]),
@@ -513,8 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         fence_proxy_async();
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive_remote(p_leader + pb.i * 8);
-      pb.next(kWeights);
+      if (lane == 0) mbar_arrive_remote(p_leader + group * 8);
     };
     auto hide = [](float (&v)[32], int lim) {
       if (!__all_sync(0xffffffffu, lim == 32))
@@ -547,70 +551,90 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           mx[s] = -INFINITY;
           sm[s] = 0.f;
         }
+        int unit = 0;
         for (int j = 0, kt = first; j < nj; ++j, kt = tile_after(kt)) {
           const int lim = visible(kt);
 #pragma unroll
           for (int s = 0; s < kMaxMaps; ++s) {
             if (s >= maps) break;
-            float v[32];
-            take(v);
-            if (!ok) continue;
+            if ((unit++ & 1) == group) {
+              float v[32];
+              take(v);
+              if (ok) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= scale[s];
-            hide(v, lim);
-            const float next = fmaxf(mx[s], largest(v)), at = next == -INFINITY ? 0.f : next;
-            float a = 0.f, b = 0.f;
+                for (int i = 0; i < 32; ++i) v[i] *= scale[s];
+                hide(v, lim);
+                const float next = fmaxf(mx[s], largest(v)), at = next == -INFINITY ? 0.f : next;
+                float a = 0.f, b = 0.f;
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              a += ex2(v[i] - at);
-              b += ex2(v[i + 1] - at);
+                for (int i = 0; i < 32; i += 2) {
+                  a += ex2(v[i] - at);
+                  b += ex2(v[i + 1] - at);
+                }
+                sm[s] = fmaf(sm[s], mx[s] == -INFINITY ? 1.f : ex2(mx[s] - at), a + b);  // (the sum is 0 then, or NaN)
+                mx[s] = next;
+              }
             }
-            sm[s] = fmaf(sm[s], mx[s] == -INFINITY ? 1.f : ex2(mx[s] - at), a + b);  // (the sum is 0 then, or NaN)
-            mx[s] = next;
+            sb.next(kScores);
           }
         }
+        named_bar_sync(1, 32 * kSoftmaxWarps);  // (every score product is over)
 #pragma unroll
         for (int s = 0; s < kMaxMaps; ++s) {
           if (s >= maps) break;
-          // the four threads of a row: two halves of the keys, two parts of them
-          float m = mx[s], a = ok ? sm[s] : NAN;
+          scratch[(group * 2 + part) * 128 + l] = mx[s];
+          scratch[512 + (group * 2 + part) * 128 + l] = ok ? sm[s] : NAN;
+          named_bar_sync(1, 32 * kSoftmaxWarps);
+          if (group == 0 && part == 0 && half == 0) {  // the eight threads of a row: groups, parts and halves
+            float m = -INFINITY, a = 0.f;
 #pragma unroll
-          for (int step = 0; step < 2; ++step) {
-            top[0][part][l] = m;
-            top[1][part][l] = a;
-            named_bar_sync(1, 32 * kSoftmaxWarps);
-            const float m1 = step ? top[0][part][l ^ 64] : top[0][part ^ 1][l], a1 = step ? top[1][part][l ^ 64] : top[1][part ^ 1][l];
-            const float to = fmaxf(m, m1), at = to == -INFINITY ? 0.f : to;
-            const float own = a * (m == -INFINITY ? 1.f : ex2(m - at)), other = a1 * (m1 == -INFINITY ? 1.f : ex2(m1 - at));
-            a = own + other;
-            m = to;
-            named_bar_sync(1, 32 * kSoftmaxWarps);
-          }
-          if (half == 0 && part == 0) {
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, scratch[(i >> 1) * 128 + (i & 1) * 64 + r]);
+            const float at = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float mi = scratch[(i >> 1) * 128 + (i & 1) * 64 + r];
+              a += scratch[512 + (i >> 1) * 128 + (i & 1) * 64 + r] * (mi == -INFINITY ? 1.f : ex2(mi - at));
+            }
             float* dst = p.stats + ((size_t)piece * 2 * maps + s) * 128 + trow;
             dst[0] = m;
             dst[(size_t)maps * 128] = a;
           }
+          named_bar_sync(1, 32 * kSoftmaxWarps);
         }
       } else {
         // ---- the pieces' sums of this row; offsets so that the mixture's largest weight is near 1
         float off[kMaxMaps], al[kMaxMaps], shift = -INFINITY;
+        {
+          const float* src = p.stats + (size_t)tile.x * 2 * maps * 128 + trow;
+          const size_t next = (size_t)2 * maps * 128;
+          float m[kMaxMaps], a[kMaxMaps];
 #pragma unroll
-        for (int s = 0; s < kMaxMaps; ++s) {
-          off[s] = al[s] = 0.f;
-          if (s < maps) {
-            const float* src = p.stats + ((size_t)tile.x * 2 * maps + s) * 128 + trow;
-            const size_t next = (size_t)2 * maps * 128;
-            float m = -INFINITY, a = 0.f;
-            for (int i = 0; i < tile.y; ++i) m = fmaxf(m, src[i * next]);
-            const float at = m == -INFINITY ? 0.f : m;
-            for (int i = 0; i < tile.y; ++i) {
-              const float mi = src[i * next], ai = src[i * next + (size_t)maps * 128];
-              a += ai * (mi == -INFINITY ? 1.f : ex2(mi - at));
+          for (int s = 0; s < kMaxMaps; ++s) {
+            m[s] = -INFINITY;
+            a[s] = 0.f;
+          }
+#pragma unroll 2
+          for (int i = 0; i < tile.y; ++i, src += next) {
+            float mi[kMaxMaps], ai[kMaxMaps];
+#pragma unroll
+            for (int s = 0; s < kMaxMaps; ++s) {
+              mi[s] = s < maps ? src[(size_t)s * 128] : -INFINITY;
+              ai[s] = s < maps ? src[(size_t)(maps + s) * 128] : 0.f;
             }
+#pragma unroll
+            for (int s = 0; s < kMaxMaps; ++s) {
+              const float to = fmaxf(m[s], mi[s]), at = to == -INFINITY ? 0.f : to;
+              a[s] = a[s] * (m[s] == -INFINITY ? 1.f : ex2(m[s] - at)) + ai[s] * (mi[s] == -INFINITY ? 1.f : ex2(mi[s] - at));
+              m[s] = to;
+            }
+          }
+#pragma unroll
+          for (int s = 0; s < kMaxMaps; ++s) {
+            off[s] = al[s] = 0.f;
+            if (s >= maps) continue;
             al[s] = p.weights ? p.weights[s] : 1.f;
-            off[s] = m + log2f(a);
-            shift = fmaxf(shift, log2f(fabsf(al[s])) - log2f(a));
+            off[s] = m[s] + log2f(a[s]);
+            shift = fmaxf(shift, log2f(fabsf(al[s])) - log2f(a[s]));
           }
         }
         shift = fminf(fmaxf(shift, -100.f), 100.f);
@@ -618,6 +642,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 #pragma unroll
         for (int s = 0; s < kMaxMaps; ++s) off[s] += shift;
         for (int j = 0, kt = first; j < nj; ++j, kt = tile_after(kt)) {
+          if ((j & 1) != group) {
+            for (int s = 0; s < maps; ++s) sb.next(kScores);
+            continue;
+          }
           const int lim = visible(kt);
           float pm[32];
 #pragma unroll
@@ -625,6 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             if (s >= maps) break;
             float v[32];
             take(v);
+            sb.next(kScores);
             if (!ok) continue;
             hide(v, lim);
 #pragma unroll
@@ -637,47 +666,55 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         }
       }
     } else {
-      // ---- one map: weights against a maximum that follows the row
+      // ---- one map: weights against a maximum that follows the row.  The offset of tile j + 1 starts from tile j's, which the
+      // other group leaves in row_ref.
       const float scale = p.scales[0] * gsc;
-      for (int j = 0, kt = first; j < nj; ++j, kt = tile_after(kt)) {
-        float v[32];
+      for (int j = 0, kt = first; j < nj; ++j, kt = tile_after(kt), sb.next(kScores)) {
+        if ((j & 1) != group) continue;
+        float v[32], big = -INFINITY;
         take(v);
-        float big = -INFINITY;
         if (ok) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] *= scale;
           hide(v, visible(kt));
           big = largest(v);
         }
-        float (&mine)[2][128] = top[j & 1];
+        float (&mine)[2][128] = top[group];
         mine[part][l] = big;
-        named_bar_sync(1, 32 * kSoftmaxWarps);
+        if (j) named_bar_sync(3 + group, 32 * kSoftmaxWarps);  // tile j - 1's offsets are there (and the maxima)
+        else named_bar_sync(5, 32 * kGroupWarps);
         big = fmaxf(fmaxf(mine[0][l], mine[1][l]), fmaxf(mine[0][l ^ 64], mine[1][l ^ 64]));
+        const float last = j ? row_ref[r] : -INFINITY;
+        if (last != ref) {  // the other group's tile raised it
+          if (ref != -INFINITY) sum *= ex2(ref - last);
+          ref = last;
+        }
         const bool grown = big > ref + kGrow || (ref == -INFINITY && big > ref);
-        if (__any_sync(0xffffffffu, grown)) {
-          const float next = grown ? big : ref;
-          const float c = !grown || ref == -INFINITY ? 1.f : ex2(ref - next);
-          ref = next;
+        const float next = grown ? big : ref;
+        const bool rescale = grown && ref != -INFINITY;
+        const bool any = named_bar_or(5 + group, 32 * kGroupWarps, rescale);  // (row_ref is read: it may be written)
+        if (half == 0 && part == 0) row_ref[r] = next;
+        if (j + 1 < nj) named_bar_arrive(4 - group, 32 * kSoftmaxWarps);
+        if (any) {  // the outputs so far, once the products into them are done: tile j - 1's
+          const float c = rescale ? ex2(ref - next) : 1.f;
           sum *= c;
-          if (j > 0 && ok && __any_sync(0xffffffffu, c != 1.f)) {  // the outputs so far, once the products into them are done
-            const int before = pb.i == 0 ? kWeights - 1 : pb.i - 1;
-            ok = mbar_wait(&p_empty[before], pb.i == 0 ? pb.phase ^ 1u : pb.phase, ab, 80);
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) {
-              tc_fence_after();
-              for (int col = part * (p.D / 4); col < (part + 1) * (p.D / 4); col += 32) {
-                float o[32];
-                tmem_ld32(tmem + lanes + (uint32_t)col, o);
-                tmem_wait_ld();
+          if (ok) ok = mbar_wait(&p_empty[group ^ 1], group ? p_phase ^ 1u : p_phase, ab, 80);
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok) {
+            tc_fence_after();
+            for (int col = part * (p.D / 4); col < (part + 1) * (p.D / 4); col += 32) {
+              float o[32];
+              tmem_ld32(tmem + lanes + (uint32_t)col, o);
+              tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] *= c;
-                tmem_st32(tmem + lanes + (uint32_t)col, o);
-              }
-              tmem_wait_st();
-              tc_fence_before();
+              for (int i = 0; i < 32; ++i) o[i] *= c;
+              tmem_st32(tmem + lanes + (uint32_t)col, o);
             }
+            tmem_wait_st();
+            tc_fence_before();
           }
         }
+        ref = next;
         const float at = ref == -INFINITY ? 0.f : ref;
         float a = 0.f, b = 0.f;
 #pragma unroll
@@ -697,10 +734,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       named_bar_sync(2, 32 * (kSoftmaxWarps + 1));
       const bool wrong = !tile.w || *reinterpret_cast<volatile int*>(&bad_flag);
       if (wrong && warp == kFirstSoftmax && lane == 0) atomicOr(p.status, DA_DEV_BAD_PAGE);
-      if (!kMix) {
-        top[0][part][l] = sum;
+      if (!kMix) {  // (the group that had the tile before the last one may have an older offset)
+        const float last = row_ref[r];
+        if (ref != -INFINITY && ref != last) sum *= ex2(ref - last);
+        ref = last;
+        scratch[(group * 2 + part) * 128 + l] = sum;
         named_bar_sync(1, 32 * kSoftmaxWarps);
-        sum = (top[0][0][r] + top[0][1][r]) + (top[0][0][r + 64] + top[0][1][r + 64]);
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += scratch[i * 128 + r] + scratch[i * 128 + 64 + r];
+        named_bar_sync(1, 32 * kSoftmaxWarps);
       }
       if (ok) ok = mbar_wait(&o_full, 0, ab, 81);
       ok = __all_sync(0xffffffffu, ok);
@@ -708,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       const bool single = tile.y == 1;
       if (!kMix && single) factor = 1.f / sum;
       if (wrong || !ok) factor = NAN;
-      if (!kMix && !single && part == 0 && half == 0 && t < n) {
+      if (!kMix && !single && group == 0 && part == 0 && half == 0 && t < n) {
         p.part_ml[(size_t)piece * 256 + trow] = ref;
         p.part_ml[(size_t)piece * 256 + 128 + trow] = wrong || !ok ? NAN : sum;
       }
@@ -718,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         // are stored side by side.
         const uint32_t stage = smem_u32(smem + L.off_k) + (uint32_t)(warp - kFirstSoftmax) * 4096;
         const int base = trow - lane;       // tile row of lane 0 (a warp's lanes are consecutive rows)
-        for (int tc = part * (p.D / 4); tc < (part + 1) * (p.D / 4); tc += 32) {
+        for (int tc = (group * 2 + part) * 32; tc < p.D / 2; tc += 128) {
           const int col = tc / (L.nc / 2) * L.nc + half * (L.nc / 2) + tc % (L.nc / 2);
           float o[32];
           tmem_ld32(tmem + lanes + (uint32_t)tc, o);
