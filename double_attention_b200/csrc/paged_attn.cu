@@ -808,7 +808,7 @@ extern "C" int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_r
   p.few_most = chunked ? few_most(lanes) : 0x7fffffff;
   p.chunked = chunked;
   if (chunked) p.chunks = paged::chunk_plan(workspace, tokens, B, p.few_most);
-  p.few_rows = f.few_rows;
+  p.few_rows = f.few_rows < p.few_most ? f.few_rows : p.few_most;
   p.stages = f.stages;
   p.stage_bytes = f.stage_bytes;
   p.key_bytes = f.key_bytes;

@@ -43,7 +43,8 @@ struct Shape {
   int off_k, off_v, off_p, smem, tmem_cols;
 };
 
-inline Shape make_shape(int maps, int group, int R, int D) {
+// outputs: values and weights have room too (else scores alone).
+inline Shape make_shape(int maps, int group, int R, int D, bool outputs) {
   Shape s;
   s.rpb = R / 64;
   s.chunks = group * s.rpb;
@@ -55,16 +56,16 @@ inline Shape make_shape(int maps, int group, int R, int D) {
   s.k_stage = s.wide * 64 * 128;
   s.v_stage = 64 * D;  // 64 keys, half of D columns
   s.p_bytes = kRows * kTile * 2;
-  const int rings = kSmem - s.q_bytes - kWeights * s.p_bytes;
+  const int rings = kSmem - s.q_bytes - (outputs ? kWeights * s.p_bytes : 0);
   // (several maps: one P V for the keys of all of them, so that keys want the room)
   s.nvs = maps > 1 ? 2 : (rings - 2 * s.k_stage) / s.v_stage;
-  s.nvs = s.nvs > kMaxV ? kMaxV : s.nvs < 2 ? 2 : s.nvs;
+  s.nvs = !outputs ? 0 : s.nvs > kMaxV ? kMaxV : s.nvs < 2 ? 2 : s.nvs;
   s.kslots = (rings - s.nvs * s.v_stage) / s.k_stage;
   s.kslots = s.kslots > kMaxK ? kMaxK : s.kslots;
   s.off_k = s.q_bytes;
   s.off_v = s.off_k + s.kslots * s.k_stage;
   s.off_p = s.off_v + s.nvs * s.v_stage;
-  const int used = s.off_p + kWeights * s.p_bytes;
+  const int used = s.off_p + (outputs ? kWeights * s.p_bytes : 0);
   s.smem = used < 120 * 1024 ? 120 * 1024 : used;  // one CTA an SM: TMEM
   s.tmem_cols = D / 2 + kScores * 64 > 256 ? 512 : 256;
   if (D / 2 + kScores * 64 > 512) s.tmem_cols = 0;
@@ -82,7 +83,7 @@ struct ChunkParams {
   const float *scales, *weights;
   void* y;
   int64_t y_row;       // elements from row to row
-  float* part;         // [pieces][128][D]
+  float* part;         // [pieces][2 CTAs][D / 16] blocks of 32 rows by 32 columns
   float* part_ml;      // [pieces][2][128]: one map's maximum (log2) and sum
   float* stats;        // [pieces][2][maps][128]: phase 1's
   int few_most;
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
       carry[0] = tile0 + tiles;
       carry[1] = piece0 + count;
     }
-    if (b < c.B && lane == 0) plan.seq_piece[b] = piece0;
+    if (b < c.B && lane == 0) plan.odd[b] = 0;
     const Sequence whole = sequence(c, b < c.B ? b : 0);
     for (int i0 = 0; i0 < tiles; i0 += 32) {
       const int i = i0 + lane, keys = i < tiles ? keys_of(s, i) : 0, own = (unsigned)(keys + best - 1) / (unsigned)best;
@@ -205,7 +206,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
           plan.pieces[3 * (from + m)] = make_int4(b, i0 + j, m * best, min(best, last - m * best));
           plan.pieces[3 * (from + m) + 1] = make_int4(from, many, whole.n, whole.fits);
           plan.pieces[3 * (from + m) + 2] = make_int4((int)whole.first, (int)whole.held, 0, 0);
-          *reinterpret_cast<int2*>(plan.odd + 2 * (from + m)) = make_int2(0, 0);
         }
       }
       piece0 += all;
@@ -213,7 +213,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    plan.seq_piece[c.B] = carry[1];
     plan.tile_piece[carry[0]] = carry[1];
     *reinterpret_cast<int4*>(plan.head) = make_int4(carry[1], carry[0], 0, 0);
   }
@@ -327,6 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       const uint32_t qf = mapa_shared(smem_u32(&q_full), 0), kf = mapa_shared(smem_u32(&k_full[0]), 0);
       const int row = seq.x + t0 + 64 * (int)rank;  // (rows past the last token are zeros)
       uint8_t* dst = smem;
+      int slot = slot_of((int64_t)(here.z + first) * kTile + (int)rank * 64);
       for (int s = 0; s < maps; ++s)
         for (int gi = 0; gi < p.group; ++gi)
           for (int kb = 0; kb < L.rpb; ++kb, dst += kRows * 128)
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       int used = 0;
       for (int j = 0, kt = first; ok && j < nj; ++j, kt = tile_after(kt)) {
         const int64_t pos = (int64_t)(here.z + kt) * kTile + (int)rank * 64;
-        const int slot = slot_of(pos);
+        if (j) slot = slot_of(pos);
         for (int s = 0; ok && s < maps; ++s)
           for (int c = 0; c < L.chunks; c += L.wide, st.next(L.kslots), ++used) {
             if (!(ok = mbar_wait(&k_empty[st.i], st.phase ^ 1u, ab, 71))) break;
@@ -603,38 +603,42 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         }
       } else {
         // ---- the pieces' sums of this row; offsets so that the mixture's largest weight is near 1
+        // (the row's eight threads share them out: a map and every other piece each)
         float off[kMaxMaps], al[kMaxMaps], shift = -INFINITY;
         {
-          const float* src = p.stats + (size_t)tile.x * 2 * maps * 128 + trow;
-          const size_t next = (size_t)2 * maps * 128;
-          float m[kMaxMaps], a[kMaxMaps];
-#pragma unroll
-          for (int s = 0; s < kMaxMaps; ++s) {
-            m[s] = -INFINITY;
-            a[s] = 0.f;
-          }
-#pragma unroll 2
-          for (int i = 0; i < tile.y; ++i, src += next) {
-            float mi[kMaxMaps], ai[kMaxMaps];
-#pragma unroll
-            for (int s = 0; s < kMaxMaps; ++s) {
-              mi[s] = s < maps ? src[(size_t)s * 128] : -INFINITY;
-              ai[s] = s < maps ? src[(size_t)(maps + s) * 128] : 0.f;
-            }
-#pragma unroll
-            for (int s = 0; s < kMaxMaps; ++s) {
-              const float to = fmaxf(m[s], mi[s]), at = to == -INFINITY ? 0.f : to;
-              a[s] = a[s] * (m[s] == -INFINITY ? 1.f : ex2(m[s] - at)) + ai[s] * (mi[s] == -INFINITY ? 1.f : ex2(mi[s] - at));
-              m[s] = to;
+          float* meet = &top[0][0][0];  // [4][2][64]
+          const int s = group * 2 + part;
+          float m = -INFINITY, a = 0.f;
+          if (s < maps) {
+            const float* src = p.stats + ((size_t)tile.x * 2 * maps + s) * 128 + trow;
+            const size_t next = (size_t)2 * maps * 128;
+#pragma unroll 4
+            for (int i = half; i < tile.y; i += 2) {
+              const float mi = src[i * next], ai = src[i * next + (size_t)maps * 128];
+              const float to = fmaxf(m, mi), at = to == -INFINITY ? 0.f : to;
+              a = a * (m == -INFINITY ? 1.f : ex2(m - at)) + ai * (mi == -INFINITY ? 1.f : ex2(mi - at));
+              m = to;
             }
           }
+          meet[(s * 2 + half) * 64 + r] = m;
+          named_bar_sync(1, 32 * kSoftmaxWarps);
+          const float to = fmaxf(meet[s * 128 + r], meet[s * 128 + 64 + r]), at = to == -INFINITY ? 0.f : to;
+          a *= m == -INFINITY ? 1.f : ex2(m - at);
+          named_bar_sync(1, 32 * kSoftmaxWarps);
+          meet[(s * 2 + half) * 64 + r] = a;
+          named_bar_sync(1, 32 * kSoftmaxWarps);
+          a = meet[s * 128 + r] + meet[s * 128 + 64 + r];
+          named_bar_sync(1, 32 * kSoftmaxWarps);
+          meet[(s * 2 + half) * 64 + r] = half ? log2f(a) : to;
+          named_bar_sync(1, 32 * kSoftmaxWarps);
 #pragma unroll
-          for (int s = 0; s < kMaxMaps; ++s) {
-            off[s] = al[s] = 0.f;
-            if (s >= maps) continue;
-            al[s] = p.weights ? p.weights[s] : 1.f;
-            off[s] = m[s] + log2f(a[s]);
-            shift = fmaxf(shift, log2f(fabsf(al[s])) - log2f(a[s]));
+          for (int i = 0; i < kMaxMaps; ++i) {
+            off[i] = al[i] = 0.f;
+            if (i >= maps) continue;
+            const float log_sum = meet[i * 128 + 64 + r];
+            al[i] = p.weights ? p.weights[i] : 1.f;
+            off[i] = meet[i * 128 + r] + log_sum;
+            shift = fmaxf(shift, log2f(fabsf(al[i])) - log_sum);
           }
         }
         shift = fminf(fmaxf(shift, -100.f), 100.f);
@@ -757,9 +761,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       }
       float odd = 0.f;  // becomes NaN with any output that is no number
       if (ok) {
-        // 32 rows by 32 columns at a time go through shared memory (the keys' ring, done with), so that a row's columns
-        // are stored side by side.
-        const uint32_t stage = smem_u32(smem + L.off_k) + (uint32_t)(warp - kFirstSoftmax) * 4096;
+        // 32 rows by 32 columns at a time go through shared memory (the rings, done with), each to a place of its own: a
+        // piece's part as one bulk copy into a block of 4 KB (4500 cycles for a CTA's 128 KB when all write, against 7000
+        // by stores), a finished row's columns so that they are stored side by side.
         const int base = trow - lane;       // tile row of lane 0 (a warp's lanes are consecutive rows)
         for (int tc = (group * 2 + part) * 32; tc < p.D / 2; tc += 128) {
           const int col = tc / (L.nc / 2) * L.nc + half * (L.nc / 2) + tc % (L.nc / 2);
@@ -771,20 +775,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             odd = fmaf(o[e], 0.f, odd);
             o[e] *= factor;
           }
-          __syncwarp();
+          const int blk = tc / 32 * 4 + quad;
+          const uint32_t stage = smem_u32(smem + L.off_k) + (uint32_t)blk * 4096;
           if (!single) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               st_shared_v4(stage + sw128_offset(lane, e), __float_as_uint(o[4 * e]), __float_as_uint(o[4 * e + 1]),
                            __float_as_uint(o[4 * e + 2]), __float_as_uint(o[4 * e + 3]));
+            fence_proxy_async();
             __syncwarp();
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int row = e * 4 + lane / 8;
-              const uint4 w = ld_shared_v4(stage + sw128_offset(row, lane & 7));
-              if (t0 + base + row < n)
-                *reinterpret_cast<uint4*>(p.part + ((size_t)piece * 128 + base + row) * p.D + col + (lane & 7) * 4) = w;
-            }
+            if (lane == 0)
+              bulk_store(p.part + (((size_t)piece * 2 + rank) * (p.D / 16) + blk) * 1024, smem + L.off_k + blk * 4096, 4096);
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -802,8 +803,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           }
         }
       }
+      if (!single && lane == 0) {
+        tma_store_commit();
+        tma_store_wait_all();
+      }
       const bool spoiled = named_bar_or(1, 32 * kSoftmaxWarps, t < n && !wrong && ok && odd != 0.f);
-      if (warp == kFirstSoftmax && lane == 0) p.plan.odd[2 * piece + (int)rank] |= spoiled;
+      if (spoiled && warp == kFirstSoftmax && lane == 0) atomicOr(p.plan.odd + here.x, 1);
     }
   }
 
@@ -833,7 +838,11 @@ __global__ void __launch_bounds__(256) join_kernel(const ChunkParams p, const bo
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (top == -INFINITY) top = 0.f;
   }
-  const float* src = p.part + ((size_t)first * 128 + trow) * p.D + col;
+  // the block of 32 rows by 32 columns, as the chunk kernel's TMEM has them, and the place in its row
+  const int nc = p.shape.nc, half = col % nc / (nc / 2), tc = col / nc * (nc / 2) + col % (nc / 2), r = trow & 63;
+  const int blk = tc / 32 * 4 + half * 2 + r / 32;
+  const float* src = p.part + (((size_t)first * 2 + trow / 64) * (p.D / 16) + blk) * 1024 + (r % 32) * 32 +
+                     ((tc % 32 / 4) ^ (r & 7)) * 4;
   const size_t step = (size_t)128 * p.D;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int base = 0; base < pieces; base += 32) {
@@ -880,7 +889,7 @@ void most(int64_t tokens, int64_t B, int few_most, int64_t* tiles, int64_t* piec
 }
 
 int64_t plan_bytes(int64_t B, int64_t tiles, int64_t pieces) {
-  return 16 + round16((B + 1) * 4) + round16((tiles + 1) * 4) + pieces * 48 + round16(pieces * 8);
+  return 16 + round16(B * 4) + round16((tiles + 1) * 4) + pieces * 48;
 }
 
 template <typename T>
@@ -903,8 +912,8 @@ int run(const ChunkArgs& a, cudaStream_t st) {
   p.status = a.status;
   const bool mix = a.maps > 1 && !a.per_map;
   p.maps = mix ? a.maps : 1;
-  p.shape = make_shape(p.maps, a.group, a.R, a.D);
-  const Shape& L = p.shape;
+  p.shape = make_shape(p.maps, a.group, a.R, a.D, true);
+  const Shape L = p.shape;
   if (L.kslots < 2 || !L.tmem_cols) return DA_ERR_UNSUPPORTED;
   p.brow = a.c.page < 64 ? a.c.page : 64;
   const bool whole = p.brow == 64;
@@ -945,8 +954,10 @@ int run(const ChunkArgs& a, cudaStream_t st) {
     p.phase = 0;
     if (mix) {
       p.phase = 1;
-      if (int rc = launch_kernel(chunk_kernel<T, true>, grid, block, L.smem, st, true, tq, tk, tv, p)) return rc;
+      p.shape = make_shape(p.maps, a.group, a.R, a.D, false);
+      if (int rc = launch_kernel(chunk_kernel<T, true>, grid, block, p.shape.smem, st, true, tq, tk, tv, p)) return rc;
       p.phase = 2;
+      p.shape = L;
       if (int rc = launch_kernel(chunk_kernel<T, true>, grid, block, L.smem, st, true, tq, tk, tv, p)) return rc;
     } else if (int rc = launch_kernel(chunk_kernel<T, false>, grid, block, L.smem, st, true, tq, tk, tv, p)) {
       return rc;
@@ -972,13 +983,11 @@ Plan chunk_plan(void* workspace, int64_t tokens, int64_t B, int few_most) {
   Plan p;
   p.head = reinterpret_cast<int*>(at);
   at += 16;
-  p.seq_piece = reinterpret_cast<int*>(at);
-  at += round16((B + 1) * 4);
+  p.odd = reinterpret_cast<int*>(at);
+  at += round16(B * 4);
   p.tile_piece = reinterpret_cast<int*>(at);
   at += round16((tiles + 1) * 4);
   p.pieces = reinterpret_cast<int4*>(at);
-  at += pieces * 48;
-  p.odd = reinterpret_cast<int*>(at);
   p.tiles_most = (int)tiles;
   p.pieces_most = (int)pieces;
   return p;

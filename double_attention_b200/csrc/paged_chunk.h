@@ -6,16 +6,15 @@
 namespace da {
 namespace paged {
 
-// The chunk kernel's plan, made on the device from the step's lengths: `head` is {pieces, tiles, 0, 0}; sequence b's tiles
-// of 128 tokens have pieces seq_piece[b] .. seq_piece[b + 1], tile k the pieces tile_piece[k] .. tile_piece[k + 1];
-// piece i is {sequence, tile of the sequence, first key tile, key tiles}, {first piece of its tile, pieces of its
-// tile, the sequence's new tokens, whether the table holds it} and {its first packed row, tokens that it had, 0, 0}.  odd[2 * piece + rank] says that live rows of that CTA came out NaN.
+// The chunk kernel's plan, made on the device from the step's lengths: `head` is {pieces, tiles, 0, 0}; tile k, of 128 new
+// tokens, has the pieces tile_piece[k] .. tile_piece[k + 1]; piece i is {sequence, tile of the sequence, first key tile, key
+// tiles}, {first piece of its tile, pieces of its tile, the sequence's new tokens, whether the table holds it} and {its
+// first packed row, tokens that it had, 0, 0}.  odd[b] says that live rows of sequence b came out NaN.
 struct Plan {
   int* head;
-  int* seq_piece;
+  int* odd;
   int* tile_piece;
   int4* pieces;
-  int* odd;
   int tiles_most, pieces_most;
 };
 
@@ -40,11 +39,7 @@ int chunk_attention(const ChunkArgs& a, cudaStream_t st);
 
 // Whether the chunk kernel left NaN in live rows of sequence b, the other kernel's to compute again: a masked value that is no
 // number spoils the rows of a matrix product, which weigh it with 0.
-DA_DEV bool left_odd(const Plan& p, int b) {
-  int any = 0;
-  for (int i = 2 * p.seq_piece[b]; i < 2 * p.seq_piece[b + 1]; ++i) any |= p.odd[i];
-  return any != 0;
-}
+DA_DEV bool left_odd(const Plan& p, int b) { return p.odd[b] != 0; }
 
 }  // namespace paged
 }  // namespace da
