@@ -29,7 +29,8 @@ using attn::kMaxMaps;
 constexpr int kThreads = 640, kSoftmaxWarps = 16, kGroupWarps = 8, kFirstSoftmax = 4;
 constexpr int kRows = 64;   // query rows a CTA
 constexpr int kTile = 128;  // keys a tile: 64 a CTA's box, and 64 score columns a TMEM lane
-constexpr int kMaxK = 8, kMaxV = 4, kScores = 4, kWeights = 2;  // most stages; score and weight buffers
+constexpr int kMaxK = 8, kMaxV = 4;        // most stages
+constexpr int kScores = 4, kWeights = 2;  // buffers of scores, two a group of softmax warps, and of weights, one a group
 constexpr int kSmem = 224 * 1024;
 constexpr float kGrow = 8.f;  // log2 of the growth of a row's maximum that its outputs bear
 
@@ -410,12 +411,19 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       const uint64_t qd = sdesc_sw128(smem_u32(smem), 16, 1024), kd = sdesc_sw128(smem_u32(smem + L.off_k), 16, 1024);
       bool ok = mbar_wait(&q_full, 0, ab, 73);
       tc_fence_after();
-      Turn st{0, 0}, sb{0, 0};
+      Turn st{0, 0}, sb0{0, 0}, sb1{0, 0};
+      int unit = 0;
       for (int j = 0; ok && j < nj; ++j) {
         uint64_t a = qd;
-        for (int s = 0; s < maps; ++s, sb.next(kScores)) {
-          if (!(ok = mbar_wait(&s_empty[sb.i], sb.phase ^ 1u, ab, 74))) break;
-          const uint32_t d = tmem + (uint32_t)(p.D / 2 + sb.i * 64);
+        for (int s = 0; s < maps; ++s, ++unit) {
+          // the group's own two buffers (one that the groups shared would complete phases that a group never waits for, and a
+          // wait for the phase after those would end at once)
+          const int group = (outputs ? j : unit) & 1;
+          Turn& sb = group ? sb1 : sb0;
+          const int buffer = 2 * group + sb.i;
+          if (!(ok = mbar_wait(&s_empty[buffer], sb.phase ^ 1u, ab, 74))) break;
+          sb.next(2);
+          const uint32_t d = tmem + (uint32_t)(p.D / 2 + buffer * 64);
           for (int c = 0; c < L.chunks; c += L.wide, st.next(L.kslots)) {
             if (!(ok = mbar_wait(&k_full[st.i], st.phase, ab, 75))) break;
             tc_fence_after();
@@ -427,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             mma_commit_pair(smem_u32(&k_empty[st.i]));
           }
           if (!ok) break;
-          mma_commit_pair(smem_u32(&s_full[sb.i]));
+          mma_commit_pair(smem_u32(&s_full[buffer]));
         }
       }
       if (!outputs) {
@@ -478,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     const int t = t0 + trow;              // token of the sequence
     const int64_t sees = min((int64_t)held + t + 1, end);
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    const uint32_t scores = tmem + lanes + (uint32_t)(p.D / 2 + part * 32);
+    const uint32_t scores = tmem + lanes + (uint32_t)(p.D / 2 + group * 128 + part * 32);
     float* scratch = reinterpret_cast<float*>(smem + L.off_k);  // [2][4][128]: the keys' ring, when they are done with
     const uint32_t s_leader = mapa_shared(smem_u32(&s_empty[0]), 0), p_leader = mapa_shared(smem_u32(&p_full[0]), 0);
     const float kLog2e = 1.4426950408889634f;
@@ -486,9 +494,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     bool ok = true;
     Turn sb{0, 0};
 
-    // The next unit's scores, 32 a thread; the buffer is given back.
+    // The group's next scores, 32 a thread; the buffer is given back.
     auto take = [&](float (&v)[32]) {
-      if (ok) ok = mbar_wait(&s_full[sb.i], sb.phase, ab, 78);
+      if (ok) ok = mbar_wait(&s_full[2 * group + sb.i], sb.phase, ab, 78);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
@@ -497,7 +505,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         tc_fence_before();
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster_relaxed(s_leader + sb.i * 8);
+      if (lane == 0) mbar_arrive_cluster_relaxed(s_leader + (2 * group + sb.i) * 8);
+      sb.next(2);
     };
     // Visible keys among the thread's 32 of tile kt.
     auto visible = [&](int kt) -> int {
@@ -575,7 +584,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 mx[s] = next;
               }
             }
-            sb.next(kScores);
           }
         }
         named_bar_sync(1, 32 * kSoftmaxWarps);  // (every score product is over)
@@ -646,10 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 #pragma unroll
         for (int s = 0; s < kMaxMaps; ++s) off[s] += shift;
         for (int j = 0, kt = first; j < nj; ++j, kt = tile_after(kt)) {
-          if ((j & 1) != group) {
-            for (int s = 0; s < maps; ++s) sb.next(kScores);
-            continue;
-          }
+          if ((j & 1) != group) continue;
           const int lim = visible(kt);
           float pm[32];
 #pragma unroll
@@ -657,7 +662,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             if (s >= maps) break;
             float v[32];
             take(v);
-            sb.next(kScores);
             if (!ok) continue;
             hide(v, lim);
 #pragma unroll
@@ -673,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       // ---- one map: weights against a maximum that follows the row.  The offset of tile j + 1 starts from tile j's, which the
       // other group leaves in row_ref.
       const float scale = p.scales[0] * gsc;
-      for (int j = 0, kt = first; j < nj; ++j, kt = tile_after(kt), sb.next(kScores)) {
+      for (int j = 0, kt = first; j < nj; ++j, kt = tile_after(kt)) {
         if ((j & 1) != group) continue;
         float v[32], big = -INFINITY;
         take(v);
@@ -702,7 +706,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         if (any) {  // the outputs so far, once the products into them are done: tile j - 1's
           const float c = rescale ? ex2(ref - next) : 1.f;
           sum *= c;
-          if (ok) ok = mbar_wait(&p_empty[group ^ 1], group ? p_phase ^ 1u : p_phase, ab, 80);
+          // (its buffer's products before those, tile j - 3's, may be under way still: a wait for the later ones alone would
+          // end at once then)
+          const uint32_t done = group ? p_phase ^ 1u : p_phase;
+          if (ok && j >= 3) ok = mbar_wait(&p_empty[group ^ 1], done ^ 1u, ab, 80);
+          if (ok) ok = mbar_wait(&p_empty[group ^ 1], done, ab, 80);
           ok = __all_sync(0xffffffffu, ok);
           if (ok) {
             tc_fence_after();

@@ -10,6 +10,10 @@ element is  eps / 2 (A + |y|) + A (2 H R 2^-24 gamma |q| |k| + 1e-5).
 from __future__ import annotations
 
 import math
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -356,6 +360,27 @@ def test_a_long_cache_past_32_bits_of_elements() -> None:
     bound = 2**-8 * (big + (p @ v.double()).abs()) + big * (2 * r * 2.0**-24 * 16 * 1.02 + 1e-5)
     assert ((y.double() - p @ v.double()).abs() <= bound).all()
     assert ops.device_status() == 0
+
+
+_ALONE = """
+import sys
+sys.path.insert(0, {tests!r})
+from test_gpu_paged import BF16, FP16, Case
+for shape in [(1, 1, 256, 512, 64), (4, 4, 128, 512, 64), (3, 3, 128, 256, 32), (2, 2, 256, 512, 16), (4, 2, 64, 128, 128)]:
+    for held, new in (([4000, 300], [500, 129]), ([0], [640]), ([20000], [65])):
+        case = Case(*shape, FP16, held, new, fill=5.0, seed=16)
+        case.append()
+        for _ in range(3):
+            case.check(case.attend())
+print("alone: ok")
+"""
+
+
+def test_kernels_one_after_another() -> None:
+    """Each kernel alone on the GPU (launches that block), so that none finds its input's producer still running."""
+    done = subprocess.run([sys.executable, "-c", _ALONE.format(tests=str(Path(__file__).parent))], capture_output=True, text=True,
+                          timeout=300, env=os.environ | {"CUDA_LAUNCH_BLOCKING": "1"}, cwd=Path(__file__).parent.parent)
+    assert done.returncode == 0 and "alone: ok" in done.stdout, done.stdout[-2000:] + done.stderr[-2000:]
 
 
 def test_refusals() -> None:
