@@ -348,6 +348,18 @@ DA_DEV void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32
         :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
+// mma_f16_ss from the halves of the descriptors: the low ones move from product to product, the high ones stay.
+template <int kCtaGroup>
+DA_DEV void mma_f16_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t a_hi, uint32_t b_hi, uint32_t idesc,
+                       uint32_t accumulate) {
+  static_assert(kCtaGroup == 2, "paired CTAs");
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %5, p;\n\t}"
+      :: "r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(a_hi), "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+
 // D[tmem] (+)= A[smem] * B[smem]^T, kind::i8 (signed int8 operands, int32 accumulation, K = 32 bytes).
 template <int kCtaGroup>
 DA_DEV void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {

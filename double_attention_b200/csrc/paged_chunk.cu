@@ -92,13 +92,13 @@ struct ChunkParams {
 };
 
 // ------------------------------------------------------------------------------------------------ plan
-constexpr int kPlanThreads = 1024, kLengths = 10, kEnds = 4;
+constexpr int kPlanThreads = 256, kPlanWarps = kPlanThreads / 32, kLengths = 10, kEnds = 6;
 
 // One CTA: a warp a sequence, a tile a lane.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const Plan plan, int few_most, int pairs) {
-  __shared__ int2 kept[kPlanThreads];  // the first sequences' new tokens (of chunks), and tokens that they had
+  __shared__ int2 kept[1024];  // the first sequences' new tokens (of chunks), and tokens that they had
   __shared__ unsigned long long units;
-  __shared__ int counts[kLengths], carry[2], sums[2][32];
+  __shared__ int counts[kLengths], lengths[kLengths], carry[2], sums[2][kPlanWarps], best;
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -107,21 +107,21 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
     return make_int2(s.n > few_most ? s.n : 0, (int)s.held);
   };
   constexpr int nk_shift = 7;  // of kTile
-  if (threadIdx.x < c.B) kept[threadIdx.x] = load(threadIdx.x);
+  for (int b = threadIdx.x; b < c.B && b < 1024; b += kPlanThreads) kept[b] = load(b);
   if (threadIdx.x < kLengths) counts[threadIdx.x] = 0;
   if (threadIdx.x == 0) {
     units = 0;
     carry[0] = carry[1] = 0;
   }
   __syncthreads();
-  auto get = [&](int b) { return b < kPlanThreads ? kept[b] : load(b); };
+  auto get = [&](int b) { return b < 1024 ? kept[b] : load(b); };
   auto tiles_of = [](int2 s) { return (s.x + 127) >> 7; };
   auto keys_of = [&](int2 s, int i) {  // key tiles of query tile i
     const int64_t e = (int64_t)s.y + min(s.x, (i + 1) * 128);
     return (int)(((e < c.capacity ? e : c.capacity) + (1 << nk_shift) - 1) >> nk_shift);
   };
   unsigned long long mine = 0;
-  for (int b = warp; b < c.B; b += kPlanThreads / 32) {
+  for (int b = warp; b < c.B; b += kPlanWarps) {
     const int2 s = get(b);
     for (int i = lane; i < tiles_of(s); i += 32) mine += keys_of(s, i);
   }
@@ -129,25 +129,25 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
   __syncthreads();
   // The pieces' length: of a few that suit one or two rounds of the CTA pairs, the one that is done first, counting a
   // piece's start and end as kEnds key tiles.
-  const int64_t total = (int64_t)units;
-  auto length = [&](int f) {
-    const int64_t round = (int64_t)pairs * (f < 5 ? 1 : 2), base = (total + round - 1) / round;
-    const int64_t more = f % 5 == 0 ? 0 : (base + (16 >> (f % 5 - 1)) - 1) / (16 >> (f % 5 - 1));  // none, a 16th, 8th, 4th, half
-    const int64_t len = base + more;
-    return (int)(len < 1 ? 1 : len);
-  };
-  int len[kLengths], n[kLengths];
-#pragma unroll
-  for (int f = 0; f < kLengths; ++f) {
-    len[f] = length(f);
-    n[f] = 0;
+  if (threadIdx.x < kLengths) {
+    const int f = threadIdx.x, extra = 16 >> (f % 5 - 1 < 0 ? 0 : f % 5 - 1);  // none, a 16th, an 8th, a 4th, half more
+    const int64_t round = (int64_t)pairs * (f < 5 ? 1 : 2), base = ((int64_t)units + round - 1) / round;
+    const int64_t len = base + (f % 5 ? (base + extra - 1) / extra : 0);
+    lengths[f] = (int)(len < 1 ? 1 : len);
   }
-  for (int b = warp; b < c.B; b += kPlanThreads / 32) {
+  __syncthreads();
+  int n[kLengths];
+#pragma unroll
+  for (int f = 0; f < kLengths; ++f) n[f] = 0;
+  for (int b = warp; b < c.B; b += kPlanWarps) {
     const int2 s = get(b);
     for (int i = lane; i < tiles_of(s); i += 32) {
-      const int t = keys_of(s, i);
+      const unsigned t = keys_of(s, i);
 #pragma unroll
-      for (int f = 0; f < kLengths; ++f) n[f] += (unsigned)(t + len[f] - 1) / (unsigned)len[f];
+      for (int f = 0; f < kLengths; ++f) {
+        const unsigned len = lengths[f];
+        n[f] += (t + len - 1) / len;
+      }
     }
   }
 #pragma unroll
@@ -156,18 +156,19 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
     if (lane == 0 && n[f]) atomicAdd(&counts[f], n[f]);
   }
   __syncthreads();
-  int best = 1;
-  int64_t best_cost = INT64_MAX;
-#pragma unroll
-  for (int f = 0; f < kLengths; ++f) {
-    const int64_t cost = (int64_t)((counts[f] + pairs - 1) / pairs) * (len[f] + kEnds);
-    if (cost < best_cost) {
-      best_cost = cost;
-      best = len[f];
+  if (threadIdx.x == 0) {
+    int64_t least = INT64_MAX;
+    for (int f = 0; f < kLengths; ++f) {
+      const int64_t cost = (int64_t)((counts[f] + pairs - 1) / pairs) * (lengths[f] + kEnds);
+      if (cost < least) {
+        least = cost;
+        best = lengths[f];
+      }
     }
   }
-  // tiles and pieces in order: 32 sequences a turn, one a warp
-  for (int base = 0; base < c.B; base += 32) {
+  __syncthreads();
+  // tiles and pieces in order: a warp a sequence, a turn's sequences side by side
+  for (int base = 0; base < c.B; base += kPlanWarps) {
     const int b = base + warp;
     const int2 s = b < c.B ? get(b) : make_int2(0, 0);
     const int tiles = tiles_of(s);
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
       sums[1][warp] = count;
     }
     __syncthreads();
-    const int t = sums[0][lane], k = sums[1][lane];
+    const int t = lane < kPlanWarps ? sums[0][lane] : 0, k = lane < kPlanWarps ? sums[1][lane] : 0;
     int tile0 = carry[0] + __reduce_add_sync(0xffffffffu, lane < warp ? t : 0);
     int piece0 = carry[1] + __reduce_add_sync(0xffffffffu, lane < warp ? k : 0);
     __syncthreads();
@@ -408,31 +409,36 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     // ---------------------------------------------------------------- scores (the pair's leader)
     if (rank == 0 && elect_one()) {
       const uint32_t idesc = idesc_f16(128, kTile, std::is_same<T, __nv_bfloat16>::value, false, false);
-      const uint64_t qd = sdesc_sw128(smem_u32(smem), 16, 1024), kd = sdesc_sw128(smem_u32(smem + L.off_k), 16, 1024);
+      const uint64_t qd = sdesc_sw128(smem_u32(smem), 16, 1024);
+      const uint32_t hi = (uint32_t)(qd >> 32), q_lo = (uint32_t)qd, k_lo = (uint32_t)sdesc_sw128(smem_u32(smem + L.off_k), 16, 1024);
+      const uint32_t d0 = tmem + (uint32_t)(p.D / 2);
+      const int chunks = L.chunks, wide = L.wide, slots = L.kslots;
+      const uint32_t step = (uint32_t)L.k_stage >> 4;
       bool ok = mbar_wait(&q_full, 0, ab, 73);
       tc_fence_after();
-      Turn st{0, 0}, sb0{0, 0}, sb1{0, 0};
+      Turn st{0, 0};
       int unit = 0;
       for (int j = 0; ok && j < nj; ++j) {
-        uint64_t a = qd;
+        uint32_t a = q_lo;
         for (int s = 0; s < maps; ++s, ++unit) {
-          // the group's own two buffers (one that the groups shared would complete phases that a group never waits for, and a
-          // wait for the phase after those would end at once)
-          const int group = (outputs ? j : unit) & 1;
-          Turn& sb = group ? sb1 : sb0;
-          const int buffer = 2 * group + sb.i;
-          if (!(ok = mbar_wait(&s_empty[buffer], sb.phase ^ 1u, ab, 74))) break;
-          sb.next(2);
-          const uint32_t d = tmem + (uint32_t)(p.D / 2 + buffer * 64);
-          for (int c = 0; c < L.chunks; c += L.wide, st.next(L.kslots)) {
+          // a group's units take its own two buffers in turn (one that the groups shared would complete phases that a group
+          // never waits for, and a wait for the phase after those would end at once)
+          const int group = (outputs ? j : unit) & 1, turn = outputs ? (j >> 1) * maps + s : unit >> 1;
+          const int buffer = 2 * group + (turn & 1);
+          if (!(ok = mbar_wait(&s_empty[buffer], ((turn >> 1) & 1u) ^ 1u, ab, 74))) break;
+          const uint32_t d = d0 + (uint32_t)(buffer * 64);
+          for (int c = 0; c < chunks; c += wide, st.next(slots)) {
             if (!(ok = mbar_wait(&k_full[st.i], st.phase, ab, 75))) break;
             tc_fence_after();
-            uint64_t b = kd + (uint64_t)(st.i * (L.k_stage >> 4));
-            for (int e = 0; e < L.wide; ++e, a += kRows * 128 / 16, b += kRows * 128 / 16)
+            uint32_t b = k_lo + (uint32_t)st.i * step;
+            {
+              for (int e = 0; e < wide; ++e, a += kRows * 128 / 16, b += kRows * 128 / 16) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k)  // +32 B per K step of 16 = +2 in the encoded address
-                mma_f16_ss<2>(d, a + 2 * k, b + 2 * k, idesc, (c | e | k) ? 1u : 0u);
-            mma_commit_pair(smem_u32(&k_empty[st.i]));
+                for (int k = 0; k < 4; ++k)  // +32 B per K step of 16 = +2 in the encoded address
+                  mma_f16_lo<2>(d, a + 2 * k, b + 2 * k, hi, hi, idesc, (c | e | k) ? 1u : 0u);
+              }
+              mma_commit_pair(smem_u32(&k_empty[st.i]));
+            }
           }
           if (!ok) break;
           mma_commit_pair(smem_u32(&s_full[buffer]));
@@ -450,25 +456,29 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       const uint64_t pd = sdesc_sw128(smem_u32(smem + L.off_p), 16, 1024);
       // MN-major V: rows are keys (K), 128 B = 64 value columns (N); LBO = distance between 64-column boxes, SBO = 8 key rows
       const uint64_t vd = sdesc_sw128(smem_u32(smem + L.off_v), 64 * 128, 1024);
-      const uint64_t group = (uint64_t)(L.per * (64 * 128) >> 4);
+      const uint32_t p_hi = (uint32_t)(pd >> 32), v_hi = (uint32_t)(vd >> 32);
+      const uint32_t group = (uint32_t)(L.per * (64 * 128) >> 4), step = (uint32_t)L.v_stage >> 4;
+      const uint32_t d1 = tmem + (uint32_t)(L.nc / 2);
+      const bool two = L.npv == 2;
+      const int slots = L.nvs;
       Turn st{0, 0}, pb{0, 0};
       bool ok = true;
-      uint32_t more = 0;
       for (int j = 0; ok && j < nj; ++j, pb.next(kWeights)) {
         if (!(ok = mbar_wait(&p_full[pb.i], pb.phase, ab, 76))) break;
         tc_fence_after();
-        uint64_t a = pd + (uint64_t)(pb.i * (L.p_bytes >> 4));
-        for (int c = 0; c < 2; ++c, a += kRows * 128 / 16, st.next(L.nvs)) {
+        uint32_t a = (uint32_t)pd + (uint32_t)(pb.i * (L.p_bytes >> 4));
+        for (int c = 0; c < 2; ++c, a += kRows * 128 / 16, st.next(slots)) {
           if (!(ok = mbar_wait(&v_full[st.i], st.phase, ab, 77))) break;
           tc_fence_after();
-          const uint64_t b = vd + (uint64_t)(st.i * (L.v_stage >> 4));
+          const uint32_t b = (uint32_t)vd + (uint32_t)st.i * step;
+          {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {  // K step of 16 keys: A +32 B (+2), B +16 rows x 128 B (+128)
-            mma_f16_ss<2>(tmem, a + 2 * k, b + 128 * k, idesc, more);
-            if (L.npv == 2) mma_f16_ss<2>(tmem + (uint32_t)(L.nc / 2), a + 2 * k, b + group + 128 * k, idesc, more);
-            more = 1;
+            for (int k = 0; k < 4; ++k) {  // K step of 16 keys: A +32 B (+2), B +16 rows x 128 B (+128)
+              mma_f16_lo<2>(tmem, a + 2 * k, b + 128 * k, p_hi, v_hi, idesc, (j | c | k) ? 1u : 0u);
+              if (two) mma_f16_lo<2>(d1, a + 2 * k, b + group + 128 * k, p_hi, v_hi, idesc, (j | c | k) ? 1u : 0u);
+            }
+            mma_commit_pair(smem_u32(&v_empty[st.i]));
           }
-          mma_commit_pair(smem_u32(&v_empty[st.i]));
         }
         if (!ok) break;
         mma_commit_pair(smem_u32(&p_empty[pb.i]));
