@@ -168,6 +168,13 @@ DA_DEV bool mbar_wait(uint64_t* bar, uint32_t parity, const Abort& ab, int site 
   }
 }
 
+// mbar_wait for two barriers, their first probes side by side.
+DA_DEV bool mbar_wait2(uint64_t* bar0, uint32_t parity0, uint64_t* bar1, uint32_t parity1, const Abort& ab, int site) {
+  const bool a = mbar_test(smem_u32(bar0), parity0), b = mbar_test(smem_u32(bar1), parity1);
+  if (a && b) return true;
+  return mbar_wait(bar0, parity0, ab, site) && mbar_wait(bar1, parity1, ab, site);
+}
+
 // Like mbar_wait but ignores the abort flag: used while draining in-flight
 // asynchronous work before teardown.  Still bounded by the timeout.
 DA_DEV bool mbar_wait_drain(uint64_t* bar, uint32_t parity) {

@@ -302,6 +302,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
   // (After a wait that gave up every warp still walks all pieces, its waits failing at once: the barriers meet.)
 
   if (warp < kScoreWarps) {
+    // (queries of 512 columns take 128 registers: given by the output warps.  232 + 104, or 192 + 144, are two 168s, what
+    // every warp starts with)
+    if constexpr (kSteps == 32 && kNT < 16) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    if constexpr (kSteps == 32 && kNT == 16) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // ------------------------------------------------------------------ scores and weights of 8 positions a warp
     const int steps = p.H * p.R / 16;
     const float kLog2e = 1.4426950408889634f;
@@ -425,6 +429,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
   }
 
   // ------------------------------------------------------------------ outputs of D / 4 columns a warp
+  if constexpr (kSteps == 32 && kNT < 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+  if constexpr (kSteps == 32 && kNT == 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 144;");
   const int w4 = warp - kScoreWarps, col0 = w4 * (kNT * 8);
   const int kr = lane & 15;  // position of a half tile (a box of 16, or half of one of 32)
   const uint32_t value_off = (col0 >> 6) * block + kr * 128 + (((((col0 & 63) >> 3) | (lane >> 4)) ^ (kr & 7)) << 4);

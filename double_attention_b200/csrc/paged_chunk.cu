@@ -38,6 +38,7 @@ constexpr float kGrow = 8.f;  // log2 of the growth of a row's maximum that its 
 // tensor cores consumes about 2000 cycles' worth: rings of 64 KB and more for keys and values keep them fed.
 struct Shape {
   int rpb, chunks;   // 64-column blocks a branch, and a map
+  int blocks, runs;  // key columns side by side, in blocks (all maps', or a map's), and how many such runs a tile has
   int wide, kslots;  // blocks a key stage, stages
   int nc, npv, per;  // columns a P V product, products, 64-column blocks of one in a CTA
   int q_bytes, k_stage, v_stage, p_bytes, nvs;
@@ -45,23 +46,27 @@ struct Shape {
 };
 
 // outputs: values and weights have room too (else scores alone).
-inline Shape make_shape(int maps, int group, int R, int D, bool outputs) {
+inline Shape make_shape(int maps, int group, int R, int D, bool outputs, bool repeated) {
   Shape s;
   s.rpb = R / 64;
   s.chunks = group * s.rpb;
-  s.wide = s.rpb % 4 == 0 ? 4 : s.rpb % 2 == 0 ? 2 : 1;
+  s.runs = repeated ? maps : 1;  // (maps that repeat a branch read its columns once each)
+  s.blocks = repeated ? s.chunks : maps * s.chunks;
   s.nc = D < 256 ? D : 256;
   s.npv = D / s.nc;
   s.per = s.nc / 128;
   s.q_bytes = kRows * maps * group * R * 2;
-  s.k_stage = s.wide * 64 * 128;
   s.v_stage = 64 * D;  // 64 keys, half of D columns
   s.p_bytes = kRows * kTile * 2;
   const int rings = kSmem - s.q_bytes - (outputs ? kWeights * s.p_bytes : 0);
   // (several maps: one P V for the keys of all of them, so that keys want the room)
-  s.nvs = maps > 1 ? 2 : (rings - 2 * s.k_stage) / s.v_stage;
+  s.nvs = maps > 1 ? 2 : (rings - 65536) / s.v_stage;
   s.nvs = !outputs ? 0 : s.nvs > kMaxV ? kMaxV : s.nvs < 2 ? 2 : s.nvs;
-  s.kslots = (rings - s.nvs * s.v_stage) / s.k_stage;
+  for (s.wide = 4;; s.wide /= 2) {  // wide boxes, but four stages where the units are small
+    s.k_stage = s.wide * 64 * 128;
+    s.kslots = (rings - s.nvs * s.v_stage) / s.k_stage;
+    if (s.blocks % s.wide == 0 && (s.kslots >= (maps > 1 ? 4 : 2) || s.wide == 1)) break;
+  }
   s.kslots = s.kslots > kMaxK ? kMaxK : s.kslots;
   s.off_k = s.q_bytes;
   s.off_v = s.off_k + s.kslots * s.k_stage;
@@ -340,12 +345,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       for (int j = 0, kt = first; ok && j < nj; ++j, kt = tile_after(kt)) {
         const int64_t pos = (int64_t)(here.z + kt) * kTile + (int)rank * 64;
         if (j) slot = slot_of(pos);
-        for (int s = 0; ok && s < maps; ++s)
-          for (int c = 0; c < L.chunks; c += L.wide, st.next(L.kslots), ++used) {
+        for (int s = 0; ok && s < L.runs; ++s)
+          for (int c = 0; c < L.blocks; c += L.wide, st.next(L.kslots), ++used) {
             if (!(ok = mbar_wait(&k_empty[st.i], st.phase ^ 1u, ab, 71))) break;
             if (rank == 0) mbar_arrive_expect_tx(&k_full[st.i], 2 * L.k_stage);
             uint8_t* to = smem + L.off_k + st.i * L.k_stage;
-            const int block = p.branch0[s] * L.rpb + c;  // (a map's branches lie side by side)
+            const int block = p.branch0[s] * L.rpb + c;
             if (whole) {
               tma_load_3d_pair(&tk, kf + st.i * 8, to, 0, slot, block);
             } else {
@@ -417,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       bool ok = mbar_wait(&q_full, 0, ab, 73);
       tc_fence_after();
       Turn st{0, 0};
-      int unit = 0;
+      int unit = 0, in = 0;  // block of the stage
       for (int j = 0; ok && j < nj; ++j) {
         uint32_t a = q_lo;
         for (int s = 0; s < maps; ++s, ++unit) {
@@ -425,19 +430,24 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           // never waits for, and a wait for the phase after those would end at once)
           const int group = (outputs ? j : unit) & 1, turn = outputs ? (j >> 1) * maps + s : unit >> 1;
           const int buffer = 2 * group + (turn & 1);
-          if (!(ok = mbar_wait(&s_empty[buffer], ((turn >> 1) & 1u) ^ 1u, ab, 74))) break;
-          const uint32_t d = d0 + (uint32_t)(buffer * 64);
-          for (int c = 0; c < chunks; c += wide, st.next(slots)) {
-            if (!(ok = mbar_wait(&k_full[st.i], st.phase, ab, 75))) break;
-            tc_fence_after();
-            uint32_t b = k_lo + (uint32_t)st.i * step;
-            {
-              for (int e = 0; e < wide; ++e, a += kRows * 128 / 16, b += kRows * 128 / 16) {
+          const uint32_t d = d0 + (uint32_t)(buffer * 64), parity = ((turn >> 1) & 1u) ^ 1u;
+          if (in == 0) ok = mbar_wait2(&s_empty[buffer], parity, &k_full[st.i], st.phase, ab, 74);
+          else ok = mbar_wait(&s_empty[buffer], parity, ab, 74);
+          if (!ok) break;
+          tc_fence_after();
+          for (int c = 0; c < chunks; ++c, a += kRows * 128 / 16) {
+            if (c && in == 0) {
+              if (!(ok = mbar_wait(&k_full[st.i], st.phase, ab, 75))) break;
+              tc_fence_after();
+            }
+            const uint32_t b = k_lo + (uint32_t)st.i * step + (uint32_t)in * (kRows * 128 / 16);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)  // +32 B per K step of 16 = +2 in the encoded address
-                  mma_f16_lo<2>(d, a + 2 * k, b + 2 * k, hi, hi, idesc, (c | e | k) ? 1u : 0u);
-              }
+            for (int k = 0; k < 4; ++k)  // +32 B per K step of 16 = +2 in the encoded address
+              mma_f16_lo<2>(d, a + 2 * k, b + 2 * k, hi, hi, idesc, (c | k) ? 1u : 0u);
+            if (++in == wide) {
               mma_commit_pair(smem_u32(&k_empty[st.i]));
+              st.next(slots);
+              in = 0;
             }
           }
           if (!ok) break;
@@ -930,24 +940,25 @@ int run(const ChunkArgs& a, cudaStream_t st) {
   p.status = a.status;
   const bool mix = a.maps > 1 && !a.per_map;
   p.maps = mix ? a.maps : 1;
-  p.shape = make_shape(p.maps, a.group, a.R, a.D, true);
+  const bool repeated = p.maps > a.H;
+  p.shape = make_shape(p.maps, a.group, a.R, a.D, true, repeated);
   const Shape L = p.shape;
   if (L.kslots < 2 || !L.tmem_cols) return DA_ERR_UNSUPPORTED;
   p.brow = a.c.page < 64 ? a.c.page : 64;
   const bool whole = p.brow == 64;
   const CUtensorMapDataType dt = a.dtype == DA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap tq, tk, tv;
+  auto map_keys = [&](int wide) {  // (column in its block, slot, block)
+    const uint64_t dims[3] = {64, (uint64_t)a.c.pages * a.c.page, (uint64_t)a.H * a.R / 64};
+    const uint64_t strides[2] = {(uint64_t)a.H * a.R * 2, 128};
+    const uint32_t box[3] = {64, (uint32_t)p.brow, (uint32_t)(whole ? wide : 1)};
+    return make_tmap_blocks(&tk, a.key_pages, dt, 2, 3, dims, strides, box);
+  };
   {  // queries: (column in its block of 64, row, branch, block)
     const uint64_t dims[4] = {64, (uint64_t)a.c.tokens, (uint64_t)a.H, (uint64_t)a.R / 64};
     const uint64_t strides[3] = {(uint64_t)a.q_row * 2, a.H > 1 ? (uint64_t)a.q_branch * 2 : 16, 128};
     const uint32_t box[4] = {64, (uint32_t)kRows, 1, 1};
     if (int rc = make_tmap_blocks(&tq, a.q, dt, 2, 4, dims, strides, box)) return rc;
-  }
-  {  // keys: (column in its block, slot, block)
-    const uint64_t dims[3] = {64, (uint64_t)a.c.pages * a.c.page, (uint64_t)a.H * a.R / 64};
-    const uint64_t strides[2] = {(uint64_t)a.H * a.R * 2, 128};
-    const uint32_t box[3] = {64, (uint32_t)p.brow, (uint32_t)(whole ? L.wide : 1)};
-    if (int rc = make_tmap_blocks(&tk, a.key_pages, dt, 2, 3, dims, strides, box)) return rc;
   }
   {  // values: (column in its block, slot, block inside an nc-wide group, group)
     const uint64_t dims[4] = {64, (uint64_t)a.c.pages * a.c.page, (uint64_t)L.nc / 64, (uint64_t)a.D / L.nc};
@@ -972,13 +983,16 @@ int run(const ChunkArgs& a, cudaStream_t st) {
     p.phase = 0;
     if (mix) {
       p.phase = 1;
-      p.shape = make_shape(p.maps, a.group, a.R, a.D, false);
+      p.shape = make_shape(p.maps, a.group, a.R, a.D, false, repeated);
+      if (int rc = map_keys(p.shape.wide)) return rc;
       if (int rc = launch_kernel(chunk_kernel<T, true>, grid, block, p.shape.smem, st, true, tq, tk, tv, p)) return rc;
       p.phase = 2;
       p.shape = L;
+      if (int rc = map_keys(L.wide)) return rc;
       if (int rc = launch_kernel(chunk_kernel<T, true>, grid, block, L.smem, st, true, tq, tk, tv, p)) return rc;
-    } else if (int rc = launch_kernel(chunk_kernel<T, false>, grid, block, L.smem, st, true, tq, tk, tv, p)) {
-      return rc;
+    } else {
+      if (int rc = map_keys(L.wide)) return rc;
+      if (int rc = launch_kernel(chunk_kernel<T, false>, grid, block, L.smem, st, true, tq, tk, tv, p)) return rc;
     }
     if (int rc = launch_kernel(join_kernel<T>, dim3((unsigned)tiles, (unsigned)(16 * a.D / 128)), dim3(256), 0, st, false, p, !mix)) return rc;
   }
