@@ -56,6 +56,12 @@ DA_DEV int64_t sequence_tiles(const FewParams& p, const Sequence& s, int b) {
   return (int64_t)((s.n + tokens - 1) / tokens) * job_tiles(p.c, s);
 }
 
+// Tiles a CTA of `ctas`.
+DA_DEV int64_t share_of(int64_t total, int ctas) {
+  if (total < 0x7fff0000) return ((uint32_t)total + (uint32_t)ctas - 1) / (uint32_t)ctas;
+  return (total + ctas - 1) / ctas;
+}
+
 // Sum over `threads` threads' values (all of them call it; every one gets it).  `buf` holds 32 entries.
 template <int threads>
 DA_DEV int64_t block_sum(int64_t v, int64_t* buf) {
@@ -100,6 +106,8 @@ DA_DEV void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
 struct Walk {
   int b;
   int64_t off, left;  // tile of sequence b's list, tiles still to do
+  Sequence s;         // sequence b, if known
+  bool known;
 };
 
 struct Piece {
@@ -110,12 +118,14 @@ struct Piece {
 
 DA_DEV bool next_piece(const FewParams& p, Walk& w, Piece& x) {
   while (w.left > 0 && w.b < p.c.B) {
-    x.s = sequence(p.c, w.b);
+    if (!w.known) w.s = sequence(p.c, w.b);
+    w.known = true;
+    x.s = w.s;
     const int64_t all = sequence_tiles(p, x.s, w.b);
     if (w.off < all) {
       x.b = w.b;
       x.tiles = job_tiles(p.c, x.s);
-      x.job = (int)(w.off / x.tiles);
+      x.job = w.off < 0x7fffffff ? (int)((uint32_t)w.off / (uint32_t)x.tiles) : (int)(w.off / x.tiles);
       x.t0 = (int)(w.off - (int64_t)x.job * x.tiles);
       x.t1 = (int)(x.t0 + w.left < x.tiles ? x.t0 + w.left : x.tiles);
       w.left -= x.t1 - x.t0;
@@ -124,6 +134,7 @@ DA_DEV bool next_piece(const FewParams& p, Walk& w, Piece& x) {
     }
     ++w.b;
     w.off = 0;
+    w.known = false;
   }
   return false;
 }
@@ -148,6 +159,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
   __shared__ __align__(16) float warp_max[2][16][kScoreWarps];
   __shared__ float rescale[2][16], row_max[16], row_sum[kScoreWarps][16];
   __shared__ int64_t buf[32], start_off;
+  __shared__ Sequence start_seq;
   __shared__ int start_b, abort_flag, piece_bad;
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -169,15 +181,23 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
   // ---- this CTA's share of the flat list of tiles
   const int64_t used = p.zero_rest ? clamp64(p.c.starts[p.c.B], 0, p.c.tokens) : p.c.tokens;
   int64_t total = 0;
-  for (int b = tid; b < p.c.B; b += kThreads) total += sequence_tiles(p, sequence(p.c, b), b);
+  Sequence own{0, 0, 0, true};
+  for (int b = tid; b < p.c.B; b += kThreads) {
+    own = sequence(p.c, b);
+    total += sequence_tiles(p, own, b);
+  }
   const bool short_list = p.c.B <= kThreads;  // then `total` is still the thread's own sequence's, scanned below
   if (!short_list) total = block_sum<kThreads>(total, buf);
-  int64_t share = (total + p.ctas - 1) / p.ctas, begin = (int64_t)blockIdx.x * share;
+  int64_t share = share_of(total, p.ctas), begin = (int64_t)blockIdx.x * share;
   if (short_list || begin < total) {
     int64_t before = 0;  // tiles of the sequences before this round's
     for (int base = 0;; base += kThreads) {
       const int b = base + tid;
-      const int64_t v = short_list ? total : b < p.c.B ? sequence_tiles(p, sequence(p.c, b), b) : 0;
+      int64_t v = total;
+      if (!short_list) {
+        if (b < p.c.B) own = sequence(p.c, b);
+        v = b < p.c.B ? sequence_tiles(p, own, b) : 0;
+      }
       int64_t inc = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -195,12 +215,13 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
       }
       if (short_list) {
         total = all;
-        share = (total + p.ctas - 1) / p.ctas;
+        share = share_of(total, p.ctas);
         begin = (int64_t)blockIdx.x * share;
       }
       if (begin >= at && begin < at + v) {
         start_b = b;
         start_off = begin - at;
+        start_seq = own;
       }
       before += all;
       if (short_list || begin < before) break;  // (total > begin: found at the latest with the last sequence)
@@ -214,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
       rest[i] = make_uint4(0, 0, 0, 0);
   }
   if (begin >= total) return;
-  Walk walk{start_b, start_off, share < total - begin ? share : total - begin};
+  Walk walk{start_b, start_off, share < total - begin ? share : total - begin, start_seq, true};
   Abort ab{&abort_flag, p.status};
   const int tokens = 16 / p.lanes;
   Piece x;
@@ -311,6 +332,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
     const float kLog2e = 1.4426950408889634f;
     const float scale0 = s0 < p.maps ? p.scales[s0] * rsqrtf((float)p.group) * kLog2e : 0.f;
     const float scale1 = s1 < p.maps ? p.scales[s1] * rsqrtf((float)p.group) * kLog2e : 0.f;
+    const uint32_t queries = smem_u32(smem + p.stages * p.stage_bytes);
     const int key = warp * 8 + (lane & 7), kr = p.brow == 32 ? key : key & 15;
     const uint32_t key_off = (p.brow == 32 ? 0 : (key >> 4) * key_box) + kr * 128 + (((lane >> 3) ^ (kr & 7)) << 4);
     while (next_piece(p, walk, x)) {
@@ -321,21 +343,22 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
       const bool on0 = s0 < p.maps && k0 < live, on1 = s1 < p.maps && k1 < live;
       const int64_t sees0 = on0 ? min(x.s.held + x.job * tokens + k0 + 1, end) : 0;
       const int64_t sees1 = on1 ? min(x.s.held + x.job * tokens + k1 + 1, end) : 0;
+      // the job's rows, each with its map's branches and zeros elsewhere, by way of shared memory
+      const int row_chunks = p.H * p.R / 8;
+      for (int i = tid; i < 16 * row_chunks; i += 32 * kScoreWarps) {
+        const int row = i / row_chunks, c = i - row * row_chunks, h = c * 8 / p.R, s = row >> map_shift, k = row & token_of;
+        const int h0 = p.H >= p.maps ? s * p.group : s * p.H / p.maps;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (s < p.maps && k < live && h >= h0 && h < h0 + p.group)
+          w = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + h * p.q_branch + (q0 + k) * p.q_row + (c * 8 - h * p.R));
+        st_shared_v4(queries + (c >> 3) * 2048 + sw128_offset(row, c & 7), w.x, w.y, w.z, w.w);
+      }
+      named_bar_sync(1, 32 * kScoreWarps);
       uint32_t qf[kSteps][4];
-      {
-        const int h0 = p.H >= p.maps ? s0 * p.group : s0 * p.H / p.maps, h1 = p.H >= p.maps ? s1 * p.group : s1 * p.H / p.maps;
-        const T* q = static_cast<const T*>(p.q);
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const int h = i * 16 / p.R;  // (a step lies in one branch)
-          const int64_t at = h * p.q_branch + (i * 16 - h * p.R) + pair;
-          const bool in0 = on0 && i < steps && h >= h0 && h < h0 + p.group, in1 = on1 && i < steps && h >= h1 && h < h1 + p.group;
-          const T *r0 = q + at + (q0 + k0) * p.q_row, *r1 = q + at + (q0 + k1) * p.q_row;
-          qf[i][0] = in0 ? *reinterpret_cast<const uint32_t*>(r0) : 0;
-          qf[i][1] = in1 ? *reinterpret_cast<const uint32_t*>(r1) : 0;
-          qf[i][2] = in0 ? *reinterpret_cast<const uint32_t*>(r0 + 8) : 0;
-          qf[i][3] = in1 ? *reinterpret_cast<const uint32_t*>(r1 + 8) : 0;
-        }
+      for (int i = 0; i < kSteps; ++i) {
+        if (i < steps) ldmatrix4(qf[i], queries + (i >> 2) * 2048 + sw128_offset(lane & 15, (i & 3) * 2 + (lane >> 4)));
+        else qf[i][0] = qf[i][1] = qf[i][2] = qf[i][3] = 0;
       }
       float ref0 = -INFINITY, ref1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // rows g and g + 8: offsets, this thread's sums
       bool wrong = !x.s.fits, ok = true;
@@ -672,7 +695,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const FewParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
   if (!mine) return;
-  const int64_t share = (total + p.ctas - 1) / p.ctas;
+  const int64_t share = share_of(total, p.ctas);
   const int tokens = 16 / p.lanes, tiles = job_tiles(p.c, s);
   for (int i = blockIdx.x % p.few_rows; i < s.n; i += p.few_rows) {
     const int64_t f0 = ahead + (int64_t)(i / tokens) * tiles, f1 = f0 + tiles;
@@ -702,9 +725,9 @@ FewPlan few_plan(int64_t tokens, int64_t B, int64_t capacity, int64_t max_new, i
   f.key_bytes = paged::kKeys * 2 * wide;
   f.stage_bytes = f.key_bytes + paged::kKeys * 2 * D;
   const int per_sm = ctas_per_sm(wide, D);
-  f.stages = (227 * 1024 / per_sm - 1024 - 6 * 1024) / f.stage_bytes;  // (a CTA's own 1 KB, fixed buffers, alignment)
+  f.stages = (227 * 1024 / per_sm - 1024 - 6 * 1024 - 32 * wide) / f.stage_bytes;  // (a CTA's own 1 KB, fixed buffers, alignment, queries)
   if (f.stages > paged::kMaxStages) f.stages = paged::kMaxStages;
-  f.smem = f.stages * f.stage_bytes + 1024;
+  f.smem = f.stages * f.stage_bytes + 32 * wide + 1024;
   const int64_t rows = 16 / lanes, jobs = tokens / rows + B < tokens ? tokens / rows + B : tokens;
   const int64_t tiles = (capacity + paged::kKeys - 1) / paged::kKeys;
   const int64_t most = (int64_t)sm_count() * per_sm, need = jobs * (tiles > 0 ? tiles : 1);
