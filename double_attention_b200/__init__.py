@@ -35,7 +35,7 @@ from .modules import (
     SharedDictionaryBank,
 )
 from .ops import assemble_score_maps, dictionary_route, routed_attention
-from .paged import PagedBatch, append_paged, routed_attention_paged
+from .paged import PagedBatch, RoutedCache, append_paged, routed_attention_paged
 from .scoring import TokenLogProbs, token_log_probs
 
 __all__ = [
@@ -50,6 +50,7 @@ __all__ = [
     "Int8Linear",
     "Int8Rows",
     "PagedBatch",
+    "RoutedCache",
     "SharedDictionaryAttention",
     "SharedDictionaryBank",
     "TokenLogProbs",

@@ -15,13 +15,15 @@ tokens in 1.44 ms (2.39), replayed from a CUDA graph 1.34 (1.62); 64 x 1024 4.65
 from __future__ import annotations
 
 import copy
+from typing import Sequence
 
 import torch
 from torch import Tensor, nn
 
-from . import ops
+from . import ops, paged
 from .eight_bit import Int8Rows, add_layernorm_int8, int8_linear, layernorm_int8, own_forward, quantize_int8
 from .modules import DoubleAttentionBlock, DoubleAttentionLM
+from .scoring import TokenLogProbs, token_log_probs
 
 _HALF = (torch.float16, torch.bfloat16)
 _ATTENTION_ROWS = 128  # rows (batch times length) below which the attention kernels have no tile
@@ -101,10 +103,16 @@ class _Int8Block(nn.Module):
         logits = attention.map_mix_logits
         self.register_buffer("map_weights", None if logits is None else torch.softmax(logits.float(), dim=0))
 
-    def attend(self, rows: Int8Rows, views: ops.DictionaryViews) -> Tensor:
+    def attend(self, rows: Int8Rows, views: ops.DictionaryViews,
+               cache: tuple[Tensor, Tensor, paged.PagedBatch] | None = None) -> Tensor:
         cfg = self.config
         batch, tokens = rows.scale.shape
         projected, value = self.query_key(rows), self.value(rows)
+        if cache is not None:
+            routed = ops.route_projected(projected.view(tokens, -1), views, self.beta, cfg, 1, tokens)
+            weights = self.map_weights if cfg.map_combine == "weighted_sum" else None
+            combined = paged.extend(routed, value, cache, self.scales, weights).view(1, tokens, -1)
+            return combined if self.output is None else self.output(combined)
         length = tokens
         if cfg.causal and batch * tokens < _ATTENTION_ROWS:
             # positions after the last one, which no query sees, fill the attention's smallest tile
@@ -119,13 +127,14 @@ class _Int8Block(nn.Module):
         combined = combined[:, :tokens]
         return combined if self.output is None else self.output(combined)
 
-    def forward(self, x: Tensor, pending: Tensor | None, views: ops.DictionaryViews) -> tuple[Tensor, Tensor]:
+    def forward(self, x: Tensor, pending: Tensor | None, views: ops.DictionaryViews,
+                cache: tuple[Tensor, Tensor, paged.PagedBatch] | None = None) -> tuple[Tensor, Tensor]:
         """``x + pending`` through the block; returns the residual and the feed-forward branch still to be added."""
         if pending is None:
             rows = layernorm_int8(x, self.attention_norm)
         else:
             x, rows = add_layernorm_int8(x, pending, self.attention_norm)
-        x, rows = add_layernorm_int8(x, self.attend(rows, views), self.feedforward_norm)
+        x, rows = add_layernorm_int8(x, self.attend(rows, views, cache), self.feedforward_norm)
         return x, self.second(self.first(rows, gelu=True))
 
 
@@ -164,9 +173,37 @@ class Int8DoubleAttentionLM(_FixedTypes):
         if not token_ids.numel():
             return self.token_embedding.weight.new_empty(*token_ids.shape, self.lm_head.weight.shape[0], dtype=self.lm_head.dtype)
         positions = torch.arange(length, device=token_ids.device)
-        x = (self.token_embedding(token_ids) + self.position_embedding(positions)[None]).float()
+        return self._logits((self.token_embedding(token_ids) + self.position_embedding(positions)[None]).float())
+
+    def _logits(self, x: Tensor, cache: paged.RoutedCache | None = None, batch: paged.PagedBatch | None = None) -> Tensor:
         views = [bank.views() for bank in self.banks]
         pending = None
-        for block, bank in zip(self.blocks, self._bank_of):
-            x, pending = block(x, pending, views[bank])
+        for index, (block, bank) in enumerate(zip(self.blocks, self._bank_of)):
+            x, pending = block(x, pending, views[bank], None if cache is None else (*cache.layer(index), batch))
         return self.lm_head(add_layernorm_int8(x, pending, self.final_norm)[1])
+
+    def new_cache(self, sequences: int, max_length: int | None = None, *, page_size: int = 64,
+                  pages: int | None = None) -> paged.RoutedCache:
+        """An empty cache for :meth:`extend`."""
+        return paged.RoutedCache(self.blocks[0].config, len(self.blocks), sequences, max_length or self.max_sequence_length,
+                                 page_size=page_size, pages=pages, dtype=self.lm_head.dtype, device=self.lm_head.weight.device)
+
+    @torch.no_grad()
+    def extend(self, token_ids: Tensor, cache: paged.RoutedCache, counts: Sequence[int] | None = None) -> Tensor:
+        """Logits of new tokens behind those in ``cache``, which takes them in: as ``DoubleAttentionLM.extend``."""
+        ids, numbers = cache.rows(token_ids, counts, self.max_sequence_length)
+        batch = cache.step(numbers)
+        if not ids.numel():
+            return self.token_embedding.weight.new_empty(*token_ids.shape, self.lm_head.weight.shape[0], dtype=self.lm_head.dtype)
+        positions = cache.positions(batch, numbers, self.max_sequence_length)
+        logits = self._logits((self.token_embedding(ids) + self.position_embedding(positions)).float()[None], cache, batch)
+        cache.advance(numbers, batch)
+        return logits.view(*token_ids.shape, -1)
+
+    @torch.no_grad()
+    def score(self, token_ids: Tensor, *, top: int = 0) -> TokenLogProbs:
+        """Log probabilities of ``token_ids`` [B, T] from the second on, each under the tokens before it, with the entropy
+        of its distribution and its ``top`` likeliest tokens: [B, T - 1]."""
+        if token_ids.ndim != 2 or token_ids.shape[1] < 2:
+            raise ValueError("token_ids must have shape [B, T] with T at least 2")
+        return token_log_probs(self(token_ids[:, :-1]), token_ids[:, 1:], top=top)

@@ -14,13 +14,15 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from typing import Sequence
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
-from . import eight_bit, ops
+from . import eight_bit, ops, paged
+from .scoring import TokenLogProbs, token_log_probs
 from .config import DoubleAttentionConfig
 
 # The reference exposes this switch to compare fused and separate Q/K
@@ -145,10 +147,15 @@ class SharedDictionaryAttention(nn.Module):
         bank: SharedDictionaryBank | None = None,
         normalized_dictionary: tuple[Tensor, Tensor] | None = None,
         return_aux: bool = False,
+        cache: tuple[Tensor, Tensor, paged.PagedBatch] | None = None,
     ) -> Tensor | tuple[Tensor, DoubleAttentionAux]:
+        """``cache``: key pages, value pages and the step's batch; x then holds the packed new tokens [1, N, dim], whose
+        keys and values go into the pages and which attend over them (inference only)."""
         cfg = self.config
         if x.ndim != 3 or x.shape[-1] != cfg.model_dim:
             raise ValueError(f"expected x with shape [B, T, {cfg.model_dim}], got {tuple(x.shape)}")
+        if cache is not None and (return_aux or not cfg.causal or x.shape[0] != 1):
+            raise ValueError("a cache takes the packed new tokens [1, N, dim] of a causal attention, without return_aux")
         active_bank = bank if bank is not None else self.bank
         if active_bank is None:
             raise ValueError("no dictionary bank supplied")
@@ -186,15 +193,21 @@ class SharedDictionaryAttention(nn.Module):
             map_weights = None
 
         if cfg.map_combine == "weighted_sum":
-            combined = ops.routed_attention_mixed(routed, dense_value, score_scales, map_weights, cfg)
+            if cache is not None:
+                combined = paged.extend(routed, dense_value, cache, score_scales, map_weights)[None]
+            else:
+                combined = ops.routed_attention_mixed(routed, dense_value, score_scales, map_weights, cfg)
             if (ops.BLOCK_LINEAR_ON_TCGEN05 and isinstance(self.output, nn.Linear)
                     and ops.linear_supported(combined, self.output)):
                 output = ops.linear(combined, self.output)  # the output projection on the tcgen05 GEMM
             else:
                 output = self.output(combined.to(self._output_dtype(combined)))
         else:
-            per_map = ops.routed_attention_maps(routed, dense_value, score_scales, cfg)  # [B,S,T,D]
-            output = self.output(per_map.permute(0, 2, 1, 3).flatten(2))
+            if cache is not None:
+                per_map = paged.extend(routed, dense_value, cache, score_scales, None).view(1, x.shape[1], cfg.outer_maps, -1)
+            else:
+                per_map = ops.routed_attention_maps(routed, dense_value, score_scales, cfg).permute(0, 2, 1, 3)  # [B,T,S,D]
+            output = self.output(per_map.flatten(2))
 
         if not return_aux:
             return output
@@ -246,15 +259,18 @@ class DoubleAttentionBlock(nn.Module):
                                              nn.Linear(feedforward_dim, config.model_dim), nn.Dropout(dropout))
 
     def forward(self, x: Tensor, bank: SharedDictionaryBank, *,
-                normalized_dictionary: tuple[Tensor, Tensor] | None = None) -> Tensor:
+                normalized_dictionary: tuple[Tensor, Tensor] | None = None,
+                cache: tuple[Tensor, Tensor, paged.PagedBatch] | None = None) -> Tensor:
         if ops.layernorm_supported(x, self.attention_norm, self.feedforward_norm):
-            x, branch = self._forward_fused(x, None, bank, normalized_dictionary)
+            x, branch = self._forward_fused(x, None, bank, normalized_dictionary, cache)
             return x + branch
-        x = x + self.attention(self.attention_norm(x), bank=bank, normalized_dictionary=normalized_dictionary)
+        x = x + self.attention(self.attention_norm(x), bank=bank, normalized_dictionary=normalized_dictionary,
+                               **({} if cache is None else {"cache": cache}))
         return x + self._feedforward_branch(self.feedforward_norm(x), bank, normalized_dictionary)
 
     def _forward_fused(self, x: Tensor, pending: Tensor | None, bank: SharedDictionaryBank,
-                       normalized_dictionary: tuple[Tensor, Tensor] | None) -> tuple[Tensor, Tensor]:
+                       normalized_dictionary: tuple[Tensor, Tensor] | None,
+                       cache: tuple[Tensor, Tensor, paged.PagedBatch] | None = None) -> tuple[Tensor, Tensor]:
         """The block on the fp32 residual stream with fused norms: ``x + pending`` (the previous block's
         feed-forward branch, not yet added) is normalised by the same kernel that adds it; returns the
         residual after the attention branch and this block's feed-forward branch, still to be added."""
@@ -262,7 +278,8 @@ class DoubleAttentionBlock(nn.Module):
             normalized_x = ops.layernorm(x, self.attention_norm)
         else:
             x, normalized_x = ops.add_layernorm(x, pending, self.attention_norm)
-        branch = self.attention(normalized_x, bank=bank, normalized_dictionary=normalized_dictionary)
+        branch = self.attention(normalized_x, bank=bank, normalized_dictionary=normalized_dictionary,
+                                **({} if cache is None else {"cache": cache}))
         x, normalized_x = ops.add_layernorm(x, branch, self.feedforward_norm)
         return x, self._feedforward_branch(normalized_x, bank, normalized_dictionary)
 
@@ -323,18 +340,22 @@ class DoubleAttentionStack(nn.Module):
         x, pending = self._forward_pending(x)
         return x if pending is None else x + pending
 
-    def _forward_pending(self, x: Tensor) -> tuple[Tensor, Tensor | None]:
+    def _forward_pending(self, x: Tensor, cache: paged.RoutedCache | None = None,
+                         batch: paged.PagedBatch | None = None) -> tuple[Tensor, Tensor | None]:
         """Runs the blocks; with the fused norms the last block's feed-forward branch is returned
-        unadded (``pending``), so that a following norm can add it in its own kernel."""
+        unadded (``pending``), so that a following norm can add it in its own kernel.  With a cache, x holds the packed
+        new tokens [1, N, dim] of ``batch``."""
         normalized = tuple(bank.normalized(self.config.eps) for bank in self.banks)
         fused = all(ops.layernorm_supported(x, b.attention_norm, b.feedforward_norm) for b in self.blocks)
         pending = None
         for index, block in enumerate(self.blocks):
             bank_index = min(index // self.dictionary_group_size, len(self.banks) - 1)
+            pages = None if cache is None else (*cache.layer(index), batch)
             if fused:
-                x, pending = block._forward_fused(x, pending, self.banks[bank_index], normalized[bank_index])
+                x, pending = block._forward_fused(x, pending, self.banks[bank_index], normalized[bank_index], pages)
             else:
-                x = block(x, self.banks[bank_index], normalized_dictionary=normalized[bank_index])
+                x = block(x, self.banks[bank_index], normalized_dictionary=normalized[bank_index],
+                          **({} if pages is None else {"cache": pages}))
         return x, pending
 
 
@@ -361,20 +382,49 @@ class DoubleAttentionLM(nn.Module):
         if length > self.max_sequence_length:
             raise ValueError(f"sequence length {length} exceeds configured maximum {self.max_sequence_length}")
         positions = torch.arange(length, device=token_ids.device)
-        hidden, pending = self.stack._forward_pending(
-            self.token_embedding(token_ids) + self.position_embedding(positions)[None])
-        if pending is not None and ops.layernorm_supported(hidden, self.final_norm):
-            logits = self.lm_head(ops.add_layernorm(hidden, pending, self.final_norm)[1])
-        else:
-            if pending is not None:
-                hidden = hidden + pending
-            if ops.layernorm_supported(hidden, self.final_norm):
-                logits = self.lm_head(ops.layernorm(hidden, self.final_norm))
-            else:
-                logits = self.lm_head(self.final_norm(hidden))
+        logits = self._head(*self.stack._forward_pending(
+            self.token_embedding(token_ids) + self.position_embedding(positions)[None]))
         loss = None
         if targets is not None:
             if targets.shape != token_ids.shape:
                 raise ValueError("targets must match token_ids shape")
             loss = F.cross_entropy(logits.flatten(0, 1), targets.flatten())
         return logits, loss
+
+    def _head(self, hidden: Tensor, pending: Tensor | None) -> Tensor:
+        if pending is not None and ops.layernorm_supported(hidden, self.final_norm):
+            return self.lm_head(ops.add_layernorm(hidden, pending, self.final_norm)[1])
+        if pending is not None:
+            hidden = hidden + pending
+        if ops.layernorm_supported(hidden, self.final_norm):
+            return self.lm_head(ops.layernorm(hidden, self.final_norm))
+        return self.lm_head(self.final_norm(hidden))
+
+    def new_cache(self, sequences: int, max_length: int | None = None, *, page_size: int = 64, pages: int | None = None,
+                  dtype: torch.dtype = torch.bfloat16) -> paged.RoutedCache:
+        """An empty cache for :meth:`extend`; ``dtype`` is the type that the attention computes in (autocast's, or the
+        parameters')."""
+        return paged.RoutedCache(self.stack.config, self.stack.num_layers, sequences, max_length or self.max_sequence_length,
+                                 page_size=page_size, pages=pages, dtype=dtype, device=self.token_embedding.weight.device)
+
+    @torch.no_grad()
+    def extend(self, token_ids: Tensor, cache: paged.RoutedCache, counts: Sequence[int] | None = None) -> Tensor:
+        """Logits of new tokens behind those in ``cache``, which takes them in.
+
+        ``token_ids`` [B, T], T new tokens of every sequence of the cache, or [N] with ``counts``, packed one sequence after
+        another: logits [B, T, V] or [N, V].  What :meth:`forward` gives for the whole sequences, up to rounding."""
+        ids, numbers = cache.rows(token_ids, counts, self.max_sequence_length)
+        batch = cache.step(numbers)
+        if not ids.numel():
+            return self.lm_head.weight.new_empty(*token_ids.shape, self.lm_head.out_features)
+        x = self.token_embedding(ids) + self.position_embedding(cache.positions(batch, numbers, self.max_sequence_length))
+        logits = self._head(*self.stack._forward_pending(x[None], cache, batch))
+        cache.advance(numbers, batch)
+        return logits.view(*token_ids.shape, -1)
+
+    def score(self, token_ids: Tensor, *, top: int = 0) -> TokenLogProbs:
+        """Log probabilities of ``token_ids`` [B, T] from the second on, each under the tokens before it, with the entropy
+        of its distribution and its ``top`` likeliest tokens: [B, T - 1].  Differentiable (see :func:`token_log_probs`)."""
+        if token_ids.ndim != 2 or token_ids.shape[1] < 2:
+            raise ValueError("token_ids must have shape [B, T] with T at least 2")
+        return token_log_probs(self(token_ids[:, :-1])[0], token_ids[:, 1:], top=top)

@@ -181,3 +181,126 @@ def routed_attention_paged(query: Tensor, key_pages: Tensor, value_pages: Tensor
             scales.data_ptr(), ptr(weights), int(per_map), int(out is None), y.data_ptr(), ptr(work), max(need, 0),
             ops.workspace(query.device).status.data_ptr())
     return y
+
+
+def extend(routed: Tensor, value: Tensor, cache: tuple[Tensor, Tensor, PagedBatch], scales: Tensor,
+           map_weights: Tensor | None) -> Tensor:
+    """Module path: routed [2, H, 1, N, R] and value [1, N, D] of packed new tokens into the pages, and their attention over
+    them."""
+    key_pages, value_pages, batch = cache
+    if routed.dtype != key_pages.dtype:
+        raise ValueError(f"the attention computes in {routed.dtype}, the cache holds {key_pages.dtype}")
+    append_paged(routed[1, :, 0], value[0], key_pages, value_pages, batch)
+    return routed_attention_paged(routed[0, :, 0], key_pages, value_pages, batch, scales, map_weights)
+
+
+class RoutedCache:
+    """The pages of all layers of a model for ``sequences`` sequences, and who has which.
+
+    ``max_length`` positions a sequence.  Without ``pages`` every sequence owns its pages from the start, and a step
+    (``DoubleAttentionLM.extend``, ``Int8DoubleAttentionLM.extend``) can be captured into a CUDA graph: the device's
+    ``lengths`` advance with every replay.  With fewer ``pages`` sequences share a pool: a step takes what its new tokens
+    need and raises if there is none left; ``release`` gives a sequence's pages back.  Not for several threads at once."""
+
+    def __init__(self, config, layers: int, sequences: int, max_length: int, *, page_size: int = 64, pages: int | None = None,
+                 dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda") -> None:
+        if not config.causal:
+            raise ValueError("a cache serves causal attention: later tokens change nothing of earlier ones")
+        if dtype not in _HALF:
+            raise ValueError(f"a cache holds bfloat16 or float16, got {dtype}")
+        if layers < 1 or sequences < 1 or max_length < 1:
+            raise ValueError(f"a cache has at least one layer, sequence and position, got {layers}, {sequences} and {max_length}")
+        if page_size < 16 or page_size > 65536 or page_size & (page_size - 1):
+            raise ValueError(f"pages have 16 to 65536 positions, a power of two, got {page_size}")
+        columns = -(-max_length // page_size)
+        own = pages is None
+        pages = sequences * columns if own else pages
+        if pages < 1:
+            raise ValueError(f"a cache has at least one page, got {pages}")
+        self.page_size, self.max_length, self.sequences, self.layers, self.dtype = page_size, max_length, sequences, layers, dtype
+        shape = (config.qk_branches, config.routing_dim)
+        # (zeros: a chunk over slots that hold NaN is computed twice)
+        self.key_pages = torch.zeros(layers, pages, page_size, *shape, dtype=dtype, device=device)
+        self.value_pages = torch.zeros(layers, pages, page_size, config.model_dim, dtype=dtype, device=device)
+        self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
+        self.table = torch.zeros(sequences, columns, dtype=torch.int32, device=device)
+        self._owned: list[list[int]] = [[] for _ in range(sequences)]
+        self._free = list(range(pages - 1, -1, -1))
+        self._held = [0] * sequences  # the lengths as the host knows them
+        if own:
+            self.table.copy_(torch.arange(pages, dtype=torch.int32).view(sequences, columns))
+            self._owned = [list(range(b * columns, (b + 1) * columns)) for b in range(sequences)]
+            self._free = []
+        self._fixed = own
+
+    def layer(self, index: int) -> tuple[Tensor, Tensor]:
+        """Key and value pages of one layer."""
+        return self.key_pages[index], self.value_pages[index]
+
+    def step(self, counts: Sequence[int]) -> PagedBatch:
+        """The batch of a step that brings ``counts[b]`` new tokens of sequence b, its pages reserved."""
+        if len(counts) != self.sequences or any(n < 0 for n in counts):
+            raise ValueError(f"a step takes a number of new tokens for each of the {self.sequences} sequences, got {list(counts)}")
+        for b, n in enumerate(counts):
+            if self._held[b] + n > self.max_length:
+                raise ValueError(f"sequence {b} has {self._held[b]} tokens: {n} more exceed the cache's {self.max_length}")
+        if not self._fixed:
+            want = [max(0, -(-(held + n) // self.page_size) - len(owned))
+                    for held, n, owned in zip(self._held, counts, self._owned)]
+            if sum(want) > len(self._free):
+                raise RuntimeError(f"the step needs {sum(want)} more pages, the cache has {len(self._free)} left")
+            for b, n in enumerate(want):
+                if n:
+                    have = len(self._owned[b])
+                    taken = [self._free.pop() for _ in range(n)]
+                    self._owned[b] += taken
+                    self.table[b, have:have + n] = torch.tensor(taken, dtype=torch.int32).to(self.table.device)
+        n = counts[0]
+        if all(c == n for c in counts):
+            starts = torch.arange(self.sequences + 1, dtype=torch.int32, device=self.table.device) * n
+        else:
+            ends = [0]
+            for c in counts:
+                ends.append(ends[-1] + c)
+            starts = torch.tensor(ends, dtype=torch.int32).to(self.table.device)
+        return PagedBatch(self.table, self.lengths, starts, max(counts))
+
+    def advance(self, counts: Sequence[int], batch: PagedBatch) -> None:
+        """Counts a step's tokens in, after its last layer."""
+        self.lengths.add_(batch.starts[1:] - batch.starts[:-1])
+        self._held = [held + n for held, n in zip(self._held, counts)]
+
+    def release(self, sequence: int | None = None) -> None:
+        """Forgets a sequence's tokens, or all: its next step starts at position 0."""
+        for b in range(self.sequences) if sequence is None else (sequence,):
+            self._held[b] = 0
+            self.lengths[b] = 0
+            if not self._fixed:
+                self._free += reversed(self._owned[b])
+                self._owned[b] = []
+
+    def rows(self, token_ids: Tensor, counts: Sequence[int] | None, positions: int) -> tuple[Tensor, list[int]]:
+        """The packed ids of a step and its counts, checked against a model of ``positions`` positions: ids [B, T], or [N]
+        with ``counts``."""
+        if counts is None:
+            if token_ids.ndim != 2 or token_ids.shape[0] != self.sequences:
+                raise ValueError(f"token_ids must have shape [{self.sequences}, T], or [N] with counts, got {tuple(token_ids.shape)}")
+            numbers = [token_ids.shape[1]] * self.sequences
+        else:
+            numbers = [int(n) for n in counts]
+            if token_ids.ndim != 1 or token_ids.shape[0] != sum(numbers):
+                raise ValueError(f"token_ids must have shape [{sum(numbers)}], one sequence after another, got {tuple(token_ids.shape)}")
+        for b, n in enumerate(numbers[:self.sequences]):
+            if self._held[b] + n > positions:
+                raise ValueError(f"sequence length {self._held[b] + n} exceeds configured maximum {positions}")
+        return token_ids.reshape(-1), numbers
+
+    def positions(self, batch: PagedBatch, numbers: Sequence[int], most: int) -> Tensor:
+        """Each packed row's position in its sequence (at most ``most - 1``, where a replayed graph runs over it)."""
+        n, first = sum(numbers), numbers[0]
+        row = torch.arange(n, device=self.lengths.device)
+        if all(c == first for c in numbers):
+            sequence = row // max(first, 1)
+        else:
+            sequence = torch.repeat_interleave(torch.arange(self.sequences), torch.tensor(numbers)).to(self.lengths.device)
+        return (self.lengths[sequence] + row - batch.starts[sequence]).clamp(max=most - 1)
