@@ -387,6 +387,30 @@ PyObject* score(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// score_backward(logits, tokens, stats, entropy, d_log_probs, d_entropy) -> d_logits
+PyObject* score_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6) return PyErr_Format(PyExc_TypeError, "score_backward takes 6 arguments");
+  Call c;
+  const Tensor* x = a[0] == Py_None || !THPVariable_Check(a[0]) ? nullptr : &THPVariable_Unpack(a[0]);
+  const Tensor *tokens = c.dense(a[1]), *stats = c.dense(a[2]), *entropy = c.dense(a[3]), *g = c.dense(a[4]), *h = c.dense(a[5]);
+  if (!c.ok || !x || !tokens || !stats || !entropy || !x->is_cuda() || x->get_device() != c.device || !x->is_contiguous() ||
+      x->dim() < 1 || x->numel() < 1 || code(x) < 0)
+    Py_RETURN_NONE;
+  const int64_t v = x->sizes().back(), rows = x->numel() / v;
+  for (const Tensor* t : {g, h})
+    if (t && (t->scalar_type() != at::kFloat || t->numel() != rows)) Py_RETURN_NONE;
+  if (tokens->numel() != rows || entropy->numel() != rows || stats->numel() != 2 * rows) Py_RETURN_NONE;
+  Tensor d = c.empty(x->sizes(), x->scalar_type());
+  const int status = da_token_log_probs_bwd(
+      x->data_ptr(), code(x), v, rows, v, static_cast<const int64_t*>(tokens->data_ptr()),
+      static_cast<const float*>(stats->data_ptr()), static_cast<const float*>(entropy->data_ptr()),
+      static_cast<const float*>(data(g)), static_cast<const float*>(data(h)), d.data_ptr(), v, c.stream());
+  if (status) return done("da_token_log_probs_bwd", status, nullptr);
+  return THPVariable_Wrap(std::move(d));
+  END_HANDLE_TH_ERRORS
+}
+
 // set_check(check): what raises the exception for a status
 PyObject* set_check(PyObject*, PyObject* check) {
   Py_INCREF(check);
@@ -408,6 +432,7 @@ PyMethodDef g_methods[] = {{"norm", fast<norm>(), METH_FASTCALL, nullptr},
                            {"append_paged", fast<append_paged>(), METH_FASTCALL, nullptr},
                            {"attend_paged", fast<attend_paged>(), METH_FASTCALL, nullptr},
                            {"score", fast<score>(), METH_FASTCALL, nullptr},
+                           {"score_backward", fast<score_backward>(), METH_FASTCALL, nullptr},
                            {"set_check", set_check, METH_O, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 

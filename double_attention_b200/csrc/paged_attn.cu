@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], p_full[2], p_empty[2];
   __shared__ int bad[kMaxStages];  // the tile's pages are not all in the cache
-  __shared__ __align__(16) uint16_t weight[2][16 * kPPitch];
+  __shared__ __align__(16) uint16_t weight[2][2][16 * kPPitch];  // rounded to T, and what that left, rounded too
   __shared__ __align__(16) float warp_max[2][16][kScoreWarps];
   __shared__ float rescale[2][16], row_max[16], row_sum[kScoreWarps][16];
   __shared__ int64_t buf[32], start_off;
@@ -397,9 +397,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
           warp_max[pb][g + 8][warp] = top1;
         }
         named_bar_sync(1, 32 * kScoreWarps);
-        const float4 w0 = *reinterpret_cast<const float4*>(warp_max[pb][g]), w1 = *reinterpret_cast<const float4*>(warp_max[pb][g + 8]);
-        top0 = fmaxf(fmaxf(w0.x, w0.y), fmaxf(w0.z, w0.w));
-        top1 = fmaxf(fmaxf(w1.x, w1.y), fmaxf(w1.z, w1.w));
+        const float4 m0 = *reinterpret_cast<const float4*>(warp_max[pb][g]), m1 = *reinterpret_cast<const float4*>(warp_max[pb][g + 8]);
+        top0 = fmaxf(fmaxf(m0.x, m0.y), fmaxf(m0.z, m0.w));
+        top1 = fmaxf(fmaxf(m1.x, m1.y), fmaxf(m1.z, m1.w));
         float c0 = 1.f, c1 = 1.f;
         if (top0 > ref0 + kGrow || (ref0 == -INFINITY && top0 > ref0)) {
           c0 = ref0 == -INFINITY ? 1.f : ex2(ref0 - top0);
@@ -415,8 +415,13 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
         l1 = fmaf(l1, c1, p10 + p11);
         ok &= mbar_wait(&p_empty[pb], tile_phase ^ 1u, ab, 63);
         __syncwarp();
-        *reinterpret_cast<uint32_t*>(&weight[pb][g * kPPitch + warp * 8 + pair]) = pack2<T>(p00, p01);
-        *reinterpret_cast<uint32_t*>(&weight[pb][(g + 8) * kPPitch + warp * 8 + pair]) = pack2<T>(p10, p11);
+        const uint32_t w0 = pack2<T>(p00, p01), w1 = pack2<T>(p10, p11);
+        const float2 r0 = unpack2<T>(w0), r1 = unpack2<T>(w1);
+        const int own = g * kPPitch + warp * 8 + pair;
+        *reinterpret_cast<uint32_t*>(&weight[pb][0][own]) = w0;
+        *reinterpret_cast<uint32_t*>(&weight[pb][0][own + 8 * kPPitch]) = w1;
+        *reinterpret_cast<uint32_t*>(&weight[pb][1][own]) = pack2<T>(p00 - r0.x, p01 - r0.y);
+        *reinterpret_cast<uint32_t*>(&weight[pb][1][own + 8 * kPPitch]) = pack2<T>(p10 - r1.x, p11 - r1.y);
         if (warp == 0 && (lane & 3) == 0) {
           rescale[pb][g] = c0;
           rescale[pb][g + 8] = c1;
@@ -512,7 +517,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
       if (odd) {
 #pragma unroll 1
         for (int key = 0; key < kKeys; ++key) {
-          const float w0 = unpack2<T>(weight[pb][g * kPPitch + key]).x, w1 = unpack2<T>(weight[pb][(g + 8) * kPPitch + key]).x;
+          const int own = g * kPPitch + key;
+          const float w0 = unpack2<T>(weight[pb][0][own]).x + unpack2<T>(weight[pb][1][own]).x;
+          const float w1 = unpack2<T>(weight[pb][0][own + 8 * kPPitch]).x + unpack2<T>(weight[pb][1][own + 8 * kPPitch]).x;
           const int box = p.brow == 32 ? 0 : key >> 4, in = p.brow == 32 ? key : key & 15;
 #pragma unroll
           for (int i = 0; i < kNT; ++i) {
@@ -530,8 +537,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
       } else {
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2) {
-          uint32_t a[4];
-          ldmatrix4(a, smem_u32(weight[pb]) + ((lane & 15) * kPPitch + k2 * 16 + (lane >> 4) * 8) * 2);
+          uint32_t a[4], rest[4];
+          const uint32_t from = smem_u32(weight[pb][0]) + ((lane & 15) * kPPitch + k2 * 16 + (lane >> 4) * 8) * 2;
+          ldmatrix4(a, from);
+          ldmatrix4(rest, from + 16 * kPPitch * 2);
           const uint32_t at = vb + value_off + k2 * half_off;
 #pragma unroll
           for (int n2 = 0; n2 < kNT / 2; ++n2) {
@@ -539,6 +548,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
             ldmatrix4_trans(b, (at + (n2 >> 2) * block) ^ ((n2 & 3) << 5));
             mma16816<T>(acc[2 * n2], a, b[0], b[1]);
             mma16816<T>(acc[2 * n2 + 1], a, b[2], b[3]);
+            mma16816<T>(acc[2 * n2], rest, b[0], b[1]);
+            mma16816<T>(acc[2 * n2 + 1], rest, b[2], b[3]);
           }
         }
       }
@@ -725,7 +736,7 @@ FewPlan few_plan(int64_t tokens, int64_t B, int64_t capacity, int64_t max_new, i
   f.key_bytes = paged::kKeys * 2 * wide;
   f.stage_bytes = f.key_bytes + paged::kKeys * 2 * D;
   const int per_sm = ctas_per_sm(wide, D);
-  f.stages = (227 * 1024 / per_sm - 1024 - 6 * 1024 - 32 * wide) / f.stage_bytes;  // (a CTA's own 1 KB, fixed buffers, alignment, queries)
+  f.stages = (227 * 1024 / per_sm - 1024 - 8 * 1024 - 32 * wide) / f.stage_bytes;  // (a CTA's own 1 KB, fixed buffers, alignment, queries)
   if (f.stages > paged::kMaxStages) f.stages = paged::kMaxStages;
   f.smem = f.stages * f.stage_bytes + 32 * wide + 1024;
   const int64_t rows = 16 / lanes, jobs = tokens / rows + B < tokens ? tokens / rows + B : tokens;
@@ -752,7 +763,7 @@ bool attn_shape(int H, int R, int D, int maps) {
 
 template <typename T, int kSteps, int kNT, int kCtas>
 int launch_few(const paged::FewParams& p, const FewPlan& f, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
-  if (int rc = allow_smem<paged::few_kernel<T, kSteps, kNT, kCtas>>(221 * 1024)) return rc;
+  if (int rc = allow_smem<paged::few_kernel<T, kSteps, kNT, kCtas>>(219 * 1024)) return rc;
   if (int rc = launch_kernel(paged::few_kernel<T, kSteps, kNT, kCtas>, dim3((unsigned)f.ctas), dim3(paged::kThreads), f.smem, st,
                              false, tk, tv, p))
     return rc;

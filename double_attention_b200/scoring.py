@@ -77,6 +77,9 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     def _gradient(ctx, d_log_probs: Tensor | None, d_entropy: Tensor | None) -> Tensor:
         logits, tokens, stats, entropy = ctx.saved_tensors
+        done = _host().score_backward(logits, tokens, stats, entropy, d_log_probs, d_entropy)
+        if done is not None:
+            return done
         x, rows, ld = _rows(logits)
         v = logits.shape[-1]
         g = None if d_log_probs is None else d_log_probs.float().contiguous()
