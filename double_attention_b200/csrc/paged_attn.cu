@@ -6,7 +6,8 @@
 // of up to 16 / maps tokens of a sequence are the 16 rows of one matrix product: row (s, t) holds q's branches of map
 // s and zeros in the other branches' columns, so all maps' scores come from one pass over the H R columns of a key
 // tile, and all rows share the value tile.  Each row keeps its own running maximum, sum and output; the maps are
-// mixed once, at the end, which needs no second pass over the keys for their sums.
+// mixed once, at the end, which needs no second pass over the keys for their sums.  (Where 8 rows hold a sequence's new
+// tokens the other 8 take what the rounding of the weights left.)
 //
 // Work: the (sequence, 16 rows) jobs' tiles of 32 keys form one flat list, which the CTAs share evenly, whatever the
 // sequences' lengths.  A job that lies in one CTA is finished there; the pieces of one that does not leave their
@@ -38,7 +39,8 @@ struct FewParams {
   void* y;
   float* part;  // [2 * CTAs][16][D] rows, then [2 * CTAs][2][16] maxima (log2) and sums
   int* status;
-  int H, R, D, maps, group, lanes;  // lanes: maps rounded up to a power of two; 16 / lanes tokens a job
+  int H, R, D, maps, group, lanes;  // lanes: maps rounded up to a power of two
+  int job_rows;                     // 16, or 8: job_rows / lanes tokens a job
   int few_most;                     // sequences with more new tokens are another kernel's
   int few_rows;                     // combine_kernel's rows a sequence
   int stages, stage_bytes, key_bytes, brow;
@@ -52,7 +54,7 @@ struct FewParams {
 DA_DEV int job_tiles(const Cache& c, const Sequence& s) { return (int)((positions(c, s) + kKeys - 1) / kKeys); }
 DA_DEV int64_t sequence_tiles(const FewParams& p, const Sequence& s, int b) {
   if (s.n == 0 || (s.n > p.few_most && !(p.chunked && left_odd(p.chunks, b)))) return 0;
-  const int tokens = 16 / p.lanes;
+  const int tokens = p.job_rows / p.lanes;
   return (int64_t)((s.n + tokens - 1) / tokens) * job_tiles(p.c, s);
 }
 
@@ -146,9 +148,11 @@ DA_DEV int64_t job_end(const Cache& c, const Sequence& s, int job, int tokens) {
   return e < c.capacity ? e : c.capacity;
 }
 
+// kHalf: 8 rows a job.  A weight is multiplied in two parts, rounded to T and what that left: as two products, or, with 8 rows,
+// in the other 8 rows of one.
 // kSteps: column steps of 16 that the queries' registers hold (H R at most 16 kSteps); kNT: value columns in tiles of 8 a
 // warp (D = 32 kNT); kCtas: CTAs an SM.
-template <typename T, int kSteps, int kNT, int kCtas>
+template <typename T, int kSteps, int kNT, int kCtas, bool kHalf>
 __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_constant__ CUtensorMap tk,
                                                              const __grid_constant__ CUtensorMap tv, const FewParams p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -237,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
   if (begin >= total) return;
   Walk walk{start_b, start_off, share < total - begin ? share : total - begin, start_seq, true};
   Abort ab{&abort_flag, p.status};
-  const int tokens = 16 / p.lanes;
+  const int tokens = p.job_rows / p.lanes;
   Piece x;
   int st = 0;         // stage of the next tile
   uint32_t phase = 0;  // of its barriers
@@ -315,8 +319,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
   }
 
   const int g = lane / 4, pair = (lane % 4) * 2;
-  const int map_shift = p.lanes == 1 ? 4 : p.lanes == 2 ? 3 : 2, token_of = tokens - 1;
-  // row r: map r >> map_shift, token r & token_of
+  const int map_shift = 31 - __clz(tokens), token_of = tokens - 1;
+  // row r: map r >> map_shift (at least `maps`, so none, for the upper rows of kHalf), token r & token_of
   const int s0 = g >> map_shift, s1 = (g + 8) >> map_shift, k0 = g & token_of, k1 = (g + 8) & token_of;
   uint32_t tile_phase = 0;  // of p_full and p_empty, buffer `pb`
   int pb = 0;
@@ -419,12 +423,14 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
         const float2 r0 = unpack2<T>(w0), r1 = unpack2<T>(w1);
         const int own = g * kPPitch + warp * 8 + pair;
         *reinterpret_cast<uint32_t*>(&weight[pb][0][own]) = w0;
-        *reinterpret_cast<uint32_t*>(&weight[pb][0][own + 8 * kPPitch]) = w1;
-        *reinterpret_cast<uint32_t*>(&weight[pb][1][own]) = pack2<T>(p00 - r0.x, p01 - r0.y);
-        *reinterpret_cast<uint32_t*>(&weight[pb][1][own + 8 * kPPitch]) = pack2<T>(p10 - r1.x, p11 - r1.y);
+        *reinterpret_cast<uint32_t*>(&weight[pb][kHalf ? 0 : 1][own + (kHalf ? 8 * kPPitch : 0)]) = pack2<T>(p00 - r0.x, p01 - r0.y);
+        if constexpr (!kHalf) {
+          *reinterpret_cast<uint32_t*>(&weight[pb][0][own + 8 * kPPitch]) = w1;
+          *reinterpret_cast<uint32_t*>(&weight[pb][1][own + 8 * kPPitch]) = pack2<T>(p10 - r1.x, p11 - r1.y);
+        }
         if (warp == 0 && (lane & 3) == 0) {
           rescale[pb][g] = c0;
-          rescale[pb][g + 8] = c1;
+          rescale[pb][g + 8] = kHalf ? c0 : c1;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[pb]);
@@ -518,8 +524,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
 #pragma unroll 1
         for (int key = 0; key < kKeys; ++key) {
           const int own = g * kPPitch + key;
-          const float w0 = unpack2<T>(weight[pb][0][own]).x + unpack2<T>(weight[pb][1][own]).x;
-          const float w1 = unpack2<T>(weight[pb][0][own + 8 * kPPitch]).x + unpack2<T>(weight[pb][1][own + 8 * kPPitch]).x;
+          auto part = [&](int i, int at) { return unpack2<T>(weight[pb][i][at]).x; };
+          const float w0 = kHalf ? part(0, own) + part(0, own + 8 * kPPitch) : part(0, own) + part(1, own);
+          const float w1 = kHalf ? 0.f : part(0, own + 8 * kPPitch) + part(1, own + 8 * kPPitch);
           const int box = p.brow == 32 ? 0 : key >> 4, in = p.brow == 32 ? key : key & 15;
 #pragma unroll
           for (int i = 0; i < kNT; ++i) {
@@ -540,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
           uint32_t a[4], rest[4];
           const uint32_t from = smem_u32(weight[pb][0]) + ((lane & 15) * kPPitch + k2 * 16 + (lane >> 4) * 8) * 2;
           ldmatrix4(a, from);
-          ldmatrix4(rest, from + 16 * kPPitch * 2);
+          if constexpr (!kHalf) ldmatrix4(rest, from + 16 * kPPitch * 2);
           const uint32_t at = vb + value_off + k2 * half_off;
 #pragma unroll
           for (int n2 = 0; n2 < kNT / 2; ++n2) {
@@ -548,8 +555,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
             ldmatrix4_trans(b, (at + (n2 >> 2) * block) ^ ((n2 & 3) << 5));
             mma16816<T>(acc[2 * n2], a, b[0], b[1]);
             mma16816<T>(acc[2 * n2 + 1], a, b[2], b[3]);
-            mma16816<T>(acc[2 * n2], rest, b[0], b[1]);
-            mma16816<T>(acc[2 * n2 + 1], rest, b[2], b[3]);
+            if constexpr (!kHalf) {
+              mma16816<T>(acc[2 * n2], rest, b[0], b[1]);
+              mma16816<T>(acc[2 * n2 + 1], rest, b[2], b[3]);
+            }
           }
         }
       }
@@ -563,6 +572,13 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
     }
 
     // ---- the job's output, or this piece of it
+    if constexpr (kHalf) {
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) {
+        acc[i][0] += acc[i][2];
+        acc[i][1] += acc[i][3];
+      }
+    }
     named_bar_sync(2, 32 * (kScoreWarps + kValueWarps));
     float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
@@ -587,15 +603,19 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
             *reinterpret_cast<uint32_t*>(y + ((q0 + k1) * p.maps + s1) * p.D + col) = pack2<T>(b0, b1);
           continue;
         }
-        if (p.lanes == 1) {
-          if (k1 < live) *reinterpret_cast<uint32_t*>(y + (q0 + k1) * p.D + col) = pack2<T>(b0, b1);
-        } else {  // maps of a token: rows 8 apart, and with four maps rows 4 apart too
+        // maps of a token: rows 8 apart (a thread's own), then 4 (lanes 16 apart), then 2
+        if (!kHalf && p.lanes == 1 && k1 < live) *reinterpret_cast<uint32_t*>(y + (q0 + k1) * p.D + col) = pack2<T>(b0, b1);
+        if (!kHalf && p.lanes > 1) {
           a0 += b0;
           a1 += b1;
-          if (p.lanes == 4) {
-            a0 += __shfl_xor_sync(0xffffffffu, a0, 16);
-            a1 += __shfl_xor_sync(0xffffffffu, a1, 16);
-          }
+        }
+        if (p.lanes > (kHalf ? 1 : 2)) {
+          a0 += __shfl_xor_sync(0xffffffffu, a0, 16);
+          a1 += __shfl_xor_sync(0xffffffffu, a1, 16);
+        }
+        if (kHalf && p.lanes == 4) {
+          a0 += __shfl_xor_sync(0xffffffffu, a0, 8);
+          a1 += __shfl_xor_sync(0xffffffffu, a1, 8);
         }
         if (s0 == 0 && k0 < live) *reinterpret_cast<uint32_t*>(y + (q0 + k0) * p.D + col) = pack2<T>(a0, a1);
       }
@@ -626,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
 // slots 2 c.
 template <typename T>
 DA_DEV void join(const FewParams& p, int64_t row, int t, int c0, int pieces, int slot0, float (*wts)[512], float4 (*sums)[17]) {
-  const int tid = threadIdx.x, tokens = 16 / p.lanes;
+  const int tid = threadIdx.x, tokens = p.job_rows / p.lanes;
   const float* ml = p.part + (size_t)2 * p.ctas * 16 * p.D;
   // each map's weights of the pieces: 2^(m_c - M) / sum, times alpha
   const int warp = tid / 32, lane = tid % 32;
@@ -707,7 +727,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const FewParams p) {
   grid_launch_dependents();
   if (!mine) return;
   const int64_t share = share_of(total, p.ctas);
-  const int tokens = 16 / p.lanes, tiles = job_tiles(p.c, s);
+  const int tokens = p.job_rows / p.lanes, tiles = job_tiles(p.c, s);
   for (int i = blockIdx.x % p.few_rows; i < s.n; i += p.few_rows) {
     const int64_t f0 = ahead + (int64_t)(i / tokens) * tiles, f1 = f0 + tiles;
     const int c0 = (int)(f0 / share), c1 = (int)((f1 - 1) / share);
@@ -724,7 +744,7 @@ namespace {
 using namespace da;
 
 struct FewPlan {
-  int stages, stage_bytes, key_bytes, smem, ctas, few_rows;
+  int stages, stage_bytes, key_bytes, smem, ctas, few_rows, job_rows;
 };
 
 // Two CTAs an SM where queries and outputs leave registers for them (H R and D up to 256): one computes while the other
@@ -733,13 +753,14 @@ int ctas_per_sm(int wide, int D) { return wide <= 256 && D <= 256 ? 2 : 1; }
 
 FewPlan few_plan(int64_t tokens, int64_t B, int64_t capacity, int64_t max_new, int wide, int D, int lanes) {
   FewPlan f;
+  f.job_rows = max_new * lanes <= 8 ? 8 : 16;  // a sequence's new tokens in one job, if it can be
   f.key_bytes = paged::kKeys * 2 * wide;
   f.stage_bytes = f.key_bytes + paged::kKeys * 2 * D;
   const int per_sm = ctas_per_sm(wide, D);
   f.stages = (227 * 1024 / per_sm - 1024 - 8 * 1024 - 32 * wide) / f.stage_bytes;  // (a CTA's own 1 KB, fixed buffers, alignment, queries)
   if (f.stages > paged::kMaxStages) f.stages = paged::kMaxStages;
   f.smem = f.stages * f.stage_bytes + 32 * wide + 1024;
-  const int64_t rows = 16 / lanes, jobs = tokens / rows + B < tokens ? tokens / rows + B : tokens;
+  const int64_t rows = f.job_rows / lanes, jobs = tokens / rows + B < tokens ? tokens / rows + B : tokens;
   const int64_t tiles = (capacity + paged::kKeys - 1) / paged::kKeys;
   const int64_t most = (int64_t)sm_count() * per_sm, need = jobs * (tiles > 0 ? tiles : 1);
   f.ctas = (int)(need < most ? need : most);
@@ -761,10 +782,10 @@ bool attn_shape(int H, int R, int D, int maps) {
   return D == 128 || D == 256 || D == 512;
 }
 
-template <typename T, int kSteps, int kNT, int kCtas>
+template <typename T, int kSteps, int kNT, int kCtas, bool kHalf>
 int launch_few(const paged::FewParams& p, const FewPlan& f, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
-  if (int rc = allow_smem<paged::few_kernel<T, kSteps, kNT, kCtas>>(219 * 1024)) return rc;
-  if (int rc = launch_kernel(paged::few_kernel<T, kSteps, kNT, kCtas>, dim3((unsigned)f.ctas), dim3(paged::kThreads), f.smem, st,
+  if (int rc = allow_smem<paged::few_kernel<T, kSteps, kNT, kCtas, kHalf>>(219 * 1024)) return rc;
+  if (int rc = launch_kernel(paged::few_kernel<T, kSteps, kNT, kCtas, kHalf>, dim3((unsigned)f.ctas), dim3(paged::kThreads), f.smem, st,
                              false, tk, tv, p))
     return rc;
   if (f.ctas == 1) return DA_OK;
@@ -772,16 +793,21 @@ int launch_few(const paged::FewParams& p, const FewPlan& f, const CUtensorMap& t
                        false, p);
 }
 
-template <typename T>
+template <typename T, bool kHalf>
 int launch_few(const paged::FewParams& p, const FewPlan& f, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
   const int wide = p.H * p.R;
   if (wide <= 256)
-    return p.D == 512   ? launch_few<T, 16, 16, 1>(p, f, tk, tv, st)
-           : p.D == 256 ? launch_few<T, 16, 8, 2>(p, f, tk, tv, st)
-                        : launch_few<T, 16, 4, 2>(p, f, tk, tv, st);
-  return p.D == 512   ? launch_few<T, 32, 16, 1>(p, f, tk, tv, st)
-         : p.D == 256 ? launch_few<T, 32, 8, 1>(p, f, tk, tv, st)
-                      : launch_few<T, 32, 4, 1>(p, f, tk, tv, st);
+    return p.D == 512   ? launch_few<T, 16, 16, 1, kHalf>(p, f, tk, tv, st)
+           : p.D == 256 ? launch_few<T, 16, 8, 2, kHalf>(p, f, tk, tv, st)
+                        : launch_few<T, 16, 4, 2, kHalf>(p, f, tk, tv, st);
+  return p.D == 512   ? launch_few<T, 32, 16, 1, kHalf>(p, f, tk, tv, st)
+         : p.D == 256 ? launch_few<T, 32, 8, 1, kHalf>(p, f, tk, tv, st)
+                      : launch_few<T, 32, 4, 1, kHalf>(p, f, tk, tv, st);
+}
+
+template <typename T>
+int launch_few(const paged::FewParams& p, const FewPlan& f, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
+  return p.job_rows == 8 ? launch_few<T, true>(p, f, tk, tv, st) : launch_few<T, false>(p, f, tk, tv, st);
 }
 
 }  // namespace
@@ -845,6 +871,7 @@ extern "C" int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_r
   p.maps = maps;
   p.group = H >= maps ? H / maps : 1;
   p.lanes = lanes;
+  p.job_rows = f.job_rows;
   p.few_most = chunked ? few_most(lanes) : 0x7fffffff;
   p.chunked = chunked;
   if (chunked) p.chunks = paged::chunk_plan(workspace, tokens, B, p.few_most);
