@@ -184,23 +184,44 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
 
   // ---- this CTA's share of the flat list of tiles
   const int64_t used = p.zero_rest ? clamp64(p.c.starts[p.c.B], 0, p.c.tokens) : p.c.tokens;
-  int64_t total = 0;
-  Sequence own{0, 0, 0, true};
-  for (int b = tid; b < p.c.B; b += kThreads) {
-    own = sequence(p.c, b);
-    total += sequence_tiles(p, own, b);
-  }
-  const bool short_list = p.c.B <= kThreads;  // then `total` is still the thread's own sequence's, scanned below
-  if (!short_list) total = block_sum<kThreads>(total, buf);
-  int64_t share = share_of(total, p.ctas), begin = (int64_t)blockIdx.x * share;
-  if (short_list || begin < total) {
+  int64_t total, share, begin;
+  Walk walk{0, 0, 0, {0, 0, 0, true}, true};
+  if (p.c.B <= 32) {  // every warp for itself, a sequence a lane
+    const Sequence own = lane < p.c.B ? sequence(p.c, lane) : Sequence{0, 0, 0, true};
+    const int64_t v = lane < p.c.B ? sequence_tiles(p, own, lane) : 0;
+    int64_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    total = __shfl_sync(0xffffffffu, inc, 31);
+    share = share_of(total, p.ctas);
+    begin = (int64_t)blockIdx.x * share;
+    const int b = __ffs(__ballot_sync(0xffffffffu, begin >= inc - v && begin < inc)) - 1;
+    if (b >= 0) {
+      walk.b = b;
+      walk.off = begin - __shfl_sync(0xffffffffu, inc - v, b);
+      walk.s.first = __shfl_sync(0xffffffffu, own.first, b);
+      walk.s.held = __shfl_sync(0xffffffffu, own.held, b);
+      walk.s.n = __shfl_sync(0xffffffffu, own.n, b);
+      walk.s.fits = __shfl_sync(0xffffffffu, (int)own.fits, b) != 0;
+    }
+    __syncthreads();  // (the barriers are initialised)
+  } else {
+    int64_t mine = 0;
+    Sequence own{0, 0, 0, true};
+    for (int b = tid; b < p.c.B; b += kThreads) mine += sequence_tiles(p, sequence(p.c, b), b);
+    total = block_sum<kThreads>(mine, buf);
+    share = share_of(total, p.ctas);
+    begin = (int64_t)blockIdx.x * share;
     int64_t before = 0;  // tiles of the sequences before this round's
-    for (int base = 0;; base += kThreads) {
+    for (int base = 0; begin < total; base += kThreads) {
       const int b = base + tid;
-      int64_t v = total;
-      if (!short_list) {
-        if (b < p.c.B) own = sequence(p.c, b);
-        v = b < p.c.B ? sequence_tiles(p, own, b) : 0;
+      int64_t v = 0;
+      if (b < p.c.B) {
+        own = sequence(p.c, b);
+        v = sequence_tiles(p, own, b);
       }
       int64_t inc = v;
 #pragma unroll
@@ -217,20 +238,16 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
         if (i < warp) at += buf[i];
         all += buf[i];
       }
-      if (short_list) {
-        total = all;
-        share = share_of(total, p.ctas);
-        begin = (int64_t)blockIdx.x * share;
-      }
       if (begin >= at && begin < at + v) {
         start_b = b;
         start_off = begin - at;
         start_seq = own;
       }
       before += all;
-      if (short_list || begin < before) break;  // (total > begin: found at the latest with the last sequence)
+      if (begin < before) break;  // (found at the latest with the last sequence)
     }
     __syncthreads();
+    if (begin < total) walk = {start_b, start_off, 0, start_seq, true};
   }
   if (used < p.c.tokens) {
     const int64_t words = (int64_t)(p.per_map ? p.maps : 1) * p.D / 8;
@@ -239,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
       rest[i] = make_uint4(0, 0, 0, 0);
   }
   if (begin >= total) return;
-  Walk walk{start_b, start_off, share < total - begin ? share : total - begin, start_seq, true};
+  walk.left = share < total - begin ? share : total - begin;
   Abort ab{&abort_flag, p.status};
   const int tokens = p.job_rows / p.lanes;
   Piece x;
@@ -714,7 +731,16 @@ __global__ void __launch_bounds__(256) combine_kernel(const FewParams p) {
   const Sequence s = sequence(p.c, b);
   const bool mine = (int)(blockIdx.x % p.few_rows) < s.n && sequence_tiles(p, s, b) > 0;
   int64_t total = 0, ahead = 0;
-  if (mine) {
+  if (mine && p.c.B <= 32) {
+    const int i = tid % 32;
+    total = i < p.c.B ? sequence_tiles(p, sequence(p.c, i), i) : 0;
+    ahead = i < b ? total : 0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+    }
+  } else if (mine) {
     for (int i = tid; i < p.c.B; i += 256) {
       const int64_t v = sequence_tiles(p, sequence(p.c, i), i);
       total += v;
