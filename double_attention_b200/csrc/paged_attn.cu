@@ -64,6 +64,54 @@ DA_DEV int64_t share_of(int64_t total, int ctas) {
   return (total + ctas - 1) / ctas;
 }
 
+// How up to 32 sequences' jobs are cut up, worked out by a warp (all lanes alike, but for a lane's own sequence).  Either into
+// pieces of their own, one a CTA, of `share` tiles at most -- a CTA then loads one job's queries and leaves one piece -- or,
+// where that takes longer pieces than even shares (their share and one tile more), into even shares of the flat list.
+struct Cut {
+  Sequence s;               // the lane's own
+  int64_t tiles, ahead;     // of the lane's sequence, and of those before it
+  int64_t total, share;
+  int pieces, pieces_ahead;  // of a job of the lane's sequence (0: even shares), of the sequences before it
+};
+
+DA_DEV Cut cut(const FewParams& p) {
+  const int lane = threadIdx.x % 32;
+  Cut c;
+  c.s = lane < p.c.B ? sequence(p.c, lane) : Sequence{0, 0, 0, true};
+  c.tiles = lane < p.c.B ? sequence_tiles(p, c.s, lane) : 0;
+  int64_t inc = c.tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  c.ahead = inc - c.tiles;
+  c.total = __shfl_sync(0xffffffffu, inc, 31);
+  c.share = share_of(c.total, p.ctas);
+  c.pieces = c.pieces_ahead = 0;
+  const int job = c.tiles ? job_tiles(p.c, c.s) : 1;
+  const int64_t jobs = c.total < 0x7fffffff ? (uint32_t)c.tiles / (uint32_t)job : c.tiles / job;
+  if (!__all_sync(0xffffffffu, jobs <= p.ctas)) return c;
+  const int64_t least = c.share;
+#pragma unroll 1
+  for (int64_t share = least; share <= least + 1; ++share) {
+    const int k = share < 0x7fffffff ? (int)(((uint32_t)job + (uint32_t)share - 1) / (uint32_t)share) : 1;
+    int n = (int)jobs * k;  // (k is at most ctas + 1, as share is at least total / ctas)
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) n += u;
+    }
+    if (__shfl_sync(0xffffffffu, n, 31) <= p.ctas) {
+      c.share = share;
+      c.pieces = k;
+      c.pieces_ahead = n - (int)jobs * k;
+      break;
+    }
+  }
+  return c;
+}
+
 // Sum over `threads` threads' values (all of them call it; every one gets it).  `buf` holds 32 entries.
 template <int threads>
 DA_DEV int64_t block_sum(int64_t v, int64_t* buf) {
@@ -187,25 +235,29 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
   int64_t total, share, begin;
   Walk walk{0, 0, 0, {0, 0, 0, true}, true};
   if (p.c.B <= 32) {  // every warp for itself, a sequence a lane
-    const Sequence own = lane < p.c.B ? sequence(p.c, lane) : Sequence{0, 0, 0, true};
-    const int64_t v = lane < p.c.B ? sequence_tiles(p, own, lane) : 0;
-    int64_t inc = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += u;
-    }
-    total = __shfl_sync(0xffffffffu, inc, 31);
-    share = share_of(total, p.ctas);
+    const Cut c = cut(p);
+    total = c.total;
+    share = c.share;
     begin = (int64_t)blockIdx.x * share;
-    const int b = __ffs(__ballot_sync(0xffffffffu, begin >= inc - v && begin < inc)) - 1;
+    int64_t off = begin - c.ahead, left = share < total - begin ? share : total - begin;
+    bool here = off >= 0 && off < c.tiles;
+    if (__any_sync(0xffffffffu, c.pieces)) {
+      const int tiles = c.tiles ? job_tiles(p.c, c.s) : 1, piece = (int)blockIdx.x - c.pieces_ahead;
+      const int length = (tiles + c.pieces - 1) / c.pieces, job = piece / c.pieces, part = piece - job * c.pieces;
+      off = (int64_t)job * tiles + part * length;
+      left = min(length, tiles - part * length);
+      here = piece >= 0 && off < c.tiles;
+      begin = __any_sync(0xffffffffu, here) ? 0 : total;
+    }
+    const int b = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
     if (b >= 0) {
       walk.b = b;
-      walk.off = begin - __shfl_sync(0xffffffffu, inc - v, b);
-      walk.s.first = __shfl_sync(0xffffffffu, own.first, b);
-      walk.s.held = __shfl_sync(0xffffffffu, own.held, b);
-      walk.s.n = __shfl_sync(0xffffffffu, own.n, b);
-      walk.s.fits = __shfl_sync(0xffffffffu, (int)own.fits, b) != 0;
+      walk.off = __shfl_sync(0xffffffffu, off, b);
+      walk.left = __shfl_sync(0xffffffffu, left, b);
+      walk.s.first = __shfl_sync(0xffffffffu, c.s.first, b);
+      walk.s.held = __shfl_sync(0xffffffffu, c.s.held, b);
+      walk.s.n = __shfl_sync(0xffffffffu, c.s.n, b);
+      walk.s.fits = __shfl_sync(0xffffffffu, (int)c.s.fits, b) != 0;
     }
     __syncthreads();  // (the barriers are initialised)
   } else {
@@ -247,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
       if (begin < before) break;  // (found at the latest with the last sequence)
     }
     __syncthreads();
-    if (begin < total) walk = {start_b, start_off, 0, start_seq, true};
+    if (begin < total) walk = {start_b, start_off, share < total - begin ? share : total - begin, start_seq, true};
   }
   if (used < p.c.tokens) {
     const int64_t words = (int64_t)(p.per_map ? p.maps : 1) * p.D / 8;
@@ -256,7 +308,6 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
       rest[i] = make_uint4(0, 0, 0, 0);
   }
   if (begin >= total) return;
-  walk.left = share < total - begin ? share : total - begin;
   Abort ab{&abort_flag, p.status};
   const int tokens = p.job_rows / p.lanes;
   Piece x;
@@ -731,15 +782,13 @@ __global__ void __launch_bounds__(256) combine_kernel(const FewParams p) {
   const Sequence s = sequence(p.c, b);
   const bool mine = (int)(blockIdx.x % p.few_rows) < s.n && sequence_tiles(p, s, b) > 0;
   int64_t total = 0, ahead = 0;
+  int job_pieces = 0, first_piece = 0;
   if (mine && p.c.B <= 32) {
-    const int i = tid % 32;
-    total = i < p.c.B ? sequence_tiles(p, sequence(p.c, i), i) : 0;
-    ahead = i < b ? total : 0;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      total += __shfl_xor_sync(0xffffffffu, total, o);
-      ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
-    }
+    const Cut c = cut(p);
+    total = c.total;
+    ahead = __shfl_sync(0xffffffffu, c.ahead, b);
+    job_pieces = __shfl_sync(0xffffffffu, c.pieces, b);
+    first_piece = __shfl_sync(0xffffffffu, c.pieces_ahead, b);
   } else if (mine) {
     for (int i = tid; i < p.c.B; i += 256) {
       const int64_t v = sequence_tiles(p, sequence(p.c, i), i);
@@ -755,6 +804,11 @@ __global__ void __launch_bounds__(256) combine_kernel(const FewParams p) {
   const int64_t share = share_of(total, p.ctas);
   const int tokens = p.job_rows / p.lanes, tiles = job_tiles(p.c, s);
   for (int i = blockIdx.x % p.few_rows; i < s.n; i += p.few_rows) {
+    if (job_pieces) {
+      const int c = first_piece + i / tokens * job_pieces;
+      if (job_pieces > 1) join<T>(p, s.first + i, i % tokens, c, job_pieces, 2 * c, wts, sums);
+      continue;
+    }
     const int64_t f0 = ahead + (int64_t)(i / tokens) * tiles, f1 = f0 + tiles;
     const int c0 = (int)(f0 / share), c1 = (int)((f1 - 1) / share);
     if (c0 < c1)  // (else finished where it was computed)
