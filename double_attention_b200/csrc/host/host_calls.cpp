@@ -343,7 +343,7 @@ PyObject* attend_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Tensor y = per_map ? c.empty({tokens, maps, p.D}, q->scalar_type()) : c.empty({tokens, p.D}, q->scalar_type()), work;
   if (need > 0) work = c.empty({need}, at::kByte);
   const int status = da_paged_attn(
-      q->data_ptr(), q->stride(0), q->stride(1), tokens, kp->data_ptr(), vp->data_ptr(), p.type, p.pages, (int)p.page, (int)p.H,
+      q->data_ptr(), q->stride(0), tokens > 1 ? q->stride(1) : p.R, tokens, kp->data_ptr(), vp->data_ptr(), p.type, p.pages, (int)p.page, (int)p.H,
       (int)p.R, (int)p.D, (int)maps, s.at(s.table), s.cols, s.cols, s.at(s.lengths), s.at(s.starts), s.B, max_new,
       static_cast<const float*>(scales->data_ptr()), per_map ? nullptr : static_cast<const float*>(data(weights)), per_map, 1,
       y.data_ptr(), need > 0 ? work.data_ptr() : nullptr, need, static_cast<int*>(word->data_ptr()), c.stream());

@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
 
   // ---- this CTA's share of the flat list of tiles
   const int64_t used = p.zero_rest ? clamp64(p.c.starts[p.c.B], 0, p.c.tokens) : p.c.tokens;
+  const int64_t before = p.zero_rest ? clamp64(p.c.starts[0], 0, used) : 0;
   int64_t total, share, begin;
   Walk walk{0, 0, 0, {0, 0, 0, true}, true};
   if (p.c.B <= 32) {  // every warp for itself, a sequence a lane
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
     total = block_sum<kThreads>(mine, buf);
     share = share_of(total, p.ctas);
     begin = (int64_t)blockIdx.x * share;
-    int64_t before = 0;  // tiles of the sequences before this round's
+    int64_t done = 0;  // tiles of the sequences before this round's
     for (int base = 0; begin < total; base += kThreads) {
       const int b = base + tid;
       int64_t v = 0;
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
       __syncthreads();
       if (lane == 31) buf[warp] = inc;
       __syncthreads();
-      int64_t at = before + inc - v, all = 0;
+      int64_t at = done + inc - v, all = 0;
 #pragma unroll
       for (int i = 0; i < kThreads / 32; ++i) {
         if (i < warp) at += buf[i];
@@ -295,17 +296,17 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
         start_off = begin - at;
         start_seq = own;
       }
-      before += all;
-      if (begin < before) break;  // (found at the latest with the last sequence)
+      done += all;
+      if (begin < done) break;  // (found at the latest with the last sequence)
     }
     __syncthreads();
     if (begin < total) walk = {start_b, start_off, share < total - begin ? share : total - begin, start_seq, true};
   }
-  if (used < p.c.tokens) {
-    const int64_t words = (int64_t)(p.per_map ? p.maps : 1) * p.D / 8;
-    uint4* rest = static_cast<uint4*>(p.y) + used * words;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < (p.c.tokens - used) * words; i += (int64_t)gridDim.x * kThreads)
-      rest[i] = make_uint4(0, 0, 0, 0);
+  if (before || used < p.c.tokens) {  // rows of no sequence
+    const int64_t words = (int64_t)(p.per_map ? p.maps : 1) * p.D / 8, gap = (used - before) * words;
+    uint4* y = static_cast<uint4*>(p.y);
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < p.c.tokens * words - gap; i += (int64_t)gridDim.x * kThreads)
+      y[i < before * words ? i : i + gap] = make_uint4(0, 0, 0, 0);
   }
   if (begin >= total) return;
   Abort ab{&abort_flag, p.status};

@@ -103,7 +103,7 @@ constexpr int kPlanThreads = 256, kPlanWarps = kPlanThreads / 32, kLengths = 10,
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const Plan plan, int few_most, int pairs) {
   __shared__ int2 kept[1024];  // the first sequences' new tokens (of chunks), and tokens that they had
   __shared__ unsigned long long units;
-  __shared__ int counts[kLengths], lengths[kLengths], carry[2], sums[2][kPlanWarps], best;
+  __shared__ int counts[kLengths], lengths[kLengths], carry[2], made[2], sums[2][kPlanWarps], best;
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
   if (threadIdx.x < kLengths) counts[threadIdx.x] = 0;
   if (threadIdx.x == 0) {
     units = 0;
-    carry[0] = carry[1] = 0;
+    carry[0] = carry[1] = made[0] = made[1] = 0;
   }
   __syncthreads();
   auto get = [&](int b) { return b < 1024 ? kept[b] : load(b); };
@@ -194,6 +194,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
       carry[1] = piece0 + count;
     }
     if (b < c.B && lane == 0) plan.odd[b] = 0;
+    __syncwarp();
     const Sequence whole = sequence(c, b < c.B ? b : 0);
     for (int i0 = 0; i0 < tiles; i0 += 32) {
       const int i = i0 + lane, keys = i < tiles ? keys_of(s, i) : 0, own = (unsigned)(keys + best - 1) / (unsigned)best;
@@ -204,10 +205,17 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
         if (lane >= o) at += u;
       }
       const int all = __shfl_sync(0xffffffffu, at, 31), first = piece0 + at - own;
-      if (i < tiles) plan.tile_piece[tile0 + i] = first;
+      // (starts that do not rise bring more tokens than there are rows: what the plan has no room for is the other kernel's)
+      const bool fits = i < tiles && tile0 + i < plan.tiles_most && first + own <= plan.pieces_most;
+      if (fits) plan.tile_piece[tile0 + i] = first;
+      if (i < tiles && !fits) plan.odd[b] = 1;
+      if (fits) {
+        atomicMax(&made[0], tile0 + i + 1);
+        atomicMax(&made[1], first + own);
+      }
       // (a tile's pieces side by side: the warp writes one tile after another, a piece a lane)
       for (int j = 0; j < min(32, tiles - i0); ++j) {
-        const int from = __shfl_sync(0xffffffffu, first, j), many = __shfl_sync(0xffffffffu, own, j);
+        const int from = __shfl_sync(0xffffffffu, first, j), many = __shfl_sync(0xffffffffu, fits ? own : 0, j);
         const int last = __shfl_sync(0xffffffffu, keys, j);
         for (int m = lane; m < many; m += 32) {
           plan.pieces[3 * (from + m)] = make_int4(b, i0 + j, m * best, min(best, last - m * best));
@@ -220,8 +228,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    plan.tile_piece[carry[0]] = carry[1];
-    *reinterpret_cast<int4*>(plan.head) = make_int4(carry[1], carry[0], 0, 0);
+    plan.tile_piece[made[0]] = made[1];
+    *reinterpret_cast<int4*>(plan.head) = make_int4(made[1], made[0], 0, 0);
   }
 }
 

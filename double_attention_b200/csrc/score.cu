@@ -231,7 +231,7 @@ DA_DEV float nth_largest(float x, int top) {
 
 // kThreads a row: 32 (eight rows a CTA) or 1024.
 template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads == 32 ? 256 : 1024) forward_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads == 32 ? 256 : 1024, kThreads == 32 ? 6 : 1) forward_kernel(const Params p) {
   using V = Vec<T>;
   constexpr int kBatch = 4;  // loads in flight a thread, their largest value found together
   constexpr int kFound = kThreads == 32 ? 256 : 1024;  // entries that a row has room for

@@ -84,7 +84,8 @@ def _check_pages(name: str, key_pages: Tensor, value_pages: Tensor) -> tuple[int
 def append_paged(keys: Tensor, values: Tensor, key_pages: Tensor, value_pages: Tensor, batch: PagedBatch) -> None:
     """Writes the packed new tokens' keys [H, N, R] and values [N, D] behind what their sequences have, in place.
 
-    Token i of sequence b goes to position ``batch.lengths[b] + i``; the lengths stay as they are.  Keys and values in
+    Token i of sequence b goes to position ``batch.lengths[b] + i``, in a page that no other sequence writes; the lengths stay as
+    they are.  Keys and values in
     fp32, bf16 or fp16 with unit column stride or any other (copied first then), rounded once to the pages' type.  Nothing
     but the new positions is written."""
     name = "append_paged"
@@ -132,7 +133,7 @@ def routed_attention_paged(query: Tensor, key_pages: Tensor, value_pages: Tensor
     query [H, N, R] of the pages' type; ``scales`` [S] the maps' temperatures, S of H branches as in
     :func:`assemble_score_maps`.  Token i of sequence b sees positions 0 to ``batch.lengths[b] + i``.  With
     ``map_weights`` [S], or one map, returns the maps' mixture [N, D]; without, several maps' outputs [N, S, D].  The
-    keys may be of any length: the softmax takes off each row's own maximum.  Rows behind the last sequence are zero,
+    keys may be of any length: the softmax takes off each row's own maximum.  Rows of no sequence are zero,
     or left as they are in ``out``.
 
     Supported: R a multiple of 64, D 128, 256 or 512, up to 4 maps and ``max(H, S) * R`` up to 512."""
@@ -175,7 +176,7 @@ def routed_attention_paged(query: Tensor, key_pages: Tensor, value_pages: Tensor
     with torch.cuda.device(device):
         need = _lib.lib().da_paged_attn_workspace_size(n, b, table.shape[1], page, most, h, r, d, maps, int(per_map))
     work = torch.empty(need, dtype=torch.uint8, device=query.device) if need > 0 else None
-    _launch(device, "da_paged_attn", query.data_ptr(), query.stride(0), query.stride(1), n, key_pages.data_ptr(),
+    _launch(device, "da_paged_attn", query.data_ptr(), query.stride(0), query.stride(1) if n > 1 else r, n, key_pages.data_ptr(),
             value_pages.data_ptr(), _CODES[query.dtype], pages, page, h, r, d, maps, table.data_ptr(),
             table.stride(0) if b > 1 else table.shape[1], table.shape[1], lengths.data_ptr(), starts.data_ptr(), b, most,
             scales.data_ptr(), ptr(weights), int(per_map), int(out is None), y.data_ptr(), ptr(work), max(need, 0),

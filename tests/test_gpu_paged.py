@@ -328,6 +328,56 @@ def test_no_tokens_and_no_sequences() -> None:
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("new", [[3, 20], [150, 200]])
+@pytest.mark.parametrize("weights", [[0.0, 1.0], [-0.5, 1.5], [0.0, 0.0], [1e-6, 2.0]])
+def test_map_weights_of_any_sign(weights, new) -> None:
+    case = Case(2, 2, 128, 256, 32, BF16, [100, 300], new, seed=17, fill=5.0)
+    case.append()
+    case.weights = torch.tensor(weights, device="cuda")
+    want, _ = case.expected()
+    per_map, each = case.expected(per_map=True)
+    # (each map's bound counts by its weight; the mixture is rounded once)
+    bound = (each * case.weights.abs()[:, None].double()).sum(1) + torch.finfo(BF16).eps / 2 * want.abs() + 1e-12
+    assert ((case.attend().double() - want).abs() <= bound).all()
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("new", [[3, 20], [150, 200]])
+@pytest.mark.parametrize("scale", [0.0, -16.0, 200.0])
+def test_temperatures_of_any_sign(scale, new) -> None:
+    for h, s in ((1, 1), (4, 4)):
+        case = Case(h, s, 128, 256, 32, FP16, [100, 700], new, scale=scale, seed=18, fill=5.0)
+        case.append()
+        want, bound = case.expected()
+        if scale < 0:
+            bound = bound + 2 * 2 * h * 128 * 2.0**-24 * 16 * 1.3 * want.abs().max()  # (expected() counts the drift of gamma, not |gamma|)
+        assert ((case.attend().double() - want).abs() <= bound).all()
+
+
+def test_starts_that_leave_rows_out_or_do_not_rise() -> None:
+    case = Case(1, 1, 128, 128, 16, BF16, [100, 300, 40], [70, 80, 90], seed=19, fill=5.0)
+    case.append()
+    starts = case.batch.starts.clone()
+    starts[0] = 66  # rows 0 to 65 belong to no sequence; the first one's four rows are its first four
+    y = case.attend(batch=case.batch._replace(starts=starts))
+    assert not y[:66].any() and torch.equal(y[70:], case.attend()[70:])
+    # sequences that overlap, more tokens than rows: nothing outside is touched, and nothing is waited for
+    table, lengths = case.batch.table[:1].repeat(64, 1), torch.zeros(64, dtype=torch.int32, device="cuda")
+    falling = torch.tensor([0, 240] * 32 + [0], dtype=torch.int32, device="cuda")
+    around = torch.full((242, 128), 7.0, dtype=BF16, device="cuda")
+    case.attend(batch=da.PagedBatch(table, lengths, falling), out=around[1:241])
+    assert (around[0] == 7.0).all() and (around[241] == 7.0).all()
+    ops.device_status()
+
+
+def test_one_token_of_any_strides() -> None:
+    case = Case(2, 2, 128, 256, 32, BF16, [100], [1], seed=20)
+    case.append()
+    odd = torch.as_strided(case.q.transpose(0, 1).contiguous(), (2, 1, 128), (128, 3, 1))
+    assert torch.equal(da.routed_attention_paged(odd, case.key_pages, case.value_pages, case.batch, case.scales, case.weights),
+                       case.attend())
+
+
 def test_many_sequences() -> None:
     held, new = [b * 37 % 200 for b in range(700)], [b % 3 for b in range(700)]
     case = Case(1, 1, 64, 128, 16, BF16, held, new, seed=13)

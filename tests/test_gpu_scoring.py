@@ -181,6 +181,21 @@ def test_gradient(rows, v, dtype, which) -> None:
     assert not got[x.isneginf()].any()
 
 
+def test_gradient_of_strided_logits() -> None:
+    x, tokens = _logits(37, 1000, BF16, 13)
+    g = torch.randn(37, device="cuda")
+    want = _gradient(x, tokens, g, g)
+    wide = torch.zeros(37, 1011, dtype=BF16, device="cuda")
+    wide[:, 5:1005] = x
+    for t in (wide.requires_grad_(), x.t().contiguous().requires_grad_()):
+        view = t[:, 5:1005] if t.shape[1] == 1011 else t.t()
+        made = da.token_log_probs(view, tokens.int())
+        d, = torch.autograd.grad((made.log_probs, made.entropy), t, (g, g))
+        d = d[:, 5:1005] if t.shape[1] == 1011 else d.t()
+        # (sums in another order: both sides round, half a step, 2^-8, each)
+        assert ((d.float() - want.float()).abs() <= 2.0**-7 * want.float().abs() + 1e-6).all()
+
+
 def test_gradient_against_differences() -> None:
     x, tokens = _logits(4, 300, FP32, 7)
     g, h = torch.tensor([1.0, -2.0, 0.5, 1.5], device="cuda"), torch.tensor([0.3, 0.0, -1.0, 2.0], device="cuda")
