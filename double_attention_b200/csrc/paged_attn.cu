@@ -895,10 +895,12 @@ int launch_few(const paged::FewParams& p, const FewPlan& f, const CUtensorMap& t
 
 namespace {
 
-// Sequences of more new tokens go to the chunk kernel, whose tiles have 128 of them: the tiles here, of 16 (map, token) rows,
-// would read the cache once for every 16 / maps of them.
-int few_most(int lanes) { return 64 / lanes; }
-bool has_chunks(int64_t tokens, int64_t max_new, int lanes) { return tokens >= 64 && max_new > few_most(lanes); }
+// A sequence whose new tokens are one job here, 16 (map, token) rows, reads its cache once; more of them go to the chunk
+// kernel, whose tiles have 128 tokens.  Eight sequences of 4096 tokens (one map of 256 columns, D 512): 8 new ones each
+// 34 us here, 30 there, 32 new ones 108 and 32; one sequence of 32768, 64 new ones: 185 and 40; but one of 2048 tokens 1 new
+// one: 10 here, 21 there.
+int few_most(int lanes) { return 16 / lanes; }
+bool has_chunks(int64_t max_new, int lanes) { return max_new > few_most(lanes); }
 
 }  // namespace
 
@@ -908,7 +910,7 @@ extern "C" int64_t da_paged_attn_workspace_size(int64_t tokens, int64_t B, int64
   if (tokens == 0 || B == 0) return 0;
   if (max_new < 1 || max_new > tokens) max_new = tokens;
   const int lanes = lanes_of(maps);
-  const int64_t chunks = has_chunks(tokens, max_new, lanes) ? paged::chunk_workspace(tokens, B, few_most(lanes), D, maps, per_map) : 0;
+  const int64_t chunks = has_chunks(max_new, lanes) ? paged::chunk_workspace(tokens, B, few_most(lanes), D, maps, per_map) : 0;
   return chunks + few_workspace(few_plan(tokens, B, table_cols * page, max_new, H * R, D, lanes), D);
 }
 
@@ -932,7 +934,7 @@ extern "C" int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_r
   if (max_new < 1 || max_new > tokens) max_new = tokens;
   if (int rc = bind_device(key_pages)) return rc;
   const int lanes = lanes_of(maps);
-  const bool chunked = has_chunks(tokens, max_new, lanes);
+  const bool chunked = has_chunks(max_new, lanes);
   const FewPlan f = few_plan(tokens, B, p.c.capacity, max_new, H * R, D, lanes);
   const int64_t chunk_bytes = chunked ? paged::chunk_workspace(tokens, B, few_most(lanes), D, maps, per_map) : 0;
   const int64_t need = chunk_bytes + few_workspace(f, D);

@@ -84,7 +84,7 @@ struct ChunkParams {
   Shape shape;
   int H, R, D, maps, group, dtype;
   int branch0[kMaxMaps];
-  int brow;            // positions a box
+  int brow, qrow;      // positions a box of keys or values, rows a box of queries
   int phase;           // several maps: 1 sums, 2 outputs; one map: 0
   const float *scales, *weights;
   void* y;
@@ -337,7 +337,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   } else if (warp == 0) {
     // ---------------------------------------------------------------- keys (both CTAs)
     if (elect_one()) {
-      if (rank == 0) mbar_arrive_expect_tx(&q_full, 2 * L.q_bytes);
+      // (fewer packed rows than a CTA's 64: the other rows hold anything, and are no sequence's)
+      if (rank == 0) mbar_arrive_expect_tx(&q_full, 2 * L.q_bytes / kRows * p.qrow);
       const uint32_t qf = mapa_shared(smem_u32(&q_full), 0), kf = mapa_shared(smem_u32(&k_full[0]), 0);
       const int row = seq.x + t0 + 64 * (int)rank;  // (rows past the last token are zeros)
       uint8_t* dst = smem;
@@ -953,6 +954,7 @@ int run(const ChunkArgs& a, cudaStream_t st) {
   const Shape L = p.shape;
   if (L.kslots < 2 || !L.tmem_cols) return DA_ERR_UNSUPPORTED;
   p.brow = a.c.page < 64 ? a.c.page : 64;
+  p.qrow = a.c.tokens < kRows ? (int)a.c.tokens : kRows;
   const bool whole = p.brow == 64;
   const CUtensorMapDataType dt = a.dtype == DA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap tq, tk, tv;
@@ -965,7 +967,7 @@ int run(const ChunkArgs& a, cudaStream_t st) {
   {  // queries: (column in its block of 64, row, branch, block)
     const uint64_t dims[4] = {64, (uint64_t)a.c.tokens, (uint64_t)a.H, (uint64_t)a.R / 64};
     const uint64_t strides[3] = {(uint64_t)a.q_row * 2, a.H > 1 ? (uint64_t)a.q_branch * 2 : 16, 128};
-    const uint32_t box[4] = {64, (uint32_t)kRows, 1, 1};
+    const uint32_t box[4] = {64, (uint32_t)p.qrow, 1, 1};
     if (int rc = make_tmap_blocks(&tq, a.q, dt, 2, 4, dims, strides, box)) return rc;
   }
   {  // values: (column in its block, slot, block inside an nc-wide group, group)

@@ -136,7 +136,9 @@ def test_lengths_around_tiles_and_pages(shape, held, new) -> None:
                                                     ((1, 1, 256, 512, 64), [3, 9000, 0, 700], [2, 65, 257, 1030]),
                                                     ((4, 4, 128, 512, 64), [2, 6000, 0, 700], [20, 65, 257, 630]),
                                                     ((3, 3, 128, 256, 128), [513], [300]), ((4, 2, 64, 128, 256), [513], [300]),
-                                                    ((1, 1, 192, 256, 64), [513, 0], [300, 128])])
+                                                    ((1, 1, 192, 256, 64), [513, 0], [300, 128]),
+                                                    ((1, 1, 256, 512, 64), [300], [17]), ((4, 4, 128, 512, 64), [300, 0], [5, 6]),
+                                                    ((2, 2, 128, 256, 16), [3000, 5], [9, 40]), ((1, 1, 512, 512, 64), [1000], [63])])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("fill", [math.nan, 30000.0])
 def test_chunks(shape, held, new, dtype, fill) -> None:
