@@ -42,7 +42,7 @@ struct FewParams {
   int H, R, D, maps, group, lanes;  // lanes: maps rounded up to a power of two
   int job_rows;                     // 16, or 8: job_rows / lanes tokens a job
   int few_most;                     // sequences with more new tokens are another kernel's
-  int few_rows;                     // combine_kernel's rows a sequence
+  int few_rows, slice;              // combine_kernel's rows a sequence, columns a CTA: 64 or 16
   int stages, stage_bytes, key_bytes, brow;
   int ctas;
   int per_map, zero_rest;
@@ -711,53 +711,70 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
   }
 }
 
-// One packed row from its pieces c0, c0 + 1, ...: the first in slot `slot0`, the later ones, which open their CTAs, in
-// slots 2 c.
+constexpr int kMaxPieces = 512;
+struct Joining {
+  float w[4][kMaxPieces], l[4][kMaxPieces];  // each map's weights and sums of the pieces
+  float4 o[8][16];                           // each warp's part of the columns
+};
+
+// One packed row's p.slice columns from its pieces c0, c0 + 1, ...: the first in slot `slot0`, the later ones, which open
+// their CTAs, in slots 2 c.  A thread takes four columns of every 1024 / p.slice-th piece.
 template <typename T>
-DA_DEV void join(const FewParams& p, int64_t row, int t, int c0, int pieces, int slot0, float (*wts)[512], float4 (*sums)[17]) {
-  const int tid = threadIdx.x, tokens = p.job_rows / p.lanes;
+DA_DEV void join(const FewParams& p, int64_t row, int t, int c0, int pieces, int slot0, Joining& j) {
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, tokens = p.job_rows / p.lanes, across = p.slice / 4;
   const float* ml = p.part + (size_t)2 * p.ctas * 16 * p.D;
   // each map's weights of the pieces: 2^(m_c - M) / sum, times alpha
-  const int warp = tid / 32, lane = tid % 32;
   if (warp < p.maps) {
     const int r = warp * tokens + t;
     float top = -INFINITY, sum = 0.f;
-    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, ml[(size_t)(i ? 2 * (c0 + i) : slot0) * 32 + r]);
+#pragma unroll 4
+    for (int i = lane; i < pieces; i += 32) {
+      const float* at = ml + (size_t)(i ? 2 * (c0 + i) : slot0) * 32 + r;
+      const float m = at[0], l = at[16];
+      j.w[warp][i] = m;
+      j.l[warp][i] = l;
+      top = fmaxf(top, m);
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     for (int i = lane; i < pieces; i += 32) {
-      const float* at = ml + (size_t)(i ? 2 * (c0 + i) : slot0) * 32;
-      const float e = at[r] == -INFINITY ? 0.f : ex2(at[r] - top);
-      sum += at[16 + r] * e;  // (a NaN sum, of a piece with a bad page, stays)
-      wts[warp][i] = e;
+      const float m = j.w[warp][i], e = m == -INFINITY ? 0.f : ex2(m - top);
+      sum += j.l[warp][i] * e;  // (a NaN sum, of a piece with a bad page, stays)
+      j.w[warp][i] = e;
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float f = (p.weights ? p.weights[warp] : 1.f) / sum;
-    for (int i = lane; i < pieces; i += 32) wts[warp][i] *= f;
+    for (int i = lane; i < pieces; i += 32) j.w[warp][i] *= f;
   }
   __syncthreads();
-  const int col = blockIdx.y * 64 + (tid % 16) * 4, part = tid / 16;
+  const int c4 = tid % across, col = blockIdx.y * p.slice + c4 * 4, part = tid / across, parts = 256 / across;
   T* y = static_cast<T*>(p.y);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int m = 0; m < p.maps; ++m) {
 #pragma unroll 4
-    for (int i = part; i < pieces; i += 16) {
-      const float w = wts[m][i];
+    for (int i = part; i < pieces; i += parts) {
+      const float w = j.w[m][i];
       const float4 v = *reinterpret_cast<const float4*>(
           p.part + ((size_t)(i ? 2 * (c0 + i) : slot0) * 16 + m * tokens + t) * p.D + col);
       if (w == 0.f) continue;  // (a piece that the row does not see)
-      o.x += w * v.x;
-      o.y += w * v.y;
-      o.z += w * v.z;
-      o.w += w * v.w;
+      o.x = fmaf(w, v.x, o.x);
+      o.y = fmaf(w, v.y, o.y);
+      o.z = fmaf(w, v.z, o.z);
+      o.w = fmaf(w, v.w, o.w);
     }
     if (!p.per_map && m + 1 < p.maps) continue;
-    sums[part][tid % 16] = o;
+    for (int k = across; k < 32; k <<= 1) {
+      o.x += __shfl_xor_sync(0xffffffffu, o.x, k);
+      o.y += __shfl_xor_sync(0xffffffffu, o.y, k);
+      o.z += __shfl_xor_sync(0xffffffffu, o.z, k);
+      o.w += __shfl_xor_sync(0xffffffffu, o.w, k);
+    }
+    if (lane < across) j.o[warp][lane] = o;
     __syncthreads();
-    if (part == 0) {
-      for (int i = 1; i < 16; ++i) {
-        const float4 v = sums[i][tid];
+    if (tid < across) {
+      for (int i = 1; i < 8; ++i) {
+        const float4 v = j.o[i][tid];
         o.x += v.x;
         o.y += v.y;
         o.z += v.z;
@@ -771,12 +788,11 @@ DA_DEV void join(const FewParams& p, int64_t row, int t, int c0, int pieces, int
   }
 }
 
-// Joins the pieces of the jobs that lie in several CTAs: one CTA a packed token and 64 columns.
+// Joins the pieces of the jobs that lie in several CTAs: one CTA a packed token and p.slice columns.
 template <typename T>
 __global__ void __launch_bounds__(256) combine_kernel(const FewParams p) {
   __shared__ int64_t buf[32];
-  __shared__ float wts[4][512];
-  __shared__ float4 sums[16][17];
+  __shared__ Joining j;
   const int tid = threadIdx.x, b = blockIdx.x / p.few_rows;
   // (The pieces' kernel lets this one start after it has itself waited for the kernels before it, so what those wrote --
   // the step's lengths and the chunks' plan -- may be read before the wait for the pieces.)
@@ -807,13 +823,13 @@ __global__ void __launch_bounds__(256) combine_kernel(const FewParams p) {
   for (int i = blockIdx.x % p.few_rows; i < s.n; i += p.few_rows) {
     if (job_pieces) {
       const int c = first_piece + i / tokens * job_pieces;
-      if (job_pieces > 1) join<T>(p, s.first + i, i % tokens, c, job_pieces, 2 * c, wts, sums);
+      if (job_pieces > 1) join<T>(p, s.first + i, i % tokens, c, job_pieces, 2 * c, j);
       continue;
     }
     const int64_t f0 = ahead + (int64_t)(i / tokens) * tiles, f1 = f0 + tiles;
     const int c0 = (int)(f0 / share), c1 = (int)((f1 - 1) / share);
     if (c0 < c1)  // (else finished where it was computed)
-      join<T>(p, s.first + i, i % tokens, c0, c1 - c0 + 1, 2 * c0 + (f0 > c0 * share ? 1 : 0), wts, sums);
+      join<T>(p, s.first + i, i % tokens, c0, c1 - c0 + 1, 2 * c0 + (f0 > c0 * share ? 1 : 0), j);
   }
 }
 
@@ -846,7 +862,7 @@ FewPlan few_plan(int64_t tokens, int64_t B, int64_t capacity, int64_t max_new, i
   const int64_t most = (int64_t)sm_count() * per_sm, need = jobs * (tiles > 0 ? tiles : 1);
   f.ctas = (int)(need < most ? need : most);
   if (f.ctas < 1) f.ctas = 1;
-  if (f.ctas > 512) f.ctas = 512;  // pieces that combine_kernel has room for
+  if (f.ctas > paged::kMaxPieces) f.ctas = paged::kMaxPieces;
   f.few_rows = (int)(max_new < 64 ? max_new : 64);
   return f;
 }
@@ -870,7 +886,7 @@ int launch_few(const paged::FewParams& p, const FewPlan& f, const CUtensorMap& t
                              false, tk, tv, p))
     return rc;
   if (f.ctas == 1) return DA_OK;
-  return launch_kernel(paged::combine_kernel<T>, dim3((unsigned)(p.c.B * p.few_rows), (unsigned)(p.D / 64)), dim3(256), 0, st,
+  return launch_kernel(paged::combine_kernel<T>, dim3((unsigned)(p.c.B * p.few_rows), (unsigned)(p.D / p.slice)), dim3(256), 0, st,
                        false, p);
 }
 
@@ -959,6 +975,7 @@ extern "C" int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_r
   p.chunked = chunked;
   if (chunked) p.chunks = paged::chunk_plan(workspace, tokens, B, p.few_most);
   p.few_rows = f.few_rows < p.few_most ? f.few_rows : p.few_most;
+  p.slice = (int64_t)p.c.B * p.few_rows * (D / 64) >= sm_count() ? 64 : 16;
   p.stages = f.stages;
   p.stage_bytes = f.stage_bytes;
   p.key_bytes = f.key_bytes;
