@@ -2,8 +2,8 @@
 //
 // A call on one token is over on the device in 2 to 10 us; from Python, checking the tensors, allocating the outputs
 // and converting the arguments takes 8 to 15.  The functions here do the same for tensors that lie as the kernels
-// want them (dense, on the current device, of the right types, nothing requiring a gradient or carrying a tangent) in
-// 4 to 6 us, launch included, and return None for anything else, which the Python functions then check, copy or
+// want them (dense, on the current device, of the right types, nothing carrying a tangent or, but for the scores,
+// requiring a gradient) in 4 to 6 us, launch included, and return None for anything else, which the Python functions then check, copy or
 // refuse.  The kernels and their C entry points are the same either way.
 #include <Python.h>
 
@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "da_b200.h"
@@ -38,8 +39,8 @@ at::ScalarType type_of(int64_t code) {
 }
 
 // The tensor of an argument; null for None.  Sets `ok` to false for anything else, and where a kernel could not read
-// the tensor in place: off the device, not dense, or part of a gradient or of a forward-mode derivative.
-const Tensor* plain(PyObject* o, c10::DeviceIndex device, bool dense, bool* ok) {
+// the tensor in place: off the device, not dense, or part of a gradient (but for `grad`) or of a forward-mode derivative.
+const Tensor* plain(PyObject* o, c10::DeviceIndex device, bool dense, bool* ok, bool grad = false) {
   if (o == Py_None) return nullptr;
   if (!THPVariable_Check(o)) {
     *ok = false;
@@ -47,7 +48,7 @@ const Tensor* plain(PyObject* o, c10::DeviceIndex device, bool dense, bool* ok) 
   }
   const Tensor& t = THPVariable_Unpack(o);
   if (!t.is_cuda() || t.get_device() != device || (dense && !t.is_contiguous()) ||
-      (t.requires_grad() && c10::GradMode::is_enabled()) ||
+      (!grad && t.requires_grad() && c10::GradMode::is_enabled()) ||
       (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()))
     *ok = false;
   return &t;
@@ -352,62 +353,113 @@ PyObject* attend_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// score(logits, tokens, top, keep) -> (log_probs, entropy, top_log_probs, top_tokens, stats)
-PyObject* score(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  if (n != 4) return PyErr_Format(PyExc_TypeError, "score takes 4 arguments");
-  Call c;
-  const Tensor *x = c.dense(a[0]), *tokens = c.dense(a[1]);
-  const int64_t top = PyLong_AsLongLong(a[2]);
-  const int keep = PyObject_IsTrue(a[3]);
-  if (PyErr_Occurred()) return nullptr;
-  if (!c.ok || !x || !tokens || code(x) < 0 || x->dim() < 1 || tokens->scalar_type() != at::kLong) Py_RETURN_NONE;
-  const at::IntArrayRef sizes = x->sizes(), lead = sizes.slice(0, sizes.size() - 1);
-  const int64_t v = sizes.back(), rows = v ? x->numel() / v : 0;
-  if (rows < 1 || tokens->sizes() != lead || top < 0 || top > 32 || top > v) Py_RETURN_NONE;
-  Tensor log_probs = c.empty(lead, at::kFloat), entropy = c.empty(lead, at::kFloat), top_lp, top_tokens, stats;
+// The scores of dense logits [rows, v], and in `stats`, where it is defined, what their backward pass needs; a status.
+int score_rows(const Call& c, const Tensor& x, const Tensor& tokens, int64_t top, Tensor* made, Tensor* stats) {
+  const at::IntArrayRef sizes = x.sizes(), lead = sizes.slice(0, sizes.size() - 1);
+  const int64_t v = sizes.back(), rows = x.numel() / v;
+  made[0] = c.empty(lead, at::kFloat);
+  made[1] = c.empty(lead, at::kFloat);
   if (top) {
     c10::SmallVector<int64_t, 6> wide(sizes.begin(), sizes.end());
     wide.back() = top;
-    top_lp = c.empty(wide, at::kFloat);
-    top_tokens = c.empty(wide, at::kLong);
+    made[2] = c.empty(wide, at::kFloat);
+    made[3] = c.empty(wide, at::kLong);
   }
-  if (keep) stats = c.empty({rows, 2}, at::kFloat);
-  const int status = da_token_log_probs(
-      x->data_ptr(), code(x), v, rows, v, static_cast<const int64_t*>(tokens->data_ptr()), (int)top,
-      static_cast<float*>(log_probs.data_ptr()), static_cast<float*>(entropy.data_ptr()),
-      top ? static_cast<float*>(top_lp.data_ptr()) : nullptr, top ? static_cast<int64_t*>(top_tokens.data_ptr()) : nullptr,
-      keep ? static_cast<float*>(stats.data_ptr()) : nullptr, c.stream());
-  if (status) return done("da_token_log_probs", status, nullptr);
-  PyObject* r = PyTuple_New(5);
-  int i = 0;
-  for (Tensor* t : {&log_probs, &entropy, &top_lp, &top_tokens, &stats})
-    PyTuple_SET_ITEM(r, i++, t->defined() ? THPVariable_Wrap(std::move(*t)) : (Py_INCREF(Py_None), Py_None));
-  return r;
-  END_HANDLE_TH_ERRORS
+  if (stats) *stats = c.empty({rows, 2}, at::kFloat);
+  return da_token_log_probs(
+      x.data_ptr(), code(&x), v, rows, v, static_cast<const int64_t*>(tokens.data_ptr()), (int)top,
+      static_cast<float*>(made[0].data_ptr()), static_cast<float*>(made[1].data_ptr()),
+      top ? static_cast<float*>(made[2].data_ptr()) : nullptr, top ? static_cast<int64_t*>(made[3].data_ptr()) : nullptr,
+      stats ? static_cast<float*>(stats->data_ptr()) : nullptr, c.stream());
 }
 
-// score_backward(logits, tokens, stats, entropy, d_log_probs, d_entropy) -> d_logits
-PyObject* score_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// The package's exception for a status, thrown out of a backward pass, whose thread does not hold the interpreter.
+void check(const char* name, int status) {
+  if (status == DA_OK) return;
+  const PyGILState_STATE held = PyGILState_Ensure();
+  done(name, status, nullptr);
+  python_error error;
+  error.persist();
+  PyGILState_Release(held);
+  throw error;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// A gradient as it is; differentiated again, it raises.
+struct FirstOrder : torch::autograd::Function<FirstOrder> {
+  static Tensor forward(AutogradContext*, const Tensor& d, const Tensor&) { return d.view_as(d); }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "token_log_probs has no second derivative");
+  }
+};
+
+// As the Python function of the same passes; an eager training step on few tokens is over 40 us sooner by it.
+struct Score : torch::autograd::Function<Score> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& tokens, int64_t top, const Call* c,
+                               int* status) {
+    variable_list made(top ? 4 : 2);
+    Tensor stats;
+    *status = score_rows(*c, x, tokens, top, made.data(), &stats);
+    ctx->set_materialize_grads(false);
+    if (top) ctx->mark_non_differentiable({made[2], made[3]});
+    ctx->save_for_backward({x, tokens, stats, made[1]});
+    return made;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor &g = grads[0], &h = grads[1];
+    variable_list d(5);
+    if (!g.defined() && !h.defined()) return d;
+    const variable_list kept = ctx->get_saved_variables();
+    const Tensor &x = kept[0], &tokens = kept[1], &stats = kept[2], &entropy = kept[3];
+    {
+      const c10::AutoGradMode none(false);
+      const Call c;  // (the engine has made the device and the stream of the forward pass current)
+      const int64_t v = x.sizes().back();
+      Tensor gs, hs;
+      if (g.defined()) gs = g.to(at::kFloat).contiguous();
+      if (h.defined()) hs = h.to(at::kFloat).contiguous();
+      d[0] = c.empty(x.sizes(), x.scalar_type());
+      check("da_token_log_probs_bwd",
+            da_token_log_probs_bwd(x.data_ptr(), code(&x), v, x.numel() / v, v, static_cast<const int64_t*>(tokens.data_ptr()),
+                                   static_cast<const float*>(stats.data_ptr()), static_cast<const float*>(entropy.data_ptr()),
+                                   g.defined() ? static_cast<const float*>(gs.data_ptr()) : nullptr,
+                                   h.defined() ? static_cast<const float*>(hs.data_ptr()) : nullptr, d[0].data_ptr(), v,
+                                   c.stream()));
+    }
+    if (c10::GradMode::is_enabled()) d[0] = FirstOrder::apply(d[0].requires_grad_(), g.defined() ? g : h);
+    return d;
+  }
+};
+
+// score(logits, tokens, top) -> (log_probs, entropy, top_log_probs, top_tokens), differentiable in logits
+PyObject* score(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 6) return PyErr_Format(PyExc_TypeError, "score_backward takes 6 arguments");
+  if (n != 3) return PyErr_Format(PyExc_TypeError, "score takes 3 arguments");
   Call c;
-  const Tensor* x = a[0] == Py_None || !THPVariable_Check(a[0]) ? nullptr : &THPVariable_Unpack(a[0]);
-  const Tensor *tokens = c.dense(a[1]), *stats = c.dense(a[2]), *entropy = c.dense(a[3]), *g = c.dense(a[4]), *h = c.dense(a[5]);
-  if (!c.ok || !x || !tokens || !stats || !entropy || !x->is_cuda() || x->get_device() != c.device || !x->is_contiguous() ||
-      x->dim() < 1 || x->numel() < 1 || code(x) < 0)
-    Py_RETURN_NONE;
-  const int64_t v = x->sizes().back(), rows = x->numel() / v;
-  for (const Tensor* t : {g, h})
-    if (t && (t->scalar_type() != at::kFloat || t->numel() != rows)) Py_RETURN_NONE;
-  if (tokens->numel() != rows || entropy->numel() != rows || stats->numel() != 2 * rows) Py_RETURN_NONE;
-  Tensor d = c.empty(x->sizes(), x->scalar_type());
-  const int status = da_token_log_probs_bwd(
-      x->data_ptr(), code(x), v, rows, v, static_cast<const int64_t*>(tokens->data_ptr()),
-      static_cast<const float*>(stats->data_ptr()), static_cast<const float*>(entropy->data_ptr()),
-      static_cast<const float*>(data(g)), static_cast<const float*>(data(h)), d.data_ptr(), v, c.stream());
-  if (status) return done("da_token_log_probs_bwd", status, nullptr);
-  return THPVariable_Wrap(std::move(d));
+  const bool grad = c10::GradMode::is_enabled() && THPVariable_Check(a[0]) && THPVariable_Unpack(a[0]).requires_grad();
+  const Tensor *x = plain(a[0], c.device, true, &c.ok, true), *tokens = c.dense(a[1]);
+  const int64_t top = PyLong_AsLongLong(a[2]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!c.ok || !x || !tokens || code(x) < 0 || x->dim() < 1 || tokens->scalar_type() != at::kLong) Py_RETURN_NONE;
+  const at::IntArrayRef sizes = x->sizes(), lead = sizes.slice(0, sizes.size() - 1);
+  const int64_t v = sizes.back();
+  if (x->numel() < 1 || tokens->sizes() != lead || top < 0 || top > 32 || top > v) Py_RETURN_NONE;
+  variable_list made(4);
+  int status = DA_OK;
+  if (grad) {
+    made = Score::apply(*x, *tokens, top, static_cast<const Call*>(&c), &status);
+    made.resize(4);
+  } else {
+    status = score_rows(c, *x, *tokens, top, made.data(), nullptr);
+  }
+  if (status) return done("da_token_log_probs", status, nullptr);
+  PyObject* r = PyTuple_New(4);
+  int i = 0;
+  for (Tensor& t : made)
+    PyTuple_SET_ITEM(r, i++, t.defined() ? THPVariable_Wrap(std::move(t)) : (Py_INCREF(Py_None), Py_None));
+  return r;
   END_HANDLE_TH_ERRORS
 }
 
@@ -432,7 +484,6 @@ PyMethodDef g_methods[] = {{"norm", fast<norm>(), METH_FASTCALL, nullptr},
                            {"append_paged", fast<append_paged>(), METH_FASTCALL, nullptr},
                            {"attend_paged", fast<attend_paged>(), METH_FASTCALL, nullptr},
                            {"score", fast<score>(), METH_FASTCALL, nullptr},
-                           {"score_backward", fast<score_backward>(), METH_FASTCALL, nullptr},
                            {"set_check", set_check, METH_O, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 

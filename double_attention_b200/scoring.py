@@ -34,9 +34,6 @@ class TokenLogProbs(NamedTuple):
 
 
 def _forward(logits: Tensor, tokens: Tensor, top: int, device: int, keep: bool):
-    done = _host().score(logits, tokens, top, keep)
-    if done is not None:
-        return done
     lead, v = logits.shape[:-1], logits.shape[-1]
     x, rows, ld = _rows(logits)
     made = _new(lead, torch.float32, logits.device), _new(lead, torch.float32, logits.device)
@@ -77,9 +74,6 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     def _gradient(ctx, d_log_probs: Tensor | None, d_entropy: Tensor | None) -> Tensor:
         logits, tokens, stats, entropy = ctx.saved_tensors
-        done = _host().score_backward(logits, tokens, stats, entropy, d_log_probs, d_entropy)
-        if done is not None:
-            return done
         x, rows, ld = _rows(logits)
         v = logits.shape[-1]
         g = None if d_log_probs is None else d_log_probs.float().contiguous()
@@ -101,9 +95,9 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, top: int = 0) -> TokenLog
     Differentiable in ``logits`` through ``log_probs`` and ``entropy`` (the alternatives carry no gradient)."""
     name = "token_log_probs"
     if logits.is_cuda:
-        done = _host().score(logits, tokens, top, False)  # (None where a gradient or a tangent is wanted)
+        done = _host().score(logits, tokens, top)
         if done is not None:
-            return TokenLogProbs(*done[:4])
+            return TokenLogProbs(*done)
     if logits.dtype not in _CODES:
         raise ValueError(f"{name} takes logits in float32, bfloat16 or float16, got {logits.dtype}")
     if not logits.ndim or not logits.shape[-1] or tokens.shape != logits.shape[:-1]:

@@ -267,6 +267,60 @@ def test_captured_and_on_another_stream() -> None:
             assert torch.equal(got, value)
 
 
+def test_a_training_step_in_a_graph() -> None:
+    x, tokens = _logits(40, 1001, BF16, 12)
+    g, h = torch.randn(40, device="cuda"), torch.randn(40, device="cuda")
+    x.requires_grad_()
+
+    def step():
+        made = da.token_log_probs(x, tokens)
+        return torch.autograd.grad((made.log_probs, made.entropy), x, (g, h))[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in (13, 14):
+        with torch.no_grad():
+            x.copy_(_logits(40, 1001, BF16, seed)[0])
+        graph.replay()
+        assert torch.equal(captured, step())
+
+
+def test_ways_to_the_gradient() -> None:
+    """One gradient however it is asked for: of several uses, of an expanded one, of tokens in 32 bits, of strided
+    logits, under saved-tensor hooks; and the graph's own checks of what was kept."""
+    x, tokens = _logits(24, 500, FP32, 15)
+    x.requires_grad_()
+    made = da.token_log_probs(x, tokens)
+    want, = torch.autograd.grad(made.log_probs, x, torch.ones(24, device="cuda"), retain_graph=True)
+    again, = torch.autograd.grad(made.log_probs.sum(), x, retain_graph=True)
+    assert torch.equal(again, want)
+    assert torch.equal(torch.autograd.grad(made.log_probs.view(4, 6).t().sum(), x)[0], want)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(made.log_probs.sum(), x)
+    assert torch.equal(torch.autograd.grad(da.token_log_probs(x, tokens.int()).log_probs.sum(), x)[0], want)
+    wide = torch.zeros(24, 700, device="cuda")
+    wide[:, 100:600] = x.detach()
+    wide.requires_grad_()
+    d, = torch.autograd.grad(da.token_log_probs(wide[:, 100:600], tokens).log_probs.sum(), wide)
+    assert torch.equal(d[:, 100:600], want) and not d[:, :100].any() and not d[:, 600:].any()
+    with torch.autograd.graph.save_on_cpu():
+        made = da.token_log_probs(x, tokens)
+    assert torch.equal(torch.autograd.grad(made.log_probs.sum(), x)[0], want)
+    made = da.token_log_probs(x, tokens, top=3)
+    assert made.log_probs.requires_grad and made.entropy.requires_grad and not made.top_log_probs.requires_grad
+    with torch.no_grad():
+        assert not da.token_log_probs(x, tokens).entropy.requires_grad
+        x.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(made.log_probs.sum(), x)
+
+
 def test_refusals() -> None:
     x, tokens = _logits(4, 50, BF16, 11)
     with pytest.raises(ValueError, match="float32"):
