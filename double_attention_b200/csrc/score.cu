@@ -4,16 +4,24 @@
 //   log p_i = x_i - m - ln 2 log2 l,     H = -sum p log p = ln 2 (log2 l - w / l),
 //   dL/dx_i = g ([i = token] - p_i) - h p_i (log p_i + H)   for g = dL/d log p_token, h = dL/dH.
 // m, l and w are kept against a running maximum, so the forward reads the logits once (16 bytes a load); the backward
-// reads them again and writes the gradient.  Both are bound by those bytes.  Differences from the row's maximum are
-// formed first and scaled then, so that logits far from zero lose nothing and a row of nothing but the type's lowest value
-// is an even one; an entry of minus infinity counts 0 in l, w and the gradient.  A row with a NaN, with plus infinity or with nothing but minus infinity is
+// reads them again and writes the gradient.  Differences from the row's maximum are formed first and scaled then, so that
+// logits far from zero lose nothing and a row of nothing but the type's lowest value is an even one; an entry of minus
+// infinity counts 0 in l, w and the gradient.  A row with a NaN, with plus infinity or with nothing but minus infinity is
 // NaN, as a softmax of it is.
 //
 // Top alternatives: in order of (value, lowest index), NaN before numbers.  The first pass leaves every warp's (or, where
 // a warp has a row, every lane's) largest value; the top-th largest of those is at most the top-th largest value of the
 // row, and few values lie above it (about 32 H_32 - 32 H_(32 - top) on independent ones), so a second pass, out of L1 and
-// L2, collects what is not below it and ranks it.  Where ties or hostile orders leave more than there is room for, every
-// warp keeps a sorted list instead, one entry a lane.
+// L2, collects what is not below it and ranks it.  Where a warp has a row it looks only at the vectors of lanes that have
+// any (16384 rows of 2048 in bf16, top 8: 23.4 us, 28.9 with a second pass over the whole row), takes its floor from
+// every lane's two largest where the top are many and halves what is left (top 32: 42.9 us; 65.5 without the second
+// values, 104 without either).  Where ties or hostile orders leave more than there is room for, every warp keeps a sorted
+// list instead, one entry a lane.
+//
+// What bounds them, in bf16: the forward at 65536 x 2048 (51 us, 5.2 TB/s) its instructions, with 2^t on a unit of 16 a
+// clock taking 30 us alone; the backward there (80 us, 6.7 TB/s read and written) HBM; 16384 x 2048 without alternatives
+// 14.4 us; one row (4 us) the latency of two dependent reads of it and of a reduction over 32 warps.  A warp a row, with
+// no barrier, is the faster where rows are short and many; a long row needs more loads in flight than a warp has.
 #include <math.h>
 
 #include "host_util.h"
@@ -129,9 +137,9 @@ struct Sums {
       m = to;
     }
   }
-  // k vectors at once.
+  // k vectors at once; their largest value.
   template <typename V, int k>
-  DA_DEV void add(const uint4* raw) {
+  DA_DEV float add(const uint4* raw) {
     float top = V::top(raw[0]);
 #pragma unroll
     for (int i = 1; i < k; ++i) top = fmaxf(top, V::top(raw[i]));
@@ -156,6 +164,7 @@ struct Sums {
     l = a + b;
     split(ws, a, b);
     w = a + b;
+    return top;
   }
   DA_DEV void add_one(float x) {
     raise(x);
@@ -215,8 +224,8 @@ struct List {
   }
 };
 
-// The top-th largest of the lanes' values (no NaN), in every lane: sorted over the warp, the smallest first.
-DA_DEV float nth_largest(float x, int top) {
+// The lanes' values (no NaN) sorted over the warp, the smallest first.
+DA_DEV float sorted(float x) {
   const int lane = threadIdx.x % 32;
 #pragma unroll
   for (int k = 2; k <= 32; k <<= 1)
@@ -226,7 +235,20 @@ DA_DEV float nth_largest(float x, int top) {
       const bool low = ((lane & j) == 0) == ((lane & k) == 0 || k == 32);
       x = low ? fminf(x, o) : fmaxf(x, o);
     }
-  return __shfl_sync(0xffffffffu, x, 32 - top);
+  return x;
+}
+// The top-th largest of them, in every lane.
+DA_DEV float nth_largest(float x, int top) { return __shfl_sync(0xffffffffu, sorted(x), 32 - top); }
+// The top-th largest of the lanes' firsts and seconds, no second larger than its first: of i firsts and top - i seconds,
+// the smallest is at most it, and is it for one i.
+DA_DEV float nth_largest(float first, float second, int top) {
+  const int lane = threadIdx.x % 32;
+  const float a = __shfl_sync(0xffffffffu, sorted(first), 31 - lane);  // the (lane + 1)-th largest
+  const float b = __shfl_sync(0xffffffffu, sorted(second), (33 - top + lane) & 31);
+  float x = lane >= top ? -INFINITY : lane == top - 1 ? a : fminf(a, b);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
 }
 
 // kThreads a row: 32 (eight rows a CTA) or 1024.
@@ -238,6 +260,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : 1024, kThreads == 32 ? 
   __shared__ Sums sums[32];
   __shared__ uint64_t found_all[kThreads == 32 ? 8 : 1][kFound];
   __shared__ int counts[kThreads == 32 ? 8 : 1];
+  __shared__ int lanes_all[kThreads == 32 ? 8 : 1][32];
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -253,11 +276,30 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : 1024, kThreads == 32 ? 
   if (tid == 0) *count = 0;
   const Row<T> row(p.logits, r * p.ld, p.V);
   Sums s{-INFINITY, 0.f, 0.f};
+  float second = -INFINITY;  // where a warp has a row: the lane's largest value but for the vectors with the largest
   {
     const int odd = row.odd(tid);
     float x = -INFINITY;
     if (odd >= 0) x = V::one(row.p + odd);
-    for (int v = tid; v < row.vecs; v += kBatch * kThreads) {
+    int v = tid;
+    if constexpr (kThreads == 32) {
+      // (a turn with vectors that are not there costs a warp as much as a full one: the last ones go singly.  A CTA, of
+      // which there are few, has them all in flight instead)
+      for (; v - lane + (kBatch - 1) * 32 < row.vecs; v += kBatch * 32) {
+        uint4 raw[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) raw[i] = v + i * 32 < row.vecs ? row.load(v + i * 32) : V::none();
+        const float before = s.m;
+        second = fmaxf(second, fminf(before, s.add<V, kBatch>(raw)));
+      }
+#pragma unroll 1
+      for (; v - lane < row.vecs; v += 32) {
+        const uint4 raw = v < row.vecs ? row.load(v) : V::none();
+        const float before = s.m;
+        second = fmaxf(second, fminf(before, s.add<V, 1>(&raw)));
+      }
+    }
+    for (; v < row.vecs; v += kBatch * kThreads) {
       uint4 raw[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) raw[i] = v + i * kThreads < row.vecs ? row.load(v + i * kThreads) : V::none();
@@ -285,7 +327,8 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : 1024, kThreads == 32 ? 
   }
   if (p.top == 0) return;
 
-  float floor = nth_largest(group, p.top);
+  // (few more than the top are above the floor of 32 values where the top are few: 9 for 8, but 130 for 32; of 64, 44)
+  float floor = kThreads == 32 && p.top > 8 ? nth_largest(group, second, p.top) : nth_largest(group, p.top);
   meet();
   auto write = [&](uint64_t e, int rank) {
     p.top_log_probs[r * p.top + rank] = value_of((uint32_t)(e >> 32)) - at - log_l * kLn2;
@@ -293,25 +336,79 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : 1024, kThreads == 32 ? 
   };
   {
     auto take = [&](float x, int index) {
-      if (x < floor) return;
       const int i = atomicAdd(count, 1);
       if (i < kFound) found[i] = entry_of(x, index);
     };
-#pragma unroll 2
-    for (int v = tid; v < row.vecs; v += kThreads) {
+    auto look = [&](int v) {
       const uint4 raw = row.load(v);
-      if (V::or_nan(raw) < floor) continue;
+      if (V::or_nan(raw) < floor) return;
       float x[V::n];
       values<V>(raw, x);
       const int index = row.index(v);
+      uint32_t in = 0;
 #pragma unroll
-      for (int i = 0; i < V::n; ++i) take(x[i], index + i);
+      for (int i = 0; i < V::n; ++i) in |= (uint32_t)!(x[i] < floor) << i;
+      for (; in; in &= in - 1) {
+        const int i = index + __ffs(in) - 1;
+        take(V::one(row.p + i), i);
+      }
+    };
+    if constexpr (kThreads == 32) {
+      // Only lanes whose largest value is not below the floor have any (and, in a row with a NaN, which that value
+      // passes over, all may): their vectors, dealt out to the whole warp.
+      const bool has = !(group < floor) || s.l != s.l;
+      const uint32_t who = __ballot_sync(0xffffffffu, has);
+      const int k = __popc(who), bits = 32 - __clz(k - 1);  // (a floor is some lane's value: k > 0)
+      int* lanes = lanes_all[warp];
+      if (has) lanes[__popc(who & ((1u << lane) - 1))] = lane;
+      __syncwarp();
+      const int f = lane & ((1 << bits) - 1);
+      if (f < k)
+        for (int v = lanes[f] + (lane >> bits) * 32; v < row.vecs; v += 1024 >> bits) look(v);
+    } else {
+#pragma unroll 2
+      for (int v = tid; v < row.vecs; v += kThreads) look(v);
     }
     const int odd = row.odd(tid);
-    if (odd >= 0) take(V::one(row.p + odd), odd);
+    if (odd >= 0) {
+      const float x = V::one(row.p + odd);
+      if (!(x < floor)) take(x, odd);
+    }
   }
   meet();
-  const int n = *count;
+  int n = *count;
+  if constexpr (kThreads == 32) {
+    // Ranking takes n^2 / 32 comparisons a lane: where that is many, a higher floor first, halving between this one and
+    // the largest until at most `most` of them are left (or no fewer can be, as of equal ones).
+    const int most = p.top <= 16 ? 32 : 64;
+    if (n > 64 && n <= kFound) {
+      uint32_t lo = order_of(floor), hi = 0;
+      for (int k = lane; k < n; k += 32) hi = max(hi, (uint32_t)(found[k] >> 32));
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      while (lo < hi) {  // top or more are not below lo, fewer above hi
+        const uint32_t mid = hi - (hi - lo) / 2;
+        int c = 0;
+        for (int k = lane; k < n; k += 32) c += (uint32_t)(found[k] >> 32) >= mid;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (c < p.top) {
+          hi = mid - 1;
+        } else {
+          lo = mid;
+          if (c <= most) break;
+        }
+      }
+      int left = 0;
+      for (int k = 0; k < n; k += 32) {  // to the front, never past what has been read
+        const uint64_t e = k + lane < n ? found[k + lane] : 0;
+        const bool in = k + lane < n && (uint32_t)(e >> 32) >= lo;
+        const uint32_t who = __ballot_sync(0xffffffffu, in);
+        if (in) found[left + __popc(who & ((1u << lane) - 1))] = e;
+        left += __popc(who);
+      }
+      __syncwarp();
+      n = left;
+    }
+  }
   if (n <= kFound) {
     for (int k = tid; k < n; k += kThreads) {  // no two entries are alike: every one has its rank, in whatever place it lies
       const uint64_t e = found[k];
