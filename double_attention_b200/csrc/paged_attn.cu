@@ -10,12 +10,23 @@
 // tokens the other 8 take what the rounding of the weights left.)
 //
 // Work: the (sequence, 16 rows) jobs' tiles of 32 keys form one flat list, which the CTAs share evenly, whatever the
-// sequences' lengths.  A job that lies in one CTA is finished there; the pieces of one that does not leave their
-// unnormalised rows in the workspace, and combine_kernel joins them in order.  Which CTA has which piece follows from
-// the lengths alone, so both kernels work it out from the device's own data and the host needs no lengths.
+// sequences' lengths (up to 32 sequences: pieces of their own, one a CTA, where those are no longer; struct Cut).  A job
+// that lies in one CTA is finished there; the pieces of one that does not leave their unnormalised rows in the
+// workspace, and combine_kernel joins them in order.  Which CTA has which piece follows from the lengths alone, so both
+// kernels work it out from the device's own data and the host needs no lengths.
 //
-// A tile: one thread brings the keys and values of 32 positions by TMA (one box each where a page has 32 positions),
-// several tiles ahead; eight warps split the H R columns of the score product and the D columns of the output.
+// A tile: one warp brings the keys and values of 32 positions by TMA (one box each where a page has 32 positions), as
+// many tiles ahead as shared memory holds.  Four warps take 8 keys each over all H R columns, keep the rows' maxima and
+// sums, and hand the weights over through shared memory to four warps that take D / 4 columns each of the output, so
+// that a tile's scores overlap the outputs of the one before.  (Eight warps doing both in turn: 192 us at 64 sequences of up to
+// 8192, against 107.)  The products are 16 x 8 x 16 instructions: 16 rows fill them, and 128-row ones
+// would spend 8 times the work on rows that do not exist.  Weights go in as two 16-bit parts, for an error of the output's own
+// rounding and nothing else (1.7e-3 in bf16 against 64 bits; one part 2.3e-3).
+//
+// Measured (bf16, 512 value columns, joining included): 64 sequences of 4096 to 8192, 256 key columns, 609 MB, 104 us, 5.9
+// TB/s, where a copy's rate would take 93 us; one sequence of 131072, 512 key columns, 268 MB, 56.4 us, 4.8 TB/s: two launches,
+// the first tiles' way from memory and the join count there.  One token of a sequence of 512 takes 10.2 us, and five drafted
+// tokens of eight sequences of up to 2008 (two maps) 20.8 us: latency of those steps and of a CTA's few dependent tiles.
 #include <math.h>
 
 #include "host_util.h"
