@@ -9,10 +9,10 @@
 // infinity counts 0 in l, w and the gradient.  A row with a NaN, with plus infinity or with nothing but minus infinity is
 // NaN, as a softmax of it is.
 //
-// Top alternatives: in order of (value, lowest index), NaN before numbers.  The first pass leaves every warp's (or, where
-// a warp has a row, every lane's) largest value; the top-th largest of those is at most the top-th largest value of the
-// row, and few values lie above it (about 32 H_32 - 32 H_(32 - top) on independent ones), so a second pass, out of L1 and
-// L2, collects what is not below it and ranks it.  Where a warp has a row it looks only at the vectors of lanes that have
+// Top alternatives: in order of (value, lowest index), NaN before numbers.  The first pass leaves the largest values of 32
+// groups (of a lane each where a warp has a row, else of 8 lanes or of a warp); the top-th largest of those is at most the
+// top-th largest value of the row, and few values lie above it (about 32 H_32 - 32 H_(32 - top) on independent ones), so a
+// second pass, out of L1 and L2, collects what is not below it and ranks it.  Where a warp has a row it looks only at the vectors of lanes that have
 // any (16384 rows of 2048 in bf16, top 8: 23.4 us, 28.9 with a second pass over the whole row), takes its floor from
 // every lane's two largest where the top are many and halves what is left (top 32: 42.9 us; 65.5 without the second
 // values, 104 without either).  Where ties or hostile orders leave more than there is room for, every warp keeps a sorted
@@ -20,8 +20,7 @@
 //
 // What bounds them, in bf16: the forward at 65536 x 2048 (51 us, 5.2 TB/s) its instructions, with 2^t on a unit of 16 a
 // clock taking 30 us alone; the backward there (80 us, 6.7 TB/s read and written) HBM; 16384 x 2048 without alternatives
-// 14.4 us; one row (4 us) the latency of two dependent reads of it and of a reduction over 32 warps.  A warp a row, with
-// no barrier, is the faster where rows are short and many; a long row needs more loads in flight than a warp has.
+// 14.4 us; one row of 2048 (2.6 us, with alternatives 4) the latency of a launch, of two dependent reads and of reductions.
 #include <math.h>
 
 #include "host_util.h"
@@ -251,13 +250,14 @@ DA_DEV float nth_largest(float first, float second, int top) {
   return x;
 }
 
-// kThreads a row: 32 (eight rows a CTA) or 1024.
+// kThreads a row: 32 (eight rows a CTA), 256 or 1024.
 template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads == 32 ? 256 : 1024, kThreads == 32 ? 6 : 1) forward_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads == 1024 ? 1024 : 256, kThreads == 1024 ? 1 : 6) forward_kernel(const Params p) {
   using V = Vec<T>;
   constexpr int kBatch = 4;  // loads in flight a thread, their largest value found together
   constexpr int kFound = kThreads == 32 ? 256 : 1024;  // entries that a row has room for
   __shared__ Sums sums[32];
+  __shared__ float groups[32];
   __shared__ uint64_t found_all[kThreads == 32 ? 8 : 1][kFound];
   __shared__ int counts[kThreads == 32 ? 8 : 1];
   __shared__ int lanes_all[kThreads == 32 ? 8 : 1][32];
@@ -307,13 +307,18 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : 1024, kThreads == 32 ? 
     }
     if (odd >= 0) s.add_one(x);
   }
-  float group = s.m;  // lane i: group i's largest value
+  float group = s.m;  // lane i: group i's largest value; a group is a lane, or 8 lanes, or a warp
+  if constexpr (kThreads == 256) {
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
+    if (lane % 8 == 0) groups[threadIdx.x / 8] = group;
+  }
   s.reduce();
   if constexpr (kThreads > 32) {
     if (lane == 0) sums[warp] = s;
     __syncthreads();
-    s = sums[lane];
-    group = s.m;
+    s = lane < kThreads / 32 ? sums[lane] : Sums{-INFINITY, 0.f, 0.f};
+    group = kThreads == 256 ? groups[lane] : s.m;
     s.reduce();
   }
   const float at = s.m == -INFINITY ? 0.f : s.m, log_l = log2f(s.l);
@@ -542,12 +547,19 @@ int check(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t V, co
   return DA_OK;
 }
 
-// A warp a row where rows are short and many, else a CTA of 1024 threads a row.
+// How many threads take a row.  In 16-byte pieces of a row (8 elements of 16 bits): 32 where there are rows enough for that,
+// pieces^2 / 312 (16384 x 2048 in bf16: 15 us with 32 threads, 63 with 256, 240 with 1024; 4096 x 8192: 20, 18, 91; 64 x 8192:
+// 6.8, 2.7, 4.0), and where 256 threads would not have a piece for each of top groups of 8 (64 x 500, top 20: 4.7, 12.6,
+// 11.4).  1024 for rows of more than 2048 pieces, two an SM at most (64 x 50021: 32, 6.3, 5.7; 600 x 50021: 33, 17, 24).
 template <typename T>
 int forward(const Params& p, cudaStream_t st) {
-  const bool warps = p.V <= 8192 && p.rows >= 4 * sm_count();
-  if (warps)
+  const int64_t pieces = p.V / Vec<T>::n;
+  const int threads = p.rows * 312 >= pieces * pieces || pieces < 8 * p.top  ? 32
+                      : pieces > 2048 && p.rows <= 2 * (int64_t)sm_count() ? 1024
+                                                                           : 256;
+  if (threads == 32)
     return launch_kernel(forward_kernel<T, 32>, dim3((unsigned)((p.rows + 7) / 8)), dim3(256), 0, st, false, p);
+  if (threads == 256) return launch_kernel(forward_kernel<T, 256>, dim3((unsigned)p.rows), dim3(256), 0, st, false, p);
   return launch_kernel(forward_kernel<T, 1024>, dim3((unsigned)p.rows), dim3(1024), 0, st, false, p);
 }
 

@@ -78,6 +78,26 @@ def test_rows_that_are_hard_to_rank(rows, dtype) -> None:
         _check(x.contiguous(), torch.arange(rows, device="cuda") % v, 32)
 
 
+@pytest.mark.parametrize(("rows", "v"), [(2000, 3001), (40, 3001), (40, 20001), (400, 20001), (3, 257), (20, 1999)])
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("top", [1, 9, 32])
+def test_alternatives_by_few_and_by_many_threads_a_row(rows, v, top, dtype) -> None:
+    x, tokens = _logits(rows, v, dtype, 21)
+    _check(x, tokens, top)
+    x[:, v // 3: v // 3 + 200] = 20.0   # more equal ones than the top, side by side
+    x[1::2, 5] = 21.0
+    _check(x, tokens, top)
+    x[:, ::2] = -math.inf
+    x[0, 1:] = -math.inf                 # fewer numbers than the top
+    x[0, 1] = 1.0
+    tokens[:] = 1
+    _check(x, tokens, top)
+    x[:, 7::11] = math.nan
+    made = da.token_log_probs(x, tokens, top=top)
+    want = torch.arange(7, v, 11, device="cuda")[:top]
+    assert torch.equal(made.top_tokens[:, :len(want)], want.expand(rows, -1)) and made.entropy.isnan().all()
+
+
 @pytest.mark.parametrize("rows", [6, 900])
 @pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
 def test_infinities_and_nan(rows, dtype) -> None:
