@@ -94,6 +94,7 @@ struct ChunkParams {
   int R, D, maps, group;
   int branch0[kMaxMaps];
   int brow, qrow;      // positions a box of keys or values, rows a box of queries
+  int pairs;           // CTA pairs that run side by side
   int phase;           // several maps: 1 sums, 2 outputs; one map: 0
   const float *scales, *weights;
   void* y;
@@ -106,12 +107,15 @@ struct ChunkParams {
 
 // ------------------------------------------------------------------------------------------------ plan
 constexpr int kPlanThreads = 256, kPlanWarps = kPlanThreads / 32, kLengths = 10, kEnds = 6;
+constexpr int kAtOnce = 1024;  // sequences
 
-// One CTA: a warp a sequence, a tile a lane.
+// One CTA; a warp a sequence, but for the sums over sequences.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const Plan plan, int few_most, int pairs) {
-  __shared__ int2 kept[1024];  // the first sequences' new tokens (of chunks), and tokens that they had
-  __shared__ unsigned long long units;
-  __shared__ int counts[kLengths], lengths[kLengths], carry[2], made[2], sums[2][kPlanWarps], best;
+  __shared__ int2 kept[kAtOnce];    // the first sequences' new tokens (of chunks), and tokens that they had
+  __shared__ int2 before[kAtOnce];  // tiles and pieces of a sequence, then of those before it
+  __shared__ unsigned long long units[kPlanWarps];
+  __shared__ long long sums[2][kPlanWarps];
+  __shared__ int counts[kLengths], made[2], several, best;
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -120,124 +124,167 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Cache c, const
     return make_int2(s.n > few_most ? s.n : 0, (int)s.held);
   };
   constexpr int nk_shift = 7;  // of kTile
-  for (int b = threadIdx.x; b < c.B && b < 1024; b += kPlanThreads) kept[b] = load(b);
+  for (int b = threadIdx.x; b < c.B && b < kAtOnce; b += kPlanThreads) kept[b] = load(b);
+  for (int b = threadIdx.x; b < c.B; b += kPlanThreads) plan.odd[b] = 0;
   if (threadIdx.x < kLengths) counts[threadIdx.x] = 0;
-  if (threadIdx.x == 0) {
-    units = 0;
-    carry[0] = carry[1] = made[0] = made[1] = 0;
-  }
+  if (threadIdx.x == 0) made[0] = made[1] = several = 0;
   __syncthreads();
-  auto get = [&](int b) { return b < 1024 ? kept[b] : load(b); };
+  auto get = [&](int b) { return b < kAtOnce ? kept[b] : load(b); };
   auto tiles_of = [](int2 s) { return (s.x + 127) >> 7; };
   auto keys_of = [&](int2 s, int i) {  // key tiles of query tile i
     const int64_t e = (int64_t)s.y + min(s.x, (i + 1) * 128);
     return (int)(((e < c.capacity ? e : c.capacity) + (1 << nk_shift) - 1) >> nk_shift);
   };
-  unsigned long long mine = 0;
+  unsigned long long all = 0;
   for (int b = warp; b < c.B; b += kPlanWarps) {
     const int2 s = get(b);
-    for (int i = lane; i < tiles_of(s); i += 32) mine += keys_of(s, i);
+    for (int i = lane; i < tiles_of(s); i += 32) all += keys_of(s, i);
   }
-  if (mine) atomicAdd(&units, mine);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  if (lane == 0) units[warp] = all;
   __syncthreads();
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWarps; ++w) all += units[w];
   // The pieces' length: of a few that suit one or two rounds of the CTA pairs, the one that is done first, counting a
-  // piece's start and end as kEnds key tiles.
-  if (threadIdx.x < kLengths) {
-    const int f = threadIdx.x, extra = 16 >> (f % 5 - 1 < 0 ? 0 : f % 5 - 1);  // none, a 16th, an 8th, a 4th, half more
-    const int64_t round = (int64_t)pairs * (f < 5 ? 1 : 2), base = ((int64_t)units + round - 1) / round;
+  // piece's start and end as kEnds key tiles.  Lane f + 10 k counts the pieces of the f-th in every third tile.
+  const int f = lane % kLengths, third = lane / kLengths;
+  int length;
+  {
+    const int extra = 16 >> (f % 5 - 1 < 0 ? 0 : f % 5 - 1);  // none, a 16th, an 8th, a 4th, half more
+    const int64_t round = (int64_t)pairs * (f < 5 ? 1 : 2), base = ((int64_t)all + round - 1) / round;
     const int64_t len = base + (f % 5 ? (base + extra - 1) / extra : 0);
-    lengths[f] = (int)(len < 1 ? 1 : len);
+    length = (int)(len < 1 ? 1 : len);
   }
-  __syncthreads();
-  int n[kLengths];
-#pragma unroll
-  for (int f = 0; f < kLengths; ++f) n[f] = 0;
+  int n = 0;
   for (int b = warp; b < c.B; b += kPlanWarps) {
     const int2 s = get(b);
-    for (int i = lane; i < tiles_of(s); i += 32) {
-      const unsigned t = keys_of(s, i);
-#pragma unroll
-      for (int f = 0; f < kLengths; ++f) {
-        const unsigned len = lengths[f];
-        n[f] += (t + len - 1) / len;
-      }
-    }
+    if (third < 3)
+      for (int i = third; i < tiles_of(s); i += 3) n += ((unsigned)keys_of(s, i) + length - 1) / (unsigned)length;
   }
+  if (n) atomicAdd(&counts[f], n);
+  __syncthreads();
+  if (warp == 0) {
+    const int64_t cost = (int64_t)((counts[f] + pairs - 1) / pairs) * (length + kEnds);
+    int64_t least = cost;
 #pragma unroll
-  for (int f = 0; f < kLengths; ++f) {
-    n[f] = __reduce_add_sync(0xffffffffu, n[f]);
-    if (lane == 0 && n[f]) atomicAdd(&counts[f], n[f]);
+    for (int o = 16; o; o >>= 1) least = min(least, (int64_t)__shfl_xor_sync(0xffffffffu, (long long)least, o));
+    const int from = __ffs(__ballot_sync(0xffffffffu, cost == least)) - 1;
+    if (lane == from) best = length;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int64_t least = INT64_MAX;
-    for (int f = 0; f < kLengths; ++f) {
-      const int64_t cost = (int64_t)((counts[f] + pairs - 1) / pairs) * (lengths[f] + kEnds);
-      if (cost < least) {
-        least = cost;
-        best = lengths[f];
+  // tiles and pieces in order
+  constexpr long long kMost = 1 << 30;  // (of starts that do not rise: no plan has room for as many)
+  long long tiles_before = 0, pieces_before = 0;
+  for (int base = 0; base < c.B; base += kAtOnce) {
+    const int at_once = min(c.B - base, kAtOnce);
+    for (int k = warp; k < at_once; k += kPlanWarps) {
+      const int2 s = get(base + k);
+      const int tiles = tiles_of(s);
+      int count = 0;
+      for (int i = lane; i < tiles; i += 32) count += (unsigned)(keys_of(s, i) + best - 1) / (unsigned)best;
+      count = __reduce_add_sync(0xffffffffu, count);
+      if (lane == 0) before[k] = make_int2(tiles, count);
+    }
+    __syncthreads();
+    {  // four sequences a thread
+      constexpr int kEach = kAtOnce / kPlanThreads;
+      int2 own[kEach];
+      long long t = 0, m = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int k = threadIdx.x * kEach + i;
+        own[i] = k < at_once ? before[k] : make_int2(0, 0);
+        t += own[i].x;
+        m += own[i].y;
       }
-    }
-  }
-  __syncthreads();
-  // tiles and pieces in order: a warp a sequence, a turn's sequences side by side
-  for (int base = 0; base < c.B; base += kPlanWarps) {
-    const int b = base + warp;
-    const int2 s = b < c.B ? get(b) : make_int2(0, 0);
-    const int tiles = tiles_of(s);
-    int count = 0;
-    for (int i = lane; i < tiles; i += 32) count += (unsigned)(keys_of(s, i) + best - 1) / (unsigned)best;
-    count = __reduce_add_sync(0xffffffffu, count);
-    if (lane == 0) {
-      sums[0][warp] = tiles;
-      sums[1][warp] = count;
-    }
-    __syncthreads();
-    const int t = lane < kPlanWarps ? sums[0][lane] : 0, k = lane < kPlanWarps ? sums[1][lane] : 0;
-    int tile0 = carry[0] + __reduce_add_sync(0xffffffffu, lane < warp ? t : 0);
-    int piece0 = carry[1] + __reduce_add_sync(0xffffffffu, lane < warp ? k : 0);
-    __syncthreads();
-    if (threadIdx.x == kPlanThreads - 1) {
-      carry[0] = tile0 + tiles;
-      carry[1] = piece0 + count;
-    }
-    if (b < c.B && lane == 0) plan.odd[b] = 0;
-    __syncwarp();
-    const Sequence whole = sequence(c, b < c.B ? b : 0);
-    for (int i0 = 0; i0 < tiles; i0 += 32) {
-      const int i = i0 + lane, keys = i < tiles ? keys_of(s, i) : 0, own = (unsigned)(keys + best - 1) / (unsigned)best;
-      int at = own;
+      long long ts = t, ms = m;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, at, o);
-        if (lane >= o) at += u;
-      }
-      const int all = __shfl_sync(0xffffffffu, at, 31), first = piece0 + at - own;
-      // (starts that do not rise bring more tokens than there are rows: what the plan has no room for is the other kernel's)
-      const bool fits = i < tiles && tile0 + i < plan.tiles_most && first + own <= plan.pieces_most;
-      if (fits) plan.tile_piece[tile0 + i] = first;
-      if (i < tiles && !fits) plan.odd[b] = 1;
-      if (fits) {
-        atomicMax(&made[0], tile0 + i + 1);
-        atomicMax(&made[1], first + own);
-      }
-      // (a tile's pieces side by side: the warp writes one tile after another, a piece a lane)
-      for (int j = 0; j < min(32, tiles - i0); ++j) {
-        const int from = __shfl_sync(0xffffffffu, first, j), many = __shfl_sync(0xffffffffu, fits ? own : 0, j);
-        const int last = __shfl_sync(0xffffffffu, keys, j);
-        for (int m = lane; m < many; m += 32) {
-          plan.pieces[3 * (from + m)] = make_int4(b, i0 + j, m * best, min(best, last - m * best));
-          plan.pieces[3 * (from + m) + 1] = make_int4(from, many, whole.n, whole.fits);
-          plan.pieces[3 * (from + m) + 2] = make_int4((int)whole.first, (int)whole.held, 0, 0);
+        const long long u = __shfl_up_sync(0xffffffffu, ts, o), v = __shfl_up_sync(0xffffffffu, ms, o);
+        if (lane >= o) {
+          ts += u;
+          ms += v;
         }
       }
-      piece0 += all;
+      if (lane == 31) {
+        sums[0][warp] = ts;
+        sums[1][warp] = ms;
+      }
+      __syncthreads();
+      t = tiles_before + ts - t;
+      m = pieces_before + ms - m;
+#pragma unroll
+      for (int w = 0; w < kPlanWarps; ++w) {
+        if (w < warp) {
+          t += sums[0][w];
+          m += sums[1][w];
+        }
+        tiles_before += sums[0][w];
+        pieces_before += sums[1][w];
+      }
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int k = threadIdx.x * kEach + i;
+        if (k < at_once) before[k] = make_int2((int)min(t, kMost), (int)min(m, kMost));
+        t += own[i].x;
+        m += own[i].y;
+      }
+    }
+    __syncthreads();
+    for (int k = warp; k < at_once; k += kPlanWarps) {
+      const int b = base + k;
+      const int2 s = get(b);
+      const int tiles = tiles_of(s), tile0 = before[k].x;
+      if (tiles == 0) continue;
+      int piece0 = before[k].y;
+      const Sequence whole = sequence(c, b);
+      for (int i0 = 0; i0 < tiles; i0 += 32) {
+        const int i = i0 + lane, keys = i < tiles ? keys_of(s, i) : 0, own = (unsigned)(keys + best - 1) / (unsigned)best;
+        int at = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, at, o);
+          if (lane >= o) at += u;
+        }
+        const int more = __shfl_sync(0xffffffffu, at, 31), first = piece0 + at - own;
+        // (starts that do not rise bring more tokens than there are rows: what the plan has no room for is the other kernel's)
+        const bool fits = i < tiles && tile0 + i < plan.tiles_most && first + own <= plan.pieces_most;
+        if (fits) plan.tile_piece[tile0 + i] = first;
+        if (i < tiles && !fits) plan.odd[b] = 1;
+        if (fits) {
+          atomicMax(&made[0], tile0 + i + 1);
+          atomicMax(&made[1], first + own);
+          if (own > 1) several = 1;
+        }
+        const int4 tokens = make_int4((int)whole.first, (int)whole.held, 0, 0);
+        if (__all_sync(0xffffffffu, own <= 1)) {  // a piece a tile: a lane each
+          if (fits && own) {
+            plan.pieces[3 * first] = make_int4(b, i, 0, keys);
+            plan.pieces[3 * first + 1] = make_int4(first, 1, whole.n, whole.fits);
+            plan.pieces[3 * first + 2] = tokens;
+          }
+        } else {
+          // (a tile's pieces side by side: the warp writes one tile after another, a piece a lane)
+          for (int j = 0; j < min(32, tiles - i0); ++j) {
+            const int from = __shfl_sync(0xffffffffu, first, j), many = __shfl_sync(0xffffffffu, fits ? own : 0, j);
+            const int last = __shfl_sync(0xffffffffu, keys, j);
+            for (int m = lane; m < many; m += 32) {
+              plan.pieces[3 * (from + m)] = make_int4(b, i0 + j, m * best, min(best, last - m * best));
+              plan.pieces[3 * (from + m) + 1] = make_int4(from, many, whole.n, whole.fits);
+              plan.pieces[3 * (from + m) + 2] = tokens;
+            }
+          }
+        }
+        piece0 = (int)min((long long)piece0 + more, kMost);
+      }
     }
     __syncthreads();
   }
   if (threadIdx.x == 0) {
     plan.tile_piece[made[0]] = made[1];
-    *reinterpret_cast<int4*>(plan.head) = make_int4(made[1], made[0], 0, 0);
+    *reinterpret_cast<int4*>(plan.head) = make_int4(made[1], made[0], several, 0);
   }
 }
 
@@ -277,6 +324,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   const Shape& L = p.shape;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_ctarank() & 1u;
+  const int piece = blockIdx.x / 2;  // (the plan has room for every CTA pair's piece)
+  if (piece >= p.pairs) {  // behind the first round there is no launch to overlap with, but pieces that a plan of the most has
+    grid_dependency_wait();
+    if (piece >= p.plan.head[0]) return;
+  }
   if (threadIdx.x == 0) {
     abort_flag = bad_flag = 0;
     mbar_init(&q_full, 1);
@@ -316,7 +368,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 
   grid_dependency_wait();  // the plan and the appended tokens are visible from here on
   grid_launch_dependents();
-  const int piece = blockIdx.x / 2;  // (the plan has room for every CTA pair's piece)
   const int4 here = p.plan.pieces[3 * piece], tile = p.plan.pieces[3 * piece + 1], seq = p.plan.pieces[3 * piece + 2];
   const bool on = piece < p.plan.head[0];
   const int t0 = here.y * 128;  // first token of the tile in its sequence
@@ -863,13 +914,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   if (warp == 1) tmem_dealloc<2>(tmem, L.tmem_cols);
 }
 
-// Adds the pieces of the tiles that have several: a warp takes 128 columns of a row.
+// Adds the pieces of a tile that has several: a warp takes 128 columns of a row.
 template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const ChunkParams p, const bool weighted) {
-  grid_dependency_wait();
-  grid_launch_dependents();
-  if ((int)blockIdx.x >= p.plan.head[1]) return;
-  const int first = p.plan.tile_piece[blockIdx.x], pieces = p.plan.tile_piece[blockIdx.x + 1] - first;
+DA_DEV void join_tile(const ChunkParams& p, const bool weighted, int index) {
+  const int first = p.plan.tile_piece[index], pieces = p.plan.tile_piece[index + 1] - first;
   if (pieces < 2) return;
   const int4 here = p.plan.pieces[3 * first], tile = p.plan.pieces[3 * first + 1], seq = p.plan.pieces[3 * first + 2];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, parts = p.D / 128;
@@ -921,6 +969,15 @@ __global__ void __launch_bounds__(256) join_kernel(const ChunkParams p, const bo
   *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(o.x * f, o.y * f), pack2<T>(o.z * f, o.w * f));
 }
 
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const ChunkParams p, const bool weighted) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int4 head = *reinterpret_cast<const int4*>(p.plan.head);
+  if (!head.z) return;
+  for (int tile = blockIdx.x; tile < head.y; tile += gridDim.x) join_tile<T>(p, weighted, tile);
+}
+
 // ------------------------------------------------------------------------------------------------ host
 namespace {
 
@@ -952,6 +1009,7 @@ int run(const ChunkArgs& a, cudaStream_t st) {
   p.D = a.D;
   p.group = a.group;
   p.status = a.status;
+  p.pairs = sm_count() / 2;
   const bool mix = a.maps > 1 && !a.per_map;
   p.maps = mix ? a.maps : 1;
   const bool repeated = p.maps > a.H;
@@ -1009,7 +1067,10 @@ int run(const ChunkArgs& a, cudaStream_t st) {
       if (int rc = map_keys(L.wide)) return rc;
       if (int rc = launch_kernel(chunk_kernel<T, false>, grid, block, L.smem, st, true, tq, tk, tv, p)) return rc;
     }
-    if (int rc = launch_kernel(join_kernel<T>, dim3((unsigned)tiles, (unsigned)(16 * a.D / 128)), dim3(256), 0, st, false, p, !mix)) return rc;
+    const int64_t rows = 16 * a.D / 128, side = 8 * (int64_t)sm_count() / rows + 1;  // (as many CTAs as run side by side)
+    if (int rc = launch_kernel(join_kernel<T>, dim3((unsigned)(tiles < side ? tiles : side), (unsigned)rows), dim3(256), 0, st,
+                               false, p, !mix))
+      return rc;
   }
   return DA_OK;
 }

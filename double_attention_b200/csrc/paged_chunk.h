@@ -6,7 +6,7 @@
 namespace da {
 namespace paged {
 
-// The chunk kernel's plan, made on the device from the step's lengths: `head` is {pieces, tiles, 0, 0}; tile k, of 128 new
+// The chunk kernel's plan, made on the device from the step's lengths: `head` is {pieces, tiles, whether a tile has several pieces, 0}; tile k, of 128 new
 // tokens, has the pieces tile_piece[k] .. tile_piece[k + 1]; piece i is {sequence, tile of the sequence, first key tile, key
 // tiles}, {first piece of its tile, pieces of its tile, the sequence's new tokens, whether the table holds it} and {its
 // first packed row, tokens that it had, 0, 0}.  odd[b] says that live rows of sequence b came out NaN.
