@@ -53,7 +53,7 @@ struct FewParams {
   int H, R, D, maps, group, lanes;  // lanes: maps rounded up to a power of two
   int job_rows;                     // 16, or 8: job_rows / lanes tokens a job
   int few_most;                     // sequences with more new tokens are another kernel's
-  int few_rows, slice;              // combine_kernel's rows a sequence, columns a CTA: 64 or 16
+  int few_rows, slice;              // combine_kernel's rows a sequence, columns a CTA: D, 64 or 16
   int stages, stage_bytes, key_bytes, brow;
   int ctas;
   int per_map, zero_rest;
@@ -725,7 +725,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
 constexpr int kMaxPieces = 512;
 struct Joining {
   float w[4][kMaxPieces], l[4][kMaxPieces];  // each map's weights and sums of the pieces
-  float4 o[8][16];                           // each warp's part of the columns
+  float4 o[256];                             // the columns' sums of each warp's, or each turn's, pieces
 };
 
 // One packed row's p.slice columns from its pieces c0, c0 + 1, ...: the first in slot `slot0`, the later ones, which open
@@ -775,17 +775,18 @@ DA_DEV void join(const FewParams& p, int64_t row, int t, int c0, int pieces, int
       o.w = fmaf(w, v.w, o.w);
     }
     if (!p.per_map && m + 1 < p.maps) continue;
-    for (int k = across; k < 32; k <<= 1) {
+    for (int k = across; k < 32; k <<= 1) {  // (the lanes of a warp that have the same columns)
       o.x += __shfl_xor_sync(0xffffffffu, o.x, k);
       o.y += __shfl_xor_sync(0xffffffffu, o.y, k);
       o.z += __shfl_xor_sync(0xffffffffu, o.z, k);
       o.w += __shfl_xor_sync(0xffffffffu, o.w, k);
     }
-    if (lane < across) j.o[warp][lane] = o;
+    if (across >= 32) j.o[tid] = o;
+    else if (lane < across) j.o[warp * across + lane] = o;
     __syncthreads();
     if (tid < across) {
-      for (int i = 1; i < 8; ++i) {
-        const float4 v = j.o[i][tid];
+      for (int i = 1; i < min(8, parts); ++i) {
+        const float4 v = j.o[i * across + tid];
         o.x += v.x;
         o.y += v.y;
         o.z += v.z;
@@ -986,7 +987,10 @@ extern "C" int da_paged_attn(const void* q, int64_t q_branch_stride, int64_t q_r
   p.chunked = chunked;
   if (chunked) p.chunks = paged::chunk_plan(workspace, tokens, B, p.few_most);
   p.few_rows = f.few_rows < p.few_most ? f.few_rows : p.few_most;
-  p.slice = (int64_t)p.c.B * p.few_rows * (D / 64) >= sm_count() ? 64 : 16;
+  // The join, D 512: whole rows where sequences are many and so have few pieces each (128 sequences of 250 to 500, 4 tokens:
+  // the call takes 34 us, 50 by 64 columns), narrower slices where few rows have many (one of 32000: 37 and 21 us).
+  const int64_t rows = (int64_t)p.c.B * p.few_rows;
+  p.slice = B >= 32 ? D : rows * (D / 64) >= sm_count() ? 64 : 16;
   p.stages = f.stages;
   p.stage_bytes = f.stage_bytes;
   p.key_bytes = f.key_bytes;
