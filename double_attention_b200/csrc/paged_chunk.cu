@@ -782,10 +782,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         if (any) {  // the outputs so far, once the products into them are done: tile j - 1's
           const float c = rescale ? ex2(ref - next) : 1.f;
           sum *= c;
-          // (its buffer's products before those, tile j - 3's, may be under way still: a wait for the later ones alone would
-          // end at once then)
+          // (its buffer's products before those, tile j - 3's, may be under way still, and a wait for the later ones would end
+          // at once then; those of the group's own tile j - 2 come after them and cannot be two phases on)
           const uint32_t done = group ? p_phase ^ 1u : p_phase;
-          if (ok && j >= 3) ok = mbar_wait(&p_empty[group ^ 1], done ^ 1u, ab, 80);
+          if (ok && j >= 2) ok = mbar_wait(&p_empty[group], p_phase, ab, 80);
           if (ok) ok = mbar_wait(&p_empty[group ^ 1], done, ab, 80);
           ok = __all_sync(0xffffffffu, ok);
           if (ok) {

@@ -474,3 +474,13 @@ def test_refusals() -> None:
     with pytest.raises(RuntimeError, match="no backward"):
         da.append_paged(case.k, case.v.clone().requires_grad_(), case.key_pages, case.value_pages, case.batch)
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize(("dims", "held", "new"), [((2, 1, 256, 256, 16), [1099] * 9, [176] * 9), ((1, 1, 256, 512, 64), [9000], [300]),
+                                                   ((2, 1, 256, 512, 32), [30000], [73])])
+def test_a_maximum_that_grows_at_any_tile(dims, held, new) -> None:
+    """Scores so far apart that rows' maxima grow by much at late tiles too, whose products the two groups wait for."""
+    case = Case(*dims, BF16, held, new, scale=1000.0)
+    case.append()
+    for _ in range(3):
+        case.check(case.attend())
