@@ -21,7 +21,8 @@
 // that a tile's scores overlap the outputs of the one before.  (Eight warps doing both in turn: 192 us at 64 sequences of up to
 // 8192, against 107.)  The products are 16 x 8 x 16 instructions: 16 rows fill them, and 128-row ones
 // would spend 8 times the work on rows that do not exist.  Weights go in as two 16-bit parts, for an error of the output's own
-// rounding and nothing else (1.7e-3 in bf16 against 64 bits; one part 2.3e-3).
+// rounding (1.7e-3 in bf16 against 64 bits; one part 2.3e-3); in fp16 also of 2^-32 of the row's largest weight a key, half its
+// smallest step (kLift).
 //
 // Measured (bf16, 512 value columns, joining included): 64 sequences of 4096 to 8192, 256 key columns, 609 MB, 104 us, 5.9
 // TB/s, where a copy's rate would take 93 us; one sequence of 131072, 512 key columns, 268 MB, 56.4 us, 4.8 TB/s: two launches,
@@ -41,6 +42,10 @@ constexpr int kThreads = 32 * (kScoreWarps + kValueWarps + 1);
 constexpr int kMaxStages = 8;
 constexpr int kPPitch = 40;    // 16-bit weights a row
 constexpr float kGrow = 8.f;   // log2 of the growth of a row's maximum that its output bears
+// log2 by which weights are larger than 2^(score - offset): fp16 has nothing below 2^-24, so a far tail of small weights would
+// count in the fp32 sum and not in the product.  Up to 2^(kGrow + 7) = 2^15 they still fit.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
 
 struct FewParams {
   Cache c;
@@ -493,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) few_kernel(const __grid_const
           c1 = ref1 == -INFINITY ? 1.f : ex2(ref1 - top1);
           ref1 = top1;
         }
-        const float off0 = ref0 == -INFINITY ? 0.f : ref0, off1 = ref1 == -INFINITY ? 0.f : ref1;
+        const float off0 = ref0 == -INFINITY ? 0.f : ref0 - kLift<T>, off1 = ref1 == -INFINITY ? 0.f : ref1 - kLift<T>;
         const float p00 = ex2(v00 - off0), p01 = ex2(v01 - off0), p10 = ex2(v10 - off1), p11 = ex2(v11 - off1);
         l0 = fmaf(l0, c0, p00 + p01);
         l1 = fmaf(l1, c1, p10 + p11);

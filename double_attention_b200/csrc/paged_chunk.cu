@@ -42,6 +42,11 @@ constexpr int kMaxK = 8, kMaxV = 4;        // most stages
 constexpr int kScores = 4, kWeights = 2;  // buffers of scores, two a group of softmax warps, and of weights, one a group
 constexpr int kSmem = 224 * 1024;
 constexpr float kGrow = 8.f;  // log2 of the growth of a row's maximum that its outputs bear
+// log2 by which weights are larger than their offsets make them: fp16 has nothing below 2^-24, so a far tail, or a flat map
+// beside a sharp one, would count in the fp32 sums and not in the product.  One map's reach 2^(kGrow + 7) = 2^15, four maps',
+// of at most 1 each, 4 x 2^13.
+template <typename T, bool kMix>
+constexpr float kLift = std::is_same<T, __half>::value ? (kMix ? 13.f : 7.f) : 0.f;
 
 // A CTA's shared memory.  Paired loads take about 0.9 us from a stage's release to its next tile, in which a pair of
 // tensor cores consumes about 2000 cycles' worth: rings of 64 KB and more for keys and values keep them fed.
@@ -686,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           named_bar_sync(1, 32 * kSoftmaxWarps);
         }
       } else {
-        // ---- the pieces' sums of this row; offsets so that the mixture's largest weight is near 1
+        // ---- the pieces' sums of this row; offsets so that the mixture's largest weight is near 1 (2^13 in fp16)
         // (the row's eight threads share them out: a map and every other piece each)
         float off[kMaxMaps], al[kMaxMaps], shift = -INFINITY;
         {
@@ -725,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             shift = fmaxf(shift, log2f(fabsf(al[i])) - log_sum);
           }
         }
-        shift = fminf(fmaxf(shift, -100.f), 100.f);
+        shift = fminf(fmaxf(shift, -100.f), 100.f) - kLift<T, true>;
         factor = ex2(shift);
 #pragma unroll
         for (int s = 0; s < kMaxMaps; ++s) off[s] += shift;
@@ -803,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           }
         }
         ref = next;
-        const float at = ref == -INFINITY ? 0.f : ref;
+        const float at = ref == -INFINITY ? 0.f : ref - kLift<T, false>;
         float a = 0.f, b = 0.f;
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
