@@ -492,6 +492,11 @@ __global__ void __launch_bounds__(256) backward_kernel(const BackwardParams p) {
   };
   constexpr int kVecs = kSegment / V::n, kBatch = 4;
   const int v0 = seg * kVecs, v1 = min(row.vecs, v0 + kVecs);
+  if (token == kIgnore && h == 0.f) {  // zeros, whatever the row holds
+    for (int i = row.index(v0) + lane; i < row.index(v1); i += 32) out[i] = T(0.f);
+    if (seg == 0 && row.odd(lane) >= 0) out[row.odd(lane)] = T(0.f);
+    return;
+  }
   const F2 scale = dup(kLog2e), at_m = dup(-st.x), at_l = dup(-st.y), hs = dup(-h), cs = dup(-c);
   for (int v = v0 + lane; v < v1; v += 32 * kBatch) {
     uint4 raw[kBatch];

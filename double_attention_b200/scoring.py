@@ -90,7 +90,7 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, top: int = 0) -> TokenLog
 
     logits in fp32, bf16 or fp16, any strides; all sums in fp32.  Entries of minus infinity have probability 0; a row
     with a NaN, with plus infinity or with no finite entry is NaN.  A token of -100 has log probability 0 and passes no
-    gradient; any other outside [0, V) is NaN.  ``top`` at most 32; NaN comes before numbers there.
+    gradient, whatever its row holds; any other outside [0, V) is NaN.  ``top`` at most 32; NaN comes before numbers there.
 
     Differentiable in ``logits`` through ``log_probs`` and ``entropy`` (the alternatives carry no gradient)."""
     name = "token_log_probs"

@@ -594,7 +594,8 @@ DA_API int da_token_log_probs(const void* logits, int dtype, int64_t ld, int64_t
                               int top, float* log_probs, float* entropy, float* top_log_probs, int64_t* top_tokens,
                               float* stats, void* stream);
 /* d_logits[r, i] = d_log_probs[r] ([i = token] - p_i) - d_entropy[r] p_i (log p_i + entropy[r]) in dtype, row stride
- * ldd; either of d_log_probs and d_entropy may be null (zeros). */
+ * ldd; either of d_log_probs and d_entropy may be null (zeros).  A row of the token -100 whose d_entropy is 0 gets
+ * zeros, whatever it holds. */
 DA_API int da_token_log_probs_bwd(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t V, const int64_t* tokens,
                                   const float* stats, const float* entropy, const float* d_log_probs,
                                   const float* d_entropy, void* d_logits, int64_t ldd, void* stream);
