@@ -744,13 +744,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             float v[32];
             take(v);
             if (!ok) continue;
-            hide(v, lim);
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const float e = ex2(fmaf(v[i], scale[s], -off[s]));
               pm[i] = s == 0 ? al[0] * e : fmaf(al[s], e, pm[i]);
             }
           }
+          // (a temperature may have any sign: a hidden key's weight is set, not made by a score of minus infinity)
+          if (!__all_sync(0xffffffffu, lim == 32))
+#pragma unroll
+            for (int i = 0; i < 32; ++i) pm[i] = i < lim ? pm[i] : 0.f;
           give(pm);
         }
       }
