@@ -105,6 +105,7 @@ DA_DEV Cut cut(const FewParams& p) {
   c.total = __shfl_sync(0xffffffffu, inc, 31);
   c.share = share_of(c.total, p.ctas);
   c.pieces = c.pieces_ahead = 0;
+  if (c.total == 0) return c;  // (all sequences are the chunk kernel's: no share to divide by)
   const int job = c.tiles ? job_tiles(p.c, c.s) : 1;
   const int64_t jobs = c.total < 0x7fffffff ? (uint32_t)c.tiles / (uint32_t)job : c.tiles / job;
   if (!__all_sync(0xffffffffu, jobs <= p.ctas)) return c;

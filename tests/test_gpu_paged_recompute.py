@@ -52,3 +52,12 @@ def test_a_later_value_that_is_no_number_has_its_sequence_computed_again() -> No
     case.v[199, 7] = math.nan
     case.append()
     assert _spoilt(case) == [1, 0]
+
+
+@pytest.mark.parametrize("sequences", [1, 2, 31, 32])
+def test_chunks_alone_leave_the_other_kernel_the_rows_of_no_sequence(sequences) -> None:
+    case = Case(1, 1, 64, 128, 16, BF16, [b % 5 for b in range(sequences)], [17 + b for b in range(sequences)], seed=23, behind=9)
+    case.append()
+    y = case.attend()
+    case.check(y)
+    assert not y[sum(case.new):].any()
