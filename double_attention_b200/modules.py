@@ -30,6 +30,7 @@ from .config import DoubleAttentionConfig
 # projection GEMM over the concatenated weights; the flag is kept for
 # compatibility and selects the same computation either way.
 FUSED_QUERY_KEY_PROJECTION = True
+_ATTENTION_ROWS = 64  # rows (batch times length) that the attention kernels take at least: a box of values
 
 
 class NormalizedDictionary(tuple):
@@ -427,4 +428,9 @@ class DoubleAttentionLM(nn.Module):
         of its distribution and its ``top`` likeliest tokens: [B, T - 1].  Differentiable (see :func:`token_log_probs`)."""
         if token_ids.ndim != 2 or token_ids.shape[1] < 2:
             raise ValueError("token_ids must have shape [B, T] with T at least 2")
-        return token_log_probs(self(token_ids[:, :-1])[0], token_ids[:, 1:], top=top)
+        ids, batch = token_ids[:, :-1], token_ids.shape[0]
+        # sequences of the token 0 beside them, which change nothing of theirs, fill the attention's smallest tile
+        short = -(-_ATTENTION_ROWS // ids.shape[1]) - batch
+        if short > 0:
+            ids = F.pad(ids, (0, 0, 0, short))
+        return token_log_probs(self(ids)[0][:batch], token_ids[:, 1:], top=top)
