@@ -224,7 +224,8 @@ class RoutedCache:
         self.key_pages = torch.zeros(layers, pages, page_size, *shape, dtype=dtype, device=device)
         self.value_pages = torch.zeros(layers, pages, page_size, config.model_dim, dtype=dtype, device=device)
         self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
-        self.table = torch.zeros(sequences, columns, dtype=torch.int32, device=device)
+        # (-1 where a sequence has no page: a step that was not reserved is reported, and writes nothing)
+        self.table = torch.full((sequences, columns), -1, dtype=torch.int32, device=device)
         self._owned: list[list[int]] = [[] for _ in range(sequences)]
         self._free = list(range(pages - 1, -1, -1))
         self._held = [0] * sequences  # the lengths as the host knows them
@@ -279,6 +280,7 @@ class RoutedCache:
             if not self._fixed:
                 self._free += reversed(self._owned[b])
                 self._owned[b] = []
+                self.table[b] = -1
 
     def rows(self, token_ids: Tensor, counts: Sequence[int] | None, positions: int) -> tuple[Tensor, list[int]]:
         """The packed ids of a step and its counts, checked against a model of ``positions`` positions: ids [B, T], or [N]

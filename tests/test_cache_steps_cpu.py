@@ -1,0 +1,41 @@
+"""Steps of a cache that nobody reserved, without a GPU: which pages the table names."""
+
+from __future__ import annotations
+
+import torch
+
+import double_attention_b200 as da
+from double_attention_b200 import experiment_config
+
+
+def _cache(**kw) -> da.RoutedCache:
+    return da.RoutedCache(experiment_config("qk4-s4"), 2, 3, 100, device="cpu", page_size=16, **kw)
+
+
+def _named(cache: da.RoutedCache) -> list[list[int]]:
+    """Pages that each sequence's row of the table names."""
+    return [[page for page in row if page >= 0] for row in cache.table.tolist()]
+
+
+def test_a_shared_table_names_nothing_but_a_sequences_own_pages() -> None:
+    cache = _cache(pages=9)
+    assert _named(cache) == [[], [], []]
+    cache.advance([33, 1, 0], cache.step([33, 1, 0]))
+    first, second, third = _named(cache)
+    assert (len(first), len(second), len(third)) == (3, 1, 0) and len({*first, *second}) == 4
+    assert cache.table[0, 3:].eq(-1).all()
+    cache.release(0)
+    assert _named(cache) == [[], second, []]
+    cache.advance([0, 0, 80], cache.step([0, 0, 80]))
+    assert _named(cache)[0] == [] and len({*_named(cache)[2], *second}) == 6
+    cache.release()
+    assert cache.table.eq(-1).all()
+
+
+def test_sequences_with_pages_of_their_own_keep_them() -> None:
+    cache = _cache()
+    before = cache.table.clone()
+    assert sorted(before.flatten().tolist()) == list(range(21))
+    cache.release(1)
+    cache.release()
+    assert torch.equal(cache.table, before)

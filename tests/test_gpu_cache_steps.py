@@ -1,0 +1,64 @@
+"""Steps of a cache on the GPU that nobody reserved: reported, and nothing of another sequence is written."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from double_attention_b200 import DoubleAttentionLM, append_paged, experiment_config, ops, paged, routed_attention_paged
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def _lm(preset: str = "a1", positions: int = 400) -> DoubleAttentionLM:
+    torch.manual_seed(0)
+    return DoubleAttentionLM(512, positions, experiment_config(preset), 2, feedforward_dim=1536).cuda().eval()
+
+
+def _ids(batch: int, length: int, seed: int = 1) -> torch.Tensor:
+    return torch.randint(0, 512, (batch, length), device="cuda", generator=torch.Generator("cuda").manual_seed(seed))
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_step_past_a_sequences_pages_writes_nothing(new) -> None:
+    """A batch used for a second step, whose tokens no page was reserved for."""
+    config = experiment_config("a1")
+    cache = paged.RoutedCache(config, 1, 2, 400, page_size=16, pages=12)
+    cache.advance([32, 32], cache.step([32, 32]))  # two pages each, full
+    keys = torch.randn(1, 2 * new, config.routing_dim, device="cuda").to(BF16)
+    values = torch.randn(2 * new, 512, device="cuda").to(BF16)
+    starts = torch.tensor([0, new, 2 * new], dtype=torch.int32, device="cuda")
+    cache.table[1, 2:5] = torch.tensor([9, 10, 11], dtype=torch.int32)  # (the second sequence has pages for them)
+    batch = paged.PagedBatch(cache.table, cache.lengths, starts, new)
+    before = [t.clone() for t in cache.layer(0)]
+    append_paged(keys, values, *cache.layer(0), batch)
+    assert ops.device_status() == paged.BAD_PAGE
+    written = torch.zeros(12, dtype=torch.bool, device="cuda")
+    written[9:9 + -(-new // 16)] = True
+    for now, was in zip(cache.layer(0), before):
+        assert torch.equal(now[~written], was[~written]) and not torch.equal(now[written], was[written])
+    y = routed_attention_paged(keys, *cache.layer(0), batch, torch.tensor([16.0], device="cuda"))
+    assert ops.device_status() == paged.BAD_PAGE
+    assert y[:new].isnan().all() and y[new:].isfinite().all()
+
+
+def test_a_released_sequences_pages_are_another_ones() -> None:
+    lm, ids = _lm(), _ids(2, 100)
+    with torch.no_grad(), torch.autocast("cuda", dtype=BF16):
+        cache = lm.new_cache(2, page_size=16, pages=7)
+        lm.extend(ids[0], cache, [100, 0])
+        cache.release(0)
+        want = lm.extend(ids[1], cache, [0, 100])
+        assert ops.device_status() == 0
+        # the first sequence's old entries lead nowhere
+        stale = paged.PagedBatch(cache.table, torch.tensor([50, 0], dtype=torch.int32, device="cuda"),
+                                 torch.tensor([0, 1, 1], dtype=torch.int32, device="cuda"), 1)
+        before = [t.clone() for t in cache.layer(0)]
+        key = torch.randn(1, 1, lm.stack.config.routing_dim, device="cuda").to(BF16)
+        append_paged(key, torch.randn(1, 512, device="cuda").to(BF16), *cache.layer(0), stale)
+        assert ops.device_status() == paged.BAD_PAGE
+        assert all(torch.equal(now, was) for now, was in zip(cache.layer(0), before))
+        cache.release()
+        again = lm.extend(ids[1], cache, [0, 100])
+    assert torch.equal(want, again)
