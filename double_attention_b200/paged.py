@@ -199,9 +199,10 @@ class RoutedCache:
     """The pages of all layers of a model for ``sequences`` sequences, and who has which.
 
     ``max_length`` positions a sequence.  Without ``pages`` every sequence owns its pages from the start, and a step
-    (``DoubleAttentionLM.extend``, ``Int8DoubleAttentionLM.extend``) can be captured into a CUDA graph: the device's
-    ``lengths`` advance with every replay.  With fewer ``pages`` sequences share a pool: a step takes what its new tokens
-    need and raises if there is none left; ``release`` gives a sequence's pages back.  Not for several threads at once."""
+    (``DoubleAttentionLM.extend``, ``Int8DoubleAttentionLM.extend``) of as many new tokens of every sequence can be captured into
+    a CUDA graph: the device's ``lengths`` advance with every replay.  With fewer ``pages`` sequences share a pool: a step takes
+    what its new tokens need and raises if there is none left; ``release`` gives a sequence's pages back.  A pool's steps cannot
+    be captured, as no replay would reserve pages.  Not for several threads at once."""
 
     def __init__(self, config, layers: int, sequences: int, max_length: int, *, page_size: int = 64, pages: int | None = None,
                  dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda") -> None:
@@ -239,10 +240,18 @@ class RoutedCache:
         """Key and value pages of one layer."""
         return self.key_pages[index], self.value_pages[index]
 
+    def _capturing(self) -> bool:
+        return self.table.is_cuda and torch.cuda.is_current_stream_capturing()
+
     def step(self, counts: Sequence[int]) -> PagedBatch:
         """The batch of a step that brings ``counts[b]`` new tokens of sequence b, its pages reserved."""
         if len(counts) != self.sequences or any(n < 0 for n in counts):
             raise ValueError(f"a step takes a number of new tokens for each of the {self.sequences} sequences, got {list(counts)}")
+        if self._capturing():
+            if not self._fixed:
+                raise RuntimeError("a step of a cache whose sequences share a pool cannot be captured: replays reserve no pages")
+            if any(n != counts[0] for n in counts):
+                raise RuntimeError(f"a captured step brings as many new tokens of every sequence, got {list(counts)}")
         for b, n in enumerate(counts):
             if self._held[b] + n > self.max_length:
                 raise ValueError(f"sequence {b} has {self._held[b]} tokens: {n} more exceed the cache's {self.max_length}")
@@ -274,6 +283,8 @@ class RoutedCache:
 
     def release(self, sequence: int | None = None) -> None:
         """Forgets a sequence's tokens, or all: its next step starts at position 0."""
+        if not self._fixed and self._capturing():
+            raise RuntimeError("pages given back to a pool cannot be captured: replays would give back others' pages")
         for b in range(self.sequences) if sequence is None else (sequence,):
             self._held[b] = 0
             self.lengths[b] = 0

@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import pytest
 import torch
 
 import double_attention_b200 as da
@@ -39,3 +40,19 @@ def test_sequences_with_pages_of_their_own_keep_them() -> None:
     cache.release(1)
     cache.release()
     assert torch.equal(cache.table, before)
+
+
+def test_no_captured_step_of_a_pool_and_none_of_uneven_counts(monkeypatch: pytest.MonkeyPatch) -> None:
+    pool, own = _cache(pages=9), _cache()
+    pool.advance([20, 1, 0], pool.step([20, 1, 0]))
+    monkeypatch.setattr(da.RoutedCache, "_capturing", lambda cache: True)
+    before = pool.table.clone()
+    for counts in ([1, 1, 1], [0, 0, 0]):
+        with pytest.raises(RuntimeError, match="share a pool"):
+            pool.step(counts)
+    with pytest.raises(RuntimeError, match="pool"):
+        pool.release(0)
+    assert torch.equal(pool.table, before) and pool.lengths.tolist() == [20, 1, 0]
+    with pytest.raises(RuntimeError, match="as many"):
+        own.step([1, 0, 1])
+    assert own.step([2, 2, 2]).starts.tolist() == [0, 2, 4, 6]

@@ -62,3 +62,25 @@ def test_a_released_sequences_pages_are_another_ones() -> None:
         cache.release()
         again = lm.extend(ids[1], cache, [0, 100])
     assert torch.equal(want, again)
+
+
+def test_steps_that_replays_cannot_follow_are_not_captured() -> None:
+    lm, ids = _lm(), _ids(2, 3)
+    with torch.no_grad(), torch.autocast("cuda", dtype=BF16, cache_enabled=False):
+        pool, own = lm.new_cache(2, page_size=16, pages=7), lm.new_cache(2)
+        lm.extend(ids, pool)
+        lm.extend(ids, own)
+        pool.release()
+        refused = []
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            for call in (lambda: lm.extend(ids, pool), lambda: pool.release(), lambda: lm.extend(ids[0], own, [1, 2])):
+                try:
+                    call()
+                except RuntimeError as error:
+                    refused.append(str(error))
+        assert len(refused) == 3 and "pool" in refused[0] and "pool" in refused[1] and "as many" in refused[2]
+        # (the capture went on, and the caches are as they were)
+        assert own.lengths.tolist() == [3, 3] and pool.lengths.tolist() == [0, 0]
+        want = lm.new_cache(2)
+        assert torch.equal(lm.extend(ids, pool), lm.extend(ids, want))
+    assert ops.device_status() == 0
