@@ -202,7 +202,8 @@ class RoutedCache:
     (``DoubleAttentionLM.extend``, ``Int8DoubleAttentionLM.extend``) of as many new tokens of every sequence can be captured into
     a CUDA graph: the device's ``lengths`` advance with every replay.  With fewer ``pages`` sequences share a pool: a step takes
     what its new tokens need and raises if there is none left; ``release`` gives a sequence's pages back.  A pool's steps cannot
-    be captured, as no replay would reserve pages.  Not for several threads at once."""
+    be captured, as no replay would reserve pages.  Once a step has been captured, every other one reads the lengths back from
+    the device first, and waits for it: replays have moved them.  Not for several threads at once."""
 
     def __init__(self, config, layers: int, sequences: int, max_length: int, *, page_size: int = 64, pages: int | None = None,
                  dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda") -> None:
@@ -230,6 +231,7 @@ class RoutedCache:
         self._owned: list[list[int]] = [[] for _ in range(sequences)]
         self._free = list(range(pages - 1, -1, -1))
         self._held = [0] * sequences  # the lengths as the host knows them
+        self._captured = False        # whether it may not, as replays move them
         if own:
             self.table.copy_(torch.arange(pages, dtype=torch.int32).view(sequences, columns))
             self._owned = [list(range(b * columns, (b + 1) * columns)) for b in range(sequences)]
@@ -243,6 +245,15 @@ class RoutedCache:
     def _capturing(self) -> bool:
         return self.table.is_cuda and torch.cuda.is_current_stream_capturing()
 
+    def _known_lengths(self) -> list[int]:
+        """The lengths that a step is checked against (none in a capture: its replays bring their own)."""
+        if self._capturing():
+            self._captured |= self._fixed
+            return [0] * self.sequences
+        if self._captured:
+            self._held = self.lengths.tolist()
+        return self._held
+
     def step(self, counts: Sequence[int]) -> PagedBatch:
         """The batch of a step that brings ``counts[b]`` new tokens of sequence b, its pages reserved."""
         if len(counts) != self.sequences or any(n < 0 for n in counts):
@@ -252,9 +263,10 @@ class RoutedCache:
                 raise RuntimeError("a step of a cache whose sequences share a pool cannot be captured: replays reserve no pages")
             if any(n != counts[0] for n in counts):
                 raise RuntimeError(f"a captured step brings as many new tokens of every sequence, got {list(counts)}")
+        lengths = self._known_lengths()
         for b, n in enumerate(counts):
-            if self._held[b] + n > self.max_length:
-                raise ValueError(f"sequence {b} has {self._held[b]} tokens: {n} more exceed the cache's {self.max_length}")
+            if lengths[b] + n > self.max_length:
+                raise ValueError(f"sequence {b} has {lengths[b]} tokens: {n} more exceed the cache's {self.max_length}")
         if not self._fixed:
             want = [max(0, -(-(held + n) // self.page_size) - len(owned))
                     for held, n, owned in zip(self._held, counts, self._owned)]
@@ -279,12 +291,15 @@ class RoutedCache:
     def advance(self, counts: Sequence[int], batch: PagedBatch) -> None:
         """Counts a step's tokens in, after its last layer."""
         self.lengths.add_(batch.starts[1:] - batch.starts[:-1])
-        self._held = [held + n for held, n in zip(self._held, counts)]
+        if not self._capturing():
+            self._held = [held + n for held, n in zip(self._held, counts)]
 
     def release(self, sequence: int | None = None) -> None:
         """Forgets a sequence's tokens, or all: its next step starts at position 0."""
-        if not self._fixed and self._capturing():
-            raise RuntimeError("pages given back to a pool cannot be captured: replays would give back others' pages")
+        if self._capturing():
+            if not self._fixed:
+                raise RuntimeError("pages given back to a pool cannot be captured: replays would give back others' pages")
+            self._captured = True
         for b in range(self.sequences) if sequence is None else (sequence,):
             self._held[b] = 0
             self.lengths[b] = 0
@@ -304,9 +319,9 @@ class RoutedCache:
             numbers = [int(n) for n in counts]
             if token_ids.ndim != 1 or token_ids.shape[0] != sum(numbers):
                 raise ValueError(f"token_ids must have shape [{sum(numbers)}], one sequence after another, got {tuple(token_ids.shape)}")
-        for b, n in enumerate(numbers[:self.sequences]):
-            if self._held[b] + n > positions:
-                raise ValueError(f"sequence length {self._held[b] + n} exceeds configured maximum {positions}")
+        for held, n in zip(self._known_lengths(), numbers):
+            if held + n > positions:
+                raise ValueError(f"sequence length {held + n} exceeds configured maximum {positions}")
         return token_ids.reshape(-1), numbers
 
     def positions(self, batch: PagedBatch, numbers: Sequence[int], most: int) -> Tensor:

@@ -56,3 +56,32 @@ def test_no_captured_step_of_a_pool_and_none_of_uneven_counts(monkeypatch: pytes
     with pytest.raises(RuntimeError, match="as many"):
         own.step([1, 0, 1])
     assert own.step([2, 2, 2]).starts.tolist() == [0, 2, 4, 6]
+
+
+def test_steps_after_replays_are_checked_against_the_devices_lengths(monkeypatch: pytest.MonkeyPatch) -> None:
+    cache = _cache()
+    ids = torch.zeros(3, 1, dtype=torch.long)
+    cache.advance([4, 4, 4], cache.step([4, 4, 4]))
+    with monkeypatch.context() as m:  # a captured step, which changes nothing here but the lengths' tensor
+        m.setattr(da.RoutedCache, "_capturing", lambda cache: True)
+        cache.rows(ids, None, 100)
+        batch = cache.step([1, 1, 1])
+        kept = cache.lengths.clone()
+        cache.advance([1, 1, 1], batch)
+        cache.lengths.copy_(kept)     # (nothing runs in a capture)
+    cache.rows(ids.expand(3, 96), None, 100)
+    cache.step([96, 96, 96])          # the four tokens that there are, and no fifth
+    for _ in range(95):               # replays
+        cache.lengths.add_(1)
+    cache.rows(ids, None, 100)
+    cache.step([1, 1, 1])
+    with pytest.raises(ValueError, match="has 99 tokens"):
+        cache.step([0, 2, 0])
+    with pytest.raises(ValueError, match="length 101"):
+        cache.rows(ids.expand(3, 2), None, 100)
+    cache.advance([1, 0, 0], cache.step([1, 0, 0]))
+    assert cache.lengths.tolist() == [100, 99, 99]
+    with pytest.raises(ValueError, match="has 100 tokens"):
+        cache.step([1, 1, 1])
+    cache.release(0)
+    assert cache.step([100, 1, 1]).max_new == 100

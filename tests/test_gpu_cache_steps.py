@@ -84,3 +84,28 @@ def test_steps_that_replays_cannot_follow_are_not_captured() -> None:
         want = lm.new_cache(2)
         assert torch.equal(lm.extend(ids, pool), lm.extend(ids, want))
     assert ops.device_status() == 0
+
+
+def test_eager_steps_after_replays_know_the_length() -> None:
+    lm, ids = _lm(positions=64), _ids(2, 64)
+    with torch.no_grad(), torch.autocast("cuda", dtype=BF16, cache_enabled=False):
+        cache, other = lm.new_cache(2), lm.new_cache(2)
+        token = ids[:, :1].clone()
+        lm.extend(token, cache)
+        cache.release()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            lm.extend(token, cache)
+        for i in range(60):
+            token.copy_(ids[:, i:i + 1])
+            graph.replay()
+        with pytest.raises(ValueError, match="length 65 exceeds"):
+            lm.extend(ids[:, 59:], cache)
+        last = lm.extend(ids[:, 60:], cache)
+        want = lm.extend(ids, other)[:, 60:]
+        assert cache.lengths.tolist() == [64, 64]
+        with pytest.raises(ValueError, match="exceeds"):
+            lm.extend(token, cache)
+    # (as through the cache in one step or several: roundings to bf16 differ, 0.1 of the logits' spread and half a step each)
+    assert ((last.double() - want.double()).abs() <= 0.1 * 512**0.5 + 2.0**-7 * want.double().abs()).all()
+    assert ops.device_status() == 0
