@@ -192,7 +192,7 @@ class Int8DoubleAttentionLM(_FixedTypes):
     def extend(self, token_ids: Tensor, cache: paged.RoutedCache, counts: Sequence[int] | None = None) -> Tensor:
         """Logits of new tokens behind those in ``cache``, which takes them in: as ``DoubleAttentionLM.extend``."""
         ids, numbers = cache.rows(token_ids, counts, self.max_sequence_length)
-        batch = cache.step(numbers)
+        batch = cache.step(numbers, self.max_sequence_length)
         if not ids.numel():
             return self.token_embedding.weight.new_empty(*token_ids.shape, self.lm_head.weight.shape[0], dtype=self.lm_head.dtype)
         positions = cache.positions(batch, numbers, self.max_sequence_length)

@@ -415,7 +415,7 @@ class DoubleAttentionLM(nn.Module):
         ``token_ids`` [B, T], T new tokens of every sequence of the cache, or [N] with ``counts``, packed one sequence after
         another: logits [B, T, V] or [N, V].  What :meth:`forward` gives for the whole sequences, up to rounding."""
         ids, numbers = cache.rows(token_ids, counts, self.max_sequence_length)
-        batch = cache.step(numbers)
+        batch = cache.step(numbers, self.max_sequence_length)
         if not ids.numel():
             return self.lm_head.weight.new_empty(*token_ids.shape, self.lm_head.out_features)
         x = self.token_embedding(ids) + self.position_embedding(cache.positions(batch, numbers, self.max_sequence_length))

@@ -7,9 +7,10 @@ sequences, packed one sequence after another (:class:`PagedBatch`); :func:`appen
 into the pages, :func:`routed_attention_paged` lets each new token attend over its sequence up to itself, from single
 tokens to long chunks.  :class:`RoutedCache` holds the pages of all layers of a model and hands them out.
 
-The sizes that vary from step to step are read by the kernels on the device: no call waits for the GPU, and a captured
+The sizes that vary from step to step are read by the kernels on the device: neither operator waits for the GPU, and a captured
 graph follows them.  A page number outside the cache, or a length that the table has no room for, is never followed:
-those positions are not written, the tokens that would need them (and others of their tile of 128 new tokens) get NaN, and ``ops.device_status`` reports bit 8.
+those positions are not written, the tokens that would need them (and others of their tile of 128 new tokens) get NaN, and
+``ops.device_status`` reports bit 8, on the stream that the call ran on or was captured on.
 
 Inference only: the operators raise on tensors that require a gradient.
 """
@@ -203,7 +204,9 @@ class RoutedCache:
     a CUDA graph: the device's ``lengths`` advance with every replay.  With fewer ``pages`` sequences share a pool: a step takes
     what its new tokens need and raises if there is none left; ``release`` gives a sequence's pages back.  A pool's steps cannot
     be captured, as no replay would reserve pages.  Once a step has been captured, every other one reads the lengths back from
-    the device first, and waits for it: replays have moved them.  Not for several threads at once."""
+    the device first, and waits for it: replays have moved them.  A replay that runs past ``max_length``, or the positions that
+    the model has, writes nothing of such a sequence, gives it NaN and sets ``ops.device_status`` bit 8.  Not for several
+    threads at once."""
 
     def __init__(self, config, layers: int, sequences: int, max_length: int, *, page_size: int = 64, pages: int | None = None,
                  dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda") -> None:
@@ -254,8 +257,9 @@ class RoutedCache:
             self._held = self.lengths.tolist()
         return self._held
 
-    def step(self, counts: Sequence[int]) -> PagedBatch:
-        """The batch of a step that brings ``counts[b]`` new tokens of sequence b, its pages reserved."""
+    def step(self, counts: Sequence[int], positions: int | None = None) -> PagedBatch:
+        """The batch of a step that brings ``counts[b]`` new tokens of sequence b, its pages reserved.  ``positions``: the most
+        that the model has, which replays of a captured step are held to."""
         if len(counts) != self.sequences or any(n < 0 for n in counts):
             raise ValueError(f"a step takes a number of new tokens for each of the {self.sequences} sequences, got {list(counts)}")
         if self._capturing():
@@ -286,7 +290,12 @@ class RoutedCache:
             for c in counts:
                 ends.append(ends[-1] + c)
             starts = torch.tensor(ends, dtype=torch.int32).to(self.table.device)
-        return PagedBatch(self.table, self.lengths, starts, max(counts))
+        held = self.lengths
+        if self._capturing():
+            # (the table's last page may have room behind max_length: a length that no table has room for, instead)
+            most = self.max_length if positions is None else min(self.max_length, positions)
+            held = held.masked_fill(held > most - n, torch.iinfo(torch.int32).max)
+        return PagedBatch(self.table, held, starts, max(counts))
 
     def advance(self, counts: Sequence[int], batch: PagedBatch) -> None:
         """Counts a step's tokens in, after its last layer."""
@@ -325,7 +334,8 @@ class RoutedCache:
         return token_ids.reshape(-1), numbers
 
     def positions(self, batch: PagedBatch, numbers: Sequence[int], most: int) -> Tensor:
-        """Each packed row's position in its sequence (at most ``most - 1``, where a replayed graph runs over it)."""
+        """Each packed row's position in its sequence (at most ``most - 1``, where a replayed graph runs over it and its rows
+        become NaN)."""
         n, first = sum(numbers), numbers[0]
         row = torch.arange(n, device=self.lengths.device)
         if all(c == first for c in numbers):

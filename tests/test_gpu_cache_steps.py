@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from double_attention_b200 import DoubleAttentionLM, append_paged, experiment_config, ops, paged, routed_attention_paged
+from double_attention_b200 import DoubleAttentionLM, Int8DoubleAttentionLM, append_paged, experiment_config, ops, paged, routed_attention_paged
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -109,3 +109,45 @@ def test_eager_steps_after_replays_know_the_length() -> None:
     # (as through the cache in one step or several: roundings to bf16 differ, 0.1 of the logits' spread and half a step each)
     assert ((last.double() - want.double()).abs() <= 0.1 * 512**0.5 + 2.0**-7 * want.double().abs()).all()
     assert ops.device_status() == 0
+
+
+def _status(stream: torch.cuda.Stream) -> int:
+    """What calls captured on ``stream`` have reported."""
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        return ops.device_status()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize(("positions", "most"), [(400, 40), (40, None), (40, 64), (64, 64)])
+@pytest.mark.parametrize("new", [1, 3, 20])
+def test_replays_past_the_last_position_are_reported(new, positions, most, int8) -> None:
+    """Of two sequences the longer one runs past the most positions: NaN and a status, and the other goes on."""
+    lm = _lm(positions=positions)
+    lm, limit = Int8DoubleAttentionLM(lm) if int8 else lm, min(positions, most or positions)
+    ids = _ids(2, new, 3)
+    with torch.no_grad(), torch.autocast("cuda", dtype=BF16, cache_enabled=False):
+        cache, other = lm.new_cache(2, most), lm.new_cache(2, most)
+        lm.extend(ids, cache)
+        cache.release()
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=stream):
+            logits = lm.extend(ids, cache)
+        first = _ids(1, limit - 2 * new)[0]
+        for c in (cache, other):  # two more steps fit the second sequence
+            lm.extend(first, c, [0, limit - 2 * new])
+        for _ in range(2):
+            graph.replay()
+            want = lm.extend(ids, other)
+            assert ((logits.double() - want.double()).abs() <= 0.1 * 512**0.5 + 2.0**-7 * want.double().abs()).all()
+            assert _status(stream) == 0
+        before = [t.clone() for t in (cache.key_pages, cache.value_pages)]
+        graph.replay()
+        assert _status(stream) == paged.BAD_PAGE
+        want = lm.extend(ids[0], other, [new, 0]) if limit >= 3 * new else None
+    assert logits[1].isnan().all()
+    if want is not None:
+        assert ((logits[0].double() - want.double()).abs() <= 0.1 * 512**0.5 + 2.0**-7 * want.double().abs()).all()
+    own = cache.table[1].long()  # nothing of the second sequence is written
+    for now, was in zip((cache.key_pages, cache.value_pages), before):
+        assert torch.equal(now[:, own], was[:, own])
