@@ -185,7 +185,8 @@ class Int8DoubleAttentionLM(_FixedTypes):
     def new_cache(self, sequences: int, max_length: int | None = None, *, page_size: int = 64,
                   pages: int | None = None) -> paged.RoutedCache:
         """An empty cache for :meth:`extend`."""
-        return paged.RoutedCache(self.blocks[0].config, len(self.blocks), sequences, max_length or self.max_sequence_length,
+        return paged.RoutedCache(self.blocks[0].config, len(self.blocks), sequences,
+                                 self.max_sequence_length if max_length is None else max_length,
                                  page_size=page_size, pages=pages, dtype=self.lm_head.dtype, device=self.lm_head.weight.device)
 
     @torch.no_grad()

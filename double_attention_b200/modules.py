@@ -405,7 +405,8 @@ class DoubleAttentionLM(nn.Module):
                   dtype: torch.dtype = torch.bfloat16) -> paged.RoutedCache:
         """An empty cache for :meth:`extend`; ``dtype`` is the type that the attention computes in (autocast's, or the
         parameters')."""
-        return paged.RoutedCache(self.stack.config, self.stack.num_layers, sequences, max_length or self.max_sequence_length,
+        return paged.RoutedCache(self.stack.config, self.stack.num_layers, sequences,
+                                 self.max_sequence_length if max_length is None else max_length,
                                  page_size=page_size, pages=pages, dtype=dtype, device=self.token_embedding.weight.device)
 
     @torch.no_grad()
