@@ -207,4 +207,6 @@ class Int8DoubleAttentionLM(_FixedTypes):
         of its distribution and its ``top`` likeliest tokens: [B, T - 1]."""
         if token_ids.ndim != 2 or token_ids.shape[1] < 2:
             raise ValueError("token_ids must have shape [B, T] with T at least 2")
+        if not self.blocks[0].config.causal:
+            raise ValueError("tokens are scored under those before them, which a causal attention alone sees")
         return token_log_probs(self(token_ids[:, :-1]), token_ids[:, 1:], top=top)

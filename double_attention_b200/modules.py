@@ -429,6 +429,8 @@ class DoubleAttentionLM(nn.Module):
         of its distribution and its ``top`` likeliest tokens: [B, T - 1].  Differentiable (see :func:`token_log_probs`)."""
         if token_ids.ndim != 2 or token_ids.shape[1] < 2:
             raise ValueError("token_ids must have shape [B, T] with T at least 2")
+        if not self.stack.config.causal:
+            raise ValueError("tokens are scored under those before them, which a causal attention alone sees")
         ids, batch = token_ids[:, :-1], token_ids.shape[0]
         # sequences of the token 0 beside them, which change nothing of theirs, fill the attention's smallest tile
         short = -(-_ATTENTION_ROWS // ids.shape[1]) - batch

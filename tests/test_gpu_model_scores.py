@@ -73,3 +73,8 @@ def test_a_model_of_few_positions_is_scored() -> None:
         with pytest.raises(ValueError, match="maximum"):
             lm.score(_ids(1, 22))
         assert lm.score(_ids(1, 5)[:0]).log_probs.shape == (0, 4)
+
+
+def test_an_int8_model_that_sees_later_tokens_is_not_scored() -> None:
+    with pytest.raises(ValueError, match="causal"):
+        da.Int8DoubleAttentionLM(_lm("a1", causal=False)).score(_ids(2, 10))
