@@ -127,6 +127,20 @@ def _aligned_query(q: Tensor) -> Tensor:
     return q
 
 
+def _extent(t: Tensor) -> tuple[int, int]:
+    """First byte of ``t``, and the one behind its last."""
+    last = sum((n - 1) * step for n, step in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size() if t.numel() else t.data_ptr()
+
+
+def _check_apart(name: str, out: Tensor, *inputs: Tensor) -> None:
+    first, end = _extent(out)
+    for t in inputs:
+        a, b = _extent(t)
+        if t.device == out.device and first < b and a < end:
+            raise ValueError(f"{name} cannot write over what it reads: out shares memory with an input")
+
+
 def routed_attention_paged(query: Tensor, key_pages: Tensor, value_pages: Tensor, batch: PagedBatch, scales: Tensor,
                            map_weights: Tensor | None = None, *, out: Tensor | None = None) -> Tensor:
     """Outer routed attention of the packed new tokens over the pages, after :func:`append_paged` put them there.
@@ -134,8 +148,9 @@ def routed_attention_paged(query: Tensor, key_pages: Tensor, value_pages: Tensor
     query [H, N, R] of the pages' type; ``scales`` [S] the maps' temperatures, S of H branches as in
     :func:`assemble_score_maps`.  Token i of sequence b sees positions 0 to ``batch.lengths[b] + i``.  With
     ``map_weights`` [S], or one map, returns the maps' mixture [N, D]; without, several maps' outputs [N, S, D].  The
-    keys may be of any length: the softmax takes off each row's own maximum.  Rows of no sequence are zero,
-    or left as they are in ``out``.
+    keys may be of any length: the softmax takes off each row's own maximum.  What a token does not see may hold anything;
+    where a key or a value that it sees is not finite, its outputs (of any map) are not.  Rows of no sequence are zero,
+    or left as they are in ``out``, which shares no memory with the inputs.
 
     Supported: R a multiple of 64, D 128, 256 or 512, up to 4 maps and ``max(H, S) * R`` up to 512."""
     name = "routed_attention_paged"
@@ -162,6 +177,8 @@ def routed_attention_paged(query: Tensor, key_pages: Tensor, value_pages: Tensor
     if out is not None and (out.shape != shape or out.dtype != query.dtype or not out.is_contiguous()
                             or out.data_ptr() % 16):
         raise ValueError(f"{name} writes a contiguous, 16-byte aligned {query.dtype} tensor {shape}, got {out.dtype} {tuple(out.shape)}")
+    if out is not None:
+        _check_apart(name, out, query, key_pages, value_pages)
     device = _device_of(name, key_pages, value_pages, query, scales, map_weights, out, *batch[:3])
     _inference_only(name, query, key_pages, value_pages, scales, map_weights, out)
     y = torch.empty(shape, dtype=query.dtype, device=query.device) if out is None else out
