@@ -3,7 +3,7 @@
 Every ``csrc/*.cu`` file is compiled with nvcc for ``sm_100a`` and linked
 into one shared library exporting the C ABI declared in
 ``include/da_b200.h``.  ``csrc/host/host_calls.cpp``, the host side of the
-eight-bit operators' calls, becomes the extension module ``_host_calls``
+eight-bit, paged and scoring operators' calls, becomes the extension module ``_host_calls``
 beside it (the host compiler against this Python and PyTorch); where that cannot be built the library can, and
 the calls do without it.  Object files go to ``_build/`` at the repository
 root; a file is recompiled only when it or a header changed.
@@ -138,8 +138,8 @@ def build(force: bool = False, jobs: int | None = None, verbose_ptxas: bool = Fa
         build_host_calls(force)
     except (RuntimeError, OSError, ImportError) as error:  # no host compiler, no headers of Python or PyTorch
         HOST_PATH.unlink(missing_ok=True)
-        warnings.warn(f"{HOST_PATH.name} was not built: the eight-bit operators' calls take their Python path, about 8 us "
-                      f"slower each ({error})", RuntimeWarning, stacklevel=2)
+        warnings.warn(f"{HOST_PATH.name} was not built: the eight-bit, paged and scoring operators' calls take their "
+                      f"Python path, 8 to 20 us slower each ({error})", RuntimeWarning, stacklevel=2)
     if verbose_ptxas and logs:
         print("\n".join(logs))
     return LIB_PATH

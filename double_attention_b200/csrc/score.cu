@@ -543,12 +543,11 @@ __global__ void __launch_bounds__(256) backward_kernel(const BackwardParams p) {
   }
 }
 
-int check(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t V, const void* tokens) {
+int check(const void* logits, int dtype, int64_t rows, int64_t V, const void* tokens) {
   if (dtype != DA_F16 && dtype != DA_BF16 && dtype != DA_F32) return DA_ERR_DTYPE;
   if (rows < 0 || rows > 0x7fffffff || V < 1 || V > 0x7fffff00) return DA_ERR_SHAPE;
   if (rows && (!logits || !tokens)) return DA_ERR_NULL;
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == DA_F32 ? 4 : 2)) return DA_ERR_ALIGN;
-  (void)ld;
   return DA_OK;
 }
 
@@ -575,7 +574,7 @@ extern "C" int da_token_log_probs(const void* logits, int dtype, int64_t ld, int
                                   int top, float* log_probs, float* entropy, float* top_log_probs, int64_t* top_tokens,
                                   float* stats, void* stream) {
   using namespace da;
-  if (int rc = score::check(logits, dtype, ld, rows, V, tokens)) return rc;
+  if (int rc = score::check(logits, dtype, rows, V, tokens)) return rc;
   if (top < 0 || top > 32 || top > V) return DA_ERR_SHAPE;
   if (rows == 0) return DA_OK;
   if (!log_probs || !entropy || (top && (!top_log_probs || !top_tokens))) return DA_ERR_NULL;
@@ -593,7 +592,7 @@ extern "C" int da_token_log_probs_bwd(const void* logits, int dtype, int64_t ld,
                                       const float* d_log_probs, const float* d_entropy, void* d_logits, int64_t ldd,
                                       void* stream) {
   using namespace da;
-  if (int rc = score::check(logits, dtype, ld, rows, V, tokens)) return rc;
+  if (int rc = score::check(logits, dtype, rows, V, tokens)) return rc;
   if (rows == 0) return DA_OK;
   if (!stats || !entropy || !d_logits) return DA_ERR_NULL;
   if (reinterpret_cast<uintptr_t>(stats) % 8 || reinterpret_cast<uintptr_t>(d_logits) % (dtype == DA_F32 ? 4 : 2))

@@ -67,8 +67,8 @@ def _host():
             if built_for != torch.__version__:
                 raise ImportError(f"built for PyTorch {built_for}, this is {torch.__version__}")
         except ImportError as error:
-            warnings.warn(f"the _host_calls extension cannot be used ({error}): eight-bit calls take about 8 us longer on the "
-                          "host; `python -m double_attention_b200.build` builds it", RuntimeWarning, stacklevel=3)
+            warnings.warn(f"the _host_calls extension cannot be used ({error}): eight-bit, paged and scoring calls take 8 to "
+                          "20 us longer on the host; `python -m double_attention_b200.build` builds it", RuntimeWarning, stacklevel=3)
             _host_module = _NoHostCalls()
         else:
             _host_calls.set_check(_lib.check)
