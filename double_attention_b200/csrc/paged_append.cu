@@ -3,8 +3,9 @@
 // Row j of the packed tokens, the i-th new one of its sequence b, goes to position lengths[b] + i: H R key elements from
 // [H, tokens, R] and D value elements from [tokens, D], converted to the cache's type with one rounding.  Bytes in and
 // out are all there is: a warp takes one token, finds its sequence with a 32-way search of the starts (two dependent
-// loads up to 1024 sequences) and copies 16 bytes a lane.  11100 tokens of 512 + 512 columns in bf16, 46 MB in and out: 7.2
-// us, 6.3 TB/s, a copy's rate; 64 single tokens 2.9 us, a launch's latency.
+// loads up to 1024 sequences) and copies 16 bytes a lane.  11100 tokens of 512 + 512 columns in bf16, 46 MB in and out: 12.5
+// us from memory, 3.7 TB/s (a warp has two to four loads in flight), 7.0 where all of it lies in L2; 64 single tokens 2.9 us, a
+// launch's latency.  Sources off 16 bytes go element by element.
 #include "host_util.h"
 #include "paged.cuh"
 #include "vec8.cuh"

@@ -24,10 +24,12 @@
 // rounding (1.7e-3 in bf16 against 64 bits; one part 2.3e-3); in fp16 also of 2^-32 of the row's largest weight a key, half its
 // smallest step (kLift).
 //
-// Measured (bf16, 512 value columns, joining included): 64 sequences of 4096 to 8192, 256 key columns, 609 MB, 104 us, 5.9
-// TB/s, where a copy's rate would take 93 us; one sequence of 131072, 512 key columns, 268 MB, 56.4 us, 4.8 TB/s: two launches,
-// the first tiles' way from memory and the join count there.  One token of a sequence of 512 takes 10.2 us, and five drafted
-// tokens of eight sequences of up to 2008 (two maps) 20.8 us: latency of those steps and of a CTA's few dependent tiles.
+// Measured (bf16, 512 value columns, joining included): 64 sequences of 4096 to 8192, 256 key columns, 609 MB, 104 us, 5.8
+// TB/s, where a copy's rate would take 93 us; one sequence of 131072, 512 key columns, 268 MB, 57 us, 4.7 TB/s: two launches,
+// the first tiles' way from memory and the join count there.  One token of a sequence of 512 takes 10.6 us, and five drafted
+// tokens of eight sequences of up to 2008 (two maps) 21 us: latency of those steps and of a CTA's few dependent tiles.
+// With 256 and 128 value columns, two CTAs an SM, 96 registers a thread and 194 to 226 bytes of spills, the 64 sequences take 98 and
+// 95 us, 4.1 and 3.2 TB/s.
 #include <math.h>
 
 #include "host_util.h"

@@ -11,12 +11,14 @@
 //   * the (query tile, key range) pieces are planned on the device from the lengths: equal key ranges of all tiles, so
 //     that few or uneven tiles fill the GPU; join_kernel adds the pieces of a tile in order.
 // A value behind a row's last position weighs 0, and 0 times a NaN or an infinity is NaN: such rows are found when they
-// are written and computed again by the other kernel, which tells them apart.
+// are written and their sequences computed again by the other kernel, which tells them apart and reads the cache once per 16 rows
+// (512 tokens behind 32768: 376 us instead of 47).  Weights are rounded to 16 bits once, as a second part would double the
+// product with the values: 2.3e-3 against 64 bits in bf16, where the outputs' own rounding is 1.7e-3; 2.9e-4 and 2.1e-4 in fp16.
 //
 // Measured on the device, all launches of a call together: 512 tokens behind 32768 (bf16, one map of 256 columns, 512 value
-// columns) 47 us, 0.55 PFLOP/s, of which this file's chunk kernel takes 36 with its tensor pipe 41 % active.  Six
-// uneven chunks of up to 700 tokens behind up to 4001 (fp16, four maps of 128 columns) 90 us, 0.25 PFLOP/s: 2^x is asked for
-// twice a score and map, 16 a clock, which is 32 to 37 % of both phases, issue slots 35 to 40 %.  What bounds both is latency: before
+// columns) 47 us, 0.55 PFLOP/s, of which this file's chunk kernel takes 35 with its tensor pipe 44 % active.  Six
+// uneven chunks of up to 700 tokens behind up to 4001 (fp16, four maps of 128 columns) 87 us, 0.26 PFLOP/s: 2^x is asked for
+// twice a score and map, 16 a clock, which is 41 and 35 % of the phases, issue slots 43 and 36 %.  What bounds both is latency: before
 // its first product a CTA pair takes about 6000 cycles (plan, descriptors, barriers between the two, first keys), after the
 // last about 4500 to leave a piece's outputs, 128 KB a CTA; between them a tile of 128 keys waits on a chain of scores,
 // maxima, weights and products, of which two groups of softmax warps keep two under way (one group: 115 us instead of 105
