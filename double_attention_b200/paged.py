@@ -317,7 +317,9 @@ class RoutedCache:
     def advance(self, counts: Sequence[int], batch: PagedBatch) -> None:
         """Counts a step's tokens in, after its last layer."""
         self.lengths.add_(batch.starts[1:] - batch.starts[:-1])
-        if not self._capturing():
+        if self._capturing():  # (nothing has come yet; replays bring them)
+            self._captured = True
+        else:
             self._held = [held + n for held, n in zip(self._held, counts)]
 
     def release(self, sequence: int | None = None) -> None:

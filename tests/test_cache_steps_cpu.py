@@ -85,3 +85,15 @@ def test_steps_after_replays_are_checked_against_the_devices_lengths(monkeypatch
         cache.step([1, 1, 1])
     cache.release(0)
     assert cache.step([100, 1, 1]).max_new == 100
+
+
+@pytest.mark.parametrize("pages", [None, 9])
+def test_a_step_made_before_a_capture_that_counts_it_in(pages, monkeypatch: pytest.MonkeyPatch) -> None:
+    cache = _cache(pages=pages)
+    batch = cache.step([2, 2, 2])
+    with monkeypatch.context() as m:
+        m.setattr(da.RoutedCache, "_capturing", lambda cache: True)
+        cache.advance([2, 2, 2], batch)  # (counts on the CPU at once, as a replay does)
+    assert cache.lengths.tolist() == [2, 2, 2]
+    with pytest.raises(ValueError, match="has 2 tokens"):
+        cache.step([99, 0, 0])
